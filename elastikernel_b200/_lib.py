@@ -20,6 +20,7 @@ EK_ERR_DEVICE = 5
 EK_DTYPE_BF16 = 0
 EK_DTYPE_FP16 = 1
 EK_DTYPE_E4M3 = 2
+EK_DTYPE_FP32 = 3
 
 EK_QUANT_POW2_SCALES = 1
 
@@ -116,6 +117,16 @@ _SIGNATURES = {
     "ek_ep_capacity_layout": (_c_int, [_c_vp, _c_vp, _c_int, _c_int, _c_int, _c_vp, _c_vp, _c_int, _c_vp, _c_vp, _c_vp,
                                        _c_vp, _c_vp]),
     "ek_moe_combine_rows": (_c_int, [_c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_vp]),
+    "ek_moe_dispatch": (_c_int, [_c_vp, _c_int, _c_int, _c_int, _c_vp, _c_int, _c_int] + [_c_vp] * 7),
+    "ek_moe_dispatch_grad": (_c_int, [_c_vp, _c_vp] + [_c_int] * 5 + [_c_vp, _c_vp]),
+    "ek_moe_combine_weighted": (_c_int, [_c_vp] * 3 + [_c_int] * 5 + [_c_vp, _c_vp]),
+    "ek_moe_combine_weighted_grad": (_c_int, [_c_vp] * 5 + [_c_int] * 5 + [_c_vp] * 3),
+    "ek_moe_route_grad": (_c_int, [_c_vp] * 3 + [_c_int] * 3 + [_c_vp, _c_vp]),
+    "ek_quant_w4": (_c_int, [_c_vp, _c_int, ctypes.c_longlong] + [_c_int] * 4 + [_c_vp] * 4),
+    "ek_dequant_w4": (_c_int, [_c_vp] * 3 + [ctypes.c_longlong] + [_c_int] * 3 + [_c_vp, _c_vp]),
+    "ek_gemm_w4": (_c_int, [_c_vp] * 5 + [_c_int] * 6 + [_c_vp]),
+    "ek_moe_gate_up_w4": (_c_int, [_c_vp, _c_vp, _c_int, _c_int] + [_c_vp] * 8 + [_c_int] * 6 + [_c_vp]),
+    "ek_moe_down_w4": (_c_int, [_c_vp] * 6 + [_c_int] * 6 + [_c_vp]),
     "ek_moe_segment_gemm": (_c_int, [_c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
                                      _c_vp]),
 }

@@ -647,6 +647,312 @@ def fused_moe(hidden_states: torch.Tensor, gate_logits: torch.Tensor, w1: torch.
     return moe_combine(y, T, topk, out=out)
 
 
+# ------------------------------------------------- token rows to experts and back
+_ROW_DTYPES = {torch.bfloat16: _lib.EK_DTYPE_BF16, torch.float16: _lib.EK_DTYPE_FP16,
+               torch.float32: _lib.EK_DTYPE_FP32}
+
+
+def _check_rows(name: str, t: torch.Tensor, rows: int | None = None) -> int:
+    """dtype code of a contiguous bf16/fp16/fp32 row matrix (of `rows` rows)."""
+    dt = _ROW_DTYPES.get(t.dtype)
+    if dt is None or t.dim() != 2:
+        raise RuntimeError(f"{name} must be a 2-D bf16, fp16 or fp32 tensor")
+    if rows is not None and t.shape[0] != rows:
+        raise RuntimeError(f"{name} must have {rows} rows, got {t.shape[0]}")
+    if t.shape[1] == 0:
+        raise RuntimeError(f"{name} has rows of no elements")
+    _contig(name, t)
+    return dt
+
+
+def _check_slots(name: str, t: torch.Tensor, T: int, k: int, dtype: torch.dtype) -> None:
+    if t.dtype != dtype or tuple(t.shape) != (T, k):
+        raise RuntimeError(f"{name} must be a {dtype} tensor of shape {(T, k)}")
+    _contig(name, t)
+
+
+def _slot_rows(perm: dict) -> torch.Tensor:
+    if perm.get("slot_rows") is None:
+        raise RuntimeError("the permutation has no slot_rows (make it with moe_dispatch)")
+    return perm["slot_rows"]
+
+
+def moe_dispatch(x: torch.Tensor | None, topk_ids: torch.Tensor, num_experts: int) -> dict:
+    """Token rows in expert-major order, for training and for batches with padding.
+
+    The (token, choice) slots are sorted stably by expert id and x's rows
+    (bf16, fp16 or fp32, any width) copied into that order. A negative id
+    drops its slot: a padding token, or a slot over its expert's capacity. An
+    id past num_experts drops it too and raises EK_STATUS_BAD_INDEX. x=None
+    makes the order alone.
+
+    Returns the packed layout the *_packed and *_w4 products take (as
+    moe_permute(..., block_m=1), without block_expert): x_perm [T*k, H] with
+    zero rows past the last kept one, sorted_slots, expert_counts and
+    num_rows_padded, plus slot_rows [T*k], the row of each slot (-1: dropped),
+    which the way back and the gradients need."""
+    dev = _require_cuda(topk_ids, x)
+    if topk_ids.dtype != torch.int32 or topk_ids.dim() != 2:
+        raise RuntimeError("topk_ids must be a 2-D int32 tensor")
+    _contig("topk_ids", topk_ids)
+    T, k = topk_ids.shape
+    E, n = int(num_experts), T * k
+    H = dt = 0
+    x_perm = None
+    if x is not None:
+        dt = _check_rows("x", x, T)
+        H = x.shape[1]
+        x_perm = torch.empty((n, H), dtype=x.dtype, device=dev)
+    L = lib()
+    ints = int(L.ek_moe_permute_scratch_bytes(T, k, E)) // 4
+    sorted_slots, slot_rows, counts, num_rows, scratch = torch.empty(
+        2 * n + max(E, 0) + 1 + ints, dtype=torch.int32, device=dev).split([n, n, max(E, 0), 1, ints])
+    with _on_device(dev):
+        check(L.ek_moe_dispatch(topk_ids.data_ptr(), T, k, E, _ptr(x), H, dt, sorted_slots.data_ptr(),
+                                slot_rows.data_ptr(), counts.data_ptr(), num_rows.data_ptr(), _ptr(x_perm),
+                                scratch.data_ptr(), current_stream_handle(dev)), "ek_moe_dispatch")
+    return {"sorted_slots": sorted_slots, "slot_rows": slot_rows, "block_expert": None, "num_rows_padded": num_rows,
+            "expert_counts": counts, "x_perm": x_perm, "max_rows": n, "T": T, "topk": k, "E": E, "block_m": 1}
+
+
+def moe_dispatch_grad(perm: dict, d_rows: torch.Tensor) -> torch.Tensor:
+    """Gradient of moe_dispatch's copy: d_x[t] = the sum of the gradients of
+    token t's rows (fp32 in choice order, rounded once), [T, H]."""
+    slot_rows = _slot_rows(perm)
+    dev = _require_cuda(d_rows, slot_rows)
+    dt = _check_rows("d_rows", d_rows)
+    T, k, (n, H) = perm["T"], perm["topk"], d_rows.shape
+    d_x = torch.empty((T, H), dtype=d_rows.dtype, device=dev)
+    with _on_device(dev):
+        check(lib().ek_moe_dispatch_grad(d_rows.data_ptr(), slot_rows.data_ptr(), T, k, n, H, dt, d_x.data_ptr(),
+                                         current_stream_handle(dev)), "ek_moe_dispatch_grad")
+    return d_x
+
+
+def moe_combine_weighted(perm: dict, rows: torch.Tensor, topk_weights: torch.Tensor,
+                         out: torch.Tensor | None = None) -> torch.Tensor:
+    """out[t] = sum_j topk_weights[t, j] * (row of slot t, j) over the kept slots:
+    expert-major rows back to the tokens (fp32 in choice order, rounded once)."""
+    slot_rows = _slot_rows(perm)
+    dev = _require_cuda(rows, topk_weights, slot_rows, out)
+    dt = _check_rows("rows", rows)
+    T, k, (n, H) = perm["T"], perm["topk"], rows.shape
+    _check_slots("topk_weights", topk_weights, T, k, torch.float32)
+    if out is None:
+        out = torch.empty((T, H), dtype=rows.dtype, device=dev)
+    elif out.dtype != rows.dtype or tuple(out.shape) != (T, H) or not out.is_contiguous():
+        raise RuntimeError("out must be a contiguous [T, H] tensor of the rows' dtype")
+    with _on_device(dev):
+        check(lib().ek_moe_combine_weighted(rows.data_ptr(), slot_rows.data_ptr(), topk_weights.data_ptr(), T, k, n, H,
+                                            dt, out.data_ptr(), current_stream_handle(dev)),
+              "ek_moe_combine_weighted")
+    return out
+
+
+def moe_combine_weighted_grad(perm: dict, rows: torch.Tensor, topk_weights: torch.Tensor,
+                              d_out: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Gradient of moe_combine_weighted: d_rows (the rows' dtype; zero past the
+    last kept row) and d_weights [T, k] (fp32; zero for a dropped slot)."""
+    slot_rows = _slot_rows(perm)
+    dev = _require_cuda(rows, topk_weights, d_out, slot_rows)
+    dt = _check_rows("rows", rows)
+    T, k, (n, H) = perm["T"], perm["topk"], rows.shape
+    _check_slots("topk_weights", topk_weights, T, k, torch.float32)
+    if d_out.dtype != rows.dtype or tuple(d_out.shape) != (T, H):
+        raise RuntimeError(f"d_out must be a {rows.dtype} tensor of shape {(T, H)}")
+    _contig("d_out", d_out)
+    d_rows = torch.empty_like(rows)
+    d_weights = torch.empty((T, k), dtype=torch.float32, device=dev)
+    with _on_device(dev):
+        check(lib().ek_moe_combine_weighted_grad(rows.data_ptr(), slot_rows.data_ptr(), topk_weights.data_ptr(),
+                                                 d_out.data_ptr(), perm["num_rows_padded"].data_ptr(), T, k, n, H, dt,
+                                                 d_rows.data_ptr(), d_weights.data_ptr(), current_stream_handle(dev)),
+              "ek_moe_combine_weighted_grad")
+    return d_rows, d_weights
+
+
+def moe_route_grad(topk_ids: torch.Tensor, topk_weights: torch.Tensor, d_weights: torch.Tensor,
+                   num_experts: int) -> torch.Tensor:
+    """Gradient of moe_route's weights with respect to the gate logits, fp32 [T, E].
+
+    The renormalised weights are the softmax of the chosen logits, so
+    d_logits[t, ids_j] = w_j (dw_j - sum_i w_i dw_i) and every other entry is 0."""
+    dev = _require_cuda(topk_ids, topk_weights, d_weights)
+    if topk_ids.dim() != 2:
+        raise RuntimeError("topk_ids must be a 2-D int32 tensor")
+    T, k = topk_ids.shape
+    _check_slots("topk_ids", topk_ids, T, k, torch.int32)
+    _check_slots("topk_weights", topk_weights, T, k, torch.float32)
+    _check_slots("d_weights", d_weights, T, k, torch.float32)
+    E = int(num_experts)
+    if E < 1:
+        raise RuntimeError("num_experts must be positive")
+    d_logits = torch.empty((T, E), dtype=torch.float32, device=dev)
+    with _on_device(dev):
+        check(lib().ek_moe_route_grad(topk_ids.data_ptr(), topk_weights.data_ptr(), d_weights.data_ptr(), T, E, k,
+                                      d_logits.data_ptr(), current_stream_handle(dev)), "ek_moe_route_grad")
+    return d_logits
+
+
+# ------------------------------------------------------------------ 4-bit weights
+W4_GROUPS = (32, 64, 128)
+
+
+def quant_w4(w: torch.Tensor, group: int = 128, symmetric: bool = True, dtype: torch.dtype | None = None) -> dict:
+    """4-bit codes of weights w [..., N, K] (bf16, fp16 or fp32; finite) with a
+    scale, and with symmetric=False a minimum, per `group` elements of a row.
+
+    Returns {"codes": uint8 [..., N, ceil(K/32)*16], "scales": [..., N,
+    ceil(K/group)], "mins": same or None, "K", "group"}; two codes per byte,
+    the even element in the low nibble. Scales and minima are in `dtype` (bf16
+    or fp16; default w's, bf16 for fp32 w), the type of the activations the
+    products take. The weight is s * (q - 8), or s * q + m with minima; weights
+    quantised elsewhere go in by building this dict."""
+    dev = _require_cuda(w)
+    if w.dtype not in _ROW_DTYPES or w.dim() < 2 or w.shape[-1] == 0:
+        raise RuntimeError("quant_w4 takes bf16, fp16 or fp32 weights [..., N, K]")
+    if dtype is None:
+        dtype = w.dtype if w.dtype in _DTYPES else torch.bfloat16
+    if dtype not in _DTYPES or group not in W4_GROUPS:
+        raise RuntimeError(f"quant_w4: dtype must be bf16 or fp16 and group one of {W4_GROUPS}")
+    _contig("w", w)
+    K = w.shape[-1]
+    lead = tuple(w.shape[:-1])
+    rows = w.numel() // K
+    codes = torch.empty(lead + (-(-K // 32) * 16,), dtype=torch.uint8, device=dev)
+    scales = torch.empty(lead + (-(-K // group),), dtype=dtype, device=dev)
+    mins = None if symmetric else torch.empty_like(scales)
+    with _on_device(dev):
+        check(lib().ek_quant_w4(w.data_ptr(), _ROW_DTYPES[w.dtype], rows, K, group, 1 if symmetric else 0,
+                                _DTYPES[dtype], codes.data_ptr(), scales.data_ptr(), _ptr(mins),
+                                current_stream_handle(dev)), "ek_quant_w4")
+    return {"codes": codes, "scales": scales, "mins": mins, "K": K, "group": group}
+
+
+def _check_w4(name: str, qw: dict, dtype: torch.dtype | None = None) -> tuple:
+    """(codes, scales, mins, leading shape, K, group) of a 4-bit weight."""
+    codes, scales, mins, K, group = qw["codes"], qw["scales"], qw.get("mins"), int(qw["K"]), int(qw["group"])
+    if group not in W4_GROUPS or K < 1:
+        raise RuntimeError(f"{name}: need K >= 1 and a group out of {W4_GROUPS}")
+    lead = tuple(codes.shape[:-1])
+    if codes.dtype != torch.uint8 or not lead or codes.shape[-1] != -(-K // 32) * 16:
+        raise RuntimeError(f"{name}: codes must be uint8 [..., N, {-(-K // 32) * 16}]")
+    if scales.dtype not in _DTYPES or tuple(scales.shape) != lead + (-(-K // group),):
+        raise RuntimeError(f"{name}: scales must be bf16 or fp16 [..., N, {-(-K // group)}]")
+    if dtype is not None and scales.dtype != dtype:
+        raise RuntimeError(f"{name}: scales must be {dtype}, got {scales.dtype}")
+    if mins is not None and (mins.dtype != scales.dtype or mins.shape != scales.shape):
+        raise RuntimeError(f"{name}: mins must match the scales")
+    for t in (codes, scales, mins):
+        if t is not None:
+            _contig(name, t)
+    return codes, scales, mins, lead, K, group
+
+
+def dequant_w4(qw: dict) -> torch.Tensor:
+    """The weights a 4-bit dict stands for, rounded once to the scales' dtype."""
+    codes, scales, mins, lead, K, group = _check_w4("dequant_w4", qw)
+    dev = _require_cuda(codes, scales, mins)
+    out = torch.empty(lead + (K,), dtype=scales.dtype, device=dev)
+    with _on_device(dev):
+        check(lib().ek_dequant_w4(codes.data_ptr(), scales.data_ptr(), _ptr(mins), out.numel() // K, K, group,
+                                  _DTYPES[scales.dtype], out.data_ptr(), current_stream_handle(dev)), "ek_dequant_w4")
+    return out
+
+
+def gemm_w4(a: torch.Tensor, qw: dict, out: torch.Tensor | None = None, num_sms: int | None = None) -> torch.Tensor:
+    """C = a @ W^T with a [M, K] (bf16 or fp16) and a 4-bit weight W [N, K]
+    (quant_w4) whose scales have a's dtype; C [M, N] in that dtype, fp32 sums."""
+    codes, scales, mins, lead, K, group = _check_w4("gemm_w4", qw, a.dtype)
+    dev = _require_cuda(a, codes, scales, mins, out)
+    if a.dim() != 2 or a.shape[1] != K or len(lead) != 1:
+        raise RuntimeError(f"gemm_w4 takes a [M, {K}] and a 2-D weight")
+    _contig("a", a)
+    M, N = a.shape[0], lead[0]
+    if out is None:
+        out = torch.empty((M, N), device=dev, dtype=a.dtype)
+    elif tuple(out.shape) != (M, N) or out.dtype != a.dtype or not out.is_contiguous():
+        raise RuntimeError("out must be a contiguous [M, N] tensor of the input dtype")
+    with _on_device(dev):
+        check(lib().ek_gemm_w4(a.data_ptr(), codes.data_ptr(), scales.data_ptr(), _ptr(mins), out.data_ptr(), M, N, K,
+                               group, _DTYPES[a.dtype], int(num_sms or 0), current_stream_handle(dev)), "ek_gemm_w4")
+    return out
+
+
+def quant_moe_weights_w4(w1: torch.Tensor, w2: torch.Tensor, w3: torch.Tensor, group: int = 128,
+                         symmetric: bool = True) -> dict:
+    """4-bit expert weights (w1, w3 [E, I, H], w2 [E, H, I]) for fused_moe_w4."""
+    E, I, H = w1.shape
+    if w3.shape != w1.shape or tuple(w2.shape) != (E, H, I):
+        raise RuntimeError("quant_moe_weights_w4: w1 and w3 must be [E, I, H] and w2 [E, H, I]")
+    q = {n: quant_w4(w, group, symmetric, torch.bfloat16) for n, w in (("w1", w1), ("w3", w3), ("w2", w2))}
+    return {"E": E, "H": H, "I": I, **q}
+
+
+def moe_gate_up_w4(perm: dict, qw: dict, x: torch.Tensor | None = None, num_sms: int | None = None) -> torch.Tensor:
+    """act[r] = silu(row . w1[e]) * (row . w3[e]) over the packed rows, 4-bit experts.
+    The rows are perm["x_perm"], or with x (the tokens [T, H]) fetched through
+    the permutation, so nothing has to be copied first. Rows past the last
+    kept one are left unwritten."""
+    E, H, I = qw["E"], qw["H"], qw["I"]
+    c1, s1, m1, l1, k1, group = _check_w4("w1", qw["w1"], torch.bfloat16)
+    c3, s3, m3, l3, k3, g3 = _check_w4("w3", qw["w3"], torch.bfloat16)
+    src = perm["x_perm"] if x is None else x
+    if src is None:
+        raise RuntimeError("moe_gate_up_w4: the permutation has no rows; give x")
+    dev = _require_cuda(src, c1, s1, m1, c3, s3, m3, perm["expert_counts"])
+    _check_bf16("x", src)
+    rows = perm["max_rows"]
+    if l1 != (E, I) or l3 != l1 or k1 != H or k3 != H or g3 != group or (m1 is None) != (m3 is None) or \
+            perm["E"] != E or tuple(src.shape) != (rows if x is None else perm["T"], H) or perm["block_m"] != 1:
+        raise RuntimeError("gate_up_w4: shape mismatch")
+    act = torch.empty((rows, I), dtype=torch.bfloat16, device=dev)
+    with _on_device(dev):
+        check(lib().ek_moe_gate_up_w4(src.data_ptr(), None if x is None else perm["sorted_slots"].data_ptr(),
+                                      perm["topk"], perm["T"] * perm["topk"], c1.data_ptr(), s1.data_ptr(), _ptr(m1),
+                                      c3.data_ptr(), s3.data_ptr(), _ptr(m3), perm["expert_counts"].data_ptr(),
+                                      act.data_ptr(), rows, E, H, I, group, int(num_sms or 0),
+                                      current_stream_handle(dev)), "ek_moe_gate_up_w4")
+    return act
+
+
+def moe_down_w4(perm: dict, act: torch.Tensor, qw: dict, num_sms: int | None = None) -> torch.Tensor:
+    """y[r] = act[r] . w2[e] over the packed rows, 4-bit experts (no routing
+    weight: moe_combine_weighted applies it). Rows past the last are left unwritten."""
+    E, H, I = qw["E"], qw["H"], qw["I"]
+    c2, s2, m2, l2, k2, group = _check_w4("w2", qw["w2"], torch.bfloat16)
+    dev = _require_cuda(act, c2, s2, m2, perm["expert_counts"])
+    _check_bf16("act", act)
+    rows = perm["max_rows"]
+    if l2 != (E, H) or k2 != I or perm["E"] != E or tuple(act.shape) != (rows, I) or perm["block_m"] != 1:
+        raise RuntimeError("down_w4: shape mismatch")
+    y = torch.empty((rows, H), dtype=torch.bfloat16, device=dev)
+    with _on_device(dev):
+        check(lib().ek_moe_down_w4(act.data_ptr(), c2.data_ptr(), s2.data_ptr(), _ptr(m2),
+                                   perm["expert_counts"].data_ptr(), y.data_ptr(), rows, E, H, I, group,
+                                   int(num_sms or 0), current_stream_handle(dev)), "ek_moe_down_w4")
+    return y
+
+
+def fused_moe_w4(hidden_states: torch.Tensor, gate_logits: torch.Tensor, qw: dict, topk: int,
+                 out: torch.Tensor | None = None, num_sms: int | None = None) -> torch.Tensor:
+    """MoE layer over 4-bit experts (quant_moe_weights_w4), for batches of a few
+    tokens per expert: route -> expert order -> gate/up SwiGLU and down over
+    the codes -> weighted combine. act and the experts' rows are bf16."""
+    _require_cuda(hidden_states, gate_logits, out)
+    _check_bf16("hidden_states", hidden_states)
+    T = hidden_states.shape[0]
+    if tuple(gate_logits.shape) != (T, qw["E"]):
+        raise RuntimeError("gate_logits must have one row per token and one column per expert")
+    if T == 0:
+        return out if out is not None else torch.empty_like(hidden_states)
+    ids, wts = moe_route(gate_logits, topk)
+    perm = moe_dispatch(None, ids, qw["E"])
+    act = moe_gate_up_w4(perm, qw, x=hidden_states, num_sms=num_sms)
+    y = moe_down_w4(perm, act, qw, num_sms=num_sms)
+    return moe_combine_weighted(perm, y, wts, out=out)
+
+
 def moe_segment_gemm(hidden_states: torch.Tensor, weights: torch.Tensor, expert_offsets: torch.Tensor,
                      num_experts: int, N: int, K: int, num_sms: int | None = None,
                      out: torch.Tensor | None = None) -> torch.Tensor:

@@ -220,6 +220,14 @@ def call_sm_aware(a, b, num_sms=None):
     return _ops.gemm(a, b, num_sms=num_sms)
 
 
+def call_sm_aware_w4(a, qw, num_sms=None):
+    """C = a @ W^T with a 4-bit weight W (_ops.quant_w4) on the current stream's
+    partition: products of a few tokens stream a quarter of the bf16 bytes."""
+    from . import _ops
+
+    return _ops.gemm_w4(a, qw, num_sms=num_sms)
+
+
 def run_benchmark(sm_levels=None, test_cases=None, rep_ms: float = 50.0) -> list:
     """Vanilla vs SM-aware tcgen05 GEMM under green-context partitions
     (the reference's benchmark, sm_aware_matmul.py:237-295), timed with CUDA

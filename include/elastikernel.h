@@ -35,6 +35,7 @@ extern "C" {
 #define EK_DTYPE_BF16 0
 #define EK_DTYPE_FP16 1
 #define EK_DTYPE_E4M3 2
+#define EK_DTYPE_FP32 3
 
 /* Layout of the B operand of a dense GEMM. */
 #define EK_B_KN 0 /* B is [K, N] row-major (the reference's b: b.stride(0) == N) */
@@ -434,6 +435,93 @@ int ek_moe_combine(const void* y, void* out, int T, int topk, int H, void* strea
  * fp16 / bf16 in and out (dtype), fp32 accumulate. */
 int ek_moe_segment_gemm(const void* hs, const void* weights, const int* offsets, void* out, int M, int N, int K,
                         int E, int dtype, int num_sms, void* stream);
+
+/* --------------------------------------- token rows to experts and back
+ * The order, the copies and the gradients around the experts' products, for
+ * training and for rows that some slots drop out of. No counterpart in the
+ * reference (its operator is forward only and keeps every slot). dtype is
+ * EK_DTYPE_BF16, EK_DTYPE_FP16 or EK_DTYPE_FP32 for every row operand; H is
+ * any size, and rows need only their elements' alignment (16-byte rows on
+ * 16-byte bases are fastest). T * topk <= 2^30. */
+
+/* Order the T * topk slots stably by expert and copy the token rows into that
+ * order. A negative id drops its slot (a padding token, a slot over an
+ * expert's capacity); an id >= E does too and raises EK_STATUS_BAD_INDEX.
+ *   sorted_slots[T*topk]  slot of each row; T*topk for the rows past the last
+ *   slot_rows[T*topk]     row of each slot; -1 for a dropped one
+ *   expert_counts[E]      rows of each expert (consecutive, expert-major)
+ *   num_rows[1]           rows in use
+ *   x_rows[T*topk, H]     x[slot / topk] per row, 0 past the last (x NULL: no
+ *                         rows are copied)
+ * This is the packed layout of ek_moe_gate_up_packed / ek_moe_down_packed and
+ * the _w4 products. E <= 1024. scratch: ek_moe_permute_scratch_bytes(T, topk,
+ * E) bytes, no initial contents. */
+int ek_moe_dispatch(const int* topk_ids, int T, int topk, int E, const void* x, int H, int dtype, int* sorted_slots,
+                    int* slot_rows, int* expert_counts, int* num_rows, void* x_rows, void* scratch, void* stream);
+
+/* Gradient of the copy: d_x[t] = sum_j d_rows[slot_rows[t, j]] over the kept
+ * slots (fp32 sum in j order; rows outside [0, n_rows) count as dropped). */
+int ek_moe_dispatch_grad(const void* d_rows, const int* slot_rows, int T, int topk, int n_rows, int H, int dtype,
+                         void* d_x, void* stream);
+
+/* The way back: out[t] = sum_j weights[t, j] * rows[slot_rows[t, j]] over the
+ * kept slots (fp32 in j order, rounded once). */
+int ek_moe_combine_weighted(const void* rows, const int* slot_rows, const float* weights, int T, int topk, int n_rows,
+                            int H, int dtype, void* out, void* stream);
+
+/* Its gradient: d_rows[r] = weights[s] * d_out[s / topk] for the slot s of each
+ * row (0 for the rows past *num_rows), d_weights[s] = <d_out[s / topk], rows[r]>
+ * (0 for a dropped slot). */
+int ek_moe_combine_weighted_grad(const void* rows, const int* slot_rows, const float* weights, const void* d_out,
+                                 const int* num_rows, int T, int topk, int n_rows, int H, int dtype, void* d_rows,
+                                 float* d_weights, void* stream);
+
+/* Gradient of ek_moe_route's weights with respect to the logits: the
+ * renormalised weights are a softmax over the chosen logits, so
+ * d_logits[t, ids_j] += w_j (dw_j - sum_i w_i dw_i), every other entry 0.
+ * Ids outside [0, E) take part in the sum and write nothing. */
+int ek_moe_route_grad(const int* topk_ids, const float* topk_weights, const float* d_weights, int T, int E, int topk,
+                      float* d_logits, void* stream);
+
+/* ------------------------------------------------------ 4-bit weights
+ * Weights of 4-bit codes with a scale (and optionally a minimum) per `group`
+ * consecutive elements of a row (group 32, 64 or 128). No counterpart in the
+ * reference. A row of K elements takes ceil(K / 32) * 16 bytes of codes, two
+ * per byte with the even element in the low nibble (codes past K are
+ * ignored), and ceil(K / group) scales and minima, in the 16-bit type `dtype`
+ * names (EK_DTYPE_BF16 or EK_DTYPE_FP16). The weight is s * (q - 8), or
+ * s * q + m where minima are given. Codes are 16-byte aligned. */
+
+/* Quantise w [rows, K] (w_dtype bf16, fp16 or fp32; finite values). symmetric:
+ * s = amax / 7, q = rint(w / s) + 8, mins unused. Otherwise m = min,
+ * s = (max - m) / 15, q = rint((w - m) / s). Both are rounded to dtype before
+ * the codes are taken; codes are clamped to [0, 15]; a scale of 0 becomes 1. */
+int ek_quant_w4(const void* w, int w_dtype, long long rows, int K, int group, int symmetric, int dtype, void* codes,
+                void* scales, void* mins, void* stream);
+
+/* The weights themselves, [rows, K] in dtype (mins NULL: symmetric). */
+int ek_dequant_w4(const void* codes, const void* scales, const void* mins, long long rows, int K, int group, int dtype,
+                  void* out, void* stream);
+
+/* C[M, N] = A[M, K] @ W[N, K]^T with 4-bit W; A, C, scales and mins in dtype,
+ * fp32 sums rounded once. Any M, N and K; made for M of a few tokens, where the
+ * codes are streamed once. */
+int ek_gemm_w4(const void* A, const void* codes, const void* scales, const void* mins, void* C, int M, int N, int K,
+               int group, int dtype, int num_sms, void* stream);
+
+/* The experts' products over the packed layout with 4-bit weights w1, w3
+ * [E, I, H] and w2 [E, H, I] (bf16 rows, scales and minima; E <= 1024):
+ *   act[r] = silu(x . w1[e]) * (x . w3[e]),  y[r] = act[r] . w2[e]
+ * for the rows r of every expert e (the rows past the last are not written).
+ * x holds the packed rows, or, with sorted_slots (n_slots = T * topk), the
+ * tokens: row r then reads x[sorted_slots[r] / topk]. */
+int ek_moe_gate_up_w4(const void* x, const int* sorted_slots, int topk, int n_slots, const void* w1_codes,
+                      const void* w1_scales, const void* w1_mins, const void* w3_codes, const void* w3_scales,
+                      const void* w3_mins, const int* expert_counts, void* act, int rows, int E, int H, int I,
+                      int group, int num_sms, void* stream);
+int ek_moe_down_w4(const void* act, const void* w2_codes, const void* w2_scales, const void* w2_mins,
+                   const int* expert_counts, void* y, int rows, int E, int H, int I, int group, int num_sms,
+                   void* stream);
 
 #ifdef __cplusplus
 }

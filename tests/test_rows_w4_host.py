@@ -1,0 +1,194 @@
+"""Host-only checks (no GPU) of the row dispatch / combine / gradient entry
+points and the 4-bit-weight entry points: the oracles' gradients against
+differences, the quantisation's error bound, and every refusal of the C ABI,
+which returns before anything is launched."""
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from elastikernel_b200 import _lib, _ops
+from elastikernel_b200._lib import lib
+from oracle import rows as orows
+from oracle import w4 as ow4
+
+
+def _p(v: int = 256) -> ctypes.c_void_p:
+    return ctypes.c_void_p(v)
+
+
+# ------------------------------------------------------------------ oracles
+def test_order_oracle_is_stable_and_drops():
+    ids = np.array([[1, 0], [-1, 1], [0, 2]], np.int32)
+    slots, rows, counts = orows.order(ids, 4)
+    assert slots.tolist() == [1, 4, 0, 3, 5, 6]
+    assert rows.tolist() == [2, 0, -1, 3, 1, 4]
+    assert counts.tolist() == [2, 2, 1, 0]
+
+
+def test_combine_gradient_against_differences():
+    rng = np.random.default_rng(0)
+    T, k, E, H = 5, 3, 4, 6
+    ids = rng.integers(-1, E, (T, k)).astype(np.int32)
+    _, sr, _ = orows.order(ids, E)
+    y, w, d = rng.normal(size=(T * k, H)), rng.normal(size=(T, k)), rng.normal(size=(T, H))
+    d_y, d_w = orows.combine_grad(y, sr, w, d)
+    h = 1e-5
+
+    def loss(y, w):
+        return (orows.combine(y, sr, w) * d).sum()
+
+    for i in np.ndindex(*y.shape):
+        a, b = y.copy(), y.copy()
+        a[i] += h
+        b[i] -= h
+        assert abs((loss(a, w) - loss(b, w)) / (2 * h) - d_y[i]) < 1e-8
+    for i in np.ndindex(*w.shape):
+        a, b = w.copy(), w.copy()
+        a[i] += h
+        b[i] -= h
+        assert abs((loss(y, a) - loss(y, b)) / (2 * h) - d_w[i]) < 1e-8
+
+
+def test_route_gradient_against_differences():
+    rng = np.random.default_rng(1)
+    T, E, k = 4, 7, 3
+    z = rng.normal(size=(T, E))
+    ids = np.argsort(-z, axis=1)[:, :k].astype(np.int32)
+    d = rng.normal(size=(T, k))
+    g = orows.route_grad(ids, orows.route_weights(z, ids), d, E)
+    h = 1e-6
+    for i in np.ndindex(T, E):
+        a, b = z.copy(), z.copy()
+        a[i] += h
+        b[i] -= h
+        num = ((orows.route_weights(a, ids) - orows.route_weights(b, ids)) * d).sum() / (2 * h)
+        assert abs(num - g[i]) < 1e-8
+
+
+@pytest.mark.parametrize("symmetric", [True, False])
+@pytest.mark.parametrize("K,group", [(128, 32), (200, 64), (257, 128), (1, 32)])
+def test_quantisation_error_is_half_a_step(symmetric, K, group):
+    """|w - value| <= s / 2 plus the clamp's excess: rounding s down by half an ulp
+    of bf16 (2^-8) leaves up to 15 * 2^-8 of a step past the last code, and the
+    rounded minimum up to 2^-8 |min| below the first."""
+    g = torch.Generator().manual_seed(K)
+    w = torch.randn((9, K), generator=g)
+    codes, s, m = ow4.quantise(w, group, symmetric, torch.bfloat16)
+    v = ow4.values(codes, s, m, K, group)
+    step = s.double().numpy()[:, np.arange(K) // group]
+    slack = 0 if m is None else np.abs(m.double().numpy()[:, np.arange(K) // group]) * 2.0 ** -8
+    assert (np.abs(v - w.double().numpy()) <= step * (0.5 + 15 * 2.0 ** -8) + slack + 1e-6).all()
+
+
+# ------------------------------------------------------------------ refusals
+def _bad(rc: int, text: str) -> None:
+    assert rc == _lib.EK_ERR_INVALID
+    assert text in _lib.last_error()
+
+
+def test_dispatch_refusals():
+    f = lib().ek_moe_dispatch
+    n = None
+    _bad(f(_p(), 4, 2, 0, n, 0, 0, _p(), _p(), _p(), _p(), n, _p(), n), "1 <= E")
+    _bad(f(_p(), 4, 2, 1025, n, 0, 0, _p(), _p(), _p(), _p(), n, _p(), n), "1 <= E")
+    _bad(f(_p(), -1, 2, 8, n, 0, 0, _p(), _p(), _p(), _p(), n, _p(), n), "bad sizes")
+    _bad(f(_p(), 4, 0, 8, n, 0, 0, _p(), _p(), _p(), _p(), n, _p(), n), "bad sizes")
+    _bad(f(_p(), 4, 2, 8, _p(), 0, 0, _p(), _p(), _p(), _p(), _p(), _p(), n), "bad sizes")
+    _bad(f(_p(), 4, 2, 8, _p(), 16, 2, _p(), _p(), _p(), _p(), _p(), _p(), n), "bad sizes or type")
+    _bad(f(_p(), 1 << 28, 8, 8, n, 0, 0, _p(), _p(), _p(), _p(), n, _p(), n), "too many slots")
+    _bad(f(n, 4, 2, 8, n, 0, 0, _p(), _p(), _p(), _p(), n, _p(), n), "null pointer")
+    _bad(f(_p(), 4, 2, 8, n, 0, 0, _p(), n, _p(), _p(), n, _p(), n), "null pointer")
+    _bad(f(_p(), 4, 2, 8, _p(), 16, 0, _p(), _p(), _p(), _p(), n, _p(), n), "null pointer")
+    _bad(f(_p(), 4, 2, 8, _p(257), 16, 0, _p(), _p(), _p(), _p(), _p(), _p(), n), "aligned")
+
+
+def test_row_gradient_refusals():
+    L = lib()
+    n = None
+    _bad(L.ek_moe_dispatch_grad(_p(), _p(), 4, 2, 8, 0, 0, _p(), n), "bad sizes")
+    _bad(L.ek_moe_dispatch_grad(_p(), n, 4, 2, 8, 16, 0, _p(), n), "null pointer")
+    _bad(L.ek_moe_dispatch_grad(_p(258), _p(), 4, 2, 8, 16, 3, _p(), n), "aligned")
+    _bad(L.ek_moe_combine_weighted(_p(), _p(), _p(), 4, 2, -1, 16, 0, _p(), n), "bad sizes")
+    _bad(L.ek_moe_combine_weighted(_p(), _p(), n, 4, 2, 8, 16, 0, _p(), n), "null pointer")
+    _bad(L.ek_moe_combine_weighted(_p(), _p(), _p(), 4, 2, 8, 16, 7, _p(), n), "type")
+    _bad(L.ek_moe_combine_weighted_grad(_p(), _p(), _p(), _p(), n, 4, 2, 8, 16, 0, _p(), _p(), n), "null pointer")
+    _bad(L.ek_moe_combine_weighted_grad(_p(), _p(), _p(), _p(), _p(), 4, 2, 8, 16, 0, _p(), n, n), "null pointer")
+    _bad(L.ek_moe_route_grad(_p(), _p(), _p(), 4, 0, 2, _p(), n), "bad sizes")
+    _bad(L.ek_moe_route_grad(_p(), _p(), n, 4, 8, 2, _p(), n), "null pointer")
+    # an empty batch is nothing to do
+    assert L.ek_moe_dispatch_grad(n, n, 0, 2, 0, 16, 0, n, n) == _lib.EK_OK
+    assert L.ek_moe_combine_weighted(n, n, n, 0, 2, 0, 16, 0, n, n) == _lib.EK_OK
+    assert L.ek_moe_route_grad(n, n, n, 0, 8, 2, n, n) == _lib.EK_OK
+
+
+def test_w4_refusals():
+    L = lib()
+    n = None
+    _bad(L.ek_quant_w4(_p(), 0, 8, 64, 48, 1, 0, _p(), _p(), n, n), "group")
+    _bad(L.ek_quant_w4(_p(), 2, 8, 64, 32, 1, 0, _p(), _p(), n, n), "types")
+    _bad(L.ek_quant_w4(_p(), 0, 8, 64, 32, 1, 3, _p(), _p(), n, n), "types")
+    _bad(L.ek_quant_w4(_p(), 0, 8, 64, 32, 0, 0, _p(), _p(), n, n), "null pointer")
+    _bad(L.ek_quant_w4(_p(), 0, 8, 0, 32, 1, 0, _p(), _p(), n, n), "K >= 1")
+    _bad(L.ek_dequant_w4(_p(264), _p(), n, 8, 64, 32, 0, _p(), n), "16-byte aligned")
+    _bad(L.ek_dequant_w4(_p(), _p(), n, 8, 64, 32, 0, n, n), "null pointer")
+    _bad(L.ek_gemm_w4(_p(), _p(), _p(), n, _p(), 1, 8, 64, 16, 0, 0, n), "group")
+    _bad(L.ek_gemm_w4(_p(), _p(), _p(), n, _p(), -1, 8, 64, 32, 0, 0, n), "bad sizes")
+    _bad(L.ek_gemm_w4(_p(), _p(), _p(), n, _p(), 1, 8, 64, 32, 3, 0, n), "type")
+    _bad(L.ek_gemm_w4(n, _p(), _p(), n, _p(), 1, 8, 64, 32, 0, 0, n), "null pointer")
+    _bad(L.ek_gemm_w4(_p(), _p(264), _p(), n, _p(), 1, 8, 64, 32, 0, 0, n), "16-byte aligned")
+    _bad(L.ek_gemm_w4(_p(), _p(), _p(257), n, _p(), 1, 8, 64, 32, 0, 0, n), "misaligned")
+    assert L.ek_gemm_w4(n, n, n, n, n, 0, 8, 64, 32, 0, 0, n) == _lib.EK_OK
+
+
+def test_moe_w4_refusals():
+    L = lib()
+    n = None
+
+    def gate_up(x=_p(), slots=n, topk=2, c1=_p(), m1=n, c3=_p(), m3=n, counts=_p(), act=_p(), rows=8, E=4, H=64,
+                I=32, group=32):
+        return L.ek_moe_gate_up_w4(x, slots, topk, rows, c1, _p(), m1, c3, _p(), m3, counts, act, rows, E, H, I, group,
+                                   0, n)
+
+    _bad(gate_up(E=0), "bad sizes")
+    _bad(gate_up(slots=_p(), topk=0), "bad sizes")
+    _bad(gate_up(group=100), "group")
+    _bad(gate_up(m1=_p()), "null pointer")
+    _bad(gate_up(counts=n), "null pointer")
+    _bad(gate_up(c3=_p(264)), "16-byte aligned")
+    _bad(L.ek_moe_down_w4(_p(), _p(), _p(), n, _p(), n, 8, 4, 64, 32, 32, 0, n), "null pointer")
+    _bad(L.ek_moe_down_w4(_p(), _p(), _p(), n, _p(), _p(), 8, 4, 0, 32, 32, 0, n), "bad sizes")
+    assert gate_up(rows=0) == _lib.EK_OK
+
+
+def test_front_end_refuses_cpu_tensors():
+    ids = torch.zeros((2, 2), dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        _ops.moe_dispatch(torch.zeros((2, 8)), ids, 4)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        _ops.quant_w4(torch.zeros((2, 64)))
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        _ops.moe_route_grad(ids, torch.zeros((2, 2)), torch.zeros((2, 2)), 4)
+
+
+def test_front_end_refuses_a_permutation_without_slot_rows():
+    perm = {"sorted_slots": None, "T": 2, "topk": 2}
+    with pytest.raises(RuntimeError, match="moe_dispatch"):
+        _ops.moe_dispatch_grad(perm, torch.zeros((4, 8)))
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(group=16), "group"), (dict(K=65), "codes"), (dict(codes=torch.zeros((4, 32), dtype=torch.int8)), "codes"),
+    (dict(scales=torch.zeros((4, 2))), "scales"), (dict(scales=torch.zeros((4, 3), dtype=torch.bfloat16)), "scales"),
+    (dict(scales=torch.zeros((4, 2), dtype=torch.float16)), "must be torch.bfloat16"),
+    (dict(mins=torch.zeros((4, 1), dtype=torch.bfloat16)), "mins"),
+    (dict(codes=torch.zeros((32, 4), dtype=torch.uint8).t()), "contiguous")])
+def test_front_end_checks_the_weight(change, text):
+    qw = dict(codes=torch.zeros((4, 32), dtype=torch.uint8), scales=torch.zeros((4, 2), dtype=torch.bfloat16),
+              mins=None, K=64, group=32)
+    qw.update(change)
+    with pytest.raises(RuntimeError, match=text):
+        _ops.gemm_w4(torch.zeros((1, 64), dtype=torch.bfloat16), qw)

@@ -1,0 +1,360 @@
+"""4-bit-weight products on the GPU against the float64 oracle (oracle/w4.py).
+
+Tolerances (derived, not fitted). A product of K terms summed in fp32 in any
+order, scaled per group, costs at most K/4 + 32 effective roundings of 2^-24
+of S, the sum of the terms' magnitudes (groups of at least 16 terms are added
+at once by the tensor cores, which may drop the bits below the largest one:
+two units of 2^-24 per 16 terms and one per group); the result is then
+rounded once (eps/2). Small integers with power-of-two scales are exact and
+compared bit for bit after the one rounding.
+"""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from elastikernel_b200 import _lib, _ops
+from elastikernel_b200.sm_aware_matmul import call_sm_aware_w4
+from oracle import w4 as ow4
+from oracle.moe import route_ref
+
+pytestmark = pytest.mark.gpu
+
+BF, FP = torch.bfloat16, torch.float16
+
+
+def _np(t):
+    return t.double().cpu().numpy()
+
+
+def _integer_weight(N, K, group, mins, dtype, seed, dev, lead=()):
+    """Random codes with power-of-two scales (and small integer minima)."""
+    g = torch.Generator().manual_seed(seed)
+    shape = lead + (N,)
+    G = -(-K // group)
+    codes = torch.randint(0, 256, shape + (-(-K // 32) * 16,), generator=g, dtype=torch.uint8)  # padding codes too
+    scales = (2.0 ** torch.randint(-2, 2, shape + (G,), generator=g)).to(dtype)
+    m = torch.randint(-3, 4, shape + (G,), generator=g).to(dtype) if mins else None
+    return {"codes": codes.to(dev), "scales": scales.to(dev), "mins": None if m is None else m.to(dev), "K": K,
+            "group": group}
+
+
+def _values(qw):
+    return ow4.values(qw["codes"], qw["scales"], qw["mins"], qw["K"], qw["group"])
+
+
+def _bound(qw):
+    return ow4.abs_bound(qw["codes"], qw["scales"], qw["mins"], qw["K"], qw["group"])
+
+
+def _close(got, exact, S, K, extra=0.0):
+    eps = torch.finfo(got.dtype).eps / 2
+    tiny = torch.finfo(got.dtype).smallest_normal * torch.finfo(got.dtype).eps
+    err = np.abs(_np(got) - exact)
+    bound = eps * np.abs(exact) * (1 + 2.0 ** -8) + (K / 4 + 32) * 2.0 ** -24 * S + extra + tiny
+    assert np.isfinite(_np(got)).all()
+    assert (err <= bound).all(), f"worst {np.max(err - bound):.3e} over its bound"
+
+
+# ------------------------------------------------------------------ quantisation
+@pytest.mark.parametrize("symmetric", [True, False])
+@pytest.mark.parametrize("N,K,group,src,dtype", [
+    (1, 1, 32, torch.float32, BF), (7, 31, 32, BF, BF), (16, 128, 128, FP, FP), (33, 200, 64, torch.float32, FP),
+    (5, 4096, 128, BF, BF), (300, 257, 128, torch.float32, BF), (3, 160, 32, FP, BF)])
+def test_quantise_is_bit_exact(N, K, group, symmetric, src, dtype, cuda_dev):
+    g = torch.Generator().manual_seed(N + K)
+    w = (torch.randn((N, K), generator=g) * 0.02).to(src)
+    w[0] = 0
+    if N > 2:
+        w[1] = 0.5      # a constant row: no range
+        w[2] *= 1e-9    # scales that fp16 cannot hold
+    qw = _ops.quant_w4(w.to(cuda_dev), group, symmetric, dtype)
+    codes, s, m = ow4.quantise(w, group, symmetric, dtype)
+    assert torch.equal(qw["codes"].cpu(), codes)
+    assert torch.equal(qw["scales"].cpu(), s)
+    assert (qw["mins"] is None) if symmetric else torch.equal(qw["mins"].cpu(), m)
+    v = torch.from_numpy(ow4.values(codes, s, m, K, group))
+    # the fp32 value s * q + m is rounded once more to dtype
+    d = _ops.dequant_w4(qw).double().cpu()
+    assert ((d - v).abs() <= (torch.finfo(dtype).eps / 2 + 2.0 ** -23) * v.abs() + 2.0 ** -25).all()
+
+
+def test_quantise_extremes(cuda_dev):
+    w = torch.tensor([[3e38, -3e38] + [0.0] * 30], device=cuda_dev)
+    for sym in (True, False):
+        qw = _ops.quant_w4(w, 32, sym, FP)
+        assert qw["scales"].isfinite().all() and _ops.dequant_w4(qw).isfinite().sum() >= 30
+    qw = _ops.quant_w4(torch.empty((0, 64), device=cuda_dev), 32)
+    assert qw["codes"].shape == (0, 32) and _ops.dequant_w4(qw).shape == (0, 64)
+
+
+# ------------------------------------------------------------------ dense products
+GEMM = [  # M, N, K, group
+    (1, 1, 1, 32), (1, 16, 128, 128), (1, 4096, 4096, 128), (2, 33, 96, 32), (3, 100, 257, 64), (5, 17, 1000, 128),
+    (8, 130, 4096, 128), (9, 48, 2048, 64), (16, 2304, 512, 32), (17, 65, 7168, 128), (33, 129, 640, 64),
+    (64, 256, 1024, 128), (65, 40, 130, 32), (100, 24, 512, 128), (1, 28672, 256, 128), (7, 64, 14336, 128),
+    (200, 136, 384, 64),
+]
+
+
+@pytest.mark.parametrize("mins", [False, True])
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("M,N,K,group", GEMM)
+def test_gemm_integers_exact(M, N, K, group, dtype, mins, cuda_dev):
+    qw = _integer_weight(N, K, group, mins, dtype, M + N + K, cuda_dev)
+    g = torch.Generator().manual_seed(K)
+    x = torch.randint(-2, 3, (M, K), generator=g).to(dtype)
+    got = _ops.gemm_w4(x.to(cuda_dev), qw)
+    exact = torch.from_numpy(_np(x) @ _values(qw).T)  # multiples of 1/4 below 2^20: exact in fp32
+    assert torch.equal(got.cpu(), exact.to(dtype))
+
+
+@pytest.mark.parametrize("symmetric", [True, False])
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("M,N,K,group", GEMM)
+def test_gemm_random(M, N, K, group, dtype, symmetric, cuda_dev):
+    g = torch.Generator().manual_seed(M * 7 + K)
+    w = torch.randn((N, K), generator=g) / K ** 0.5
+    x = (torch.randn((M, K), generator=g) + 0.5).to(dtype)
+    qw = _ops.quant_w4(w.to(cuda_dev), group, symmetric, dtype)
+    got = _ops.gemm_w4(x.to(cuda_dev), qw)
+    _close(got, _np(x) @ _values(qw).T, np.abs(_np(x)) @ _bound(qw).T, K)
+    out = torch.full((M, N), 9.0, dtype=dtype, device=cuda_dev)
+    assert _ops.gemm_w4(x.to(cuda_dev), qw, out=out) is out and torch.equal(out, got)
+
+
+def test_gemm_rows_do_not_mix(cuda_dev):
+    """A non-finite token spoils its own output row alone; infinite and NaN
+    values beyond K or M are never read."""
+    M, N, K = 5, 70, 200
+    qw = _ops.quant_w4(torch.randn((N, K), device=cuda_dev), 64)
+    buf = torch.full((M * K + 64,), float("nan"), dtype=BF, device=cuda_dev)
+    x = buf[8:8 + M * K].view(M, K)
+    x.copy_(torch.randn((M, K), device=cuda_dev))
+    clean = _ops.gemm_w4(x.clone(), qw)
+    assert torch.equal(_ops.gemm_w4(x, qw), clean)
+    x[3, 7] = float("inf")
+    got = _ops.gemm_w4(x, qw)
+    keep = [0, 1, 2, 4]
+    assert torch.equal(got[keep], clean[keep]) and not got[3].isfinite().any()
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_gemm_misaligned_views(dtype, cuda_dev):
+    for M, N, K in ((1, 64, 256), (4, 50, 257), (20, 33, 130)):
+        qw = _integer_weight(N, K, 32, True, dtype, 1, cuda_dev)
+        x = torch.randint(-2, 3, (M * K + 1,), device=cuda_dev).to(dtype)[1:].view(M, K)
+        out = torch.empty((M * N + 1,), dtype=dtype, device=cuda_dev)[1:].view(M, N)
+        _ops.gemm_w4(x, qw, out=out)
+        assert torch.equal(out, _ops.gemm_w4(x.clone(), qw))
+        assert torch.equal(out.cpu(), torch.from_numpy(_np(x) @ _values(qw).T).to(dtype))
+
+
+def test_gemm_large_values_and_scales(cuda_dev):
+    """fp16 tokens near the type's limit against tiny scales: no overflow on the way."""
+    K = 512
+    x = torch.full((2, K), 6e4, dtype=FP, device=cuda_dev)
+    qw = _integer_weight(24, K, 64, False, FP, 4, cuda_dev)
+    qw["scales"] = torch.full_like(qw["scales"], 2.0 ** -20)
+    _close(_ops.gemm_w4(x, qw), _np(x) @ _values(qw).T, np.abs(_np(x)) @ _bound(qw).T, K)
+
+
+def test_gemm_past_2_31_weights(cuda_dev):
+    N, K = 270000, 8192  # 2.2e9 weights, 1.1 GB of codes
+    qw = {"codes": torch.randint(0, 256, (N, K // 2), dtype=torch.uint8, device=cuda_dev),
+          "scales": torch.ones((N, K // 128), dtype=BF, device=cuda_dev), "mins": None, "K": K, "group": 128}
+    x = torch.zeros((1, K), dtype=BF, device=cuda_dev)
+    x[0, 5], x[0, K - 1] = 1.0, 2.0
+    got = _ops.gemm_w4(x, qw)
+    want = ((qw["codes"][:, 2] >> 4).float() - 8) + 2 * ((qw["codes"][:, -1] >> 4).float() - 8)
+    assert torch.equal(got[0], want.to(BF))
+
+
+def test_gemm_on_a_partition_and_in_a_graph(cuda_dev):
+    from elastikernel_b200.green_ctx import create_sm_partition
+
+    qw = _integer_weight(520, 1024, 128, True, BF, 2, cuda_dev)
+    x = torch.randint(-2, 3, (6, 1024), device=cuda_dev).to(BF)
+    want = torch.from_numpy(_np(x) @ _values(qw).T).to(BF)
+    stream, _ = create_sm_partition(cuda_dev, 32)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        part = call_sm_aware_w4(x, qw)
+    stream.synchronize()
+    assert torch.equal(part.cpu(), want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = _ops.gemm_w4(x, qw)
+    x.neg_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(held.cpu(), -want)
+
+
+def test_gemm_empty_and_refusals(cuda_dev):
+    qw = _integer_weight(16, 64, 32, False, BF, 3, cuda_dev)
+    x = torch.zeros((2, 64), dtype=BF, device=cuda_dev)
+    assert _ops.gemm_w4(x[:0], qw).shape == (0, 16)
+    for call, text in [(lambda: _ops.gemm_w4(x.half(), qw), "scales must be"),
+                       (lambda: _ops.gemm_w4(x[:, :32].contiguous(), qw), r"a \[M, 64\]"),
+                       (lambda: _ops.gemm_w4(x.t().contiguous().t(), qw), "contiguous"),
+                       (lambda: _ops.gemm_w4(x, qw, out=x), "out must be"),
+                       (lambda: _ops.quant_w4(x, 100), "group"),
+                       (lambda: _ops.quant_w4(x.double()), "bf16, fp16 or fp32"),
+                       (lambda: _ops.quant_w4(x, 32, dtype=torch.float32), "dtype")]:
+        with pytest.raises(RuntimeError, match=text):
+            call()
+
+
+# ------------------------------------------------------------------ experts
+MOE = [  # T, k, E, H, I, group, mins
+    (1, 1, 1, 32, 32, 32, False), (1, 2, 8, 4096, 512, 128, False), (3, 2, 4, 200, 136, 64, True),
+    (17, 8, 60, 512, 260, 32, False), (64, 8, 32, 1024, 256, 128, False), (40, 3, 5, 257, 65, 64, True),
+    (300, 2, 4, 256, 384, 128, False), (33, 1, 300, 64, 96, 32, False),
+]
+
+
+def _moe_setup(case, dev):
+    T, k, E, H, I, group, mins = case
+    g = torch.Generator().manual_seed(T + E + H)
+    ws = [torch.randn(s, generator=g) / s[-1] ** 0.5 for s in ((E, I, H), (E, H, I), (E, I, H))]
+    qw = _ops.quant_moe_weights_w4(*(w.to(dev) for w in ws), group=group, symmetric=not mins)
+    x = torch.randn((T, H), generator=g).to(BF).to(dev)
+    ids = torch.topk(torch.randn((T, E), generator=g), k, dim=1).indices.int().to(dev)
+    return x, ids, qw
+
+
+@pytest.mark.parametrize("drop", [False, True])
+@pytest.mark.parametrize("case", MOE, ids=lambda c: f"T{c[0]}k{c[1]}E{c[2]}H{c[3]}I{c[4]}")
+def test_expert_products(case, drop, cuda_dev):
+    """gate/up and down, each against the oracle on its own inputs."""
+    T, k, E, H, I, group, mins = case
+    x, ids, qw = _moe_setup(case, cuda_dev)
+    if drop:
+        ids[::2, 0] = -1
+    p = _ops.moe_dispatch(x, ids, E)
+    kept = int(p["num_rows_padded"])
+    act = _ops.moe_gate_up_w4(p, qw)
+    assert torch.equal(act[:kept], _ops.moe_gate_up_w4(p, qw, x=x)[:kept])  # fetched through the permutation
+    y = _ops.moe_down_w4(p, act, qw)
+    counts = p["expert_counts"].tolist()
+    v = {n: _values(qw[n]) for n in ("w1", "w3", "w2")}
+    b = {n: _bound(qw[n]) for n in ("w1", "w3", "w2")}
+    xp, r = _np(p["x_perm"]), 0
+    for e, c in enumerate(counts):
+        if c:
+            rows = slice(r, r + c)
+            h, u = xp[rows] @ v["w1"][e].T, xp[rows] @ v["w3"][e].T
+            n = (H / 4 + 32) * 2.0 ** -24
+            dh, du = n * (np.abs(xp[rows]) @ b["w1"][e].T), n * (np.abs(xp[rows]) @ b["w3"][e].T)
+            silu = h / (1 + np.exp(-h))
+            # |silu'| <= 1.1; exp, the quotient and the product: 8 roundings of 2^-24
+            extra = 1.1 * dh * (np.abs(u) + du) + np.abs(silu) * du + 8 * 2.0 ** -24 * np.abs(silu * u)
+            _close(act[rows], silu * u, 0.0, 0, extra)
+            a = _np(act[rows])
+            _close(y[rows], a @ v["w2"][e].T, np.abs(a) @ b["w2"][e].T, I)
+        r += c
+    assert r == kept
+
+
+@pytest.mark.parametrize("case", MOE, ids=lambda c: f"T{c[0]}k{c[1]}E{c[2]}H{c[3]}I{c[4]}")
+def test_fused_layer(case, cuda_dev):
+    """The layer against the oracle: act and the experts' rows are bf16, so an
+    output carries their roundings (2^-8 of each term) beside its own."""
+    T, k, E, H, I, group, mins = case
+    if E > 256:
+        pytest.skip("moe_route takes up to 256 experts")
+    x, _, qw = _moe_setup(case, cuda_dev)
+    logits = torch.randn((T, E), generator=torch.Generator().manual_seed(T)).to(cuda_dev)
+    got = _ops.fused_moe_w4(x, logits, qw, k)
+    ids, w = route_ref(logits.cpu().numpy(), k)
+    v = {n: _values(qw[n]) for n in ("w1", "w3", "w2")}
+    exact, spread = np.zeros((T, H)), np.zeros((T, H))
+    for t in range(T):
+        xt = _np(x[t])
+        for j in range(k):
+            e = int(ids[t, j])
+            h = v["w1"][e] @ xt
+            a = h / (1 + np.exp(-h)) * (v["w3"][e] @ xt)
+            y = v["w2"][e] @ a
+            exact[t] += w[t, j] * y
+            spread[t] += w[t, j] * (np.abs(y) + np.abs(v["w2"][e]) @ np.abs(a))
+    # the fp32 sums inside are 2^-24-sized; 1 % on top of the two bf16 roundings covers them
+    bound = 2.0 ** -8 * (np.abs(exact) + 1.01 * spread) + 1e-30
+    assert (np.abs(_np(got) - exact) <= bound).all()
+    p = _ops.moe_dispatch(None, torch.from_numpy(np.asarray(ids, np.int32)).to(cuda_dev), E)
+    y = _ops.moe_down_w4(p, _ops.moe_gate_up_w4(p, qw, x=x), qw)
+    same = _ops.moe_combine_weighted(p, y, _ops.moe_route(logits, k)[1])
+    assert torch.equal(same, got)
+    out = torch.empty_like(x)
+    assert _ops.fused_moe_w4(x, logits, qw, k, out=out) is out and torch.equal(out, got)
+
+
+def test_layer_forward_and_router_backward(cuda_dev):
+    """The operators together, as a router is trained over frozen 4-bit experts:
+    the logits' gradient against differences of the oracle's layer."""
+    T, k, E, H, I = 6, 2, 5, 64, 96
+    x, _, qw = _moe_setup((T, k, E, H, I, 32, False), cuda_dev)
+    g = torch.Generator().manual_seed(11)
+    logits, d_out = torch.randn((T, E), generator=g), torch.randn((T, H), generator=g).to(BF)
+    ids, w = _ops.moe_route(logits.to(cuda_dev), k)
+    p = _ops.moe_dispatch(x, ids, E)
+    y = _ops.moe_down_w4(p, _ops.moe_gate_up_w4(p, qw), qw)
+    d_y, d_w = _ops.moe_combine_weighted_grad(p, y, w, d_out.to(cuda_dev))
+    d_logits = _np(_ops.moe_route_grad(ids, w, d_w, E))
+    rows = _np(y)[p["slot_rows"].cpu().numpy()].reshape(T, k, H)
+    chosen = ids.cpu().numpy().astype(np.int64)
+
+    def loss(z):
+        c = np.take_along_axis(z, chosen, axis=1)
+        c = np.exp(c - c.max(axis=1, keepdims=True))
+        c /= c.sum(axis=1, keepdims=True)
+        return ((c[:, :, None] * rows).sum(axis=1) * _np(d_out)).sum()
+
+    z = logits.double().numpy()
+    for i in np.ndindex(T, E):
+        a, b = z.copy(), z.copy()
+        a[i] += 1e-5
+        b[i] -= 1e-5
+        num = (loss(a) - loss(b)) / 2e-5
+        # differences: h^2 |f'''| ~ 1e-10 |f| and rounding 1e-16 |f| / h; fp32 sums: (H + k) 2^-24 |f|
+        scale = np.abs(rows[i[0]] * _np(d_out)[i[0]]).sum()
+        assert abs(num - d_logits[i]) <= ((H + 16) * 2.0 ** -24 + 1e-9) * scale
+    # and the tokens' gradient of the way in, for rows' gradients that come back from the experts
+    d_x = _ops.moe_dispatch_grad(p, d_y)
+    wts = _np(w)
+    want = (wts.sum(axis=1, keepdims=True) * _np(d_out))
+    # two bf16 roundings: each row's and the sum's
+    assert (np.abs(_np(d_x) - want) <= 2.0 ** -7 * 1.01 * np.abs(want) + 1e-6).all()
+
+
+def test_layer_in_a_graph(cuda_dev):
+    x, _, qw = _moe_setup((9, 2, 8, 256, 128, 64, True), cuda_dev)
+    logits = torch.randn((9, 8), device=cuda_dev)
+    _ops.fused_moe_w4(x, logits, qw, 2)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = _ops.fused_moe_w4(x, logits, qw, 2)
+    for _ in range(2):
+        logits.normal_()
+        x.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(held, _ops.fused_moe_w4(x, logits, qw, 2))
+
+
+def test_layer_empty_and_refusals(cuda_dev):
+    x, ids, qw = _moe_setup((4, 2, 4, 64, 32, 32, False), cuda_dev)
+    assert _ops.fused_moe_w4(x[:0], torch.empty((0, 4), device=cuda_dev), qw, 2).shape == (0, 64)
+    p = _ops.moe_dispatch(None, ids, 4)
+    for call, text in [(lambda: _ops.moe_gate_up_w4(p, qw), "no rows"),
+                       (lambda: _ops.moe_gate_up_w4(p, qw, x=x[:3]), "shape"),
+                       (lambda: _ops.moe_gate_up_w4(p, qw, x=x.half()), "bfloat16"),
+                       (lambda: _ops.moe_down_w4(p, x, qw), "shape"),
+                       (lambda: _ops.moe_gate_up_w4(_ops.moe_permute(ids, 4, x=x), qw), "shape"),
+                       (lambda: _ops.fused_moe_w4(x, torch.empty((4, 3), device=cuda_dev), qw, 2), "gate_logits"),
+                       (lambda: _ops.quant_moe_weights_w4(*[torch.zeros((2, 8, 32), device=cuda_dev)] * 3), "w2")]:
+        with pytest.raises(RuntimeError, match=text):
+            call()
+    assert _lib.device_status(0) == 0
