@@ -124,9 +124,12 @@ _SIGNATURES = {
     "ek_moe_route_grad": (_c_int, [_c_vp] * 3 + [_c_int] * 3 + [_c_vp, _c_vp]),
     "ek_quant_w4": (_c_int, [_c_vp, _c_int, ctypes.c_longlong] + [_c_int] * 4 + [_c_vp] * 4),
     "ek_dequant_w4": (_c_int, [_c_vp] * 3 + [ctypes.c_longlong] + [_c_int] * 3 + [_c_vp, _c_vp]),
-    "ek_gemm_w4": (_c_int, [_c_vp] * 5 + [_c_int] * 6 + [_c_vp]),
-    "ek_moe_gate_up_w4": (_c_int, [_c_vp, _c_vp, _c_int, _c_int] + [_c_vp] * 8 + [_c_int] * 6 + [_c_vp]),
-    "ek_moe_down_w4": (_c_int, [_c_vp] * 6 + [_c_int] * 6 + [_c_vp]),
+    "ek_gemm_w4_workspace_bytes": (_c_size, [_c_int] * 4),
+    "ek_gemm_w4": (_c_int, [_c_vp] * 5 + [_c_int] * 6 + [_c_vp, _c_size, _c_vp]),
+    "ek_moe_w4_workspace_bytes": (_c_size, [_c_int] * 6),
+    "ek_moe_gate_up_w4": (_c_int, [_c_vp, _c_int, _c_vp, _c_int] + [_c_vp] * 8 + [_c_int] * 7 + [_c_vp, _c_size, _c_vp]),
+    "ek_moe_down_w4": (_c_int, [_c_vp, _c_int] + [_c_vp] * 5 + [_c_int] * 7 + [_c_vp, _c_size, _c_vp]),
+    "ek_moe_experts_w4": (_c_int, [_c_vp, _c_int, _c_int] + [_c_vp] * 15 + [_c_int] * 5 + [_c_vp, _c_size, _c_vp]),
     "ek_moe_segment_gemm": (_c_int, [_c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
                                      _c_vp]),
 }

@@ -862,7 +862,11 @@ def dequant_w4(qw: dict) -> torch.Tensor:
 
 def gemm_w4(a: torch.Tensor, qw: dict, out: torch.Tensor | None = None, num_sms: int | None = None) -> torch.Tensor:
     """C = a @ W^T with a [M, K] (bf16 or fp16) and a 4-bit weight W [N, K]
-    (quant_w4) whose scales have a's dtype; C [M, N] in that dtype, fp32 sums."""
+    (quant_w4) whose scales have a's dtype; C [M, N] in that dtype, fp32 sums.
+
+    Made for a few tokens; any M is right, but from a few hundred rows
+    gemm(a, dequant_w4(qw), b_layout="nk") is faster (with the weights rounded
+    to a's dtype, which this product does not do)."""
     codes, scales, mins, lead, K, group = _check_w4("gemm_w4", qw, a.dtype)
     dev = _require_cuda(a, codes, scales, mins, out)
     if a.dim() != 2 or a.shape[1] != K or len(lead) != 1:
@@ -873,10 +877,24 @@ def gemm_w4(a: torch.Tensor, qw: dict, out: torch.Tensor | None = None, num_sms:
         out = torch.empty((M, N), device=dev, dtype=a.dtype)
     elif tuple(out.shape) != (M, N) or out.dtype != a.dtype or not out.is_contiguous():
         raise RuntimeError("out must be a contiguous [M, N] tensor of the input dtype")
+    if M == 0 or N == 0:
+        return out
+    L = lib()
+    stream = current_stream_handle(dev)
+    sms = int(num_sms) if num_sms else _stream_sms(dev, stream)
+    ws = _scratch(L.ek_gemm_w4_workspace_bytes(M, N, K, sms), dev)
     with _on_device(dev):
-        check(lib().ek_gemm_w4(a.data_ptr(), codes.data_ptr(), scales.data_ptr(), _ptr(mins), out.data_ptr(), M, N, K,
-                               group, _DTYPES[a.dtype], int(num_sms or 0), current_stream_handle(dev)), "ek_gemm_w4")
+        check(L.ek_gemm_w4(a.data_ptr(), codes.data_ptr(), scales.data_ptr(), _ptr(mins), out.data_ptr(), M, N, K,
+                           group, _DTYPES[a.dtype], sms, ws.data_ptr(), ws.numel(), stream), "ek_gemm_w4")
     return out
+
+
+def _scratch(nbytes: int, dev: torch.device) -> torch.Tensor:
+    """Workspace of one call, from torch's allocator: nothing in it outlives the
+    call, and a captured graph gets its own."""
+    if nbytes == _SIZE_MAX:
+        check(_lib.EK_ERR_INVALID, "workspace size")
+    return torch.empty(nbytes, dtype=torch.uint8, device=dev)
 
 
 def quant_moe_weights_w4(w1: torch.Tensor, w2: torch.Tensor, w3: torch.Tensor, group: int = 128,
@@ -889,56 +907,121 @@ def quant_moe_weights_w4(w1: torch.Tensor, w2: torch.Tensor, w3: torch.Tensor, g
     return {"E": E, "H": H, "I": I, **q}
 
 
-def moe_gate_up_w4(perm: dict, qw: dict, x: torch.Tensor | None = None, num_sms: int | None = None) -> torch.Tensor:
+_ACT_DTYPES = {torch.bfloat16: _lib.EK_DTYPE_BF16, torch.float32: _lib.EK_DTYPE_FP32}
+
+
+def _check_experts(qw: dict, *names: str) -> list:
+    """(codes, scales, mins) of the named expert weights, checked against qw's E, H, I."""
+    E, H, I = qw["E"], qw["H"], qw["I"]
+    out, kinds = [], set()
+    for name in names:
+        c, s, m, lead, K, group = _check_w4(name, qw[name], torch.bfloat16)
+        if lead != ((E, H) if name == "w2" else (E, I)) or K != (I if name == "w2" else H):
+            raise RuntimeError(f"{name}: shape mismatch")
+        kinds.add((group, m is None))
+        out.append((c, s, m, group))
+    if len(kinds) != 1:
+        raise RuntimeError("the experts' weights must share one group and be all symmetric or all with minima")
+    return out
+
+
+def moe_gate_up_w4(perm: dict, qw: dict, x: torch.Tensor | None = None, num_sms: int | None = None,
+                   dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """act[r] = silu(row . w1[e]) * (row . w3[e]) over the packed rows, 4-bit experts.
     The rows are perm["x_perm"], or with x (the tokens [T, H]) fetched through
-    the permutation, so nothing has to be copied first. Rows past the last
-    kept one are left unwritten."""
+    the permutation, so nothing has to be copied first. act in `dtype` (bf16
+    or fp32). Rows past the last kept one are left unwritten."""
     E, H, I = qw["E"], qw["H"], qw["I"]
-    c1, s1, m1, l1, k1, group = _check_w4("w1", qw["w1"], torch.bfloat16)
-    c3, s3, m3, l3, k3, g3 = _check_w4("w3", qw["w3"], torch.bfloat16)
+    (c1, s1, m1, group), (c3, s3, m3, _) = _check_experts(qw, "w1", "w3")
     src = perm["x_perm"] if x is None else x
     if src is None:
         raise RuntimeError("moe_gate_up_w4: the permutation has no rows; give x")
     dev = _require_cuda(src, c1, s1, m1, c3, s3, m3, perm["expert_counts"])
     _check_bf16("x", src)
-    rows = perm["max_rows"]
-    if l1 != (E, I) or l3 != l1 or k1 != H or k3 != H or g3 != group or (m1 is None) != (m3 is None) or \
-            perm["E"] != E or tuple(src.shape) != (rows if x is None else perm["T"], H) or perm["block_m"] != 1:
+    rows, x_rows = perm["max_rows"], perm["max_rows"] if x is None else perm["T"]
+    if perm["E"] != E or tuple(src.shape) != (x_rows, H) or perm["block_m"] != 1 or dtype not in _ACT_DTYPES:
         raise RuntimeError("gate_up_w4: shape mismatch")
-    act = torch.empty((rows, I), dtype=torch.bfloat16, device=dev)
+    act = torch.empty((rows, I), dtype=dtype, device=dev)
+    L = lib()
+    stream = current_stream_handle(dev)
+    sms = int(num_sms) if num_sms else _stream_sms(dev, stream)
+    ws = _scratch(L.ek_moe_w4_workspace_bytes(x_rows, rows, E, H, I, sms), dev)
     with _on_device(dev):
-        check(lib().ek_moe_gate_up_w4(src.data_ptr(), None if x is None else perm["sorted_slots"].data_ptr(),
-                                      perm["topk"], perm["T"] * perm["topk"], c1.data_ptr(), s1.data_ptr(), _ptr(m1),
-                                      c3.data_ptr(), s3.data_ptr(), _ptr(m3), perm["expert_counts"].data_ptr(),
-                                      act.data_ptr(), rows, E, H, I, group, int(num_sms or 0),
-                                      current_stream_handle(dev)), "ek_moe_gate_up_w4")
+        check(L.ek_moe_gate_up_w4(src.data_ptr(), x_rows, None if x is None else perm["sorted_slots"].data_ptr(),
+                                  1 if x is None else perm["topk"], c1.data_ptr(), s1.data_ptr(), _ptr(m1),
+                                  c3.data_ptr(), s3.data_ptr(), _ptr(m3), perm["expert_counts"].data_ptr(),
+                                  act.data_ptr(), _ACT_DTYPES[dtype], rows, E, H, I, group, sms, ws.data_ptr(),
+                                  ws.numel(), stream), "ek_moe_gate_up_w4")
     return act
 
 
-def moe_down_w4(perm: dict, act: torch.Tensor, qw: dict, num_sms: int | None = None) -> torch.Tensor:
+def moe_down_w4(perm: dict, act: torch.Tensor, qw: dict, num_sms: int | None = None,
+                dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """y[r] = act[r] . w2[e] over the packed rows, 4-bit experts (no routing
-    weight: moe_combine_weighted applies it). Rows past the last are left unwritten."""
+    weight: moe_combine_weighted applies it), in `dtype` (bf16 or fp32); act is
+    bf16 or fp32. Rows past the last are left unwritten."""
     E, H, I = qw["E"], qw["H"], qw["I"]
-    c2, s2, m2, l2, k2, group = _check_w4("w2", qw["w2"], torch.bfloat16)
+    ((c2, s2, m2, group),) = _check_experts(qw, "w2")
     dev = _require_cuda(act, c2, s2, m2, perm["expert_counts"])
-    _check_bf16("act", act)
+    _contig("act", act)
     rows = perm["max_rows"]
-    if l2 != (E, H) or k2 != I or perm["E"] != E or tuple(act.shape) != (rows, I) or perm["block_m"] != 1:
+    if perm["E"] != E or tuple(act.shape) != (rows, I) or perm["block_m"] != 1 or act.dtype not in _ACT_DTYPES or \
+            dtype not in _ACT_DTYPES:
         raise RuntimeError("down_w4: shape mismatch")
-    y = torch.empty((rows, H), dtype=torch.bfloat16, device=dev)
+    y = torch.empty((rows, H), dtype=dtype, device=dev)
+    L = lib()
+    stream = current_stream_handle(dev)
+    sms = int(num_sms) if num_sms else _stream_sms(dev, stream)
+    ws = _scratch(L.ek_moe_w4_workspace_bytes(0, rows, E, H, I, sms), dev)
     with _on_device(dev):
-        check(lib().ek_moe_down_w4(act.data_ptr(), c2.data_ptr(), s2.data_ptr(), _ptr(m2),
-                                   perm["expert_counts"].data_ptr(), y.data_ptr(), rows, E, H, I, group,
-                                   int(num_sms or 0), current_stream_handle(dev)), "ek_moe_down_w4")
+        check(L.ek_moe_down_w4(act.data_ptr(), _ACT_DTYPES[act.dtype], c2.data_ptr(), s2.data_ptr(), _ptr(m2),
+                               perm["expert_counts"].data_ptr(), y.data_ptr(), _ACT_DTYPES[dtype], rows, E, H, I, group,
+                               sms, ws.data_ptr(), ws.numel(), stream), "ek_moe_down_w4")
     return y
+
+
+def moe_experts_w4(perm: dict, x: torch.Tensor, topk_ids: torch.Tensor, topk_weights: torch.Tensor, qw: dict,
+                   out: torch.Tensor | None = None, num_sms: int | None = None) -> torch.Tensor:
+    """The experts' part of a layer over 4-bit weights: gate/up, down and the
+    weighted combine for the tokens x [T, H] (bf16) and a moe_dispatch order of
+    topk_ids. Activations and the experts' rows stay in the workspace (11
+    significant bits and fp32); the output [T, H] is rounded once."""
+    E, H, I = qw["E"], qw["H"], qw["I"]
+    (c1, s1, m1, group), (c3, s3, m3, _), (c2, s2, m2, _) = _check_experts(qw, "w1", "w3", "w2")
+    slot_rows = _slot_rows(perm)
+    dev = _require_cuda(x, topk_ids, topk_weights, c1, s1, m1, c3, s3, m3, c2, s2, m2, slot_rows, out)
+    _check_bf16("x", x)
+    T, k = perm["T"], perm["topk"]
+    _check_slots("topk_ids", topk_ids, T, k, torch.int32)
+    _check_slots("topk_weights", topk_weights, T, k, torch.float32)
+    if perm["E"] != E or tuple(x.shape) != (T, H):
+        raise RuntimeError("experts_w4: shape mismatch")
+    if out is None:
+        out = torch.empty_like(x)
+    else:
+        _check_bf16("out", out)
+        if out.shape != x.shape:
+            raise RuntimeError("out must be a [T, H] tensor")
+    if T == 0:
+        return out
+    L = lib()
+    stream = current_stream_handle(dev)
+    sms = int(num_sms) if num_sms else _stream_sms(dev, stream)
+    ws = _scratch(L.ek_moe_w4_workspace_bytes(T, T * k, E, H, I, sms), dev)
+    with _on_device(dev):
+        check(L.ek_moe_experts_w4(x.data_ptr(), T, k, topk_ids.data_ptr(), topk_weights.data_ptr(),
+                                  perm["sorted_slots"].data_ptr(), slot_rows.data_ptr(),
+                                  perm["expert_counts"].data_ptr(), c1.data_ptr(), s1.data_ptr(), _ptr(m1),
+                                  c3.data_ptr(), s3.data_ptr(), _ptr(m3), c2.data_ptr(), s2.data_ptr(), _ptr(m2),
+                                  out.data_ptr(), E, H, I, group, sms, ws.data_ptr(), ws.numel(), stream),
+              "ek_moe_experts_w4")
+    return out
 
 
 def fused_moe_w4(hidden_states: torch.Tensor, gate_logits: torch.Tensor, qw: dict, topk: int,
                  out: torch.Tensor | None = None, num_sms: int | None = None) -> torch.Tensor:
     """MoE layer over 4-bit experts (quant_moe_weights_w4), for batches of a few
-    tokens per expert: route -> expert order -> gate/up SwiGLU and down over
-    the codes -> weighted combine. act and the experts' rows are bf16."""
+    tokens per expert: route -> expert order -> moe_experts_w4."""
     _require_cuda(hidden_states, gate_logits, out)
     _check_bf16("hidden_states", hidden_states)
     T = hidden_states.shape[0]
@@ -948,9 +1031,7 @@ def fused_moe_w4(hidden_states: torch.Tensor, gate_logits: torch.Tensor, qw: dic
         return out if out is not None else torch.empty_like(hidden_states)
     ids, wts = moe_route(gate_logits, topk)
     perm = moe_dispatch(None, ids, qw["E"])
-    act = moe_gate_up_w4(perm, qw, x=hidden_states, num_sms=num_sms)
-    y = moe_down_w4(perm, act, qw, num_sms=num_sms)
-    return moe_combine_weighted(perm, y, wts, out=out)
+    return moe_experts_w4(perm, hidden_states, ids, wts, qw, out=out, num_sms=num_sms)
 
 
 def moe_segment_gemm(hidden_states: torch.Tensor, weights: torch.Tensor, expert_offsets: torch.Tensor,

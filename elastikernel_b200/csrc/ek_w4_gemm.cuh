@@ -1,0 +1,53 @@
+// The dense product of one element type (a translation unit each).
+#pragma once
+#include "ek_w4_kernel.cuh"
+
+namespace ek {
+namespace w4 {
+
+struct GemmArgs {
+  const void *A, *codes, *scales, *mins;
+  void* C;
+  int M, N, K, group, sms;
+  void* workspace;
+  cudaStream_t stream;
+};
+
+inline Layout gemm_layout(int M, int N, int K, int sms, int* nt, int* grid) {
+  *nt = pick_nt(M, 1);
+  *grid = sms * occupancy(*nt);
+  const long long tiles = (long long)max_token_tiles(M, 0, *nt) * ((N + kRows - 1) / kRows);
+  return layout(M, K, tiles, *grid, 8 * *nt);
+}
+
+int gemm_bf16(const GemmArgs& a);
+int gemm_fp16(const GemmArgs& a);
+
+template <class T>
+int gemm(const GemmArgs& a) {
+  int nt = 0, grid = 0;
+  const Layout l = gemm_layout(a.M, a.N, a.K, a.sms, &nt, &grid);
+  uint8_t* ws = static_cast<uint8_t*>(a.workspace);
+  Params<T> p = {};
+  p.w[0] = {static_cast<const T*>(a.scales), static_cast<const T*>(a.mins)};
+  p.K = a.K;
+  p.N = a.N;
+  p.feature_tiles = (a.N + kRows - 1) / kRows;
+  p.x = {reinterpret_cast<__half*>(ws), reinterpret_cast<float*>(ws + l.scales)};
+  p.n_rows = a.M;
+  p.max_y = max_token_tiles(a.M, 0, nt);
+  p.parts = reinterpret_cast<float*>(ws + l.parts);
+  CUtensorMap map;
+  int rc = codes_map(&map, a.codes, a.N, a.K, kRows);
+  if (!rc) rc = launch_tokens(static_cast<const T*>(a.A), a.M, a.K, p.x, a.stream, true);
+  if (!rc) rc = launch_product<T, kDense>(nt, a.group, map, map, p, grid, a.stream);
+  if (rc) return rc;
+  const dim3 g(p.feature_tiles, std::min(p.max_y * 8 * nt, 4096));
+  T* out = static_cast<T*>(a.C);
+  if (nt == 1) return launch("w4 sums launch", finish_kernel<kDense, 8, T, T>, g, kRows, 0, a.stream, false, p, grid, out);
+  if (nt == 2) return launch("w4 sums launch", finish_kernel<kDense, 16, T, T>, g, kRows, 0, a.stream, false, p, grid, out);
+  return launch("w4 sums launch", finish_kernel<kDense, 32, T, T>, g, kRows, 0, a.stream, false, p, grid, out);
+}
+
+}  // namespace w4
+}  // namespace ek

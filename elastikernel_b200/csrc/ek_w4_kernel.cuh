@@ -1,0 +1,865 @@
+// Products of a few token rows with 4-bit weights on the tensor cores.
+//
+// out[tok, n] = sum_k x[tok, k] w[n, k], w = s (q - 8) or s q + m per group of
+// 32, 64 or 128 k. The codes are streamed once from HBM, so the aim is to keep
+// the memory system full while the SM converts: at 6.5 TB/s an SM receives 23
+// bytes (46 weights) per clock, and its integer pipe does 64 operations per
+// clock, so a weight may cost about one. Neither fp32 FMAs (one per weight and
+// token) nor byte-wise unpacking keep up. Hence
+//   * mma.sync m16n8k16 with 16 weight rows as the M side and 8 tokens as the N
+//     side. A code word (8 weights) becomes four half2 registers of exact
+//     integers with one shift, four and/ors (the nibbles over the exponent of
+//     1024) and four half2 operations (which run on the floating-point pipe).
+//     tcgen05 would need the converted tile in shared memory (its M side is 128
+//     rows and it reads no registers), which costs more than the product
+//     itself at these token counts;
+//   * the tokens as fp16 too, whatever their type: a small kernel scales each
+//     run of 256 elements by a power of two so that its largest magnitude lies
+//     in [2^14, 2^15) and writes it in the order the nibbles come out. bf16 has
+//     8 significant bits to fp16's 11 and elements below 2^-29 of the run's
+//     largest lose at most 2^-40 of it, less than the fp32 sums do; fp32 rows
+//     (the experts' activations) are rounded to 11 bits;
+//   * sums of one group in fp32 accumulators, then multiplied by the group's
+//     fp32 scale: both operands are exact, so no weight is ever rounded; the
+//     minima enter as m * sum(x), the sum taken by the same instruction with a
+//     matrix of ones;
+//   * codes by TMA, 32 KB a stage (16 KB boxes and up are what the TMA engine
+//     streams at full bandwidth), from one producer warp to eight consumer
+//     warps of 32 weight rows each;
+//   * the stages of all tiles, laid end to end, are cut into equal runs, one per
+//     CTA, so that a few tiles fill every SM. A CTA leaves its fp32 sums of each
+//     tile, or part of a tile, in the workspace; the launch that follows (the
+//     one that rounds, applies SwiGLU or combines the experts' rows) adds the
+//     parts in K order. An epilogue in the kernel itself cost more: its
+//     registers spill in the main loop, and the last CTA's fence, ticket and
+//     loads lie bare at the end.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <type_traits>
+
+#include "ek_internal.h"
+#include "ek_ptx.cuh"
+
+namespace ek {
+namespace w4 {
+
+constexpr int kPiece = 32;       // elements per 16-byte piece of a code row; divides every group
+constexpr int kStagePieces = 8;  // pieces per pipeline stage: 128 bytes of each row
+constexpr int kStageElems = kStagePieces * kPiece;
+constexpr int kWarps = 8;                    // consumer warps
+constexpr int kThreads = 32 * (kWarps + 1);  // and the producer
+constexpr int kRows = 32 * kWarps;           // weight rows per tile (gate/up: half of each matrix)
+constexpr int kStageBytes = kRows * 128;
+constexpr int kTokenPitch = kStageElems * 2 + 64;  // bytes of a token's run in a stage; + 64: conflict-free reads
+
+__host__ __device__ inline int pieces(int K) { return (K + kPiece - 1) / kPiece; }
+__host__ __device__ inline int groups(int K, int group) { return (K + group - 1) / group; }
+
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f(float v) { return v; }
+template <class T>
+__device__ __forceinline__ T from_f(float v);
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ float from_f<float>(float v) { return v; }
+
+// (w & mask) | 0x6400 6400: the masked nibbles over the exponent of 1024.
+__device__ __forceinline__ uint32_t nibbles(uint32_t w, uint32_t mask) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(0x64006400u));
+  return r;
+}
+
+// Pairs (k = c, c + 4), c = 2 h and 2 h + 1, of a code word as exact fp16
+// integers q - 8 (kMin: q). The low nibble gives 1024 + q, the high one
+// 1024 + 16 q.
+template <bool kMin>
+__device__ __forceinline__ void code_pairs(uint32_t w, int h, uint32_t& lo, uint32_t& hi) {
+  const uint32_t v = h ? w >> 8 : w;
+  const uint32_t a = nibbles(v, 0x000f000fu), b = nibbles(v, 0x00f000f0u);
+  const uint32_t ca = kMin ? 0xe400e400u : 0xe408e408u;  // -1024, -1032
+  const uint32_t cb = kMin ? 0xd400d400u : 0xd480d480u;  // -64, -72
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(a), "r"(ca));
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(hi) : "r"(b), "r"(0x2c002c00u), "r"(cb));  // 1/16
+}
+
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// The same with a zero accumulator.
+__device__ __forceinline__ void mma16816_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+// Arrive on `bar` when this thread's cp.async so far have landed (one of the
+// barrier's expected arrivals).
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+
+// ------------------------------------------------------------------ tokens
+// A row of K elements takes row_halfs(K) halfs of the workspace, zero past K,
+// so that whole stages can be read; a warp reads up to a stage ahead, hence the
+// slack behind the last row.
+__host__ __device__ inline int stages(int K) { return (K + kStageElems - 1) / kStageElems; }
+__host__ __device__ inline int row_halfs(int K) { return stages(K) * kStageElems; }
+
+struct Tokens {
+  __half* x;     // [rows][row_halfs(K)], each run of 8 in the order 0 4 1 5 2 6 3 7
+  float* scale;  // [rows][stages(K)]: what each run of 256 was divided by
+};
+
+// The workspace of one product: the tokens, their scales, and the CTAs' sums.
+struct Layout {
+  size_t scales, parts, bytes;
+};
+inline Layout layout(long long rows, int K, long long tiles, int ctas, int tok) {
+  auto up = [](size_t v) { return (v + 255) / 256 * 256; };
+  Layout l;
+  l.scales = up(((size_t)rows * row_halfs(K) + kStageElems) * 2);
+  l.parts = l.scales + up(((size_t)rows * stages(K) + 1) * 4);
+  l.bytes = l.parts + ((size_t)tiles + ctas) * kRows * tok * 4;
+  return l;
+}
+
+__device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void griddep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// A warp writes run `st` of row `row`: eight elements v per lane. The scale
+// comes from the largest finite magnitude, so an infinity or a NaN stays what it
+// is and its neighbours stay finite. kScaled = false (fp16 rows): as they are.
+template <bool kScaled>
+__device__ __forceinline__ void write_run(const Tokens& out, size_t row, int st, int nst, const float (&v)[8]) {
+  const int lane = threadIdx.x & 31;
+  float f = 1.f, inv = 1.f;
+  if constexpr (kScaled) {
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (fabsf(v[i]) < INFINITY) m = fmaxf(m, fabsf(v[i]));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    // m in [2^(b - 127), 2^(b - 126)) -> factor 2^(14 + 127 - b), kept normal
+    const int b = (int)(__float_as_uint(m) >> 23);
+    const int up = m > 0.f ? max(-113, min(126, 14 + 127 - b)) : 0;
+    f = __uint_as_float((uint32_t)(127 + up) << 23);
+    inv = __uint_as_float((uint32_t)(127 - up) << 23);
+  }
+  __half2 h[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(v[i] * f, v[i + 4] * f);
+  *reinterpret_cast<uint4*>(out.x + (row * nst + st) * kStageElems + lane * 8) = *reinterpret_cast<const uint4*>(h);
+  if (lane == 0) out.scale[row * nst + st] = inv;
+}
+
+// Rows of x [rows, K] into tokens, a warp per run. vec: rows of a multiple of
+// 8 elements on a 16-byte base.
+template <class T>
+__global__ void __launch_bounds__(256)
+    tokens_kernel(const T* __restrict__ x, int rows, int K, bool vec, Tokens out) {
+  griddep_launch();
+  griddep_wait();
+  const int lane = threadIdx.x & 31, nst = stages(K);
+  const long long warps = ((long long)gridDim.x * blockDim.x) >> 5;
+  for (long long u = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5; u < (long long)rows * nst; u += warps) {
+    const int row = (int)(u / nst), st = (int)(u - (long long)row * nst);
+    const T* src = x + (size_t)row * K;
+    const int k = st * kStageElems + lane * 8;
+    float v[8];
+    if (vec && k < K) {
+      uint4 raw[sizeof(T) / 2];
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[i] = __ldg(reinterpret_cast<const uint4*>(src + k) + i);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = to_f(reinterpret_cast<const T*>(raw)[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = k + i < K ? to_f(src[k + i]) : 0.f;
+    }
+    write_run<!std::is_same<T, __half>::value>(out, row, st, nst, v);
+  }
+}
+
+// ------------------------------------------------------------------ products
+enum Mode { kDense, kGateUp, kDown };
+
+// Scales and minima [rows, G] of one weight matrix.
+template <class T>
+struct Scales {
+  const T* s;
+  const T* m;  // null: symmetric
+};
+
+template <class T>
+struct Params {
+  Scales<T> w[2];            // gate/up: w1 and w3
+  int K, N;                  // N: weight rows (of an expert; of one matrix)
+  int feature_tiles;         // tiles along N
+  Tokens x;
+  int n_rows;                // token rows: M, or the packed rows
+  int max_y;                 // token tiles there is room for
+  const int* counts;         // rows per expert (null: dense)
+  int E;
+  const int* sorted_slots;   // fetch x through the permutation (null: x holds the rows)
+  int n_slots;
+  int topk;
+  float* parts;
+};
+
+// NT: 8 NT tokens a tile; FL: pieces per group (1, 2 or 4); kMin: minima;
+// STAGES: ring depth; OCC: CTAs per SM it is compiled for.
+template <int NT_, int FL_, bool kMin_, int STAGES_, int OCC_>
+struct Shape {
+  static constexpr int NT = NT_, FL = FL_, STAGES = STAGES_, OCC = OCC_;
+  static constexpr bool kMin = kMin_;
+  static constexpr int kTokens = 8 * NT;
+  static constexpr int kTokenBytes = kTokens * kTokenPitch;  // of a stage
+  static constexpr int kSmem = STAGES * (kStageBytes + kTokenBytes) + 1024;  // + alignment of the swizzled stages
+};
+
+// A token tile: rows [r0, r0 + m) of expert e.
+struct TokenTile {
+  int e, r0, m;
+};
+
+// The packed layout's token tiles of `tok` rows: s_end[e] = tiles of experts
+// 0..e, s_row[e] = first row of expert e, s_row[E] the rows in all (2 E + 1
+// ints of shared memory); returns the tiles in all. Called by one warp.
+__device__ __forceinline__ int expert_tiles(const int* __restrict__ counts, int E, int tok, int* s_end, int* s_row) {
+  const int lane = threadIdx.x & 31;
+  int row = 0, end = 0;
+  for (int e0 = 0; e0 < E; e0 += 32) {
+    const int c = e0 + lane < E ? max(0, __ldg(counts + e0 + lane)) : 0;
+    const int k = (c + tok - 1) / tok;
+    int ci = c, ki = k;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int a = __shfl_up_sync(0xffffffffu, ci, o), b = __shfl_up_sync(0xffffffffu, ki, o);
+      if (lane >= o) {
+        ci += a;
+        ki += b;
+      }
+    }
+    if (e0 + lane < E) {
+      s_end[e0 + lane] = end + ki;
+      s_row[e0 + lane] = row + ci - c;
+    }
+    row += __shfl_sync(0xffffffffu, ci, 31);
+    end += __shfl_sync(0xffffffffu, ki, 31);
+  }
+  if (lane == 0) s_row[E] = row;
+  return end;
+}
+
+template <Mode kMode, int TOK, class T>
+__device__ __forceinline__ TokenTile open_tile(const Params<T>& p, int y, const int* s_end, const int* s_row) {
+  if constexpr (kMode == kDense) {
+    const int r0 = y * TOK;
+    return {0, r0, min(TOK, p.n_rows - r0)};
+  } else {
+    int lo = 0, hi = p.E - 1;  // the first expert whose tiles end past y
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (s_end[mid] > y) hi = mid; else lo = mid + 1;
+    }
+    const int at = (y - (lo ? s_end[lo - 1] : 0)) * TOK, r0 = min(s_row[lo] + at, p.n_rows - 1);
+    return {lo, r0, max(1, min(min(s_row[lo + 1] - s_row[lo] - at, TOK), p.n_rows - r0))};
+  }
+}
+
+// The Tokens row of token i of a tile (the last one where there is none: the
+// columns of a product do not mix, and what has no token is not stored).
+template <class T>
+__device__ __forceinline__ int token_row(const Params<T>& p, const TokenTile& t, int i) {
+  const int r = t.r0 + min(i, t.m - 1);
+  return p.sorted_slots ? min(max(__ldg(p.sorted_slots + r), 0), p.n_slots - 1) / p.topk : r;
+}
+
+// The runs of stages: U stages of tiles of nst, cut for `ctas` CTAs (at most U,
+// so that none is empty).
+struct Runs {
+  long long U;
+  int ctas, nst;
+
+  __device__ __forceinline__ long long begin(int cta) const { return U * cta / ctas; }
+  // The CTA whose run holds stage u: the last one that begins at u or before.
+  __device__ __forceinline__ int owner(long long u) const { return (int)(((u + 1) * ctas - 1) / U); }
+  // Where CTA `cta` leaves its sums of a tile, [token][kRows] floats. Along the
+  // stages each new (tile, CTA) pair raises tile + cta, so the slots are distinct
+  // and there are fewer than tiles + CTAs.
+  template <int TOK>
+  __device__ __forceinline__ float* part(float* parts, int cta, int tile) const {
+    return parts + (size_t)(tile + cta) * (kRows * TOK);
+  }
+};
+
+template <class T, class S, Mode kMode>
+__global__ void __launch_bounds__(kThreads, S::OCC)
+    w4_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUtensorMap map1,
+              const __grid_constant__ Params<T> p) {
+  constexpr int NT = S::NT, FL = S::FL;
+  constexpr int kFeatures = kMode == kGateUp ? kRows / 2 : kRows;  // output features per tile
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t s_full[S::STAGES], s_empty[S::STAGES];
+  __shared__ int s_abort, s_y;
+  uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  uint8_t* smem_x = smem + S::STAGES * kStageBytes;
+  int* s_end = reinterpret_cast<int*>(smem_x + S::STAGES * S::kTokenBytes);
+  int* s_row = s_end + p.E;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+
+  griddep_launch();
+  if (warp == 0) {
+    int y = p.max_y;
+    if (kMode != kDense) y = min(y, expert_tiles(p.counts, p.E, S::kTokens, s_end, s_row));
+    if (lane == 0) {
+      s_y = y;
+      s_abort = 0;
+    }
+  } else if (warp == kWarps && lane == 0) {
+    for (int i = 0; i < S::STAGES; ++i) {
+      mbar_init(&s_full[i], 1 + 32);
+      mbar_init(&s_empty[i], kWarps);
+    }
+    fence_mbar_init();
+    tma_prefetch_desc(&map0);
+    if (kMode == kGateUp) tma_prefetch_desc(&map1);
+  }
+  __syncthreads();
+
+  // This CTA's run of the stages: [u0, u1) of the tiles' stages laid end to end.
+  const int np = pieces(p.K), nst = (np + kStagePieces - 1) / kStagePieces;
+  const long long U = (long long)s_y * p.feature_tiles * nst;
+  const Runs run{U, (int)min((long long)gridDim.x, U), nst};
+  if (blockIdx.x >= run.ctas) return;
+  const long long u0 = run.begin(blockIdx.x), u1 = run.begin(blockIdx.x + 1);
+  int tile = (int)(u0 / nst), st = (int)(u0 - (long long)tile * nst);
+  int y = tile / p.feature_tiles, f = tile - y * p.feature_tiles;
+  int n_units = (int)(u1 - u0);
+
+  if (warp == kWarps) {  // ---------------------------------------------- producer
+    // Two cursors: the codes' (lane 0, by TMA), which starts on the first
+    // stages before the tokens are ready, and the tokens' (all lanes, 16 bytes
+    // of a token's run each).
+    struct Cursor {
+      int st, f, y;
+      TokenTile tl;
+    };
+    auto next = [&](Cursor& c) {
+      if (++c.st == nst) {
+        c.st = 0;
+        if (++c.f == p.feature_tiles) {
+          c.f = 0;
+          if (++c.y < s_y) c.tl = open_tile<kMode, S::kTokens>(p, c.y, s_end, s_row);
+        }
+      }
+    };
+    Cursor cw{st, f, y, open_tile<kMode, S::kTokens>(p, y, s_end, s_row)}, cx = cw;
+    auto copy_codes = [&](int slot) {
+      if (lane == 0) {
+        uint8_t* dst = smem + slot * kStageBytes;
+        mbar_arrive_expect_tx(&s_full[slot], kStageBytes);
+        const int row = cw.tl.e * p.N + cw.f * kFeatures;
+        tma_load_2d(dst, &map0, &s_full[slot], cw.st * 128, row);
+        if (kMode == kGateUp) tma_load_2d(dst + kStageBytes / 2, &map1, &s_full[slot], cw.st * 128, row);
+      }
+      next(cw);
+    };
+    const int ahead = min(S::STAGES, n_units);
+    for (int i = 0; i < ahead; ++i) copy_codes(i);
+    griddep_wait();
+    int slot = 0, my_row = token_row(p, cx.tl, lane);  // lane j: the row of the tile's token j
+    uint32_t parity = 1;
+    for (int i = 0; i < n_units; ++i) {
+      if (i >= ahead) {
+        if (!mbar_wait(&s_empty[slot], parity, &s_abort)) break;
+        copy_codes(slot);
+      }
+      const uint32_t dst = smem_u32(smem_x + slot * S::kTokenBytes) + lane * 16;
+      const __half* src = p.x.x + (size_t)cx.st * kStageElems + lane * 8;
+      for (int j = 0; j < cx.tl.m; ++j)
+        cp_async16(dst + j * kTokenPitch, src + (size_t)__shfl_sync(0xffffffffu, my_row, j) * row_halfs(p.K));
+      cp_async_arrive(&s_full[slot]);
+      const int y0 = cx.y;
+      next(cx);
+      if (cx.y != y0) my_row = token_row(p, cx.tl, lane);
+      if (++slot == S::STAGES) {
+        slot = 0;
+        parity ^= 1;
+      }
+    }
+    cp_async_wait_all();
+    return;
+  }
+
+  // ------------------------------------------------------------------ consumers
+  constexpr int kSG = kStagePieces / FL;             // groups per stage
+  constexpr int kSR = (kSG + 3) / 4;                 // of which lane t holds t, t + 4
+  const int g = lane >> 2, t = lane & 3;
+  const int G = groups(p.K, FL * kPiece);
+  // Set s, row i of this warp: gate/up, matrix s, feature 16 warp + i; else
+  // feature 32 warp + 16 s + i. In shared memory, 128 bytes a row, 16-byte unit
+  // u at u ^ (row % 8) (TMA's 128-byte swizzle).
+  const int set_row = kMode == kGateUp ? warp * 16 : warp * 32;
+  const int set_step = kMode == kGateUp ? kRows / 2 : 16;
+  const uint32_t base = smem_u32(smem);
+  const int lrow = lane & 15, lpiece = lane >> 4;
+  uint32_t lm[kStagePieces / 2];
+#pragma unroll
+  for (int i = 0; i < kStagePieces / 2; ++i)
+    lm[i] = base + (set_row + lrow) * 128 + (((2 * i + lpiece) ^ (lrow & 7)) << 4);
+
+  TokenTile tl = open_tile<kMode, S::kTokens>(p, y, s_end, s_row);
+  // Scales run one stage ahead: first scale of rows g, g + 8 of each set.
+  uint32_t srow[2][2];
+  auto open_scales = [&](int e, int ft) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = ft * kFeatures + set_row + (kMode == kGateUp ? 0 : 16 * s) + g + 8 * h;
+        srow[s][h] = (uint32_t)(e * p.N + min(r, p.N - 1)) * (uint32_t)G;
+      }
+  };
+  const float* xscale[NT][2];  // of the tokens of the columns this lane sums
+  float x_next[NT][2];
+  T s_next[2][2][kSR], m_next[2][2][kSR];
+  auto load_scales = [&](int stage) {
+#pragma unroll
+    for (int i = 0; i < kSR; ++i) {
+      const uint32_t gi = min(stage * kSG + (t + 4 * i) % kSG, G - 1);
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const Scales<T>& w = p.w[kMode == kGateUp ? s : 0];
+          s_next[s][h][i] = __ldg(w.s + (srow[s][h] + gi));
+          if constexpr (S::kMin) m_next[s][h][i] = __ldg(w.m + (srow[s][h] + gi));
+        }
+    }
+  };
+  open_scales(tl.e, f);
+  load_scales(st);
+
+  griddep_wait();  // the weights are older than this launch's predecessor, the tokens are its output
+  auto load_xscales = [&](int stage) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) x_next[n][c] = __ldg(xscale[n][c] + stage);
+  };
+  auto open_tokens = [&](const TokenTile& tk) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) xscale[n][c] = p.x.scale + (size_t)token_row(p, tk, n * 8 + t * 2 + c) * nst;
+  };
+  open_tokens(tl);
+  load_xscales(st);
+  const uint32_t xs = smem_u32(smem_x) + g * kTokenPitch + t * 16;  // this lane's run of 8 of token g
+
+  float tot[2][NT][4] = {};
+  int slot = 0;
+  uint32_t parity = 0;
+  for (; n_units > 0; --n_units) {
+    // what comes after this stage: the next one of the tile, or the next tile's first
+    const bool tile_end = st + 1 == nst;
+    int next_f = f, next_y = y;
+    TokenTile next_tl = tl;
+    if (tile_end && n_units > 1) {
+      if (++next_f == p.feature_tiles) {
+        next_f = 0;
+        next_tl = open_tile<kMode, S::kTokens>(p, ++next_y, s_end, s_row);
+        open_tokens(next_tl);
+      }
+      open_scales(next_tl.e, next_f);
+    }
+    float s_cur[2][2][kSR], m_cur[2][2][kSR];
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < kSR; ++i) {
+          s_cur[s][h][i] = to_f(s_next[s][h][i]);
+          if constexpr (S::kMin) m_cur[s][h][i] = to_f(m_next[s][h][i]);
+        }
+    float x_cur[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) x_cur[n][c] = x_next[n][c];
+    load_scales(tile_end ? 0 : st + 1);
+    load_xscales(tile_end ? 0 : st + 1);
+
+    // A wait that ran out has raised the status word; the sums are then of no
+    // use, but every warp goes on to the end of its run.
+    mbar_wait(&s_full[slot], parity, &s_abort);
+    auto stage = [&](auto blocks) {
+      constexpr int NB = decltype(blocks)::value;  // blocks of 8 tokens there are
+      float part[2][NB][4], xsum[NB][4];
+      uint32_t code[2][4];
+#pragma unroll
+      for (int pp = 0; pp < kStagePieces; ++pp) {
+        if (pp % 2 == 0) {
+#pragma unroll
+          for (int s = 0; s < 2; ++s) ldmatrix4(code[s], lm[pp / 2] + slot * kStageBytes + s * set_step * 128);
+        }
+        uint4 xb[NB];
+#pragma unroll
+        for (int n = 0; n < NB; ++n) xb[n] = lds128(xs + slot * S::kTokenBytes + n * 8 * kTokenPitch + pp * 64);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const uint32_t wa = code[s][2 * (pp % 2)], wb = code[s][2 * (pp % 2) + 1];
+          uint32_t a[4];
+          code_pairs<S::kMin>(wa, 0, a[0], a[2]);
+          code_pairs<S::kMin>(wb, 0, a[1], a[3]);
+#pragma unroll
+          for (int n = 0; n < NB; ++n)
+            if (pp % FL == 0) mma16816_first(part[s][n], a, xb[n].x, xb[n].y);
+            else mma16816(part[s][n], a, xb[n].x, xb[n].y);
+          code_pairs<S::kMin>(wa, 1, a[0], a[2]);
+          code_pairs<S::kMin>(wb, 1, a[1], a[3]);
+#pragma unroll
+          for (int n = 0; n < NB; ++n) mma16816(part[s][n], a, xb[n].z, xb[n].w);
+        }
+        if constexpr (S::kMin) {
+          const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+#pragma unroll
+          for (int n = 0; n < NB; ++n) {
+            if (pp % FL == 0) mma16816_first(xsum[n], ones, xb[n].x, xb[n].y);
+            else mma16816(xsum[n], ones, xb[n].x, xb[n].y);
+            mma16816(xsum[n], ones, xb[n].z, xb[n].w);
+          }
+        }
+        if ((pp + 1) % FL == 0) {
+          const int gi = pp / FL, from = (lane & ~3) + gi % 4;
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            float sv[2], mv[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              sv[h] = __shfl_sync(0xffffffffu, s_cur[s][h][gi / 4], from);
+              if constexpr (S::kMin) mv[h] = __shfl_sync(0xffffffffu, m_cur[s][h][gi / 4], from);
+            }
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                float v = sv[c >> 1] * part[s][n][c];
+                if constexpr (S::kMin) v = fmaf(mv[c >> 1], xsum[n][c], v);
+                tot[s][n][c] = fmaf(x_cur[n][c & 1], v, tot[s][n][c]);
+              }
+          }
+        }
+      }
+    };
+    if constexpr (NT == 1) {
+      stage(std::integral_constant<int, 1>{});
+    } else {
+      const int nb = (tl.m + 7) / 8;
+      if (nb == 1) stage(std::integral_constant<int, 1>{});
+      else if (NT == 2 || nb == 2) stage(std::integral_constant<int, 2>{});
+      else if (nb == 3) stage(std::integral_constant<int, NT < 3 ? NT : 3>{});
+      else stage(std::integral_constant<int, NT>{});
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&s_empty[slot]);
+    if (++slot == S::STAGES) {
+      slot = 0;
+      parity ^= 1;
+    }
+
+    // ---- the tile, or this CTA's part of it, is done
+    if (tile_end || n_units == 1) {
+      float* mine = run.part<S::kTokens>(p.parts, blockIdx.x, y * p.feature_tiles + f) + set_row + g;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int tok = n * 8 + t * 2 + (c & 1);
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            if (tok < tl.m) mine[tok * kRows + s * set_step + (c >> 1) * 8] = tot[s][n][c];
+            tot[s][n][c] = 0.f;
+          }
+        }
+    }
+    st = tile_end ? 0 : st + 1;
+    f = next_f;
+    y = next_y;
+    tl = next_tl;
+  }
+}
+
+// ------------------------------------------------------------------ sums
+// The token tiles, set up by every thread of a CTA that reads the parts.
+template <Mode kMode, int TOK, class T>
+__device__ __forceinline__ Runs open_runs(const Params<T>& p, int grid, int* s_end, int* s_row, int* s_y) {
+  if (threadIdx.x < 32) {
+    int y = p.max_y;
+    if (kMode != kDense) y = min(y, expert_tiles(p.counts, p.E, TOK, s_end, s_row));
+    if (threadIdx.x == 0) *s_y = y;
+  }
+  __syncthreads();
+  const int nst = stages(p.K);
+  const long long U = (long long)*s_y * p.feature_tiles * nst;
+  return {U, (int)min((long long)grid, U), nst};
+}
+
+// Sum of the parts of `tile` at [token][row .. row + kV) in K order (kV = 1, or
+// 8 with row a multiple of 8).
+template <int TOK, int kV>
+__device__ __forceinline__ void sum_parts(const Runs& run, float* parts, int tile, int tok, int row, float (&v)[kV]) {
+  const int c0 = run.owner((long long)tile * run.nst), c1 = run.owner((long long)(tile + 1) * run.nst - 1);
+#pragma unroll
+  for (int i = 0; i < kV; ++i) v[i] = 0.f;
+  constexpr int kB = kV == 1 ? 8 : 2;  // parts whose loads are in flight together
+  for (int c = c0; c <= c1; c += kB) {
+    float b[kB][kV];
+#pragma unroll
+    for (int j = 0; j < kB; ++j)
+      if (c + j <= c1) {
+        const float* q = run.part<TOK>(parts, c + j, tile) + tok * kRows + row;
+        if constexpr (kV == 1) {
+          b[j][0] = __ldg(q);
+        } else {
+#pragma unroll
+          for (int i = 0; i < kV; i += 4) *reinterpret_cast<float4*>(&b[j][i]) = __ldg(reinterpret_cast<const float4*>(q + i));
+        }
+      }
+#pragma unroll
+    for (int j = 0; j < kB; ++j)
+      if (c + j <= c1) {
+#pragma unroll
+        for (int i = 0; i < kV; ++i) v[i] += b[j][i];
+      }
+  }
+}
+
+__device__ __forceinline__ float swiglu(float h, float u) { return h / (1.f + expf(-h)) * u; }
+
+// out[r, n] of a dense product or a down projection, act[r, n] of a gate/up: a
+// CTA per feature tile and token, a thread per feature. `grid`: the product's.
+template <Mode kMode, int TOK, class T, class O>
+__global__ void __launch_bounds__(kRows) finish_kernel(const __grid_constant__ Params<T> p, int grid, O* __restrict__ out) {
+  extern __shared__ int s_index[];
+  __shared__ int s_y;
+  griddep_launch();
+  griddep_wait();
+  int *s_end = s_index, *s_row = s_index + p.E;
+  const Runs run = open_runs<kMode, TOK>(p, grid, s_end, s_row, &s_y);
+  constexpr int kFeatures = kMode == kGateUp ? kRows / 2 : kRows;
+  constexpr int kPer = kRows / kFeatures;  // tokens a CTA takes at a time
+  const int f = blockIdx.x, r = threadIdx.x % kFeatures, n = f * kFeatures + r;
+  if (n >= p.N) return;
+  for (int i = blockIdx.y * kPer + threadIdx.x / kFeatures; i < s_y * TOK; i += gridDim.y * kPer) {
+    const int y = i / TOK, tok = i - y * TOK, tile = y * p.feature_tiles + f;
+    const TokenTile tl = open_tile<kMode, TOK>(p, y, s_end, s_row);
+    if (tok >= tl.m) continue;
+    float a[1], u[1];
+    sum_parts<TOK, 1>(run, p.parts, tile, tok, r, a);
+    if constexpr (kMode == kGateUp) {
+      sum_parts<TOK, 1>(run, p.parts, tile, tok, kFeatures + r, u);
+      a[0] = swiglu(a[0], u[0]);
+    }
+    out[(size_t)(tl.r0 + tok) * p.N + n] = from_f<O>(a[0]);
+  }
+}
+
+// The activations of a gate/up product straight into the tokens of the down
+// projection: a warp per packed row and run of 256 features (two tiles).
+template <int TOK, class T>
+__global__ void __launch_bounds__(256) act_tokens_kernel(const __grid_constant__ Params<T> p, int grid, Tokens act) {
+  extern __shared__ int s_index[];
+  __shared__ int s_y;
+  griddep_launch();
+  griddep_wait();
+  int *s_end = s_index, *s_row = s_index + p.E;
+  const Runs run = open_runs<kGateUp, TOK>(p, grid, s_end, s_row, &s_y);
+  const int lane = threadIdx.x & 31, nst = stages(p.N);
+  const long long warps = ((long long)gridDim.x * blockDim.x) >> 5, total = (long long)s_y * TOK * nst;
+  for (long long w = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5; w < total; w += warps) {
+    const int st = (int)(w % nst), ty = (int)(w / nst), y = ty / TOK, tok = ty - y * TOK;
+    const TokenTile tl = open_tile<kGateUp, TOK>(p, y, s_end, s_row);
+    if (tok >= tl.m) continue;
+    const int n = st * kStageElems + lane * 8, f = n / (kRows / 2);
+    float a[8] = {}, u[8] = {};
+    if (f < p.feature_tiles) {
+      const int tile = y * p.feature_tiles + f;
+      sum_parts<TOK, 8>(run, p.parts, tile, tok, n % (kRows / 2), a);
+      sum_parts<TOK, 8>(run, p.parts, tile, tok, kRows / 2 + n % (kRows / 2), u);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a[i] = n + i < p.N ? swiglu(a[i], u[i]) : 0.f;
+    write_run<true>(act, tl.r0 + tok, st, nst, a);
+  }
+}
+
+// out[t] = sum_j w[t, j] y[row of slot (t, j)] from the parts of the down
+// projection, fp32 in j order, rounded once. A CTA per token and 256 features.
+template <int TOK, class T>
+__global__ void __launch_bounds__(kRows)
+    combine_parts_kernel(const __grid_constant__ Params<T> p, int grid, const int* __restrict__ slot_rows,
+                         const int* __restrict__ ids, const float* __restrict__ weights, int tokens, int topk,
+                         T* __restrict__ out) {
+  extern __shared__ int s_index[];
+  __shared__ int s_y;
+  griddep_launch();
+  griddep_wait();
+  int *s_end = s_index, *s_row = s_index + p.E;
+  const Runs run = open_runs<kDown, TOK>(p, grid, s_end, s_row, &s_y);
+  const int f = blockIdx.x, n = f * kRows + threadIdx.x;
+  if (n >= p.N) return;
+  for (int t = blockIdx.y; t < tokens; t += gridDim.y) {
+    float acc = 0.f;
+    for (int j = 0; j < topk; ++j) {
+      const long long s = (long long)t * topk + j;
+      const int r = __ldg(slot_rows + s), e = __ldg(ids + s);
+      if (r < 0 || r >= p.n_rows || e < 0 || e >= p.E) continue;
+      const int at = r - s_row[e], y = (e ? s_end[e - 1] : 0) + at / TOK;
+      if (at < 0 || y >= min(s_end[e], s_y)) continue;
+      float v[1];
+      sum_parts<TOK, 1>(run, p.parts, y * p.feature_tiles + f, at % TOK, threadIdx.x, v);
+      acc = fmaf(__ldg(weights + s), v[0], acc);
+    }
+    out[(size_t)t * p.N + n] = from_f<T>(acc);
+  }
+}
+
+// ------------------------------------------------------------------ launches
+// One launch that may begin before its predecessor on the stream has ended (the
+// kernels above wait for it themselves), or, with after = true, not.
+template <class... P, class... A>
+int launch(const char* what, void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t stream, bool after,
+           A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = after ? 0 : 1;
+  return check_cuda(cudaLaunchKernelEx(&cfg, kernel, args...), what);
+}
+
+// Tokens of a tile for `rows` token rows over `experts` weight matrices: blocks
+// of 8 up to 32, to hold the mean and two standard deviations of an even
+// spread, so that few experts need a second tile (which streams the codes
+// again). The kernel computes only the blocks a tile has.
+inline int pick_nt(long long rows, int experts) {
+  const double used = (double)std::max<long long>(1, std::min<long long>(experts, rows));
+  const double mean = rows / used, want = experts > 1 ? mean + 2.0 * std::sqrt(mean) : mean;
+  return want <= 8 ? 1 : want <= 16 ? 2 : 4;
+}
+inline int occupancy(int nt) { return nt <= 2 ? 2 : 1; }
+
+inline int max_token_tiles(long long rows, int experts, int nt) {
+  const int tok = 8 * nt;
+  if (experts <= 0) return (int)((rows + tok - 1) / tok);
+  return (int)std::min<long long>(rows, std::min<long long>(experts, rows) + rows / tok);
+}
+
+template <class T, class S, Mode kMode>
+int launch_product_shape(const CUtensorMap& a, const CUtensorMap& b, const Params<T>& p, int grid, cudaStream_t stream) {
+  static bool attr_done[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return set_error(EK_ERR_CUDA, "device index out of range");
+  constexpr int kIndexMax = (2 * 1024 + 1) * (int)sizeof(int);
+  if (!attr_done[dev]) {
+    const int rc = check_cuda(cudaFuncSetAttribute(w4_kernel<T, S, kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   S::kSmem + (kMode == kDense ? 0 : kIndexMax)),
+                              "cudaFuncSetAttribute(w4)");
+    if (rc) return rc;
+    attr_done[dev] = true;
+  }
+  return launch("w4 product launch", w4_kernel<T, S, kMode>, dim3(grid), kThreads,
+                S::kSmem + (kMode == kDense ? 0 : (2 * p.E + 1) * sizeof(int)), stream, false, a, b, p);
+}
+
+template <class T, Mode kMode, int FL, bool kMin>
+int launch_product_nt(int nt, const CUtensorMap& a, const CUtensorMap& b, const Params<T>& p, int grid, cudaStream_t stream) {
+  if (nt == 1) return launch_product_shape<T, Shape<1, FL, kMin, 2, 2>, kMode>(a, b, p, grid, stream);
+  if (nt == 2) return launch_product_shape<T, Shape<2, FL, kMin, 2, 2>, kMode>(a, b, p, grid, stream);
+  return launch_product_shape<T, Shape<4, FL, kMin, 4, 1>, kMode>(a, b, p, grid, stream);
+}
+
+// The product over the tokens p.x, its sums left in p.parts.
+template <class T, Mode kMode>
+int launch_product(int nt, int group, const CUtensorMap& a, const CUtensorMap& b, const Params<T>& p, int grid,
+                   cudaStream_t stream) {
+  const bool mins = p.w[0].m != nullptr;
+  switch (group) {
+    case 32:
+      return mins ? launch_product_nt<T, kMode, 1, true>(nt, a, b, p, grid, stream)
+                  : launch_product_nt<T, kMode, 1, false>(nt, a, b, p, grid, stream);
+    case 64:
+      return mins ? launch_product_nt<T, kMode, 2, true>(nt, a, b, p, grid, stream)
+                  : launch_product_nt<T, kMode, 2, false>(nt, a, b, p, grid, stream);
+    default:
+      return mins ? launch_product_nt<T, kMode, 4, true>(nt, a, b, p, grid, stream)
+                  : launch_product_nt<T, kMode, 4, false>(nt, a, b, p, grid, stream);
+  }
+}
+
+template <class T>
+int launch_tokens(const T* x, int rows, int K, const Tokens& out, cudaStream_t stream, bool after) {
+  const long long warps = (long long)rows * stages(K);
+  const bool vec = K % 8 == 0 && aligned16(x);
+  return launch("w4 tokens launch", tokens_kernel<T>, dim3((unsigned)std::min<long long>((warps + 7) / 8, 148 * 16)), 256, 0,
+                stream, after, x, rows, K, vec, out);
+}
+
+// Codes [rows, K] as the TMA sees them: boxes of `box` rows x 128 bytes.
+inline int codes_map(CUtensorMap* m, const void* codes, long long rows, int K, int box) {
+  const uint64_t pitch = (uint64_t)pieces(K) * 16;
+  return make_tmap_2d(m, codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, pitch, (uint64_t)rows, pitch, 128, box);
+}
+
+inline int check_w4(const char* what, const void* codes, const void* scales, const void* mins, int K, int group) {
+  if (K < 1 || (group != 32 && group != 64 && group != 128))
+    return set_error(EK_ERR_INVALID, "%s: need K >= 1 and a group of 32, 64 or 128 (K=%d group=%d)", what, K, group);
+  if (!codes || !scales) return set_error(EK_ERR_INVALID, "%s: null pointer", what);
+  if (!aligned16(codes)) return set_error(EK_ERR_INVALID, "%s: codes must be 16-byte aligned", what);
+  if ((reinterpret_cast<uintptr_t>(scales) | reinterpret_cast<uintptr_t>(mins)) & 1u)
+    return set_error(EK_ERR_INVALID, "%s: misaligned scales", what);
+  return EK_OK;
+}
+
+}  // namespace w4
+}  // namespace ek

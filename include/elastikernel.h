@@ -505,23 +505,44 @@ int ek_dequant_w4(const void* codes, const void* scales, const void* mins, long 
 
 /* C[M, N] = A[M, K] @ W[N, K]^T with 4-bit W; A, C, scales and mins in dtype,
  * fp32 sums rounded once. Any M, N and K; made for M of a few tokens, where the
- * codes are streamed once. */
+ * codes are streamed once (per 32 tokens). A's elements enter as fp16 scaled
+ * per run of 256 by a power of two: exact up to 2^-40 of the run's largest.
+ * workspace: ek_gemm_w4_workspace_bytes(M, N, K, SMs of the launch) bytes of
+ * 16-byte aligned device memory, no initial contents; nothing in it is kept
+ * between calls. */
+size_t ek_gemm_w4_workspace_bytes(int M, int N, int K, int num_sms);
 int ek_gemm_w4(const void* A, const void* codes, const void* scales, const void* mins, void* C, int M, int N, int K,
-               int group, int dtype, int num_sms, void* stream);
+               int group, int dtype, int num_sms, void* workspace, size_t ws_bytes, void* stream);
 
 /* The experts' products over the packed layout with 4-bit weights w1, w3
- * [E, I, H] and w2 [E, H, I] (bf16 rows, scales and minima; E <= 1024):
+ * [E, I, H] and w2 [E, H, I] (bf16 scales and minima; E <= 1024):
  *   act[r] = silu(x . w1[e]) * (x . w3[e]),  y[r] = act[r] . w2[e]
  * for the rows r of every expert e (the rows past the last are not written).
- * x holds the packed rows, or, with sorted_slots (n_slots = T * topk), the
- * tokens: row r then reads x[sorted_slots[r] / topk]. */
-int ek_moe_gate_up_w4(const void* x, const int* sorted_slots, int topk, int n_slots, const void* w1_codes,
+ * x is bf16: the packed rows (x_rows = rows), or, with sorted_slots, the tokens
+ * (x_rows = T, rows = T * topk): row r then reads x[sorted_slots[r] / topk].
+ * act and y are bf16 or fp32 (act_dtype, y_dtype). An fp32 act enters the down
+ * product rounded to 11 significant bits, a bf16 one as it is. workspace:
+ * ek_moe_w4_workspace_bytes(x_rows, rows, E, H, I, SMs of the launch) bytes (the
+ * down product: x_rows 0), as ek_gemm_w4's. */
+size_t ek_moe_w4_workspace_bytes(int x_rows, int rows, int E, int H, int I, int num_sms);
+int ek_moe_gate_up_w4(const void* x, int x_rows, const int* sorted_slots, int topk, const void* w1_codes,
                       const void* w1_scales, const void* w1_mins, const void* w3_codes, const void* w3_scales,
-                      const void* w3_mins, const int* expert_counts, void* act, int rows, int E, int H, int I,
-                      int group, int num_sms, void* stream);
-int ek_moe_down_w4(const void* act, const void* w2_codes, const void* w2_scales, const void* w2_mins,
-                   const int* expert_counts, void* y, int rows, int E, int H, int I, int group, int num_sms,
-                   void* stream);
+                      const void* w3_mins, const int* expert_counts, void* act, int act_dtype, int rows, int E, int H,
+                      int I, int group, int num_sms, void* workspace, size_t ws_bytes, void* stream);
+int ek_moe_down_w4(const void* act, int act_dtype, const void* w2_codes, const void* w2_scales, const void* w2_mins,
+                   const int* expert_counts, void* y, int y_dtype, int rows, int E, int H, int I, int group,
+                   int num_sms, void* workspace, size_t ws_bytes, void* stream);
+
+/* Both products and the weighted combine: out[t] = sum_j topk_weights[t, j] *
+ * y[row of slot (t, j)], bf16 [T, H], from the maps of ek_moe_dispatch. The
+ * activations and the experts' rows stay in the workspace
+ * (ek_moe_w4_workspace_bytes(T, T * topk, ...)): act with 11 significant bits,
+ * the rows in fp32; the output is rounded once. */
+int ek_moe_experts_w4(const void* x, int T, int topk, const int* topk_ids, const float* topk_weights,
+                      const int* sorted_slots, const int* slot_rows, const int* expert_counts, const void* w1_codes,
+                      const void* w1_scales, const void* w1_mins, const void* w3_codes, const void* w3_scales,
+                      const void* w3_mins, const void* w2_codes, const void* w2_scales, const void* w2_mins, void* out,
+                      int E, int H, int I, int group, int num_sms, void* workspace, size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }

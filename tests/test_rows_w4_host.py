@@ -135,33 +135,77 @@ def test_w4_refusals():
     _bad(L.ek_quant_w4(_p(), 0, 8, 0, 32, 1, 0, _p(), _p(), n, n), "K >= 1")
     _bad(L.ek_dequant_w4(_p(264), _p(), n, 8, 64, 32, 0, _p(), n), "16-byte aligned")
     _bad(L.ek_dequant_w4(_p(), _p(), n, 8, 64, 32, 0, n, n), "null pointer")
-    _bad(L.ek_gemm_w4(_p(), _p(), _p(), n, _p(), 1, 8, 64, 16, 0, 0, n), "group")
-    _bad(L.ek_gemm_w4(_p(), _p(), _p(), n, _p(), -1, 8, 64, 32, 0, 0, n), "bad sizes")
-    _bad(L.ek_gemm_w4(_p(), _p(), _p(), n, _p(), 1, 8, 64, 32, 3, 0, n), "type")
-    _bad(L.ek_gemm_w4(n, _p(), _p(), n, _p(), 1, 8, 64, 32, 0, 0, n), "null pointer")
-    _bad(L.ek_gemm_w4(_p(), _p(264), _p(), n, _p(), 1, 8, 64, 32, 0, 0, n), "16-byte aligned")
-    _bad(L.ek_gemm_w4(_p(), _p(), _p(257), n, _p(), 1, 8, 64, 32, 0, 0, n), "misaligned")
-    assert L.ek_gemm_w4(n, n, n, n, n, 0, 8, 64, 32, 0, 0, n) == _lib.EK_OK
+    def gemm(A=_p(), codes=_p(), scales=_p(), C=_p(), M=1, N=8, K=64, group=32, dtype=0, ws=_p(), size=1 << 40):
+        return L.ek_gemm_w4(A, codes, scales, n, C, M, N, K, group, dtype, 148, ws, size, n)
+
+    _bad(gemm(group=16), "group")
+    _bad(gemm(M=-1), "bad sizes")
+    _bad(gemm(dtype=3), "type")
+    _bad(gemm(A=n), "null pointer")
+    _bad(gemm(ws=n), "null pointer")
+    _bad(gemm(codes=_p(264)), "16-byte aligned")
+    _bad(gemm(scales=_p(257)), "misaligned")
+    _bad(gemm(C=_p(257)), "aligned")
+    _bad(gemm(size=L.ek_gemm_w4_workspace_bytes(1, 8, 64, 148) - 1), "workspace")
+    _bad(gemm(ws=_p(264)), "workspace")
+    assert gemm(M=0, A=n) == _lib.EK_OK
+    assert L.ek_gemm_w4_workspace_bytes(0, 8, 64, 148) == 0
+    assert L.ek_gemm_w4_workspace_bytes(1, 8, 0, 148) == L.ek_gemm_w4_workspace_bytes(1, 8, 64, 0) == _ops._SIZE_MAX
 
 
 def test_moe_w4_refusals():
     L = lib()
     n = None
+    big = 1 << 40
 
-    def gate_up(x=_p(), slots=n, topk=2, c1=_p(), m1=n, c3=_p(), m3=n, counts=_p(), act=_p(), rows=8, E=4, H=64,
-                I=32, group=32):
-        return L.ek_moe_gate_up_w4(x, slots, topk, rows, c1, _p(), m1, c3, _p(), m3, counts, act, rows, E, H, I, group,
-                                   0, n)
+    def gate_up(x=_p(), x_rows=8, slots=n, topk=1, c1=_p(), m1=n, c3=_p(), counts=_p(), act=_p(), dt=0, rows=8, E=4,
+                H=64, I=32, group=32, ws=_p(), size=big):
+        return L.ek_moe_gate_up_w4(x, x_rows, slots, topk, c1, _p(), m1, c3, _p(), n, counts, act, dt, rows, E, H, I,
+                                   group, 148, ws, size, n)
 
     _bad(gate_up(E=0), "bad sizes")
-    _bad(gate_up(slots=_p(), topk=0), "bad sizes")
+    _bad(gate_up(E=1025), "bad sizes")
+    _bad(gate_up(x_rows=4), "do not match")
+    _bad(gate_up(slots=_p(), topk=0), "do not match")
+    _bad(gate_up(slots=_p(), topk=2), "do not match")
+    _bad(gate_up(dt=1), "bf16 or fp32")
     _bad(gate_up(group=100), "group")
     _bad(gate_up(m1=_p()), "null pointer")
     _bad(gate_up(counts=n), "null pointer")
+    _bad(gate_up(ws=n), "null pointer")
     _bad(gate_up(c3=_p(264)), "16-byte aligned")
-    _bad(L.ek_moe_down_w4(_p(), _p(), _p(), n, _p(), n, 8, 4, 64, 32, 32, 0, n), "null pointer")
-    _bad(L.ek_moe_down_w4(_p(), _p(), _p(), n, _p(), _p(), 8, 4, 0, 32, 32, 0, n), "bad sizes")
-    assert gate_up(rows=0) == _lib.EK_OK
+    _bad(gate_up(act=_p(258), dt=3), "aligned")
+    _bad(gate_up(size=16), "workspace")
+    assert gate_up(rows=0, x_rows=0) == _lib.EK_OK
+
+    def down(act=_p(), adt=0, codes=_p(), counts=_p(), y=_p(), ydt=3, rows=8, E=4, H=64, size=big):
+        return L.ek_moe_down_w4(act, adt, codes, _p(), n, counts, y, ydt, rows, E, H, 32, 32, 148, _p(), size, n)
+
+    _bad(down(counts=n), "null pointer")
+    _bad(down(H=0), "bad sizes")
+    _bad(down(adt=2), "bf16 or fp32")
+    _bad(down(ydt=1), "bf16 or fp32")
+    _bad(down(y=_p(258)), "aligned")
+    _bad(down(size=0), "workspace")
+    assert down(rows=0) == _lib.EK_OK
+
+    def experts(x=_p(), T=4, topk=2, ids=_p(), slots=_p(), rows=_p(), counts=_p(), c2=_p(), m3=n, out=_p(), E=4,
+                group=32, size=big):
+        return L.ek_moe_experts_w4(x, T, topk, ids, _p(), slots, rows, counts, _p(), _p(), n, _p(), _p(), m3, c2, _p(),
+                                   n, out, E, 64, 32, group, 148, _p(), size, n)
+
+    _bad(experts(topk=0), "bad sizes")
+    _bad(experts(T=-1), "bad sizes")
+    _bad(experts(T=1 << 24), "too many rows")
+    _bad(experts(ids=n), "null pointer")
+    _bad(experts(rows=n), "null pointer")
+    _bad(experts(counts=n), "null pointer")
+    _bad(experts(m3=_p()), "null pointer")
+    _bad(experts(c2=_p(8)), "16-byte aligned")
+    _bad(experts(out=_p(257)), "aligned")
+    _bad(experts(size=8), "workspace")
+    assert experts(T=0) == _lib.EK_OK
+    assert L.ek_moe_w4_workspace_bytes(4, 8, 4, 64, 32, 0) == _ops._SIZE_MAX
 
 
 def test_front_end_refuses_cpu_tensors():

@@ -237,7 +237,10 @@ def test_expert_products(case, drop, cuda_dev):
     kept = int(p["num_rows_padded"])
     act = _ops.moe_gate_up_w4(p, qw)
     assert torch.equal(act[:kept], _ops.moe_gate_up_w4(p, qw, x=x)[:kept])  # fetched through the permutation
+    wide = _ops.moe_gate_up_w4(p, qw, dtype=torch.float32)
+    assert torch.equal(wide[:kept].to(BF), act[:kept])
     y = _ops.moe_down_w4(p, act, qw)
+    assert torch.equal(_ops.moe_down_w4(p, act, qw, dtype=torch.float32)[:kept].to(BF), y[:kept])
     counts = p["expert_counts"].tolist()
     v = {n: _values(qw[n]) for n in ("w1", "w3", "w2")}
     b = {n: _bound(qw[n]) for n in ("w1", "w3", "w2")}
@@ -260,8 +263,8 @@ def test_expert_products(case, drop, cuda_dev):
 
 @pytest.mark.parametrize("case", MOE, ids=lambda c: f"T{c[0]}k{c[1]}E{c[2]}H{c[3]}I{c[4]}")
 def test_fused_layer(case, cuda_dev):
-    """The layer against the oracle: act and the experts' rows are bf16, so an
-    output carries their roundings (2^-8 of each term) beside its own."""
+    """The layer against the oracle: act has 11 significant bits (2^-11 of each
+    term), the experts' rows are fp32, the output is rounded once (2^-8)."""
     T, k, E, H, I, group, mins = case
     if E > 256:
         pytest.skip("moe_route takes up to 256 experts")
@@ -280,13 +283,14 @@ def test_fused_layer(case, cuda_dev):
             y = v["w2"][e] @ a
             exact[t] += w[t, j] * y
             spread[t] += w[t, j] * (np.abs(y) + np.abs(v["w2"][e]) @ np.abs(a))
-    # the fp32 sums inside are 2^-24-sized; 1 % on top of the two bf16 roundings covers them
-    bound = 2.0 ** -8 * (np.abs(exact) + 1.01 * spread) + 1e-30
+    # the fp32 sums inside are 2^-24-sized; 1 % on top of the roundings covers them
+    bound = 2.0 ** -8 * np.abs(exact) * 1.01 + 2.0 ** -11 * 1.01 * spread + 1e-30
     assert (np.abs(_np(got) - exact) <= bound).all()
+    # stage by stage with bf16 activations and rows: their roundings on top (2^-8 of each term, twice)
     p = _ops.moe_dispatch(None, torch.from_numpy(np.asarray(ids, np.int32)).to(cuda_dev), E)
     y = _ops.moe_down_w4(p, _ops.moe_gate_up_w4(p, qw, x=x), qw)
-    same = _ops.moe_combine_weighted(p, y, _ops.moe_route(logits, k)[1])
-    assert torch.equal(same, got)
+    staged = _ops.moe_combine_weighted(p, y, _ops.moe_route(logits, k)[1])
+    assert (np.abs(_np(staged) - exact) <= 2.0 ** -8 * (1.01 * np.abs(exact) + 1.01 * spread) + 1e-30).all()
     out = torch.empty_like(x)
     assert _ops.fused_moe_w4(x, logits, qw, k, out=out) is out and torch.equal(out, got)
 
