@@ -17,6 +17,7 @@
 
 #include "ek_gemm_kernel.cuh"
 #include "ek_internal.h"
+#include "ek_moe_order.cuh"
 
 namespace ek {
 
@@ -35,8 +36,6 @@ int read_status(int clear, int* v) {
 }
 const int s_status_reg = register_status_reader(read_status);
 
-constexpr int kRouteMaxE = 256;   // logits per token held in registers: 8 per lane
-constexpr int kRouteMaxK = 8;
 constexpr int kPermChunk = 1024;  // slots per permutation CTA
 constexpr int kPermMaxE = 1024;
 // up to this many slots the routing and the permutation run as one launch of
@@ -45,70 +44,6 @@ constexpr int kPermMaxE = 1024;
 constexpr int kFrontMaxSlots = 128;
 
 // ------------------------------------------------------------------ routing
-// One token's routing by one warp: logits row -> k expert ids and
-// renormalised weights (written by lane 0).
-__device__ __forceinline__ void route_token(const float* __restrict__ row, int E, int k, int lane,
-                                            int* __restrict__ ids_out, float* __restrict__ wts_out) {
-  float v[kRouteMaxE / 32];
-  float mx = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < kRouteMaxE / 32; ++i) {
-    const int e = lane + 32 * i;
-    v[i] = (e < E) ? row[e] : -INFINITY;
-    mx = fmaxf(mx, v[i]);
-  }
-#pragma unroll
-  for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-  float s = 0.f;
-#pragma unroll
-  for (int i = 0; i < kRouteMaxE / 32; ++i)
-    if (lane + 32 * i < E) s += expf(v[i] - mx);
-#pragma unroll
-  for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-
-  // Selection on the logits (softmax is monotone): largest first, ties to the
-  // lower expert id.
-  uint32_t taken = 0;
-  float p[kRouteMaxK];
-  int sel[kRouteMaxK];
-  float psum = 0.f;
-#pragma unroll
-  for (int j = 0; j < kRouteMaxK; ++j) {
-    if (j >= k) break;
-    float bv = -INFINITY;
-    int bi = 0x7fffffff;
-#pragma unroll
-    for (int i = 0; i < kRouteMaxE / 32; ++i) {
-      const int e = lane + 32 * i;
-      if (e < E && !(taken & (1u << i)) && (v[i] > bv || (v[i] == bv && e < bi))) {
-        bv = v[i];
-        bi = e;
-      }
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      const float ov = __shfl_xor_sync(0xffffffffu, bv, o);
-      const int oi = __shfl_xor_sync(0xffffffffu, bi, o);
-      if (ov > bv || (ov == bv && oi < bi)) {
-        bv = ov;
-        bi = oi;
-      }
-    }
-    if ((bi & 31) == lane) taken |= 1u << (bi >> 5);
-    sel[j] = bi;
-    p[j] = expf(bv - mx) / s;
-    psum += p[j];
-  }
-  if (lane == 0) {
-#pragma unroll
-    for (int j = 0; j < kRouteMaxK; ++j) {
-      if (j >= k) break;
-      ids_out[j] = sel[j];
-      wts_out[j] = p[j] / psum;
-    }
-  }
-}
-
 __global__ void __launch_bounds__(256) route_kernel(const float* __restrict__ logits, int T, int E, int k,
                                                     int* __restrict__ ids, float* __restrict__ wts) {
   const int t = (blockIdx.x * blockDim.x + threadIdx.x) >> 5;

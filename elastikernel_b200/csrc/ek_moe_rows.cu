@@ -17,9 +17,10 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "ek_internal.h"
-#include "ek_ptx.cuh"
+#include "ek_moe_order.cuh"
 
 namespace ek {
 
@@ -38,8 +39,8 @@ int read_status(int clear, int* v) {
 }
 const int s_status_reg = register_status_reader(read_status);
 
-constexpr int kChunk = 1024;  // slots per sorting CTA, one per thread
-constexpr int kMaxE = 1024;
+constexpr int kChunk = kOrderThreads;  // slots per sorting CTA, one per thread
+constexpr int kMaxE = kOrderMaxE;
 
 // ------------------------------------------------------------------ dispatch: the order
 __global__ void __launch_bounds__(kChunk) dispatch_count_kernel(const int* __restrict__ ids, int n_slots, int E,
@@ -68,19 +69,30 @@ __global__ void __launch_bounds__(kChunk)
                           int* __restrict__ expert_counts, int* __restrict__ num_rows) {
   extern __shared__ int s_wcnt[];  // [32][E] counts of each warp
   __shared__ int s_next[kMaxE];    // first row of the chunk's slots of each expert
+  __shared__ int s_tot[kMaxE], s_before[kMaxE];
   __shared__ int s_wsum[32];
   __shared__ int s_total;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int chunk = blockIdx.x;
-  int total = 0, before = 0;
-  if (tid < E) {
-    for (int c = 0; c < n_chunks; ++c) {
-      const int v = __ldg(chunk_counts + (size_t)c * E + tid);
-      total += v;
-      if (c < chunk) before += v;
-    }
-  }
+  if (tid < E) s_tot[tid] = s_before[tid] = 0;
   for (int i = tid; i < 32 * E; i += kChunk) s_wcnt[i] = 0;
+  __syncthreads();
+  // thread (group, e) adds every `groups`-th chunk's count of expert e
+  const int ep = E <= 32 ? 32 : 1 << (32 - __clz(E - 1)), groups = kChunk / ep;
+  const int e_of = tid & (ep - 1);
+  if (e_of < E) {
+    int sum = 0, pre = 0;
+#pragma unroll 8
+    for (int c = tid / ep; c < n_chunks; c += groups) {
+      const int v = __ldg(chunk_counts + (size_t)c * E + e_of);
+      sum += v;
+      if (c < chunk) pre += v;
+    }
+    atomicAdd(&s_tot[e_of], sum);
+    atomicAdd(&s_before[e_of], pre);
+  }
+  __syncthreads();
+  const int total = tid < E ? s_tot[tid] : 0, before = tid < E ? s_before[tid] : 0;
   int incl = total;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -170,114 +182,290 @@ struct Elems {
   }
 };
 
-// Zero the rows past the last kept one ([*num_rows, n_rows)).
+// Zero the rows past the last kept one ([kept, n_rows)).
 template <class Raw>
-__device__ __forceinline__ void zero_tail(Raw* __restrict__ rows, const int* __restrict__ num_rows, int n_rows,
-                                          int nvec) {
-  const long long first = (long long)max(0, min(*num_rows, n_rows)) * nvec, end = (long long)n_rows * nvec;
+__device__ __forceinline__ void zero_tail(Raw* __restrict__ rows, int kept, int n_rows, int nvec) {
+  const long long first = (long long)max(0, min(kept, n_rows)) * nvec, end = (long long)n_rows * nvec;
   for (long long i = first + (long long)blockIdx.x * blockDim.x + threadIdx.x; i < end;
        i += (long long)gridDim.x * blockDim.x)
     rows[i] = Raw{};
 }
 
-// rows[slot_rows[t*k + j]] = x[t] for the kept slots of each token. A thread
-// takes one vector of a token and stores it to the token's k rows.
+// The unit of the copies and sums: a warp, one token and a run of kRun vectors
+// per lane. The token's k rows are fetched once per unit (lane j holds slot j's)
+// and the run's loads are all in flight together.
+struct Unit {
+  int t, c0;  // token, first vector of this lane
+};
+template <int kRun>
+__device__ __forceinline__ Unit unit_of(long long u, int runs) {
+  const int t = (int)(u / runs);
+  return {t, (int)(u - (long long)t * runs) * (32 * kRun) + (int)(threadIdx.x & 31)};
+}
+template <int kRun>
+__host__ __device__ inline int runs_per_row(int nvec) { return (nvec + 32 * kRun - 1) / (32 * kRun); }
+
+constexpr int kCopyRun = 4;
+
+// Copy x[t] to the rows of token t; row_of(s): the row of slot s (negative:
+// dropped).
+template <class Raw, class RowOf>
+__device__ __forceinline__ void copy_rows(const Raw* __restrict__ x, int T, int k, int nvec, const RowOf& row_of,
+                                          Raw* __restrict__ rows) {
+  const int lane = threadIdx.x & 31, runs = runs_per_row<kCopyRun>(nvec);
+  const long long warps = ((long long)gridDim.x * blockDim.x) >> 5, units = (long long)T * runs;
+  for (long long u = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5; u < units; u += warps) {
+    const Unit w = unit_of<kCopyRun>(u, runs);
+    Raw v[kCopyRun];
+#pragma unroll
+    for (int i = 0; i < kCopyRun; ++i)
+      if (w.c0 + 32 * i < nvec) v[i] = __ldg(x + (long long)w.t * nvec + w.c0 + 32 * i);
+    for (int j0 = 0; j0 < k; j0 += 32) {
+      const int mine = j0 + lane < k ? row_of((long long)w.t * k + j0 + lane) : -1;
+      const int kn = min(32, k - j0);
+      for (int j = 0; j < kn; ++j) {
+        const int r = __shfl_sync(0xffffffffu, mine, j);
+        if (r < 0) continue;
+        Raw* dst = rows + (long long)r * nvec + w.c0;
+#pragma unroll
+        for (int i = 0; i < kCopyRun; ++i)
+          if (w.c0 + 32 * i < nvec) dst[32 * i] = v[i];
+      }
+    }
+  }
+}
+
+// rows[slot_rows[t*k + j]] = x[t] for the kept slots of each token.
 template <int V>
 __global__ void __launch_bounds__(256)
     dispatch_copy_kernel(const typename Vec<V>::type* __restrict__ x, const int* __restrict__ slot_rows,
                          const int* __restrict__ num_rows, int T, int k, int nvec,
                          typename Vec<V>::type* __restrict__ rows) {
-  using Raw = typename Vec<V>::type;
-  const long long items = (long long)T * nvec;
-  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < items;
-       i += (long long)gridDim.x * blockDim.x) {
-    const int t = (int)(i / nvec), c = (int)(i - (long long)t * nvec);
-    const Raw v = x[i];
-    for (int j = 0; j < k; ++j) {
-      const int r = __ldg(slot_rows + (long long)t * k + j);
-      if (r >= 0) rows[(long long)r * nvec + c] = v;
+  copy_rows(x, T, k, nvec, [&](long long s) { return __ldg(slot_rows + s); }, rows);
+  zero_tail(rows, *num_rows, T * k, nvec);
+}
+
+// Small batches (T * k <= kOrderThreads) in one launch: every CTA works out the
+// whole order (about 2 us, against two more launches) and copies its share of
+// the rows; the first one writes the maps.
+template <int V>
+__global__ void __launch_bounds__(kOrderThreads)
+    dispatch_small_kernel(const int* __restrict__ ids, int T, int k, int E, const typename Vec<V>::type* __restrict__ x,
+                          int nvec, int* __restrict__ sorted_slots, int* __restrict__ slot_rows,
+                          int* __restrict__ expert_counts, int* __restrict__ num_rows,
+                          typename Vec<V>::type* __restrict__ rows) {
+  extern __shared__ int sm[];
+  __shared__ int s_row[kOrderThreads];
+  const int tid = threadIdx.x, n = T * k;
+  int id = tid < n ? ids[tid] : -1;
+  if (id >= E) {
+    if (blockIdx.x == 0) atomicOr(&g_ek_status, kStatusBadIndex);
+    id = -1;
+  }
+  int kept;
+  const int row = order_slots(max(id, -1), n, E, sm, &kept);
+  s_row[tid] = row;
+  if (blockIdx.x == 0) {
+    const int* start = sm + (n + 31) / 32 * E;
+    if (tid < E) expert_counts[tid] = (tid + 1 < E ? start[tid + 1] : kept) - start[tid];
+    if (tid == 0) *num_rows = kept;
+    if (tid < n) {
+      slot_rows[tid] = row;
+      if (row >= 0) sorted_slots[row] = tid;
+      if (tid >= kept) sorted_slots[tid] = n;
     }
   }
-  zero_tail(rows, num_rows, T * k, nvec);
+  if (x == nullptr) return;
+  __syncthreads();
+  copy_rows(x, T, k, nvec, [&](long long s) { return s_row[s]; }, rows);
+  zero_tail(rows, kept, n, nvec);
 }
 
 // out[t] = sum_j w[t,j] rows[slot_rows[t,j]] (w = 1 without weights), fp32 sum
-// in j order, rounded once to T.
-template <class T, int V, bool kWeighted>
+// in j order, rounded once. kK: rows whose loads are in flight together.
+template <class T, int V, bool kWeighted, int kK>
 __global__ void __launch_bounds__(256)
     sum_rows_kernel(const typename Vec<V>::type* __restrict__ rows, const int* __restrict__ slot_rows,
                     const float* __restrict__ weights, int T_tokens, int k, int n_rows, int nvec,
                     typename Vec<V>::type* __restrict__ out) {
   using E = Elems<T, V>;
-  const long long items = (long long)T_tokens * nvec;
-  for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < items;
-       i += (long long)gridDim.x * blockDim.x) {
-    const int t = (int)(i / nvec), c = (int)(i - (long long)t * nvec);
-    float acc[E::N] = {};
-    for (int j = 0; j < k; ++j) {
-      const int r = __ldg(slot_rows + (long long)t * k + j);
-      if (r < 0 || r >= n_rows) continue;
-      const float w = kWeighted ? __ldg(weights + (long long)t * k + j) : 1.f;
-      float f[E::N];
-      E::unpack(rows[(long long)r * nvec + c], f);
+  constexpr int kRun = kK <= 2 ? 2 : 1;
+  const int lane = threadIdx.x & 31, runs = runs_per_row<kRun>(nvec);
+  const long long warps = ((long long)gridDim.x * blockDim.x) >> 5, units = (long long)T_tokens * runs;
+  for (long long u = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5; u < units; u += warps) {
+    const Unit w = unit_of<kRun>(u, runs);
+    float acc[kRun][E::N] = {};
+    for (int j0 = 0; j0 < k; j0 += kK) {
+      int mine = -1;
+      float wt = 1.f;
+      if (lane < kK && j0 + lane < k) {
+        mine = __ldg(slot_rows + (long long)w.t * k + j0 + lane);
+        if (kWeighted) wt = __ldg(weights + (long long)w.t * k + j0 + lane);
+      }
+      typename E::Raw v[kK][kRun];
 #pragma unroll
-      for (int e = 0; e < E::N; ++e) acc[e] += w * f[e];
+      for (int j = 0; j < kK; ++j) {
+        const int r = __shfl_sync(0xffffffffu, mine, j);
+#pragma unroll
+        for (int i = 0; i < kRun; ++i)
+          if (r >= 0 && r < n_rows && w.c0 + 32 * i < nvec) v[j][i] = __ldg(rows + (long long)r * nvec + w.c0 + 32 * i);
+      }
+#pragma unroll
+      for (int j = 0; j < kK; ++j) {
+        const int r = __shfl_sync(0xffffffffu, mine, j);
+        const float wj = kWeighted ? __shfl_sync(0xffffffffu, wt, j) : 1.f;
+        if (r < 0 || r >= n_rows) continue;
+#pragma unroll
+        for (int i = 0; i < kRun; ++i) {
+          float f[E::N];
+          E::unpack(v[j][i], f);
+#pragma unroll
+          for (int e = 0; e < E::N; ++e) acc[i][e] = kWeighted ? fmaf(wj, f[e], acc[i][e]) : acc[i][e] + f[e];
+        }
+      }
     }
-    out[i] = E::pack(acc);
+#pragma unroll
+    for (int i = 0; i < kRun; ++i)
+      if (w.c0 + 32 * i < nvec)
+        out[(long long)w.t * nvec + w.c0 + 32 * i] = E::pack(acc[i]);
   }
 }
 
-// d_rows[r] = w[s] d_out[t] and d_weights[s] = <d_out[t], rows[r]> (fp32), one
-// CTA per token.
-template <class T, int V>
-__global__ void __launch_bounds__(256)
+// d_rows[r] = w[s] d_out[t] and d_weights[s] = <d_out[t], rows[r]> (fp32). kTpt
+// threads per token; d_out[t] is read once (per kK slots), the kK rows' loads
+// are in flight together, and the kK dot products stay in registers until the
+// row's end.
+template <class T, int V, int kK, int kTpt>
+__global__ void __launch_bounds__(128)
     combine_grad_kernel(const typename Vec<V>::type* __restrict__ rows, const int* __restrict__ slot_rows,
                         const float* __restrict__ weights, const typename Vec<V>::type* __restrict__ d_out,
                         const int* __restrict__ num_rows, int T_tokens, int k, int n_rows, int nvec,
                         typename Vec<V>::type* __restrict__ d_rows, float* __restrict__ d_weights) {
   using E = Elems<T, V>;
-  __shared__ float s_red[8];
-  for (int t = blockIdx.x; t < T_tokens; t += gridDim.x) {
-    for (int j = 0; j < k; ++j) {
-      const long long s = (long long)t * k + j;
-      const int r = __ldg(slot_rows + s);
-      const bool live = r >= 0 && r < n_rows;
-      float dot = 0.f;
-      if (live) {
-        const float w = __ldg(weights + s);
-        for (int c = threadIdx.x; c < nvec; c += blockDim.x) {
-          float d[E::N], y[E::N];
-          E::unpack(d_out[(long long)t * nvec + c], d);
-          E::unpack(rows[(long long)r * nvec + c], y);
+  constexpr int kWarpsPer = kTpt / 32, kPer = 128 / kTpt;  // warps per token, tokens per CTA
+  __shared__ float s_red[4][kK];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, at = threadIdx.x % kTpt;
+  // every warp of a CTA takes the same number of turns (the barriers below)
+  for (long long t0 = (long long)blockIdx.x * kPer; t0 < T_tokens; t0 += (long long)gridDim.x * kPer) {
+    const long long t = t0 + warp / kWarpsPer;
+    for (int j0 = 0; j0 < k; j0 += kK) {
+      int mine = -1;
+      float wt = 0.f;
+      if (t < T_tokens && lane < kK && j0 + lane < k) {
+        mine = __ldg(slot_rows + t * k + j0 + lane);
+        wt = __ldg(weights + t * k + j0 + lane);
+        if (mine >= n_rows) mine = -1;
+      }
+      int r[kK];
+      float w[kK], dot[kK];
 #pragma unroll
-          for (int e = 0; e < E::N; ++e) {
-            dot += d[e] * y[e];
-            d[e] *= w;
-          }
-          d_rows[(long long)r * nvec + c] = E::pack(d);
+      for (int j = 0; j < kK; ++j) {
+        r[j] = __shfl_sync(0xffffffffu, mine, j);
+        w[j] = __shfl_sync(0xffffffffu, wt, j);
+        dot[j] = 0.f;
+      }
+      if (t < T_tokens) {
+        for (int c = at; c < nvec; c += kTpt) {
+          typename E::Raw y[kK];
+#pragma unroll
+          for (int j = 0; j < kK; ++j)
+            if (r[j] >= 0) y[j] = __ldg(rows + (long long)r[j] * nvec + c);
+          float d[E::N];
+          E::unpack(__ldg(d_out + t * nvec + c), d);
+#pragma unroll
+          for (int j = 0; j < kK; ++j)
+            if (r[j] >= 0) {
+              float f[E::N];
+              E::unpack(y[j], f);
+#pragma unroll
+              for (int e = 0; e < E::N; ++e) {
+                dot[j] = fmaf(d[e], f[e], dot[j]);
+                f[e] = w[j] * d[e];
+              }
+              d_rows[(long long)r[j] * nvec + c] = E::pack(f);
+            }
         }
       }
 #pragma unroll
-      for (int o = 16; o; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-      if ((threadIdx.x & 31) == 0) s_red[threadIdx.x >> 5] = dot;
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        float sum = 0.f;
-        for (int w = 0; w < 8; ++w) sum += s_red[w];
-        d_weights[s] = live ? sum : 0.f;
+      for (int j = 0; j < kK; ++j) {
+#pragma unroll
+        for (int o = 16; o; o >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], o);
       }
-      __syncthreads();
+      if constexpr (kWarpsPer > 1) {
+        if (lane == 0) {
+#pragma unroll
+          for (int j = 0; j < kK; ++j) s_red[warp][j] = dot[j];
+        }
+        __syncthreads();
+        if (threadIdx.x < kK) {
+          float sum = 0.f;
+#pragma unroll
+          for (int i = 0; i < kWarpsPer; ++i) sum += s_red[i][threadIdx.x];
+          if (j0 + threadIdx.x < k && t < T_tokens) d_weights[t * k + j0 + threadIdx.x] = mine >= 0 ? sum : 0.f;
+        }
+        __syncthreads();
+      } else {
+#pragma unroll
+        for (int j = 0; j < kK; ++j)
+          if (lane == j && j0 + j < k && t < T_tokens) d_weights[t * k + j0 + j] = mine >= 0 ? dot[j] : 0.f;
+      }
     }
   }
-  zero_tail(d_rows, num_rows, n_rows, nvec);
+  zero_tail(d_rows, *num_rows, n_rows, nvec);
 }
 
 // ------------------------------------------------------------------ route gradient
 // The renormalised weights are the softmax of the chosen logits alone, so
 // d_logit[ids_j] += w_j (dw_j - sum_i w_i dw_i) and every other logit gets 0.
+// kp lanes (a power of two >= k, up to 32) per token, 32 / kp tokens per warp:
+// the warp clears its tokens' rows with wide stores, then each lane puts its
+// slot's value where it belongs (the lowest lane, where an id repeats).
 __global__ void __launch_bounds__(256)
     route_grad_kernel(const int* __restrict__ ids, const float* __restrict__ weights,
-                      const float* __restrict__ d_weights, int T, int E, int k, float* __restrict__ d_logits) {
+                      const float* __restrict__ d_weights, int T, int E, int k, int kp, bool wide,
+                      float* __restrict__ d_logits) {
+  const int lane = threadIdx.x & 31, j = lane & (kp - 1), per = 32 / kp;
+  const long long warps = ((long long)gridDim.x * blockDim.x) >> 5, groups = ((long long)T + per - 1) / per;
+  for (long long u = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5; u < groups; u += warps) {
+    const long long t = u * per + lane / kp;
+    const bool live = j < k && t < T;
+    int id = -1;
+    float w = 0.f, d = 0.f;
+    if (live) {
+      id = __ldg(ids + t * k + j);
+      w = __ldg(weights + t * k + j);
+      d = __ldg(d_weights + t * k + j);
+    }
+    const long long first = u * per * E, n = min((long long)per, T - u * per) * E;
+    if (wide) {
+      float4* dst = reinterpret_cast<float4*>(d_logits + first);
+      for (int i = lane; i < n / 4; i += 32) dst[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    } else {
+      for (int i = lane; i < n; i += 32) d_logits[first + i] = 0.f;
+    }
+    float mean = w * d;
+    for (int o = kp >> 1; o; o >>= 1) mean += __shfl_xor_sync(0xffffffffu, mean, o);
+    float g = w * (d - mean);
+    // lanes with this token's same expert: their values go to the lowest one
+    const unsigned same = __match_any_sync(0xffffffffu, id >= 0 ? (long long)(lane / kp) << 32 | id : (long long)-1 - lane);
+    if (__any_sync(0xffffffffu, __popc(same) > 1)) {
+      float sum = 0.f;
+      for (int i = 0; i < 32; ++i) {
+        const float v = __shfl_sync(0xffffffffu, g, i);
+        if (same >> i & 1u) sum += v;
+      }
+      g = sum;
+    }
+    __syncwarp();  // the zeros above come first
+    if (live && id >= 0 && id < E && __ffs(same) - 1 == lane) d_logits[t * E + id] = g;
+    __syncwarp();
+  }
+}
+
+// More than 32 choices: a warp per token, every logit looks through them.
+__global__ void __launch_bounds__(256)
+    route_grad_any_kernel(const int* __restrict__ ids, const float* __restrict__ weights,
+                          const float* __restrict__ d_weights, int T, int E, int k, float* __restrict__ d_logits) {
   const int lane = threadIdx.x & 31;
   const int warps = (gridDim.x * blockDim.x) >> 5;
   for (int t = (blockIdx.x * blockDim.x + threadIdx.x) >> 5; t < T; t += warps) {
@@ -322,52 +510,121 @@ bool misaligned(int dtype, std::initializer_list<const void*> ptrs) {
   return false;
 }
 
+struct Rows {  // what the sums take
+  const void* rows;
+  const int* slot_rows;
+  const float* w;
+  int T, k, n_rows, H;
+  cudaStream_t s;
+};
+
 template <class T, int V, bool kWeighted>
-int launch_sum(const void* rows, const int* slot_rows, const float* w, int Tt, int k, int n_rows, int H, void* out,
-               cudaStream_t s) {
-  using Raw = typename Vec<V>::type;
-  const int nvec = H * (int)sizeof(T) / V;
-  sum_rows_kernel<T, V, kWeighted><<<rows_grid((long long)Tt * nvec), 256, 0, s>>>(
-      static_cast<const Raw*>(rows), slot_rows, w, Tt, k, n_rows, nvec, static_cast<Raw*>(out));
+int launch_sum(const Rows& a, void* dst) {
+  const int nvec = a.H * (int)sizeof(T) / V;
+  const auto* rows = static_cast<const typename Vec<V>::type*>(a.rows);
+  auto* out = static_cast<typename Vec<V>::type*>(dst);
+  if (a.k <= 2)
+    sum_rows_kernel<T, V, kWeighted, 2><<<rows_grid((long long)a.T * runs_per_row<2>(nvec) * 32), 256, 0, a.s>>>(
+        rows, a.slot_rows, a.w, a.T, a.k, a.n_rows, nvec, out);
+  else if (a.k <= 4)
+    sum_rows_kernel<T, V, kWeighted, 4><<<rows_grid((long long)a.T * runs_per_row<1>(nvec) * 32), 256, 0, a.s>>>(
+        rows, a.slot_rows, a.w, a.T, a.k, a.n_rows, nvec, out);
+  else
+    sum_rows_kernel<T, V, kWeighted, 8><<<rows_grid((long long)a.T * runs_per_row<1>(nvec) * 32), 256, 0, a.s>>>(
+        rows, a.slot_rows, a.w, a.T, a.k, a.n_rows, nvec, out);
   return check_cuda(cudaGetLastError(), "sum rows launch");
 }
 
 template <class T, bool kWeighted>
-int sum_vec(int v, const void* rows, const int* slot_rows, const float* w, int Tt, int k, int n_rows, int H, void* out,
-            cudaStream_t s) {
-  if (v == 16) return launch_sum<T, 16, kWeighted>(rows, slot_rows, w, Tt, k, n_rows, H, out, s);
-  if (v == 8) return launch_sum<T, 8, kWeighted>(rows, slot_rows, w, Tt, k, n_rows, H, out, s);
-  if (v == 4) return launch_sum<T, 4, kWeighted>(rows, slot_rows, w, Tt, k, n_rows, H, out, s);
-  return launch_sum<T, (int)sizeof(T), kWeighted>(rows, slot_rows, w, Tt, k, n_rows, H, out, s);
+int sum_rows(const Rows& a, void* out) {
+  switch (vec_bytes((size_t)a.H * sizeof(T), {a.rows, out})) {
+    case 16: return launch_sum<T, 16, kWeighted>(a, out);
+    case 8: return launch_sum<T, 8, kWeighted>(a, out);
+    case 4: return launch_sum<T, 4, kWeighted>(a, out);
+    default: return launch_sum<T, (int)sizeof(T), kWeighted>(a, out);
+  }
 }
 
 template <bool kWeighted>
-int sum_rows(const void* rows, const int* slot_rows, const float* w, int Tt, int k, int n_rows, int H, int dtype,
-             void* out, cudaStream_t s) {
-  const int v = vec_bytes((size_t)H * elem_bytes(dtype), {rows, out});
-  if (dtype == EK_DTYPE_BF16) return sum_vec<__nv_bfloat16, kWeighted>(v, rows, slot_rows, w, Tt, k, n_rows, H, out, s);
-  if (dtype == EK_DTYPE_FP16) return sum_vec<__half, kWeighted>(v, rows, slot_rows, w, Tt, k, n_rows, H, out, s);
-  return sum_vec<float, kWeighted>(v, rows, slot_rows, w, Tt, k, n_rows, H, out, s);
+int sum_rows(const Rows& a, int dtype, void* out) {
+  if (dtype == EK_DTYPE_BF16) return sum_rows<__nv_bfloat16, kWeighted>(a, out);
+  if (dtype == EK_DTYPE_FP16) return sum_rows<__half, kWeighted>(a, out);
+  return sum_rows<float, kWeighted>(a, out);
 }
 
-template <class T, int V>
-int launch_combine_grad(const void* rows, const int* slot_rows, const float* w, const void* d_out, const int* num_rows,
-                        int Tt, int k, int n_rows, int H, void* d_rows, float* d_w, cudaStream_t s) {
+template <class T, int V, int kK>
+int launch_combine_grad(const Rows& a, const void* d_out, const int* num_rows, void* d_rows, float* d_w) {
   using Raw = typename Vec<V>::type;
-  const int nvec = H * (int)sizeof(T) / V;
-  combine_grad_kernel<T, V><<<std::max(1, std::min(Tt, 148 * 64)), 256, 0, s>>>(
-      static_cast<const Raw*>(rows), slot_rows, w, static_cast<const Raw*>(d_out), num_rows, Tt, k, n_rows, nvec,
-      static_cast<Raw*>(d_rows), d_w);
+  const int nvec = a.H * (int)sizeof(T) / V;
+  const auto* rows = static_cast<const Raw*>(a.rows);
+  const auto* d = static_cast<const Raw*>(d_out);
+  auto* o = static_cast<Raw*>(d_rows);
+  // short rows: a warp per token; else a CTA of four
+  if (nvec <= 64)
+    combine_grad_kernel<T, V, kK, 32><<<std::max(1, std::min((a.T + 3) / 4, 148 * 64)), 128, 0, a.s>>>(
+        rows, a.slot_rows, a.w, d, num_rows, a.T, a.k, a.n_rows, nvec, o, d_w);
+  else
+    combine_grad_kernel<T, V, kK, 128><<<std::max(1, std::min(a.T, 148 * 64)), 128, 0, a.s>>>(
+        rows, a.slot_rows, a.w, d, num_rows, a.T, a.k, a.n_rows, nvec, o, d_w);
   return check_cuda(cudaGetLastError(), "combine gradient launch");
 }
 
+template <class T, int V>
+int combine_grad_k(const Rows& a, const void* d_out, const int* num_rows, void* d_rows, float* d_w) {
+  if (a.k <= 2) return launch_combine_grad<T, V, 2>(a, d_out, num_rows, d_rows, d_w);
+  if (a.k <= 4) return launch_combine_grad<T, V, 4>(a, d_out, num_rows, d_rows, d_w);
+  return launch_combine_grad<T, V, 8>(a, d_out, num_rows, d_rows, d_w);
+}
+
 template <class T>
-int combine_grad_vec(int v, const void* rows, const int* slot_rows, const float* w, const void* d_out,
-                     const int* num_rows, int Tt, int k, int n_rows, int H, void* d_rows, float* d_w, cudaStream_t s) {
-  if (v == 16) return launch_combine_grad<T, 16>(rows, slot_rows, w, d_out, num_rows, Tt, k, n_rows, H, d_rows, d_w, s);
-  if (v == 8) return launch_combine_grad<T, 8>(rows, slot_rows, w, d_out, num_rows, Tt, k, n_rows, H, d_rows, d_w, s);
-  if (v == 4) return launch_combine_grad<T, 4>(rows, slot_rows, w, d_out, num_rows, Tt, k, n_rows, H, d_rows, d_w, s);
-  return launch_combine_grad<T, (int)sizeof(T)>(rows, slot_rows, w, d_out, num_rows, Tt, k, n_rows, H, d_rows, d_w, s);
+int combine_grad(const Rows& a, const void* d_out, const int* num_rows, void* d_rows, float* d_w) {
+  switch (vec_bytes((size_t)a.H * sizeof(T), {a.rows, d_out, d_rows})) {
+    case 16: return combine_grad_k<T, 16>(a, d_out, num_rows, d_rows, d_w);
+    case 8: return combine_grad_k<T, 8>(a, d_out, num_rows, d_rows, d_w);
+    case 4: return combine_grad_k<T, 4>(a, d_out, num_rows, d_rows, d_w);
+    default: return combine_grad_k<T, (int)sizeof(T)>(a, d_out, num_rows, d_rows, d_w);
+  }
+}
+
+struct Dispatch {
+  const int* ids;
+  int T, k, E, H;
+  const void* x;
+  int *sorted_slots, *slot_rows, *counts, *num_rows;
+  void* rows;
+  cudaStream_t s;
+};
+
+template <int V>
+int launch_small(const Dispatch& d, size_t row_bytes) {
+  using Raw = typename Vec<V>::type;
+  const int n = d.T * d.k, nvec = (int)(row_bytes / V);
+  const size_t smem = order_smem_ints(n, d.E) * sizeof(int);
+  static bool attr_done[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64 && !attr_done[dev]) {
+    const int rc = check_cuda(cudaFuncSetAttribute(dispatch_small_kernel<V>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   order_smem_ints(kOrderThreads, kMaxE) * (int)sizeof(int)),
+                              "cudaFuncSetAttribute(dispatch)");
+    if (rc) return rc;
+    attr_done[dev] = true;
+  }
+  // one warp per unit of the copy, at most a CTA per SM
+  const int grid = d.x ? std::max(1, std::min(148, (d.T * runs_per_row<kCopyRun>(nvec) + 31) / 32)) : 1;
+  dispatch_small_kernel<V><<<grid, kOrderThreads, smem, d.s>>>(d.ids, d.T, d.k, d.E, static_cast<const Raw*>(d.x), nvec,
+                                                             d.sorted_slots, d.slot_rows, d.counts, d.num_rows,
+                                                             static_cast<Raw*>(d.rows));
+  return check_cuda(cudaGetLastError(), "dispatch launch");
+}
+
+template <int V>
+int launch_copy(const Dispatch& d, size_t row_bytes) {
+  using Raw = typename Vec<V>::type;
+  const int nvec = (int)(row_bytes / V);
+  dispatch_copy_kernel<V><<<rows_grid((long long)d.T * runs_per_row<kCopyRun>(nvec) * 32), 256, 0, d.s>>>(
+      static_cast<const Raw*>(d.x), d.slot_rows, d.num_rows, d.T, d.k, nvec, static_cast<Raw*>(d.rows));
+  return check_cuda(cudaGetLastError(), "dispatch copy launch");
 }
 
 }  // namespace
@@ -389,8 +646,17 @@ int ek_moe_dispatch(const int* topk_ids, int T, int topk, int E, const void* x, 
   if (x && misaligned(dtype, {x, x_rows}))
     return set_error(EK_ERR_INVALID, "dispatch: rows must be aligned to their elements");
   const int n_slots = T * topk;
-  const int n_chunks = std::max((n_slots + kChunk - 1) / kChunk, 1);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const Dispatch d{topk_ids, T, topk, E, H, x, sorted_slots, slot_rows, expert_counts, num_rows, x_rows, s};
+  const size_t row_bytes = x ? (size_t)H * elem_bytes(dtype) : 16;
+  const int v = x ? vec_bytes(row_bytes, {x, x_rows}) : 16;
+  if (n_slots <= kOrderThreads) {
+    if (v == 16) return launch_small<16>(d, row_bytes);
+    if (v == 8) return launch_small<8>(d, row_bytes);
+    if (v == 4) return launch_small<4>(d, row_bytes);
+    return launch_small<2>(d, row_bytes);
+  }
+  const int n_chunks = (n_slots + kChunk - 1) / kChunk;
   int* chunk_counts = static_cast<int*>(scratch);
   static bool attr_done[64] = {false};
   int dev = 0;
@@ -406,29 +672,11 @@ int ek_moe_dispatch(const int* topk_ids, int T, int topk, int E, const void* x, 
   dispatch_place_kernel<<<n_chunks, kChunk, 32 * E * sizeof(int), s>>>(topk_ids, n_slots, E, chunk_counts, n_chunks,
                                                                       sorted_slots, slot_rows, expert_counts, num_rows);
   rc = check_cuda(cudaGetLastError(), "dispatch order launch");
-  if (rc || !x || T == 0) return rc;
-  const size_t row_bytes = (size_t)H * elem_bytes(dtype);
-  const int v = vec_bytes(row_bytes, {x, x_rows});
-  const int nvec = (int)(row_bytes / v);
-  const int grid = rows_grid((long long)T * nvec);
-  switch (v) {
-    case 16:
-      dispatch_copy_kernel<16><<<grid, 256, 0, s>>>(static_cast<const uint4*>(x), slot_rows, num_rows, T, topk, nvec,
-                                                    static_cast<uint4*>(x_rows));
-      break;
-    case 8:
-      dispatch_copy_kernel<8><<<grid, 256, 0, s>>>(static_cast<const uint2*>(x), slot_rows, num_rows, T, topk, nvec,
-                                                   static_cast<uint2*>(x_rows));
-      break;
-    case 4:
-      dispatch_copy_kernel<4><<<grid, 256, 0, s>>>(static_cast<const uint32_t*>(x), slot_rows, num_rows, T, topk, nvec,
-                                                   static_cast<uint32_t*>(x_rows));
-      break;
-    default:
-      dispatch_copy_kernel<2><<<grid, 256, 0, s>>>(static_cast<const uint16_t*>(x), slot_rows, num_rows, T, topk, nvec,
-                                                   static_cast<uint16_t*>(x_rows));
-  }
-  return check_cuda(cudaGetLastError(), "dispatch copy launch");
+  if (rc || !x) return rc;
+  if (v == 16) return launch_copy<16>(d, row_bytes);
+  if (v == 8) return launch_copy<8>(d, row_bytes);
+  if (v == 4) return launch_copy<4>(d, row_bytes);
+  return launch_copy<2>(d, row_bytes);
 }
 
 int ek_moe_dispatch_grad(const void* d_rows, const int* slot_rows, int T, int topk, int n_rows, int H, int dtype,
@@ -439,7 +687,7 @@ int ek_moe_dispatch_grad(const void* d_rows, const int* slot_rows, int T, int to
   if (!slot_rows || !d_x || (n_rows > 0 && !d_rows)) return set_error(EK_ERR_INVALID, "dispatch gradient: null pointer");
   if (misaligned(dtype, {d_rows, d_x}))
     return set_error(EK_ERR_INVALID, "dispatch gradient: rows must be aligned to their elements");
-  return sum_rows<false>(d_rows, slot_rows, nullptr, T, topk, n_rows, H, dtype, d_x, static_cast<cudaStream_t>(stream));
+  return sum_rows<false>({d_rows, slot_rows, nullptr, T, topk, n_rows, H, static_cast<cudaStream_t>(stream)}, dtype, d_x);
 }
 
 int ek_moe_combine_weighted(const void* rows, const int* slot_rows, const float* weights, int T, int topk, int n_rows,
@@ -451,7 +699,7 @@ int ek_moe_combine_weighted(const void* rows, const int* slot_rows, const float*
     return set_error(EK_ERR_INVALID, "weighted combine: null pointer");
   if (misaligned(dtype, {rows, out}))
     return set_error(EK_ERR_INVALID, "weighted combine: rows must be aligned to their elements");
-  return sum_rows<true>(rows, slot_rows, weights, T, topk, n_rows, H, dtype, out, static_cast<cudaStream_t>(stream));
+  return sum_rows<true>({rows, slot_rows, weights, T, topk, n_rows, H, static_cast<cudaStream_t>(stream)}, dtype, out);
 }
 
 int ek_moe_combine_weighted_grad(const void* rows, const int* slot_rows, const float* weights, const void* d_out,
@@ -464,15 +712,10 @@ int ek_moe_combine_weighted_grad(const void* rows, const int* slot_rows, const f
     return set_error(EK_ERR_INVALID, "weighted combine gradient: null pointer");
   if (misaligned(dtype, {rows, d_out, d_rows}))
     return set_error(EK_ERR_INVALID, "weighted combine gradient: rows must be aligned to their elements");
-  const int v = vec_bytes((size_t)H * elem_bytes(dtype), {rows, d_out, d_rows});
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == EK_DTYPE_BF16)
-    return combine_grad_vec<__nv_bfloat16>(v, rows, slot_rows, weights, d_out, num_rows, T, topk, n_rows, H, d_rows,
-                                           d_weights, s);
-  if (dtype == EK_DTYPE_FP16)
-    return combine_grad_vec<__half>(v, rows, slot_rows, weights, d_out, num_rows, T, topk, n_rows, H, d_rows, d_weights,
-                                    s);
-  return combine_grad_vec<float>(v, rows, slot_rows, weights, d_out, num_rows, T, topk, n_rows, H, d_rows, d_weights, s);
+  const Rows a{rows, slot_rows, weights, T, topk, n_rows, H, static_cast<cudaStream_t>(stream)};
+  if (dtype == EK_DTYPE_BF16) return combine_grad<__nv_bfloat16>(a, d_out, num_rows, d_rows, d_weights);
+  if (dtype == EK_DTYPE_FP16) return combine_grad<__half>(a, d_out, num_rows, d_rows, d_weights);
+  return combine_grad<float>(a, d_out, num_rows, d_rows, d_weights);
 }
 
 int ek_moe_route_grad(const int* topk_ids, const float* topk_weights, const float* d_weights, int T, int E, int topk,
@@ -482,8 +725,16 @@ int ek_moe_route_grad(const int* topk_ids, const float* topk_weights, const floa
   if (T == 0) return EK_OK;
   if (!topk_ids || !topk_weights || !d_weights || !d_logits)
     return set_error(EK_ERR_INVALID, "route gradient: null pointer");
-  route_grad_kernel<<<rows_grid((long long)T * 32), 256, 0, static_cast<cudaStream_t>(stream)>>>(
-      topk_ids, topk_weights, d_weights, T, E, topk, d_logits);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (topk > 32) {
+    route_grad_any_kernel<<<rows_grid((long long)T * 32), 256, 0, s>>>(topk_ids, topk_weights, d_weights, T, E, topk,
+                                                                      d_logits);
+  } else {
+    int kp = 1;
+    while (kp < topk) kp *= 2;
+    route_grad_kernel<<<rows_grid((long long)T * kp), 256, 0, s>>>(topk_ids, topk_weights, d_weights, T, E, topk, kp,
+                                                                  E % 4 == 0 && aligned16(d_logits), d_logits);
+  }
   return check_cuda(cudaGetLastError(), "route gradient launch");
 }
 
