@@ -130,6 +130,8 @@ _SIGNATURES = {
     "ek_moe_gate_up_w4": (_c_int, [_c_vp, _c_int, _c_vp, _c_int] + [_c_vp] * 8 + [_c_int] * 7 + [_c_vp, _c_size, _c_vp]),
     "ek_moe_down_w4": (_c_int, [_c_vp, _c_int] + [_c_vp] * 5 + [_c_int] * 7 + [_c_vp, _c_size, _c_vp]),
     "ek_moe_experts_w4": (_c_int, [_c_vp, _c_int, _c_int] + [_c_vp] * 15 + [_c_int] * 5 + [_c_vp, _c_size, _c_vp]),
+    "ek_fused_moe_w4_workspace_bytes": (_c_size, [_c_int] * 6),
+    "ek_fused_moe_w4": (_c_int, [_c_vp, _c_vp, _c_int, _c_int] + [_c_vp] * 10 + [_c_int] * 5 + [_c_vp, _c_size, _c_vp]),
     "ek_moe_segment_gemm": (_c_int, [_c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
                                      _c_vp]),
 }

@@ -50,8 +50,16 @@ def plan(M: int, N: int, K: int, num_sms: int, dtype=torch.bfloat16, b_layout: s
     return p.as_dict()
 
 
+# torch's own accessors of the current device and raw stream: the public ones
+# build a Stream object per call (2-3 us, as much as a small launch)
+_RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_CURRENT_DEVICE = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def current_stream_handle(device: torch.device) -> int:
-    return _lib.stream_ptr(torch.cuda.current_stream(device))
+    if _RAW_STREAM is None or device.index is None:
+        return _lib.stream_ptr(torch.cuda.current_stream(device))
+    return _RAW_STREAM(device.index)
 
 
 def gemm(a: torch.Tensor, b: torch.Tensor, out: torch.Tensor | None = None, num_sms: int | None = None,
@@ -225,8 +233,7 @@ _NULL = _NullCtx()
 
 def _on_device(dev: torch.device):
     """Make `dev` current for a launch (a no-op when it already is)."""
-    idx = dev.index if dev.index is not None else torch.cuda.current_device()
-    return _NULL if torch.cuda.current_device() == idx else torch.cuda.device(dev)
+    return _NULL if dev.index is None or dev.index == _CURRENT_DEVICE() else torch.cuda.device(dev)
 
 
 def _stream_sms(dev: torch.device, stream: int) -> int:
@@ -666,7 +673,7 @@ def _check_rows(name: str, t: torch.Tensor, rows: int | None = None) -> int:
 
 
 def _check_slots(name: str, t: torch.Tensor, T: int, k: int, dtype: torch.dtype) -> None:
-    if t.dtype != dtype or tuple(t.shape) != (T, k):
+    if t.dtype != dtype or t.shape != (T, k):
         raise RuntimeError(f"{name} must be a {dtype} tensor of shape {(T, k)}")
     _contig(name, t)
 
@@ -740,7 +747,7 @@ def moe_combine_weighted(perm: dict, rows: torch.Tensor, topk_weights: torch.Ten
     _check_slots("topk_weights", topk_weights, T, k, torch.float32)
     if out is None:
         out = torch.empty((T, H), dtype=rows.dtype, device=dev)
-    elif out.dtype != rows.dtype or tuple(out.shape) != (T, H) or not out.is_contiguous():
+    elif out.dtype != rows.dtype or out.shape != (T, H) or not out.is_contiguous():
         raise RuntimeError("out must be a contiguous [T, H] tensor of the rows' dtype")
     with _on_device(dev):
         check(lib().ek_moe_combine_weighted(rows.data_ptr(), slot_rows.data_ptr(), topk_weights.data_ptr(), T, k, n, H,
@@ -758,7 +765,7 @@ def moe_combine_weighted_grad(perm: dict, rows: torch.Tensor, topk_weights: torc
     dt = _check_rows("rows", rows)
     T, k, (n, H) = perm["T"], perm["topk"], rows.shape
     _check_slots("topk_weights", topk_weights, T, k, torch.float32)
-    if d_out.dtype != rows.dtype or tuple(d_out.shape) != (T, H):
+    if d_out.dtype != rows.dtype or d_out.shape != (T, H):
         raise RuntimeError(f"d_out must be a {rows.dtype} tensor of shape {(T, H)}")
     _contig("d_out", d_out)
     d_rows = torch.empty_like(rows)
@@ -834,18 +841,18 @@ def _check_w4(name: str, qw: dict, dtype: torch.dtype | None = None) -> tuple:
     codes, scales, mins, K, group = qw["codes"], qw["scales"], qw.get("mins"), int(qw["K"]), int(qw["group"])
     if group not in W4_GROUPS or K < 1:
         raise RuntimeError(f"{name}: need K >= 1 and a group out of {W4_GROUPS}")
-    lead = tuple(codes.shape[:-1])
-    if codes.dtype != torch.uint8 or not lead or codes.shape[-1] != -(-K // 32) * 16:
+    *lead, width = codes.shape
+    if codes.dtype != torch.uint8 or not lead or width != -(-K // 32) * 16:
         raise RuntimeError(f"{name}: codes must be uint8 [..., N, {-(-K // 32) * 16}]")
-    if scales.dtype not in _DTYPES or tuple(scales.shape) != lead + (-(-K // group),):
+    if scales.dtype not in _DTYPES or scales.shape != (*lead, -(-K // group)):
         raise RuntimeError(f"{name}: scales must be bf16 or fp16 [..., N, {-(-K // group)}]")
     if dtype is not None and scales.dtype != dtype:
         raise RuntimeError(f"{name}: scales must be {dtype}, got {scales.dtype}")
-    if mins is not None and (mins.dtype != scales.dtype or mins.shape != scales.shape):
+    if mins is not None and (mins.dtype != scales.dtype or mins.shape != scales.shape or not mins.is_contiguous()):
         raise RuntimeError(f"{name}: mins must match the scales")
-    for t in (codes, scales, mins):
-        if t is not None:
-            _contig(name, t)
+    _contig(name, codes)
+    _contig(name, scales)
+    lead = tuple(lead)
     return codes, scales, mins, lead, K, group
 
 
@@ -875,7 +882,7 @@ def gemm_w4(a: torch.Tensor, qw: dict, out: torch.Tensor | None = None, num_sms:
     M, N = a.shape[0], lead[0]
     if out is None:
         out = torch.empty((M, N), device=dev, dtype=a.dtype)
-    elif tuple(out.shape) != (M, N) or out.dtype != a.dtype or not out.is_contiguous():
+    elif out.shape != (M, N) or out.dtype != a.dtype or not out.is_contiguous():
         raise RuntimeError("out must be a contiguous [M, N] tensor of the input dtype")
     if M == 0 or N == 0:
         return out
@@ -1021,17 +1028,34 @@ def moe_experts_w4(perm: dict, x: torch.Tensor, topk_ids: torch.Tensor, topk_wei
 def fused_moe_w4(hidden_states: torch.Tensor, gate_logits: torch.Tensor, qw: dict, topk: int,
                  out: torch.Tensor | None = None, num_sms: int | None = None) -> torch.Tensor:
     """MoE layer over 4-bit experts (quant_moe_weights_w4), for batches of a few
-    tokens per expert: route -> expert order -> moe_experts_w4."""
-    _require_cuda(hidden_states, gate_logits, out)
+    tokens per expert: moe_route -> moe_dispatch -> moe_experts_w4 in one call
+    (five launches up to 1024 slots)."""
+    E, H, I = qw["E"], qw["H"], qw["I"]
+    (c1, s1, m1, group), (c3, s3, m3, _), (c2, s2, m2, _) = _check_experts(qw, "w1", "w3", "w2")
+    dev = _require_cuda(hidden_states, gate_logits, c1, s1, m1, c3, s3, m3, c2, s2, m2, out)
     _check_bf16("hidden_states", hidden_states)
     T = hidden_states.shape[0]
-    if tuple(gate_logits.shape) != (T, qw["E"]):
-        raise RuntimeError("gate_logits must have one row per token and one column per expert")
-    if T == 0:
-        return out if out is not None else torch.empty_like(hidden_states)
-    ids, wts = moe_route(gate_logits, topk)
-    perm = moe_dispatch(None, ids, qw["E"])
-    return moe_experts_w4(perm, hidden_states, ids, wts, qw, out=out, num_sms=num_sms)
+    if hidden_states.shape != (T, H):
+        raise RuntimeError("fused_moe_w4: shape mismatch")
+    if gate_logits.dtype != torch.float32 or gate_logits.shape != (T, E):
+        raise RuntimeError("gate_logits must be float32 with one row per token and one column per expert")
+    _contig("gate_logits", gate_logits)
+    if out is None:
+        out = torch.empty_like(hidden_states)
+    else:
+        _check_bf16("out", out)
+        if out.shape != hidden_states.shape:
+            raise RuntimeError("out must be a [T, H] tensor")
+    L, k = lib(), int(topk)
+    stream = current_stream_handle(dev)
+    sms = int(num_sms) if num_sms else _stream_sms(dev, stream)
+    ws = _scratch(L.ek_fused_moe_w4_workspace_bytes(T, k, E, H, I, sms), dev)
+    with _on_device(dev):
+        check(L.ek_fused_moe_w4(hidden_states.data_ptr(), gate_logits.data_ptr(), T, k, c1.data_ptr(), s1.data_ptr(),
+                                _ptr(m1), c3.data_ptr(), s3.data_ptr(), _ptr(m3), c2.data_ptr(), s2.data_ptr(),
+                                _ptr(m2), out.data_ptr(), E, H, I, group, sms, ws.data_ptr(), ws.numel(), stream),
+              "ek_fused_moe_w4")
+    return out
 
 
 def moe_segment_gemm(hidden_states: torch.Tensor, weights: torch.Tensor, expert_offsets: torch.Tensor,

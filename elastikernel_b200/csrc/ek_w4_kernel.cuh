@@ -183,16 +183,13 @@ __device__ __forceinline__ void write_run(const Tokens& out, size_t row, int st,
   if (lane == 0) out.scale[row * nst + st] = inv;
 }
 
-// Rows of x [rows, K] into tokens, a warp per run. vec: rows of a multiple of
-// 8 elements on a 16-byte base.
+// Rows of x [rows, K] into tokens, a warp per run (runs first, first + step,
+// ...). vec: rows of a multiple of 8 elements on a 16-byte base.
 template <class T>
-__global__ void __launch_bounds__(256)
-    tokens_kernel(const T* __restrict__ x, int rows, int K, bool vec, Tokens out) {
-  griddep_launch();
-  griddep_wait();
+__device__ __forceinline__ void write_tokens(const T* __restrict__ x, int rows, int K, bool vec, const Tokens& out,
+                                             long long first, long long step) {
   const int lane = threadIdx.x & 31, nst = stages(K);
-  const long long warps = ((long long)gridDim.x * blockDim.x) >> 5;
-  for (long long u = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5; u < (long long)rows * nst; u += warps) {
+  for (long long u = first; u < (long long)rows * nst; u += step) {
     const int row = (int)(u / nst), st = (int)(u - (long long)row * nst);
     const T* src = x + (size_t)row * K;
     const int k = st * kStageElems + lane * 8;
@@ -209,6 +206,15 @@ __global__ void __launch_bounds__(256)
     }
     write_run<!std::is_same<T, __half>::value>(out, row, st, nst, v);
   }
+}
+
+template <class T>
+__global__ void __launch_bounds__(256)
+    tokens_kernel(const T* __restrict__ x, int rows, int K, bool vec, Tokens out) {
+  griddep_launch();
+  griddep_wait();
+  write_tokens(x, rows, K, vec, out, ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5,
+               ((long long)gridDim.x * blockDim.x) >> 5);
 }
 
 // ------------------------------------------------------------------ products
@@ -235,6 +241,7 @@ struct Params {
   int n_slots;
   int topk;
   float* parts;
+  bool wait_first;           // the predecessor makes the counts and the order too
 };
 
 // NT: 8 NT tokens a tile; FL: pieces per group (1, 2 or 4); kMin: minima;
@@ -260,7 +267,7 @@ __device__ __forceinline__ int expert_tiles(const int* __restrict__ counts, int 
   const int lane = threadIdx.x & 31;
   int row = 0, end = 0;
   for (int e0 = 0; e0 < E; e0 += 32) {
-    const int c = e0 + lane < E ? max(0, __ldg(counts + e0 + lane)) : 0;
+    const int c = e0 + lane < E ? max(0, __ldcg(counts + e0 + lane)) : 0;
     const int k = (c + tok - 1) / tok;
     int ci = c, ki = k;
 #pragma unroll
@@ -303,7 +310,7 @@ __device__ __forceinline__ TokenTile open_tile(const Params<T>& p, int y, const 
 template <class T>
 __device__ __forceinline__ int token_row(const Params<T>& p, const TokenTile& t, int i) {
   const int r = t.r0 + min(i, t.m - 1);
-  return p.sorted_slots ? min(max(__ldg(p.sorted_slots + r), 0), p.n_slots - 1) / p.topk : r;
+  return p.sorted_slots ? min(max(__ldcg(p.sorted_slots + r), 0), p.n_slots - 1) / p.topk : r;
 }
 
 // The runs of stages: U stages of tiles of nst, cut for `ctas` CTAs (at most U,
@@ -314,7 +321,10 @@ struct Runs {
 
   __device__ __forceinline__ long long begin(int cta) const { return U * cta / ctas; }
   // The CTA whose run holds stage u: the last one that begins at u or before.
-  __device__ __forceinline__ int owner(long long u) const { return (int)(((u + 1) * ctas - 1) / U); }
+  __device__ __forceinline__ int owner(long long u) const {
+    const long long a = (u + 1) * ctas - 1;  // < U * ctas; a 64-bit division costs some 100 instructions
+    return U * ctas < (1ll << 31) ? (int)((uint32_t)a / (uint32_t)U) : (int)(a / U);
+  }
   // Where CTA `cta` leaves its sums of a tile, [token][kRows] floats. Along the
   // stages each new (tile, CTA) pair raises tile + cta, so the slots are distinct
   // and there are fewer than tiles + CTAs.
@@ -339,6 +349,10 @@ __global__ void __launch_bounds__(kThreads, S::OCC)
   int* s_row = s_end + p.E;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 
+  // The next launch may start from here on. What this one reads of the counts
+  // and the order is older than its predecessor (or waited for), and so than
+  // everything that can run beside it.
+  if (p.wait_first) griddep_wait();
   griddep_launch();
   if (warp == 0) {
     int y = p.max_y;
@@ -638,32 +652,41 @@ __device__ __forceinline__ Runs open_runs(const Params<T>& p, int grid, int* s_e
   return {U, (int)min((long long)grid, U), nst};
 }
 
-// Sum of the parts of `tile` at [token][row .. row + kV) in K order (kV = 1, or
-// 8 with row a multiple of 8).
-template <int TOK, int kV>
-__device__ __forceinline__ void sum_parts(const Runs& run, float* parts, int tile, int tok, int row, float (&v)[kV]) {
+// Sums of the parts of `tile` at [token][row .. row + kV) and, kN = 2, at
+// kRows / 2 rows on, in K order (kV = 1, or 8 with row a multiple of 8).
+template <int TOK, int kV, int kN>
+__device__ __forceinline__ void sum_parts(const Runs& run, const float* parts, int tile, int tok, int row,
+                                          float (&v)[kN][kV]) {
   const int c0 = run.owner((long long)tile * run.nst), c1 = run.owner((long long)(tile + 1) * run.nst - 1);
 #pragma unroll
-  for (int i = 0; i < kV; ++i) v[i] = 0.f;
+  for (int n = 0; n < kN; ++n)
+#pragma unroll
+    for (int i = 0; i < kV; ++i) v[n][i] = 0.f;
   constexpr int kB = kV == 1 ? 8 : 2;  // parts whose loads are in flight together
-  for (int c = c0; c <= c1; c += kB) {
-    float b[kB][kV];
+  const float* q = parts + (size_t)(tile + c0) * (kRows * TOK) + tok * kRows + row;
+  for (int c = c0; c <= c1; c += kB, q += (size_t)kB * (kRows * TOK)) {
+    float b[kB][kN][kV];
 #pragma unroll
     for (int j = 0; j < kB; ++j)
       if (c + j <= c1) {
-        const float* q = run.part<TOK>(parts, c + j, tile) + tok * kRows + row;
-        if constexpr (kV == 1) {
-          b[j][0] = __ldg(q);
-        } else {
 #pragma unroll
-          for (int i = 0; i < kV; i += 4) *reinterpret_cast<float4*>(&b[j][i]) = __ldg(reinterpret_cast<const float4*>(q + i));
+        for (int n = 0; n < kN; ++n) {
+          const float* at = q + (size_t)j * (kRows * TOK) + n * (kRows / 2);
+          if constexpr (kV == 1) {
+            b[j][n][0] = __ldg(at);
+          } else {
+#pragma unroll
+            for (int i = 0; i < kV; i += 4) *reinterpret_cast<float4*>(&b[j][n][i]) = __ldg(reinterpret_cast<const float4*>(at + i));
+          }
         }
       }
 #pragma unroll
     for (int j = 0; j < kB; ++j)
       if (c + j <= c1) {
 #pragma unroll
-        for (int i = 0; i < kV; ++i) v[i] += b[j][i];
+        for (int n = 0; n < kN; ++n)
+#pragma unroll
+          for (int i = 0; i < kV; ++i) v[n][i] += b[j][n][i];
       }
   }
 }
@@ -688,13 +711,10 @@ __global__ void __launch_bounds__(kRows) finish_kernel(const __grid_constant__ P
     const int y = i / TOK, tok = i - y * TOK, tile = y * p.feature_tiles + f;
     const TokenTile tl = open_tile<kMode, TOK>(p, y, s_end, s_row);
     if (tok >= tl.m) continue;
-    float a[1], u[1];
-    sum_parts<TOK, 1>(run, p.parts, tile, tok, r, a);
-    if constexpr (kMode == kGateUp) {
-      sum_parts<TOK, 1>(run, p.parts, tile, tok, kFeatures + r, u);
-      a[0] = swiglu(a[0], u[0]);
-    }
-    out[(size_t)(tl.r0 + tok) * p.N + n] = from_f<O>(a[0]);
+    constexpr int kN = kMode == kGateUp ? 2 : 1;
+    float v[kN][1];
+    sum_parts<TOK, 1, kN>(run, p.parts, tile, tok, r, v);
+    out[(size_t)(tl.r0 + tok) * p.N + n] = from_f<O>(kN == 2 ? swiglu(v[0][0], v[kN - 1][0]) : v[0][0]);
   }
 }
 
@@ -715,14 +735,11 @@ __global__ void __launch_bounds__(256) act_tokens_kernel(const __grid_constant__
     const TokenTile tl = open_tile<kGateUp, TOK>(p, y, s_end, s_row);
     if (tok >= tl.m) continue;
     const int n = st * kStageElems + lane * 8, f = n / (kRows / 2);
-    float a[8] = {}, u[8] = {};
-    if (f < p.feature_tiles) {
-      const int tile = y * p.feature_tiles + f;
-      sum_parts<TOK, 8>(run, p.parts, tile, tok, n % (kRows / 2), a);
-      sum_parts<TOK, 8>(run, p.parts, tile, tok, kRows / 2 + n % (kRows / 2), u);
-    }
+    float v[2][8] = {}, a[8];
+    if (f < p.feature_tiles)
+      sum_parts<TOK, 8, 2>(run, p.parts, y * p.feature_tiles + f, tok, n % (kRows / 2), v);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) a[i] = n + i < p.N ? swiglu(a[i], u[i]) : 0.f;
+    for (int i = 0; i < 8; ++i) a[i] = n + i < p.N ? swiglu(v[0][i], v[1][i]) : 0.f;
     write_run<true>(act, tl.r0 + tok, st, nst, a);
   }
 }
@@ -740,21 +757,52 @@ __global__ void __launch_bounds__(kRows)
   griddep_wait();
   int *s_end = s_index, *s_row = s_index + p.E;
   const Runs run = open_runs<kDown, TOK>(p, grid, s_end, s_row, &s_y);
+  // Where the slots' sums lie: first part, parts (0: dropped) and weight, found
+  // by one lane each; then every thread adds its feature's.
+  constexpr int kSlots = 32;
+  __shared__ size_t s_at[kSlots];
+  __shared__ int s_parts[kSlots];
+  __shared__ float s_w[kSlots];
   const int f = blockIdx.x, n = f * kRows + threadIdx.x;
-  if (n >= p.N) return;
   for (int t = blockIdx.y; t < tokens; t += gridDim.y) {
     float acc = 0.f;
-    for (int j = 0; j < topk; ++j) {
-      const long long s = (long long)t * topk + j;
-      const int r = __ldg(slot_rows + s), e = __ldg(ids + s);
-      if (r < 0 || r >= p.n_rows || e < 0 || e >= p.E) continue;
-      const int at = r - s_row[e], y = (e ? s_end[e - 1] : 0) + at / TOK;
-      if (at < 0 || y >= min(s_end[e], s_y)) continue;
-      float v[1];
-      sum_parts<TOK, 1>(run, p.parts, y * p.feature_tiles + f, at % TOK, threadIdx.x, v);
-      acc = fmaf(__ldg(weights + s), v[0], acc);
+    for (int j0 = 0; j0 < topk; j0 += kSlots) {
+      const int kn = min(kSlots, topk - j0);
+      __syncthreads();
+      if (threadIdx.x < kn) {
+        const long long s = (long long)t * topk + j0 + threadIdx.x;
+        const int r = __ldg(slot_rows + s), e = __ldg(ids + s);
+        s_parts[threadIdx.x] = 0;
+        s_w[threadIdx.x] = __ldg(weights + s);
+        if (r >= 0 && r < p.n_rows && e >= 0 && e < p.E) {
+          const int at = r - s_row[e], y = (e ? s_end[e - 1] : 0) + at / TOK;
+          if (at >= 0 && y < min(s_end[e], s_y)) {
+            const int tile = y * p.feature_tiles + f;
+            const int c0 = run.owner((long long)tile * run.nst), c1 = run.owner((long long)(tile + 1) * run.nst - 1);
+            s_at[threadIdx.x] = (size_t)(tile + c0) * (kRows * TOK) + (at % TOK) * kRows;
+            s_parts[threadIdx.x] = c1 - c0 + 1;
+          }
+        }
+      }
+      __syncthreads();
+      if (n >= p.N) continue;
+      constexpr int kB = 8;  // slots, and parts of a slot, whose loads are in flight together
+      for (int j = 0; j < kn; j += kB) {
+        float v[kB];
+#pragma unroll
+        for (int i = 0; i < kB; ++i)
+          if (j + i < kn && s_parts[j + i] > 0) v[i] = __ldg(p.parts + s_at[j + i] + threadIdx.x);
+#pragma unroll
+        for (int i = 0; i < kB; ++i) {
+          if (j + i >= kn || s_parts[j + i] == 0) continue;
+          const float* q = p.parts + s_at[j + i] + threadIdx.x;
+#pragma unroll 8
+          for (int c = 1; c < s_parts[j + i]; ++c) v[i] += __ldg(q + (size_t)c * (kRows * TOK));
+          acc = fmaf(s_w[j + i], v[i], acc);
+        }
+      }
     }
-    out[(size_t)t * p.N + n] = from_f<T>(acc);
+    if (n < p.N) out[(size_t)t * p.N + n] = from_f<T>(acc);
   }
 }
 

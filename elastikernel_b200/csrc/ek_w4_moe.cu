@@ -1,4 +1,5 @@
 // The experts' products of a fused MoE layer with 4-bit weights.
+#include "ek_moe_order.cuh"
 #include "ek_w4_kernel.cuh"
 
 namespace ek {
@@ -47,6 +48,43 @@ MoeLayout moe_layout(long long x_rows, int rows, int E, int H, int I, int sms) {
   return l;
 }
 
+// The start of a layer in one launch, for up to kOrderThreads slots: the first
+// CTA routes the tokens and orders their slots, the others write the tokens of
+// the gate/up product, a warp per run.
+struct Order {
+  int *ids, *sorted_slots, *slot_rows, *counts;
+  float* weights;
+};
+__global__ void __launch_bounds__(kOrderThreads)
+    front_kernel(const float* __restrict__ logits, const bf16* __restrict__ x, int T, int k, int E, int H, bool vec,
+                 Order o, Tokens tokens) {
+  extern __shared__ int sm[];
+  griddep_launch();  // the next launch waits for the whole of this one
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = T * k;
+  if (blockIdx.x > 0) {
+    write_tokens(x, T, H, vec, tokens, (long long)(blockIdx.x - 1) * (kOrderThreads / 32) + warp,
+                 (long long)(gridDim.x - 1) * (kOrderThreads / 32));
+    return;
+  }
+  for (int t = warp; t < T; t += kOrderThreads / 32)
+    route_token(logits + (size_t)t * E, E, k, lane, o.ids + (size_t)t * k, o.weights + (size_t)t * k);
+  __syncthreads();
+  int id = tid < n ? o.ids[tid] : -1;
+  if (id >= E) {  // a row of NaN
+    atomicOr(&g_ek_status, kStatusBadIndex);
+    id = -1;
+  }
+  int kept;
+  const int row = order_slots(id, n, E, sm, &kept);
+  const int* start = sm + (n + 31) / 32 * E;
+  if (tid < E) o.counts[tid] = (tid + 1 < E ? start[tid + 1] : kept) - start[tid];
+  if (tid < n) {
+    o.slot_rows[tid] = row;
+    if (row >= 0) o.sorted_slots[row] = tid;
+    if (tid >= kept) o.sorted_slots[tid] = n;
+  }
+}
+
 struct Matrix {
   const void *codes, *scales, *mins;
 };
@@ -77,7 +115,8 @@ struct Moe {
     p.parts = reinterpret_cast<float*>(ws + l.parts);
     return p;
   }
-  // x (x_rows of them) -> the sums of the gate/up product
+  // x (x_rows of them; null: the tokens x() are being written by the launch
+  // before, with the counts and the order) -> the sums of the gate/up product
   int gate_up(const bf16* xin, int x_rows, const int* sorted_slots, int topk, const Matrix& w1, const Matrix& w3,
               Params<bf16>* out) const {
     Params<bf16> p = params(H, I, kRows / 2, x());
@@ -86,11 +125,12 @@ struct Moe {
     p.sorted_slots = sorted_slots;
     p.topk = topk;
     p.n_slots = rows;
+    p.wait_first = xin == nullptr;
     *out = p;
     CUtensorMap m1, m3;
     int rc = codes_map(&m1, w1.codes, (long long)E * I, H, kRows / 2);
     if (!rc) rc = codes_map(&m3, w3.codes, (long long)E * I, H, kRows / 2);
-    if (!rc) rc = launch_tokens(xin, x_rows, H, p.x, stream, true);
+    if (!rc && xin) rc = launch_tokens(xin, x_rows, H, p.x, stream, true);
     if (!rc) rc = launch_product<bf16, kGateUp>(l.nt, group, m1, m3, p, l.grid, stream);
     return rc;
   }
@@ -111,6 +151,18 @@ struct Moe {
   template <Mode kMode, class O>
   int finish(const Params<bf16>& p, O* out) const {
     return l.nt == 1 ? finish_tok<kMode, 8>(p, out) : l.nt == 2 ? finish_tok<kMode, 16>(p, out) : finish_tok<kMode, 32>(p, out);
+  }
+  // gate/up, down and combine, from an order of the slots
+  int layer(const bf16* xin, const Order& o, int T, int topk, const Matrix& w1, const Matrix& w3, const Matrix& w2,
+            bf16* out) const {
+    Params<bf16> p;
+    int rc = gate_up(xin, T, o.sorted_slots, topk, w1, w3, &p);
+    if (!rc) rc = l.nt == 1 ? act_tokens<8>(p) : l.nt == 2 ? act_tokens<16>(p) : act_tokens<32>(p);
+    if (!rc) rc = down(w2, &p);
+    if (rc) return rc;
+    return l.nt == 1   ? combine<8>(p, o.slot_rows, o.ids, o.weights, T, topk, out)
+           : l.nt == 2 ? combine<16>(p, o.slot_rows, o.ids, o.weights, T, topk, out)
+                       : combine<32>(p, o.slot_rows, o.ids, o.weights, T, topk, out);
   }
   template <int TOK>
   int act_tokens(const Params<bf16>& p) const {
@@ -238,17 +290,70 @@ int ek_moe_experts_w4(const void* x, int T, int topk, const int* topk_ids, const
   if (misaligned16bit({x, out})) return set_error(EK_ERR_INVALID, "experts_w4: x and out must be aligned to their elements");
   Moe m;
   rc = open_moe("experts_w4", &m, T, expert_counts, (int)rows, E, H, I, group, num_sms, workspace, ws_bytes, stream);
-  Params<bf16> p;
-  if (!rc)
-    rc = m.gate_up(static_cast<const bf16*>(x), T, sorted_slots, topk, {w1_codes, w1_scales, w1_mins},
-                   {w3_codes, w3_scales, w3_mins}, &p);
-  if (!rc) rc = m.l.nt == 1 ? m.act_tokens<8>(p) : m.l.nt == 2 ? m.act_tokens<16>(p) : m.act_tokens<32>(p);
-  if (!rc) rc = m.down({w2_codes, w2_scales, w2_mins}, &p);
   if (rc) return rc;
-  bf16* o = static_cast<bf16*>(out);
-  return m.l.nt == 1   ? m.combine<8>(p, slot_rows, topk_ids, topk_weights, T, topk, o)
-         : m.l.nt == 2 ? m.combine<16>(p, slot_rows, topk_ids, topk_weights, T, topk, o)
-                       : m.combine<32>(p, slot_rows, topk_ids, topk_weights, T, topk, o);
+  // the maps are read only
+  const Order o{const_cast<int*>(topk_ids), const_cast<int*>(sorted_slots), const_cast<int*>(slot_rows),
+                const_cast<int*>(expert_counts), const_cast<float*>(topk_weights)};
+  return m.layer(static_cast<const bf16*>(x), o, T, topk, {w1_codes, w1_scales, w1_mins}, {w3_codes, w3_scales, w3_mins},
+                 {w2_codes, w2_scales, w2_mins}, static_cast<bf16*>(out));
+}
+
+size_t ek_fused_moe_w4_workspace_bytes(int T, int topk, int E, int H, int I, int num_sms) {
+  if (T < 0 || topk < 1 || topk > kRouteMaxK || E < 1 || E > kRouteMaxE) return (size_t)-1;
+  const size_t experts = ek_moe_w4_workspace_bytes(T, (int)std::min<long long>((long long)T * topk, 0x7fffffff), E, H, I, num_sms);
+  if (experts == (size_t)-1 || T == 0) return experts;
+  return experts + 256 + ((size_t)4 * T * topk + E + 1) * sizeof(int) + ek_moe_permute_scratch_bytes(T, topk, E);
+}
+
+int ek_fused_moe_w4(const void* x, const float* logits, int T, int topk, const void* w1_codes, const void* w1_scales,
+                    const void* w1_mins, const void* w3_codes, const void* w3_scales, const void* w3_mins,
+                    const void* w2_codes, const void* w2_scales, const void* w2_mins, void* out, int E, int H, int I,
+                    int group, int num_sms, void* workspace, size_t ws_bytes, void* stream) {
+  clear_error();
+  if (E < 1 || E > kRouteMaxE || topk < 1 || topk > kRouteMaxK || topk > E)
+    return set_error(EK_ERR_INVALID, "fused_moe_w4: need 1 <= E <= %d and 1 <= k <= min(%d, E) (E=%d k=%d)", kRouteMaxE,
+                     kRouteMaxK, E, topk);
+  const long long rows = (long long)T * topk;
+  int rc = check_sizes("fused_moe_w4", T, rows, E, H, I);
+  if (rc || T == 0) return rc;
+  rc = check_w4("fused_moe_w4", w1_codes, w1_scales, w1_mins, H, group);
+  if (!rc) rc = check_w4("fused_moe_w4", w3_codes, w3_scales, w3_mins, H, group);
+  if (!rc) rc = check_w4("fused_moe_w4", w2_codes, w2_scales, w2_mins, I, group);
+  if (rc) return rc;
+  if (!x || !logits || !out || !workspace || !w1_mins != !w3_mins)
+    return set_error(EK_ERR_INVALID, "fused_moe_w4: null pointer");
+  if (misaligned16bit({x, out}) || (reinterpret_cast<uintptr_t>(logits) & 3u))
+    return set_error(EK_ERR_INVALID, "fused_moe_w4: x, logits and out must be aligned to their elements");
+  int sms = 0;
+  rc = resolve_num_sms(num_sms, stream, &sms);
+  if (rc) return rc;
+  const size_t need = ek_fused_moe_w4_workspace_bytes(T, topk, E, H, I, sms);
+  if (!aligned16(workspace) || ws_bytes < need)
+    return set_error(EK_ERR_INVALID, "fused_moe_w4: workspace must be 16-byte aligned and hold %zu bytes (got %zu)", need,
+                     ws_bytes);
+  const size_t experts = ek_moe_w4_workspace_bytes(T, (int)rows, E, H, I, sms);
+  int* ints = reinterpret_cast<int*>(static_cast<uint8_t*>(workspace) + (experts + 255) / 256 * 256);
+  const int n = (int)rows;
+  const Order o{ints, ints + n, ints + 2 * n, ints + 4 * n, reinterpret_cast<float*>(ints + 3 * n)};
+  Moe m;
+  rc = open_moe("fused_moe_w4", &m, T, o.counts, n, E, H, I, group, sms, workspace, experts, stream);
+  if (rc) return rc;
+  const bf16* xin = static_cast<const bf16*>(x);
+  if (n <= kOrderThreads) {
+    const int warps = T * stages(H), per = kOrderThreads / 32;
+    const int grid = 1 + std::min((warps + per - 1) / per, 147);
+    rc = launch("w4 front launch", front_kernel, dim3(grid), kOrderThreads, order_smem_ints(n, E) * sizeof(int), m.stream,
+                true, logits, xin, T, topk, E, H, H % 8 == 0 && aligned16(xin), o, m.x());
+    xin = nullptr;
+  } else {
+    rc = ek_moe_route(logits, T, E, topk, o.ids, o.weights, stream);
+    if (!rc)
+      rc = ek_moe_dispatch(o.ids, T, topk, E, nullptr, 0, 0, o.sorted_slots, o.slot_rows, o.counts, o.counts + E, nullptr,
+                           o.counts + E + 1, stream);
+  }
+  if (rc) return rc;
+  return m.layer(xin, o, T, topk, {w1_codes, w1_scales, w1_mins}, {w3_codes, w3_scales, w3_mins},
+                 {w2_codes, w2_scales, w2_mins}, static_cast<bf16*>(out));
 }
 
 }  // extern "C"

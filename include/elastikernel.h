@@ -544,6 +544,16 @@ int ek_moe_experts_w4(const void* x, int T, int topk, const int* topk_ids, const
                       const void* w3_mins, const void* w2_codes, const void* w2_scales, const void* w2_mins, void* out,
                       int E, int H, int I, int group, int num_sms, void* workspace, size_t ws_bytes, void* stream);
 
+/* The whole layer from the gate logits: ek_moe_route, ek_moe_dispatch (order
+ * only) and ek_moe_experts_w4, the first two and the tokens' conversion as one
+ * launch up to 1024 slots. A token whose logits are all NaN is dropped and
+ * raises EK_STATUS_BAD_INDEX. E <= 256, topk <= 8. */
+size_t ek_fused_moe_w4_workspace_bytes(int T, int topk, int E, int H, int I, int num_sms);
+int ek_fused_moe_w4(const void* x, const float* logits, int T, int topk, const void* w1_codes, const void* w1_scales,
+                    const void* w1_mins, const void* w3_codes, const void* w3_scales, const void* w3_mins,
+                    const void* w2_codes, const void* w2_scales, const void* w2_mins, void* out, int E, int H, int I,
+                    int group, int num_sms, void* workspace, size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

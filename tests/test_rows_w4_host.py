@@ -207,6 +207,24 @@ def test_moe_w4_refusals():
     assert experts(T=0) == _lib.EK_OK
     assert L.ek_moe_w4_workspace_bytes(4, 8, 4, 64, 32, 0) == _ops._SIZE_MAX
 
+    def fused(x=_p(), logits=_p(), T=4, topk=2, c1=_p(), m2=n, out=_p(), E=4, group=32, ws=_p(), size=big):
+        return L.ek_fused_moe_w4(x, logits, T, topk, c1, _p(), n, _p(), _p(), n, _p(), _p(), m2, out, E, 64, 32, group,
+                                 148, ws, size, n)
+
+    _bad(fused(E=257), "1 <= E <= 256")
+    _bad(fused(topk=5), "1 <= k")
+    _bad(fused(topk=9, E=16), "1 <= k")
+    _bad(fused(T=-1), "bad sizes")
+    _bad(fused(T=1 << 24), "too many rows")
+    _bad(fused(logits=n), "null pointer")
+    _bad(fused(ws=n), "null pointer")
+    _bad(fused(logits=_p(258)), "aligned")
+    _bad(fused(c1=_p(8)), "16-byte aligned")
+    _bad(fused(group=8), "group")
+    _bad(fused(size=L.ek_fused_moe_w4_workspace_bytes(4, 2, 4, 64, 32, 148) - 1), "workspace")
+    assert fused(T=0) == _lib.EK_OK
+    assert L.ek_fused_moe_w4_workspace_bytes(4, 9, 16, 64, 32, 148) == _ops._SIZE_MAX
+
 
 def test_front_end_refuses_cpu_tensors():
     ids = torch.zeros((2, 2), dtype=torch.int32)

@@ -211,7 +211,8 @@ def test_gemm_empty_and_refusals(cuda_dev):
 MOE = [  # T, k, E, H, I, group, mins
     (1, 1, 1, 32, 32, 32, False), (1, 2, 8, 4096, 512, 128, False), (3, 2, 4, 200, 136, 64, True),
     (17, 8, 60, 512, 260, 32, False), (64, 8, 32, 1024, 256, 128, False), (40, 3, 5, 257, 65, 64, True),
-    (300, 2, 4, 256, 384, 128, False), (33, 1, 300, 64, 96, 32, False),
+    (300, 2, 4, 256, 384, 128, False), (33, 1, 300, 64, 96, 32, False), (700, 2, 6, 128, 192, 64, True),
+    (128, 8, 16, 136, 72, 32, False),
 ]
 
 
@@ -286,6 +287,9 @@ def test_fused_layer(case, cuda_dev):
     # the fp32 sums inside are 2^-24-sized; 1 % on top of the roundings covers them
     bound = 2.0 ** -8 * np.abs(exact) * 1.01 + 2.0 ** -11 * 1.01 * spread + 1e-30
     assert (np.abs(_np(got) - exact) <= bound).all()
+    # the same from its parts, bit for bit
+    rids, rw = _ops.moe_route(logits, k)
+    assert torch.equal(_ops.moe_experts_w4(_ops.moe_dispatch(None, rids, E), x, rids, rw, qw), got)
     # stage by stage with bf16 activations and rows: their roundings on top (2^-8 of each term, twice)
     p = _ops.moe_dispatch(None, torch.from_numpy(np.asarray(ids, np.int32)).to(cuda_dev), E)
     y = _ops.moe_down_w4(p, _ops.moe_gate_up_w4(p, qw, x=x), qw)
@@ -293,6 +297,34 @@ def test_fused_layer(case, cuda_dev):
     assert (np.abs(_np(staged) - exact) <= 2.0 ** -8 * (1.01 * np.abs(exact) + 1.01 * spread) + 1e-30).all()
     out = torch.empty_like(x)
     assert _ops.fused_moe_w4(x, logits, qw, k, out=out) is out and torch.equal(out, got)
+
+
+def test_experts_with_dropped_slots(cuda_dev):
+    """Dropped slots weigh nothing; a token without any gets zero."""
+    T, k, E, H, I = 21, 3, 6, 96, 160
+    x, ids, qw = _moe_setup((T, k, E, H, I, 32, True), cuda_dev)
+    ids[5] = -1
+    ids[::4, 1] = -1
+    w = torch.rand((T, k), device=cuda_dev)
+    p = _ops.moe_dispatch(x, ids, E)
+    got = _ops.moe_experts_w4(p, x, ids, w, qw)
+    y = _ops.moe_down_w4(p, _ops.moe_gate_up_w4(p, qw, dtype=torch.float32), qw, dtype=torch.float32)
+    kept = int(p["num_rows_padded"])
+    want = _ops.moe_combine_weighted(p, torch.where(torch.arange(T * k, device=cuda_dev)[:, None] < kept, y, 0.0), w)
+    assert torch.equal(want.to(BF), got) and not got[5].any()
+    none = torch.full_like(ids, -1)
+    assert not _ops.moe_experts_w4(_ops.moe_dispatch(None, none, E), x, none, w, qw).any()
+
+
+def test_token_of_nan_logits_is_reported_and_dropped(cuda_dev):
+    x, _, qw = _moe_setup((5, 2, 8, 64, 96, 32, False), cuda_dev)
+    logits = torch.randn((5, 8), device=cuda_dev)
+    clean = _ops.fused_moe_w4(x, logits, qw, 2)
+    logits[3] = float("nan")
+    got = _ops.fused_moe_w4(x, logits, qw, 2)
+    assert _lib.device_status(0) == _lib.EK_STATUS_BAD_INDEX
+    keep = [0, 1, 2, 4]
+    assert torch.equal(got[keep], clean[keep]) and not got[3].any()
 
 
 def test_layer_forward_and_router_backward(cuda_dev):
