@@ -709,11 +709,11 @@ def moe_dispatch(x: torch.Tensor | None, topk_ids: torch.Tensor, num_experts: in
     if x is not None:
         dt = _check_rows("x", x, T)
         H = x.shape[1]
-        x_perm = torch.empty((n, H), dtype=x.dtype, device=dev)
+        x_perm = x.new_empty((n, H))
     L = lib()
     ints = int(L.ek_moe_permute_scratch_bytes(T, k, E)) // 4
     sorted_slots, slot_rows, counts, num_rows, scratch = torch.empty(
-        2 * n + max(E, 0) + 1 + ints, dtype=torch.int32, device=dev).split([n, n, max(E, 0), 1, ints])
+        2 * n + max(E, 0) + 1 + ints, dtype=torch.int32, device=dev).split_with_sizes([n, n, max(E, 0), 1, ints])
     with _on_device(dev):
         check(L.ek_moe_dispatch(topk_ids.data_ptr(), T, k, E, _ptr(x), H, dt, sorted_slots.data_ptr(),
                                 slot_rows.data_ptr(), counts.data_ptr(), num_rows.data_ptr(), _ptr(x_perm),
@@ -729,7 +729,7 @@ def moe_dispatch_grad(perm: dict, d_rows: torch.Tensor) -> torch.Tensor:
     dev = _require_cuda(d_rows, slot_rows)
     dt = _check_rows("d_rows", d_rows)
     T, k, (n, H) = perm["T"], perm["topk"], d_rows.shape
-    d_x = torch.empty((T, H), dtype=d_rows.dtype, device=dev)
+    d_x = d_rows.new_empty((T, H))
     with _on_device(dev):
         check(lib().ek_moe_dispatch_grad(d_rows.data_ptr(), slot_rows.data_ptr(), T, k, n, H, dt, d_x.data_ptr(),
                                          current_stream_handle(dev)), "ek_moe_dispatch_grad")
@@ -746,7 +746,7 @@ def moe_combine_weighted(perm: dict, rows: torch.Tensor, topk_weights: torch.Ten
     T, k, (n, H) = perm["T"], perm["topk"], rows.shape
     _check_slots("topk_weights", topk_weights, T, k, torch.float32)
     if out is None:
-        out = torch.empty((T, H), dtype=rows.dtype, device=dev)
+        out = rows.new_empty((T, H))
     elif out.dtype != rows.dtype or out.shape != (T, H) or not out.is_contiguous():
         raise RuntimeError("out must be a contiguous [T, H] tensor of the rows' dtype")
     with _on_device(dev):
@@ -769,7 +769,7 @@ def moe_combine_weighted_grad(perm: dict, rows: torch.Tensor, topk_weights: torc
         raise RuntimeError(f"d_out must be a {rows.dtype} tensor of shape {(T, H)}")
     _contig("d_out", d_out)
     d_rows = torch.empty_like(rows)
-    d_weights = torch.empty((T, k), dtype=torch.float32, device=dev)
+    d_weights = torch.empty_like(topk_weights)
     with _on_device(dev):
         check(lib().ek_moe_combine_weighted_grad(rows.data_ptr(), slot_rows.data_ptr(), topk_weights.data_ptr(),
                                                  d_out.data_ptr(), perm["num_rows_padded"].data_ptr(), T, k, n, H, dt,
@@ -794,7 +794,7 @@ def moe_route_grad(topk_ids: torch.Tensor, topk_weights: torch.Tensor, d_weights
     E = int(num_experts)
     if E < 1:
         raise RuntimeError("num_experts must be positive")
-    d_logits = torch.empty((T, E), dtype=torch.float32, device=dev)
+    d_logits = d_weights.new_empty((T, E))
     with _on_device(dev):
         check(lib().ek_moe_route_grad(topk_ids.data_ptr(), topk_weights.data_ptr(), d_weights.data_ptr(), T, E, k,
                                       d_logits.data_ptr(), current_stream_handle(dev)), "ek_moe_route_grad")

@@ -9,17 +9,18 @@
 
 namespace ek {
 
-constexpr int kRouteMaxE = 256;   // logits per token held in registers: 8 per lane
+constexpr int kRouteMaxE = 256;   // logits per token held in registers: up to 8 per lane
 constexpr int kRouteMaxK = 8;
 
 // One token's routing by one warp: logits row -> k expert ids and
-// renormalised weights (written by lane 0).
-__device__ __forceinline__ void route_token(const float* __restrict__ row, int E, int k, int lane,
-                                            int* __restrict__ ids_out, float* __restrict__ wts_out) {
-  float v[kRouteMaxE / 32];
+// renormalised weights (written by lane 0); kRegs logits per lane, 32 kRegs >= E.
+template <int kRegs>
+__device__ __forceinline__ void route_token_regs(const float* __restrict__ row, int E, int k, int lane,
+                                                 int* __restrict__ ids_out, float* __restrict__ wts_out) {
+  float v[kRegs];
   float mx = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < kRouteMaxE / 32; ++i) {
+  for (int i = 0; i < kRegs; ++i) {
     const int e = lane + 32 * i;
     v[i] = (e < E) ? row[e] : -INFINITY;
     mx = fmaxf(mx, v[i]);
@@ -28,7 +29,7 @@ __device__ __forceinline__ void route_token(const float* __restrict__ row, int E
   for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   float s = 0.f;
 #pragma unroll
-  for (int i = 0; i < kRouteMaxE / 32; ++i)
+  for (int i = 0; i < kRegs; ++i)
     if (lane + 32 * i < E) s += expf(v[i] - mx);
 #pragma unroll
   for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -45,7 +46,7 @@ __device__ __forceinline__ void route_token(const float* __restrict__ row, int E
     float bv = -INFINITY;
     int bi = 0x7fffffff;
 #pragma unroll
-    for (int i = 0; i < kRouteMaxE / 32; ++i) {
+    for (int i = 0; i < kRegs; ++i) {
       const int e = lane + 32 * i;
       if (e < E && !(taken & (1u << i)) && (v[i] > bv || (v[i] == bv && e < bi))) {
         bv = v[i];
@@ -74,6 +75,13 @@ __device__ __forceinline__ void route_token(const float* __restrict__ row, int E
       wts_out[j] = p[j] / psum;
     }
   }
+}
+
+__device__ __forceinline__ void route_token(const float* __restrict__ row, int E, int k, int lane,
+                                            int* __restrict__ ids_out, float* __restrict__ wts_out) {
+  if (E <= 32) route_token_regs<1>(row, E, k, lane, ids_out, wts_out);
+  else if (E <= 64) route_token_regs<2>(row, E, k, lane, ids_out, wts_out);
+  else route_token_regs<kRouteMaxE / 32>(row, E, k, lane, ids_out, wts_out);
 }
 
 // ------------------------------------------------------------------ order

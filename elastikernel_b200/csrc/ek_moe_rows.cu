@@ -610,8 +610,8 @@ int launch_small(const Dispatch& d, size_t row_bytes) {
     if (rc) return rc;
     attr_done[dev] = true;
   }
-  // one warp per unit of the copy, at most a CTA per SM
-  const int grid = d.x ? std::max(1, std::min(148, (d.T * runs_per_row<kCopyRun>(nvec) + 31) / 32)) : 1;
+  // the units of the copy over up to a CTA per SM
+  const int grid = d.x ? std::max(1, std::min(148, d.T * runs_per_row<kCopyRun>(nvec))) : 1;
   dispatch_small_kernel<V><<<grid, kOrderThreads, smem, d.s>>>(d.ids, d.T, d.k, d.E, static_cast<const Raw*>(d.x), nvec,
                                                              d.sorted_slots, d.slot_rows, d.counts, d.num_rows,
                                                              static_cast<Raw*>(d.rows));

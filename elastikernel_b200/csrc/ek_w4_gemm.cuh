@@ -33,19 +33,22 @@ int gemm(const GemmArgs& a) {
   p.K = a.K;
   p.N = a.N;
   p.feature_tiles = (a.N + kRows - 1) / kRows;
-  p.x = {reinterpret_cast<__half*>(ws), reinterpret_cast<float*>(ws + l.scales)};
+  p.x = {ws};
   p.n_rows = a.M;
   p.max_y = max_token_tiles(a.M, 0, nt);
   p.parts = reinterpret_cast<float*>(ws + l.parts);
   CUtensorMap map;
   int rc = codes_map(&map, a.codes, a.N, a.K, kRows);
-  if (!rc) rc = launch_tokens(static_cast<const T*>(a.A), a.M, a.K, p.x, a.stream, true);
+  p.rows = static_cast<const T*>(a.A);
+  p.vec = a.K % 8 == 0 && aligned16(a.A);
+  if (!rc && nt > 1) rc = launch_tokens(p.rows, a.M, a.K, a.group, p.x, a.stream);
   if (!rc) rc = launch_product<T, kDense>(nt, a.group, map, map, p, grid, a.stream);
   if (rc) return rc;
   const dim3 g(p.feature_tiles, std::min(p.max_y * 8 * nt, 4096));
   T* out = static_cast<T*>(a.C);
   if (nt == 1) return launch("w4 sums launch", finish_kernel<kDense, 8, T, T>, g, kRows, 0, a.stream, false, p, grid, out);
   if (nt == 2) return launch("w4 sums launch", finish_kernel<kDense, 16, T, T>, g, kRows, 0, a.stream, false, p, grid, out);
+  if (nt == 3) return launch("w4 sums launch", finish_kernel<kDense, 24, T, T>, g, kRows, 0, a.stream, false, p, grid, out);
   return launch("w4 sums launch", finish_kernel<kDense, 32, T, T>, g, kRows, 0, a.stream, false, p, grid, out);
 }
 

@@ -20,9 +20,9 @@
 //     largest lose at most 2^-40 of it, less than the fp32 sums do; fp32 rows
 //     (the experts' activations) are rounded to 11 bits;
 //   * sums of one group in fp32 accumulators, then multiplied by the group's
-//     fp32 scale: both operands are exact, so no weight is ever rounded; the
-//     minima enter as m * sum(x), the sum taken by the same instruction with a
-//     matrix of ones;
+//     fp32 scale: both operands are exact, so no weight is ever rounded. With
+//     minima w = s (q - 8) + (m + 8 s), and the second term meets the sum of the
+//     group's tokens, which the token kernel has left beside them;
 //   * codes by TMA, 32 KB a stage (16 KB boxes and up are what the TMA engine
 //     streams at full bandwidth), from one producer warp to eight consumer
 //     warps of 32 weight rows each;
@@ -55,7 +55,10 @@ constexpr int kWarps = 8;                    // consumer warps
 constexpr int kThreads = 32 * (kWarps + 1);  // and the producer
 constexpr int kRows = 32 * kWarps;           // weight rows per tile (gate/up: half of each matrix)
 constexpr int kStageBytes = kRows * 128;
-constexpr int kTokenPitch = kStageElems * 2 + 64;  // bytes of a token's run in a stage; + 64: conflict-free reads
+// Bytes of a token's record of a stage: 256 halfs, then its scale and the sums
+// of its groups (fp32; at most 8). 64 more than 512 also keeps the reads of
+// eight tokens free of bank conflicts.
+constexpr int kRecord = kStageElems * 2 + 64;
 
 __host__ __device__ inline int pieces(int K) { return (K + kPiece - 1) / kPiece; }
 __host__ __device__ inline int groups(int K, int group) { return (K + group - 1) / group; }
@@ -80,16 +83,12 @@ __device__ __forceinline__ uint32_t nibbles(uint32_t w, uint32_t mask) {
 }
 
 // Pairs (k = c, c + 4), c = 2 h and 2 h + 1, of a code word as exact fp16
-// integers q - 8 (kMin: q). The low nibble gives 1024 + q, the high one
-// 1024 + 16 q.
-template <bool kMin>
+// integers q - 8. The low nibble gives 1024 + q, the high one 1024 + 16 q.
 __device__ __forceinline__ void code_pairs(uint32_t w, int h, uint32_t& lo, uint32_t& hi) {
   const uint32_t v = h ? w >> 8 : w;
   const uint32_t a = nibbles(v, 0x000f000fu), b = nibbles(v, 0x00f000f0u);
-  const uint32_t ca = kMin ? 0xe400e400u : 0xe408e408u;  // -1024, -1032
-  const uint32_t cb = kMin ? 0xd400d400u : 0xd480d480u;  // -64, -72
-  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(a), "r"(ca));
-  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(hi) : "r"(b), "r"(0x2c002c00u), "r"(cb));  // 1/16
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(a), "r"(0xe408e408u));                        // - 1032
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(hi) : "r"(b), "r"(0x2c002c00u), "r"(0xd480d480u));  // / 16 - 72
 }
 
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -121,6 +120,12 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   return v;
 }
 
+__device__ __forceinline__ float lds32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+  return v;
+}
+
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -129,26 +134,21 @@ __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
 }
 
 // ------------------------------------------------------------------ tokens
-// A row of K elements takes row_halfs(K) halfs of the workspace, zero past K,
-// so that whole stages can be read; a warp reads up to a stage ahead, hence the
-// slack behind the last row.
+// A token row of K elements is stages(K) records, zero past K.
 __host__ __device__ inline int stages(int K) { return (K + kStageElems - 1) / kStageElems; }
-__host__ __device__ inline int row_halfs(int K) { return stages(K) * kStageElems; }
 
+// [rows][stages(K)] records; each run of 8 halfs in the order 0 4 1 5 2 6 3 7.
 struct Tokens {
-  __half* x;     // [rows][row_halfs(K)], each run of 8 in the order 0 4 1 5 2 6 3 7
-  float* scale;  // [rows][stages(K)]: what each run of 256 was divided by
+  uint8_t* rec;
 };
 
-// The workspace of one product: the tokens, their scales, and the CTAs' sums.
+// The workspace of one product: the token records and the CTAs' sums.
 struct Layout {
-  size_t scales, parts, bytes;
+  size_t parts, bytes;
 };
 inline Layout layout(long long rows, int K, long long tiles, int ctas, int tok) {
-  auto up = [](size_t v) { return (v + 255) / 256 * 256; };
   Layout l;
-  l.scales = up(((size_t)rows * row_halfs(K) + kStageElems) * 2);
-  l.parts = l.scales + up(((size_t)rows * stages(K) + 1) * 4);
+  l.parts = ((size_t)rows * stages(K) * kRecord + 255) / 256 * 256;
   l.bytes = l.parts + ((size_t)tiles + ctas) * kRows * tok * 4;
   return l;
 }
@@ -156,11 +156,12 @@ inline Layout layout(long long rows, int K, long long tiles, int ctas, int tok) 
 __device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void griddep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-// A warp writes run `st` of row `row`: eight elements v per lane. The scale
-// comes from the largest finite magnitude, so an infinity or a NaN stays what it
-// is and its neighbours stay finite. kScaled = false (fp16 rows): as they are.
+// A warp writes record `at`: eight elements v per lane. The scale comes from the
+// largest finite magnitude, so an infinity or a NaN stays what it is and its
+// neighbours stay finite. kScaled = false (fp16 rows): as they are. The sums are
+// those of the rounded halfs, per `group` elements.
 template <bool kScaled>
-__device__ __forceinline__ void write_run(const Tokens& out, size_t row, int st, int nst, const float (&v)[8]) {
+__device__ __forceinline__ void write_run(const Tokens& out, size_t at, int group, const float (&v)[8]) {
   const int lane = threadIdx.x & 31;
   float f = 1.f, inv = 1.f;
   if constexpr (kScaled) {
@@ -177,43 +178,56 @@ __device__ __forceinline__ void write_run(const Tokens& out, size_t row, int st,
     inv = __uint_as_float((uint32_t)(127 - up) << 23);
   }
   __half2 h[4];
+  float sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(v[i] * f, v[i + 4] * f);
-  *reinterpret_cast<uint4*>(out.x + (row * nst + st) * kStageElems + lane * 8) = *reinterpret_cast<const uint4*>(h);
-  if (lane == 0) out.scale[row * nst + st] = inv;
+  for (int i = 0; i < 4; ++i) {
+    h[i] = __floats2half2_rn(v[i] * f, v[i + 4] * f);
+    const float2 r = __half22float2(h[i]);
+    sum += r.x + r.y;
+  }
+  for (int o = group / 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);  // lanes of one group
+  uint8_t* rec = out.rec + at * kRecord;
+  *reinterpret_cast<uint4*>(rec + lane * 16) = *reinterpret_cast<const uint4*>(h);
+  float* tail = reinterpret_cast<float*>(rec + kStageElems * 2);
+  if (lane == 0) tail[0] = inv;
+  if (lane % (group / 8) == 0) tail[4 + lane / (group / 8)] = sum;
 }
 
-// Rows of x [rows, K] into tokens, a warp per run (runs first, first + step,
-// ...). vec: rows of a multiple of 8 elements on a 16-byte base.
+// A lane's eight elements of a row at k, zero past K. vec: rows of a multiple
+// of 8 elements on a 16-byte base.
 template <class T>
-__device__ __forceinline__ void write_tokens(const T* __restrict__ x, int rows, int K, bool vec, const Tokens& out,
+__device__ __forceinline__ void load_run(const T* __restrict__ src, int k, int K, bool vec, float (&v)[8]) {
+  if (vec && k < K) {
+    uint4 raw[sizeof(T) / 2];
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[i] = __ldg(reinterpret_cast<const uint4*>(src + k) + i);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = to_f(reinterpret_cast<const T*>(raw)[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = k + i < K ? to_f(src[k + i]) : 0.f;
+  }
+}
+
+// Rows of x [rows, K] into tokens, a warp per run (runs first, first + step, ...).
+template <class T>
+__device__ __forceinline__ void write_tokens(const T* __restrict__ x, int rows, int K, int group, bool vec, const Tokens& out,
                                              long long first, long long step) {
   const int lane = threadIdx.x & 31, nst = stages(K);
   for (long long u = first; u < (long long)rows * nst; u += step) {
     const int row = (int)(u / nst), st = (int)(u - (long long)row * nst);
-    const T* src = x + (size_t)row * K;
-    const int k = st * kStageElems + lane * 8;
     float v[8];
-    if (vec && k < K) {
-      uint4 raw[sizeof(T) / 2];
-#pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i) raw[i] = __ldg(reinterpret_cast<const uint4*>(src + k) + i);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = to_f(reinterpret_cast<const T*>(raw)[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = k + i < K ? to_f(src[k + i]) : 0.f;
-    }
-    write_run<!std::is_same<T, __half>::value>(out, row, st, nst, v);
+    load_run(x + (size_t)row * K, st * kStageElems + lane * 8, K, vec, v);
+    write_run<!std::is_same<T, __half>::value>(out, u, group, v);
   }
 }
 
 template <class T>
 __global__ void __launch_bounds__(256)
-    tokens_kernel(const T* __restrict__ x, int rows, int K, bool vec, Tokens out) {
+    tokens_kernel(const T* __restrict__ x, int rows, int K, int group, bool vec, Tokens out) {
   griddep_launch();
   griddep_wait();
-  write_tokens(x, rows, K, vec, out, ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5,
+  write_tokens(x, rows, K, group, vec, out, ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5,
                ((long long)gridDim.x * blockDim.x) >> 5);
 }
 
@@ -233,6 +247,8 @@ struct Params {
   int K, N;                  // N: weight rows (of an expert; of one matrix)
   int feature_tiles;         // tiles along N
   Tokens x;
+  const T* rows;             // the rows themselves, where the kernel makes the records (Shape::kMakes)
+  bool vec;                  // wide loads can read them
   int n_rows;                // token rows: M, or the packed rows
   int max_y;                 // token tiles there is room for
   const int* counts;         // rows per expert (null: dense)
@@ -245,13 +261,15 @@ struct Params {
 };
 
 // NT: 8 NT tokens a tile; FL: pieces per group (1, 2 or 4); kMin: minima;
-// STAGES: ring depth; OCC: CTAs per SM it is compiled for.
-template <int NT_, int FL_, bool kMin_, int STAGES_, int OCC_>
+// STAGES: ring depth; OCC: CTAs per SM it is compiled for. kMakes: the producer
+// warp makes the token records itself, from the rows (a dense product of up to
+// 8 tokens: one launch less, and the work is small enough to repeat per CTA).
+template <int NT_, int FL_, bool kMin_, int STAGES_, int OCC_, bool kMakes_ = false>
 struct Shape {
   static constexpr int NT = NT_, FL = FL_, STAGES = STAGES_, OCC = OCC_;
-  static constexpr bool kMin = kMin_;
+  static constexpr bool kMin = kMin_, kMakes = kMakes_;
   static constexpr int kTokens = 8 * NT;
-  static constexpr int kTokenBytes = kTokens * kTokenPitch;  // of a stage
+  static constexpr int kTokenBytes = kTokens * kRecord;  // of a stage
   static constexpr int kSmem = STAGES * (kStageBytes + kTokenBytes) + 1024;  // + alignment of the swizzled stages
 };
 
@@ -413,6 +431,7 @@ __global__ void __launch_bounds__(kThreads, S::OCC)
     const int ahead = min(S::STAGES, n_units);
     for (int i = 0; i < ahead; ++i) copy_codes(i);
     griddep_wait();
+    constexpr int kTail = S::kMin ? 1 + (kStagePieces / FL + 3) / 4 : 1;  // 16-byte units: scale, sums
     int slot = 0, my_row = token_row(p, cx.tl, lane);  // lane j: the row of the tile's token j
     uint32_t parity = 1;
     for (int i = 0; i < n_units; ++i) {
@@ -420,10 +439,28 @@ __global__ void __launch_bounds__(kThreads, S::OCC)
         if (!mbar_wait(&s_empty[slot], parity, &s_abort)) break;
         copy_codes(slot);
       }
+      if constexpr (S::kMakes) {
+        const Tokens rec{smem_x + slot * S::kTokenBytes};
+        for (int j = 0; j < cx.tl.m; ++j) {
+          float v[8];
+          load_run(p.rows + (size_t)(cx.tl.r0 + j) * p.K, cx.st * kStageElems + lane * 8, p.K, p.vec, v);
+          write_run<!std::is_same<T, __half>::value>(rec, j, FL * kPiece, v);
+        }
+        mbar_arrive(&s_full[slot]);
+        next(cx);
+        if (++slot == S::STAGES) {
+          slot = 0;
+          parity ^= 1;
+        }
+        continue;
+      }
       const uint32_t dst = smem_u32(smem_x + slot * S::kTokenBytes) + lane * 16;
-      const __half* src = p.x.x + (size_t)cx.st * kStageElems + lane * 8;
-      for (int j = 0; j < cx.tl.m; ++j)
-        cp_async16(dst + j * kTokenPitch, src + (size_t)__shfl_sync(0xffffffffu, my_row, j) * row_halfs(p.K));
+      const uint8_t* src = p.x.rec + (size_t)cx.st * kRecord + lane * 16;
+      for (int j = 0; j < cx.tl.m; ++j) {
+        const uint8_t* rec = src + (size_t)__shfl_sync(0xffffffffu, my_row, j) * (nst * kRecord);
+        cp_async16(dst + j * kRecord, rec);
+        if (lane < kTail) cp_async16(dst + j * kRecord + kStageElems * 2, rec + kStageElems * 2);
+      }
       cp_async_arrive(&s_full[slot]);
       const int y0 = cx.y;
       next(cx);
@@ -466,8 +503,6 @@ __global__ void __launch_bounds__(kThreads, S::OCC)
         srow[s][h] = (uint32_t)(e * p.N + min(r, p.N - 1)) * (uint32_t)G;
       }
   };
-  const float* xscale[NT][2];  // of the tokens of the columns this lane sums
-  float x_next[NT][2];
   T s_next[2][2][kSR], m_next[2][2][kSR];
   auto load_scales = [&](int stage) {
 #pragma unroll
@@ -486,22 +521,11 @@ __global__ void __launch_bounds__(kThreads, S::OCC)
   open_scales(tl.e, f);
   load_scales(st);
 
-  griddep_wait();  // the weights are older than this launch's predecessor, the tokens are its output
-  auto load_xscales = [&](int stage) {
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) x_next[n][c] = __ldg(xscale[n][c] + stage);
-  };
-  auto open_tokens = [&](const TokenTile& tk) {
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) xscale[n][c] = p.x.scale + (size_t)token_row(p, tk, n * 8 + t * 2 + c) * nst;
-  };
-  open_tokens(tl);
-  load_xscales(st);
-  const uint32_t xs = smem_u32(smem_x) + g * kTokenPitch + t * 16;  // this lane's run of 8 of token g
+  // the weights are older than this launch's predecessor, the tokens are its
+  // output; the consumers see them through the producer's copies
+  // this lane's run of 8 of token g, and the tail of the record of token 2 t
+  const uint32_t xs = smem_u32(smem_x) + g * kRecord + t * 16;
+  const uint32_t xt = smem_u32(smem_x) + t * 2 * kRecord + kStageElems * 2;
 
   float tot[2][NT][4] = {};
   int slot = 0;
@@ -515,7 +539,6 @@ __global__ void __launch_bounds__(kThreads, S::OCC)
       if (++next_f == p.feature_tiles) {
         next_f = 0;
         next_tl = open_tile<kMode, S::kTokens>(p, ++next_y, s_end, s_row);
-        open_tokens(next_tl);
       }
       open_scales(next_tl.e, next_f);
     }
@@ -529,20 +552,14 @@ __global__ void __launch_bounds__(kThreads, S::OCC)
           s_cur[s][h][i] = to_f(s_next[s][h][i]);
           if constexpr (S::kMin) m_cur[s][h][i] = to_f(m_next[s][h][i]);
         }
-    float x_cur[NT][2];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int c = 0; c < 2; ++c) x_cur[n][c] = x_next[n][c];
     load_scales(tile_end ? 0 : st + 1);
-    load_xscales(tile_end ? 0 : st + 1);
 
     // A wait that ran out has raised the status word; the sums are then of no
     // use, but every warp goes on to the end of its run.
     mbar_wait(&s_full[slot], parity, &s_abort);
     auto stage = [&](auto blocks) {
       constexpr int NB = decltype(blocks)::value;  // blocks of 8 tokens there are
-      float part[2][NB][4], xsum[NB][4];
+      float part[2][NB][4];
       uint32_t code[2][4];
 #pragma unroll
       for (int pp = 0; pp < kStagePieces; ++pp) {
@@ -552,62 +569,59 @@ __global__ void __launch_bounds__(kThreads, S::OCC)
         }
         uint4 xb[NB];
 #pragma unroll
-        for (int n = 0; n < NB; ++n) xb[n] = lds128(xs + slot * S::kTokenBytes + n * 8 * kTokenPitch + pp * 64);
+        for (int n = 0; n < NB; ++n) xb[n] = lds128(xs + slot * S::kTokenBytes + n * 8 * kRecord + pp * 64);
+        // the four products of a piece: both sets, then their second halves, so
+        // that the two that share accumulators are as far apart as they can be
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          const uint32_t wa = code[s][2 * (pp % 2)], wb = code[s][2 * (pp % 2) + 1];
-          uint32_t a[4];
-          code_pairs<S::kMin>(wa, 0, a[0], a[2]);
-          code_pairs<S::kMin>(wb, 0, a[1], a[3]);
-#pragma unroll
-          for (int n = 0; n < NB; ++n)
-            if (pp % FL == 0) mma16816_first(part[s][n], a, xb[n].x, xb[n].y);
-            else mma16816(part[s][n], a, xb[n].x, xb[n].y);
-          code_pairs<S::kMin>(wa, 1, a[0], a[2]);
-          code_pairs<S::kMin>(wb, 1, a[1], a[3]);
-#pragma unroll
-          for (int n = 0; n < NB; ++n) mma16816(part[s][n], a, xb[n].z, xb[n].w);
-        }
-        if constexpr (S::kMin) {
-          const uint32_t ones[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
-#pragma unroll
-          for (int n = 0; n < NB; ++n) {
-            if (pp % FL == 0) mma16816_first(xsum[n], ones, xb[n].x, xb[n].y);
-            else mma16816(xsum[n], ones, xb[n].x, xb[n].y);
-            mma16816(xsum[n], ones, xb[n].z, xb[n].w);
-          }
-        }
-        if ((pp + 1) % FL == 0) {
-          const int gi = pp / FL, from = (lane & ~3) + gi % 4;
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int s = 0; s < 2; ++s) {
-            float sv[2], mv[2];
+            const uint32_t wa = code[s][2 * (pp % 2)], wb = code[s][2 * (pp % 2) + 1];
+            uint32_t a[4];
+            code_pairs(wa, h, a[0], a[2]);
+            code_pairs(wb, h, a[1], a[3]);
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+              const uint32_t b0 = h ? xb[n].z : xb[n].x, b1 = h ? xb[n].w : xb[n].y;
+              if (pp % FL == 0 && h == 0) mma16816_first(part[s][n], a, b0, b1);
+              else mma16816(part[s][n], a, b0, b1);
+            }
+          }
+        if ((pp + 1) % FL == 0) {
+          const int gi = pp / FL, from = (lane & ~3) + gi % 4;
+          float sv[2][2], mv[2][2];
+#pragma unroll
+          for (int s = 0; s < 2; ++s)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              sv[h] = __shfl_sync(0xffffffffu, s_cur[s][h][gi / 4], from);
-              if constexpr (S::kMin) mv[h] = __shfl_sync(0xffffffffu, m_cur[s][h][gi / 4], from);
+              sv[s][h] = __shfl_sync(0xffffffffu, s_cur[s][h][gi / 4], from);
+              if constexpr (S::kMin)
+                mv[s][h] = fmaf(8.f, sv[s][h], __shfl_sync(0xffffffffu, m_cur[s][h][gi / 4], from));
             }
 #pragma unroll
-            for (int n = 0; n < NB; ++n)
+          for (int n = 0; n < NB; ++n)
 #pragma unroll
-              for (int c = 0; c < 4; ++c) {
-                float v = sv[c >> 1] * part[s][n][c];
-                if constexpr (S::kMin) v = fmaf(mv[c >> 1], xsum[n][c], v);
-                tot[s][n][c] = fmaf(x_cur[n][c & 1], v, tot[s][n][c]);
-              }
-          }
+            for (int c = 0; c < 2; ++c) {
+              const uint32_t tail = xt + slot * S::kTokenBytes + (n * 8 + c) * kRecord;
+              const float xscale = lds32(tail);
+              const float xsum = S::kMin ? lds32(tail + 16 + gi * 4) : 0.f;
+#pragma unroll
+              for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  float v = sv[s][h] * part[s][n][2 * h + c];
+                  if constexpr (S::kMin) v = fmaf(mv[s][h], xsum, v);
+                  tot[s][n][2 * h + c] = fmaf(xscale, v, tot[s][n][2 * h + c]);
+                }
+            }
         }
       }
     };
-    if constexpr (NT == 1) {
-      stage(std::integral_constant<int, 1>{});
-    } else {
-      const int nb = (tl.m + 7) / 8;
-      if (nb == 1) stage(std::integral_constant<int, 1>{});
-      else if (NT == 2 || nb == 2) stage(std::integral_constant<int, 2>{});
-      else if (nb == 3) stage(std::integral_constant<int, NT < 3 ? NT : 3>{});
-      else stage(std::integral_constant<int, NT>{});
-    }
+    const int nb = NT == 1 ? 1 : (tl.m + 7) / 8;
+    if (nb <= 1) stage(std::integral_constant<int, 1>{});
+    else if (NT == 2 || nb == 2) stage(std::integral_constant<int, NT < 2 ? NT : 2>{});
+    else if (NT == 3 || nb == 3) stage(std::integral_constant<int, NT < 3 ? NT : 3>{});
+    else stage(std::integral_constant<int, NT>{});
     __syncwarp();
     if (lane == 0) mbar_arrive(&s_empty[slot]);
     if (++slot == S::STAGES) {
@@ -721,7 +735,7 @@ __global__ void __launch_bounds__(kRows) finish_kernel(const __grid_constant__ P
 // The activations of a gate/up product straight into the tokens of the down
 // projection: a warp per packed row and run of 256 features (two tiles).
 template <int TOK, class T>
-__global__ void __launch_bounds__(256) act_tokens_kernel(const __grid_constant__ Params<T> p, int grid, Tokens act) {
+__global__ void __launch_bounds__(256) act_tokens_kernel(const __grid_constant__ Params<T> p, int grid, int group, Tokens act) {
   extern __shared__ int s_index[];
   __shared__ int s_y;
   griddep_launch();
@@ -740,14 +754,14 @@ __global__ void __launch_bounds__(256) act_tokens_kernel(const __grid_constant__
       sum_parts<TOK, 8, 2>(run, p.parts, y * p.feature_tiles + f, tok, n % (kRows / 2), v);
 #pragma unroll
     for (int i = 0; i < 8; ++i) a[i] = n + i < p.N ? swiglu(v[0][i], v[1][i]) : 0.f;
-    write_run<true>(act, tl.r0 + tok, st, nst, a);
+    write_run<true>(act, (size_t)(tl.r0 + tok) * nst + st, group, a);
   }
 }
 
 // out[t] = sum_j w[t, j] y[row of slot (t, j)] from the parts of the down
 // projection, fp32 in j order, rounded once. A CTA per token and 256 features.
 template <int TOK, class T>
-__global__ void __launch_bounds__(kRows)
+__global__ void __launch_bounds__(kRows, 4)
     combine_parts_kernel(const __grid_constant__ Params<T> p, int grid, const int* __restrict__ slot_rows,
                          const int* __restrict__ ids, const float* __restrict__ weights, int tokens, int topk,
                          T* __restrict__ out) {
@@ -796,8 +810,16 @@ __global__ void __launch_bounds__(kRows)
         for (int i = 0; i < kB; ++i) {
           if (j + i >= kn || s_parts[j + i] == 0) continue;
           const float* q = p.parts + s_at[j + i] + threadIdx.x;
-#pragma unroll 8
-          for (int c = 1; c < s_parts[j + i]; ++c) v[i] += __ldg(q + (size_t)c * (kRows * TOK));
+          const int np = s_parts[j + i];
+          for (int c = 1; c < np; c += kB) {
+            float b[kB];
+#pragma unroll
+            for (int u = 0; u < kB; ++u)
+              if (c + u < np) b[u] = __ldg(q + (size_t)(c + u) * (kRows * TOK));
+#pragma unroll
+            for (int u = 0; u < kB; ++u)
+              if (c + u < np) v[i] += b[u];
+          }
           acc = fmaf(s_w[j + i], v[i], acc);
         }
       }
@@ -832,9 +854,9 @@ int launch(const char* what, void (*kernel)(P...), dim3 grid, int threads, size_
 inline int pick_nt(long long rows, int experts) {
   const double used = (double)std::max<long long>(1, std::min<long long>(experts, rows));
   const double mean = rows / used, want = experts > 1 ? mean + 2.0 * std::sqrt(mean) : mean;
-  return want <= 8 ? 1 : want <= 16 ? 2 : 4;
+  return want <= 8 ? 1 : want <= 16 ? 2 : want <= 24 ? 3 : 4;
 }
-inline int occupancy(int nt) { return nt <= 2 ? 2 : 1; }
+inline int occupancy(int nt) { return nt <= 3 ? 2 : 1; }
 
 inline int max_token_tiles(long long rows, int experts, int nt) {
   const int tok = 8 * nt;
@@ -857,13 +879,14 @@ int launch_product_shape(const CUtensorMap& a, const CUtensorMap& b, const Param
     attr_done[dev] = true;
   }
   return launch("w4 product launch", w4_kernel<T, S, kMode>, dim3(grid), kThreads,
-                S::kSmem + (kMode == kDense ? 0 : (2 * p.E + 1) * sizeof(int)), stream, false, a, b, p);
+                S::kSmem + (kMode == kDense ? 0 : (2 * p.E + 1) * sizeof(int)), stream, S::kMakes, a, b, p);
 }
 
 template <class T, Mode kMode, int FL, bool kMin>
 int launch_product_nt(int nt, const CUtensorMap& a, const CUtensorMap& b, const Params<T>& p, int grid, cudaStream_t stream) {
-  if (nt == 1) return launch_product_shape<T, Shape<1, FL, kMin, 2, 2>, kMode>(a, b, p, grid, stream);
+  if (nt == 1) return launch_product_shape<T, Shape<1, FL, kMin, 2, 2, kMode == kDense>, kMode>(a, b, p, grid, stream);
   if (nt == 2) return launch_product_shape<T, Shape<2, FL, kMin, 2, 2>, kMode>(a, b, p, grid, stream);
+  if (nt == 3) return launch_product_shape<T, Shape<3, FL, kMin, 2, 2>, kMode>(a, b, p, grid, stream);
   return launch_product_shape<T, Shape<4, FL, kMin, 4, 1>, kMode>(a, b, p, grid, stream);
 }
 
@@ -886,11 +909,11 @@ int launch_product(int nt, int group, const CUtensorMap& a, const CUtensorMap& b
 }
 
 template <class T>
-int launch_tokens(const T* x, int rows, int K, const Tokens& out, cudaStream_t stream, bool after) {
+int launch_tokens(const T* x, int rows, int K, int group, const Tokens& out, cudaStream_t stream) {
   const long long warps = (long long)rows * stages(K);
   const bool vec = K % 8 == 0 && aligned16(x);
   return launch("w4 tokens launch", tokens_kernel<T>, dim3((unsigned)std::min<long long>((warps + 7) / 8, 148 * 16)), 256, 0,
-                stream, after, x, rows, K, vec, out);
+                stream, true, x, rows, K, group, vec, out);
 }
 
 // Codes [rows, K] as the TMA sees them: boxes of `box` rows x 128 bytes.

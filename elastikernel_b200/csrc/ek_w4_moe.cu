@@ -29,7 +29,7 @@ using bf16 = __nv_bfloat16;
 // projection writes its sums after the gate/up's have been read).
 struct MoeLayout {
   int nt, grid, max_y;
-  size_t x, xs, a, as, parts, bytes;
+  size_t x, a, parts, bytes;
 };
 MoeLayout moe_layout(long long x_rows, int rows, int E, int H, int I, int sms) {
   MoeLayout l;
@@ -40,9 +40,7 @@ MoeLayout moe_layout(long long x_rows, int rows, int E, int H, int I, int sms) {
   const long long ft1 = (I + kRows / 2 - 1) / (kRows / 2), ft2 = (H + kRows - 1) / kRows;
   const Layout x = layout(x_rows, H, l.max_y * ft1, l.grid, tok), a = layout(rows, I, l.max_y * ft2, l.grid, tok);
   l.x = 0;
-  l.xs = x.scales;
   l.a = x.parts;
-  l.as = l.a + a.scales;
   l.parts = l.a + a.parts;
   l.bytes = l.parts + std::max(x.bytes - x.parts, a.bytes - a.parts);
   return l;
@@ -56,13 +54,13 @@ struct Order {
   float* weights;
 };
 __global__ void __launch_bounds__(kOrderThreads)
-    front_kernel(const float* __restrict__ logits, const bf16* __restrict__ x, int T, int k, int E, int H, bool vec,
-                 Order o, Tokens tokens) {
+    front_kernel(const float* __restrict__ logits, const bf16* __restrict__ x, int T, int k, int E, int H,
+                 int group, bool vec, Order o, Tokens tokens) {
   extern __shared__ int sm[];
   griddep_launch();  // the next launch waits for the whole of this one
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = T * k;
   if (blockIdx.x > 0) {
-    write_tokens(x, T, H, vec, tokens, (long long)(blockIdx.x - 1) * (kOrderThreads / 32) + warp,
+    write_tokens(x, T, H, group, vec, tokens, (long long)(blockIdx.x - 1) * (kOrderThreads / 32) + warp,
                  (long long)(gridDim.x - 1) * (kOrderThreads / 32));
     return;
   }
@@ -98,8 +96,8 @@ struct Moe {
   MoeLayout l;
   cudaStream_t stream;
   size_t index_bytes() const { return (2 * E + 1) * sizeof(int); }
-  Tokens x() const { return {reinterpret_cast<__half*>(ws + l.x), reinterpret_cast<float*>(ws + l.xs)}; }
-  Tokens act() const { return {reinterpret_cast<__half*>(ws + l.a), reinterpret_cast<float*>(ws + l.as)}; }
+  Tokens x() const { return {ws + l.x}; }
+  Tokens act() const { return {ws + l.a}; }
 
   Params<bf16> params(int K, int N, int features, const Tokens& tokens) const {
     Params<bf16> p = {};
@@ -130,7 +128,7 @@ struct Moe {
     CUtensorMap m1, m3;
     int rc = codes_map(&m1, w1.codes, (long long)E * I, H, kRows / 2);
     if (!rc) rc = codes_map(&m3, w3.codes, (long long)E * I, H, kRows / 2);
-    if (!rc && xin) rc = launch_tokens(xin, x_rows, H, p.x, stream, true);
+    if (!rc && xin) rc = launch_tokens(xin, x_rows, H, group, p.x, stream);
     if (!rc) rc = launch_product<bf16, kGateUp>(l.nt, group, m1, m3, p, l.grid, stream);
     return rc;
   }
@@ -150,25 +148,29 @@ struct Moe {
   }
   template <Mode kMode, class O>
   int finish(const Params<bf16>& p, O* out) const {
-    return l.nt == 1 ? finish_tok<kMode, 8>(p, out) : l.nt == 2 ? finish_tok<kMode, 16>(p, out) : finish_tok<kMode, 32>(p, out);
+    return l.nt == 1   ? finish_tok<kMode, 8>(p, out)
+           : l.nt == 2 ? finish_tok<kMode, 16>(p, out)
+           : l.nt == 3 ? finish_tok<kMode, 24>(p, out)
+                       : finish_tok<kMode, 32>(p, out);
   }
   // gate/up, down and combine, from an order of the slots
   int layer(const bf16* xin, const Order& o, int T, int topk, const Matrix& w1, const Matrix& w3, const Matrix& w2,
             bf16* out) const {
     Params<bf16> p;
     int rc = gate_up(xin, T, o.sorted_slots, topk, w1, w3, &p);
-    if (!rc) rc = l.nt == 1 ? act_tokens<8>(p) : l.nt == 2 ? act_tokens<16>(p) : act_tokens<32>(p);
+    if (!rc) rc = l.nt == 1 ? act_tokens<8>(p) : l.nt == 2 ? act_tokens<16>(p) : l.nt == 3 ? act_tokens<24>(p) : act_tokens<32>(p);
     if (!rc) rc = down(w2, &p);
     if (rc) return rc;
     return l.nt == 1   ? combine<8>(p, o.slot_rows, o.ids, o.weights, T, topk, out)
            : l.nt == 2 ? combine<16>(p, o.slot_rows, o.ids, o.weights, T, topk, out)
+           : l.nt == 3 ? combine<24>(p, o.slot_rows, o.ids, o.weights, T, topk, out)
                        : combine<32>(p, o.slot_rows, o.ids, o.weights, T, topk, out);
   }
   template <int TOK>
   int act_tokens(const Params<bf16>& p) const {
     const long long warps = (long long)l.max_y * TOK * stages(I);
     return launch("w4 act launch", act_tokens_kernel<TOK, bf16>, dim3((unsigned)std::min<long long>((warps + 7) / 8, 148 * 8)),
-                  256, index_bytes(), stream, false, p, l.grid, act());
+                  256, index_bytes(), stream, false, p, l.grid, group, act());
   }
   template <int TOK>
   int combine(const Params<bf16>& p, const int* slot_rows, const int* ids, const float* weights, int T, int topk,
@@ -263,8 +265,8 @@ int ek_moe_down_w4(const void* act, int act_dtype, const void* w2_codes, const v
   Moe m;
   rc = open_moe("down_w4", &m, 0, expert_counts, rows, E, H, I, group, num_sms, workspace, ws_bytes, stream);
   if (!rc)
-    rc = act_dtype == EK_DTYPE_BF16 ? launch_tokens(static_cast<const bf16*>(act), rows, I, m.act(), m.stream, true)
-                                    : launch_tokens(static_cast<const float*>(act), rows, I, m.act(), m.stream, true);
+    rc = act_dtype == EK_DTYPE_BF16 ? launch_tokens(static_cast<const bf16*>(act), rows, I, group, m.act(), m.stream)
+                                    : launch_tokens(static_cast<const float*>(act), rows, I, group, m.act(), m.stream);
   Params<bf16> p;
   if (!rc) rc = m.down({w2_codes, w2_scales, w2_mins}, &p);
   if (rc) return rc;
@@ -343,7 +345,7 @@ int ek_fused_moe_w4(const void* x, const float* logits, int T, int topk, const v
     const int warps = T * stages(H), per = kOrderThreads / 32;
     const int grid = 1 + std::min((warps + per - 1) / per, 147);
     rc = launch("w4 front launch", front_kernel, dim3(grid), kOrderThreads, order_smem_ints(n, E) * sizeof(int), m.stream,
-                true, logits, xin, T, topk, E, H, H % 8 == 0 && aligned16(xin), o, m.x());
+                true, logits, xin, T, topk, E, H, group, H % 8 == 0 && aligned16(xin), o, m.x());
     xin = nullptr;
   } else {
     rc = ek_moe_route(logits, T, E, topk, o.ids, o.weights, stream);
