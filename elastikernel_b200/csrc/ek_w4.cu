@@ -12,7 +12,7 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "ek_w4_kernel.cuh"
+#include "ek_w4_launch.cuh"
 
 namespace ek {
 namespace {

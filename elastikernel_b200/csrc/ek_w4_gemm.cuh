@@ -1,6 +1,6 @@
 // The dense product of one element type (a translation unit each).
 #pragma once
-#include "ek_w4_kernel.cuh"
+#include "ek_w4_launch.cuh"
 
 namespace ek {
 namespace w4 {
@@ -15,7 +15,7 @@ struct GemmArgs {
 
 inline Layout gemm_layout(int M, int N, int K, int sms, int* nt, int* grid) {
   *nt = pick_nt(M, 1);
-  *grid = sms * occupancy(*nt);
+  *grid = sms * kCtasPerSm;
   const long long tiles = (long long)max_token_tiles(M, 0, *nt) * ((N + kRows - 1) / kRows);
   return layout(M, K, tiles, *grid, 8 * *nt);
 }
@@ -47,9 +47,7 @@ int gemm(const GemmArgs& a) {
   const dim3 g(p.feature_tiles, std::min(p.max_y * 8 * nt, 4096));
   T* out = static_cast<T*>(a.C);
   if (nt == 1) return launch("w4 sums launch", finish_kernel<kDense, 8, T, T>, g, kRows, 0, a.stream, false, p, grid, out);
-  if (nt == 2) return launch("w4 sums launch", finish_kernel<kDense, 16, T, T>, g, kRows, 0, a.stream, false, p, grid, out);
-  if (nt == 3) return launch("w4 sums launch", finish_kernel<kDense, 24, T, T>, g, kRows, 0, a.stream, false, p, grid, out);
-  return launch("w4 sums launch", finish_kernel<kDense, 32, T, T>, g, kRows, 0, a.stream, false, p, grid, out);
+  return launch("w4 sums launch", finish_kernel<kDense, 16, T, T>, g, kRows, 0, a.stream, false, p, grid, out);
 }
 
 }  // namespace w4

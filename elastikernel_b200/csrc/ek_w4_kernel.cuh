@@ -55,6 +55,7 @@ constexpr int kWarps = 8;                    // consumer warps
 constexpr int kThreads = 32 * (kWarps + 1);  // and the producer
 constexpr int kRows = 32 * kWarps;           // weight rows per tile (gate/up: half of each matrix)
 constexpr int kStageBytes = kRows * 128;
+constexpr int kStages = 2;  // ring depth (two CTAs per SM; more stages of one CTA were no faster)
 // Bytes of a token's record of a stage: 256 halfs, then its scale and the sums
 // of its groups (fp32; at most 8). 64 more than 512 also keeps the reads of
 // eight tokens free of bank conflicts.
@@ -74,6 +75,20 @@ template <>
 __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
 template <>
 __device__ __forceinline__ float from_f<float>(float v) { return v; }
+
+__device__ __forceinline__ uint32_t pack2(__half a, __half b) {
+  const __half2 r = __halves2half2(a, b);
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t pack2(__nv_bfloat16 a, __nv_bfloat16 b) {
+  const __nv_bfloat162 r = __halves2bfloat162(a, b);
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+template <class T>
+__device__ __forceinline__ float2 unpack2(uint32_t v) {
+  if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&v));
+  else return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
+}
 
 // (w & mask) | 0x6400 6400: the masked nibbles over the exponent of 1024.
 __device__ __forceinline__ uint32_t nibbles(uint32_t w, uint32_t mask) {
@@ -107,12 +122,6 @@ __device__ __forceinline__ void mma16816_first(float (&c)[4], const uint32_t (&a
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-// Arrive on `bar` when this thread's cp.async so far have landed (one of the
-// barrier's expected arrivals).
-__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
-  asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   uint4 v;
@@ -260,17 +269,17 @@ struct Params {
   bool wait_first;           // the predecessor makes the counts and the order too
 };
 
-// NT: 8 NT tokens a tile; FL: pieces per group (1, 2 or 4); kMin: minima;
-// STAGES: ring depth; OCC: CTAs per SM it is compiled for. kMakes: the producer
-// warp makes the token records itself, from the rows (a dense product of up to
-// 8 tokens: one launch less, and the work is small enough to repeat per CTA).
-template <int NT_, int FL_, bool kMin_, int STAGES_, int OCC_, bool kMakes_ = false>
+// NT: 8 NT tokens a tile; FL: pieces per group (1, 2 or 4); kMin: minima.
+// kMakes: the producer warp makes the token records itself, from the rows (a
+// dense product of up to 8 tokens: one launch less, and the work is small enough
+// to repeat per CTA).
+template <int NT_, int FL_, bool kMin_, bool kMakes_>
 struct Shape {
-  static constexpr int NT = NT_, FL = FL_, STAGES = STAGES_, OCC = OCC_;
+  static constexpr int NT = NT_, FL = FL_;
   static constexpr bool kMin = kMin_, kMakes = kMakes_;
   static constexpr int kTokens = 8 * NT;
   static constexpr int kTokenBytes = kTokens * kRecord;  // of a stage
-  static constexpr int kSmem = STAGES * (kStageBytes + kTokenBytes) + 1024;  // + alignment of the swizzled stages
+  static constexpr int kSmem = kStages * (kStageBytes + kTokenBytes) + 1024;  // + alignment of the swizzled stages
 };
 
 // A token tile: rows [r0, r0 + m) of expert e.
@@ -353,17 +362,17 @@ struct Runs {
 };
 
 template <class T, class S, Mode kMode>
-__global__ void __launch_bounds__(kThreads, S::OCC)
+__global__ void __launch_bounds__(kThreads, 2)
     w4_kernel(const __grid_constant__ CUtensorMap map0, const __grid_constant__ CUtensorMap map1,
               const __grid_constant__ Params<T> p) {
   constexpr int NT = S::NT, FL = S::FL;
   constexpr int kFeatures = kMode == kGateUp ? kRows / 2 : kRows;  // output features per tile
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t s_full[S::STAGES], s_empty[S::STAGES];
+  __shared__ uint64_t s_full[kStages], s_empty[kStages];
   __shared__ int s_abort, s_y;
   uint8_t* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-  uint8_t* smem_x = smem + S::STAGES * kStageBytes;
-  int* s_end = reinterpret_cast<int*>(smem_x + S::STAGES * S::kTokenBytes);
+  uint8_t* smem_x = smem + kStages * kStageBytes;
+  int* s_end = reinterpret_cast<int*>(smem_x + kStages * S::kTokenBytes);
   int* s_row = s_end + p.E;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 
@@ -380,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, S::OCC)
       s_abort = 0;
     }
   } else if (warp == kWarps && lane == 0) {
-    for (int i = 0; i < S::STAGES; ++i) {
+    for (int i = 0; i < kStages; ++i) {
       mbar_init(&s_full[i], 1 + 32);
       mbar_init(&s_empty[i], kWarps);
     }
@@ -428,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, S::OCC)
       }
       next(cw);
     };
-    const int ahead = min(S::STAGES, n_units);
+    const int ahead = min(kStages, n_units);
     for (int i = 0; i < ahead; ++i) copy_codes(i);
     griddep_wait();
     constexpr int kTail = S::kMin ? 1 + (kStagePieces / FL + 3) / 4 : 1;  // 16-byte units: scale, sums
@@ -448,7 +457,7 @@ __global__ void __launch_bounds__(kThreads, S::OCC)
         }
         mbar_arrive(&s_full[slot]);
         next(cx);
-        if (++slot == S::STAGES) {
+        if (++slot == kStages) {
           slot = 0;
           parity ^= 1;
         }
@@ -461,16 +470,17 @@ __global__ void __launch_bounds__(kThreads, S::OCC)
         cp_async16(dst + j * kRecord, rec);
         if (lane < kTail) cp_async16(dst + j * kRecord + kStageElems * 2, rec + kStageElems * 2);
       }
-      cp_async_arrive(&s_full[slot]);
+      cp_async_mbar_arrive(&s_full[slot]);
       const int y0 = cx.y;
       next(cx);
       if (cx.y != y0) my_row = token_row(p, cx.tl, lane);
-      if (++slot == S::STAGES) {
+      if (++slot == kStages) {
         slot = 0;
         parity ^= 1;
       }
     }
-    cp_async_wait_all();
+    cp_async_commit();
+    cp_async_wait<0>();
     return;
   }
 
@@ -503,19 +513,17 @@ __global__ void __launch_bounds__(kThreads, S::OCC)
         srow[s][h] = (uint32_t)(e * p.N + min(r, p.N - 1)) * (uint32_t)G;
       }
   };
-  T s_next[2][2][kSR], m_next[2][2][kSR];
+  uint32_t s_next[2][kSR], m_next[2][kSR];  // of rows g (low half) and g + 8
   auto load_scales = [&](int stage) {
 #pragma unroll
     for (int i = 0; i < kSR; ++i) {
       const uint32_t gi = min(stage * kSG + (t + 4 * i) % kSG, G - 1);
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const Scales<T>& w = p.w[kMode == kGateUp ? s : 0];
-          s_next[s][h][i] = __ldg(w.s + (srow[s][h] + gi));
-          if constexpr (S::kMin) m_next[s][h][i] = __ldg(w.m + (srow[s][h] + gi));
-        }
+      for (int s = 0; s < 2; ++s) {
+        const Scales<T>& w = p.w[kMode == kGateUp ? s : 0];
+        s_next[s][i] = pack2(__ldg(w.s + (srow[s][0] + gi)), __ldg(w.s + (srow[s][1] + gi)));
+        if constexpr (S::kMin) m_next[s][i] = pack2(__ldg(w.m + (srow[s][0] + gi)), __ldg(w.m + (srow[s][1] + gi)));
+      }
     }
   };
   open_scales(tl.e, f);
@@ -542,16 +550,14 @@ __global__ void __launch_bounds__(kThreads, S::OCC)
       }
       open_scales(next_tl.e, next_f);
     }
-    float s_cur[2][2][kSR], m_cur[2][2][kSR];
+    uint32_t s_cur[2][kSR], m_cur[2][kSR];
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < kSR; ++i) {
-          s_cur[s][h][i] = to_f(s_next[s][h][i]);
-          if constexpr (S::kMin) m_cur[s][h][i] = to_f(m_next[s][h][i]);
-        }
+      for (int i = 0; i < kSR; ++i) {
+        s_cur[s][i] = s_next[s][i];
+        if constexpr (S::kMin) m_cur[s][i] = m_next[s][i];
+      }
     load_scales(tile_end ? 0 : st + 1);
 
     // A wait that ran out has raised the status word; the sums are then of no
@@ -589,42 +595,38 @@ __global__ void __launch_bounds__(kThreads, S::OCC)
           }
         if ((pp + 1) % FL == 0) {
           const int gi = pp / FL, from = (lane & ~3) + gi % 4;
-          float sv[2][2], mv[2][2];
 #pragma unroll
-          for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              sv[s][h] = __shfl_sync(0xffffffffu, s_cur[s][h][gi / 4], from);
-              if constexpr (S::kMin)
-                mv[s][h] = fmaf(8.f, sv[s][h], __shfl_sync(0xffffffffu, m_cur[s][h][gi / 4], from));
+          for (int s = 0; s < 2; ++s) {
+            const float2 sv = unpack2<T>(__shfl_sync(0xffffffffu, s_cur[s][gi / 4], from));
+            float2 mv = sv;
+            if constexpr (S::kMin) {
+              mv = unpack2<T>(__shfl_sync(0xffffffffu, m_cur[s][gi / 4], from));
+              mv = make_float2(fmaf(8.f, sv.x, mv.x), fmaf(8.f, sv.y, mv.y));
             }
 #pragma unroll
-          for (int n = 0; n < NB; ++n)
+            for (int n = 0; n < NB; ++n)
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              const uint32_t tail = xt + slot * S::kTokenBytes + (n * 8 + c) * kRecord;
-              const float xscale = lds32(tail);
-              const float xsum = S::kMin ? lds32(tail + 16 + gi * 4) : 0.f;
-#pragma unroll
-              for (int s = 0; s < 2; ++s)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                  float v = sv[s][h] * part[s][n][2 * h + c];
-                  if constexpr (S::kMin) v = fmaf(mv[s][h], xsum, v);
-                  tot[s][n][2 * h + c] = fmaf(xscale, v, tot[s][n][2 * h + c]);
+              for (int c = 0; c < 2; ++c) {
+                const uint32_t tail = xt + slot * S::kTokenBytes + (n * 8 + c) * kRecord;
+                const float xscale = lds32(tail);
+                float a = sv.x * part[s][n][c], b = sv.y * part[s][n][2 + c];
+                if constexpr (S::kMin) {
+                  const float xsum = lds32(tail + 16 + gi * 4);
+                  a = fmaf(mv.x, xsum, a);
+                  b = fmaf(mv.y, xsum, b);
                 }
-            }
+                tot[s][n][c] = fmaf(xscale, a, tot[s][n][c]);
+                tot[s][n][2 + c] = fmaf(xscale, b, tot[s][n][2 + c]);
+              }
+          }
         }
       }
     };
-    const int nb = NT == 1 ? 1 : (tl.m + 7) / 8;
-    if (nb <= 1) stage(std::integral_constant<int, 1>{});
-    else if (NT == 2 || nb == 2) stage(std::integral_constant<int, NT < 2 ? NT : 2>{});
-    else if (NT == 3 || nb == 3) stage(std::integral_constant<int, NT < 3 ? NT : 3>{});
+    if (NT == 1 || tl.m <= 8) stage(std::integral_constant<int, 1>{});
     else stage(std::integral_constant<int, NT>{});
     __syncwarp();
     if (lane == 0) mbar_arrive(&s_empty[slot]);
-    if (++slot == S::STAGES) {
+    if (++slot == kStages) {
       slot = 0;
       parity ^= 1;
     }
@@ -826,110 +828,6 @@ __global__ void __launch_bounds__(kRows, 4)
     }
     if (n < p.N) out[(size_t)t * p.N + n] = from_f<T>(acc);
   }
-}
-
-// ------------------------------------------------------------------ launches
-// One launch that may begin before its predecessor on the stream has ended (the
-// kernels above wait for it themselves), or, with after = true, not.
-template <class... P, class... A>
-int launch(const char* what, void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t stream, bool after,
-           A... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = after ? 0 : 1;
-  return check_cuda(cudaLaunchKernelEx(&cfg, kernel, args...), what);
-}
-
-// Tokens of a tile for `rows` token rows over `experts` weight matrices: blocks
-// of 8 up to 32, to hold the mean and two standard deviations of an even
-// spread, so that few experts need a second tile (which streams the codes
-// again). The kernel computes only the blocks a tile has.
-inline int pick_nt(long long rows, int experts) {
-  const double used = (double)std::max<long long>(1, std::min<long long>(experts, rows));
-  const double mean = rows / used, want = experts > 1 ? mean + 2.0 * std::sqrt(mean) : mean;
-  return want <= 8 ? 1 : want <= 16 ? 2 : want <= 24 ? 3 : 4;
-}
-inline int occupancy(int nt) { return nt <= 3 ? 2 : 1; }
-
-inline int max_token_tiles(long long rows, int experts, int nt) {
-  const int tok = 8 * nt;
-  if (experts <= 0) return (int)((rows + tok - 1) / tok);
-  return (int)std::min<long long>(rows, std::min<long long>(experts, rows) + rows / tok);
-}
-
-template <class T, class S, Mode kMode>
-int launch_product_shape(const CUtensorMap& a, const CUtensorMap& b, const Params<T>& p, int grid, cudaStream_t stream) {
-  static bool attr_done[64] = {false};
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64) return set_error(EK_ERR_CUDA, "device index out of range");
-  constexpr int kIndexMax = (2 * 1024 + 1) * (int)sizeof(int);
-  if (!attr_done[dev]) {
-    const int rc = check_cuda(cudaFuncSetAttribute(w4_kernel<T, S, kMode>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                   S::kSmem + (kMode == kDense ? 0 : kIndexMax)),
-                              "cudaFuncSetAttribute(w4)");
-    if (rc) return rc;
-    attr_done[dev] = true;
-  }
-  return launch("w4 product launch", w4_kernel<T, S, kMode>, dim3(grid), kThreads,
-                S::kSmem + (kMode == kDense ? 0 : (2 * p.E + 1) * sizeof(int)), stream, S::kMakes, a, b, p);
-}
-
-template <class T, Mode kMode, int FL, bool kMin>
-int launch_product_nt(int nt, const CUtensorMap& a, const CUtensorMap& b, const Params<T>& p, int grid, cudaStream_t stream) {
-  if (nt == 1) return launch_product_shape<T, Shape<1, FL, kMin, 2, 2, kMode == kDense>, kMode>(a, b, p, grid, stream);
-  if (nt == 2) return launch_product_shape<T, Shape<2, FL, kMin, 2, 2>, kMode>(a, b, p, grid, stream);
-  if (nt == 3) return launch_product_shape<T, Shape<3, FL, kMin, 2, 2>, kMode>(a, b, p, grid, stream);
-  return launch_product_shape<T, Shape<4, FL, kMin, 4, 1>, kMode>(a, b, p, grid, stream);
-}
-
-// The product over the tokens p.x, its sums left in p.parts.
-template <class T, Mode kMode>
-int launch_product(int nt, int group, const CUtensorMap& a, const CUtensorMap& b, const Params<T>& p, int grid,
-                   cudaStream_t stream) {
-  const bool mins = p.w[0].m != nullptr;
-  switch (group) {
-    case 32:
-      return mins ? launch_product_nt<T, kMode, 1, true>(nt, a, b, p, grid, stream)
-                  : launch_product_nt<T, kMode, 1, false>(nt, a, b, p, grid, stream);
-    case 64:
-      return mins ? launch_product_nt<T, kMode, 2, true>(nt, a, b, p, grid, stream)
-                  : launch_product_nt<T, kMode, 2, false>(nt, a, b, p, grid, stream);
-    default:
-      return mins ? launch_product_nt<T, kMode, 4, true>(nt, a, b, p, grid, stream)
-                  : launch_product_nt<T, kMode, 4, false>(nt, a, b, p, grid, stream);
-  }
-}
-
-template <class T>
-int launch_tokens(const T* x, int rows, int K, int group, const Tokens& out, cudaStream_t stream) {
-  const long long warps = (long long)rows * stages(K);
-  const bool vec = K % 8 == 0 && aligned16(x);
-  return launch("w4 tokens launch", tokens_kernel<T>, dim3((unsigned)std::min<long long>((warps + 7) / 8, 148 * 16)), 256, 0,
-                stream, true, x, rows, K, group, vec, out);
-}
-
-// Codes [rows, K] as the TMA sees them: boxes of `box` rows x 128 bytes.
-inline int codes_map(CUtensorMap* m, const void* codes, long long rows, int K, int box) {
-  const uint64_t pitch = (uint64_t)pieces(K) * 16;
-  return make_tmap_2d(m, codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, pitch, (uint64_t)rows, pitch, 128, box);
-}
-
-inline int check_w4(const char* what, const void* codes, const void* scales, const void* mins, int K, int group) {
-  if (K < 1 || (group != 32 && group != 64 && group != 128))
-    return set_error(EK_ERR_INVALID, "%s: need K >= 1 and a group of 32, 64 or 128 (K=%d group=%d)", what, K, group);
-  if (!codes || !scales) return set_error(EK_ERR_INVALID, "%s: null pointer", what);
-  if (!aligned16(codes)) return set_error(EK_ERR_INVALID, "%s: codes must be 16-byte aligned", what);
-  if ((reinterpret_cast<uintptr_t>(scales) | reinterpret_cast<uintptr_t>(mins)) & 1u)
-    return set_error(EK_ERR_INVALID, "%s: misaligned scales", what);
-  return EK_OK;
 }
 
 }  // namespace w4

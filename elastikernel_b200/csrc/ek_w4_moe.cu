@@ -1,6 +1,6 @@
 // The experts' products of a fused MoE layer with 4-bit weights.
 #include "ek_moe_order.cuh"
-#include "ek_w4_kernel.cuh"
+#include "ek_w4_launch.cuh"
 
 namespace ek {
 
@@ -34,7 +34,7 @@ struct MoeLayout {
 MoeLayout moe_layout(long long x_rows, int rows, int E, int H, int I, int sms) {
   MoeLayout l;
   l.nt = pick_nt(rows, E);
-  l.grid = sms * occupancy(l.nt);
+  l.grid = sms * kCtasPerSm;
   l.max_y = max_token_tiles(rows, E, l.nt);
   const int tok = 8 * l.nt;
   const long long ft1 = (I + kRows / 2 - 1) / (kRows / 2), ft2 = (H + kRows - 1) / kRows;
@@ -148,23 +148,18 @@ struct Moe {
   }
   template <Mode kMode, class O>
   int finish(const Params<bf16>& p, O* out) const {
-    return l.nt == 1   ? finish_tok<kMode, 8>(p, out)
-           : l.nt == 2 ? finish_tok<kMode, 16>(p, out)
-           : l.nt == 3 ? finish_tok<kMode, 24>(p, out)
-                       : finish_tok<kMode, 32>(p, out);
+    return l.nt == 1 ? finish_tok<kMode, 8>(p, out) : finish_tok<kMode, 16>(p, out);
   }
   // gate/up, down and combine, from an order of the slots
   int layer(const bf16* xin, const Order& o, int T, int topk, const Matrix& w1, const Matrix& w3, const Matrix& w2,
             bf16* out) const {
     Params<bf16> p;
     int rc = gate_up(xin, T, o.sorted_slots, topk, w1, w3, &p);
-    if (!rc) rc = l.nt == 1 ? act_tokens<8>(p) : l.nt == 2 ? act_tokens<16>(p) : l.nt == 3 ? act_tokens<24>(p) : act_tokens<32>(p);
+    if (!rc) rc = l.nt == 1 ? act_tokens<8>(p) : act_tokens<16>(p);
     if (!rc) rc = down(w2, &p);
     if (rc) return rc;
-    return l.nt == 1   ? combine<8>(p, o.slot_rows, o.ids, o.weights, T, topk, out)
-           : l.nt == 2 ? combine<16>(p, o.slot_rows, o.ids, o.weights, T, topk, out)
-           : l.nt == 3 ? combine<24>(p, o.slot_rows, o.ids, o.weights, T, topk, out)
-                       : combine<32>(p, o.slot_rows, o.ids, o.weights, T, topk, out);
+    return l.nt == 1 ? combine<8>(p, o.slot_rows, o.ids, o.weights, T, topk, out)
+                     : combine<16>(p, o.slot_rows, o.ids, o.weights, T, topk, out);
   }
   template <int TOK>
   int act_tokens(const Params<bf16>& p) const {
