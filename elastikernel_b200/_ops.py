@@ -871,9 +871,10 @@ def gemm_w4(a: torch.Tensor, qw: dict, out: torch.Tensor | None = None, num_sms:
     """C = a @ W^T with a [M, K] (bf16 or fp16) and a 4-bit weight W [N, K]
     (quant_w4) whose scales have a's dtype; C [M, N] in that dtype, fp32 sums.
 
-    Made for a few tokens; any M is right, but from a few hundred rows
+    Made for a few tokens; any M is right, but from about a hundred rows
     gemm(a, dequant_w4(qw), b_layout="nk") is faster (with the weights rounded
-    to a's dtype, which this product does not do)."""
+    to a's dtype, which this product does not do): 14336 x 4096 takes 17 against
+    62 us for 16 rows, 45 against 62 for 64, 83 against 63 for 128."""
     codes, scales, mins, lead, K, group = _check_w4("gemm_w4", qw, a.dtype)
     dev = _require_cuda(a, codes, scales, mins, out)
     if a.dim() != 2 or a.shape[1] != K or len(lead) != 1:
@@ -1029,7 +1030,7 @@ def fused_moe_w4(hidden_states: torch.Tensor, gate_logits: torch.Tensor, qw: dic
                  out: torch.Tensor | None = None, num_sms: int | None = None) -> torch.Tensor:
     """MoE layer over 4-bit experts (quant_moe_weights_w4), for batches of a few
     tokens per expert: moe_route -> moe_dispatch -> moe_experts_w4 in one call
-    (five launches up to 1024 slots)."""
+    (five launches up to 128 slots)."""
     E, H, I = qw["E"], qw["H"], qw["I"]
     (c1, s1, m1, group), (c3, s3, m3, _), (c2, s2, m2, _) = _check_experts(qw, "w1", "w3", "w2")
     dev = _require_cuda(hidden_states, gate_logits, c1, s1, m1, c3, s3, m3, c2, s2, m2, out)

@@ -256,7 +256,7 @@ struct Params {
   int K, N;                  // N: weight rows (of an expert; of one matrix)
   int feature_tiles;         // tiles along N
   Tokens x;
-  const T* rows;             // the rows themselves, where the kernel makes the records (Shape::kMakes)
+  const T* rows;             // the rows themselves, where the kernel makes the records (Shape::kMakes); else null
   bool vec;                  // wide loads can read them
   int n_rows;                // token rows: M, or the packed rows
   int max_y;                 // token tiles there is room for

@@ -71,7 +71,9 @@ int launch_product_shape(const CUtensorMap& a, const CUtensorMap& b, const Param
 
 template <class T, Mode kMode, int FL, bool kMin>
 int launch_product_nt(int nt, const CUtensorMap& a, const CUtensorMap& b, const Params<T>& p, int grid, cudaStream_t stream) {
-  return nt == 1 ? launch_product_shape<T, kMode, Shape<1, FL, kMin, kMode == kDense>>(a, b, p, grid, stream)
+  if constexpr (kMode == kDense)
+    if (p.rows) return launch_product_shape<T, kMode, Shape<1, FL, kMin, true>>(a, b, p, grid, stream);
+  return nt == 1 ? launch_product_shape<T, kMode, Shape<1, FL, kMin, false>>(a, b, p, grid, stream)
                  : launch_product_shape<T, kMode, Shape<2, FL, kMin, false>>(a, b, p, grid, stream);
 }
 

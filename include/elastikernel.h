@@ -505,7 +505,7 @@ int ek_dequant_w4(const void* codes, const void* scales, const void* mins, long 
 
 /* C[M, N] = A[M, K] @ W[N, K]^T with 4-bit W; A, C, scales and mins in dtype,
  * fp32 sums rounded once. Any M, N and K; made for M of a few tokens, where the
- * codes are streamed once (per 32 tokens). A's elements enter as fp16 scaled
+ * codes are streamed once per 16 tokens. A's elements enter as fp16 scaled
  * per run of 256 by a power of two: exact up to 2^-40 of the run's largest.
  * workspace: ek_gemm_w4_workspace_bytes(M, N, K, SMs of the launch) bytes of
  * 16-byte aligned device memory, no initial contents; nothing in it is kept
@@ -546,7 +546,7 @@ int ek_moe_experts_w4(const void* x, int T, int topk, const int* topk_ids, const
 
 /* The whole layer from the gate logits: ek_moe_route, ek_moe_dispatch (order
  * only) and ek_moe_experts_w4, the first two and the tokens' conversion as one
- * launch up to 1024 slots. A token whose logits are all NaN is dropped and
+ * launch up to 128 slots. A token whose logits are all NaN is dropped and
  * raises EK_STATUS_BAD_INDEX. E <= 256, topk <= 8. */
 size_t ek_fused_moe_w4_workspace_bytes(int T, int topk, int E, int H, int I, int num_sms);
 int ek_fused_moe_w4(const void* x, const float* logits, int T, int topk, const void* w1_codes, const void* w1_scales,
