@@ -58,8 +58,11 @@ constexpr int kStageBytes = kRows * 128;
 constexpr int kStages = 2;  // ring depth (two CTAs per SM; more stages of one CTA were no faster)
 // Bytes of a token's record of a stage: 256 halfs, then its scale and the sums
 // of its groups (fp32; at most 8). 64 more than 512 also keeps the reads of
-// eight tokens free of bank conflicts.
+// eight tokens free of bank conflicts; in shared memory the scales and sums stand
+// behind the records, 48 bytes a token, for the same reason (read from the records
+// themselves, four of them collide: 3 to 7 % more time with minima).
 constexpr int kRecord = kStageElems * 2 + 64;
+constexpr int kTail = 48;
 
 __host__ __device__ inline int pieces(int K) { return (K + kPiece - 1) / kPiece; }
 __host__ __device__ inline int groups(int K, int group) { return (K + group - 1) / group; }
@@ -150,6 +153,7 @@ __host__ __device__ inline int stages(int K) { return (K + kStageElems - 1) / kS
 struct Tokens {
   uint8_t* rec;
 };
+__device__ __forceinline__ float* tail_of(uint8_t* rec) { return reinterpret_cast<float*>(rec + kStageElems * 2); }
 
 // The workspace of one product: the token records and the CTAs' sums.
 struct Layout {
@@ -165,12 +169,12 @@ inline Layout layout(long long rows, int K, long long tiles, int ctas, int tok) 
 __device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void griddep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-// A warp writes record `at`: eight elements v per lane. The scale comes from the
+// A warp writes a record and its tail: eight elements v per lane. The scale comes from the
 // largest finite magnitude, so an infinity or a NaN stays what it is and its
 // neighbours stay finite. kScaled = false (fp16 rows): as they are. The sums are
 // those of the rounded halfs, per `group` elements.
 template <bool kScaled>
-__device__ __forceinline__ void write_run(const Tokens& out, size_t at, int group, const float (&v)[8]) {
+__device__ __forceinline__ void write_run(uint8_t* rec, float* tail, int group, const float (&v)[8]) {
   const int lane = threadIdx.x & 31;
   float f = 1.f, inv = 1.f;
   if constexpr (kScaled) {
@@ -195,9 +199,7 @@ __device__ __forceinline__ void write_run(const Tokens& out, size_t at, int grou
     sum += r.x + r.y;
   }
   for (int o = group / 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);  // lanes of one group
-  uint8_t* rec = out.rec + at * kRecord;
   *reinterpret_cast<uint4*>(rec + lane * 16) = *reinterpret_cast<const uint4*>(h);
-  float* tail = reinterpret_cast<float*>(rec + kStageElems * 2);
   if (lane == 0) tail[0] = inv;
   if (lane % (group / 8) == 0) tail[4 + lane / (group / 8)] = sum;
 }
@@ -227,7 +229,8 @@ __device__ __forceinline__ void write_tokens(const T* __restrict__ x, int rows, 
     const int row = (int)(u / nst), st = (int)(u - (long long)row * nst);
     float v[8];
     load_run(x + (size_t)row * K, st * kStageElems + lane * 8, K, vec, v);
-    write_run<!std::is_same<T, __half>::value>(out, u, group, v);
+    uint8_t* rec = out.rec + u * kRecord;
+    write_run<!std::is_same<T, __half>::value>(rec, tail_of(rec), group, v);
   }
 }
 
@@ -278,7 +281,7 @@ struct Shape {
   static constexpr int NT = NT_, FL = FL_;
   static constexpr bool kMin = kMin_, kMakes = kMakes_;
   static constexpr int kTokens = 8 * NT;
-  static constexpr int kTokenBytes = kTokens * kRecord;  // of a stage
+  static constexpr int kTokenBytes = kTokens * (kRecord + kTail);  // of a stage
   static constexpr int kSmem = kStages * (kStageBytes + kTokenBytes) + 1024;  // + alignment of the swizzled stages
 };
 
@@ -440,7 +443,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int ahead = min(kStages, n_units);
     for (int i = 0; i < ahead; ++i) copy_codes(i);
     griddep_wait();
-    constexpr int kTail = S::kMin ? 1 + (kStagePieces / FL + 3) / 4 : 1;  // 16-byte units: scale, sums
+    constexpr int kTailUnits = S::kMin ? 1 + (kStagePieces / FL + 3) / 4 : 1;  // 16 bytes each: scale, sums
     int slot = 0, my_row = token_row(p, cx.tl, lane);  // lane j: the row of the tile's token j
     uint32_t parity = 1;
     for (int i = 0; i < n_units; ++i) {
@@ -449,11 +452,12 @@ __global__ void __launch_bounds__(kThreads, 2)
         copy_codes(slot);
       }
       if constexpr (S::kMakes) {
-        const Tokens rec{smem_x + slot * S::kTokenBytes};
+        uint8_t* rec = smem_x + slot * S::kTokenBytes;
         for (int j = 0; j < cx.tl.m; ++j) {
           float v[8];
           load_run(p.rows + (size_t)(cx.tl.r0 + j) * p.K, cx.st * kStageElems + lane * 8, p.K, p.vec, v);
-          write_run<!std::is_same<T, __half>::value>(rec, j, FL * kPiece, v);
+          write_run<!std::is_same<T, __half>::value>(
+              rec + j * kRecord, reinterpret_cast<float*>(rec + S::kTokens * kRecord + j * kTail), FL * kPiece, v);
         }
         mbar_arrive(&s_full[slot]);
         next(cx);
@@ -468,7 +472,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       for (int j = 0; j < cx.tl.m; ++j) {
         const uint8_t* rec = src + (size_t)__shfl_sync(0xffffffffu, my_row, j) * (nst * kRecord);
         cp_async16(dst + j * kRecord, rec);
-        if (lane < kTail) cp_async16(dst + j * kRecord + kStageElems * 2, rec + kStageElems * 2);
+        if (lane < kTailUnits) cp_async16(dst + S::kTokens * kRecord + j * kTail, rec + kStageElems * 2);
       }
       cp_async_mbar_arrive(&s_full[slot]);
       const int y0 = cx.y;
@@ -496,10 +500,7 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int set_step = kMode == kGateUp ? kRows / 2 : 16;
   const uint32_t base = smem_u32(smem);
   const int lrow = lane & 15, lpiece = lane >> 4;
-  uint32_t lm[kStagePieces / 2];
-#pragma unroll
-  for (int i = 0; i < kStagePieces / 2; ++i)
-    lm[i] = base + (set_row + lrow) * 128 + (((2 * i + lpiece) ^ (lrow & 7)) << 4);
+  const uint32_t lm = base + (set_row + lrow) * 128 + ((lpiece ^ (lrow & 7)) << 4);
 
   TokenTile tl = open_tile<kMode, S::kTokens>(p, y, s_end, s_row);
   // Scales run one stage ahead: first scale of rows g, g + 8 of each set.
@@ -531,9 +532,9 @@ __global__ void __launch_bounds__(kThreads, 2)
 
   // the weights are older than this launch's predecessor, the tokens are its
   // output; the consumers see them through the producer's copies
-  // this lane's run of 8 of token g, and the tail of the record of token 2 t
+  // this lane's run of 8 of token g, and the tail of token 2 t
   const uint32_t xs = smem_u32(smem_x) + g * kRecord + t * 16;
-  const uint32_t xt = smem_u32(smem_x) + t * 2 * kRecord + kStageElems * 2;
+  const uint32_t xt = smem_u32(smem_x) + S::kTokens * kRecord + t * 2 * kTail;
 
   float tot[2][NT][4] = {};
   int slot = 0;
@@ -571,7 +572,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       for (int pp = 0; pp < kStagePieces; ++pp) {
         if (pp % 2 == 0) {
 #pragma unroll
-          for (int s = 0; s < 2; ++s) ldmatrix4(code[s], lm[pp / 2] + slot * kStageBytes + s * set_step * 128);
+          for (int s = 0; s < 2; ++s) ldmatrix4(code[s], (lm ^ (pp << 4)) + slot * kStageBytes + s * set_step * 128);
         }
         uint4 xb[NB];
 #pragma unroll
@@ -595,6 +596,15 @@ __global__ void __launch_bounds__(kThreads, 2)
           }
         if ((pp + 1) % FL == 0) {
           const int gi = pp / FL, from = (lane & ~3) + gi % 4;
+          float xscale[NB][2], xsum[NB][2];
+#pragma unroll
+          for (int n = 0; n < NB; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const uint32_t tail = xt + slot * S::kTokenBytes + (n * 8 + c) * kTail;
+              xscale[n][c] = lds32(tail);
+              if constexpr (S::kMin) xsum[n][c] = lds32(tail + 16 + gi * 4);
+            }
 #pragma unroll
           for (int s = 0; s < 2; ++s) {
             const float2 sv = unpack2<T>(__shfl_sync(0xffffffffu, s_cur[s][gi / 4], from));
@@ -607,16 +617,13 @@ __global__ void __launch_bounds__(kThreads, 2)
             for (int n = 0; n < NB; ++n)
 #pragma unroll
               for (int c = 0; c < 2; ++c) {
-                const uint32_t tail = xt + slot * S::kTokenBytes + (n * 8 + c) * kRecord;
-                const float xscale = lds32(tail);
                 float a = sv.x * part[s][n][c], b = sv.y * part[s][n][2 + c];
                 if constexpr (S::kMin) {
-                  const float xsum = lds32(tail + 16 + gi * 4);
-                  a = fmaf(mv.x, xsum, a);
-                  b = fmaf(mv.y, xsum, b);
+                  a = fmaf(mv.x, xsum[n][c], a);
+                  b = fmaf(mv.y, xsum[n][c], b);
                 }
-                tot[s][n][c] = fmaf(xscale, a, tot[s][n][c]);
-                tot[s][n][2 + c] = fmaf(xscale, b, tot[s][n][2 + c]);
+                tot[s][n][c] = fmaf(xscale[n][c], a, tot[s][n][c]);
+                tot[s][n][2 + c] = fmaf(xscale[n][c], b, tot[s][n][2 + c]);
               }
           }
         }
@@ -756,7 +763,8 @@ __global__ void __launch_bounds__(256) act_tokens_kernel(const __grid_constant__
       sum_parts<TOK, 8, 2>(run, p.parts, y * p.feature_tiles + f, tok, n % (kRows / 2), v);
 #pragma unroll
     for (int i = 0; i < 8; ++i) a[i] = n + i < p.N ? swiglu(v[0][i], v[1][i]) : 0.f;
-    write_run<true>(act, (size_t)(tl.r0 + tok) * nst + st, group, a);
+    uint8_t* rec = act.rec + ((size_t)(tl.r0 + tok) * nst + st) * kRecord;
+    write_run<true>(rec, tail_of(rec), group, a);
   }
 }
 
