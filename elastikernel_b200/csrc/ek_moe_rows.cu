@@ -208,13 +208,14 @@ __host__ __device__ inline int runs_per_row(int nvec) { return (nvec + 32 * kRun
 constexpr int kCopyRun = 4;
 
 // Copy x[t] to the rows of token t; row_of(s): the row of slot s (negative:
-// dropped).
+// dropped). Neighbouring units go to different CTAs, so that few of them still
+// reach every SM.
 template <class Raw, class RowOf>
 __device__ __forceinline__ void copy_rows(const Raw* __restrict__ x, int T, int k, int nvec, const RowOf& row_of,
                                           Raw* __restrict__ rows) {
   const int lane = threadIdx.x & 31, runs = runs_per_row<kCopyRun>(nvec);
   const long long warps = ((long long)gridDim.x * blockDim.x) >> 5, units = (long long)T * runs;
-  for (long long u = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5; u < units; u += warps) {
+  for (long long u = (long long)(threadIdx.x >> 5) * gridDim.x + blockIdx.x; u < units; u += warps) {
     const Unit w = unit_of<kCopyRun>(u, runs);
     Raw v[kCopyRun];
 #pragma unroll
