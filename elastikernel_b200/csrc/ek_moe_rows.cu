@@ -182,6 +182,33 @@ struct Elems {
   }
 };
 
+// *p where `on`, else zero. A predicated instruction: behind branches the
+// compiler does not keep a token's loads in flight together.
+__device__ __forceinline__ uint4 load_if(const uint4* p, bool on) {
+  uint4 v = {};
+  asm volatile("{.reg .pred q; setp.ne.b32 q, %5, 0; @q ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];}"
+               : "+r"(v.x), "+r"(v.y), "+r"(v.z), "+r"(v.w)
+               : "l"(p), "r"((int)on));
+  return v;
+}
+__device__ __forceinline__ uint2 load_if(const uint2* p, bool on) {
+  uint2 v = {};
+  asm volatile("{.reg .pred q; setp.ne.b32 q, %3, 0; @q ld.global.nc.v2.u32 {%0, %1}, [%2];}"
+               : "+r"(v.x), "+r"(v.y)
+               : "l"(p), "r"((int)on));
+  return v;
+}
+__device__ __forceinline__ uint32_t load_if(const uint32_t* p, bool on) {
+  uint32_t v = 0;
+  asm volatile("{.reg .pred q; setp.ne.b32 q, %2, 0; @q ld.global.nc.u32 %0, [%1];}" : "+r"(v) : "l"(p), "r"((int)on));
+  return v;
+}
+__device__ __forceinline__ uint16_t load_if(const uint16_t* p, bool on) {
+  uint16_t v = 0;
+  asm volatile("{.reg .pred q; setp.ne.b32 q, %2, 0; @q ld.global.nc.u16 %0, [%1];}" : "+h"(v) : "l"(p), "r"((int)on));
+  return v;
+}
+
 // Zero the rows past the last kept one ([kept, n_rows)).
 template <class Raw>
 __device__ __forceinline__ void zero_tail(Raw* __restrict__ rows, int kept, int n_rows, int nvec) {
@@ -303,19 +330,21 @@ __global__ void __launch_bounds__(256)
         mine = __ldg(slot_rows + (long long)w.t * k + j0 + lane);
         if (kWeighted) wt = __ldg(weights + (long long)w.t * k + j0 + lane);
       }
+      if (mine < 0 || mine >= n_rows) {  // dropped, or past k: nothing times nothing
+        mine = -1;
+        wt = 0.f;
+      }
       typename E::Raw v[kK][kRun];
 #pragma unroll
       for (int j = 0; j < kK; ++j) {
         const int r = __shfl_sync(0xffffffffu, mine, j);
 #pragma unroll
         for (int i = 0; i < kRun; ++i)
-          if (r >= 0 && r < n_rows && w.c0 + 32 * i < nvec) v[j][i] = __ldg(rows + (long long)r * nvec + w.c0 + 32 * i);
+          v[j][i] = load_if(rows + (long long)r * nvec + w.c0 + 32 * i, r >= 0 && w.c0 + 32 * i < nvec);
       }
 #pragma unroll
       for (int j = 0; j < kK; ++j) {
-        const int r = __shfl_sync(0xffffffffu, mine, j);
         const float wj = kWeighted ? __shfl_sync(0xffffffffu, wt, j) : 1.f;
-        if (r < 0 || r >= n_rows) continue;
 #pragma unroll
         for (int i = 0; i < kRun; ++i) {
           float f[E::N];
