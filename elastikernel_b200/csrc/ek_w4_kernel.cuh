@@ -661,6 +661,24 @@ __global__ void __launch_bounds__(kThreads, 2)
 }
 
 // ------------------------------------------------------------------ sums
+// These launches set up the tiles before they wait for the product: the counts
+// and the order are older than it.
+
+// *p where `on`, else zero, from L2 (the product before has just written it; an
+// older launch on this SM may have left the last one's sums in L1). Predicated,
+// since behind branches the compiler does not keep the loads in flight together.
+__device__ __forceinline__ float load_if(const float* p, bool on) {
+  float v = 0.f;
+  asm volatile("{.reg .pred q; setp.ne.b32 q, %2, 0; @q ld.global.cg.f32 %0, [%1];}" : "+f"(v) : "l"(p), "r"((int)on));
+  return v;
+}
+__device__ __forceinline__ void load4_if(float* v, const float* p, bool on) {
+  v[0] = v[1] = v[2] = v[3] = 0.f;
+  asm volatile("{.reg .pred q; setp.ne.b32 q, %5, 0; @q ld.global.cg.v4.f32 {%0, %1, %2, %3}, [%4];}"
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3])
+               : "l"(p), "r"((int)on));
+}
+
 // The token tiles, set up by every thread of a CTA that reads the parts.
 template <Mode kMode, int TOK, class T>
 __device__ __forceinline__ Runs open_runs(const Params<T>& p, int grid, int* s_end, int* s_row, int* s_y) {
@@ -691,26 +709,22 @@ __device__ __forceinline__ void sum_parts(const Runs& run, const float* parts, i
     float b[kB][kN][kV];
 #pragma unroll
     for (int j = 0; j < kB; ++j)
-      if (c + j <= c1) {
 #pragma unroll
-        for (int n = 0; n < kN; ++n) {
-          const float* at = q + (size_t)j * (kRows * TOK) + n * (kRows / 2);
-          if constexpr (kV == 1) {
-            b[j][n][0] = __ldg(at);
-          } else {
+      for (int n = 0; n < kN; ++n) {
+        const float* at = q + (size_t)j * (kRows * TOK) + n * (kRows / 2);
+        if constexpr (kV == 1) {
+          b[j][n][0] = load_if(at, c + j <= c1);
+        } else {
 #pragma unroll
-            for (int i = 0; i < kV; i += 4) *reinterpret_cast<float4*>(&b[j][n][i]) = __ldg(reinterpret_cast<const float4*>(at + i));
-          }
+          for (int i = 0; i < kV; i += 4) load4_if(&b[j][n][i], at + i, c + j <= c1);
         }
       }
 #pragma unroll
     for (int j = 0; j < kB; ++j)
-      if (c + j <= c1) {
 #pragma unroll
-        for (int n = 0; n < kN; ++n)
+      for (int n = 0; n < kN; ++n)
 #pragma unroll
-          for (int i = 0; i < kV; ++i) v[n][i] += b[j][n][i];
-      }
+        for (int i = 0; i < kV; ++i) v[n][i] += b[j][n][i];
   }
 }
 
@@ -723,9 +737,9 @@ __global__ void __launch_bounds__(kRows) finish_kernel(const __grid_constant__ P
   extern __shared__ int s_index[];
   __shared__ int s_y;
   griddep_launch();
-  griddep_wait();
   int *s_end = s_index, *s_row = s_index + p.E;
   const Runs run = open_runs<kMode, TOK>(p, grid, s_end, s_row, &s_y);
+  griddep_wait();
   constexpr int kFeatures = kMode == kGateUp ? kRows / 2 : kRows;
   constexpr int kPer = kRows / kFeatures;  // tokens a CTA takes at a time
   const int f = blockIdx.x, r = threadIdx.x % kFeatures, n = f * kFeatures + r;
@@ -748,9 +762,9 @@ __global__ void __launch_bounds__(256) act_tokens_kernel(const __grid_constant__
   extern __shared__ int s_index[];
   __shared__ int s_y;
   griddep_launch();
-  griddep_wait();
   int *s_end = s_index, *s_row = s_index + p.E;
   const Runs run = open_runs<kGateUp, TOK>(p, grid, s_end, s_row, &s_y);
+  griddep_wait();
   const int lane = threadIdx.x & 31, nst = stages(p.N);
   const long long warps = ((long long)gridDim.x * blockDim.x) >> 5, total = (long long)s_y * TOK * nst;
   for (long long w = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5; w < total; w += warps) {
@@ -778,60 +792,73 @@ __global__ void __launch_bounds__(kRows, 4)
   extern __shared__ int s_index[];
   __shared__ int s_y;
   griddep_launch();
-  griddep_wait();
   int *s_end = s_index, *s_row = s_index + p.E;
   const Runs run = open_runs<kDown, TOK>(p, grid, s_end, s_row, &s_y);
-  // Where the slots' sums lie: first part, parts (0: dropped) and weight, found
-  // by one lane each; then every thread adds its feature's.
-  constexpr int kSlots = 32;
-  __shared__ size_t s_at[kSlots];
-  __shared__ int s_parts[kSlots];
-  __shared__ float s_w[kSlots];
-  const int f = blockIdx.x, n = f * kRows + threadIdx.x;
+  // The token's parts in order, listed by the first warp (a slot per lane): row of
+  // 256 sums, and for the last part of a slot its weight.
+  constexpr int kList = 256, kB = 8;  // kB: loads in flight together
+  __shared__ uint32_t s_part[kList];  // top bit: the slot's last
+  __shared__ float s_w[kList];
+  __shared__ int s_n;
+  const int lane = threadIdx.x & 31, f = blockIdx.x, n = f * kRows + threadIdx.x;
+  bool waited = false;
   for (int t = blockIdx.y; t < tokens; t += gridDim.y) {
-    float acc = 0.f;
-    for (int j0 = 0; j0 < topk; j0 += kSlots) {
-      const int kn = min(kSlots, topk - j0);
-      __syncthreads();
-      if (threadIdx.x < kn) {
-        const long long s = (long long)t * topk + j0 + threadIdx.x;
-        const int r = __ldg(slot_rows + s), e = __ldg(ids + s);
-        s_parts[threadIdx.x] = 0;
-        s_w[threadIdx.x] = __ldg(weights + s);
-        if (r >= 0 && r < p.n_rows && e >= 0 && e < p.E) {
-          const int at = r - s_row[e], y = (e ? s_end[e - 1] : 0) + at / TOK;
-          if (at >= 0 && y < min(s_end[e], s_y)) {
-            const int tile = y * p.feature_tiles + f;
-            const int c0 = run.owner((long long)tile * run.nst), c1 = run.owner((long long)(tile + 1) * run.nst - 1);
-            s_at[threadIdx.x] = (size_t)(tile + c0) * (kRows * TOK) + (at % TOK) * kRows;
-            s_parts[threadIdx.x] = c1 - c0 + 1;
+    float acc = 0.f, v = 0.f;
+    for (int j0 = 0; j0 < topk; j0 += 32) {
+      uint32_t part = 0;
+      int np = 0, begin = 0;
+      float w = 0.f;
+      if (threadIdx.x < 32) {
+        if (j0 + lane < topk) {
+          const long long s = (long long)t * topk + j0 + lane;
+          const int r = __ldcg(slot_rows + s), e = __ldcg(ids + s);
+          w = __ldcg(weights + s);
+          if (r >= 0 && r < p.n_rows && e >= 0 && e < p.E) {  // else dropped
+            const int at = r - s_row[e], y = (e ? s_end[e - 1] : 0) + at / TOK;
+            if (at >= 0 && y < min(s_end[e], s_y)) {
+              const int tile = y * p.feature_tiles + f;
+              const int c0 = run.owner((long long)tile * run.nst), c1 = run.owner((long long)(tile + 1) * run.nst - 1);
+              part = (uint32_t)(tile + c0) * TOK + at % TOK;
+              np = c1 - c0 + 1;
+            }
           }
         }
+        int incl = np;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int a = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += a;
+        }
+        begin = incl - np;
+        if (lane == 31) s_n = incl;
       }
-      __syncthreads();
-      if (n >= p.N) continue;
-      constexpr int kB = 8;  // slots, and parts of a slot, whose loads are in flight together
-      for (int j = 0; j < kn; j += kB) {
-        float v[kB];
-#pragma unroll
-        for (int i = 0; i < kB; ++i)
-          if (j + i < kn && s_parts[j + i] > 0) v[i] = __ldg(p.parts + s_at[j + i] + threadIdx.x);
-#pragma unroll
-        for (int i = 0; i < kB; ++i) {
-          if (j + i >= kn || s_parts[j + i] == 0) continue;
-          const float* q = p.parts + s_at[j + i] + threadIdx.x;
-          const int np = s_parts[j + i];
-          for (int c = 1; c < np; c += kB) {
-            float b[kB];
-#pragma unroll
-            for (int u = 0; u < kB; ++u)
-              if (c + u < np) b[u] = __ldg(q + (size_t)(c + u) * (kRows * TOK));
-#pragma unroll
-            for (int u = 0; u < kB; ++u)
-              if (c + u < np) v[i] += b[u];
+      for (int base = 0;; base += kList) {
+        if (threadIdx.x < 32)
+          for (int c = max(0, base - begin); c < np && begin + c < base + kList; ++c) {
+            s_part[begin + c - base] = part + c * TOK | (c + 1 == np ? 1u << 31 : 0u);
+            s_w[begin + c - base] = w;
           }
-          acc = fmaf(s_w[j + i], v[i], acc);
+        __syncthreads();
+        const int total = s_n, count = min(kList, total - base);
+        if (!waited) griddep_wait();
+        waited = true;
+        for (int i = 0; i < count; i += kB) {
+          float b[kB];
+#pragma unroll
+          for (int u = 0; u < kB; ++u)
+            b[u] = load_if(p.parts + (size_t)(s_part[min(i + u, kList - 1)] & 0x7fffffffu) * kRows + threadIdx.x, i + u < count);
+#pragma unroll
+          for (int u = 0; u < kB; ++u) {
+            if (i + u >= count) break;
+            v += b[u];
+            if (s_part[i + u] >> 31) {
+              acc = fmaf(s_w[i + u], v, acc);
+              v = 0.f;
+            }
+          }
         }
+        __syncthreads();
+        if (base + kList >= total) break;
       }
     }
     if (n < p.N) out[(size_t)t * p.N + n] = from_f<T>(acc);
