@@ -8,9 +8,13 @@
 //                  d_w[t,j] = <d_out[t], rows[r]>
 //   route_grad     gradient of the renormalised top-k softmax to the gate logits
 //
-// All of it is data movement: the token side of each copy (T rows) is read or
-// written once and kept in registers across the token's k slots, so the bytes
-// are T rows plus T*k rows, whatever k. Slots with a negative expert id are
+// All of it is data movement, bound by HBM for long batches and by the launch for
+// short ones: the token side of each copy (T rows) is read or written once and
+// kept in registers across the token's k slots, so the bytes are T rows plus T*k
+// rows, whatever k. Measured with 8192 tokens, 8 choices, 256 experts, 7168 bf16
+// (HBM copies run at 6.5 TB/s): dispatch 178 us (10 of them the order), its
+// gradient 169 us (6.3 TB/s), weighted sum 160 us (6.6 TB/s), its gradient 304 us
+// (6.6 TB/s). Slots with a negative expert id are
 // dropped: they have no row, weigh nothing and get no gradient; the rows past
 // the last kept one are zero.
 #include <cuda_bf16.h>
@@ -43,6 +47,8 @@ constexpr int kChunk = kOrderThreads;  // slots per sorting CTA, one per thread
 constexpr int kMaxE = kOrderMaxE;
 
 // ------------------------------------------------------------------ dispatch: the order
+// Chunks of 1024 slots, a CTA each: count, then place. 65536 slots, 256 experts: 3.2
+// and 8.2 us, bound by the latency of their steps (0.8 MB in all).
 __global__ void __launch_bounds__(kChunk) dispatch_count_kernel(const int* __restrict__ ids, int n_slots, int E,
                                                                 int* __restrict__ chunk_counts) {
   __shared__ int cnt[kMaxE];
@@ -263,7 +269,8 @@ __device__ __forceinline__ void copy_rows(const Raw* __restrict__ x, int T, int 
   }
 }
 
-// rows[slot_rows[t*k + j]] = x[t] for the kept slots of each token.
+// rows[slot_rows[t*k + j]] = x[t] for the kept slots of each token. 8192 tokens, 8
+// choices, 7168 bf16: 168 us, 6.3 TB/s.
 template <int V>
 __global__ void __launch_bounds__(256)
     dispatch_copy_kernel(const typename Vec<V>::type* __restrict__ x, const int* __restrict__ slot_rows,
@@ -274,8 +281,10 @@ __global__ void __launch_bounds__(256)
 }
 
 // Small batches (T * k <= kOrderThreads) in one launch: every CTA works out the
-// whole order (about 2 us, against two more launches) and copies its share of
-// the rows; the first one writes the maps.
+// whole order and copies its share of the rows; the first one writes the maps.
+// Against count, place and copy (bf16): 64 tokens, 8 choices, 256 experts, 7168 wide
+// 4.6 against 9.4 us; 1024 slots of 1024 experts 7.8 against 11.6; the order alone
+// of 512 slots 3.0 against 5.0.
 template <int V>
 __global__ void __launch_bounds__(kOrderThreads)
     dispatch_small_kernel(const int* __restrict__ ids, int T, int k, int E, const typename Vec<V>::type* __restrict__ x,
@@ -310,7 +319,9 @@ __global__ void __launch_bounds__(kOrderThreads)
 }
 
 // out[t] = sum_j w[t,j] rows[slot_rows[t,j]] (w = 1 without weights), fp32 sum
-// in j order, rounded once. kK: rows whose loads are in flight together.
+// in j order, rounded once. kK: rows whose loads are in flight together (2, 4 or
+// 8, the least that holds the choices; a lane holds kK vectors at a time, two of
+// each row for up to 2 choices).
 template <class T, int V, bool kWeighted, int kK>
 __global__ void __launch_bounds__(256)
     sum_rows_kernel(const typename Vec<V>::type* __restrict__ rows, const int* __restrict__ slot_rows,
@@ -364,7 +375,7 @@ __global__ void __launch_bounds__(256)
 // d_rows[r] = w[s] d_out[t] and d_weights[s] = <d_out[t], rows[r]> (fp32). kTpt
 // threads per token; d_out[t] is read once (per kK slots), the kK rows' loads
 // are in flight together, and the kK dot products stay in registers until the
-// row's end.
+// row's end. 4096 tokens, 8 choices, 7168 bf16: 156 us, 6.4 TB/s.
 template <class T, int V, int kK, int kTpt>
 __global__ void __launch_bounds__(128)
     combine_grad_kernel(const typename Vec<V>::type* __restrict__ rows, const int* __restrict__ slot_rows,
@@ -449,7 +460,9 @@ __global__ void __launch_bounds__(128)
 // d_logit[ids_j] += w_j (dw_j - sum_i w_i dw_i) and every other logit gets 0.
 // kp lanes (a power of two >= k, up to 32) per token, 32 / kp tokens per warp:
 // the warp clears its tokens' rows with wide stores, then each lane puts its
-// slot's value where it belongs (the lowest lane, where an id repeats).
+// slot's value where it belongs (the lowest lane, where an id repeats; the sum
+// then is in lane order, so that it does not change between runs). 32768 tokens, 256
+// experts: 9.5 us with a cold cache for 37 MB, most of it the zeros.
 __global__ void __launch_bounds__(256)
     route_grad_kernel(const int* __restrict__ ids, const float* __restrict__ weights,
                       const float* __restrict__ d_weights, int T, int E, int k, int kp, bool wide,
@@ -589,8 +602,12 @@ int launch_combine_grad(const Rows& a, const void* d_out, const int* num_rows, v
   const auto* rows = static_cast<const Raw*>(a.rows);
   const auto* d = static_cast<const Raw*>(d_out);
   auto* o = static_cast<Raw*>(d_rows);
-  // short rows: a warp per token; else a CTA of four
-  if (nvec <= 64)
+  // Short rows of many tokens: a warp per token; else a CTA of four, whose lanes
+  // each have a vector and which are enough for few tokens too. Measured (bf16),
+  // a warp against a CTA: 8192 tokens, 8 choices, 128 wide 9.4 against 24.1 us,
+  // 512 wide 26.7 against 41.1, 1024 wide 50.3 against 52.7, 2048 wide 95.4 against
+  // 90.5; 64 tokens, 8 choices, 128 wide 3.0 against 2.8, 1024 wide 5.2 against 3.0.
+  if (nvec <= 128 && a.T >= 148 * 8)
     combine_grad_kernel<T, V, kK, 32><<<std::max(1, std::min((a.T + 3) / 4, 148 * 64)), 128, 0, a.s>>>(
         rows, a.slot_rows, a.w, d, num_rows, a.T, a.k, a.n_rows, nvec, o, d_w);
   else
