@@ -678,6 +678,11 @@ def _check_slots(name: str, t: torch.Tensor, T: int, k: int, dtype: torch.dtype)
     _contig(name, t)
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two contiguous tensors share memory."""
+    return a.data_ptr() < b.data_ptr() + b.nbytes and b.data_ptr() < a.data_ptr() + a.nbytes
+
+
 def _slot_rows(perm: dict) -> torch.Tensor:
     if perm.get("slot_rows") is None:
         raise RuntimeError("the permutation has no slot_rows (make it with moe_dispatch)")
@@ -749,6 +754,8 @@ def moe_combine_weighted(perm: dict, rows: torch.Tensor, topk_weights: torch.Ten
         out = rows.new_empty((T, H))
     elif out.dtype != rows.dtype or out.shape != (T, H) or not out.is_contiguous():
         raise RuntimeError("out must be a contiguous [T, H] tensor of the rows' dtype")
+    elif _overlap(out, rows):
+        raise RuntimeError("out must not overlap the rows (they are still read while it is written)")
     with _on_device(dev):
         check(lib().ek_moe_combine_weighted(rows.data_ptr(), slot_rows.data_ptr(), topk_weights.data_ptr(), T, k, n, H,
                                             dt, out.data_ptr(), current_stream_handle(dev)),

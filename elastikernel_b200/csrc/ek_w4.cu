@@ -156,7 +156,7 @@ int ek_quant_w4(const void* w, int w_dtype, long long rows, int K, int group, in
       (dtype != EK_DTYPE_BF16 && dtype != EK_DTYPE_FP16))
     return set_error(EK_ERR_INVALID, "quant_w4: bad sizes or types (rows=%lld w_dtype=%d dtype=%d)", rows, w_dtype, dtype);
   if (rows == 0) return EK_OK;
-  int rc = check_w4("quant_w4", codes, scales, mins, K, group);
+  int rc = check_w4("quant_w4", codes, scales, mins, 0, K, group);
   if (rc) return rc;
   if (!w || (!symmetric && !mins)) return set_error(EK_ERR_INVALID, "quant_w4: null pointer");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -171,7 +171,7 @@ int ek_dequant_w4(const void* codes, const void* scales, const void* mins, long 
   if (rows < 0 || (dtype != EK_DTYPE_BF16 && dtype != EK_DTYPE_FP16))
     return set_error(EK_ERR_INVALID, "dequant_w4: bad sizes or type (rows=%lld dtype=%d)", rows, dtype);
   if (rows == 0) return EK_OK;
-  int rc = check_w4("dequant_w4", codes, scales, mins, K, group);
+  int rc = check_w4("dequant_w4", codes, scales, mins, 0, K, group);
   if (rc) return rc;
   if (!out) return set_error(EK_ERR_INVALID, "dequant_w4: null pointer");
   const long long warps = rows * ((stages(K) + kDequantRuns - 1) / kDequantRuns);

@@ -30,7 +30,7 @@ using namespace ek::w4;
 extern "C" {
 
 size_t ek_gemm_w4_workspace_bytes(int M, int N, int K, int num_sms) {
-  if (M < 0 || N < 0 || K < 1 || num_sms < 1) return (size_t)-1;
+  if (M < 0 || N < 0 || K < 1 || K > kMaxK || num_sms < 1) return (size_t)-1;
   if (M == 0 || N == 0) return 0;
   int nt = 0, grid = 0;
   return gemm_layout(M, N, K, num_sms, &nt, &grid).bytes;
@@ -42,7 +42,7 @@ int ek_gemm_w4(const void* A, const void* codes, const void* scales, const void*
   if (M < 0 || N < 0 || (dtype != EK_DTYPE_BF16 && dtype != EK_DTYPE_FP16))
     return set_error(EK_ERR_INVALID, "gemm_w4: bad sizes or type (M=%d N=%d dtype=%d)", M, N, dtype);
   if (M == 0 || N == 0) return EK_OK;
-  int rc = check_w4("gemm_w4", codes, scales, mins, K, group);
+  int rc = check_w4("gemm_w4", codes, scales, mins, N, K, group);
   if (rc) return rc;
   if (!A || !C || !workspace) return set_error(EK_ERR_INVALID, "gemm_w4: null pointer");
   if ((reinterpret_cast<uintptr_t>(A) | reinterpret_cast<uintptr_t>(C)) & 1u)

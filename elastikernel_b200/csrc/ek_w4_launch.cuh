@@ -109,9 +109,16 @@ inline int codes_map(CUtensorMap* m, const void* codes, long long rows, int K, i
   return make_tmap_2d(m, codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, pitch, (uint64_t)rows, pitch, 128, box);
 }
 
-inline int check_w4(const char* what, const void* codes, const void* scales, const void* mins, int K, int group) {
-  if (K < 1 || (group != 32 && group != 64 && group != 128))
-    return set_error(EK_ERR_INVALID, "%s: need K >= 1 and a group of 32, 64 or 128 (K=%d group=%d)", what, K, group);
+constexpr int kMaxK = 1 << 28;
+
+// rows: of the whole weight, whose scales the products index in 32 bits (0: no
+// matter); a token row's records are indexed in an int.
+inline int check_w4(const char* what, const void* codes, const void* scales, const void* mins, long long rows, int K,
+                    int group) {
+  if (K < 1 || K > kMaxK || (group != 32 && group != 64 && group != 128))
+    return set_error(EK_ERR_INVALID, "%s: need K >= 1 (at most 2^28) and a group of 32, 64 or 128 (K=%d group=%d)", what, K, group);
+  if (rows * groups(K, group) > 0xffffffffll)
+    return set_error(EK_ERR_INVALID, "%s: more than 2^32 scales (rows=%lld K=%d group=%d)", what, rows, K, group);
   if (!codes || !scales) return set_error(EK_ERR_INVALID, "%s: null pointer", what);
   if (!aligned16(codes)) return set_error(EK_ERR_INVALID, "%s: codes must be 16-byte aligned", what);
   if ((reinterpret_cast<uintptr_t>(scales) | reinterpret_cast<uintptr_t>(mins)) & 1u)

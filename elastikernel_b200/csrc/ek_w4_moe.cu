@@ -196,7 +196,7 @@ int open_moe(const char* what, Moe* m, long long x_rows, const int* counts, int 
 }
 
 int check_sizes(const char* what, long long x_rows, long long rows, int E, int H, int I) {
-  if (x_rows < 0 || rows < 0 || E < 1 || E > 1024 || H < 1 || I < 1 || (long long)E * std::max(H, I) > 0x7fffffffll)
+  if (x_rows < 0 || rows < 0 || E < 1 || E > 1024 || H < 1 || I < 1 || std::max(H, I) > kMaxK || (long long)E * std::max(H, I) > 0x7fffffffll)
     return set_error(EK_ERR_INVALID, "%s: bad sizes (rows=%lld E=%d H=%d I=%d)", what, rows, E, H, I);
   if (rows > (1ll << 24)) return set_error(EK_ERR_INVALID, "%s: too many rows", what);
   return EK_OK;
@@ -232,8 +232,8 @@ int ek_moe_gate_up_w4(const void* x, int x_rows, const int* sorted_slots, int to
   if (topk < 1 || (long long)x_rows * (sorted_slots ? topk : 1) != rows)
     return set_error(EK_ERR_INVALID, "gate_up_w4: %d rows do not match %d of x (topk=%d)", rows, x_rows, topk);
   if (rows == 0) return EK_OK;
-  rc = check_w4("gate_up_w4", w1_codes, w1_scales, w1_mins, H, group);
-  if (!rc) rc = check_w4("gate_up_w4", w3_codes, w3_scales, w3_mins, H, group);
+  rc = check_w4("gate_up_w4", w1_codes, w1_scales, w1_mins, (long long)E * I, H, group);
+  if (!rc) rc = check_w4("gate_up_w4", w3_codes, w3_scales, w3_mins, (long long)E * I, H, group);
   if (rc) return rc;
   if (!x || !act || !w1_mins != !w3_mins) return set_error(EK_ERR_INVALID, "gate_up_w4: null pointer");
   if (misaligned16bit({x, act}) || (act_dtype == EK_DTYPE_FP32 && (reinterpret_cast<uintptr_t>(act) & 3u)))
@@ -257,7 +257,7 @@ int ek_moe_down_w4(const void* act, int act_dtype, const void* w2_codes, const v
   if ((act_dtype != EK_DTYPE_BF16 && act_dtype != EK_DTYPE_FP32) || (y_dtype != EK_DTYPE_BF16 && y_dtype != EK_DTYPE_FP32))
     return set_error(EK_ERR_INVALID, "down_w4: act and y must be bf16 or fp32 (dtypes %d, %d)", act_dtype, y_dtype);
   if (rows == 0) return EK_OK;
-  rc = check_w4("down_w4", w2_codes, w2_scales, w2_mins, I, group);
+  rc = check_w4("down_w4", w2_codes, w2_scales, w2_mins, (long long)E * H, I, group);
   if (rc) return rc;
   if (!act || !y) return set_error(EK_ERR_INVALID, "down_w4: null pointer");
   if (misaligned16bit({act, y}) || (act_dtype == EK_DTYPE_FP32 && (reinterpret_cast<uintptr_t>(act) & 3u)) ||
@@ -284,9 +284,9 @@ int ek_moe_experts_w4(const void* x, int T, int topk, const int* topk_ids, const
   int rc = topk < 1 ? set_error(EK_ERR_INVALID, "experts_w4: bad sizes (topk=%d)", topk)
                     : check_sizes("experts_w4", T, rows, E, H, I);
   if (rc || T == 0) return rc;
-  rc = check_w4("experts_w4", w1_codes, w1_scales, w1_mins, H, group);
-  if (!rc) rc = check_w4("experts_w4", w3_codes, w3_scales, w3_mins, H, group);
-  if (!rc) rc = check_w4("experts_w4", w2_codes, w2_scales, w2_mins, I, group);
+  rc = check_w4("experts_w4", w1_codes, w1_scales, w1_mins, (long long)E * I, H, group);
+  if (!rc) rc = check_w4("experts_w4", w3_codes, w3_scales, w3_mins, (long long)E * I, H, group);
+  if (!rc) rc = check_w4("experts_w4", w2_codes, w2_scales, w2_mins, (long long)E * H, I, group);
   if (rc) return rc;
   if (!x || !out || !topk_ids || !topk_weights || !sorted_slots || !slot_rows || !w1_mins != !w3_mins)
     return set_error(EK_ERR_INVALID, "experts_w4: null pointer");
@@ -319,9 +319,9 @@ int ek_fused_moe_w4(const void* x, const float* logits, int T, int topk, const v
   const long long rows = (long long)T * topk;
   int rc = check_sizes("fused_moe_w4", T, rows, E, H, I);
   if (rc || T == 0) return rc;
-  rc = check_w4("fused_moe_w4", w1_codes, w1_scales, w1_mins, H, group);
-  if (!rc) rc = check_w4("fused_moe_w4", w3_codes, w3_scales, w3_mins, H, group);
-  if (!rc) rc = check_w4("fused_moe_w4", w2_codes, w2_scales, w2_mins, I, group);
+  rc = check_w4("fused_moe_w4", w1_codes, w1_scales, w1_mins, (long long)E * I, H, group);
+  if (!rc) rc = check_w4("fused_moe_w4", w3_codes, w3_scales, w3_mins, (long long)E * I, H, group);
+  if (!rc) rc = check_w4("fused_moe_w4", w2_codes, w2_scales, w2_mins, (long long)E * H, I, group);
   if (rc) return rc;
   if (!x || !logits || !out || !workspace || !w1_mins != !w3_mins)
     return set_error(EK_ERR_INVALID, "fused_moe_w4: null pointer");

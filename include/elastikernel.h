@@ -465,7 +465,7 @@ int ek_moe_dispatch_grad(const void* d_rows, const int* slot_rows, int T, int to
                          void* d_x, void* stream);
 
 /* The way back: out[t] = sum_j weights[t, j] * rows[slot_rows[t, j]] over the
- * kept slots (fp32 in j order, rounded once). */
+ * kept slots (fp32 in j order, rounded once). out must not overlap rows. */
 int ek_moe_combine_weighted(const void* rows, const int* slot_rows, const float* weights, int T, int topk, int n_rows,
                             int H, int dtype, void* out, void* stream);
 

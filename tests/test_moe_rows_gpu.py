@@ -33,6 +33,9 @@ CASES = [  # T, k, E, H, dtype, drop
     (1025, 1, 1024, 20, "fp32", "none"),
     (4100, 2, 3, 40, "fp16", "some"),
     (9000, 8, 64, 96, "bf16", "some"),
+    (1500, 3, 12, 200, "fp32", "some"),
+    (1200, 8, 9, 1024, "bf16", "some"),
+    (200, 33, 64, 48, "fp16", "some"),
     (2, 17, 5, 2050, "bf16", "some"),
 ]
 ID = [f"T{c[0]}k{c[1]}E{c[2]}H{c[3]}-{c[4]}-{c[5]}" for c in CASES]
@@ -309,6 +312,7 @@ def test_front_end_refusals(cuda_dev):
             (lambda: _ops.moe_combine_weighted(p, y, w.double()), "topk_weights"),
             (lambda: _ops.moe_combine_weighted(p, y, w[:3]), "topk_weights"),
             (lambda: _ops.moe_combine_weighted(p, y, w, out=x.float()), "out must be"),
+            (lambda: _ops.moe_combine_weighted(p, y, w, out=y[2:6]), "overlap"),
             (lambda: _ops.moe_combine_weighted_grad(p, y, w, x.float()), "d_out"),
             (lambda: _ops.moe_combine_weighted_grad(p, y, w, x[:3]), "d_out"),
             (lambda: _ops.moe_route_grad(ids, w, w, 0), "positive"),

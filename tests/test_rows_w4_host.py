@@ -148,6 +148,9 @@ def test_w4_refusals():
     _bad(gemm(C=_p(257)), "aligned")
     _bad(gemm(size=L.ek_gemm_w4_workspace_bytes(1, 8, 64, 148) - 1), "workspace")
     _bad(gemm(ws=_p(264)), "workspace")
+    _bad(gemm(K=(1 << 28) + 1), "2^28")
+    _bad(gemm(N=1 << 24, K=1 << 13), "2^32 scales")
+    assert L.ek_gemm_w4_workspace_bytes(1, 8, (1 << 31) - 1, 148) == _ops._SIZE_MAX
     assert gemm(M=0, A=n) == _lib.EK_OK
     assert L.ek_gemm_w4_workspace_bytes(0, 8, 64, 148) == 0
     assert L.ek_gemm_w4_workspace_bytes(1, 8, 0, 148) == L.ek_gemm_w4_workspace_bytes(1, 8, 64, 0) == _ops._SIZE_MAX
@@ -165,6 +168,8 @@ def test_moe_w4_refusals():
 
     _bad(gate_up(E=0), "bad sizes")
     _bad(gate_up(E=1025), "bad sizes")
+    _bad(gate_up(H=(1 << 28) + 1, E=1), "bad sizes")
+    _bad(gate_up(E=1024, I=1 << 20, H=1 << 17), "2^32 scales")
     _bad(gate_up(x_rows=4), "do not match")
     _bad(gate_up(slots=_p(), topk=0), "do not match")
     _bad(gate_up(slots=_p(), topk=2), "do not match")

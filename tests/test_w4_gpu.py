@@ -212,7 +212,7 @@ MOE = [  # T, k, E, H, I, group, mins
     (1, 1, 1, 32, 32, 32, False), (1, 2, 8, 4096, 512, 128, False), (3, 2, 4, 200, 136, 64, True),
     (17, 8, 60, 512, 260, 32, False), (64, 8, 32, 1024, 256, 128, False), (40, 3, 5, 257, 65, 64, True),
     (300, 2, 4, 256, 384, 128, False), (33, 1, 300, 64, 96, 32, False), (700, 2, 6, 128, 192, 64, True),
-    (128, 8, 16, 136, 72, 32, False),
+    (128, 8, 16, 136, 72, 32, False), (1, 8, 8, 64, 14336, 128, False), (4, 2, 3, 14336, 40, 64, True),
 ]
 
 
@@ -378,6 +378,51 @@ def test_layer_in_a_graph(cuda_dev):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(held, _ops.fused_moe_w4(x, logits, qw, 2))
+
+
+def test_experts_with_many_choices(cuda_dev):
+    """More choices than a warp has lanes, each of many parts: the combine's list in pieces."""
+    T, k, E, H, I = 3, 40, 48, 64, 4096
+    x, ids, qw = _moe_setup((T, k, E, H, I, 128, False), cuda_dev)
+    ids[1, 3] = -1
+    w = torch.rand((T, k), device=cuda_dev)
+    p = _ops.moe_dispatch(x, ids, E)
+    got = _ops.moe_experts_w4(p, x, ids, w, qw)
+    y = _ops.moe_down_w4(p, _ops.moe_gate_up_w4(p, qw, dtype=torch.float32), qw, dtype=torch.float32)
+    kept = int(p["num_rows_padded"])
+    want = _ops.moe_combine_weighted(p, torch.where(torch.arange(T * k, device=cuda_dev)[:, None] < kept, y, 0.0), w)
+    assert torch.equal(want.to(BF), got)
+
+
+def test_results_written_over_their_inputs(cuda_dev):
+    """out may be the tokens themselves: they are read before it is written."""
+    qw = _integer_weight(256, 256, 64, True, BF, 6, cuda_dev)
+    for M in (1, 3, 16, 40):
+        x = torch.randint(-2, 3, (M, 256), device=cuda_dev).to(BF)
+        want = _ops.gemm_w4(x, qw)
+        assert _ops.gemm_w4(x, qw, out=x) is x and torch.equal(x, want)
+    x, _, qw = _moe_setup((40, 2, 8, 256, 128, 64, False), cuda_dev)
+    logits = torch.randn((40, 8), device=cuda_dev)
+    want = _ops.fused_moe_w4(x, logits, qw, 2)
+    assert torch.equal(_ops.fused_moe_w4(x, logits, qw, 2, out=x), want)
+
+
+def test_two_streams_at_once(cuda_dev):
+    """Calls in flight on two streams: each has its own workspace."""
+    qw = _integer_weight(2048, 1024, 64, True, BF, 7, cuda_dev)
+    xs = [torch.randint(-2, 3, (m, 1024), device=cuda_dev).to(BF) for m in (1, 16)]
+    layer = _moe_setup((24, 2, 8, 512, 256, 64, False), cuda_dev)
+    logits = torch.randn((24, 8), device=cuda_dev)
+    want = [_ops.gemm_w4(x, qw) for x in xs] + [_ops.fused_moe_w4(layer[0], logits, layer[2], 2)]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    for _ in range(20):
+        for s, out in zip(streams, got):
+            with torch.cuda.stream(s):
+                out.append([_ops.gemm_w4(x, qw) for x in xs] + [_ops.fused_moe_w4(layer[0], logits, layer[2], 2)])
+    torch.cuda.synchronize()
+    for out in got[0] + got[1]:
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
 def test_layer_empty_and_refusals(cuda_dev):
