@@ -242,6 +242,10 @@ def _stream_sms(dev: torch.device, stream: int) -> int:
     check(lib().ek_gctx_stream_sm_count(ctypes.c_void_p(stream), ctypes.byref(v)), "ek_gctx_stream_sm_count")
     if v.value > 0:
         return v.value
+    return _device_sms(dev)
+
+
+def _device_sms(dev: torch.device) -> int:
     idx = dev.index if dev.index is not None else torch.cuda.current_device()
     n = _DEV_SMS.get(idx)
     if n is None:
@@ -717,8 +721,8 @@ def moe_dispatch(x: torch.Tensor | None, topk_ids: torch.Tensor, num_experts: in
         x_perm = x.new_empty((n, H))
     L = lib()
     ints = int(L.ek_moe_permute_scratch_bytes(T, k, E)) // 4
-    sorted_slots, slot_rows, counts, num_rows, scratch = torch.empty(
-        2 * n + max(E, 0) + 1 + ints, dtype=torch.int32, device=dev).split_with_sizes([n, n, max(E, 0), 1, ints])
+    sorted_slots, slot_rows, counts, num_rows, scratch = topk_ids.new_empty(
+        2 * n + max(E, 0) + 1 + ints).split_with_sizes([n, n, max(E, 0), 1, ints])
     with _on_device(dev):
         check(L.ek_moe_dispatch(topk_ids.data_ptr(), T, k, E, _ptr(x), H, dt, sorted_slots.data_ptr(),
                                 slot_rows.data_ptr(), counts.data_ptr(), num_rows.data_ptr(), _ptr(x_perm),
@@ -849,17 +853,17 @@ def _check_w4(name: str, qw: dict, dtype: torch.dtype | None = None) -> tuple:
     if group not in W4_GROUPS or K < 1:
         raise RuntimeError(f"{name}: need K >= 1 and a group out of {W4_GROUPS}")
     *lead, width = codes.shape
+    lead, kind = tuple(lead), scales.dtype
     if codes.dtype != torch.uint8 or not lead or width != -(-K // 32) * 16:
         raise RuntimeError(f"{name}: codes must be uint8 [..., N, {-(-K // 32) * 16}]")
-    if scales.dtype not in _DTYPES or scales.shape != (*lead, -(-K // group)):
+    if kind not in _DTYPES or scales.shape != (*lead, -(-K // group)):
         raise RuntimeError(f"{name}: scales must be bf16 or fp16 [..., N, {-(-K // group)}]")
-    if dtype is not None and scales.dtype != dtype:
-        raise RuntimeError(f"{name}: scales must be {dtype}, got {scales.dtype}")
-    if mins is not None and (mins.dtype != scales.dtype or mins.shape != scales.shape or not mins.is_contiguous()):
+    if dtype is not None and kind != dtype:
+        raise RuntimeError(f"{name}: scales must be {dtype}, got {kind}")
+    if mins is not None and (mins.dtype != kind or mins.shape != scales.shape or not mins.is_contiguous()):
         raise RuntimeError(f"{name}: mins must match the scales")
-    _contig(name, codes)
-    _contig(name, scales)
-    lead = tuple(lead)
+    if not (codes.is_contiguous() and scales.is_contiguous()):
+        raise RuntimeError(f"{name}: codes and scales must be contiguous")
     return codes, scales, mins, lead, K, group
 
 
@@ -889,27 +893,35 @@ def gemm_w4(a: torch.Tensor, qw: dict, out: torch.Tensor | None = None, num_sms:
     _contig("a", a)
     M, N = a.shape[0], lead[0]
     if out is None:
-        out = torch.empty((M, N), device=dev, dtype=a.dtype)
+        out = a.new_empty((M, N))
     elif out.shape != (M, N) or out.dtype != a.dtype or not out.is_contiguous():
         raise RuntimeError("out must be a contiguous [M, N] tensor of the input dtype")
     if M == 0 or N == 0:
         return out
     L = lib()
-    stream = current_stream_handle(dev)
-    sms = int(num_sms) if num_sms else _stream_sms(dev, stream)
-    ws = _scratch(L.ek_gemm_w4_workspace_bytes(M, N, K, sms), dev)
+    stream, sms = current_stream_handle(dev), int(num_sms or 0)
+    ws = _scratch(L.ek_gemm_w4_workspace_bytes(M, N, K, _most_sms(dev, sms)), codes)
     with _on_device(dev):
         check(L.ek_gemm_w4(a.data_ptr(), codes.data_ptr(), scales.data_ptr(), _ptr(mins), out.data_ptr(), M, N, K,
                            group, _DTYPES[a.dtype], sms, ws.data_ptr(), ws.numel(), stream), "ek_gemm_w4")
     return out
 
 
-def _scratch(nbytes: int, dev: torch.device) -> torch.Tensor:
-    """Workspace of one call, from torch's allocator: nothing in it outlives the
-    call, and a captured graph gets its own."""
+def _most_sms(dev: torch.device, num_sms: int) -> int:
+    """SMs to size a workspace for: num_sms, or with 0 (the library then asks the
+    stream for its partition's) all of the device, which no partition exceeds."""
+    if num_sms:
+        return num_sms
+    n = _DEV_SMS.get(dev.index)
+    return n if n is not None else _device_sms(dev)
+
+
+def _scratch(nbytes: int, codes: torch.Tensor) -> torch.Tensor:
+    """Workspace of one call beside the codes (bytes too), from torch's allocator:
+    nothing in it outlives the call, and a captured graph gets its own."""
     if nbytes == _SIZE_MAX:
         check(_lib.EK_ERR_INVALID, "workspace size")
-    return torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    return codes.new_empty(nbytes)
 
 
 def quant_moe_weights_w4(w1: torch.Tensor, w2: torch.Tensor, w3: torch.Tensor, group: int = 128,
@@ -958,9 +970,8 @@ def moe_gate_up_w4(perm: dict, qw: dict, x: torch.Tensor | None = None, num_sms:
         raise RuntimeError("gate_up_w4: shape mismatch")
     act = torch.empty((rows, I), dtype=dtype, device=dev)
     L = lib()
-    stream = current_stream_handle(dev)
-    sms = int(num_sms) if num_sms else _stream_sms(dev, stream)
-    ws = _scratch(L.ek_moe_w4_workspace_bytes(x_rows, rows, E, H, I, sms), dev)
+    stream, sms = current_stream_handle(dev), int(num_sms or 0)
+    ws = _scratch(L.ek_moe_w4_workspace_bytes(x_rows, rows, E, H, I, _most_sms(dev, sms)), c1)
     with _on_device(dev):
         check(L.ek_moe_gate_up_w4(src.data_ptr(), x_rows, None if x is None else perm["sorted_slots"].data_ptr(),
                                   1 if x is None else perm["topk"], c1.data_ptr(), s1.data_ptr(), _ptr(m1),
@@ -985,9 +996,8 @@ def moe_down_w4(perm: dict, act: torch.Tensor, qw: dict, num_sms: int | None = N
         raise RuntimeError("down_w4: shape mismatch")
     y = torch.empty((rows, H), dtype=dtype, device=dev)
     L = lib()
-    stream = current_stream_handle(dev)
-    sms = int(num_sms) if num_sms else _stream_sms(dev, stream)
-    ws = _scratch(L.ek_moe_w4_workspace_bytes(0, rows, E, H, I, sms), dev)
+    stream, sms = current_stream_handle(dev), int(num_sms or 0)
+    ws = _scratch(L.ek_moe_w4_workspace_bytes(0, rows, E, H, I, _most_sms(dev, sms)), c2)
     with _on_device(dev):
         check(L.ek_moe_down_w4(act.data_ptr(), _ACT_DTYPES[act.dtype], c2.data_ptr(), s2.data_ptr(), _ptr(m2),
                                perm["expert_counts"].data_ptr(), y.data_ptr(), _ACT_DTYPES[dtype], rows, E, H, I, group,
@@ -1020,9 +1030,8 @@ def moe_experts_w4(perm: dict, x: torch.Tensor, topk_ids: torch.Tensor, topk_wei
     if T == 0:
         return out
     L = lib()
-    stream = current_stream_handle(dev)
-    sms = int(num_sms) if num_sms else _stream_sms(dev, stream)
-    ws = _scratch(L.ek_moe_w4_workspace_bytes(T, T * k, E, H, I, sms), dev)
+    stream, sms = current_stream_handle(dev), int(num_sms or 0)
+    ws = _scratch(L.ek_moe_w4_workspace_bytes(T, T * k, E, H, I, _most_sms(dev, sms)), c1)
     with _on_device(dev):
         check(L.ek_moe_experts_w4(x.data_ptr(), T, k, topk_ids.data_ptr(), topk_weights.data_ptr(),
                                   perm["sorted_slots"].data_ptr(), slot_rows.data_ptr(),
@@ -1055,9 +1064,8 @@ def fused_moe_w4(hidden_states: torch.Tensor, gate_logits: torch.Tensor, qw: dic
         if out.shape != hidden_states.shape:
             raise RuntimeError("out must be a [T, H] tensor")
     L, k = lib(), int(topk)
-    stream = current_stream_handle(dev)
-    sms = int(num_sms) if num_sms else _stream_sms(dev, stream)
-    ws = _scratch(L.ek_fused_moe_w4_workspace_bytes(T, k, E, H, I, sms), dev)
+    stream, sms = current_stream_handle(dev), int(num_sms or 0)
+    ws = _scratch(L.ek_fused_moe_w4_workspace_bytes(T, k, E, H, I, _most_sms(dev, sms)), c1)
     with _on_device(dev):
         check(L.ek_fused_moe_w4(hidden_states.data_ptr(), gate_logits.data_ptr(), T, k, c1.data_ptr(), s1.data_ptr(),
                                 _ptr(m1), c3.data_ptr(), s3.data_ptr(), _ptr(m3), c2.data_ptr(), s2.data_ptr(),
