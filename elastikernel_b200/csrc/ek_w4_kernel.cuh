@@ -463,7 +463,12 @@ __global__ void __launch_bounds__(kThreads, 2)
     uint32_t parity = 1;
     for (int i = 0; i < n_units; ++i) {
       if (i >= ahead) {
-        if (!mbar_wait(&s_empty[slot], parity, &s_abort)) break;
+        if (!mbar_wait(&s_empty[slot], parity, &s_abort)) {
+          // given up: let the copies in flight land (the last kStages stages', all issued) before the CTA ends
+          int never = 0;
+          for (int j = i - kStages; j < i; ++j) mbar_wait(&s_full[j % kStages], j / kStages & 1, &never);
+          break;
+        }
         copy_codes(slot);
       }
       if constexpr (S::kMakes) {
