@@ -21,15 +21,16 @@ def _ptr(t: torch.Tensor | None) -> int | None:
 
 
 def _require_cuda(*ts: torch.Tensor) -> torch.device:
-    dev = None
+    dev, index = None, -1
     for t in ts:
         if t is None:
             continue
-        if not t.is_cuda:
+        i = t.get_device()  # an int: cheaper than building and comparing devices
+        if i < 0 or (dev is None and not t.is_cuda):
             raise RuntimeError("elastikernel_b200 operators take CUDA tensors only (no CPU path)")
         if dev is None:
-            dev = t.device
-        elif t.device != dev:
+            dev, index = t.device, i
+        elif i != index or not t.is_cuda:
             raise RuntimeError(f"tensors on different devices: {dev} vs {t.device}")
     return dev
 
@@ -665,21 +666,23 @@ _ROW_DTYPES = {torch.bfloat16: _lib.EK_DTYPE_BF16, torch.float16: _lib.EK_DTYPE_
 
 def _check_rows(name: str, t: torch.Tensor, rows: int | None = None) -> int:
     """dtype code of a contiguous bf16/fp16/fp32 row matrix (of `rows` rows)."""
-    dt = _ROW_DTYPES.get(t.dtype)
-    if dt is None or t.dim() != 2:
+    dt, shape = _ROW_DTYPES.get(t.dtype), t.shape
+    if dt is None or len(shape) != 2:
         raise RuntimeError(f"{name} must be a 2-D bf16, fp16 or fp32 tensor")
-    if rows is not None and t.shape[0] != rows:
-        raise RuntimeError(f"{name} must have {rows} rows, got {t.shape[0]}")
-    if t.shape[1] == 0:
+    if rows is not None and shape[0] != rows:
+        raise RuntimeError(f"{name} must have {rows} rows, got {shape[0]}")
+    if shape[1] == 0:
         raise RuntimeError(f"{name} has rows of no elements")
-    _contig(name, t)
+    if not t.is_contiguous():
+        raise RuntimeError(f"{name} must be contiguous")
     return dt
 
 
 def _check_slots(name: str, t: torch.Tensor, T: int, k: int, dtype: torch.dtype) -> None:
-    if t.dtype != dtype or t.shape != (T, k):
+    if t.dtype is not dtype or t.shape != (T, k):
         raise RuntimeError(f"{name} must be a {dtype} tensor of shape {(T, k)}")
-    _contig(name, t)
+    if not t.is_contiguous():
+        raise RuntimeError(f"{name} must be contiguous")
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
