@@ -523,17 +523,11 @@ __global__ void __launch_bounds__(kThreads, 2)
   const uint32_t lm = base + (set_row + lrow) * 128 + ((lpiece ^ (lrow & 7)) << 4);
 
   TokenTile tl = open_tile<kMode, S::kTokens>(p, y, s_end, s_row);
-  // Scales run one stage ahead: first scale of rows g, g + 8 of each set.
-  uint32_t srow[2][2];
-  auto open_scales = [&](int e, int ft) {
-#pragma unroll
-    for (int s = 0; s < 2; ++s)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int r = ft * kFeatures + set_row + (kMode == kGateUp ? 0 : 16 * s) + g + 8 * h;
-        srow[s][h] = (uint32_t)(e * p.N + min(r, p.N - 1)) * (uint32_t)G;
-      }
-  };
+  // Scales run one stage ahead. row0: this lane's first weight row, counted over
+  // all experts; rows past the last are read as the last (nothing of them is used).
+  const uint32_t last_row = (uint32_t)(kMode == kDense ? 1 : p.E) * (uint32_t)p.N - 1;
+  uint32_t row0 = 0;
+  auto open_scales = [&](int e, int ft) { row0 = (uint32_t)(e * p.N + ft * kFeatures + set_row + g); };
   uint32_t s_next[2][kSR], m_next[2][kSR];  // of rows g (low half) and g + 8
   auto load_scales = [&](int stage) {
 #pragma unroll
@@ -542,8 +536,10 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         const Scales<T>& w = p.w[kMode == kGateUp ? s : 0];
-        s_next[s][i] = pack2(__ldg(w.s + (srow[s][0] + gi)), __ldg(w.s + (srow[s][1] + gi)));
-        if constexpr (S::kMin) m_next[s][i] = pack2(__ldg(w.m + (srow[s][0] + gi)), __ldg(w.m + (srow[s][1] + gi)));
+        const uint32_t r = row0 + (kMode == kGateUp ? 0 : 16 * s);
+        const uint32_t lo = min(r, last_row) * (uint32_t)G + gi, hi = min(r + 8, last_row) * (uint32_t)G + gi;
+        s_next[s][i] = pack2(__ldg(w.s + lo), __ldg(w.s + hi));
+        if constexpr (S::kMin) m_next[s][i] = pack2(__ldg(w.m + lo), __ldg(w.m + hi));
       }
     }
   };
@@ -560,16 +556,12 @@ __global__ void __launch_bounds__(kThreads, 2)
   int slot = 0;
   uint32_t parity = 0;
   for (; n_units > 0; --n_units) {
-    // what comes after this stage: the next one of the tile, or the next tile's first
+    // What comes after this stage: the next one of the tile, or the next tile's
+    // first (found again at the end, so that it takes no registers meanwhile).
     const bool tile_end = st + 1 == nst;
-    int next_f = f, next_y = y;
-    TokenTile next_tl = tl;
     if (tile_end && n_units > 1) {
-      if (++next_f == p.feature_tiles) {
-        next_f = 0;
-        next_tl = open_tile<kMode, S::kTokens>(p, ++next_y, s_end, s_row);
-      }
-      open_scales(next_tl.e, next_f);
+      const bool wrap = f + 1 == p.feature_tiles;
+      open_scales(wrap ? open_tile<kMode, S::kTokens>(p, y + 1, s_end, s_row).e : tl.e, wrap ? 0 : f + 1);
     }
     uint32_t s_cur[2][kSR], m_cur[2][kSR];
 #pragma unroll
@@ -673,10 +665,15 @@ __global__ void __launch_bounds__(kThreads, 2)
           }
         }
     }
-    st = tile_end ? 0 : st + 1;
-    f = next_f;
-    y = next_y;
-    tl = next_tl;
+    if (!tile_end) {
+      ++st;
+    } else if (n_units > 1) {
+      st = 0;
+      if (++f == p.feature_tiles) {
+        f = 0;
+        tl = open_tile<kMode, S::kTokens>(p, ++y, s_end, s_row);
+      }
+    }
   }
 }
 
