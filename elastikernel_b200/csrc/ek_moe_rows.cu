@@ -238,7 +238,10 @@ __device__ __forceinline__ Unit unit_of(long long u, int runs) {
 template <int kRun>
 __host__ __device__ inline int runs_per_row(int nvec) { return (nvec + 32 * kRun - 1) / (32 * kRun); }
 
-constexpr int kCopyRun = 4;
+// Vectors of a row per lane and unit, more where they are narrow (8192 tokens, 1111
+// wide: fp32 and 8 choices 67 us against 71 with four, bf16 and 2 choices 18 against 22).
+template <class Raw>
+constexpr int kCopyRun = sizeof(Raw) < 16 ? 8 : 4;
 
 // Copy x[t] to the rows of token t; row_of(s): the row of slot s (negative:
 // dropped). Neighbouring units go to different CTAs, so that few of them still
@@ -246,13 +249,13 @@ constexpr int kCopyRun = 4;
 template <class Raw, class RowOf>
 __device__ __forceinline__ void copy_rows(const Raw* __restrict__ x, int T, int k, int nvec, const RowOf& row_of,
                                           Raw* __restrict__ rows) {
-  const int lane = threadIdx.x & 31, runs = runs_per_row<kCopyRun>(nvec);
+  const int lane = threadIdx.x & 31, runs = runs_per_row<kCopyRun<Raw>>(nvec);
   const long long warps = ((long long)gridDim.x * blockDim.x) >> 5, units = (long long)T * runs;
   for (long long u = (long long)(threadIdx.x >> 5) * gridDim.x + blockIdx.x; u < units; u += warps) {
-    const Unit w = unit_of<kCopyRun>(u, runs);
-    Raw v[kCopyRun];
+    const Unit w = unit_of<kCopyRun<Raw>>(u, runs);
+    Raw v[kCopyRun<Raw>];
 #pragma unroll
-    for (int i = 0; i < kCopyRun; ++i)
+    for (int i = 0; i < kCopyRun<Raw>; ++i)
       if (w.c0 + 32 * i < nvec) v[i] = __ldg(x + (long long)w.t * nvec + w.c0 + 32 * i);
     for (int j0 = 0; j0 < k; j0 += 32) {
       const int mine = j0 + lane < k ? row_of((long long)w.t * k + j0 + lane) : -1;
@@ -262,7 +265,7 @@ __device__ __forceinline__ void copy_rows(const Raw* __restrict__ x, int T, int 
         if (r < 0) continue;
         Raw* dst = rows + (long long)r * nvec + w.c0;
 #pragma unroll
-        for (int i = 0; i < kCopyRun; ++i)
+        for (int i = 0; i < kCopyRun<Raw>; ++i)
           if (w.c0 + 32 * i < nvec) dst[32 * i] = v[i];
       }
     }
@@ -318,17 +321,24 @@ __global__ void __launch_bounds__(kOrderThreads)
   zero_tail(rows, kept, n, nvec);
 }
 
+// Vectors of each row that a lane of the sums has in flight; twice as many where
+// the rows' alignment leaves them narrow. Measured, one against two for up to 4
+// choices: 4096 tokens, 3 choices, 4096 fp32 54 against 47 us; and for 4- and 2-byte
+// vectors, without and with the doubling: 8192 tokens, 8 choices, 1111 fp32 104
+// against 87 us, 2 choices, 1111 bf16 28 against 19 (four times as many: 141 and 21).
+template <int V, int kK>
+constexpr int kSumRun = (kK <= 4 ? 2 : 1) * (V < 16 ? 2 : 1);
+
 // out[t] = sum_j w[t,j] rows[slot_rows[t,j]] (w = 1 without weights), fp32 sum
 // in j order, rounded once. kK: rows whose loads are in flight together (2, 4 or
-// 8, the least that holds the choices; a lane holds kK vectors at a time, two of
-// each row for up to 2 choices).
+// 8, the least that holds the choices).
 template <class T, int V, bool kWeighted, int kK>
 __global__ void __launch_bounds__(256)
     sum_rows_kernel(const typename Vec<V>::type* __restrict__ rows, const int* __restrict__ slot_rows,
                     const float* __restrict__ weights, int T_tokens, int k, int n_rows, int nvec,
                     typename Vec<V>::type* __restrict__ out) {
   using E = Elems<T, V>;
-  constexpr int kRun = kK <= 2 ? 2 : 1;
+  constexpr int kRun = kSumRun<V, kK>;
   const int lane = threadIdx.x & 31, runs = runs_per_row<kRun>(nvec);
   const long long warps = ((long long)gridDim.x * blockDim.x) >> 5, units = (long long)T_tokens * runs;
   for (long long u = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5; u < units; u += warps) {
@@ -406,25 +416,36 @@ __global__ void __launch_bounds__(128)
         dot[j] = 0.f;
       }
       if (t < T_tokens) {
-        for (int c = at; c < nvec; c += kTpt) {
-          typename E::Raw y[kK];
+        // vectors of each row in flight per lane, two where they are narrow (8192
+        // tokens, 8 choices, 1111 fp32: 159 us against 176; 2 choices, bf16: 21 against 30)
+        constexpr int kU = V < 16 ? 2 : 1;
+        for (int c0 = at; c0 < nvec; c0 += kTpt * kU) {
+          typename E::Raw y[kU][kK], g[kU];
 #pragma unroll
-          for (int j = 0; j < kK; ++j)
-            if (r[j] >= 0) y[j] = __ldg(rows + (long long)r[j] * nvec + c);
-          float d[E::N];
-          E::unpack(__ldg(d_out + t * nvec + c), d);
+          for (int u = 0; u < kU; ++u) {
+            const int c = c0 + u * kTpt;
 #pragma unroll
-          for (int j = 0; j < kK; ++j)
-            if (r[j] >= 0) {
-              float f[E::N];
-              E::unpack(y[j], f);
+            for (int j = 0; j < kK; ++j) y[u][j] = load_if(rows + (long long)r[j] * nvec + c, r[j] >= 0 && c < nvec);
+            g[u] = load_if(d_out + t * nvec + c, c < nvec);
+          }
 #pragma unroll
-              for (int e = 0; e < E::N; ++e) {
-                dot[j] = fmaf(d[e], f[e], dot[j]);
-                f[e] = w[j] * d[e];
+          for (int u = 0; u < kU; ++u) {
+            const int c = c0 + u * kTpt;
+            float d[E::N];
+            E::unpack(g[u], d);
+#pragma unroll
+            for (int j = 0; j < kK; ++j)
+              if (r[j] >= 0 && c < nvec) {
+                float f[E::N];
+                E::unpack(y[u][j], f);
+#pragma unroll
+                for (int e = 0; e < E::N; ++e) {
+                  dot[j] = fmaf(d[e], f[e], dot[j]);
+                  f[e] = w[j] * d[e];
+                }
+                d_rows[(long long)r[j] * nvec + c] = E::pack(f);
               }
-              d_rows[(long long)r[j] * nvec + c] = E::pack(f);
-            }
+          }
         }
       }
 #pragma unroll
@@ -561,21 +582,20 @@ struct Rows {  // what the sums take
   cudaStream_t s;
 };
 
+template <class T, int V, bool kWeighted, int kK>
+int launch_sum_k(const Rows& a, void* dst) {
+  const int nvec = a.H * (int)sizeof(T) / V;
+  sum_rows_kernel<T, V, kWeighted, kK><<<rows_grid((long long)a.T * runs_per_row<kSumRun<V, kK>>(nvec) * 32), 256, 0, a.s>>>(
+      static_cast<const typename Vec<V>::type*>(a.rows), a.slot_rows, a.w, a.T, a.k, a.n_rows, nvec,
+      static_cast<typename Vec<V>::type*>(dst));
+  return check_cuda(cudaGetLastError(), "sum rows launch");
+}
+
 template <class T, int V, bool kWeighted>
 int launch_sum(const Rows& a, void* dst) {
-  const int nvec = a.H * (int)sizeof(T) / V;
-  const auto* rows = static_cast<const typename Vec<V>::type*>(a.rows);
-  auto* out = static_cast<typename Vec<V>::type*>(dst);
-  if (a.k <= 2)
-    sum_rows_kernel<T, V, kWeighted, 2><<<rows_grid((long long)a.T * runs_per_row<2>(nvec) * 32), 256, 0, a.s>>>(
-        rows, a.slot_rows, a.w, a.T, a.k, a.n_rows, nvec, out);
-  else if (a.k <= 4)
-    sum_rows_kernel<T, V, kWeighted, 4><<<rows_grid((long long)a.T * runs_per_row<1>(nvec) * 32), 256, 0, a.s>>>(
-        rows, a.slot_rows, a.w, a.T, a.k, a.n_rows, nvec, out);
-  else
-    sum_rows_kernel<T, V, kWeighted, 8><<<rows_grid((long long)a.T * runs_per_row<1>(nvec) * 32), 256, 0, a.s>>>(
-        rows, a.slot_rows, a.w, a.T, a.k, a.n_rows, nvec, out);
-  return check_cuda(cudaGetLastError(), "sum rows launch");
+  if (a.k <= 2) return launch_sum_k<T, V, kWeighted, 2>(a, dst);
+  if (a.k <= 4) return launch_sum_k<T, V, kWeighted, 4>(a, dst);
+  return launch_sum_k<T, V, kWeighted, 8>(a, dst);
 }
 
 template <class T, bool kWeighted>
@@ -658,7 +678,7 @@ int launch_small(const Dispatch& d, size_t row_bytes) {
     attr_done[dev] = true;
   }
   // the units of the copy over up to a CTA per SM
-  const int grid = d.x ? std::max(1, std::min(148, d.T * runs_per_row<kCopyRun>(nvec))) : 1;
+  const int grid = d.x ? std::max(1, std::min(148, d.T * runs_per_row<kCopyRun<Raw>>(nvec))) : 1;
   dispatch_small_kernel<V><<<grid, kOrderThreads, smem, d.s>>>(d.ids, d.T, d.k, d.E, static_cast<const Raw*>(d.x), nvec,
                                                              d.sorted_slots, d.slot_rows, d.counts, d.num_rows,
                                                              static_cast<Raw*>(d.rows));
@@ -669,7 +689,7 @@ template <int V>
 int launch_copy(const Dispatch& d, size_t row_bytes) {
   using Raw = typename Vec<V>::type;
   const int nvec = (int)(row_bytes / V);
-  dispatch_copy_kernel<V><<<rows_grid((long long)d.T * runs_per_row<kCopyRun>(nvec) * 32), 256, 0, d.s>>>(
+  dispatch_copy_kernel<V><<<rows_grid((long long)d.T * runs_per_row<kCopyRun<Raw>>(nvec) * 32), 256, 0, d.s>>>(
       static_cast<const Raw*>(d.x), d.slot_rows, d.num_rows, d.T, d.k, nvec, static_cast<Raw*>(d.rows));
   return check_cuda(cudaGetLastError(), "dispatch copy launch");
 }
