@@ -775,7 +775,7 @@ __global__ void __launch_bounds__(kRows) finish_kernel(const __grid_constant__ P
 
 // The activations of a gate/up product straight into the tokens of the down
 // projection: a warp per packed row and run of 256 features (two tiles). Bound by
-// latency: 6 us alone for one token, 10 us for 512 rows of 2048.
+// latency: 7 us alone for one token, 9 us for 512 rows of 2048.
 template <int TOK, class T>
 __global__ void __launch_bounds__(256) act_tokens_kernel(const __grid_constant__ Params<T> p, int grid, int group, Tokens act) {
   extern __shared__ int s_index[];
@@ -803,9 +803,10 @@ __global__ void __launch_bounds__(256) act_tokens_kernel(const __grid_constant__
 
 // out[t] = sum_j w[t, j] y[row of slot (t, j)] from the parts of the down
 // projection, fp32 in j order, rounded once. A CTA per token and 256 features; bound
-// by latency.
+// by latency (64 tokens, 8 choices, 7168 wide: 17 us alone for 15 MB of parts), so
+// six CTAs an SM (four or eight: 1 % of the layer more).
 template <int TOK, class T>
-__global__ void __launch_bounds__(kRows, 4)
+__global__ void __launch_bounds__(kRows, 6)
     combine_parts_kernel(const __grid_constant__ Params<T> p, int grid, const int* __restrict__ slot_rows,
                          const int* __restrict__ ids, const float* __restrict__ weights, int tokens, int topk,
                          T* __restrict__ out) {
