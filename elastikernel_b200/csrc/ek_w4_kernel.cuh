@@ -421,7 +421,12 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int np = pieces(p.K), nst = (np + kStagePieces - 1) / kStagePieces;
   const long long U = (long long)s_y * p.feature_tiles * nst;
   const Runs run{U, (int)min((long long)gridDim.x, U), nst};
-  if (blockIdx.x >= run.ctas) return;
+  if (blockIdx.x >= run.ctas) {
+    // Not before its predecessor either: where no CTA has a stage (every slot
+    // dropped), this grid's end must still mean that the tokens are written.
+    griddep_wait();
+    return;
+  }
   const long long u0 = run.begin(blockIdx.x), u1 = run.begin(blockIdx.x + 1);
   int tile = (int)(u0 / nst), st = (int)(u0 - (long long)tile * nst);
   int y = tile / p.feature_tiles, f = tile - y * p.feature_tiles;

@@ -439,3 +439,45 @@ def test_layer_empty_and_refusals(cuda_dev):
         with pytest.raises(RuntimeError, match=text):
             call()
     assert _lib.device_status(0) == 0
+
+
+@pytest.mark.parametrize("captured", [False, True])
+@pytest.mark.parametrize("stage", ["gate_up", "down", "experts"])
+def test_nothing_is_written_after_an_empty_product(stage, captured, cuda_dev, monkeypatch):
+    """Every slot dropped: what follows on the stream still comes after the launch
+    that writes the tokens, so the workspace may be used again at once."""
+    T, k, E, H, I = 4096, 2, 4, 2048, 2048
+    w = torch.randn((E, I, H), device=cuda_dev, dtype=BF) * 0.02
+    qw = _ops.quant_moe_weights_w4(w, w, w, group=128)
+    x = torch.randn((T, H), device=cuda_dev).to(BF)
+    act = torch.randn((T * k, I), device=cuda_dev).to(BF)
+    ids = torch.full((T, k), -1, dtype=torch.int32, device=cuda_dev)
+    wts = torch.rand((T, k), device=cuda_dev)
+    perm = _ops.moe_dispatch(None, ids, E)
+    buf = torch.empty(256 << 20, dtype=torch.uint8, device=cuda_dev)
+    monkeypatch.setattr(_ops, "_scratch", lambda nbytes, codes: buf[:nbytes])
+    bad = torch.zeros(20, dtype=torch.int64, device=cuda_dev)
+
+    def once(i):
+        if stage == "gate_up":
+            _ops.moe_gate_up_w4(perm, qw, x=x)
+        elif stage == "down":
+            _ops.moe_down_w4(perm, act, qw)
+        else:
+            assert _ops.moe_experts_w4(perm, x, ids, wts, qw).shape == (T, H)
+        buf.fill_(0x5A)
+        bad[i] = (buf != 0x5A).sum()
+
+    once(0)
+    if captured:
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for i in range(20):
+                once(i)
+        graph.replay()
+    else:
+        for i in range(20):
+            once(i)
+    torch.cuda.synchronize()
+    assert not bad.any()
