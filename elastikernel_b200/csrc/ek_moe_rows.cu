@@ -503,9 +503,9 @@ __global__ void __launch_bounds__(256)
     const long long first = u * per * E, n = min((long long)per, T - u * per) * E;
     if (wide) {
       float4* dst = reinterpret_cast<float4*>(d_logits + first);
-      for (int i = lane; i < n / 4; i += 32) dst[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (long long i = lane; i < n / 4; i += 32) dst[i] = make_float4(0.f, 0.f, 0.f, 0.f);
     } else {
-      for (int i = lane; i < n; i += 32) d_logits[first + i] = 0.f;
+      for (long long i = lane; i < n; i += 32) d_logits[first + i] = 0.f;
     }
     float mean = w * d;
     for (int o = kp >> 1; o; o >>= 1) mean += __shfl_xor_sync(0xffffffffu, mean, o);
@@ -789,6 +789,7 @@ int ek_moe_route_grad(const int* topk_ids, const float* topk_weights, const floa
                       float* d_logits, void* stream) {
   clear_error();
   if (T < 0 || E < 1 || topk < 1) return set_error(EK_ERR_INVALID, "route gradient: bad sizes (T=%d E=%d k=%d)", T, E, topk);
+  if (E > (1 << 30)) return set_error(EK_ERR_INVALID, "route gradient: more than 2^30 experts (%d)", E);
   if (T == 0) return EK_OK;
   if (!topk_ids || !topk_weights || !d_weights || !d_logits)
     return set_error(EK_ERR_INVALID, "route gradient: null pointer");

@@ -320,3 +320,14 @@ def test_front_end_refusals(cuda_dev):
             (lambda: _ops.moe_dispatch_grad(_ops.moe_permute(ids, 2, block_m=1), y), "slot_rows")]:
         with pytest.raises(RuntimeError, match=text):
             call()
+
+
+def test_route_grad_of_a_warp_past_2_31_logits(cuda_dev):
+    """A warp's 16 tokens have more than 2^31 logits (9 GB in all)."""
+    T, E = 17, (1 << 27) + 1
+    ids = torch.tensor([[E - 1, 3]], dtype=torch.int32, device=cuda_dev).expand(T, 2).contiguous()
+    w = torch.full((T, 2), 0.5, device=cuda_dev)
+    d = torch.tensor([[1.0, 3.0]], device=cuda_dev).expand(T, 2).contiguous()
+    got = _ops.moe_route_grad(ids, w, d, E)
+    assert (got[:, E - 1] == -0.5).all() and (got[:, 3] == 0.5).all()
+    assert int(torch.count_nonzero(got)) == 2 * T

@@ -259,3 +259,10 @@ def test_front_end_checks_the_weight(change, text):
     qw.update(change)
     with pytest.raises(RuntimeError, match=text):
         _ops.gemm_w4(torch.zeros((1, 64), dtype=torch.bfloat16), qw)
+
+
+def test_route_gradient_refuses_more_experts_than_its_counters_hold():
+    f = lib().ek_moe_route_grad
+    _bad(f(_p(), _p(), _p(), 4, (1 << 30) + 1, 2, _p(), None), "2^30")
+    _bad(f(_p(), _p(), _p(), 4, (1 << 31) - 1, 40, _p(), None), "2^30")
+    assert f(None, None, None, 0, 1 << 30, 2, None, None) == _lib.EK_OK
