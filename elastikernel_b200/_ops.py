@@ -356,10 +356,24 @@ def _check_bf16(name: str, t: torch.Tensor) -> None:
     _contig(name, t)
 
 
+def _check_padded(perm: dict) -> None:
+    if perm["block_expert"] is None:
+        raise RuntimeError("the padded GEMMs take a moe_permute layout (moe_dispatch's is packed)")
+
+
+def _slot_rows_out(perm: dict, H: int, dev: torch.device) -> torch.Tensor:
+    """[T*k, H] bf16 for a product that scatters its rows to their slots. It writes
+    the kept slots alone, so the others' rows are cleared where an order may
+    have dropped some."""
+    make = torch.empty if perm.get("slot_rows") is None else torch.zeros
+    return make((perm["T"] * perm["topk"], H), dtype=torch.bfloat16, device=dev)
+
+
 def moe_gate_up(perm: dict, w1: torch.Tensor, w3: torch.Tensor, num_sms: int | None = None,
                 force_bn: int = 0) -> torch.Tensor:
     """act[r] = silu(x_perm[r] . w1[e]) * (x_perm[r] . w3[e]) over the padded rows
     (a layout padded to 256 rows per expert runs on CTA pairs)."""
+    _check_padded(perm)
     x_perm = perm["x_perm"]
     dev = _require_cuda(x_perm, w1, w3)
     for n, t in (("x_perm", x_perm), ("w1", w1), ("w3", w3)):
@@ -381,6 +395,7 @@ def moe_gate_up(perm: dict, w1: torch.Tensor, w3: torch.Tensor, num_sms: int | N
 def moe_down(perm: dict, act: torch.Tensor, w2: torch.Tensor, topk_weights: torch.Tensor,
              num_sms: int | None = None, force_bn: int = 0) -> torch.Tensor:
     """y[s] = topk_weight[s] * (act[r] @ w2[e]^T) for the slot s of each used row r."""
+    _check_padded(perm)
     dev = _require_cuda(act, w2, topk_weights)
     _check_bf16("act", act)
     _check_bf16("w2", w2)
@@ -434,8 +449,9 @@ def _packed_workspace(rows: int, H: int, I: int, dev: torch.device) -> tuple[tor
 def moe_down_packed(perm: dict, act: torch.Tensor, w2: torch.Tensor, topk_weights: torch.Tensor,
                     num_sms: int | None = None, tok_tile: int = 0, pair: int = -1,
                     ksplit: bool = True) -> torch.Tensor:
-    """Swapped-operand down projection with the routing weight, scattered to slots.
-    ksplit=False withholds the workspace, so K is never split."""
+    """Swapped-operand down projection with the routing weight, scattered to slots
+    (a slot that a moe_dispatch order dropped gets zeros). ksplit=False
+    withholds the workspace, so K is never split."""
     dev = _require_cuda(act, w2, topk_weights)
     _check_bf16("act", act)
     _check_bf16("w2", w2)
@@ -444,7 +460,7 @@ def moe_down_packed(perm: dict, act: torch.Tensor, w2: torch.Tensor, topk_weight
     T, k = perm["T"], perm["topk"]
     if act.shape[1] != I or E != perm["E"] or topk_weights.numel() != T * k or perm["block_m"] != 1:
         raise RuntimeError("down_packed: shape mismatch")
-    y = torch.empty((T * k, H), dtype=torch.bfloat16, device=dev)
+    y = _slot_rows_out(perm, H, dev)
     ws, nb = _packed_workspace(perm["max_rows"], H, I, dev) if ksplit else (None, 0)
     with _on_device(dev):
         check(lib().ek_moe_down_packed(act.data_ptr(), w2.data_ptr(), perm["expert_counts"].data_ptr(),
@@ -523,14 +539,15 @@ def moe_gate_up_fp8bs(perm: dict, xq: torch.Tensor, xs: torch.Tensor, qw: dict, 
 
 def moe_down_fp8bs(perm: dict, aq: torch.Tensor, as_: torch.Tensor, qw: dict, topk_weights: torch.Tensor,
                    num_sms: int | None = None, tok_tile: int = 0, pair: int = -1, mx: bool | None = None) -> torch.Tensor:
-    """Block-scaled FP8 down projection with the routing weight, scattered to slots (bf16 [T*k, H]).
+    """Block-scaled FP8 down projection with the routing weight, scattered to slots (bf16 [T*k, H];
+    zeros for a slot that a moe_dispatch order dropped).
     as_: K-block-major act scales [I/128, rows]. mx as for moe_gate_up_fp8bs."""
     dev = _require_cuda(aq, as_, topk_weights)
     rows, E, H, I = perm["max_rows"], qw["E"], qw["H"], qw["I"]
     T, k = perm["T"], perm["topk"]
     if aq.shape != (rows, I) or as_.shape != (I // 128, rows) or topk_weights.numel() != T * k:
         raise RuntimeError("down_fp8bs: shape mismatch")
-    y = torch.empty((T * k, H), dtype=torch.bfloat16, device=dev)
+    y = _slot_rows_out(perm, H, dev)
     fn = lib().ek_moe_down_fp8mx if _mx(qw, mx) else lib().ek_moe_down_fp8bs
     with _on_device(dev):
         check(fn(aq.data_ptr(), as_.data_ptr(), qw["w2q"].data_ptr(), qw["w2s"].data_ptr(),

@@ -486,7 +486,10 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
         units += p.feat_tiles * ((c + BN - 1) / BN);
       }
       xt.start[p.num_experts] = acc;
-      const int S = swapped_ksplit(units, unit_step, p.k_blocks, p.tail_split);
+      // Slices are added slot by slot, so a scatter splits only where its rows are
+      // all the slots (an order may have dropped some).
+      const bool whole = Cfg::kEpi != kEpiScatterT || acc == p.num_slots;
+      const int S = whole ? swapped_ksplit(units, unit_step, p.k_blocks, p.tail_split) : 1;
       units = 0;
       for (int e = 0; e < p.num_experts; ++e) {
         xt.tprefix[e] = units;

@@ -299,7 +299,10 @@ int ek_moe_down(const void* act, const void* w2, const int* block_expert, const 
  * poorly (a few experts hit at small token counts): the kernel picks the
  * split from the expert counts on the device, writes fp32 slice sums to the
  * workspace, and a second launch adds the slices in order and applies the
- * SwiGLU / writes y. With NULL (or a smaller buffer) K is never split. */
+ * SwiGLU / writes y. With NULL (or a smaller buffer) K is never split. The
+ * down projection writes the rows of y whose slots are in sorted_slots and
+ * leaves the others (of slots that ek_moe_dispatch dropped) as they were: clear
+ * them before ek_moe_combine adds them. It does not split K for such an order. */
 int ek_moe_gate_up_packed(const void* x_perm, const void* w1, const void* w3, const int* expert_counts, void* act,
                           int rows, int E, int H, int I, int tok_tile, int pair, int num_sms, void* workspace,
                           size_t workspace_bytes, void* stream);
@@ -453,8 +456,9 @@ int ek_moe_segment_gemm(const void* hs, const void* weights, const int* offsets,
  *   num_rows[1]           rows in use
  *   x_rows[T*topk, H]     x[slot / topk] per row, 0 past the last (x NULL: no
  *                         rows are copied)
- * This is the packed layout of ek_moe_gate_up_packed / ek_moe_down_packed and
- * the _w4 products. E <= 1024. scratch: ek_moe_permute_scratch_bytes(T, topk,
+ * This is the packed layout of ek_moe_gate_up_packed / ek_moe_down_packed, their
+ * e4m3 forms (E <= 256; they leave a dropped slot's row of y as it was) and the
+ * _w4 products. E <= 1024. scratch: ek_moe_permute_scratch_bytes(T, topk,
  * E) bytes, no initial contents. */
 int ek_moe_dispatch(const int* topk_ids, int T, int topk, int E, const void* x, int H, int dtype, int* sorted_slots,
                     int* slot_rows, int* expert_counts, int* num_rows, void* x_rows, void* scratch, void* stream);

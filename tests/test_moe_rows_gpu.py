@@ -331,3 +331,84 @@ def test_route_grad_of_a_warp_past_2_31_logits(cuda_dev):
     got = _ops.moe_route_grad(ids, w, d, E)
     assert (got[:, E - 1] == -0.5).all() and (got[:, 3] == 0.5).all()
     assert int(torch.count_nonzero(got)) == 2 * T
+
+
+def _poisoned_empty(monkeypatch):
+    """torch.empty gives memory full of NaN, so that what nobody writes is seen."""
+    plain = torch.empty
+
+    def empty(*size, **kw):
+        t = plain(*size, **kw)
+        return t.view(torch.uint8).fill_(0xFF).view(t.dtype) if t.is_cuda and t.numel() and t.dtype != torch.int32 else t
+
+    monkeypatch.setattr(torch, "empty", empty)
+
+
+def _order_with_drops(T, k, E, drop, dev):
+    """Distinct experts per token: all ids, and the same with dropped slots at -1."""
+    g = torch.Generator().manual_seed(T + k)
+    ids = torch.topk(torch.randn((T, E), generator=g), k, dim=1).indices.int()
+    kept = ids.clone()
+    kept[torch.from_numpy(_ids(T, k, E, drop, np.random.default_rng(T)) < 0)] = -1
+    if drop == "some":
+        kept[0, 0] = -1
+    return ids.to(dev), kept.to(dev), torch.rand((T, k), generator=g).to(dev)
+
+
+@pytest.mark.parametrize("drop", ["none", "some", "tail", "all"])
+@pytest.mark.parametrize("T,H,I", [(1, 2048, 1024), (2, 2048, 1024), (4, 2048, 1024), (16, 2048, 1024), (300, 256, 640)])
+def test_dropped_slots_through_the_bf16_experts(T, H, I, drop, cuda_dev, monkeypatch):
+    """The layer over an order with dropped slots is the layer over the whole order
+    with their weights at zero, bit for bit (each output sums the same K blocks in
+    the same order); a K split sums in another order, so neither side splits."""
+    E, k = 8, 2
+    ids, kept, w = _order_with_drops(T, k, E, drop, cuda_dev)
+    g = torch.Generator().manual_seed(H + T)
+    x = torch.randn((T, H), generator=g).to(torch.bfloat16).to(cuda_dev)
+    w1, w3 = (torch.randn((E, I, H), generator=g).mul_(H ** -0.5).to(torch.bfloat16).to(cuda_dev) for _ in range(2))
+    w2 = torch.randn((E, H, I), generator=g).mul_(I ** -0.5).to(torch.bfloat16).to(cuda_dev)
+    _poisoned_empty(monkeypatch)
+    full = _ops.moe_permute(ids, E, x=x, block_m=1)
+    masked = torch.where(kept >= 0, w, 0.0)
+    want = _ops.moe_down_packed(full, _ops.moe_gate_up_packed(full, w1, w3, ksplit=False), w2, masked, ksplit=False)
+    p = _ops.moe_dispatch(x, kept, E)
+    act = _ops.moe_gate_up_packed(p, w1, w3, ksplit=False)
+    y = _ops.moe_down_packed(p, act, w2, w, ksplit=False)
+    assert torch.equal(y, want)
+    assert torch.equal(_ops.moe_combine(y, T, k), _ops.moe_combine(want, T, k))
+    if bool((kept < 0).any()):  # left to itself the product does not split an order that is not whole
+        assert torch.equal(_ops.moe_down_packed(p, act, w2, w), want)
+
+
+@pytest.mark.parametrize("pow2", [False, True])
+@pytest.mark.parametrize("drop", ["some", "tail", "all"])
+@pytest.mark.parametrize("T", [5, 300])
+def test_dropped_slots_through_the_e4m3_experts(T, drop, pow2, cuda_dev, monkeypatch):
+    H, I, E, k = 256, 512, 8, 2
+    ids, kept, w = _order_with_drops(T, k, E, drop, cuda_dev)
+    g = torch.Generator().manual_seed(T)
+    x = torch.randn((T, H), generator=g).to(torch.bfloat16).to(cuda_dev)
+    w1, w3 = (torch.randn((E, I, H), generator=g).mul_(H ** -0.5).to(torch.bfloat16).to(cuda_dev) for _ in range(2))
+    w2 = torch.randn((E, H, I), generator=g).mul_(I ** -0.5).to(torch.bfloat16).to(cuda_dev)
+    qw = _ops.quant_moe_weights_fp8(w1, w2, w3, pow2=pow2)
+    _poisoned_empty(monkeypatch)
+
+    def layer(p, weights):
+        xq, xs = _ops.quant_e4m3_kmajor(p["x_perm"], pow2=pow2)
+        act = _ops.moe_gate_up_fp8bs(p, xq, xs, qw)
+        aq, as_ = _ops.quant_e4m3_kmajor(act, pow2=pow2)
+        return _ops.moe_combine(_ops.moe_down_fp8bs(p, aq, as_, qw, weights), T, k)
+
+    want = layer(_ops.moe_permute(ids, E, x=x, block_m=1), torch.where(kept >= 0, w, 0.0))
+    assert torch.equal(layer(_ops.moe_dispatch(x, kept, E), w), want)
+
+
+def test_padded_products_refuse_a_dispatch_order(cuda_dev):
+    p = _ops.moe_dispatch(torch.zeros((4, 64), dtype=torch.bfloat16, device=cuda_dev),
+                          torch.zeros((4, 2), dtype=torch.int32, device=cuda_dev), 2)
+    w1, w2 = (torch.zeros(s, dtype=torch.bfloat16, device=cuda_dev) for s in ((2, 32, 64), (2, 64, 32)))
+    act = torch.zeros((8, 32), dtype=torch.bfloat16, device=cuda_dev)
+    for call in (lambda: _ops.moe_gate_up(p, w1, w1),
+                 lambda: _ops.moe_down(p, act, w2, torch.ones((4, 2), device=cuda_dev))):
+        with pytest.raises(RuntimeError, match="moe_permute"):
+            call()
