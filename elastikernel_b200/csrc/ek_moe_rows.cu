@@ -550,6 +550,14 @@ int elem_bytes(int dtype) {
   return dtype == EK_DTYPE_BF16 || dtype == EK_DTYPE_FP16 ? 2 : dtype == EK_DTYPE_FP32 ? 4 : 0;
 }
 
+// Vectors of a row and a run past its end are counted in ints; the bytes are not.
+constexpr int kMaxH = 1 << 30;
+
+template <class T, int V>
+int vectors(int H) {
+  return (int)((size_t)H * sizeof(T) / V);
+}
+
 // Widest vector that divides the row and every base address.
 int vec_bytes(size_t row_bytes, std::initializer_list<const void*> ptrs) {
   uintptr_t a = row_bytes;
@@ -563,6 +571,7 @@ int check_rows(const char* what, int T, int k, int n_rows, int H, int dtype) {
   if (T < 0 || k < 1 || H < 1 || n_rows < 0 || !elem_bytes(dtype))
     return set_error(EK_ERR_INVALID, "%s: bad sizes or type (T=%d k=%d rows=%d H=%d dtype=%d)", what, T, k, n_rows, H,
                      dtype);
+  if (H > kMaxH) return set_error(EK_ERR_INVALID, "%s: rows of more than 2^30 elements (H=%d)", what, H);
   if ((long long)T * k > (1ll << 30)) return set_error(EK_ERR_INVALID, "%s: too many slots", what);
   return EK_OK;
 }
@@ -584,7 +593,7 @@ struct Rows {  // what the sums take
 
 template <class T, int V, bool kWeighted, int kK>
 int launch_sum_k(const Rows& a, void* dst) {
-  const int nvec = a.H * (int)sizeof(T) / V;
+  const int nvec = vectors<T, V>(a.H);
   sum_rows_kernel<T, V, kWeighted, kK><<<rows_grid((long long)a.T * runs_per_row<kSumRun<V, kK>>(nvec) * 32), 256, 0, a.s>>>(
       static_cast<const typename Vec<V>::type*>(a.rows), a.slot_rows, a.w, a.T, a.k, a.n_rows, nvec,
       static_cast<typename Vec<V>::type*>(dst));
@@ -618,7 +627,7 @@ int sum_rows(const Rows& a, int dtype, void* out) {
 template <class T, int V, int kK>
 int launch_combine_grad(const Rows& a, const void* d_out, const int* num_rows, void* d_rows, float* d_w) {
   using Raw = typename Vec<V>::type;
-  const int nvec = a.H * (int)sizeof(T) / V;
+  const int nvec = vectors<T, V>(a.H);
   const auto* rows = static_cast<const Raw*>(a.rows);
   const auto* d = static_cast<const Raw*>(d_out);
   auto* o = static_cast<Raw*>(d_rows);

@@ -444,8 +444,8 @@ int ek_moe_segment_gemm(const void* hs, const void* weights, const int* offsets,
  * training and for rows that some slots drop out of. No counterpart in the
  * reference (its operator is forward only and keeps every slot). dtype is
  * EK_DTYPE_BF16, EK_DTYPE_FP16 or EK_DTYPE_FP32 for every row operand; H is
- * any size, and rows need only their elements' alignment (16-byte rows on
- * 16-byte bases are fastest). T * topk <= 2^30. */
+ * any size up to 2^30, and rows need only their elements' alignment (16-byte
+ * rows on 16-byte bases are fastest). T * topk <= 2^30. */
 
 /* Order the T * topk slots stably by expert and copy the token rows into that
  * order. A negative id drops its slot (a padding token, a slot over an

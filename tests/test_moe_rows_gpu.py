@@ -412,3 +412,23 @@ def test_padded_products_refuse_a_dispatch_order(cuda_dev):
                  lambda: _ops.moe_down(p, act, w2, torch.ones((4, 2), device=cuda_dev))):
         with pytest.raises(RuntimeError, match="moe_permute"):
             call()
+
+
+@pytest.mark.parametrize("H,dtype", [((1 << 29) + 12, "fp32"), ((1 << 30) - 3, "bf16"), (1 << 30, "bf16")])
+def test_rows_past_2_31_bytes(H, dtype, cuda_dev):
+    """Single rows whose bytes do not fit 31 bits, through each operator on rows."""
+    free, _ = torch.cuda.mem_get_info()
+    if free < 40 << 30:
+        pytest.skip("needs 40 GB")
+    x = torch.empty((1, H), dtype=DTYPES[dtype], device=cuda_dev).random_(-8, 9)
+    p = _ops.moe_dispatch(x, torch.zeros((1, 1), dtype=torch.int32, device=cuda_dev), 2)
+    assert torch.equal(p["x_perm"], x)
+    w = torch.full((1, 1), 2.0, device=cuda_dev)
+    out = torch.full_like(x, -77)
+    assert torch.equal(_ops.moe_combine_weighted(p, x, w, out=out), x * 2)
+    assert torch.equal(_ops.moe_dispatch_grad(p, x), x)
+    one = torch.zeros_like(x)
+    one[0, 5], one[0, H - 1] = 1, 2  # the dot product meets two elements alone: exact
+    d_y, d_w = _ops.moe_combine_weighted_grad(p, x, w, one)
+    assert torch.equal(d_y, one * 2)
+    assert d_w.item() == x[0, 5].item() + 2 * x[0, H - 1].item()

@@ -266,3 +266,14 @@ def test_route_gradient_refuses_more_experts_than_its_counters_hold():
     _bad(f(_p(), _p(), _p(), 4, (1 << 30) + 1, 2, _p(), None), "2^30")
     _bad(f(_p(), _p(), _p(), 4, (1 << 31) - 1, 40, _p(), None), "2^30")
     assert f(None, None, None, 0, 1 << 30, 2, None, None) == _lib.EK_OK
+
+
+@pytest.mark.parametrize("H", [(1 << 30) + 1, (1 << 31) - 1])
+@pytest.mark.parametrize("dtype", [_lib.EK_DTYPE_BF16, _lib.EK_DTYPE_FP32])
+def test_rows_longer_than_their_counters_are_refused(H, dtype):
+    L = lib()
+    n = None
+    _bad(L.ek_moe_dispatch(_p(), 1, 1, 8, _p(), H, dtype, _p(), _p(), _p(), _p(), _p(), _p(), n), "2^30 elements")
+    _bad(L.ek_moe_dispatch_grad(_p(), _p(), 1, 1, 1, H, dtype, _p(), n), "2^30 elements")
+    _bad(L.ek_moe_combine_weighted(_p(), _p(), _p(), 1, 1, 1, H, dtype, _p(), n), "2^30 elements")
+    _bad(L.ek_moe_combine_weighted_grad(_p(), _p(), _p(), _p(), _p(), 1, 1, 1, H, dtype, _p(), _p(), n), "2^30 elements")
