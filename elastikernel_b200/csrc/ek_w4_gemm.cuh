@@ -33,6 +33,19 @@ inline bool makes_records(int M, long long units, int grid) {
 int gemm_bf16(const GemmArgs& a);
 int gemm_fp16(const GemmArgs& a);
 
+// The sums of a product with minima may read the token rows again, so records
+// are made where they are written over.
+inline bool over_its_rows(const GemmArgs& a) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.A), c = reinterpret_cast<uintptr_t>(a.C);
+  return a.mins && x < c + (size_t)a.M * a.N * 2 && c < x + (size_t)a.M * a.K * 2;
+}
+
+template <int TOK, bool kMin, class T>
+int finish(const Params<T>& p, int grid, T* out, cudaStream_t stream) {
+  const dim3 g(p.feature_tiles, std::min(p.max_y * TOK, 4096));
+  return launch("w4 sums launch", finish_kernel<kDense, TOK, kMin, T, T>, g, kRows, 0, stream, false, p, grid, out);
+}
+
 template <class T>
 int gemm(const GemmArgs& a) {
   int nt = 0, grid = 0;
@@ -40,6 +53,8 @@ int gemm(const GemmArgs& a) {
   uint8_t* ws = static_cast<uint8_t*>(a.workspace);
   Params<T> p = {};
   p.w[0] = {static_cast<const T*>(a.scales), static_cast<const T*>(a.mins)};
+  p.codes[0] = static_cast<const uint8_t*>(a.codes);
+  p.group = a.group;
   p.K = a.K;
   p.N = a.N;
   p.feature_tiles = (a.N + kRows - 1) / kRows;
@@ -50,7 +65,7 @@ int gemm(const GemmArgs& a) {
   CUtensorMap map;
   int rc = codes_map(&map, a.codes, a.N, a.K, kRows);
   const T* x = static_cast<const T*>(a.A);
-  if (makes_records(a.M, (long long)p.feature_tiles * stages(a.K), grid)) {
+  if (makes_records(a.M, (long long)p.feature_tiles * stages(a.K), grid) && !over_its_rows(a)) {
     p.rows = x;
     p.vec = a.K % 8 == 0 && aligned16(x);
   } else if (!rc) {
@@ -58,10 +73,10 @@ int gemm(const GemmArgs& a) {
   }
   if (!rc) rc = launch_product<T, kDense>(nt, a.group, map, map, p, grid, a.stream);
   if (rc) return rc;
-  const dim3 g(p.feature_tiles, std::min(p.max_y * 8 * nt, 4096));
   T* out = static_cast<T*>(a.C);
-  if (nt == 1) return launch("w4 sums launch", finish_kernel<kDense, 8, T, T>, g, kRows, 0, a.stream, false, p, grid, out);
-  return launch("w4 sums launch", finish_kernel<kDense, 16, T, T>, g, kRows, 0, a.stream, false, p, grid, out);
+  if (a.mins)
+    return nt == 1 ? finish<8, true>(p, grid, out, a.stream) : finish<16, true>(p, grid, out, a.stream);
+  return nt == 1 ? finish<8, false>(p, grid, out, a.stream) : finish<16, false>(p, grid, out, a.stream);
 }
 
 }  // namespace w4

@@ -267,6 +267,8 @@ struct Scales {
 template <class T>
 struct Params {
   Scales<T> w[2];            // gate/up: w1 and w3
+  const uint8_t* codes[2];   // theirs, for the sums (the product has them by TMA)
+  int group;
   int K, N;                  // N: weight rows (of an expert; of one matrix)
   int feature_tiles;         // tiles along N
   Tokens x;
@@ -751,12 +753,80 @@ __device__ __forceinline__ void sum_parts(const Runs& run, const float* parts, i
 }
 
 __device__ __forceinline__ float swiglu(float h, float u) { return h / (1.f + expf(-h)) * u; }
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) < INFINITY; }
+
+// With minima the product adds two terms, s (q - 8) x and (m + 8 s) x, which for an
+// infinite x can be infinities of opposite signs, or 0 * inf beside an infinity,
+// where (s q + m) x is one infinity. So a result that is not finite is made again:
+// where the token row has infinite or NaN elements, the sum is theirs alone, against
+// the weights themselves (n: weight row over all experts); the overflow of a
+// finite row stays as it is. That is done in a second pass after a launch's own
+// work, kept small for the sake of the first one: calls (a stack) cost every
+// launch 0.6 us, 47 registers for 32 a tenth of a stage of 256 tokens, and as it
+// is a layer with minima takes 0.4 to 1 us longer (one token 68.4 to 69.1, 64 tokens
+// of 32 experts 380.6 to 383.5). What is made again is never finite: w * inf is an
+// infinity or NaN. 16 tokens with an infinity each through 14336 x 4096: 403 us
+// instead of 29.
+template <class T>
+__device__ __forceinline__ float sum_by_weights(const Params<T>& p, int matrix, size_t n, size_t row, float sum) {
+  const int G = groups(p.K, p.group);
+  const uint8_t* code = p.codes[matrix] + n * (pieces(p.K) * (kPiece / 2));
+  float exact = 0.f;
+  bool any = false;
+  auto meet = [&](int k, float x) {
+    const size_t at = n * G + k / p.group;
+    const float q = (float)(__ldg(code + k / 2) >> (k & 1 ? 4 : 0) & 15);
+    exact += fmaf(to_f(__ldg(p.w[matrix].s + at)), q, to_f(__ldg(p.w[matrix].m + at))) * x;
+    any = true;
+  };
+  if (p.rows) {  // no records in the workspace
+#pragma unroll 1
+    for (int k = 0; k < p.K && !isnan(exact); ++k) {
+      const float x = to_f(__ldg(p.rows + row * p.K + k));
+      if (!finite(x)) meet(k, x);
+    }
+  } else {
+    const uint8_t* rec = p.x.rec + row * stages(p.K) * kRecord;
+#pragma unroll 1
+    for (int k = 0; k < p.K && !isnan(exact); k += 8) {  // a record is whole past K
+      const uint4 run = __ldcg(reinterpret_cast<const uint4*>(rec + (size_t)(k / kStageElems) * kRecord + k % kStageElems * 2));
+      const uint32_t pair[4] = {run.x, run.y, run.z, run.w};  // elements i and i + 4
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 x = unpack2<__half>(pair[i]);
+        if (!finite(x.x)) meet(k + i, x.x);
+        if (!finite(x.y)) meet(k + i + 4, x.y);
+      }
+    }
+  }
+  return any ? exact : sum;
+}
+
+// Output feature n of token `tok` of the tile (y, n's feature tile), sums and all,
+// a part at a time: this must not take more registers than the first pass.
+template <Mode kMode, int TOK, class T>
+__device__ __forceinline__ float result_again(const Params<T>& p, const Runs& run, const TokenTile& tl, int y, int tok, int n) {
+  constexpr int kFeatures = kMode == kGateUp ? kRows / 2 : kRows;
+  const int tile = y * p.feature_tiles + n / kFeatures;
+  const int c0 = run.owner((long long)tile * run.nst), c1 = run.owner((long long)(tile + 1) * run.nst - 1);
+  float gate = 0.f, v = 0.f;
+#pragma unroll 1
+  for (int j = 0; j < (kMode == kGateUp ? 2 : 1); ++j) {
+    gate = v;
+    v = 0.f;
+    const float* at = p.parts + (size_t)(tile + c0) * (kRows * TOK) + tok * kRows + j * (kRows / 2) + n % kFeatures;
+#pragma unroll 1
+    for (int c = c0; c <= c1; ++c, at += kRows * TOK) v += __ldcg(at);
+    if (!finite(v)) v = sum_by_weights(p, j, (size_t)tl.e * p.N + n, token_row(p, tl, tok), v);
+  }
+  return kMode == kGateUp ? swiglu(gate, v) : v;
+}
 
 // out[r, n] of a dense product or a down projection, act[r, n] of a gate/up: a
 // CTA per feature tile and token, a thread per feature. `grid`: the product's. Bound
 // by latency: 4.6 us alone for 16 x 14336, most of it overlapping the product's end.
-template <Mode kMode, int TOK, class T, class O>
-__global__ void __launch_bounds__(kRows) finish_kernel(const __grid_constant__ Params<T> p, int grid, O* __restrict__ out) {
+template <Mode kMode, int TOK, bool kMin, class T, class O>
+__global__ void __launch_bounds__(kRows, 8) finish_kernel(const __grid_constant__ Params<T> p, int grid, O* __restrict__ out) {
   extern __shared__ int s_index[];
   __shared__ int s_y;
   griddep_launch();
@@ -767,22 +837,36 @@ __global__ void __launch_bounds__(kRows) finish_kernel(const __grid_constant__ P
   constexpr int kPer = kRows / kFeatures;  // tokens a CTA takes at a time
   const int f = blockIdx.x, r = threadIdx.x % kFeatures, n = f * kFeatures + r;
   if (n >= p.N) return;
-  for (int i = blockIdx.y * kPer + threadIdx.x / kFeatures; i < s_y * TOK; i += gridDim.y * kPer) {
+  const int i0 = blockIdx.y * kPer + threadIdx.x / kFeatures, step = gridDim.y * kPer;
+  bool odd = false;
+  for (int i = i0; i < s_y * TOK; i += step) {
     const int y = i / TOK, tok = i - y * TOK, tile = y * p.feature_tiles + f;
     const TokenTile tl = open_tile<kMode, TOK>(p, y, s_end, s_row);
     if (tok >= tl.m) continue;
     constexpr int kN = kMode == kGateUp ? 2 : 1;
     float v[kN][1];
     sum_parts<TOK, 1, kN>(run, p.parts, tile, tok, r, v);
-    out[(size_t)(tl.r0 + tok) * p.N + n] = from_f<O>(kN == 2 ? swiglu(v[0][0], v[kN - 1][0]) : v[0][0]);
+    const float o = kN == 2 ? swiglu(v[0][0], v[kN - 1][0]) : v[0][0];
+    odd |= !finite(o);
+    out[(size_t)(tl.r0 + tok) * p.N + n] = from_f<O>(o);
   }
+  if (kMin && odd)
+    for (int i = i0; i < s_y * TOK; i += step) {
+      const int y = i / TOK, tok = i - y * TOK;
+      const TokenTile tl = open_tile<kMode, TOK>(p, y, s_end, s_row);
+      O* o = out + (size_t)(tl.r0 + tok) * p.N + n;
+      if (tok < tl.m && !finite(to_f(*o))) *o = from_f<O>(result_again<kMode, TOK>(p, run, tl, y, tok, n));
+    }
 }
 
 // The activations of a gate/up product straight into the tokens of the down
 // projection: a warp per packed row and run of 256 features (two tiles). Bound by
-// latency: 7 us alone for one token, 9 us for 512 rows of 2048.
-template <int TOK, class T>
-__global__ void __launch_bounds__(256) act_tokens_kernel(const __grid_constant__ Params<T> p, int grid, int group, Tokens act) {
+// latency: 7 us alone for one token, 9 us for 512 rows of 2048. With minima the
+// infinite and NaN elements of a record may be of the wrong kind at first; its
+// scale is the finite ones', and what the down product makes of the row is not
+// finite whatever they are.
+template <int TOK, bool kMin, class T>
+__global__ void __launch_bounds__(256, kMin ? 4 : 5) act_tokens_kernel(const __grid_constant__ Params<T> p, int grid, int group, Tokens act) {
   extern __shared__ int s_index[];
   __shared__ int s_y;
   griddep_launch();
@@ -790,8 +874,10 @@ __global__ void __launch_bounds__(256) act_tokens_kernel(const __grid_constant__
   const Runs run = open_runs<kGateUp, TOK>(p, grid, s_end, s_row, &s_y);
   griddep_wait();
   const int lane = threadIdx.x & 31, nst = stages(p.N);
+  const long long w0 = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
   const long long warps = ((long long)gridDim.x * blockDim.x) >> 5, total = (long long)s_y * TOK * nst;
-  for (long long w = ((long long)blockIdx.x * blockDim.x + threadIdx.x) >> 5; w < total; w += warps) {
+  bool odd = false;
+  for (long long w = w0; w < total; w += warps) {
     const int st = (int)(w % nst), ty = (int)(w / nst), y = ty / TOK, tok = ty - y * TOK;
     const TokenTile tl = open_tile<kGateUp, TOK>(p, y, s_end, s_row);
     if (tok >= tl.m) continue;
@@ -800,9 +886,45 @@ __global__ void __launch_bounds__(256) act_tokens_kernel(const __grid_constant__
     if (f < p.feature_tiles)
       sum_parts<TOK, 8, 2>(run, p.parts, y * p.feature_tiles + f, tok, n % (kRows / 2), v);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) a[i] = n + i < p.N ? swiglu(v[0][i], v[1][i]) : 0.f;
+    for (int i = 0; i < 8; ++i) {
+      a[i] = n + i < p.N ? swiglu(v[0][i], v[1][i]) : 0.f;
+      odd |= !finite(a[i]);
+    }
     uint8_t* rec = act.rec + ((size_t)(tl.r0 + tok) * nst + st) * kRecord;
     write_run<true>(rec, tail_of(rec), group, a);
+  }
+  if (kMin && odd)
+    for (long long w = w0; w < total; w += warps) {
+      const int st = (int)(w % nst), ty = (int)(w / nst), y = ty / TOK, tok = ty - y * TOK;
+      const TokenTile tl = open_tile<kGateUp, TOK>(p, y, s_end, s_row);
+      if (tok >= tl.m) continue;
+      __half* rec = reinterpret_cast<__half*>(act.rec + ((size_t)(tl.r0 + tok) * nst + st) * kRecord) + lane * 8;
+#pragma unroll 1
+      for (int i = 0; i < 8; ++i) {
+        __half* h = rec + (i < 4 ? 2 * i : 2 * i - 7);
+        if (!finite(to_f(*h))) *h = __float2half_rn(result_again<kGateUp, TOK>(p, run, tl, y, tok, st * kStageElems + lane * 8 + i));
+      }
+    }
+}
+
+// The outputs of feature n of combine_parts_kernel that are not finite, made again.
+template <int TOK, class T>
+__device__ __forceinline__ void combine_again(const Params<T>& p, const Runs& run, const int* s_end, int y_end, const int* slot_rows,
+                                           const int* ids, const float* weights, int tokens, int topk, int n, T* out) {
+  const int* s_row = s_end + p.E;
+  for (int t = blockIdx.y; t < tokens; t += gridDim.y) {
+    if (finite(to_f(out[(size_t)t * p.N + n]))) continue;
+    float acc = 0.f;
+    for (int j = 0; j < topk; ++j) {
+      const long long s = (long long)t * topk + j;
+      const int r = __ldcg(slot_rows + s), e = __ldcg(ids + s);
+      if (r < 0 || r >= p.n_rows || e < 0 || e >= p.E) continue;
+      const int at = r - s_row[e], y = (e ? s_end[e - 1] : 0) + at / TOK;
+      if (at < 0 || y >= min(s_end[e], y_end)) continue;
+      const TokenTile tl = open_tile<kDown, TOK>(p, y, s_end, s_row);
+      acc = fmaf(__ldcg(weights + s), result_again<kDown, TOK>(p, run, tl, y, at % TOK, n), acc);
+    }
+    out[(size_t)t * p.N + n] = from_f<T>(acc);
   }
 }
 
@@ -810,7 +932,7 @@ __global__ void __launch_bounds__(256) act_tokens_kernel(const __grid_constant__
 // projection, fp32 in j order, rounded once. A CTA per token and 256 features; bound
 // by latency (64 tokens, 8 choices, 7168 wide: 17 us alone for 15 MB of parts), so
 // six CTAs an SM (four or eight: 1 % of the layer more).
-template <int TOK, class T>
+template <int TOK, bool kMin, class T>
 __global__ void __launch_bounds__(kRows, 6)
     combine_parts_kernel(const __grid_constant__ Params<T> p, int grid, const int* __restrict__ slot_rows,
                          const int* __restrict__ ids, const float* __restrict__ weights, int tokens, int topk,
@@ -827,7 +949,7 @@ __global__ void __launch_bounds__(kRows, 6)
   __shared__ float s_w[kList];
   __shared__ int s_n;
   const int lane = threadIdx.x & 31, f = blockIdx.x, n = f * kRows + threadIdx.x;
-  bool waited = false;
+  bool waited = false, odd = false;
   for (int t = blockIdx.y; t < tokens; t += gridDim.y) {
     float acc = 0.f, v = 0.f;
     for (int j0 = 0; j0 < topk; j0 += 32) {
@@ -887,8 +1009,13 @@ __global__ void __launch_bounds__(kRows, 6)
         if (base + kList >= total) break;
       }
     }
-    if (n < p.N) out[(size_t)t * p.N + n] = from_f<T>(acc);
+    if (n < p.N) {
+      out[(size_t)t * p.N + n] = from_f<T>(acc);
+      odd |= !finite(acc);
+    }
   }
+  if constexpr (kMin)
+    if (odd) combine_again<TOK>(p, run, s_end, s_y, slot_rows, ids, weights, tokens, topk, n, out);
 }
 
 }  // namespace w4

@@ -93,6 +93,7 @@ struct Matrix {
   const void *codes, *scales, *mins;
 };
 
+const uint8_t* codes_of(const Matrix& m) { return static_cast<const uint8_t*>(m.codes); }
 Scales<bf16> scales_of(const Matrix& m) { return {static_cast<const bf16*>(m.scales), static_cast<const bf16*>(m.mins)}; }
 
 struct Moe {
@@ -107,6 +108,7 @@ struct Moe {
 
   Params<bf16> params(int K, int N, int features, const Tokens& tokens) const {
     Params<bf16> p = {};
+    p.group = group;
     p.K = K;
     p.N = N;
     p.feature_tiles = (N + features - 1) / features;
@@ -126,6 +128,8 @@ struct Moe {
     Params<bf16> p = params(H, I, kRows / 2, x());
     p.w[0] = scales_of(w1);
     p.w[1] = scales_of(w3);
+    p.codes[0] = codes_of(w1);
+    p.codes[1] = codes_of(w3);
     p.sorted_slots = sorted_slots;
     p.topk = topk;
     p.n_slots = rows;
@@ -142,42 +146,55 @@ struct Moe {
   int down(const Matrix& w2, Params<bf16>* out) const {
     Params<bf16> p = params(I, H, kRows, act());
     p.w[0] = scales_of(w2);
+    p.codes[0] = codes_of(w2);
     *out = p;
     CUtensorMap m;
     const int rc = codes_map(&m, w2.codes, (long long)E * H, I, kRows);
     return rc ? rc : launch_product<bf16, kDown>(l.nt, group, m, m, p, l.grid, stream);
   }
-  template <Mode kMode, int TOK, class O>
-  int finish_tok(const Params<bf16>& p, O* out) const {
-    const dim3 g(p.feature_tiles, std::min(l.max_y * TOK, 4096));
-    return launch("w4 sums launch", finish_kernel<kMode, TOK, bf16, O>, g, kRows, index_bytes(), stream, false, p, l.grid, out);
+  // One of the sums' launches: f(tokens per tile, minima) as constants.
+  template <class F>
+  int sums(const Params<bf16>& p, const F& f) const {
+    using std::integral_constant;
+    const integral_constant<int, 8> t8;
+    const integral_constant<int, 16> t16;
+    if (p.w[0].m) return l.nt == 1 ? f(t8, std::true_type{}) : f(t16, std::true_type{});
+    return l.nt == 1 ? f(t8, std::false_type{}) : f(t16, std::false_type{});
   }
   template <Mode kMode, class O>
   int finish(const Params<bf16>& p, O* out) const {
-    return l.nt == 1 ? finish_tok<kMode, 8>(p, out) : finish_tok<kMode, 16>(p, out);
+    return sums(p, [&](auto tok, auto mins) {
+      constexpr int TOK = decltype(tok)::value;
+      const dim3 g(p.feature_tiles, std::min(l.max_y * TOK, 4096));
+      return launch("w4 sums launch", finish_kernel<kMode, TOK, decltype(mins)::value, bf16, O>, g, kRows, index_bytes(),
+                    stream, false, p, l.grid, out);
+    });
   }
   // gate/up, down and combine, from an order of the slots
   int layer(const bf16* xin, const Order& o, int T, int topk, const Matrix& w1, const Matrix& w3, const Matrix& w2,
             bf16* out) const {
     Params<bf16> p;
     int rc = gate_up(xin, T, o.sorted_slots, topk, w1, w3, &p);
-    if (!rc) rc = l.nt == 1 ? act_tokens<8>(p) : act_tokens<16>(p);
+    if (!rc) rc = act_tokens(p);
     if (!rc) rc = down(w2, &p);
-    if (rc) return rc;
-    return l.nt == 1 ? combine<8>(p, o.slot_rows, o.ids, o.weights, T, topk, out)
-                     : combine<16>(p, o.slot_rows, o.ids, o.weights, T, topk, out);
+    return rc ? rc : combine(p, o.slot_rows, o.ids, o.weights, T, topk, out);
   }
-  template <int TOK>
   int act_tokens(const Params<bf16>& p) const {
-    const long long warps = (long long)l.max_y * TOK * stages(I);
-    return launch("w4 act launch", act_tokens_kernel<TOK, bf16>, dim3((unsigned)std::min<long long>((warps + 7) / 8, 148 * 8)),
-                  256, index_bytes(), stream, false, p, l.grid, group, act());
+    return sums(p, [&](auto tok, auto mins) {
+      constexpr int TOK = decltype(tok)::value;
+      const long long warps = (long long)l.max_y * TOK * stages(I);
+      return launch("w4 act launch", act_tokens_kernel<TOK, decltype(mins)::value, bf16>,
+                    dim3((unsigned)std::min<long long>((warps + 7) / 8, 148 * 8)), 256, index_bytes(), stream, false, p,
+                    l.grid, group, act());
+    });
   }
-  template <int TOK>
   int combine(const Params<bf16>& p, const int* slot_rows, const int* ids, const float* weights, int T, int topk,
               bf16* out) const {
-    return launch("w4 combine launch", combine_parts_kernel<TOK, bf16>, dim3(p.feature_tiles, std::min(T, 4096)), kRows,
-                  index_bytes(), stream, false, p, l.grid, slot_rows, ids, weights, T, topk, out);
+    return sums(p, [&](auto tok, auto mins) {
+      return launch("w4 combine launch", combine_parts_kernel<decltype(tok)::value, decltype(mins)::value, bf16>,
+                    dim3(p.feature_tiles, std::min(T, 4096)), kRows, index_bytes(), stream, false, p, l.grid, slot_rows,
+                    ids, weights, T, topk, out);
+    });
   }
 };
 

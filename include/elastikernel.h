@@ -511,6 +511,8 @@ int ek_dequant_w4(const void* codes, const void* scales, const void* mins, long 
  * fp32 sums rounded once. Any M, N and K; made for M of a few tokens, where the
  * codes are streamed once per 16 tokens. A's elements enter as fp16 scaled
  * per run of 256 by a power of two: exact up to 2^-40 of the run's largest.
+ * Infinite and NaN elements give what their products with the weights add up to,
+ * with minima from a second look at the row (slower).
  * workspace: ek_gemm_w4_workspace_bytes(M, N, K, SMs of the launch) bytes of
  * 16-byte aligned device memory, no initial contents; nothing in it is kept
  * between calls. */

@@ -481,3 +481,95 @@ def test_nothing_is_written_after_an_empty_product(stage, captured, cuda_dev, mo
             once(i)
     torch.cuda.synchronize()
     assert not bad.any()
+
+
+def _by_definition(x, qw):
+    """sum_k w x term by term, so that infinities meet the weights themselves."""
+    with np.errstate(invalid="ignore"):
+        return (_np(x)[:, None, :] * _values(qw)[None]).sum(axis=2)
+
+
+def _same_kind(got, exact, rows):
+    """Infinities of one sign, NaN and finite values where the definition has them."""
+    a, b = _np(got)[rows], exact[rows]
+    assert np.array_equal(np.isnan(a), np.isnan(b))
+    assert np.array_equal(np.isposinf(a), np.isposinf(b)) and np.array_equal(np.isneginf(a), np.isneginf(b))
+
+
+@pytest.mark.parametrize("mins", [False, True])
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("M,N,K,group", [(1, 300, 257, 32), (2, 64, 4096, 128), (4, 40, 96, 64), (20, 70, 1030, 64),
+                                         (40, 515, 700, 128)])
+def test_gemm_infinite_tokens(M, N, K, group, dtype, mins, cuda_dev):
+    """An infinite token element gives what (s q + m) x gives, weight by weight:
+    an infinity of the product's sign, NaN where the weight is zero or two
+    infinities oppose each other."""
+    qw = _integer_weight(N, K, group, mins, dtype, M + N + K, cuda_dev)
+    g = torch.Generator().manual_seed(K)
+    x = torch.randint(-2, 3, (M, K), generator=g).to(dtype)
+    clean = _ops.gemm_w4(x.to(cuda_dev), qw)
+    bad = sorted({0, M // 2, M - 1})
+    x[0, K - 1] = float("inf")
+    if M > 1:
+        x[M // 2, 3], x[M // 2, K // 2] = float("-inf"), float("inf")  # two of them, in two groups for most K
+    if M > 2:
+        x[M - 1, 7] = float("-inf")
+        x[M - 1, 8] = float("-inf")
+    got = _ops.gemm_w4(x.to(cuda_dev), qw)
+    _same_kind(got, _by_definition(x, qw), bad)
+    rest = [i for i in range(M) if i not in bad]
+    assert torch.equal(got[rest], clean[rest])
+    x[0, 0] = float("nan")
+    assert _ops.gemm_w4(x.to(cuda_dev), qw)[0].isnan().all()
+
+
+@pytest.mark.parametrize("M", [1, 3, 40])
+def test_infinite_tokens_written_over(M, cuda_dev):
+    """In place: the rows are looked at again while their outputs are written."""
+    qw = _integer_weight(256, 256, 64, True, BF, 8, cuda_dev)
+    x = torch.randint(-2, 3, (M, 256), generator=torch.Generator().manual_seed(M)).to(BF)
+    x[0, 9] = float("inf")
+    x[M - 1, 250] = float("-inf")
+    exact, x = _by_definition(x, qw), x.to(cuda_dev)
+    want = _ops.gemm_w4(x, qw)
+    _same_kind(want, exact, [0, M - 1])
+    assert _ops.gemm_w4(x, qw, out=x) is x and torch.equal(x.nan_to_num(7.0), want.nan_to_num(7.0))
+
+
+def test_gemm_overflow_is_not_an_infinite_token(cuda_dev):
+    """Finite tokens whose sum passes the type's range: an infinity of the sum's sign."""
+    for mins in (False, True):
+        qw = _integer_weight(48, 512, 64, mins, FP, 5, cuda_dev)
+        x = torch.full((3, 512), 6e4, dtype=FP)
+        exact = torch.from_numpy(_by_definition(x, qw)).to(FP)
+        got = _ops.gemm_w4(x.to(cuda_dev), qw).cpu()
+        assert exact.isinf().any() and torch.equal(got.isinf(), exact.isinf())
+        assert torch.equal(got[got.isinf()], exact[exact.isinf()])
+
+
+@pytest.mark.parametrize("T", [3, 90])
+@pytest.mark.parametrize("mins", [False, True])
+def test_expert_products_of_infinite_tokens(T, mins, cuda_dev):
+    """gate/up, down and the layer: the kinds of the outputs follow the definition
+    from the products' own inputs."""
+    k, E, H, I = 2, 4, 264, 150
+    x, ids, qw = _moe_setup((T, k, E, H, I, 32, mins), cuda_dev)
+    x[1, 5] = float("inf")
+    x[2, 200] = float("-inf")
+    w = torch.full((T, k), 0.5, device=cuda_dev)
+    p = _ops.moe_dispatch(x, ids, E)
+    act = _ops.moe_gate_up_w4(p, qw, dtype=torch.float32)
+    y = _ops.moe_down_w4(p, act, qw, dtype=torch.float32)
+    xp, a, r = _np(p["x_perm"]), _np(act), 0
+    v = {n: _values(qw[n]) for n in ("w1", "w3", "w2")}
+    exact_y = np.zeros((T * k, H))
+    with np.errstate(invalid="ignore", over="ignore"):
+        for e, c in enumerate(p["expert_counts"].tolist()):
+            for i in range(r, r + c):
+                h, u = (xp[i] * v["w1"][e]).sum(1), (xp[i] * v["w3"][e]).sum(1)
+                _same_kind(act[i:i + 1], (h / (1 + np.exp(-h)) * u)[None], [0])
+                exact_y[i] = (a[i] * v["w2"][e]).sum(1)
+                _same_kind(y[i:i + 1], exact_y[i:i + 1], [0])
+            r += c
+        sr = p["slot_rows"].cpu().numpy().reshape(T, k)
+        _same_kind(_ops.moe_experts_w4(p, x, ids, w, qw), (exact_y[sr] * 0.5).sum(axis=1), np.arange(T))
