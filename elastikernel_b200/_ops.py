@@ -814,7 +814,11 @@ def moe_route_grad(topk_ids: torch.Tensor, topk_weights: torch.Tensor, d_weights
     """Gradient of moe_route's weights with respect to the gate logits, fp32 [T, E].
 
     The renormalised weights are the softmax of the chosen logits, so
-    d_logits[t, ids_j] = w_j (dw_j - sum_i w_i dw_i) and every other entry is 0."""
+    d_logits[t, ids_j] = w_j (dw_j - sum_i w_i dw_i), and an expert that was not
+    chosen gets 0. topk_ids are the ids as moe_route gave them, dropped slots'
+    too: a choice dropped for capacity was in the softmax, so its logit has a
+    gradient although its dw is 0. Ids masked to -1 (what moe_dispatch takes
+    for a dropped slot) would lose it."""
     dev = _require_cuda(topk_ids, topk_weights, d_weights)
     if topk_ids.dim() != 2:
         raise RuntimeError("topk_ids must be a 2-D int32 tensor")

@@ -483,7 +483,11 @@ int ek_moe_combine_weighted_grad(const void* rows, const int* slot_rows, const f
 /* Gradient of ek_moe_route's weights with respect to the logits: the
  * renormalised weights are a softmax over the chosen logits, so
  * d_logits[t, ids_j] += w_j (dw_j - sum_i w_i dw_i), every other entry 0.
- * Ids outside [0, E) take part in the sum and write nothing. E <= 2^30. */
+ * topk_ids are the ids as they were routed, a dropped slot's included: it was in
+ * the softmax, and with its dw of 0 its logit still gets -w_j sum_i w_i dw_i.
+ * (Where ek_moe_dispatch was given a -1 instead, this takes the id of before.)
+ * Ids outside [0, E) take part in the sum and write nothing, so their logits'
+ * share is lost. E <= 2^30. */
 int ek_moe_route_grad(const int* topk_ids, const float* topk_weights, const float* d_weights, int T, int E, int topk,
                       float* d_logits, void* stream);
 

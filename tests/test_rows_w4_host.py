@@ -69,6 +69,34 @@ def test_route_gradient_against_differences():
         assert abs(num - g[i]) < 1e-8
 
 
+def test_route_gradient_with_dropped_choices_against_differences():
+    """softmax over the chosen logits -> some choices dropped -> weighted combine:
+    the logits' gradient takes the routed ids, not those with -1 for the dropped."""
+    rng = np.random.default_rng(2)
+    T, E, k, H = 5, 6, 3, 4
+    z, d = rng.normal(size=(T, E)), rng.normal(size=(T, H))
+    ids = np.argsort(-z, axis=1)[:, :k].astype(np.int32)
+    kept = ids.copy()
+    kept[[0, 1, 1, 3], [1, 0, 2, 2]] = -1
+    _, sr, _ = orows.order(kept, E)
+    y = rng.normal(size=(T * k, H))
+
+    def loss(z):
+        return (orows.combine(y, sr, orows.route_weights(z, ids)) * d).sum()
+
+    w = orows.route_weights(z, ids)
+    d_w = orows.combine_grad(y, sr, w, d)[1]
+    g, masked = orows.route_grad(ids, w, d_w, E), orows.route_grad(kept, w, d_w, E)
+    h = 1e-6
+    for i in np.ndindex(T, E):
+        a, b = z.copy(), z.copy()
+        a[i] += h
+        b[i] -= h
+        assert abs((loss(a) - loss(b)) / (2 * h) - g[i]) < 1e-8
+    assert np.abs(g.sum(axis=1)).max() < 1e-12  # a softmax's gradient
+    assert np.abs(masked[[0, 1, 3]].sum(axis=1)).min() > 1e-3  # which the masked ids lose
+
+
 @pytest.mark.parametrize("symmetric", [True, False])
 @pytest.mark.parametrize("K,group", [(128, 32), (200, 64), (257, 128), (1, 32)])
 def test_quantisation_error_is_half_a_step(symmetric, K, group):

@@ -573,3 +573,40 @@ def test_expert_products_of_infinite_tokens(T, mins, cuda_dev):
             r += c
         sr = p["slot_rows"].cpu().numpy().reshape(T, k)
         _same_kind(_ops.moe_experts_w4(p, x, ids, w, qw), (exact_y[sr] * 0.5).sum(axis=1), np.arange(T))
+
+
+def test_router_backward_with_dropped_choices(cuda_dev):
+    """Choices dropped for capacity were in the softmax: the logits' gradient, from
+    the routed ids, against differences of softmax, drop and combine."""
+    T, k, E, H, I = 7, 3, 6, 64, 96
+    x, _, qw = _moe_setup((T, k, E, H, I, 32, True), cuda_dev)
+    g = torch.Generator().manual_seed(12)
+    logits, d_out = torch.randn((T, E), generator=g), torch.randn((T, H), generator=g).to(BF)
+    ids, w = _ops.moe_route(logits.to(cuda_dev), k)
+    over_capacity = torch.zeros((T, k), dtype=torch.bool, device=cuda_dev)
+    over_capacity[0, 0] = over_capacity[2, 1] = over_capacity[2, 2] = over_capacity[5] = True
+    p = _ops.moe_dispatch(x, ids.masked_fill(over_capacity, -1), E)
+    y = _ops.moe_down_w4(p, _ops.moe_gate_up_w4(p, qw), qw)
+    _, d_w = _ops.moe_combine_weighted_grad(p, y, w, d_out.to(cuda_dev))
+    d_logits = _np(_ops.moe_route_grad(ids, w, d_w, E))
+    sr = p["slot_rows"].cpu().numpy()
+    rows = np.where((sr >= 0)[:, None], _np(y)[np.maximum(sr, 0)], 0.0).reshape(T, k, H)
+    chosen = ids.cpu().numpy().astype(np.int64)
+
+    def loss(z):
+        c = np.exp(np.take_along_axis(z, chosen, axis=1))
+        c /= c.sum(axis=1, keepdims=True)
+        return ((c[:, :, None] * rows).sum(axis=1) * _np(d_out)).sum()
+
+    z = logits.double().numpy()
+    for i in np.ndindex(T, E):
+        a, b = z.copy(), z.copy()
+        a[i] += 1e-5
+        b[i] -= 1e-5
+        # differences: h^2 times the third derivative (1e-10 of the row), 2^-53 |f| / h of
+        # the whole loss (below 100: 6e-10); fp32 sums: (H + 16) 2^-24 of the row
+        scale = np.abs(rows[i[0]] * _np(d_out)[i[0]]).sum()
+        assert abs((loss(a) - loss(b)) / 2e-5 - d_logits[i]) <= ((H + 16) * 2.0 ** -24 + 1e-9) * scale + 1e-9
+    assert not d_logits[5].any()
+    lost = _np(_ops.moe_route_grad(ids.masked_fill(over_capacity, -1), w, d_w, E))
+    assert np.abs(lost - d_logits)[[0, 2]].max(axis=1).min() > 1e-3
