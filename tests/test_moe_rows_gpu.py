@@ -432,3 +432,75 @@ def test_rows_past_2_31_bytes(H, dtype, cuda_dev):
     d_y, d_w = _ops.moe_combine_weighted_grad(p, x, w, one)
     assert torch.equal(d_y, one * 2)
     assert d_w.item() == x[0, 5].item() + 2 * x[0, H - 1].item()
+
+
+@pytest.mark.parametrize("E", [3, 64, 1000])
+@pytest.mark.parametrize("k", [16, 17, 20, 31, 32, 33, 40, 100])
+def test_route_grad_of_many_choices(k, E, cuda_dev):
+    """Up to 32 choices a token's lanes hold them, past that every logit looks
+    through them; repeated ids (more choices than experts among them) and ids outside
+    [0, E) in each. |w (dw - mean)| bounds a term, an entry sums up to k of them
+    and the mean k products: 2 k + 4 roundings."""
+    T = 37
+    rng = np.random.default_rng(k * E)
+    ids = rng.integers(0, E, (T, k)).astype(np.int32)
+    ids[rng.random((T, k)) < 0.1] = -1
+    ids[rng.random((T, k)) < 0.05] = E + 3
+    ids[5] = 2  # one expert for all choices
+    w = rng.random((T, k)).astype(np.float32)
+    w /= w.sum(axis=1, keepdims=True)
+    d = rng.normal(size=(T, k)).astype(np.float32)
+    got = _ops.moe_route_grad(*(torch.from_numpy(a).to(cuda_dev) for a in (ids, w, d)), E)
+    S = np.zeros((T, E))
+    m = np.abs(w * d).sum(axis=1, keepdims=True)
+    t, j = np.nonzero((ids >= 0) & (ids < E))
+    np.add.at(S, (t, ids[t, j]), (w * (np.abs(d) + m))[t, j])
+    _close(got, orows.route_grad(ids, w, d, E), S, 2 * k + 4, torch.float32)
+    assert (_np(got)[S == 0] == 0).all()
+
+
+@pytest.mark.parametrize("integers", [True, False])
+@pytest.mark.parametrize("T,k,H,dtype", [(1300, 9, 64, "bf16"), (1300, 9, 64, "fp32"), (1200, 17, 33, "fp16"),
+                                         (1184, 12, 1024, "bf16"), (2500, 33, 7, "bf16")])
+def test_combine_grad_of_short_rows_in_several_turns(T, k, H, dtype, integers, cuda_dev):
+    """A warp per token (many short rows) with more choices than one turn takes."""
+    case = (T, k, 24, H, dtype, "some")
+    ids, rows, w = _setup(case, integers)
+    y, d = rows(T * k), rows(T)
+    sr = orows.order(ids, 24)[1]
+    p = _ops.moe_dispatch(None, torch.from_numpy(ids).to(cuda_dev), 24)
+    d_y, d_w = _ops.moe_combine_weighted_grad(p, y.to(cuda_dev), w.to(cuda_dev), d.to(cuda_dev))
+    e_y, e_w = orows.combine_grad(_np(y), sr, w.numpy(), _np(d))
+    if integers:
+        assert np.array_equal(_np(d_y), e_y) and np.array_equal(_np(d_w), e_w)
+    else:
+        _close(d_y, e_y, np.abs(e_y), 2, DTYPES[dtype])
+        S = (np.abs(orows.slot_values(_np(y), sr, T, k)) * np.abs(_np(d))[:, None, :]).sum(axis=2)
+        _close(d_w, e_w, S, H + 2, torch.float32)
+
+
+@pytest.mark.parametrize("T", [24, 600])
+def test_rows_on_a_partition(T, cuda_dev):
+    """The row operators on a partition of 32 SMs: as on the whole device."""
+    from elastikernel_b200.green_ctx import create_sm_partition
+
+    k, E, H = 4, 16, 264
+    g = torch.Generator().manual_seed(T)
+    x = torch.randn((T, H), generator=g).to(torch.bfloat16).to(cuda_dev)
+    ids = torch.randint(-1, E, (T, k), generator=g, dtype=torch.int32).to(cuda_dev)
+    w = torch.rand((T, k), generator=g).to(cuda_dev)
+
+    def once():
+        p = _ops.moe_dispatch(x, ids, E)
+        out = _ops.moe_combine_weighted(p, p["x_perm"], w)
+        d_y, d_w = _ops.moe_combine_weighted_grad(p, p["x_perm"], w, x)
+        return p["sorted_slots"], p["x_perm"], out, d_y, d_w, _ops.moe_dispatch_grad(p, d_y), _ops.moe_route_grad(
+            ids.clamp(min=0), w, d_w, E)
+
+    want = once()
+    stream, _ = create_sm_partition(cuda_dev, 32)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        got = once()
+    stream.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

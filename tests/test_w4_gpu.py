@@ -610,3 +610,44 @@ def test_router_backward_with_dropped_choices(cuda_dev):
     assert not d_logits[5].any()
     lost = _np(_ops.moe_route_grad(ids.masked_fill(over_capacity, -1), w, d_w, E))
     assert np.abs(lost - d_logits)[[0, 2]].max(axis=1).min() > 1e-3
+
+
+@pytest.mark.parametrize("T", [2, 100])
+def test_layer_on_a_partition(T, cuda_dev):
+    """The 4-bit layer and its stages on a partition of 32 SMs: other cuts of the
+    same sums, which are exact in the stages (small integers, power-of-two scales)."""
+    from elastikernel_b200.green_ctx import create_sm_partition
+
+    k, E, H, I = 2, 6, 320, 512
+    g = torch.Generator().manual_seed(T)
+    qw = {"E": E, "H": H, "I": I, "w1": _integer_weight(I, H, 64, True, BF, 1, cuda_dev, (E,)),
+          "w3": _integer_weight(I, H, 64, True, BF, 2, cuda_dev, (E,)),
+          "w2": _integer_weight(H, I, 64, True, BF, 3, cuda_dev, (E,))}
+    x = torch.randint(-2, 3, (T, H), generator=g).to(BF).to(cuda_dev)
+    act = torch.randint(-2, 3, (T * k, I), generator=g).to(BF).to(cuda_dev)
+    logits = torch.randn((T, E), generator=g).to(cuda_dev)
+    ids, w = _ops.moe_route(logits, k)
+    p = _ops.moe_dispatch(x, ids, E)
+
+    def once():
+        return (_ops.moe_gate_up_w4(p, qw), _ops.moe_down_w4(p, act, qw, dtype=torch.float32),
+                _ops.fused_moe_w4(x, logits, qw, k))
+
+    want = once()
+    stream, _ = create_sm_partition(cuda_dev, 32)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        got = once()
+    stream.synchronize()
+    # the gate and up sums are exact, so the activations are the same; so is the down product of integers
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    # The layer's down product adds the same rounded activations in other cuts, each sum within
+    # (I / 4 + 32) 2^-24 of S, its terms' magnitudes (1 + 2^-11 for their rounding); then one
+    # rounding to bf16 each (2^-8).
+    a, b, S = _np(_ops.moe_gate_up_w4(p, qw, dtype=torch.float32)), _bound(qw["w2"]), np.zeros((T, H))
+    rows, experts = p["slot_rows"].cpu().numpy().reshape(T, k), ids.cpu().numpy()
+    for t, j in np.ndindex(T, k):
+        S[t] += float(w[t, j]) * (b[experts[t, j]] @ np.abs(a[rows[t, j]])) * (1 + 2.0 ** -11)
+    one, other = _np(got[2]), _np(want[2])
+    n = (I / 4 + 32) * 2.0 ** -24
+    assert (np.abs(one - other) <= 2.0 ** -8 * (np.abs(one) + np.abs(other)) * (1 + 2.0 ** -7) + 2 * n * S).all()
