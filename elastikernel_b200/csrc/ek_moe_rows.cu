@@ -483,7 +483,9 @@ __global__ void __launch_bounds__(128)
 // the warp clears its tokens' rows with wide stores, then each lane puts its
 // slot's value where it belongs (the lowest lane, where an id repeats; the sum
 // then is in lane order, so that it does not change between runs). 32768 tokens, 256
-// experts: 9.5 us with a cold cache for 37 MB, most of it the zeros.
+// experts: 9.5 us with a cold cache for 37 MB. The zeros stay in L2; bound by the
+// latency of a warp's one turn, the loads and then the exchanges among its lanes
+// (issue slots 34 % busy, most stalls on the exchanges).
 __global__ void __launch_bounds__(256)
     route_grad_kernel(const int* __restrict__ ids, const float* __restrict__ weights,
                       const float* __restrict__ d_weights, int T, int E, int k, int kp, bool wide,

@@ -16,9 +16,14 @@
 //   * the tokens as fp16 too, whatever their type: a small kernel scales each
 //     run of 256 elements by a power of two so that its largest magnitude lies
 //     in [2^14, 2^15) and writes it in the order the nibbles come out. bf16 has
-//     8 significant bits to fp16's 11 and elements below 2^-29 of the run's
-//     largest lose at most 2^-40 of it, less than the fp32 sums do; fp32 rows
-//     (the experts' activations) are rounded to 11 bits;
+//     8 significant bits to fp16's 11: exact down to 2^-31 of the run's largest
+//     (2^-17 scaled, seven bits above fp16's smallest step of 2^-24), and below
+//     that off by half such a step, at most 2^-39 of the largest and less than
+//     the fp32 sums are. fp16 rows go in as they are. fp32 rows (the experts'
+//     activations) are rounded to 11 bits: more would need a second operand for
+//     the low bits and twice the products, and three bits below a bf16
+//     activation they hardly show beside the outputs' one rounding to 8 (error of
+//     a layer's outputs against 64 bits 1.674e-3, with fp32 activations 1.661e-3);
 //   * sums of one group in fp32 accumulators, then multiplied by the group's
 //     fp32 scale: both operands are exact, so no weight is ever rounded. With
 //     minima w = s (q - 8) + (m + 8 s), and the second term meets the sum of the
@@ -104,7 +109,10 @@ __device__ __forceinline__ float2 unpack2(uint32_t v) {
   else return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
 }
 
-// (w & mask) | 0x6400 6400: the masked nibbles over the exponent of 1024.
+// (w & mask) | 0x6400 6400: the masked nibbles over the exponent of 1024, whose
+// last mantissa bit is worth 1, so that they are integers without a conversion (a
+// published way: Kim et al., "Who Says Elephants Can't Run", 2022; the constants
+// follow from the format).
 __device__ __forceinline__ uint32_t nibbles(uint32_t w, uint32_t mask) {
   uint32_t r;
   asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(w), "r"(mask), "r"(0x64006400u));
@@ -763,7 +771,7 @@ __device__ __forceinline__ bool finite(float v) { return fabsf(v) < INFINITY; }
 // finite row stays as it is. That is done in a second pass after a launch's own
 // work, kept small for the sake of the first one: calls (a stack) cost every
 // launch 0.6 us, 47 registers for 32 a tenth of a stage of 256 tokens, and as it
-// is a layer with minima takes 0.4 to 1 us longer (one token 68.4 to 69.1, 64 tokens
+// is a layer with minima takes 0.7 to 3 us longer (one token 68.4 to 69.1, 64 tokens
 // of 32 experts 380.6 to 383.5). What is made again is never finite: w * inf is an
 // infinity or NaN. 16 tokens with an infinity each through 14336 x 4096: 403 us
 // instead of 29.

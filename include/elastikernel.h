@@ -514,7 +514,8 @@ int ek_dequant_w4(const void* codes, const void* scales, const void* mins, long 
 /* C[M, N] = A[M, K] @ W[N, K]^T with 4-bit W; A, C, scales and mins in dtype,
  * fp32 sums rounded once. Any M, N and K; made for M of a few tokens, where the
  * codes are streamed once per 16 tokens. A's elements enter as fp16 scaled
- * per run of 256 by a power of two: exact up to 2^-40 of the run's largest.
+ * per run of 256 by a power of two: fp16 always exact, bf16 down to 2^-31 of the
+ * run's largest (below that off by at most 2^-39 of it).
  * Infinite and NaN elements give what their products with the weights add up to,
  * with minima from a second look at the row (slower).
  * workspace: ek_gemm_w4_workspace_bytes(M, N, K, SMs of the launch) bytes of
@@ -530,7 +531,7 @@ int ek_gemm_w4(const void* A, const void* codes, const void* scales, const void*
  * for the rows r of every expert e (the rows past the last are not written).
  * x is bf16: the packed rows (x_rows = rows), or, with sorted_slots, the tokens
  * (x_rows = T, rows = T * topk): row r then reads x[sorted_slots[r] / topk].
- * act and y are bf16 or fp32 (act_dtype, y_dtype). An fp32 act enters the down
+ * rows <= 2^24. act and y are bf16 or fp32 (act_dtype, y_dtype). An fp32 act enters the down
  * product rounded to 11 significant bits, a bf16 one as it is. workspace:
  * ek_moe_w4_workspace_bytes(x_rows, rows, E, H, I, SMs of the launch) bytes (the
  * down product: x_rows 0), as ek_gemm_w4's. */
