@@ -681,6 +681,12 @@ _ROW_DTYPES = {torch.bfloat16: _lib.EK_DTYPE_BF16, torch.float16: _lib.EK_DTYPE_
                torch.float32: _lib.EK_DTYPE_FP32}
 
 
+# The library's own limits, checked here too: a size past 32 bits would reach it
+# as another one.
+_MAX_SLOTS = _MAX_ROW = _MAX_EXPERTS = 1 << 30
+_MAX_W4_K, _MAX_W4_ROWS = 1 << 28, 1 << 24
+
+
 def _check_rows(name: str, t: torch.Tensor, rows: int | None = None) -> int:
     """dtype code of a contiguous bf16/fp16/fp32 row matrix (of `rows` rows)."""
     dt, shape = _ROW_DTYPES.get(t.dtype), t.shape
@@ -688,8 +694,9 @@ def _check_rows(name: str, t: torch.Tensor, rows: int | None = None) -> int:
         raise RuntimeError(f"{name} must be a 2-D bf16, fp16 or fp32 tensor")
     if rows is not None and shape[0] != rows:
         raise RuntimeError(f"{name} must have {rows} rows, got {shape[0]}")
-    if shape[1] == 0:
-        raise RuntimeError(f"{name} has rows of no elements")
+    if not 0 < shape[1] <= _MAX_ROW or shape[0] > 0x7fffffff:
+        raise RuntimeError(f"{name} has rows of no elements" if shape[1] == 0 else
+                           f"{name}: rows of more than 2^30 elements, or more than 2^31 of them")
     if not t.is_contiguous():
         raise RuntimeError(f"{name} must be contiguous")
     return dt
@@ -733,6 +740,10 @@ def moe_dispatch(x: torch.Tensor | None, topk_ids: torch.Tensor, num_experts: in
     _contig("topk_ids", topk_ids)
     T, k = topk_ids.shape
     E, n = int(num_experts), T * k
+    if n > _MAX_SLOTS or k > _MAX_SLOTS:
+        raise RuntimeError(f"moe_dispatch: too many slots ({T} x {k})")
+    if abs(E) > _MAX_EXPERTS:
+        raise RuntimeError(f"moe_dispatch: need 1 <= E <= 1024 (got {E})")
     H = dt = 0
     x_perm = None
     if x is not None:
@@ -827,8 +838,8 @@ def moe_route_grad(topk_ids: torch.Tensor, topk_weights: torch.Tensor, d_weights
     _check_slots("topk_weights", topk_weights, T, k, torch.float32)
     _check_slots("d_weights", d_weights, T, k, torch.float32)
     E = int(num_experts)
-    if E < 1:
-        raise RuntimeError("num_experts must be positive")
+    if not 1 <= E <= _MAX_EXPERTS or max(T, k) > 0x7fffffff:
+        raise RuntimeError("num_experts must be positive, at most 2^30, and ids within 2^31 x 2^31")
     d_logits = d_weights.new_empty((T, E))
     with _on_device(dev):
         check(lib().ek_moe_route_grad(topk_ids.data_ptr(), topk_weights.data_ptr(), d_weights.data_ptr(), T, E, k,
@@ -851,8 +862,8 @@ def quant_w4(w: torch.Tensor, group: int = 128, symmetric: bool = True, dtype: t
     products take. The weight is s * (q - 8), or s * q + m with minima; weights
     quantised elsewhere go in by building this dict."""
     dev = _require_cuda(w)
-    if w.dtype not in _ROW_DTYPES or w.dim() < 2 or w.shape[-1] == 0:
-        raise RuntimeError("quant_w4 takes bf16, fp16 or fp32 weights [..., N, K]")
+    if w.dtype not in _ROW_DTYPES or w.dim() < 2 or not 0 < w.shape[-1] <= _MAX_W4_K:
+        raise RuntimeError("quant_w4 takes bf16, fp16 or fp32 weights [..., N, K] with K of 1 to 2^28")
     if dtype is None:
         dtype = w.dtype if w.dtype in _DTYPES else torch.bfloat16
     if dtype not in _DTYPES or group not in W4_GROUPS:
@@ -874,8 +885,8 @@ def quant_w4(w: torch.Tensor, group: int = 128, symmetric: bool = True, dtype: t
 def _check_w4(name: str, qw: dict, dtype: torch.dtype | None = None) -> tuple:
     """(codes, scales, mins, leading shape, K, group) of a 4-bit weight."""
     codes, scales, mins, K, group = qw["codes"], qw["scales"], qw.get("mins"), int(qw["K"]), int(qw["group"])
-    if group not in W4_GROUPS or K < 1:
-        raise RuntimeError(f"{name}: need K >= 1 and a group out of {W4_GROUPS}")
+    if group not in W4_GROUPS or not 1 <= K <= _MAX_W4_K:
+        raise RuntimeError(f"{name}: need K of 1 to 2^28 and a group out of {W4_GROUPS}")
     *lead, width = codes.shape
     lead, kind = tuple(lead), scales.dtype
     if codes.dtype != torch.uint8 or not lead or width != -(-K // 32) * 16:
@@ -916,6 +927,8 @@ def gemm_w4(a: torch.Tensor, qw: dict, out: torch.Tensor | None = None, num_sms:
         raise RuntimeError(f"gemm_w4 takes a [M, {K}] and a 2-D weight")
     _contig("a", a)
     M, N = a.shape[0], lead[0]
+    if max(M, N) > 0x7fffffff:
+        raise RuntimeError(f"gemm_w4: more than 2^31 rows ({M} x {N})")
     if out is None:
         out = a.new_empty((M, N))
     elif out.shape != (M, N) or out.dtype != a.dtype or not out.is_contiguous():
@@ -1078,6 +1091,8 @@ def fused_moe_w4(hidden_states: torch.Tensor, gate_logits: torch.Tensor, qw: dic
     T = hidden_states.shape[0]
     if hidden_states.shape != (T, H):
         raise RuntimeError("fused_moe_w4: shape mismatch")
+    if not 0 <= T * int(topk) <= _MAX_W4_ROWS:
+        raise RuntimeError(f"fused_moe_w4: too many rows, or a negative number of them ({T} tokens x {topk})")
     if gate_logits.dtype != torch.float32 or gate_logits.shape != (T, E):
         raise RuntimeError("gate_logits must be float32 with one row per token and one column per expert")
     _contig("gate_logits", gate_logits)

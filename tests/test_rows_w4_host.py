@@ -305,3 +305,32 @@ def test_rows_longer_than_their_counters_are_refused(H, dtype):
     _bad(L.ek_moe_dispatch_grad(_p(), _p(), 1, 1, 1, H, dtype, _p(), n), "2^30 elements")
     _bad(L.ek_moe_combine_weighted(_p(), _p(), _p(), 1, 1, 1, H, dtype, _p(), n), "2^30 elements")
     _bad(L.ek_moe_combine_weighted_grad(_p(), _p(), _p(), _p(), _p(), 1, 1, 1, H, dtype, _p(), _p(), n), "2^30 elements")
+
+
+def test_front_end_refuses_sizes_past_32_bits(monkeypatch):
+    """They would wrap to small ones on their way into the library (2^32 + 8 to 8).
+    Shapes alone: expanded tensors of one element."""
+    monkeypatch.setattr(_ops, "_require_cuda", lambda *t: torch.device("cuda", 0))
+    one, big = torch.zeros(1, dtype=torch.bfloat16), (1 << 32) + 8
+    for shape in ((1, big), (big, 1), (1, (1 << 30) + 1)):
+        with pytest.raises(RuntimeError, match="2.30 elements"):
+            _ops._check_rows("x", one.expand(shape))
+    ids = torch.zeros(1, dtype=torch.int32)
+    for shape in ((big, 1), (1, big), (1 << 20, 1 << 11)):
+        monkeypatch.setattr(_ops, "_contig", lambda *a: None)
+        with pytest.raises(RuntimeError, match="too many slots"):
+            _ops.moe_dispatch(None, ids.expand(shape), 4)
+    for E in (big, 4 - (1 << 32)):
+        with pytest.raises(RuntimeError, match="1 <= E <= 1024"):
+            _ops.moe_dispatch(None, ids.view(1, 1), E)
+    w = torch.zeros((1, 1))
+    with pytest.raises(RuntimeError, match="2.30"):
+        _ops.moe_route_grad(ids.view(1, 1), w, w, big)
+    with pytest.raises(RuntimeError, match="2.28"):
+        _ops.quant_w4(one.expand(1, big))
+    qw = dict(codes=torch.zeros((4, 32), dtype=torch.uint8), scales=torch.zeros((4, 1), dtype=torch.bfloat16), mins=None,
+              K=64, group=64)
+    with pytest.raises(RuntimeError, match="2.28"):
+        _ops._check_w4("w", dict(qw, K=big))
+    with pytest.raises(RuntimeError, match="2.31 rows"):
+        _ops.gemm_w4(one.expand(big, 64), qw)
