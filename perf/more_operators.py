@@ -134,7 +134,8 @@ def _quantise(x, rows_per_block):
     pad = torch.zeros((rb * b, kb * _G), device=x.device)
     pad[:R, :K] = x
     v = pad.view(rb, b, kb, _G)
-    s = v.abs().amax(dim=3).amax(dim=1) / _E4M3_MAX
+    s = v.abs().amax(dim=3).amax(dim=1)
+    s = s / torch.full_like(s, _E4M3_MAX)  # a tensor: by a number, torch multiplies with the reciprocal
     s = torch.where(s == 0, torch.ones_like(s), s)
     q = (v / s[:, None, :, None]).view(rb * b, kb * _G)[:R, :K]
     return q.to(torch.float8_e4m3fn).contiguous(), s.contiguous()
@@ -251,17 +252,18 @@ def _exact_values(q, s, rows_per_block):
 
 
 def _exact_round(v):
-    """v [R, K] in 64 bits through e4m3 with a scale per 1 x 128: 3 bits of mantissa,
-    exponents from -6, halves to even; the largest of a group lands on 448."""
+    """v [R, K] in 64 bits through e4m3 with a scale per 1 x 128: the scale and the
+    quotient are fp32 by definition (a 16-bit value's quotient is often on a border),
+    then 3 bits of mantissa, exponents from -6, halves to even."""
     out = torch.empty_like(v)
     for b in range(_blocks(v.shape[1])):
         p = v[:, b * _G:(b + 1) * _G]
-        top = p.abs().amax(dim=1, keepdim=True)
-        s = torch.where(top == 0, torch.ones_like(top), (top.float() / _E4M3_MAX).double())
-        z = p / s
+        top = p.abs().amax(dim=1, keepdim=True).float()
+        s = torch.where(top == 0, torch.ones_like(top), top / torch.full_like(top, _E4M3_MAX))
+        z = (p.float() / s).double()
         exponent = (torch.frexp(z).exponent - 1).clamp(min=-6).double()
         step = torch.exp2(exponent - 3.0)
-        out[:, b * _G:(b + 1) * _G] = torch.round(z / step) * step * s
+        out[:, b * _G:(b + 1) * _G] = torch.round(z / step) * step * s.double()
     return out
 
 
