@@ -24,6 +24,10 @@ EK_DTYPE_FP32 = 3
 
 EK_QUANT_POW2_SCALES = 1
 
+EK_GATE_SILU = 0
+EK_GATE_GELU = 1
+EK_GATE_GELU_TANH = 2
+
 EK_B_KN = 0
 EK_B_NK = 1
 
@@ -132,6 +136,14 @@ _SIGNATURES = {
     "ek_moe_experts_w4": (_c_int, [_c_vp, _c_int, _c_int] + [_c_vp] * 15 + [_c_int] * 5 + [_c_vp, _c_size, _c_vp]),
     "ek_fused_moe_w4_workspace_bytes": (_c_size, [_c_int] * 6),
     "ek_fused_moe_w4": (_c_int, [_c_vp, _c_vp, _c_int, _c_int] + [_c_vp] * 10 + [_c_int] * 5 + [_c_vp, _c_size, _c_vp]),
+    "ek_gemm_fp8_block_workspace_bytes": (_c_size, [_c_int] * 4),
+    "ek_gemm_fp8_block": (_c_int, [_c_vp] * 5 + [_c_int] * 5 + [_c_vp, _c_size, _c_vp]),
+    "ek_gated_ffn_workspace_bytes": (_c_size, [_c_int] * 4),
+    "ek_gated_ffn": (_c_int, [_c_vp] * 6 + [_c_int] * 6 + [_c_vp, _c_size, _c_vp]),
+    "ek_gated_ffn_grad_workspace_bytes": (_c_size, [_c_int] * 4),
+    "ek_gated_ffn_grad": (_c_int, [_c_vp] * 9 + [_c_int] * 6 + [_c_vp, _c_size, _c_vp]),
+    "ek_gated_ffn_fp8_workspace_bytes": (_c_size, [_c_int] * 4),
+    "ek_gated_ffn_fp8": (_c_int, [_c_vp] * 8 + [_c_int] * 5 + [_c_vp, _c_size, _c_vp]),
     "ek_moe_segment_gemm": (_c_int, [_c_vp, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
                                      _c_vp]),
 }

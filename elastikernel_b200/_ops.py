@@ -1113,6 +1113,203 @@ def fused_moe_w4(hidden_states: torch.Tensor, gate_logits: torch.Tensor, qw: dic
     return out
 
 
+# ---------------------------------------------------- dense feed-forward blocks
+GATES = {"silu": _lib.EK_GATE_SILU, "gelu": _lib.EK_GATE_GELU, "gelu_tanh": _lib.EK_GATE_GELU_TANH}
+_MAX_FFN_DIM = 1 << 28  # of H and I, and _MAX_TOKENS of the rows: the library's ints
+_MAX_TOKENS = 0x7fffffff
+
+
+def _check_matrix(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple) -> torch.Tensor:
+    """t, checked and 16-byte aligned (a view that starts mid-line is copied)."""
+    if t.dtype is not dtype or tuple(t.shape) != shape:
+        raise RuntimeError(f"{name} must be a {dtype} tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}")
+    if not t.is_contiguous():
+        raise RuntimeError(f"{name} must be contiguous")
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _gate(act: str) -> int:
+    if act not in GATES:
+        raise RuntimeError(f"act must be one of {tuple(GATES)}, got {act!r}")
+    return GATES[act]
+
+
+def _blocks128(n: int) -> int:
+    return -(-n // 128)
+
+
+def gemm_fp8_block(a_q: torch.Tensor, w_q: torch.Tensor, a_scale: torch.Tensor, w_scale: torch.Tensor,
+                   out: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16,
+                   num_sms: int | None = None) -> torch.Tensor:
+    """C[M, N] = A @ W^T for e4m3 a_q [M, K] and w_q [N, K] with block scales.
+
+    a_scale [M, ceil(K/128)] holds a scale per 1 x 128 group of a row, w_scale
+    [ceil(N/128), ceil(K/128)] one per 128 x 128 block, both fp32 of any value:
+    what quant_e4m3(x, block=(1, 128)) and quant_e4m3(w, block=(128, 128)) give.
+    K is a multiple of 16; M, N and the last block of each axis are any size. The
+    sums are fp32; C is bf16, fp16 or fp32 (`dtype`, or out's), rounded once."""
+    dev = _require_cuda(a_q, w_q, a_scale, w_scale, out)
+    if _FP8 is None or a_q.dtype != _FP8 or w_q.dtype != _FP8 or a_q.dim() != 2 or w_q.dim() != 2:
+        raise RuntimeError("gemm_fp8_block takes 2-D float8_e4m3fn operands")
+    (M, K), N = a_q.shape, w_q.shape[0]
+    if K == 0 or K % 16 or K > _MAX_FFN_DIM or max(M, N) > _MAX_TOKENS:
+        raise RuntimeError(f"gemm_fp8_block: K must be a positive multiple of 16 up to 2^28, M and N within 2^31 "
+                           f"(got {M} x {N} x {K})")
+    a_q = _check_matrix("a_q", a_q, _FP8, (M, K))
+    w_q = _check_matrix("w_q", w_q, _FP8, (N, K))
+    a_scale = _check_matrix("a_scale", a_scale, torch.float32, (M, _blocks128(K)))
+    w_scale = _check_matrix("w_scale", w_scale, torch.float32, (_blocks128(N), _blocks128(K)))
+    if out is not None:
+        dtype = out.dtype
+    if dtype not in _ROW_DTYPES:
+        raise RuntimeError("gemm_fp8_block: the result is bf16, fp16 or fp32")
+    if out is None:
+        out = torch.empty((M, N), dtype=dtype, device=dev)
+    elif tuple(out.shape) != (M, N) or not out.is_contiguous():
+        raise RuntimeError("out must be a contiguous [M, N] tensor")
+    if M == 0 or N == 0:
+        return out
+    L = lib()
+    stream, sms = current_stream_handle(dev), int(num_sms or 0)
+    ws = _bytes(L.ek_gemm_fp8_block_workspace_bytes(M, N, K, _most_sms(dev, sms)), dev)
+    with _on_device(dev):
+        check(L.ek_gemm_fp8_block(a_q.data_ptr(), w_q.data_ptr(), a_scale.data_ptr(), w_scale.data_ptr(),
+                                  out.data_ptr(), M, N, K, _ROW_DTYPES[dtype], sms, ws.data_ptr(), ws.numel(), stream),
+              "ek_gemm_fp8_block")
+    return out
+
+
+def _bytes(n: int, dev: torch.device) -> torch.Tensor:
+    """Workspace of one call, as _scratch."""
+    if n == _SIZE_MAX:
+        check(_lib.EK_ERR_INVALID, "workspace size")
+    return torch.empty(n, dtype=torch.uint8, device=dev)
+
+
+def _check_ffn(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, w3: torch.Tensor, dtype: torch.dtype,
+               unit: int) -> tuple:
+    """(x, w1, w2, w3, T, H, I) of a feed-forward block, checked and aligned."""
+    if x.dim() != 2 or w1.dim() != 2:
+        raise RuntimeError("x must be [T, H] and w1 [I, H]")
+    (T, H), I = x.shape, w1.shape[0]
+    if not (0 < H <= _MAX_FFN_DIM and 0 < I <= _MAX_FFN_DIM) or H % unit or I % unit or T > _MAX_TOKENS:
+        raise RuntimeError(f"H and I must be positive multiples of {unit} up to 2^28, T within 2^31 "
+                           f"(got T={T}, H={H}, I={I})")
+    wt = dtype if unit == 8 else _FP8
+    return (_check_matrix("x", x, dtype, (T, H)), _check_matrix("w1", w1, wt, (I, H)),
+            _check_matrix("w2", w2, wt, (H, I)), _check_matrix("w3", w3, wt, (I, H)), T, H, I)
+
+
+def gated_ffn(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, w3: torch.Tensor, act: str = "silu",
+              out: torch.Tensor | None = None, save: bool = False, num_sms: int | None = None):
+    """Dense gated feed-forward block: y = (f(x W1^T) * (x W3^T)) W2^T.
+
+    x [T, H], w1 and w3 [I, H], w2 [H, I] in bf16 or fp16 (H and I multiples of 8,
+    any T); f is "silu", "gelu" or "gelu_tanh". Sums are fp32; the activations are
+    rounded to x's dtype between the two products. With save=True returns (y, h),
+    h [2, T, I] the rounded pre-activations x W1^T and x W3^T that gated_ffn_grad
+    takes."""
+    dev = _require_cuda(x, w1, w2, w3, out)
+    if x.dtype not in _DTYPES:
+        raise RuntimeError("gated_ffn takes bf16 or fp16")
+    gate, dtype = _gate(act), x.dtype
+    x, w1, w2, w3, T, H, I = _check_ffn(x, w1, w2, w3, dtype, 8)
+    y = x.new_empty((T, H)) if out is None else out
+    if out is not None and (out.dtype != dtype or tuple(out.shape) != (T, H) or not out.is_contiguous()):
+        raise RuntimeError("out must be a contiguous [T, H] tensor of x's dtype")
+    if out is not None and out.data_ptr() % 16:
+        y = x.new_empty((T, H))
+    h = x.new_empty((2, T, I)) if save else None
+    if T > 0:
+        L = lib()
+        stream, sms = current_stream_handle(dev), int(num_sms or 0)
+        ws = _bytes(L.ek_gated_ffn_workspace_bytes(T, H, I, _most_sms(dev, sms)), dev)
+        with _on_device(dev):
+            check(L.ek_gated_ffn(x.data_ptr(), w1.data_ptr(), w2.data_ptr(), w3.data_ptr(), y.data_ptr(), _ptr(h), T, H,
+                                 I, _DTYPES[dtype], gate, sms, ws.data_ptr(), ws.numel(), stream), "ek_gated_ffn")
+    if out is not None and y is not out:
+        y = out.copy_(y)
+    return (y, h) if save else y
+
+
+def gated_ffn_grad(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, w3: torch.Tensor, h: torch.Tensor,
+                   d_out: torch.Tensor, act: str = "silu", num_sms: int | None = None) -> tuple:
+    """Gradients (d_x, d_w1, d_w2, d_w3) of gated_ffn from the h it saved and the
+    gradient d_out [T, H] of its result, all in x's dtype.
+
+    The gradients of the pre-activations and the activations (made again from h)
+    are rounded to that dtype between the products; sums are fp32. d_w1 and d_w3
+    are the two halves of one buffer."""
+    dev = _require_cuda(x, w1, w2, w3, h, d_out)
+    if x.dtype not in _DTYPES:
+        raise RuntimeError("gated_ffn_grad takes bf16 or fp16")
+    gate, dtype = _gate(act), x.dtype
+    x, w1, w2, w3, T, H, I = _check_ffn(x, w1, w2, w3, dtype, 8)
+    h = _check_matrix("h", h, dtype, (2, T, I))
+    d_out = _check_matrix("d_out", d_out, dtype, (T, H))
+    d_x, d_w13, d_w2 = x.new_empty((T, H)), x.new_empty((2, I, H)), x.new_empty((H, I))
+    L = lib()
+    stream, sms = current_stream_handle(dev), int(num_sms or 0)
+    ws = _bytes(L.ek_gated_ffn_grad_workspace_bytes(T, H, I, _most_sms(dev, sms)), dev)
+    with _on_device(dev):
+        check(L.ek_gated_ffn_grad(x.data_ptr(), w1.data_ptr(), w2.data_ptr(), w3.data_ptr(), h.data_ptr(),
+                                  d_out.data_ptr(), d_x.data_ptr(), d_w13.data_ptr(), d_w2.data_ptr(), T, H, I,
+                                  _DTYPES[dtype], gate, sms, ws.data_ptr(), ws.numel(), stream), "ek_gated_ffn_grad")
+    return d_x, d_w13[0], d_w2, d_w13[1]
+
+
+def quant_ffn_weights_fp8(w1: torch.Tensor, w2: torch.Tensor, w3: torch.Tensor) -> dict:
+    """e4m3 weights of a gated block (w1, w3 [I, H], w2 [H, I]; bf16 or fp32) with
+    128 x 128 fp32 block scales, for gated_ffn_fp8."""
+    I, H = w1.shape
+    if w3.shape != w1.shape or tuple(w2.shape) != (H, I):
+        raise RuntimeError("quant_ffn_weights_fp8: w1 and w3 must be [I, H] and w2 [H, I]")
+    out = {"H": H, "I": I}
+    for name, w in (("w1", w1), ("w3", w3), ("w2", w2)):
+        out[name + "q"], out[name + "s"] = quant_e4m3(w, block=(128, 128))
+    return out
+
+
+def gated_ffn_fp8(x: torch.Tensor, qw: dict, act: str = "silu", out: torch.Tensor | None = None,
+                  num_sms: int | None = None) -> torch.Tensor:
+    """gated_ffn over e4m3 weights with block scales (quant_ffn_weights_fp8), bf16 x
+    and y [T, H], H and I multiples of 16.
+
+    The tokens, and the activations from their fp32 sums, are quantised per 1 x 128
+    group as quant_e4m3(x, block=(1, 128)) does; both products are
+    gemm_fp8_block's. The result is rounded once."""
+    H, I = int(qw["H"]), int(qw["I"])
+    w1, w3, w2, s1, s3, s2 = (qw[n] for n in ("w1q", "w3q", "w2q", "w1s", "w3s", "w2s"))
+    dev = _require_cuda(x, w1, w2, w3, s1, s2, s3, out)
+    if x.dtype != torch.bfloat16 or _FP8 is None:
+        raise RuntimeError("gated_ffn_fp8 takes bfloat16 tokens")
+    gate = _gate(act)
+    x, w1, w2, w3, T, Hx, Iw = _check_ffn(x, w1, w2, w3, torch.bfloat16, 16)
+    if (Hx, Iw) != (H, I):
+        raise RuntimeError(f"gated_ffn_fp8: x and weights of H={Hx}, I={Iw}, the dict says H={H}, I={I}")
+    bh, bi = _blocks128(H), _blocks128(I)
+    s1 = _check_matrix("w1s", s1, torch.float32, (bi, bh))
+    s3 = _check_matrix("w3s", s3, torch.float32, (bi, bh))
+    s2 = _check_matrix("w2s", s2, torch.float32, (bh, bi))
+    if out is None:
+        out = x.new_empty((T, H))
+    else:
+        _check_bf16("out", out)
+        if tuple(out.shape) != (T, H):
+            raise RuntimeError("out must be a [T, H] tensor")
+    if T == 0:
+        return out
+    y = out if out.data_ptr() % 16 == 0 else x.new_empty((T, H))
+    L = lib()
+    stream, sms = current_stream_handle(dev), int(num_sms or 0)
+    ws = _bytes(L.ek_gated_ffn_fp8_workspace_bytes(T, H, I, _most_sms(dev, sms)), dev)
+    with _on_device(dev):
+        check(L.ek_gated_ffn_fp8(x.data_ptr(), w1.data_ptr(), w2.data_ptr(), w3.data_ptr(), s1.data_ptr(),
+                                 s2.data_ptr(), s3.data_ptr(), y.data_ptr(), T, H, I, gate, sms, ws.data_ptr(),
+                                 ws.numel(), stream), "ek_gated_ffn_fp8")
+    return out if y is out else out.copy_(y)
+
+
 def moe_segment_gemm(hidden_states: torch.Tensor, weights: torch.Tensor, expert_offsets: torch.Tensor,
                      num_experts: int, N: int, K: int, num_sms: int | None = None,
                      out: torch.Tensor | None = None) -> torch.Tensor:

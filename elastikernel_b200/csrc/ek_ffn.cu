@@ -1,0 +1,579 @@
+// Entry points of the dense feed-forward operators: the block-scaled e4m3 product,
+// the gated block in 16 bits and its gradients, and the gated block in 8 bits.
+// Up to kStreamTokens tokens the products run in stream_kernel, whose time is the
+// weights' bytes; past it in the 256 x 256 CTA-pair kernels.
+#include <algorithm>
+#include <cmath>
+
+#include "ek_fp8_block_kernel.cuh"
+#include "ek_internal.h"
+
+namespace ek {
+
+int register_status_reader(int (*fn)(int, int*));
+
+namespace {
+
+int read_status(int clear, int* v) {
+  int rc = check_cuda(cudaMemcpyFromSymbol(v, g_ek_status, sizeof(int)), "read status");
+  if (rc) return rc;
+  if (clear) {
+    int z = 0;
+    rc = check_cuda(cudaMemcpyToSymbol(g_ek_status, &z, sizeof(int)), "clear status");
+  }
+  return rc;
+}
+const int s_status_reg = register_status_reader(read_status);
+
+constexpr int kStreamTokens = 128;
+constexpr size_t kBad = (size_t)-1;
+
+size_t round256(size_t x) { return (x + 255) / 256 * 256; }
+int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
+
+template <class Kernel>
+int allow_smem(Kernel kernel, int bytes, bool (&done)[64]) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return set_error(EK_ERR_CUDA, "device index out of range");
+  if (done[dev]) return EK_OK;
+  const int rc = check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes),
+                            "cudaFuncSetAttribute(smem)");
+  done[dev] = rc == EK_OK;
+  return rc;
+}
+
+// cluster: CTAs per cluster (0: none); overlap: may start before its predecessor
+// on the stream has ended, which must be a launch of the same call
+template <class... P, class... A>
+int launch(const char* what, void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t stream, int cluster,
+           bool overlap, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (cluster) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = cluster;
+    attr[n].val.clusterDim.y = 1;
+    attr[n++].val.clusterDim.z = 1;
+  }
+  if (overlap) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  return check_cuda(cudaLaunchKernelEx(&cfg, kernel, args...), what);
+}
+
+CUtensorMapDataType map_type(int dtype) {
+  return dtype == EK_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+         : dtype == EK_DTYPE_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+}
+int elem_size(int dtype) { return dtype == EK_DTYPE_E4M3 ? 1 : 2; }
+
+// rows x k, the reduction axis contiguous: boxes of box_rows rows x 128 bytes
+int map_k(CUtensorMap* m, const void* base, int dtype, int rows, int k, int box_rows) {
+  const int es = elem_size(dtype);
+  return make_tmap_2d(m, base, map_type(dtype), k, rows, (uint64_t)k * es, 128 / es, box_rows);
+}
+// k x cols, the reduction axis outermost (16 bits): both 64-column chunks of a box
+// of 128 columns x 64 of K in one 3-D box where every row holds whole chunks
+int map_mn(CUtensorMap* m, const void* base, int dtype, int k, int cols, int* box3) {
+  *box3 = cols % 64 == 0;
+  if (*box3) return make_tmap_3d(m, base, map_type(dtype), 64, k, cols / 64, (uint64_t)cols * 2, 128, 64, 64, 2);
+  return make_tmap_2d(m, base, map_type(dtype), cols, k, (uint64_t)cols * 2, 64, 64);
+}
+
+int grid_for(long long work, int sms) { return (int)std::max<long long>(1, std::min<long long>(work, (long long)sms * 8)); }
+
+// ------------------------------------------------------------------ splitting K
+// Slices per tile of a pair kernel: with rounds(s) = ceil(tiles s / pairs) units
+// of k_blocks / s one after the other, each block of K costing t_kb and each unit
+// its fill and its last epilogue, against the sums' way to memory and back and one
+// more launch. cap: bytes the workspace has for the sums.
+int pick_splits(long long tiles, int k_blocks, int pairs, long long elems, double t_kb, size_t cap) {
+  constexpr double kUnitUs = 2.5, kReduceUs = 3.0, kBytesPerUs = 4.0e6;
+  int best = 1;
+  double best_us = 1e30;
+  for (int s = 1; s <= 32 && (s == 1 || k_blocks / s >= 4); ++s) {
+    const size_t bytes = (size_t)s * elems * 4;
+    if (s > 1 && bytes > cap) break;
+    const double rounds = std::ceil((double)(tiles * s) / pairs);
+    double us = rounds * (std::ceil((double)k_blocks / s) * t_kb + kUnitUs);
+    if (s > 1) us += kReduceUs + 2.0 * bytes / kBytesPerUs;
+    if (us < 0.95 * best_us) {
+      best_us = us;
+      best = s;
+    }
+  }
+  return best;
+}
+constexpr double kFfnBlockUs = 0.30, kFp8BlockUs = 0.40;
+constexpr size_t kMostSplitBytes = 256u << 20;
+
+// ------------------------------------------------------------------ few tokens
+StreamSplit stream_split(int rows, int rows_per_tile, int k, int bk, int sms) {
+  StreamSplit s;
+  s.tiles = ceil_div(rows, rows_per_tile);
+  s.k_blocks = ceil_div(k, bk);
+  const long long units = (long long)s.tiles * s.k_blocks;
+  s.per_cta = (int)std::max<long long>(2, (units + sms - 1) / sms);
+  s.ctas = ceil_div(units, s.per_cta);
+  s.max_segs = (s.per_cta - 1 + s.k_blocks - 1) / s.k_blocks + 1;
+  return s;
+}
+size_t stream_bytes(const StreamSplit& s, int T) { return (size_t)s.ctas * s.max_segs * T * 256 * 4; }
+// for any number of SMs up to sms (a smaller partition has fewer, longer runs)
+size_t stream_bytes_most(int rows, int rows_per_tile, int T, int sms) {
+  return ((size_t)ceil_div(rows, rows_per_tile) + 2 * (size_t)sms + 8) * T * 256 * 4;
+}
+
+template <class Cfg>
+int launch_stream(const CUtensorMap& tw, const CUtensorMap& tw2, const CUtensorMap& tx, const StreamParams& p,
+                  cudaStream_t s, bool overlap) {
+  static bool done[64] = {false};
+  const int rc = allow_smem(stream_kernel<Cfg>, Cfg::SMEM_BYTES, done);
+  if (rc) return rc;
+  return launch("stream product", stream_kernel<Cfg>, dim3(p.sp.ctas), Cfg::THREADS, Cfg::SMEM_BYTES, s, 0, overlap, tw,
+                tw2, tx, p);
+}
+
+template <int kElem, bool kGate>
+int launch_stream_nt(const void* w, const void* w2, const void* x, int rows, int K, StreamParams& p, cudaStream_t s,
+                     bool overlap) {
+  const int nt = p.T <= 16 ? 16 : p.T <= 32 ? 32 : p.T <= 64 ? 64 : 128;
+  CUtensorMap tw, tw2, tx;
+  int rc = map_k(&tw, w, kElem, rows, K, kGate ? 128 : 256);
+  if (rc) return rc;
+  tw2 = tw;
+  if (kGate && (rc = map_k(&tw2, w2, kElem, rows, K, 128))) return rc;
+  if ((rc = map_k(&tx, x, kElem, p.T, K, nt))) return rc;
+  switch (nt) {
+    case 16: return launch_stream<StreamCfg<kElem, 16, kGate>>(tw, tw2, tx, p, s, overlap);
+    case 32: return launch_stream<StreamCfg<kElem, 32, kGate>>(tw, tw2, tx, p, s, overlap);
+    case 64: return launch_stream<StreamCfg<kElem, 64, kGate>>(tw, tw2, tx, p, s, overlap);
+    default: return launch_stream<StreamCfg<kElem, 128, kGate>>(tw, tw2, tx, p, s, overlap);
+  }
+}
+
+struct StreamScales {
+  const float *tok = nullptr, *w = nullptr, *w2 = nullptr;
+};
+
+// out[t, n] = x[t] . w[n]
+int stream_store(int dtype, const void* w, const void* x, const StreamScales& sc, int T, int N, int K, void* out,
+                 int out_type, int sms, void* ws, size_t ws_bytes, cudaStream_t s, bool overlap) {
+  StreamParams p{};
+  p.sp = stream_split(N, 256, K, 128 / elem_size(dtype), sms);
+  if (ws_bytes < stream_bytes(p.sp, T)) return set_error(EK_ERR_INVALID, "workspace too small");
+  p.T = T;
+  p.tok_scale = sc.tok;
+  p.w_scale = sc.w;
+  p.w_blocks = ceil_div(N, 128);
+  p.ws = static_cast<float*>(ws);
+  int rc = dtype == EK_DTYPE_BF16 ? launch_stream_nt<kBF16, false>(w, w, x, N, K, p, s, overlap)
+           : dtype == EK_DTYPE_FP16 ? launch_stream_nt<kFP16, false>(w, w, x, N, K, p, s, overlap)
+                                    : launch_stream_nt<kE4M3, false>(w, w, x, N, K, p, s, overlap);
+  if (rc) return rc;
+  return launch("stream sums", stream_store_reduce_kernel, dim3(p.sp.tiles, T), 256, 0, s, 0, true, p.sp,
+                (const float*)p.ws, T, N, out, out_type);
+}
+
+// a[t, i] = f(x[t] . w1[i]) (x[t] . w3[i]); e4m3: codes and scales of a
+int stream_gate(int dtype, const void* w1, const void* w3, const void* x, const StreamScales& sc, int T, int I, int H,
+                int gate, void* a, void* h, uint8_t* codes, float* scales, int sms, void* ws, size_t ws_bytes,
+                cudaStream_t s, bool overlap) {
+  StreamParams p{};
+  p.sp = stream_split(I, 128, H, 128 / elem_size(dtype), sms);
+  if (ws_bytes < stream_bytes(p.sp, T)) return set_error(EK_ERR_INVALID, "workspace too small");
+  p.T = T;
+  p.tok_scale = sc.tok;
+  p.w_scale = sc.w;
+  p.w_scale2 = sc.w2;
+  p.w_blocks = ceil_div(I, 128);
+  p.ws = static_cast<float*>(ws);
+  int rc = dtype == EK_DTYPE_BF16 ? launch_stream_nt<kBF16, true>(w1, w3, x, I, H, p, s, overlap)
+           : dtype == EK_DTYPE_FP16 ? launch_stream_nt<kFP16, true>(w1, w3, x, I, H, p, s, overlap)
+                                    : launch_stream_nt<kE4M3, true>(w1, w3, x, I, H, p, s, overlap);
+  if (rc) return rc;
+  return launch("stream gate", stream_gate_reduce_kernel, dim3(p.sp.tiles, T), 128, 0, s, 0, true, p.sp,
+                (const float*)p.ws, T, I, gate, dtype, a, h, codes, scales);
+}
+
+// ------------------------------------------------------------------ 16-bit tiles
+template <class Cfg>
+int launch_ffn(const CUtensorMap (&ta)[2], const CUtensorMap (&tb)[2], FfnParams& p, int sms, cudaStream_t s) {
+  static bool done[64] = {false};
+  const int rc = allow_smem(ffn_gemm_kernel<Cfg>, Cfg::SMEM_BYTES, done);
+  if (rc) return rc;
+  const long long units = (long long)p.tiles_m * p.tiles_n * p.splits;
+  if (units > 0x3fffffff) return set_error(EK_ERR_INVALID, "too many tiles");
+  p.num_units = (int)units;
+  const int pairs = (int)std::min<long long>(std::max(1, sms / 2), units);
+  return launch("feed-forward product", ffn_gemm_kernel<Cfg>, dim3(2 * pairs), Cfg::THREADS, Cfg::SMEM_BYTES, s, 2, false,
+                ta[0], ta[1], tb[0], tb[1], p);
+}
+
+struct FfnOperand {
+  const void* base[2];
+  int planes;
+};
+
+// C (planes_m stacked planes) = A . B with K = k per plane. ws holds the sums of a split.
+template <int kElem, bool kAMN, bool kBMN>
+int ffn_store(const FfnOperand& A, const FfnOperand& B, int M, int N, int k, int planes_m, int planes_k, void* C, int sms,
+              void* ws, size_t ws_bytes, cudaStream_t s) {
+  CUtensorMap ta[2], tb[2];
+  FfnParams p{};
+  for (int i = 0; i < 2; ++i) {
+    const void* a = A.base[A.planes > 1 ? i : 0];
+    const void* b = B.base[B.planes > 1 ? i : 0];
+    int rc = kAMN ? map_mn(&ta[i], a, kElem, k, M, &p.a_box3) : map_k(&ta[i], a, kElem, M, k, 128);
+    if (rc) return rc;
+    rc = kBMN ? map_mn(&tb[i], b, kElem, k, N, &p.b_box3) : map_k(&tb[i], b, kElem, N, k, 128);
+    if (rc) return rc;
+  }
+  p.M = M;
+  p.N = N;
+  p.m_tiles_plane = ceil_div(M, 256);
+  p.tiles_m = p.m_tiles_plane * planes_m;
+  p.tiles_n = ceil_div(N, 256);
+  p.kb_plane = ceil_div(k, 64);
+  p.k_blocks = p.kb_plane * planes_k;
+  p.C = C;
+  p.c_plane = (long long)M * N;
+  p.ws = static_cast<float*>(ws);
+  const long long elems = (long long)planes_m * M * N;
+  p.splits = pick_splits((long long)p.tiles_m * p.tiles_n, p.k_blocks, std::max(1, sms / 2), elems, kFfnBlockUs, ws_bytes);
+  int rc = launch_ffn<FfnCfg<kElem, kAMN, kBMN, kFfnStore>>(ta, tb, p, sms, s);
+  if (rc || p.splits == 1) return rc;
+  const long long n8 = elems / 8;
+  return launch("feed-forward sums", ffn_reduce_kernel<kElem>, dim3(grid_for((n8 + 255) / 256, sms)), 256, 0, s, 0, false,
+                (const float*)p.ws, p.splits, n8, C);
+}
+
+size_t ffn_store_bytes(int M, int N, int k, int planes_m, int planes_k, int sms) {
+  const long long tiles = (long long)ceil_div(M, 256) * planes_m * ceil_div(N, 256), elems = (long long)planes_m * M * N;
+  const int s = pick_splits(tiles, ceil_div(k, 64) * planes_k, std::max(1, sms / 2), elems, kFfnBlockUs, kMostSplitBytes);
+  return s > 1 ? (size_t)s * elems * 4 : 0;
+}
+
+template <int kElem>
+int ffn_gate(const void* x, const void* w1, const void* w3, void* a, void* h, int T, int H, int I, int gate, int sms,
+             cudaStream_t s) {
+  CUtensorMap ta[2], tb[2];
+  int rc = map_k(&ta[0], x, kElem, T, H, 128);
+  if (rc || (rc = map_k(&tb[0], w1, kElem, I, H, 128)) || (rc = map_k(&tb[1], w3, kElem, I, H, 128))) return rc;
+  ta[1] = ta[0];
+  FfnParams p{};
+  p.M = T;
+  p.N = I;
+  p.tiles_m = p.m_tiles_plane = ceil_div(T, 256);
+  p.tiles_n = ceil_div(I, 128);
+  p.k_blocks = p.kb_plane = ceil_div(H, 64);
+  p.splits = 1;
+  p.gate = gate;
+  p.C = a;
+  p.H = h;
+  p.h_plane = (long long)T * I;
+  return launch_ffn<FfnCfg<kElem, false, false, kFfnGate>>(ta, tb, p, sms, s);
+}
+
+template <int kElem>
+int gated_ffn(const void* x, const void* w1, const void* w2, const void* w3, void* y, void* h, int T, int H, int I,
+              int gate, int sms, char* ws, size_t ws_bytes, cudaStream_t s) {
+  const size_t a_bytes = round256((size_t)T * I * 2);
+  if (ws_bytes < a_bytes) return set_error(EK_ERR_INVALID, "workspace of at least %zu bytes required", a_bytes);
+  void* a = ws;
+  char* rest = ws + a_bytes;
+  const size_t rest_bytes = ws_bytes - a_bytes;
+  int rc;
+  if (T <= kStreamTokens) {
+    rc = stream_gate(kElem, w1, w3, x, {}, T, I, H, gate, a, h, nullptr, nullptr, sms, rest, rest_bytes, s, false);
+    if (rc) return rc;
+    return stream_store(kElem, w2, a, {}, T, H, I, y, kElem, sms, rest, rest_bytes, s, true);
+  }
+  rc = ffn_gate<kElem>(x, w1, w3, a, h, T, H, I, gate, sms, s);
+  if (rc) return rc;
+  return ffn_store<kElem, false, false>({{a}, 1}, {{w2}, 1}, T, H, I, 1, 1, y, sms, rest, rest_bytes, s);
+}
+
+template <int kElem>
+int gated_ffn_grad(const void* x, const void* w1, const void* w2, const void* w3, const void* h, const void* d_out,
+                   void* d_x, void* d_w13, void* d_w2, int T, int H, int I, int gate, int sms, char* ws, size_t ws_bytes,
+                   cudaStream_t s) {
+  const size_t plane = (size_t)T * I * 2, dh_bytes = round256(2 * plane), a_bytes = round256(plane);
+  if (ws_bytes < dh_bytes + a_bytes)
+    return set_error(EK_ERR_INVALID, "workspace of at least %zu bytes required", dh_bytes + a_bytes);
+  char* dh = ws;
+  char* a = dh + dh_bytes;
+  char* rest = a + a_bytes;
+  const size_t rest_bytes = ws_bytes - dh_bytes - a_bytes;
+  CUtensorMap ta[2], tb[2];
+  FfnParams p{};
+  int rc = map_k(&ta[0], d_out, kElem, T, H, 128);
+  if (rc || (rc = map_mn(&tb[0], w2, kElem, H, I, &p.b_box3))) return rc;
+  ta[1] = ta[0];
+  tb[1] = tb[0];
+  p.M = T;
+  p.N = I;
+  p.tiles_m = p.m_tiles_plane = ceil_div(T, 256);
+  p.tiles_n = ceil_div(I, 256);
+  p.k_blocks = p.kb_plane = ceil_div(H, 64);
+  p.splits = 1;
+  p.gate = gate;
+  p.C = dh;
+  p.H = const_cast<void*>(h);
+  p.c_plane = p.h_plane = (long long)T * I;
+  p.Act = a;
+  if ((rc = launch_ffn<FfnCfg<kElem, false, true, kFfnGateGrad>>(ta, tb, p, sms, s))) return rc;
+  const FfnOperand dh_planes = {{dh, dh + plane}, 2};
+  // plane 1 of dh starts on a 16-byte boundary: a plane is T * I elements, I a multiple of 8
+  if ((rc = ffn_store<kElem, false, true>(dh_planes, {{w1, w3}, 2}, T, H, I, 1, 2, d_x, sms, rest, rest_bytes, s)))
+    return rc;
+  if ((rc = ffn_store<kElem, true, true>(dh_planes, {{x}, 1}, I, H, T, 2, 1, d_w13, sms, rest, rest_bytes, s))) return rc;
+  return ffn_store<kElem, true, true>({{d_out}, 1}, {{a}, 1}, H, I, T, 1, 1, d_w2, sms, rest, rest_bytes, s);
+}
+
+// ------------------------------------------------------------------ 8-bit tiles
+template <bool kGate>
+int launch_fp8(const void* a, const void* w, const void* w2, int K, Fp8BlockParams& p, int sms, cudaStream_t s) {
+  using Cfg = Fp8BlockCfg<kGate>;
+  CUtensorMap ta, tb, tb2;
+  int rc = map_k(&ta, a, EK_DTYPE_E4M3, p.M, K, 128);
+  if (rc || (rc = map_k(&tb, w, EK_DTYPE_E4M3, p.N, K, 128))) return rc;
+  tb2 = tb;
+  if (kGate && (rc = map_k(&tb2, w2, EK_DTYPE_E4M3, p.N, K, 128))) return rc;
+  static bool done[64] = {false};
+  if ((rc = allow_smem(fp8_block_kernel<Cfg>, Cfg::SMEM_BYTES, done))) return rc;
+  const long long units = (long long)p.tiles_m * p.tiles_n * p.splits;
+  if (units > 0x3fffffff) return set_error(EK_ERR_INVALID, "too many tiles");
+  p.num_units = (int)units;
+  const int pairs = (int)std::min<long long>(std::max(1, sms / 2), units);
+  return launch("block-scaled product", fp8_block_kernel<Cfg>, dim3(2 * pairs), Cfg::THREADS, Cfg::SMEM_BYTES, s, 2, false,
+                ta, tb, tb2, p);
+}
+
+int fp8_splits(int M, int N, int K, int sms, size_t cap) {
+  return pick_splits((long long)ceil_div(M, 256) * ceil_div(N, 256), ceil_div(K, 128), std::max(1, sms / 2),
+                     (long long)M * N, kFp8BlockUs, cap);
+}
+
+int fp8_store(const void* a, const void* w, const float* as, const float* wsc, void* C, int M, int N, int K, int out_type,
+              int sms, void* ws, size_t ws_bytes, cudaStream_t s, bool overlap) {
+  if (M <= kStreamTokens)
+    return stream_store(EK_DTYPE_E4M3, w, a, {as, wsc, nullptr}, M, N, K, C, out_type, sms, ws, ws_bytes, s, overlap);
+  Fp8BlockParams p{};
+  p.M = M;
+  p.N = N;
+  p.tiles_m = ceil_div(M, 256);
+  p.tiles_n = ceil_div(N, 256);
+  p.k_blocks = ceil_div(K, 128);
+  p.splits = fp8_splits(M, N, K, sms, ws_bytes);
+  p.a_scale = as;
+  p.w_scale = wsc;
+  p.w_blocks = ceil_div(N, 128);
+  p.C = C;
+  p.out_type = out_type;
+  p.wide = aligned16(C) && (size_t)N * (out_type == kOutFP32 ? 4 : 2) % 16 == 0;
+  p.ws = static_cast<float*>(ws);
+  int rc = launch_fp8<false>(a, w, w, K, p, sms, s);
+  if (rc || p.splits == 1) return rc;
+  const long long n = (long long)M * N;
+  return launch("block-scaled sums", fp8_block_reduce_kernel, dim3(grid_for((n + 255) / 256, sms)), 256, 0, s, 0, false,
+                (const float*)p.ws, p.splits, n, C, out_type);
+}
+
+size_t fp8_store_bytes(int M, int N, int K, int sms) {
+  if (M <= kStreamTokens) return stream_bytes_most(N, 256, M, sms);
+  const int s = fp8_splits(M, N, K, sms, kMostSplitBytes);
+  return s > 1 ? (size_t)s * M * N * 4 : 0;
+}
+
+struct Fp8FfnLayout {
+  size_t xq, xs, aq, as, rest, total;
+};
+Fp8FfnLayout fp8_ffn_layout(int T, int H, int I, int sms) {
+  Fp8FfnLayout L;
+  L.xq = 0;
+  L.xs = L.xq + round256((size_t)T * H);
+  L.aq = L.xs + round256((size_t)T * ceil_div(H, 128) * 4);
+  L.as = L.aq + round256((size_t)T * I);
+  L.rest = L.as + round256((size_t)T * ceil_div(I, 128) * 4);
+  const size_t gate = T <= kStreamTokens ? stream_bytes_most(I, 128, T, sms) : 0;
+  L.total = L.rest + std::max(gate, fp8_store_bytes(T, H, I, sms));
+  return L;
+}
+
+// ------------------------------------------------------------------ checks
+bool sizes_ok(int T, int H, int I, int unit) {
+  return T >= 0 && H > 0 && I > 0 && H % unit == 0 && I % unit == 0 && H <= (1 << 28) && I <= (1 << 28);
+}
+bool sms_ok(int sms) { return sms > 0 && sms <= kGemmMaxSms; }
+
+int check_ffn(int T, int H, int I, int unit, int gate) {
+  if (!sizes_ok(T, H, I, unit))
+    return set_error(EK_ERR_INVALID, "feed-forward: H and I must be positive multiples of %d up to 2^28 (got T=%d H=%d I=%d)",
+                     unit, T, H, I);
+  if (gate < kGateSilu || gate > kGateGeluTanh) return set_error(EK_ERR_INVALID, "unknown gate function %d", gate);
+  return EK_OK;
+}
+
+template <class... P>
+bool all_aligned(P... p) {
+  return (aligned16(p) && ...);
+}
+template <class... P>
+bool all_set(P... p) {
+  return ((p != nullptr) && ...);
+}
+
+int resolve(int num_sms, void* stream, int* sms) {
+  const int rc = resolve_num_sms(num_sms, stream, sms);
+  if (rc) return rc;
+  if (!sms_ok(*sms)) return set_error(EK_ERR_INVALID, "num_sms must be in [1, %d], got %d", kGemmMaxSms, *sms);
+  return EK_OK;
+}
+
+}  // namespace
+}  // namespace ek
+
+using namespace ek;
+
+extern "C" {
+
+size_t ek_gemm_fp8_block_workspace_bytes(int M, int N, int K, int num_sms) {
+  if (M < 0 || N < 0 || K <= 0 || K % 16 || !sms_ok(num_sms)) return kBad;
+  return M == 0 || N == 0 ? 0 : fp8_store_bytes(M, N, K, num_sms);
+}
+
+int ek_gemm_fp8_block(const void* A, const void* W, const float* a_scale, const float* w_scale, void* C, int M, int N,
+                      int K, int out_dtype, int num_sms, void* workspace, size_t ws_bytes, void* stream) {
+  clear_error();
+  if (M < 0 || N < 0 || K <= 0 || K % 16)
+    return set_error(EK_ERR_INVALID, "block-scaled product: K must be a positive multiple of 16 (got %d x %d x %d)", M, N, K);
+  if (out_dtype != kOutBF16 && out_dtype != kOutFP16 && out_dtype != kOutFP32)
+    return set_error(EK_ERR_INVALID, "block-scaled product: result in bf16, fp16 or fp32 (got dtype %d)", out_dtype);
+  if (M == 0 || N == 0) return EK_OK;
+  if (!all_set(A, W, a_scale, w_scale, C)) return set_error(EK_ERR_INVALID, "null operand");
+  if (!all_aligned(A, W, workspace)) return set_error(EK_ERR_INVALID, "operands must be 16-byte aligned");
+  int sms = 0;
+  const int rc = resolve(num_sms, stream, &sms);
+  if (rc) return rc;
+  return fp8_store(A, W, a_scale, w_scale, C, M, N, K, out_dtype, sms, workspace, workspace ? ws_bytes : 0,
+                   static_cast<cudaStream_t>(stream), false);
+}
+
+size_t ek_gated_ffn_workspace_bytes(int T, int H, int I, int num_sms) {
+  if (!sizes_ok(T, H, I, 8) || !sms_ok(num_sms)) return kBad;
+  if (T == 0) return 0;
+  const size_t sums = T <= kStreamTokens
+                          ? std::max(stream_bytes_most(I, 128, T, num_sms), stream_bytes_most(H, 256, T, num_sms))
+                          : ffn_store_bytes(T, H, I, 1, 1, num_sms);
+  return round256((size_t)T * I * 2) + sums;
+}
+
+int ek_gated_ffn(const void* x, const void* w1, const void* w2, const void* w3, void* y, void* h, int T, int H, int I,
+                 int dtype, int gate, int num_sms, void* workspace, size_t ws_bytes, void* stream) {
+  clear_error();
+  int rc = check_ffn(T, H, I, 8, gate);
+  if (rc) return rc;
+  if (dtype != EK_DTYPE_BF16 && dtype != EK_DTYPE_FP16)
+    return set_error(EK_ERR_INVALID, "feed-forward takes bf16 or fp16 (got dtype %d)", dtype);
+  if (T == 0) return EK_OK;
+  if (!all_set(x, w1, w2, w3, y, workspace)) return set_error(EK_ERR_INVALID, "null operand");
+  if (!all_aligned(x, w1, w2, w3, y, h, workspace))
+    return set_error(EK_ERR_INVALID, "operands must be 16-byte aligned");
+  int sms = 0;
+  if ((rc = resolve(num_sms, stream, &sms))) return rc;
+  const auto f = dtype == EK_DTYPE_BF16 ? gated_ffn<kBF16> : gated_ffn<kFP16>;
+  return f(x, w1, w2, w3, y, h, T, H, I, gate, sms, static_cast<char*>(workspace), ws_bytes,
+           static_cast<cudaStream_t>(stream));
+}
+
+size_t ek_gated_ffn_grad_workspace_bytes(int T, int H, int I, int num_sms) {
+  if (!sizes_ok(T, H, I, 8) || !sms_ok(num_sms)) return kBad;
+  if (T == 0) return 0;
+  const size_t sums = std::max({ffn_store_bytes(T, H, I, 1, 2, num_sms), ffn_store_bytes(I, H, T, 2, 1, num_sms),
+                                ffn_store_bytes(H, I, T, 1, 1, num_sms)});
+  return round256((size_t)T * I * 4) + round256((size_t)T * I * 2) + sums;
+}
+
+int ek_gated_ffn_grad(const void* x, const void* w1, const void* w2, const void* w3, const void* h, const void* d_out,
+                      void* d_x, void* d_w13, void* d_w2, int T, int H, int I, int dtype, int gate, int num_sms,
+                      void* workspace, size_t ws_bytes, void* stream) {
+  clear_error();
+  int rc = check_ffn(T, H, I, 8, gate);
+  if (rc) return rc;
+  if (dtype != EK_DTYPE_BF16 && dtype != EK_DTYPE_FP16)
+    return set_error(EK_ERR_INVALID, "feed-forward takes bf16 or fp16 (got dtype %d)", dtype);
+  if (!all_set(d_w13, d_w2)) return set_error(EK_ERR_INVALID, "null operand");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (T == 0) {  // sums over no token
+    rc = check_cuda(cudaMemsetAsync(d_w13, 0, (size_t)I * H * 4, s), "feed-forward gradient");
+    return rc ? rc : check_cuda(cudaMemsetAsync(d_w2, 0, (size_t)I * H * 2, s), "feed-forward gradient");
+  }
+  if (!all_set(x, w1, w2, w3, h, d_out, d_x, workspace)) return set_error(EK_ERR_INVALID, "null operand");
+  if (!all_aligned(x, w1, w2, w3, h, d_out, d_x, d_w13, d_w2, workspace))
+    return set_error(EK_ERR_INVALID, "operands must be 16-byte aligned");
+  int sms = 0;
+  if ((rc = resolve(num_sms, stream, &sms))) return rc;
+  const auto f = dtype == EK_DTYPE_BF16 ? gated_ffn_grad<kBF16> : gated_ffn_grad<kFP16>;
+  return f(x, w1, w2, w3, h, d_out, d_x, d_w13, d_w2, T, H, I, gate, sms, static_cast<char*>(workspace), ws_bytes, s);
+}
+
+size_t ek_gated_ffn_fp8_workspace_bytes(int T, int H, int I, int num_sms) {
+  if (!sizes_ok(T, H, I, 16) || !sms_ok(num_sms)) return kBad;
+  return T == 0 ? 0 : fp8_ffn_layout(T, H, I, num_sms).total;
+}
+
+int ek_gated_ffn_fp8(const void* x, const void* w1, const void* w2, const void* w3, const float* s1, const float* s2,
+                     const float* s3, void* y, int T, int H, int I, int gate, int num_sms, void* workspace,
+                     size_t ws_bytes, void* stream) {
+  clear_error();
+  int rc = check_ffn(T, H, I, 16, gate);
+  if (rc) return rc;
+  if (T == 0) return EK_OK;
+  if (!all_set(x, w1, w2, w3, s1, s2, s3, y, workspace)) return set_error(EK_ERR_INVALID, "null operand");
+  if (!all_aligned(x, w1, w2, w3, y, workspace)) return set_error(EK_ERR_INVALID, "operands must be 16-byte aligned");
+  int sms = 0;
+  if ((rc = resolve(num_sms, stream, &sms))) return rc;
+  const Fp8FfnLayout L = fp8_ffn_layout(T, H, I, sms);
+  if (ws_bytes < L.rest) return set_error(EK_ERR_INVALID, "workspace of at least %zu bytes required", L.rest);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  char* ws = static_cast<char*>(workspace);
+  uint8_t *xq = reinterpret_cast<uint8_t*>(ws + L.xq), *aq = reinterpret_cast<uint8_t*>(ws + L.aq);
+  float *xs = reinterpret_cast<float*>(ws + L.xs), *as = reinterpret_cast<float*>(ws + L.as);
+  char* rest = ws + L.rest;
+  const size_t rest_bytes = ws_bytes - L.rest;
+  if ((rc = ek_quant_e4m3_ex(x, EK_DTYPE_BF16, T, H, 1, 128, 0, xq, xs, stream))) return rc;
+  if (T <= kStreamTokens) {
+    rc = stream_gate(EK_DTYPE_E4M3, w1, w3, xq, {xs, s1, s3}, T, I, H, gate, nullptr, nullptr, aq, as, sms, rest,
+                     rest_bytes, s, false);
+  } else {
+    Fp8BlockParams p{};
+    p.M = T;
+    p.N = I;
+    p.tiles_m = ceil_div(T, 256);
+    p.tiles_n = ceil_div(I, 128);
+    p.k_blocks = ceil_div(H, 128);
+    p.splits = 1;
+    p.a_scale = xs;
+    p.w_scale = s1;
+    p.w_scale2 = s3;
+    p.w_blocks = p.tiles_n;
+    p.gate = gate;
+    p.codes = aq;
+    p.scales = as;
+    rc = launch_fp8<true>(xq, w1, w3, H, p, sms, s);
+  }
+  if (rc) return rc;
+  return fp8_store(aq, w2, as, s2, y, T, H, I, kOutBF16, sms, rest, rest_bytes, s, true);
+}
+
+}  // extern "C"

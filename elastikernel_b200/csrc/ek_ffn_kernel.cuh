@@ -1,0 +1,401 @@
+// Products of the gated feed-forward block on tcgen05 CTA pairs, bf16 and fp16.
+//
+//   gate/up   h1 = x W1^T, h3 = x W3^T, a = f(h1) h3          (kFfnGate)
+//   down      y = a W2^T                                      (kFfnStore, A and B K-major)
+//   backward  da = dy W2; dh1 = da h3 f'(h1); dh3 = da f(h1)  (kFfnGateGrad)
+//             dx = dh1 W1 + dh3 W3                            (kFfnStore, two K planes)
+//             dW1 = dh1^T x, dW3 = dh3^T x, dW2 = dy^T a      (kFfnStore, A MN-major)
+//
+// A persistent cluster of two CTAs computes a 256 x 256 tile with the 2-SM MMA:
+// each CTA loads its own 128 rows of A and half of the tile's B (32 KB per 64 of
+// K, no multicast) and its TMEM receives its 128 rows. Operands are used where
+// they lie: an operand whose reduction axis is not the contiguous one (the
+// weights in a backward pass, everything under a weight's gradient) is read
+// MN-major by the MMA, so nothing is transposed. The two weights of the gate, and
+// the two planes of the pre-activations, are separate tensor maps: a plane is
+// chosen by the rank (gate/up: columns [0, 128) of a tile are W1's, [128, 256)
+// W3's), by the K block (dx sums over both planes) or by the tile's row (dW1 and
+// dW3 are one launch), so no tail of one plane is ever read as the other's.
+//
+//   warp 0      TMA producer; warp 1  TMEM and MMA issue
+//   warps 2..9  epilogue, two per TMEM lane quarter, half of the columns each
+//
+// Few tiles: K is split over `splits` units per tile whose fp32 sums go to a
+// workspace, and ffn_reduce_kernel adds them in slice order. No atomics.
+#pragma once
+#include <type_traits>
+
+#include "ek_act.cuh"
+#include "ek_gemm_kernel.cuh"
+
+namespace ek {
+
+enum FfnEpi : int { kFfnStore = 0, kFfnGate = 1, kFfnGateGrad = 2 };
+
+template <int kElem_, bool kAMN_, bool kBMN_, int kEpi_>
+struct FfnCfg {
+  static constexpr int kElem = kElem_;
+  static constexpr bool kAMN = kAMN_, kBMN = kBMN_;  // operand stored with its reduction axis outermost
+  static constexpr int kEpi = kEpi_;
+  static constexpr int BN = 256, BK = 64, STAGES = 6;
+  static constexpr int HALF_BYTES = 128 * 128;  // 128 rows (or 64 x 128 columns) of one operand
+  static constexpr int STAGE_BYTES = 2 * HALF_BYTES;
+  static constexpr int EPI_WARPS = 8;
+  static constexpr int THREADS = 64 + 32 * EPI_WARPS;
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 256;
+  static constexpr uint32_t IDESC =
+      umma_idesc(kElem == kBF16 ? 1u : 0u, kBMN, 256, BN) | ((kAMN ? 1u : 0u) << 15);
+};
+
+struct FfnParams {
+  int M, N;              // rows and columns of the result (per plane)
+  int tiles_m, tiles_n;  // tiles_m counts the rows of all planes
+  int m_tiles_plane;     // row tiles of one plane (dW: two planes in M)
+  int k_blocks, kb_plane;  // K blocks in all and per plane (dx: two planes in K)
+  int splits, num_units;
+  int a_box3, b_box3;    // MN-major operand: its two 64-column chunks in one 3-D box
+  int gate;              // GateFn
+  void* C;               // result; gate: a; gate gradient: dh
+  long long c_plane;     // elements between the planes of C (dW1 / dW3, dh1 / dh3)
+  void* H;               // gate: the pre-activations to write (or null); gate gradient: those to read
+  long long h_plane;
+  void* Act;             // gate gradient: a
+  float* ws;             // splits > 1: fp32 sums [splits][planes * M][N]
+};
+
+template <int kElem>
+struct Elem16;
+template <>
+struct Elem16<kBF16> {
+  __device__ static uint32_t pack(float a, float b) {
+    __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&h);
+  }
+  __device__ static float2 unpack(uint32_t v) { return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v)); }
+};
+template <>
+struct Elem16<kFP16> {
+  __device__ static uint32_t pack(float a, float b) {
+    __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&h);
+  }
+  __device__ static float2 unpack(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
+};
+
+// 8 consecutive elements to or from global memory, 16-byte aligned.
+template <int kElem>
+__device__ __forceinline__ void store8(void* base, size_t at, const float* v) {
+  uint4 pk;
+  pk.x = Elem16<kElem>::pack(v[0], v[1]);
+  pk.y = Elem16<kElem>::pack(v[2], v[3]);
+  pk.z = Elem16<kElem>::pack(v[4], v[5]);
+  pk.w = Elem16<kElem>::pack(v[6], v[7]);
+  *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(base) + at) = pk;
+}
+template <int kElem>
+__device__ __forceinline__ void unpack8(const uint4& pk, float* v) {
+  const uint32_t w[4] = {pk.x, pk.y, pk.z, pk.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = Elem16<kElem>::unpack(w[i]);
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+
+// A producer that gave up waits (with a limit) for the copies it has in flight:
+// `issued` stages were filled in ring order. In a pair the leader's barriers count
+// both CTAs' copies, and neither CTA leaves before the closing cluster barrier.
+template <int kStages>
+__device__ __forceinline__ void wait_copies(uint64_t* full_bar, int issued) {
+  volatile int never = 0;
+  for (int i = max(0, issued - kStages); i < issued; ++i)
+    if (!mbar_wait(&full_bar[i % kStages], (i / kStages) & 1, &never)) return;
+}
+
+struct FfnUnit {
+  int tm, tn, m_plane, m_row, split, kb0, kb1;
+};
+
+template <class Cfg>
+__device__ __forceinline__ FfnUnit ffn_unit(const FfnParams& p, int u) {
+  FfnUnit w;
+  const int tile = u / p.splits;
+  w.split = u - tile * p.splits;
+  raster(tile, p.tiles_m, p.tiles_n, 8, w.tm, w.tn);
+  w.m_plane = w.tm >= p.m_tiles_plane ? 1 : 0;
+  w.m_row = (w.tm - w.m_plane * p.m_tiles_plane) * 256;
+  w.kb0 = (int)((long long)w.split * p.k_blocks / p.splits);
+  w.kb1 = (int)((long long)(w.split + 1) * p.k_blocks / p.splits);
+  return w;
+}
+
+// dh1, dh3 and a of 8 elements from da and the pre-activations
+template <int kFn>
+__device__ __forceinline__ void gate_grad8(const float* da, const float* h1, const float* h3, float* d1, float* d3,
+                                           float* a) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    float f, df;
+    gate_f_df<kFn>(h1[j], f, df);
+    d1[j] = da[j] * h3[j] * df;
+    d3[j] = da[j] * f;
+    a[j] = f * h3[j];
+  }
+}
+
+template <class Cfg>
+__global__ void __launch_bounds__(Cfg::THREADS, 1)
+    ffn_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CUtensorMap tmA1,
+                    const __grid_constant__ CUtensorMap tmB0, const __grid_constant__ CUtensorMap tmB1,
+                    const FfnParams p) {
+  constexpr int STAGES = Cfg::STAGES, BN = Cfg::BN, BK = Cfg::BK, HB = Cfg::HALF_BYTES;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + STAGES * Cfg::STAGE_BYTES);
+  uint64_t* empty_bar = full_bar + STAGES;
+  uint64_t* tfull_bar = empty_bar + STAGES;
+  uint64_t* tempty_bar = tfull_bar + 2;
+  uint64_t* drain_bar = tempty_bar + 2;
+  uint32_t* s_tmem_base = reinterpret_cast<uint32_t*>(drain_bar + 1);
+  volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem_base + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = (int)cluster_ctarank();
+  const bool leader = rank == 0;
+  const int unit0 = (int)cluster_id_x(), unit_step = (int)nclusters_x();
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&tfull_bar[b], 1);
+      mbar_init(&tempty_bar[b], Cfg::EPI_WARPS * 2);
+    }
+    mbar_init(drain_bar, 1);
+    *s_abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc<2>(s_tmem_base, 512);
+    tmem_relinquish<2>();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // the peer's barriers exist before anyone signals them
+  tc_fence_after();
+  const uint32_t tmem_base = *s_tmem_base;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      tma_prefetch_desc(&tmA0);
+      tma_prefetch_desc(&tmB0);
+      tma_prefetch_desc(&tmA1);
+      tma_prefetch_desc(&tmB1);
+      int stage = 0, issued = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      const uint32_t full0 = mapa_shared(smem_u32(&full_bar[0]), 0);  // both CTAs' loads complete on the leader's
+      for (int u = unit0; u < p.num_units && ok; u += unit_step) {
+        const FfnUnit w = ffn_unit<Cfg>(p, u);
+        const int a_mn = w.m_row + rank * 128;
+        const int b_mn = Cfg::kEpi == kFfnGate ? w.tn * 128 : w.tn * BN + rank * 128;
+        for (int kb = w.kb0; kb < w.kb1; ++kb) {
+          if (!mbar_wait(&empty_bar[stage], phase ^ 1, s_abort)) { ok = false; break; }
+          const int k_plane = kb >= p.kb_plane ? 1 : 0;
+          const int k0 = (kb - k_plane * p.kb_plane) * BK;
+          const CUtensorMap* ta = (k_plane | w.m_plane) ? &tmA1 : &tmA0;
+          const CUtensorMap* tb = (Cfg::kEpi == kFfnGate ? rank : k_plane) ? &tmB1 : &tmB0;
+          uint8_t* a_dst = smem + stage * Cfg::STAGE_BYTES;
+          uint8_t* b_dst = a_dst + HB;
+          if (leader) mbar_arrive_expect_tx(&full_bar[stage], 2 * Cfg::STAGE_BYTES);
+          const uint32_t fb = full0 + stage * 8;
+          if constexpr (Cfg::kAMN) {
+            if (p.a_box3) {
+              tma_load_3d_pair(a_dst, ta, fb, 0, k0, a_mn / 64);
+            } else {
+              tma_load_2d_pair(a_dst, ta, fb, a_mn, k0);
+              tma_load_2d_pair(a_dst + HB / 2, ta, fb, a_mn + 64, k0);
+            }
+          } else {
+            tma_load_2d_pair(a_dst, ta, fb, k0, a_mn);
+          }
+          if constexpr (Cfg::kBMN) {
+            if (p.b_box3) {
+              tma_load_3d_pair(b_dst, tb, fb, 0, k0, b_mn / 64);
+            } else {
+              tma_load_2d_pair(b_dst, tb, fb, b_mn, k0);
+              tma_load_2d_pair(b_dst + HB / 2, tb, fb, b_mn + 64, k0);
+            }
+          } else {
+            tma_load_2d_pair(b_dst, tb, fb, k0, b_mn);
+          }
+          ++issued;
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+      }
+      if (!ok && leader) wait_copies<STAGES>(full_bar, issued);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0 && leader) {
+      int stage = 0, acc_i = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int u = unit0; u < p.num_units && ok; u += unit_step, ++acc_i) {
+        const FfnUnit w = ffn_unit<Cfg>(p, u);
+        const int buf = acc_i & 1;
+        if (!mbar_wait(&tempty_bar[buf], ((acc_i >> 1) & 1) ^ 1, s_abort)) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + buf * BN;
+        for (int kb = w.kb0; kb < w.kb1; ++kb) {
+          if (!mbar_wait(&full_bar[stage], phase, s_abort)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t a0 = smem_u32(smem + stage * Cfg::STAGE_BYTES), b0 = a0 + HB;
+#pragma unroll
+          for (int k = 0; k < BK / 16; ++k) {
+            // MN-major: 16 rows of K are 2 KB on, the 64-column chunks BK * 128 bytes apart
+            const uint64_t ad = Cfg::kAMN ? umma_desc_sw128(a0 + k * 2048, BK * 128, 1024)
+                                          : umma_desc_sw128(a0 + k * 32, 16, 1024);
+            const uint64_t bd = Cfg::kBMN ? umma_desc_sw128(b0 + k * 2048, BK * 128, 1024)
+                                          : umma_desc_sw128(b0 + k * 32, 16, 1024);
+            umma_pair<false>(d_tmem, ad, bd, Cfg::IDESC, (kb > w.kb0 || k > 0) ? 1u : 0u);
+          }
+          umma_commit_pair(&empty_bar[stage], 0x3);
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+        if (!ok) break;
+        umma_commit_pair(&tfull_bar[buf], 0x3);
+      }
+      // every MMA issued so far has completed (in both CTAs) before TMEM is freed
+      umma_commit_pair(drain_bar, 0x3);
+      volatile int never = 0;
+      mbar_wait(drain_bar, 0, &never);
+    } else if (lane == 0) {
+      volatile int never = 0;
+      mbar_wait(drain_bar, 0, &never);
+    }
+    __syncwarp();
+  } else {
+    const int q = warp & 3;           // TMEM lane quarter of this warp
+    const int half = (warp - 2) >> 2;  // its half of the columns
+    const uint32_t tempty0 = mapa_shared(smem_u32(&tempty_bar[0]), 0);
+    auto release = [&](int buf) {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(tempty0 + buf * 8);
+    };
+    int acc_i = 0;
+    for (int u = unit0; u < p.num_units; u += unit_step, ++acc_i) {
+      const FfnUnit w = ffn_unit<Cfg>(p, u);
+      const int buf = acc_i & 1;
+      const bool got = mbar_wait(&tfull_bar[buf], (acc_i >> 1) & 1, s_abort);
+      if (!__all_sync(0xffffffffu, got)) break;  // the TMEM loads are warp-collective
+      tc_fence_after();
+      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buf * BN;
+      const int row = w.m_row + rank * 128 + q * 32 + lane;
+      const bool row_ok = row < p.M;
+      if constexpr (Cfg::kEpi == kFfnGate) {
+#pragma unroll 1
+        for (int c = 0; c < 2; ++c) {
+          const int f0 = half * 64 + c * 32;  // feature within the tile's 128
+          uint32_t rg[32], ru[32];
+          tmem_ld32(t_row + f0, rg);
+          tmem_ld32(t_row + 128 + f0, ru);
+          tmem_ld_wait(rg);
+          reg_dep(ru);
+          if (c == 1) release(buf);
+          const int col = w.tn * 128 + f0;
+          if (row_ok) {
+            const size_t at = (size_t)row * p.N + col;
+            if (p.H != nullptr) {
+#pragma unroll
+              for (int g = 0; g < 4; ++g)
+                if (col + g * 8 < p.N) {
+                  store8<Cfg::kElem>(p.H, at + g * 8, reinterpret_cast<float*>(rg) + g * 8);
+                  store8<Cfg::kElem>(p.H, p.h_plane + at + g * 8, reinterpret_cast<float*>(ru) + g * 8);
+                }
+            }
+            with_gate(p.gate, [&](auto fn) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                rg[j] = __float_as_uint(gate_f<decltype(fn)::value>(__uint_as_float(rg[j])) * __uint_as_float(ru[j]));
+            });
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+              if (col + g * 8 < p.N) store8<Cfg::kElem>(p.C, at + g * 8, reinterpret_cast<float*>(rg) + g * 8);
+          }
+        }
+      } else {
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          const int c0 = half * 128 + c * 32;
+          uint32_t r[32];
+          tmem_ld32(t_row + c0, r);
+          tmem_ld_wait(r);
+          if (c == 3) release(buf);
+          const int col = w.tn * BN + c0;
+          if (!row_ok) continue;
+          const float* v = reinterpret_cast<const float*>(r);
+          const size_t at = (size_t)row * p.N + col;
+          if constexpr (Cfg::kEpi == kFfnGateGrad) {
+            with_gate(p.gate, [&](auto fn) {
+#pragma unroll
+              for (int g = 0; g < 4; ++g)
+                if (col + g * 8 < p.N) {
+                  const uint16_t* h = reinterpret_cast<const uint16_t*>(p.H) + at + g * 8;
+                  float h1[8], h3[8], d1[8], d3[8], a[8];
+                  unpack8<Cfg::kElem>(__ldg(reinterpret_cast<const uint4*>(h)), h1);
+                  unpack8<Cfg::kElem>(__ldg(reinterpret_cast<const uint4*>(h + p.h_plane)), h3);
+                  gate_grad8<decltype(fn)::value>(v + g * 8, h1, h3, d1, d3, a);
+                  store8<Cfg::kElem>(p.C, at + g * 8, d1);
+                  store8<Cfg::kElem>(p.C, p.c_plane + at + g * 8, d3);
+                  store8<Cfg::kElem>(p.Act, at + g * 8, a);
+                }
+            });
+          } else if (p.splits > 1) {
+            float* out = p.ws + ((size_t)w.split * (p.tiles_m / p.m_tiles_plane) + w.m_plane) * p.M * p.N + at;
+#pragma unroll
+            for (int g = 0; g < 8; ++g)
+              if (col + g * 4 < p.N)
+                __stcg(reinterpret_cast<float4*>(out + g * 4), make_float4(v[4 * g], v[4 * g + 1], v[4 * g + 2],
+                                                                           v[4 * g + 3]));
+          } else {
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+              if (col + g * 8 < p.N) store8<Cfg::kElem>(p.C, w.m_plane * p.c_plane + at + g * 8, v + g * 8);
+          }
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // no CTA leaves while its peer may still signal it
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc<2>(tmem_base, 512);
+  }
+}
+
+// out[i] = sum over the slices, in slice order, of ws[s][i], rounded once. n8:
+// groups of 8 elements of the result (both planes); they lie end to end in both.
+template <int kElem>
+__global__ void __launch_bounds__(256) ffn_reduce_kernel(const float* __restrict__ ws, int splits, long long n8,
+                                                         void* __restrict__ out) {
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n8; i += gridDim.x * 256ll) {
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < splits; ++s) {
+      const float4* src = reinterpret_cast<const float4*>(ws) + (s * n8 + i) * 2;
+      const float4 a = __ldcg(src), b = __ldcg(src + 1);
+      v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+      v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+    }
+    store8<kElem>(out, (size_t)i * 8, v);
+  }
+}
+
+}  // namespace ek

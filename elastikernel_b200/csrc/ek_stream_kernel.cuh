@@ -1,0 +1,395 @@
+// Products of up to 128 tokens with a weight matrix, bound by the weight's bytes:
+// D[n, t] = sum_k W[n, k] x[t, k] for bf16, fp16 and block-scaled e4m3, and for the
+// gate/up pair D1 = W1 x, D3 = W3 x.
+//
+// The operands are swapped: weight rows are the MMA's 128-row side, tokens its N
+// side, so a stage is 256 weight rows x 128 bytes of K (32 KB; for gate/up 128 rows
+// of W1 and 128 of W3) and the few token rows beside them. The work is the sequence
+// of (row tile, K block) units, tile by tile, and CTA c takes the same number of
+// consecutive units whatever the matrix: every SM streams the same bytes. What a
+// CTA has of one tile is a segment; its fp32 sums go to the segment's slot of the
+// workspace, [token][256 rows], and the following launch (stream_*_reduce_kernel)
+// adds a tile's segments in K order and applies what follows: the rounding, or the
+// gate function and its rounding or quantisation. No atomics, no tickets.
+//
+// Block-scaled e4m3: a 128-byte stage is one scale block. Each K block is
+// multiplied into its own TMEM buffer, and the epilogue adds (weight-block scale x
+// token scale) x product to fp32 registers while the next block's MMA runs.
+//
+//   warp 0  TMA producer; warp 1  TMEM and MMA; warp 2  scales (e4m3)
+//   warps 3..10  epilogue: two per TMEM lane quarter, one 128-row block each
+//
+// Launches of one call overlap (programmatic dependent launch): weights are not
+// written by a predecessor within the call, so a CTA fills its stages with them
+// before it waits; everything else is read and written after the wait.
+#pragma once
+#include <cuda_fp8.h>
+
+#include "ek_ffn_kernel.cuh"
+
+namespace ek {
+
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <int kElem_, int NT_, bool kGate_>
+struct StreamCfg {
+  static constexpr int kElem = kElem_, NT = NT_;
+  static constexpr bool kGate = kGate_, kF8 = kElem == kE4M3;
+  static constexpr int BK = kF8 ? 128 : 64, KSTEPS = 4;
+  static constexpr int A_BYTES = 256 * 128, B_BYTES = NT * 128, STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int SLOTS = 8;          // K blocks of scales in flight
+  static constexpr int SLOT_STRIDE = NT + 4;  // token scales, then the two row blocks'
+  static constexpr int SCALE_BYTES = kF8 ? SLOTS * SLOT_STRIDE * 4 : 0;
+  static constexpr int STAGES_FIT = (224 * 1024 - SCALE_BYTES - 512) / STAGE_BYTES;
+  static constexpr int STAGES = STAGES_FIT > 6 ? 6 : STAGES_FIT;
+  static constexpr int TMEM_COLS = 4 * NT;  // two buffers of two accumulators
+  static constexpr int EPI_WARPS = 8;
+  static constexpr int THREADS = 96 + 32 * EPI_WARPS;
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + SCALE_BYTES + 512 + 1024;
+  static constexpr uint32_t IDESC = umma_idesc(kElem == kBF16 ? 1u : 0u, false, 128, NT);
+  static constexpr int CHUNK = NT < 32 || (kF8 && NT == 128) ? 16 : 32;  // 128 accumulators leave room for 16
+  static_assert(NT == 16 || NT == 32 || NT == 64 || NT == 128, "token tile");
+};
+
+// How the units are dealt out; the reducing launch reads it too.
+struct StreamSplit {
+  int tiles, k_blocks;  // row tiles (256 rows, or 128 gate features), K blocks
+  int per_cta, ctas;    // consecutive units of a CTA
+  int max_segs;         // slots per CTA: the tiles that per_cta units can touch
+};
+
+struct StreamParams {
+  StreamSplit sp;
+  int T;
+  const float* tok_scale;  // e4m3: [T][k_blocks]
+  const float* w_scale;    // [rows / 128][k_blocks]; gate: W1's
+  const float* w_scale2;   // gate: W3's
+  int w_blocks;            // rows of w_scale
+  float* ws;               // [ctas * max_segs][T][256]
+};
+
+template <class Cfg>
+__global__ void __launch_bounds__(Cfg::THREADS, 1)
+    stream_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmW2,
+                  const __grid_constant__ CUtensorMap tmX, const StreamParams p) {
+  constexpr int STAGES = Cfg::STAGES, NT = Cfg::NT, CH = Cfg::CHUNK, NS = Cfg::SLOTS, RS = Cfg::SLOT_STRIDE;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* s_scale = reinterpret_cast<float*>(smem + STAGES * Cfg::STAGE_BYTES);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + STAGES * Cfg::STAGE_BYTES + Cfg::SCALE_BYTES);
+  uint64_t* empty_bar = full_bar + STAGES;
+  uint64_t* tfull_bar = empty_bar + STAGES;
+  uint64_t* tempty_bar = tfull_bar + 2;
+  uint64_t* drain_bar = tempty_bar + 2;
+  uint64_t* sfull_bar = drain_bar + 1;
+  uint64_t* sempty_bar = sfull_bar + NS;
+  uint32_t* s_tmem_base = reinterpret_cast<uint32_t*>(sempty_bar + NS);
+  volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem_base + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int KB = p.sp.k_blocks;
+  const int u0 = blockIdx.x * p.sp.per_cta;
+  const int u1 = min(u0 + p.sp.per_cta, p.sp.tiles * KB);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&tfull_bar[b], 1);
+      mbar_init(&tempty_bar[b], Cfg::EPI_WARPS);
+    }
+    mbar_init(drain_bar, 1);
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(&sfull_bar[s], 32);
+      mbar_init(&sempty_bar[s], Cfg::EPI_WARPS);
+    }
+    *s_abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc<1>(s_tmem_base, Cfg::TMEM_COLS);
+    tmem_relinquish<1>();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *s_tmem_base;
+  pdl_launch();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      tma_prefetch_desc(&tmW);
+      if (Cfg::kGate) tma_prefetch_desc(&tmW2);
+      tma_prefetch_desc(&tmX);
+      auto load_w = [&](int u, int stage) {
+        const int tile = u / KB, k0 = (u - tile * KB) * Cfg::BK;
+        uint8_t* dst = smem + stage * Cfg::STAGE_BYTES;
+        mbar_arrive_expect_tx(&full_bar[stage], Cfg::STAGE_BYTES);
+        if constexpr (Cfg::kGate) {
+          tma_load_2d(dst, &tmW, &full_bar[stage], k0, tile * 128);
+          tma_load_2d(dst + 128 * 128, &tmW2, &full_bar[stage], k0, tile * 128);
+        } else {
+          tma_load_2d(dst, &tmW, &full_bar[stage], k0, tile * 256);
+        }
+      };
+      auto load_x = [&](int u, int stage) {
+        tma_load_2d(smem + stage * Cfg::STAGE_BYTES + Cfg::A_BYTES, &tmX, &full_bar[stage], (u % KB) * Cfg::BK, 0);
+      };
+      // the stages' first fill: the weights before the wait, the tokens after it
+      const int first = min(u1 - u0, STAGES);
+      for (int i = 0; i < first; ++i) load_w(u0 + i, i);
+      pdl_wait();
+      for (int i = 0; i < first; ++i) load_x(u0 + i, i);
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int u = u0 + STAGES; u < u1; ++u) {
+        if (!mbar_wait(&empty_bar[stage], phase, s_abort)) {
+          wait_copies<STAGES>(full_bar, u - u0);
+          break;
+        }
+        load_w(u, stage);
+        load_x(u, stage);
+        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      int stage = 0, flush = 0;
+      uint32_t phase = 0;
+      bool fresh = true;  // the next MMA starts a sum
+      for (int u = u0; u < u1; ++u) {
+        const int buf = flush & 1;
+        if (fresh && !mbar_wait(&tempty_bar[buf], ((flush >> 1) & 1) ^ 1, s_abort)) break;
+        if (!mbar_wait(&full_bar[stage], phase, s_abort)) break;
+        tc_fence_after();
+        const uint32_t a0 = smem_u32(smem + stage * Cfg::STAGE_BYTES), b0 = a0 + Cfg::A_BYTES;
+        const uint32_t d = tmem_base + buf * 2 * NT;
+#pragma unroll
+        for (int k = 0; k < Cfg::KSTEPS; ++k) {
+          const uint64_t bd = umma_desc_sw128(b0 + k * 32, 16, 1024);
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            umma<Cfg::kF8>(d + h * NT, umma_desc_sw128(a0 + h * (128 * 128) + k * 32, 16, 1024), bd, Cfg::IDESC,
+                           (!fresh || k > 0) ? 1u : 0u);
+        }
+        umma_commit(&empty_bar[stage]);
+        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        fresh = Cfg::kF8 || (u + 1) % KB == 0 || u + 1 == u1;
+        if (fresh) {
+          umma_commit(&tfull_bar[buf]);
+          ++flush;
+        }
+      }
+      umma_commit(drain_bar);  // every MMA has completed before TMEM is freed
+      volatile int never = 0;
+      mbar_wait(drain_bar, 0, &never);
+    }
+    __syncwarp();
+  } else if (warp == 2) {
+    if constexpr (Cfg::kF8) {
+      pdl_wait();
+      for (int u = u0; u < u1; ++u) {
+        const int g = u - u0, slot = g % NS;
+        const bool ok = mbar_wait(&sempty_bar[slot], ((g / NS) & 1) ^ 1, s_abort);
+        if (__any_sync(0xffffffffu, !ok)) break;
+        const int tile = u / KB, kb = u - tile * KB;
+        float* dst = s_scale + slot * RS;
+        for (int t = lane; t < NT; t += 32)
+          cp_async_4_zfill(dst + t, t < p.T ? p.tok_scale + (size_t)t * KB + kb : p.tok_scale, t < p.T ? 4 : 0);
+        if (lane < 2) {
+          const int blk = Cfg::kGate ? tile : 2 * tile + lane;
+          const float* src = Cfg::kGate && lane ? p.w_scale2 : p.w_scale;
+          cp_async_4_zfill(dst + NT + lane, blk < p.w_blocks ? src + (size_t)blk * KB + kb : src,
+                           blk < p.w_blocks ? 4 : 0);
+        }
+        cp_async_mbar_arrive(&sfull_bar[slot]);
+      }
+      cp_async_wait<0>();  // no copy into shared memory outlives the CTA
+    }
+    __syncwarp();
+  } else {
+    pdl_wait();
+    const int q = warp & 3, rb = (warp - 3) >> 2;
+    const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + rb * NT;
+    const int n0 = rb * 128 + q * 32 + lane;  // row within the tile's 256
+    auto release = [&](int buf) {
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&tempty_bar[buf]);
+    };
+    int flush = 0, seg = 0;
+    for (int u = u0; u < u1;) {
+      const int tile_end = min(u1, (u / KB + 1) * KB);
+      float* out = p.ws + ((size_t)(blockIdx.x * p.sp.max_segs + seg) * p.T) * 256 + n0;
+      bool good = true;
+      if constexpr (Cfg::kF8) {
+        float2 acc[NT / 2];
+#pragma unroll
+        for (int j = 0; j < NT / 2; ++j) acc[j] = make_float2(0.f, 0.f);
+        for (; u < tile_end; ++u, ++flush) {
+          const int buf = flush & 1, slot = flush % NS;
+          const bool got = mbar_wait(&tfull_bar[buf], (flush >> 1) & 1, s_abort) &&
+                           mbar_wait(&sfull_bar[slot], (flush / NS) & 1, s_abort);
+          good = __all_sync(0xffffffffu, got);
+          if (!good) break;
+          tc_fence_after();
+          const float* xs = s_scale + slot * RS;
+          const float ws = xs[NT + rb];
+#pragma unroll
+          for (int c = 0; c < NT / CH; ++c) {
+            uint32_t r[32];
+            if constexpr (CH == 32)
+              tmem_ld32(lane_base + buf * 2 * NT + c * CH, r);
+            else
+              tmem_ld16(lane_base + buf * 2 * NT + c * CH, r);
+            tmem_ld_wait(r);
+            const float4* xs4 = reinterpret_cast<const float4*>(xs + c * CH);
+#pragma unroll
+            for (int j = 0; j < CH / 4; ++j) {
+              const float4 s = xs4[j];
+              float2* a = acc + (c * CH + 4 * j) / 2;
+              a[0] = fma2(make_float2(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1])),
+                          mul2(make_float2(s.x, s.y), make_float2(ws, ws)), a[0]);
+              a[1] = fma2(make_float2(__uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3])),
+                          mul2(make_float2(s.z, s.w), make_float2(ws, ws)), a[1]);
+            }
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(&tempty_bar[buf]);
+            mbar_arrive(&sempty_bar[slot]);
+          }
+        }
+        if (!good) break;
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+          if (t < p.T) __stcg(out + (size_t)t * 256, (t & 1) ? acc[t >> 1].y : acc[t >> 1].x);
+      } else {
+        const int buf = flush & 1;
+        good = mbar_wait(&tfull_bar[buf], (flush >> 1) & 1, s_abort);
+        if (!__all_sync(0xffffffffu, good)) break;
+        tc_fence_after();
+#pragma unroll 1
+        for (int c = 0; c < NT / CH; ++c) {
+          uint32_t r[32];
+          if constexpr (CH == 32)
+            tmem_ld32(lane_base + buf * 2 * NT + c * CH, r);
+          else
+            tmem_ld16(lane_base + buf * 2 * NT + c * CH, r);
+          tmem_ld_wait(r);
+          if (c == NT / CH - 1) release(buf);
+#pragma unroll
+          for (int j = 0; j < CH; ++j)
+            if (c * CH + j < p.T) __stcg(out + (size_t)(c * CH + j) * 256, __uint_as_float(r[j]));
+        }
+        ++flush;
+        u = tile_end;
+      }
+      ++seg;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc<1>(tmem_base, Cfg::TMEM_COLS);
+  }
+}
+
+// ------------------------------------------------------------ adding the segments
+// Sum over the segments of `tile`, in K order, of row r (and r2) of token t.
+template <int kN>
+__device__ __forceinline__ void stream_sum(const StreamSplit& sp, const float* __restrict__ ws, int T, int tile, int t,
+                                           const int (&r)[kN], float (&v)[kN]) {
+#pragma unroll
+  for (int i = 0; i < kN; ++i) v[i] = 0.f;
+  const int c0 = (int)((long long)tile * sp.k_blocks / sp.per_cta);
+  const int c1 = (int)(((long long)(tile + 1) * sp.k_blocks - 1) / sp.per_cta);
+  constexpr int U = 4;  // segments with their loads in flight
+  for (int c = c0; c <= c1; c += U) {
+    float x[U][kN];
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      if (c + j > c1) break;
+      const int seg = tile - (int)((long long)(c + j) * sp.per_cta / sp.k_blocks);
+      const float* src = ws + ((size_t)((c + j) * sp.max_segs + seg) * T + t) * 256;
+#pragma unroll
+      for (int i = 0; i < kN; ++i) x[j][i] = __ldcg(src + r[i]);
+    }
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      if (c + j > c1) break;
+#pragma unroll
+      for (int i = 0; i < kN; ++i) v[i] += x[j][i];
+    }
+  }
+}
+
+enum OutType : int { kOutBF16 = 0, kOutFP16 = 1, kOutFP32 = 3 };
+
+__device__ __forceinline__ void store_out(void* out, int type, size_t at, float v) {
+  if (type == kOutBF16)
+    reinterpret_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(v);
+  else if (type == kOutFP16)
+    reinterpret_cast<__half*>(out)[at] = __float2half_rn(v);
+  else
+    reinterpret_cast<float*>(out)[at] = v;
+}
+
+// out[t, n] of a plain product; a block per (tile, token), a thread per row
+__global__ void __launch_bounds__(256) stream_store_reduce_kernel(const StreamSplit sp, const float* __restrict__ ws,
+                                                                  int T, int N, void* __restrict__ out, int type) {
+  pdl_launch();
+  pdl_wait();
+  const int tile = blockIdx.x, t = blockIdx.y, n = tile * 256 + threadIdx.x;
+  if (n >= N) return;
+  const int r[1] = {(int)threadIdx.x};
+  float v[1];
+  stream_sum<1>(sp, ws, T, tile, t, r, v);
+  store_out(out, type, (size_t)t * N + n, v[0]);
+}
+
+// a[t, f] = f(h1) h3 of the gate/up pair, h1 and h3 on request; a block per
+// (tile, token), a thread per feature. codes != null: a in e4m3 with the scale of
+// the block's 128 features (largest magnitude / 448, 1 for zeros) instead.
+__global__ void __launch_bounds__(128)
+    stream_gate_reduce_kernel(const StreamSplit sp, const float* __restrict__ ws, int T, int I, int gate, int type,
+                              void* __restrict__ a, void* __restrict__ h, uint8_t* __restrict__ codes,
+                              float* __restrict__ scales) {
+  pdl_launch();
+  pdl_wait();
+  const int tile = blockIdx.x, t = blockIdx.y, f = tile * 128 + threadIdx.x;
+  const int r[2] = {(int)threadIdx.x, 128 + (int)threadIdx.x};
+  float v[2];
+  stream_sum<2>(sp, ws, T, tile, t, r, v);  // rows past I hold zeros
+  float act;
+  with_gate(gate, [&](auto fn) { act = gate_f<decltype(fn)::value>(v[0]) * v[1]; });
+  const size_t at = (size_t)t * I + f;
+  if (codes == nullptr) {
+    if (f >= I) return;
+    store_out(a, type, at, act);
+    if (h != nullptr) {
+      store_out(h, type, at, v[0]);
+      store_out(h, type, (size_t)T * I + at, v[1]);
+    }
+    return;
+  }
+  __shared__ float s_max[4];
+  float m = f < I ? fabsf(act) : 0.f;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+  const float s = m > 0.f ? m / 448.0f : 1.0f;
+  if (f < I) codes[at] = static_cast<uint8_t>(__nv_cvt_float_to_fp8(act / s, __NV_SATFINITE, __NV_E4M3));
+  if (threadIdx.x == 0) scales[(size_t)t * ((I + 127) / 128) + tile] = s;
+}
+
+}  // namespace ek

@@ -565,6 +565,56 @@ int ek_fused_moe_w4(const void* x, const float* logits, int T, int topk, const v
                     const void* w2_codes, const void* w2_scales, const void* w2_mins, void* out, int E, int H, int I,
                     int group, int num_sms, void* workspace, size_t ws_bytes, void* stream);
 
+/* ------------------------------------------- dense feed-forward operators */
+
+/* Gate functions f of the gated block. */
+#define EK_GATE_SILU 0
+#define EK_GATE_GELU 1      /* z Phi(z) */
+#define EK_GATE_GELU_TANH 2 /* z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2 */
+
+/* Dense e4m3 product with block scales:
+ *   C[m, n] = sum_b a_scale[m, b] * w_scale[n / 128, b] * sum_{k in block b} A[m, k] * W[n, k]
+ * A [M, K] and W [N, K] e4m3, blocks of 128 along K (the last may be short),
+ * a_scale [M, ceil(K / 128)] and w_scale [ceil(N / 128), ceil(K / 128)] fp32 of any
+ * value. Products of a block and the sum over blocks are fp32; C [M, N] is bf16,
+ * fp16 or fp32 (out_dtype), rounded once. K a multiple of 16, any M and N; A, W and
+ * the workspace 16-byte aligned. workspace: ek_gemm_fp8_block_workspace_bytes
+ * bytes for the launch's SMs or more; its contents before and after do not
+ * matter, but no two calls in flight may share it. */
+size_t ek_gemm_fp8_block_workspace_bytes(int M, int N, int K, int num_sms);
+int ek_gemm_fp8_block(const void* A, const void* W, const float* a_scale, const float* w_scale, void* C, int M, int N,
+                      int K, int out_dtype, int num_sms, void* workspace, size_t ws_bytes, void* stream);
+
+/* Gated feed-forward block, bf16 or fp16, fp32 sums:
+ *   h1 = x W1^T, h3 = x W3^T, a = f(h1) h3, y = a W2^T
+ * x [T, H], w1 and w3 [I, H], w2 [H, I], y [T, H]; H and I multiples of 8. a comes
+ * from the unrounded sums and is rounded to the inputs' type between the two
+ * products. h (may be NULL): h1 and h3 rounded, [2, T, I], for the gradient.
+ * All pointers 16-byte aligned; workspace as above. */
+size_t ek_gated_ffn_workspace_bytes(int T, int H, int I, int num_sms);
+int ek_gated_ffn(const void* x, const void* w1, const void* w2, const void* w3, void* y, void* h, int T, int H, int I,
+                 int dtype, int gate, int num_sms, void* workspace, size_t ws_bytes, void* stream);
+
+/* Its gradients, from the h that ek_gated_ffn left and d_out = dL/dy [T, H]:
+ *   da = d_out W2, dh1 = da h3 f'(h1), dh3 = da f(h1)
+ *   d_x = dh1 W1 + dh3 W3 [T, H], d_w13 = (dh1^T x, dh3^T x) [2, I, H],
+ *   d_w2 = d_out^T a [H, I] with a = f(h1) h3 made again
+ * dh1, dh3 and a are rounded to the inputs' type between the products (zeros for
+ * d_w13 and d_w2 without a token). */
+size_t ek_gated_ffn_grad_workspace_bytes(int T, int H, int I, int num_sms);
+int ek_gated_ffn_grad(const void* x, const void* w1, const void* w2, const void* w3, const void* h, const void* d_out,
+                      void* d_x, void* d_w13, void* d_w2, int T, int H, int I, int dtype, int gate, int num_sms,
+                      void* workspace, size_t ws_bytes, void* stream);
+
+/* The block over e4m3 weights with 128 x 128 block scales (s1, s3 [ceil(I / 128),
+ * ceil(H / 128)], s2 [ceil(H / 128), ceil(I / 128)]); x and y bf16 [T, H], H and I
+ * multiples of 16. x, and a from its fp32 sums, are quantised per 1 x 128 group as
+ * ek_quant_e4m3 does (largest magnitude / 448). */
+size_t ek_gated_ffn_fp8_workspace_bytes(int T, int H, int I, int num_sms);
+int ek_gated_ffn_fp8(const void* x, const void* w1, const void* w2, const void* w3, const float* s1, const float* s2,
+                     const float* s3, void* y, int T, int H, int I, int gate, int num_sms, void* workspace,
+                     size_t ws_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
