@@ -94,17 +94,18 @@ int grid_for(long long work, int sms) { return (int)std::max<long long>(1, std::
 // ------------------------------------------------------------------ splitting K
 // Slices per tile of a pair kernel: with rounds(s) = ceil(tiles s / pairs) units
 // of k_blocks / s one after the other, each block of K costing t_kb and each unit
-// its fill and its last epilogue, against the sums' way to memory and back and one
-// more launch. cap: bytes the workspace has for the sums.
-int pick_splits(long long tiles, int k_blocks, int pairs, long long elems, double t_kb, size_t cap) {
-  constexpr double kUnitUs = 2.5, kReduceUs = 3.0, kBytesPerUs = 4.0e6;
+// its fill and its last epilogue (unit_us undivided, kSliceUs as a slice), against
+// the sums' way to memory and back and one more launch. cap: bytes the workspace
+// has for the sums.
+int pick_splits(long long tiles, int k_blocks, int pairs, long long elems, double t_kb, double unit_us, size_t cap) {
+  constexpr double kSliceUs = 2.5, kReduceUs = 3.0, kBytesPerUs = 4.0e6;
   int best = 1;
   double best_us = 1e30;
   for (int s = 1; s <= 32 && (s == 1 || k_blocks / s >= 4); ++s) {
     const size_t bytes = (size_t)s * elems * 4;
     if (s > 1 && bytes > cap) break;
     const double rounds = std::ceil((double)(tiles * s) / pairs);
-    double us = rounds * (std::ceil((double)k_blocks / s) * t_kb + kUnitUs);
+    double us = rounds * std::ceil((double)k_blocks / s) * t_kb + (s > 1 ? kSliceUs : unit_us);
     if (s > 1) us += kReduceUs + 2.0 * bytes / kBytesPerUs;
     if (us < 0.95 * best_us) {
       best_us = us;
@@ -113,7 +114,8 @@ int pick_splits(long long tiles, int k_blocks, int pairs, long long elems, doubl
   }
   return best;
 }
-constexpr double kFfnBlockUs = 0.30, kFp8BlockUs = 0.40;
+constexpr double kFfnBlockUs = 0.30, kFp8BlockUs = 0.35;
+constexpr double kStoreUnitUs = 2.5, kGateUnitUs = 4.0, kGateGradUnitUs = 8.0;
 constexpr size_t kMostSplitBytes = 256u << 20;
 
 // ------------------------------------------------------------------ few tokens
@@ -147,18 +149,28 @@ template <int kElem, bool kGate>
 int launch_stream_nt(const void* w, const void* w2, const void* x, int rows, int K, StreamParams& p, cudaStream_t s,
                      bool overlap) {
   const int nt = p.T <= 16 ? 16 : p.T <= 32 ? 32 : p.T <= 64 ? 64 : 128;
+  p.n = (p.T + 15) / 16 * 16;
   CUtensorMap tw, tw2, tx;
   int rc = map_k(&tw, w, kElem, rows, K, kGate ? 128 : 256);
   if (rc) return rc;
   tw2 = tw;
   if (kGate && (rc = map_k(&tw2, w2, kElem, rows, K, 128))) return rc;
-  if ((rc = map_k(&tx, x, kElem, p.T, K, nt))) return rc;
+  if ((rc = map_k(&tx, x, kElem, p.T, K, p.n))) return rc;
   switch (nt) {
     case 16: return launch_stream<StreamCfg<kElem, 16, kGate>>(tw, tw2, tx, p, s, overlap);
     case 32: return launch_stream<StreamCfg<kElem, 32, kGate>>(tw, tw2, tx, p, s, overlap);
     case 64: return launch_stream<StreamCfg<kElem, 64, kGate>>(tw, tw2, tx, p, s, overlap);
     default: return launch_stream<StreamCfg<kElem, 128, kGate>>(tw, tw2, tx, p, s, overlap);
   }
+}
+
+// Warps that share a token's segments in the reducing launch: several where a tile
+// has many and the blocks would leave SMs idle.
+int stream_ways(const StreamSplit& sp, int T, int row_tiles, int sms) {
+  const int segs = ceil_div(sp.k_blocks, sp.per_cta) + 1;
+  int ways = 1;
+  while (ways < 8 && 2 * ways <= segs && (long long)row_tiles * ceil_div(T, 8 / (2 * ways)) <= 4ll * sms) ways *= 2;
+  return ways;
 }
 
 struct StreamScales {
@@ -180,8 +192,10 @@ int stream_store(int dtype, const void* w, const void* x, const StreamScales& sc
            : dtype == EK_DTYPE_FP16 ? launch_stream_nt<kFP16, false>(w, w, x, N, K, p, s, overlap)
                                     : launch_stream_nt<kE4M3, false>(w, w, x, N, K, p, s, overlap);
   if (rc) return rc;
-  return launch("stream sums", stream_store_reduce_kernel, dim3(p.sp.tiles, T), 256, 0, s, 0, true, p.sp,
-                (const float*)p.ws, T, N, out, out_type);
+  const int ways = stream_ways(p.sp, T, 2 * p.sp.tiles, sms);
+  const int wide = aligned16(out) && N % 4 == 0;
+  return launch("stream sums", stream_store_reduce_kernel, dim3(2 * p.sp.tiles, ceil_div(T, 8 / ways)), 256, 0, s, 0, true,
+                p.sp, (const float*)p.ws, T, N, out, out_type, wide, ways);
 }
 
 // a[t, i] = f(x[t] . w1[i]) (x[t] . w3[i]); e4m3: codes and scales of a
@@ -201,8 +215,9 @@ int stream_gate(int dtype, const void* w1, const void* w3, const void* x, const 
            : dtype == EK_DTYPE_FP16 ? launch_stream_nt<kFP16, true>(w1, w3, x, I, H, p, s, overlap)
                                     : launch_stream_nt<kE4M3, true>(w1, w3, x, I, H, p, s, overlap);
   if (rc) return rc;
-  return launch("stream gate", stream_gate_reduce_kernel, dim3(p.sp.tiles, T), 128, 0, s, 0, true, p.sp,
-                (const float*)p.ws, T, I, gate, dtype, a, h, codes, scales);
+  const int ways = stream_ways(p.sp, T, p.sp.tiles, sms);
+  return launch("stream gate", stream_gate_reduce_kernel, dim3(p.sp.tiles, ceil_div(T, 8 / ways)), 256, 0, s, 0, true, p.sp,
+                (const float*)p.ws, T, I, gate, dtype, a, h, codes, scales, ways);
 }
 
 // ------------------------------------------------------------------ 16-bit tiles
@@ -249,7 +264,8 @@ int ffn_store(const FfnOperand& A, const FfnOperand& B, int M, int N, int k, int
   p.c_plane = (long long)M * N;
   p.ws = static_cast<float*>(ws);
   const long long elems = (long long)planes_m * M * N;
-  p.splits = pick_splits((long long)p.tiles_m * p.tiles_n, p.k_blocks, std::max(1, sms / 2), elems, kFfnBlockUs, ws_bytes);
+  p.splits = pick_splits((long long)p.tiles_m * p.tiles_n, p.k_blocks, std::max(1, sms / 2), elems, kFfnBlockUs,
+                         kStoreUnitUs, ws_bytes);
   int rc = launch_ffn<FfnCfg<kElem, kAMN, kBMN, kFfnStore>>(ta, tb, p, sms, s);
   if (rc || p.splits == 1) return rc;
   const long long n8 = elems / 8;
@@ -259,13 +275,31 @@ int ffn_store(const FfnOperand& A, const FfnOperand& B, int M, int N, int k, int
 
 size_t ffn_store_bytes(int M, int N, int k, int planes_m, int planes_k, int sms) {
   const long long tiles = (long long)ceil_div(M, 256) * planes_m * ceil_div(N, 256), elems = (long long)planes_m * M * N;
-  const int s = pick_splits(tiles, ceil_div(k, 64) * planes_k, std::max(1, sms / 2), elems, kFfnBlockUs, kMostSplitBytes);
+  const int s = pick_splits(tiles, ceil_div(k, 64) * planes_k, std::max(1, sms / 2), elems, kFfnBlockUs,
+                            kStoreUnitUs, kMostSplitBytes);
   return s > 1 ? (size_t)s * elems * 4 : 0;
+}
+
+int gate_splits(int T, int H, int I, int sms, size_t cap) {
+  return pick_splits((long long)ceil_div(T, 256) * ceil_div(I, 128), ceil_div(H, 64), std::max(1, sms / 2), 2ll * T * I,
+                     kFfnBlockUs, kGateUnitUs, cap);
+}
+size_t gate_bytes(int T, int H, int I, int sms) {
+  const int s = gate_splits(T, H, I, sms, kMostSplitBytes);
+  return s > 1 ? (size_t)s * T * I * 8 : 0;
+}
+int gate_grad_splits(int T, int H, int I, int sms, size_t cap) {
+  return pick_splits((long long)ceil_div(T, 256) * ceil_div(I, 256), ceil_div(H, 64), std::max(1, sms / 2),
+                     (long long)T * I, kFfnBlockUs, kGateGradUnitUs, cap);
+}
+size_t gate_grad_bytes(int T, int H, int I, int sms) {
+  const int s = gate_grad_splits(T, H, I, sms, kMostSplitBytes);
+  return s > 1 ? (size_t)s * T * I * 4 : 0;
 }
 
 template <int kElem>
 int ffn_gate(const void* x, const void* w1, const void* w3, void* a, void* h, int T, int H, int I, int gate, int sms,
-             cudaStream_t s) {
+             void* ws, size_t ws_bytes, cudaStream_t s) {
   CUtensorMap ta[2], tb[2];
   int rc = map_k(&ta[0], x, kElem, T, H, 128);
   if (rc || (rc = map_k(&tb[0], w1, kElem, I, H, 128)) || (rc = map_k(&tb[1], w3, kElem, I, H, 128))) return rc;
@@ -276,12 +310,16 @@ int ffn_gate(const void* x, const void* w1, const void* w3, void* a, void* h, in
   p.tiles_m = p.m_tiles_plane = ceil_div(T, 256);
   p.tiles_n = ceil_div(I, 128);
   p.k_blocks = p.kb_plane = ceil_div(H, 64);
-  p.splits = 1;
+  p.splits = gate_splits(T, H, I, sms, ws_bytes);
   p.gate = gate;
   p.C = a;
   p.H = h;
   p.h_plane = (long long)T * I;
-  return launch_ffn<FfnCfg<kElem, false, false, kFfnGate>>(ta, tb, p, sms, s);
+  p.ws = static_cast<float*>(ws);
+  rc = launch_ffn<FfnCfg<kElem, false, false, kFfnGate>>(ta, tb, p, sms, s);
+  if (rc || p.splits == 1) return rc;
+  return launch("feed-forward gate sums", ffn_gate_reduce_kernel<kElem>, dim3(grid_for(((long long)T * I / 8 + 255) / 256, sms)),
+                256, 0, s, 0, false, (const float*)p.ws, p.splits, T, I, gate, a, h);
 }
 
 template <int kElem>
@@ -298,7 +336,7 @@ int gated_ffn(const void* x, const void* w1, const void* w2, const void* w3, voi
     if (rc) return rc;
     return stream_store(kElem, w2, a, {}, T, H, I, y, kElem, sms, rest, rest_bytes, s, true);
   }
-  rc = ffn_gate<kElem>(x, w1, w3, a, h, T, H, I, gate, sms, s);
+  rc = ffn_gate<kElem>(x, w1, w3, a, h, T, H, I, gate, sms, rest, rest_bytes, s);
   if (rc) return rc;
   return ffn_store<kElem, false, false>({{a}, 1}, {{w2}, 1}, T, H, I, 1, 1, y, sms, rest, rest_bytes, s);
 }
@@ -325,13 +363,19 @@ int gated_ffn_grad(const void* x, const void* w1, const void* w2, const void* w3
   p.tiles_m = p.m_tiles_plane = ceil_div(T, 256);
   p.tiles_n = ceil_div(I, 256);
   p.k_blocks = p.kb_plane = ceil_div(H, 64);
-  p.splits = 1;
+  p.splits = gate_grad_splits(T, H, I, sms, rest_bytes);
+  p.ws = reinterpret_cast<float*>(rest);
   p.gate = gate;
   p.C = dh;
   p.H = const_cast<void*>(h);
   p.c_plane = p.h_plane = (long long)T * I;
   p.Act = a;
   if ((rc = launch_ffn<FfnCfg<kElem, false, true, kFfnGateGrad>>(ta, tb, p, sms, s))) return rc;
+  if (p.splits > 1 &&
+      (rc = launch("feed-forward gate gradient sums", ffn_gate_grad_reduce_kernel<kElem>,
+                   dim3(grid_for(((long long)T * I / 8 + 255) / 256, sms)), 256, 0, s, 0, false, (const float*)p.ws,
+                   p.splits, T, I, gate, h, (void*)dh, (void*)a)))
+    return rc;
   const FfnOperand dh_planes = {{dh, dh + plane}, 2};
   // plane 1 of dh starts on a 16-byte boundary: a plane is T * I elements, I a multiple of 8
   if ((rc = ffn_store<kElem, false, true>(dh_planes, {{w1, w3}, 2}, T, H, I, 1, 2, d_x, sms, rest, rest_bytes, s)))
@@ -341,12 +385,16 @@ int gated_ffn_grad(const void* x, const void* w1, const void* w2, const void* w3
 }
 
 // ------------------------------------------------------------------ 8-bit tiles
+#ifndef EXP_SINGLE
+#define EXP_SINGLE 0
+#endif
+constexpr bool kFp8Pair = !EXP_SINGLE;
 template <bool kGate>
 int launch_fp8(const void* a, const void* w, const void* w2, int K, Fp8BlockParams& p, int sms, cudaStream_t s) {
-  using Cfg = Fp8BlockCfg<kGate>;
+  using Cfg = Fp8BlockCfg<kGate, kFp8Pair>;
   CUtensorMap ta, tb, tb2;
   int rc = map_k(&ta, a, EK_DTYPE_E4M3, p.M, K, 128);
-  if (rc || (rc = map_k(&tb, w, EK_DTYPE_E4M3, p.N, K, 128))) return rc;
+  if (rc || (rc = map_k(&tb, w, EK_DTYPE_E4M3, p.N, K, kFp8Pair || kGate ? 128 : 256))) return rc;
   tb2 = tb;
   if (kGate && (rc = map_k(&tb2, w2, EK_DTYPE_E4M3, p.N, K, 128))) return rc;
   static bool done[64] = {false};
@@ -354,14 +402,14 @@ int launch_fp8(const void* a, const void* w, const void* w2, int K, Fp8BlockPara
   const long long units = (long long)p.tiles_m * p.tiles_n * p.splits;
   if (units > 0x3fffffff) return set_error(EK_ERR_INVALID, "too many tiles");
   p.num_units = (int)units;
-  const int pairs = (int)std::min<long long>(std::max(1, sms / 2), units);
-  return launch("block-scaled product", fp8_block_kernel<Cfg>, dim3(2 * pairs), Cfg::THREADS, Cfg::SMEM_BYTES, s, 2, false,
-                ta, tb, tb2, p);
+  const int groups = (int)std::min<long long>(std::max(1, sms / Cfg::CTAS), units);
+  return launch("block-scaled product", fp8_block_kernel<Cfg>, dim3(Cfg::CTAS * groups), Cfg::THREADS, Cfg::SMEM_BYTES, s,
+                kFp8Pair ? 2 : 0, false, ta, tb, tb2, p);
 }
 
 int fp8_splits(int M, int N, int K, int sms, size_t cap) {
   return pick_splits((long long)ceil_div(M, 256) * ceil_div(N, 256), ceil_div(K, 128), std::max(1, sms / 2),
-                     (long long)M * N, kFp8BlockUs, cap);
+                     (long long)M * N, kFp8BlockUs, kStoreUnitUs, cap);
 }
 
 int fp8_store(const void* a, const void* w, const float* as, const float* wsc, void* C, int M, int N, int K, int out_type,
@@ -371,7 +419,7 @@ int fp8_store(const void* a, const void* w, const float* as, const float* wsc, v
   Fp8BlockParams p{};
   p.M = M;
   p.N = N;
-  p.tiles_m = ceil_div(M, 256);
+  p.tiles_m = ceil_div(M, kFp8Pair ? 256 : 128);
   p.tiles_n = ceil_div(N, 256);
   p.k_blocks = ceil_div(K, 128);
   p.splits = fp8_splits(M, N, K, sms, ws_bytes);
@@ -474,7 +522,7 @@ size_t ek_gated_ffn_workspace_bytes(int T, int H, int I, int num_sms) {
   if (T == 0) return 0;
   const size_t sums = T <= kStreamTokens
                           ? std::max(stream_bytes_most(I, 128, T, num_sms), stream_bytes_most(H, 256, T, num_sms))
-                          : ffn_store_bytes(T, H, I, 1, 1, num_sms);
+                          : std::max(gate_bytes(T, H, I, num_sms), ffn_store_bytes(T, H, I, 1, 1, num_sms));
   return round256((size_t)T * I * 2) + sums;
 }
 
@@ -500,7 +548,7 @@ size_t ek_gated_ffn_grad_workspace_bytes(int T, int H, int I, int num_sms) {
   if (!sizes_ok(T, H, I, 8) || !sms_ok(num_sms)) return kBad;
   if (T == 0) return 0;
   const size_t sums = std::max({ffn_store_bytes(T, H, I, 1, 2, num_sms), ffn_store_bytes(I, H, T, 2, 1, num_sms),
-                                ffn_store_bytes(H, I, T, 1, 1, num_sms)});
+                                ffn_store_bytes(H, I, T, 1, 1, num_sms), gate_grad_bytes(T, H, I, num_sms)});
   return round256((size_t)T * I * 4) + round256((size_t)T * I * 2) + sums;
 }
 
@@ -559,7 +607,7 @@ int ek_gated_ffn_fp8(const void* x, const void* w1, const void* w2, const void* 
     Fp8BlockParams p{};
     p.M = T;
     p.N = I;
-    p.tiles_m = ceil_div(T, 256);
+    p.tiles_m = ceil_div(T, kFp8Pair ? 256 : 128);
     p.tiles_n = ceil_div(I, 128);
     p.k_blocks = ceil_div(H, 128);
     p.splits = 1;

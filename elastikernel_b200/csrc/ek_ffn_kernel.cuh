@@ -20,8 +20,14 @@
 //   warp 0      TMA producer; warp 1  TMEM and MMA issue
 //   warps 2..9  epilogue, two per TMEM lane quarter, half of the columns each
 //
+// A TMEM lane is a row, so a thread holds 32 consecutive columns of one row. What it
+// reads and writes goes through 2 KB of shared memory per warp: a global access
+// then covers 64 contiguous bytes of each of 8 rows, not 16 of each of 32. The
+// gradient's pre-activations are fetched a chunk ahead.
+//
 // Few tiles: K is split over `splits` units per tile whose fp32 sums go to a
-// workspace, and ffn_reduce_kernel adds them in slice order. No atomics.
+// workspace, and the ffn_*_reduce kernels add them in slice order and do what the
+// epilogue would have done. No atomics.
 #pragma once
 #include <type_traits>
 
@@ -29,6 +35,17 @@
 #include "ek_gemm_kernel.cuh"
 
 namespace ek {
+
+// One lane of a converged warp, always the same. A loop that a whole warp walks with an
+// elected lane issuing keeps the operands of tcgen05.mma uniform; issued from inside a
+// one-lane branch they are moved to the uniform registers one by one, at about 100
+// clocks an instruction (a 128-byte K block of a 256 x 256 tile: 730 clocks of issue
+// for 512 of multiplying).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+  return p != 0;
+}
 
 enum FfnEpi : int { kFfnStore = 0, kFfnGate = 1, kFfnGateGrad = 2 };
 
@@ -42,7 +59,7 @@ struct FfnCfg {
   static constexpr int STAGE_BYTES = 2 * HALF_BYTES;
   static constexpr int EPI_WARPS = 8;
   static constexpr int THREADS = 64 + 32 * EPI_WARPS;
-  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 + 256;
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_WARPS * 2048 + 1024 + 256;
   static constexpr uint32_t IDESC =
       umma_idesc(kElem == kBF16 ? 1u : 0u, kBMN, 256, BN) | ((kAMN ? 1u : 0u) << 15);
 };
@@ -60,7 +77,7 @@ struct FfnParams {
   void* H;               // gate: the pre-activations to write (or null); gate gradient: those to read
   long long h_plane;
   void* Act;             // gate gradient: a
-  float* ws;             // splits > 1: fp32 sums [splits][planes * M][N]
+  float* ws;             // splits > 1: fp32 sums [splits][planes * M][N] (gate/up: [splits][M][2 N])
 };
 
 template <int kElem>
@@ -113,6 +130,70 @@ __device__ __forceinline__ void wait_copies(uint64_t* full_bar, int issued) {
     if (!mbar_wait(&full_bar[i % kStages], (i / kStages) & 1, &never)) return;
 }
 
+// A 32-row x 64-byte tile of a warp in shared memory: written or read as one row per
+// lane, or as 64 bytes of 8 rows at a time (4 lanes a row). The 16-byte pieces of a
+// row are permuted by its number, so neither way meets a bank twice.
+struct WarpTile {
+  uint8_t* base;
+  int lane;
+  __device__ uint4& own(int j) const {
+    return *reinterpret_cast<uint4*>(base + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4));
+  }
+  __device__ uint4& across(int i) const {
+    const int r = i * 8 + (lane >> 2);
+    return *reinterpret_cast<uint4*>(base + r * 64 + (((lane & 3) ^ ((r >> 1) & 3)) << 4));
+  }
+};
+
+// Where lane's piece i of a warp's rows [row0, row0 + 32) x 16-byte groups from
+// element col0 lies in a [rows, n] matrix (kPer elements per piece); < 0: outside.
+template <int kPer>
+__device__ __forceinline__ long long warp_at(int i, int lane, int row0, int rows, int col0, int n, long long ld) {
+  const int r = row0 + i * 8 + (lane >> 2), c = col0 + (lane & 3) * kPer;
+  return r < rows && c < n ? (long long)r * ld + c : -1;
+}
+
+// 64 bytes of each of the warp's rows, the lane's own in v, to out[row0 + lane][col0 ..]
+// of a [rows, n] matrix with kPer elements per 16 bytes and rows of ld (0: n) elements
+template <int kPer>
+__device__ __forceinline__ void store_warp(const WarpTile& w, const uint4 (&v)[4], void* out, int row0, int rows, int col0,
+                                           int n, long long ld = 0) {
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w.own(j) = v[j];
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const long long at = warp_at<kPer>(i, w.lane, row0, rows, col0, n, ld ? ld : n);
+    if (at >= 0) *reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(out) + at * (16 / kPer)) = w.across(i);
+  }
+}
+// 32 columns of fp32, 16 at a time
+__device__ __forceinline__ void store_warp32(const WarpTile& w, const uint32_t (&r)[32], float* out, int row0, int rows,
+                                             int col0, int n, long long ld) {
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    uint4 v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t* q = r + half * 16 + j * 4;
+      v[j] = make_uint4(q[0], q[1], q[2], q[3]);
+    }
+    store_warp<4>(w, v, out, row0, rows, col0 + half * 16, n, ld);
+  }
+}
+
+template <int kElem>
+__device__ __forceinline__ uint4 pack8(const float* v) {
+  return make_uint4(Elem16<kElem>::pack(v[0], v[1]), Elem16<kElem>::pack(v[2], v[3]), Elem16<kElem>::pack(v[4], v[5]),
+                    Elem16<kElem>::pack(v[6], v[7]));
+}
+template <int kElem>
+__device__ __forceinline__ void pack32(const uint32_t (&r)[32], uint4 (&v)[4]) {
+#pragma unroll
+  for (int g = 0; g < 4; ++g) v[g] = pack8<kElem>(reinterpret_cast<const float*>(r) + g * 8);
+}
+
 struct FfnUnit {
   int tm, tn, m_plane, m_row, split, kb0, kb1;
 };
@@ -152,7 +233,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
   constexpr int STAGES = Cfg::STAGES, BN = Cfg::BN, BK = Cfg::BK, HB = Cfg::HALF_BYTES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + STAGES * Cfg::STAGE_BYTES);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + STAGES * Cfg::STAGE_BYTES + Cfg::EPI_WARPS * 2048);
   uint64_t* empty_bar = full_bar + STAGES;
   uint64_t* tfull_bar = empty_bar + STAGES;
   uint64_t* tempty_bar = tfull_bar + 2;
@@ -240,43 +321,46 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0 && leader) {
+    if (leader) {
       int stage = 0, acc_i = 0;
       uint32_t phase = 0;
       bool ok = true;
+      // MN-major: 16 rows of K are 2 KB on, the 64-column chunks BK * 128 bytes apart
+      constexpr uint32_t a_step = Cfg::kAMN ? 2048 >> 4 : 32 >> 4, b_step = Cfg::kBMN ? 2048 >> 4 : 32 >> 4;
+      const uint64_t a_desc = umma_desc_sw128(smem_u32(smem), Cfg::kAMN ? BK * 128 : 16, 1024);
+      const uint64_t b_desc = umma_desc_sw128(smem_u32(smem) + HB, Cfg::kBMN ? BK * 128 : 16, 1024);
       for (int u = unit0; u < p.num_units && ok; u += unit_step, ++acc_i) {
         const FfnUnit w = ffn_unit<Cfg>(p, u);
         const int buf = acc_i & 1;
-        if (!mbar_wait(&tempty_bar[buf], ((acc_i >> 1) & 1) ^ 1, s_abort)) break;
+        ok = mbar_wait(&tempty_bar[buf], ((acc_i >> 1) & 1) ^ 1, s_abort);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + buf * BN;
         for (int kb = w.kb0; kb < w.kb1; ++kb) {
-          if (!mbar_wait(&full_bar[stage], phase, s_abort)) { ok = false; break; }
+          ok = mbar_wait(&full_bar[stage], phase, s_abort);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
           tc_fence_after();
-          const uint32_t a0 = smem_u32(smem + stage * Cfg::STAGE_BYTES), b0 = a0 + HB;
+          const uint32_t off = stage * (Cfg::STAGE_BYTES >> 4);
+          if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < BK / 16; ++k) {
-            // MN-major: 16 rows of K are 2 KB on, the 64-column chunks BK * 128 bytes apart
-            const uint64_t ad = Cfg::kAMN ? umma_desc_sw128(a0 + k * 2048, BK * 128, 1024)
-                                          : umma_desc_sw128(a0 + k * 32, 16, 1024);
-            const uint64_t bd = Cfg::kBMN ? umma_desc_sw128(b0 + k * 2048, BK * 128, 1024)
-                                          : umma_desc_sw128(b0 + k * 32, 16, 1024);
-            umma_pair<false>(d_tmem, ad, bd, Cfg::IDESC, (kb > w.kb0 || k > 0) ? 1u : 0u);
+            for (int k = 0; k < BK / 16; ++k)
+              umma_pair<false>(d_tmem, a_desc + off + k * a_step, b_desc + off + k * b_step, Cfg::IDESC,
+                               (kb > w.kb0 || k > 0) ? 1u : 0u);
+            umma_commit_pair(&empty_bar[stage], 0x3);
+            if (kb + 1 == w.kb1) umma_commit_pair(&tfull_bar[buf], 0x3);
           }
-          umma_commit_pair(&empty_bar[stage], 0x3);
+          __syncwarp();
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
-        if (!ok) break;
-        umma_commit_pair(&tfull_bar[buf], 0x3);
       }
       // every MMA issued so far has completed (in both CTAs) before TMEM is freed
-      umma_commit_pair(drain_bar, 0x3);
-      volatile int never = 0;
-      mbar_wait(drain_bar, 0, &never);
-    } else if (lane == 0) {
-      volatile int never = 0;
-      mbar_wait(drain_bar, 0, &never);
+      if (elect_one()) umma_commit_pair(drain_bar, 0x3);
+      __syncwarp();
     }
+    volatile int never = 0;
+    mbar_wait(drain_bar, 0, &never);
     __syncwarp();
   } else {
     const int q = warp & 3;           // TMEM lane quarter of this warp
@@ -287,16 +371,29 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(tempty0 + buf * 8);
     };
+    const WarpTile wt{smem + STAGES * Cfg::STAGE_BYTES + (warp - 2) * 2048, lane};
     int acc_i = 0;
     for (int u = unit0; u < p.num_units; u += unit_step, ++acc_i) {
       const FfnUnit w = ffn_unit<Cfg>(p, u);
       const int buf = acc_i & 1;
+      const int row0 = w.m_row + rank * 128 + q * 32;  // first row of this warp
+      const bool split = p.splits > 1;
+      // gradient of the gate: the pre-activations of a 32-column chunk, 64 bytes of 8 rows a load
+      uint4 n1[4], n3[4];
+      auto fetch_h = [&](int c) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const long long at = warp_at<8>(i, lane, row0, p.M, w.tn * BN + half * 128 + c * 32, p.N, p.N);
+          const uint16_t* h = reinterpret_cast<const uint16_t*>(p.H);
+          n1[i] = at >= 0 ? __ldg(reinterpret_cast<const uint4*>(h + at)) : make_uint4(0, 0, 0, 0);
+          n3[i] = at >= 0 ? __ldg(reinterpret_cast<const uint4*>(h + p.h_plane + at)) : make_uint4(0, 0, 0, 0);
+        }
+      };
+      if (Cfg::kEpi == kFfnGateGrad && !split) fetch_h(0);
       const bool got = mbar_wait(&tfull_bar[buf], (acc_i >> 1) & 1, s_abort);
       if (!__all_sync(0xffffffffu, got)) break;  // the TMEM loads are warp-collective
       tc_fence_after();
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buf * BN;
-      const int row = w.m_row + rank * 128 + q * 32 + lane;
-      const bool row_ok = row < p.M;
       if constexpr (Cfg::kEpi == kFfnGate) {
 #pragma unroll 1
         for (int c = 0; c < 2; ++c) {
@@ -308,64 +405,74 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
           reg_dep(ru);
           if (c == 1) release(buf);
           const int col = w.tn * 128 + f0;
-          if (row_ok) {
-            const size_t at = (size_t)row * p.N + col;
-            if (p.H != nullptr) {
-#pragma unroll
-              for (int g = 0; g < 4; ++g)
-                if (col + g * 8 < p.N) {
-                  store8<Cfg::kElem>(p.H, at + g * 8, reinterpret_cast<float*>(rg) + g * 8);
-                  store8<Cfg::kElem>(p.H, p.h_plane + at + g * 8, reinterpret_cast<float*>(ru) + g * 8);
-                }
-            }
-            with_gate(p.gate, [&](auto fn) {
-#pragma unroll
-              for (int j = 0; j < 32; ++j)
-                rg[j] = __float_as_uint(gate_f<decltype(fn)::value>(__uint_as_float(rg[j])) * __uint_as_float(ru[j]));
-            });
-#pragma unroll
-            for (int g = 0; g < 4; ++g)
-              if (col + g * 8 < p.N) store8<Cfg::kElem>(p.C, at + g * 8, reinterpret_cast<float*>(rg) + g * 8);
+          if (split) {
+            float* out = p.ws + (size_t)w.split * p.M * (2ll * p.N);
+            store_warp32(wt, rg, out, row0, p.M, col, p.N, 2ll * p.N);
+            store_warp32(wt, ru, out + p.N, row0, p.M, col, p.N, 2ll * p.N);
+            continue;
           }
+          uint4 v[4];
+          if (p.H != nullptr) {
+            pack32<Cfg::kElem>(rg, v);
+            store_warp<8>(wt, v, p.H, row0, p.M, col, p.N);
+            pack32<Cfg::kElem>(ru, v);
+            store_warp<8>(wt, v, reinterpret_cast<uint16_t*>(p.H) + p.h_plane, row0, p.M, col, p.N);
+          }
+          with_gate(p.gate, [&](auto fn) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              rg[j] = __float_as_uint(gate_f<decltype(fn)::value>(__uint_as_float(rg[j])) * __uint_as_float(ru[j]));
+          });
+          pack32<Cfg::kElem>(rg, v);
+          store_warp<8>(wt, v, p.C, row0, p.M, col, p.N);
         }
       } else {
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
-          const int c0 = half * 128 + c * 32;
+          const int c0 = half * 128 + c * 32, col = w.tn * BN + c0;
           uint32_t r[32];
           tmem_ld32(t_row + c0, r);
           tmem_ld_wait(r);
           if (c == 3) release(buf);
-          const int col = w.tn * BN + c0;
-          if (!row_ok) continue;
-          const float* v = reinterpret_cast<const float*>(r);
-          const size_t at = (size_t)row * p.N + col;
+          if (split) {
+            const int planes = p.tiles_m / p.m_tiles_plane;
+            store_warp32(wt, r, p.ws + (size_t)(w.split * planes + w.m_plane) * p.M * p.N, row0, p.M, col, p.N, p.N);
+            continue;
+          }
+          uint4 v[4];
           if constexpr (Cfg::kEpi == kFfnGateGrad) {
+            uint4 h1[4], h3[4], va[4];
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) wt.across(i) = n1[i];
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) h1[j] = wt.own(j);
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) wt.across(i) = n3[i];
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) h3[j] = wt.own(j);
+            if (c < 3) fetch_h(c + 1);
             with_gate(p.gate, [&](auto fn) {
 #pragma unroll
-              for (int g = 0; g < 4; ++g)
-                if (col + g * 8 < p.N) {
-                  const uint16_t* h = reinterpret_cast<const uint16_t*>(p.H) + at + g * 8;
-                  float h1[8], h3[8], d1[8], d3[8], a[8];
-                  unpack8<Cfg::kElem>(__ldg(reinterpret_cast<const uint4*>(h)), h1);
-                  unpack8<Cfg::kElem>(__ldg(reinterpret_cast<const uint4*>(h + p.h_plane)), h3);
-                  gate_grad8<decltype(fn)::value>(v + g * 8, h1, h3, d1, d3, a);
-                  store8<Cfg::kElem>(p.C, at + g * 8, d1);
-                  store8<Cfg::kElem>(p.C, p.c_plane + at + g * 8, d3);
-                  store8<Cfg::kElem>(p.Act, at + g * 8, a);
-                }
+              for (int g = 0; g < 4; ++g) {
+                float z1[8], z3[8], d1[8], d3[8], a[8];
+                unpack8<Cfg::kElem>(h1[g], z1);
+                unpack8<Cfg::kElem>(h3[g], z3);
+                gate_grad8<decltype(fn)::value>(reinterpret_cast<const float*>(r) + g * 8, z1, z3, d1, d3, a);
+                v[g] = pack8<Cfg::kElem>(d1);
+                h3[g] = pack8<Cfg::kElem>(d3);
+                va[g] = pack8<Cfg::kElem>(a);
+              }
             });
-          } else if (p.splits > 1) {
-            float* out = p.ws + ((size_t)w.split * (p.tiles_m / p.m_tiles_plane) + w.m_plane) * p.M * p.N + at;
-#pragma unroll
-            for (int g = 0; g < 8; ++g)
-              if (col + g * 4 < p.N)
-                __stcg(reinterpret_cast<float4*>(out + g * 4), make_float4(v[4 * g], v[4 * g + 1], v[4 * g + 2],
-                                                                           v[4 * g + 3]));
+            store_warp<8>(wt, v, p.C, row0, p.M, col, p.N);
+            store_warp<8>(wt, h3, reinterpret_cast<uint16_t*>(p.C) + p.c_plane, row0, p.M, col, p.N);
+            store_warp<8>(wt, va, p.Act, row0, p.M, col, p.N);
           } else {
-#pragma unroll
-            for (int g = 0; g < 4; ++g)
-              if (col + g * 8 < p.N) store8<Cfg::kElem>(p.C, w.m_plane * p.c_plane + at + g * 8, v + g * 8);
+            pack32<Cfg::kElem>(r, v);
+            store_warp<8>(wt, v, reinterpret_cast<uint16_t*>(p.C) + w.m_plane * p.c_plane, row0, p.M, col, p.N);
           }
         }
       }
@@ -381,20 +488,70 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
   }
 }
 
-// out[i] = sum over the slices, in slice order, of ws[s][i], rounded once. n8:
-// groups of 8 elements of the result (both planes); they lie end to end in both.
+// The sum over the slices, in slice order, of 8 elements that lie `at` floats into
+// each slice of `stride` floats.
+__device__ __forceinline__ void sum_slices8(const float* __restrict__ ws, int splits, size_t stride, size_t at,
+                                            float (&v)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = 0.f;
+  for (int s = 0; s < splits; ++s) {
+    const float4* src = reinterpret_cast<const float4*>(ws + s * stride + at);
+    const float4 a = __ldcg(src), b = __ldcg(src + 1);
+    v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+    v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+  }
+}
+
+// out[i] = sum of the slices, rounded once; n8: groups of 8 elements of the result
+// (both planes), which lie end to end in both
 template <int kElem>
 __global__ void __launch_bounds__(256) ffn_reduce_kernel(const float* __restrict__ ws, int splits, long long n8,
                                                          void* __restrict__ out) {
   for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n8; i += gridDim.x * 256ll) {
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < splits; ++s) {
-      const float4* src = reinterpret_cast<const float4*>(ws) + (s * n8 + i) * 2;
-      const float4 a = __ldcg(src), b = __ldcg(src + 1);
-      v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
-      v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
-    }
+    float v[8];
+    sum_slices8(ws, splits, n8 * 8, i * 8, v);
     store8<kElem>(out, (size_t)i * 8, v);
+  }
+}
+
+// a = f(h1) h3 and on request h1 and h3, from slices of [T][h1 | h3]
+template <int kElem>
+__global__ void __launch_bounds__(256) ffn_gate_reduce_kernel(const float* __restrict__ ws, int splits, int T, int I,
+                                                              int gate, void* __restrict__ a, void* __restrict__ h) {
+  const long long n8 = (long long)T * I / 8;
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n8; i += gridDim.x * 256ll) {
+    const long long row = i * 8 / I, at = row * 2 * I + (i * 8 - row * I);
+    float g[8], u[8];
+    sum_slices8(ws, splits, 2ll * T * I, at, g);
+    sum_slices8(ws, splits, 2ll * T * I, at + I, u);
+    if (h != nullptr) {
+      store8<kElem>(h, i * 8, g);
+      store8<kElem>(h, (size_t)T * I + i * 8, u);
+    }
+    with_gate(gate, [&](auto fn) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) g[j] = gate_f<decltype(fn)::value>(g[j]) * u[j];
+    });
+    store8<kElem>(a, i * 8, g);
+  }
+}
+
+// dh1, dh3 and a from slices of da [T][I] and the pre-activations
+template <int kElem>
+__global__ void __launch_bounds__(256)
+    ffn_gate_grad_reduce_kernel(const float* __restrict__ ws, int splits, int T, int I, int gate,
+                                const void* __restrict__ h, void* __restrict__ dh, void* __restrict__ act) {
+  const long long n8 = (long long)T * I / 8;
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n8; i += gridDim.x * 256ll) {
+    const uint4* src = reinterpret_cast<const uint4*>(h) + i;
+    float da[8], h1[8], h3[8], d1[8], d3[8], a[8];
+    unpack8<kElem>(__ldg(src), h1);
+    unpack8<kElem>(__ldg(src + n8), h3);
+    sum_slices8(ws, splits, n8 * 8, i * 8, da);
+    with_gate(gate, [&](auto fn) { gate_grad8<decltype(fn)::value>(da, h1, h3, d1, d3, a); });
+    store8<kElem>(dh, i * 8, d1);
+    store8<kElem>(dh, (size_t)(n8 + i) * 8, d3);
+    store8<kElem>(act, i * 8, a);
   }
 }
 

@@ -7,29 +7,36 @@
 // each CTA loading its 128 token rows and half of the tile's weight rows. The
 // scales are fp32, so the tensor cores cannot apply them: each 128-wide K block is
 // multiplied into one of two TMEM buffers, and while the next block's MMA runs, the
-// epilogue warps read the product, multiply it by its one scale per row and half
-// tile (a 128-column half lies in one weight block) and add it to fp32
-// accumulators in registers. 256 threads hold 128 accumulators each; setmaxnreg
-// gives them the registers that the loading and issuing warps do not need.
+// epilogue warps read the product, multiply it by its one scale per row and weight
+// block and add it to fp32 accumulators in registers.
 //
-//   warp 0  TMA producer; warp 1  TMEM and MMA; warps 2, 3  idle
-//   warps 4..11  epilogue, two per TMEM lane quarter: plain tiles half of the
-//   columns each, gate tiles 64 gate columns and the same features' 64 up columns
+//   warp 0  TMA producer; warp 1  TMEM and MMA; warp 2  scales; warp 3  idle
+//   warps 4..11  epilogue, two per TMEM lane quarter, 128 accumulators a thread: group
+//   g has of a plain tile the columns [128 g, +128), of a gate tile 64 gate columns
+//   and the same features' 64 up columns. setmaxnreg gives them the registers that
+//   the other warps do not need. A chunk of 32 columns is always in flight from TMEM
+//   while the one before it is added, the first chunk of the next K block among them.
 #pragma once
 #include "ek_stream_kernel.cuh"
 
 namespace ek {
 
-template <bool kGate_>
+template <bool kGate_, bool kPair_>
 struct Fp8BlockCfg {
-  static constexpr bool kGate = kGate_;
-  static constexpr int STAGES = 6, HALF_BYTES = 128 * 128, STAGE_BYTES = 2 * HALF_BYTES;
+  static constexpr bool kGate = kGate_, kPair = kPair_;
+  static constexpr int CTAS = kPair ? 2 : 1;
+  static constexpr int HALF_BYTES = 128 * 128, STAGE_BYTES = (kPair ? 2 : 3) * HALF_BYTES;
+  static constexpr int STAGES = kPair ? 6 : 4;
   static constexpr int EPI_WARPS = 8;
   static constexpr int THREADS = 128 + 32 * EPI_WARPS;
-  // 384 threads are launched with 168 registers each: 4 x 32 x 56 + 8 x 32 x 224 = 64512 = 384 x 168
+  // 384 threads are launched with 168 registers each: 128 x 56 + 256 x 224 = 64512 = 384 x 168
   static constexpr int REGS_LOAD = 56, REGS_EPI = 224;
-  static constexpr uint32_t IDESC = umma_idesc(0u, false, 256, 256);
-  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 /*amax*/ + 256 + 1024;
+  static constexpr uint32_t IDESC = umma_idesc(0u, false, 128 * CTAS, 256);
+  // Scales: slots of SGROUP K blocks, each 128 rows' and the two weight blocks' scales
+  static constexpr int SGROUP = 4, SLOTS = 3, SLOT_STRIDE = 132;
+  static constexpr int SCALE_BYTES = SLOTS * SGROUP * SLOT_STRIDE * 4;
+  static constexpr int SMEM_BYTES =
+      STAGES * STAGE_BYTES + EPI_WARPS * 2048 + 1024 /*largest values*/ + SCALE_BYTES + 256 + 1024;
 };
 
 struct Fp8BlockParams {
@@ -48,36 +55,50 @@ struct Fp8BlockParams {
   float* scales;
 };
 
-// 32 consecutive columns of a row, from column col
-__device__ __forceinline__ void fp8_block_store32(const Fp8BlockParams& p, void* base, int type, size_t row_at, int col,
+// 32 consecutive columns, from column col, of the warp's rows [row0, row0 + 32): of the
+// result, or of a slice's sums
+__device__ __forceinline__ void fp8_block_store32(const Fp8BlockParams& p, const WarpTile& wt, int split, int row0, int col,
                                                   const float2* v2) {
   const float* v = reinterpret_cast<const float*>(v2);
-  if (p.wide || type == kOutFP32) {
-    if (type == kOutFP32) {
-      float* out = reinterpret_cast<float*>(base) + row_at + col;
-      if (p.wide) {
+  const bool sums = p.splits > 1;
+  if (p.wide && (sums || p.out_type == kOutFP32)) {
+    float* out = sums ? p.ws + (size_t)split * p.M * p.N : reinterpret_cast<float*>(p.C);
 #pragma unroll
-        for (int g = 0; g < 8; ++g)
-          if (col + g * 4 < p.N) *reinterpret_cast<float4*>(out + g * 4) = make_float4(v[4 * g], v[4 * g + 1],
-                                                                                   v[4 * g + 2], v[4 * g + 3]);
-      } else {
+    for (int h = 0; h < 2; ++h) {
+      uint4 pk[4];
 #pragma unroll
-        for (int j = 0; j < 32; ++j)
-          if (col + j < p.N) out[j] = v[j];
-      }
-    } else if (type == kOutBF16) {
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        if (col + g * 8 < p.N) store8<kBF16>(base, row_at + col + g * 8, v + g * 8);
-    } else {
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        if (col + g * 8 < p.N) store8<kFP16>(base, row_at + col + g * 8, v + g * 8);
+      for (int g = 0; g < 4; ++g) pk[g] = *reinterpret_cast<const uint4*>(v + h * 16 + g * 4);
+      store_warp<4>(wt, pk, out, row0, p.M, col + h * 16, p.N);
     }
-  } else {
+  } else if (p.wide) {
+    uint4 pk[4];
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (col + j < p.N) store_out(base, type, row_at + col + j, v[j]);
+    for (int g = 0; g < 4; ++g) pk[g] = p.out_type == kOutBF16 ? pack8<kBF16>(v + g * 8) : pack8<kFP16>(v + g * 8);
+    store_warp<8>(wt, pk, p.C, row0, p.M, col, p.N);
+  } else {
+    // rows that no 16-byte piece fits: 32 columns of a row at a time, one per lane
+    float* t = reinterpret_cast<float*>(wt.base);
+#pragma unroll 1
+    for (int h = 0; h < 2; ++h) {  // 2 KB hold 16 rows
+      __syncwarp();
+      if ((wt.lane >> 4) == h) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) t[(wt.lane & 15) * 32 + ((j + wt.lane) & 31)] = v[j];
+      }
+      __syncwarp();
+#pragma unroll 1
+      for (int r = 0; r < 16; ++r) {
+        const int row = row0 + h * 16 + r, c = col + wt.lane;
+        const float x = t[r * 32 + ((wt.lane + h * 16 + r) & 31)];
+        if (row < p.M && c < p.N) {
+          const size_t at = (size_t)row * p.N + c;
+          if (sums)
+            p.ws[(size_t)split * p.M * p.N + at] = x;
+          else
+            store_out(p.C, p.out_type, at, x);
+        }
+      }
+    }
   }
 }
 
@@ -85,22 +106,27 @@ template <class Cfg>
 __global__ void __launch_bounds__(Cfg::THREADS, 1)
     fp8_block_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                      const __grid_constant__ CUtensorMap tmB2, const Fp8BlockParams p) {
-  constexpr int STAGES = Cfg::STAGES, HB = Cfg::HALF_BYTES;
+  constexpr int STAGES = Cfg::STAGES, HB = Cfg::HALF_BYTES, NS = Cfg::SLOTS, SG = Cfg::SGROUP, RS = Cfg::SLOT_STRIDE;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* s_amax = reinterpret_cast<float*>(smem + STAGES * Cfg::STAGE_BYTES);  // [2][128]
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(s_amax + 256);
+  uint8_t* s_tile = smem + STAGES * Cfg::STAGE_BYTES;                           // [EPI_WARPS] of 2 KB
+  float* s_amax = reinterpret_cast<float*>(s_tile + Cfg::EPI_WARPS * 2048);     // [2][128]
+  float* s_scale = s_amax + 256;                                                // [SLOTS][SGROUP][SLOT_STRIDE]
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(s_scale + NS * SG * RS);
   uint64_t* empty_bar = full_bar + STAGES;
   uint64_t* kfull_bar = empty_bar + STAGES;
   uint64_t* kempty_bar = kfull_bar + 2;
-  uint64_t* drain_bar = kempty_bar + 2;
+  uint64_t* sfull_bar = kempty_bar + 2;
+  uint64_t* sempty_bar = sfull_bar + NS;
+  uint64_t* drain_bar = sempty_bar + NS;
   uint32_t* s_tmem_base = reinterpret_cast<uint32_t*>(drain_bar + 1);
   volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem_base + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = (int)cluster_ctarank();
+  const int rank = Cfg::kPair ? (int)cluster_ctarank() : 0;
   const bool leader = rank == 0;
-  const int unit0 = (int)cluster_id_x(), unit_step = (int)nclusters_x();
+  const int unit0 = Cfg::kPair ? (int)cluster_id_x() : (int)blockIdx.x;
+  const int unit_step = Cfg::kPair ? (int)nclusters_x() : (int)gridDim.x;
   const int KB = p.k_blocks;
 
   if (threadIdx.x == 0) {
@@ -110,19 +136,23 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&kfull_bar[b], 1);
-      mbar_init(&kempty_bar[b], Cfg::EPI_WARPS * 2);
+      mbar_init(&kempty_bar[b], Cfg::EPI_WARPS * Cfg::CTAS);
+    }
+    for (int s = 0; s < NS; ++s) {
+      mbar_init(&sfull_bar[s], 32);
+      mbar_init(&sempty_bar[s], Cfg::EPI_WARPS);
     }
     mbar_init(drain_bar, 1);
     *s_abort = 0;
     fence_mbar_init();
   }
   if (warp == 1) {
-    tmem_alloc<2>(s_tmem_base, 512);
-    tmem_relinquish<2>();
+    tmem_alloc<Cfg::CTAS>(s_tmem_base, 512);
+    tmem_relinquish<Cfg::CTAS>();
   }
   tc_fence_before();
   __syncthreads();
-  cluster_sync();  // the peer's barriers exist before anyone signals them
+  if constexpr (Cfg::kPair) cluster_sync();  // the peer's barriers exist before anyone signals them
   tc_fence_after();
   const uint32_t tmem_base = *s_tmem_base;
 
@@ -148,128 +178,189 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
       int stage = 0, issued = 0;
       uint32_t phase = 0;
       bool ok = true;
-      const uint32_t full0 = mapa_shared(smem_u32(&full_bar[0]), 0);  // both CTAs' loads complete on the leader's
-      const CUtensorMap* tb = (Cfg::kGate && !leader) ? &tmB2 : &tmB;
+      const uint32_t full0 = Cfg::kPair ? mapa_shared(smem_u32(&full_bar[0]), 0) : 0;  // loads complete on the leader's
+      const CUtensorMap* tb = (Cfg::kPair && Cfg::kGate && !leader) ? &tmB2 : &tmB;
       for (int u = unit0; u < p.num_units && ok; u += unit_step) {
         const U w = unit(u);
-        const int a_row = w.tm * 256 + rank * 128;
+        const int a_row = (w.tm * Cfg::CTAS + rank) * 128;
         const int b_row = Cfg::kGate ? w.tn * 128 : w.tn * 256 + rank * 128;
         for (int kb = w.kb0; kb < w.kb1; ++kb) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1, s_abort)) { ok = false; break; }
           uint8_t* dst = smem + stage * Cfg::STAGE_BYTES;
-          if (leader) mbar_arrive_expect_tx(&full_bar[stage], 2 * Cfg::STAGE_BYTES);
-          tma_load_2d_pair(dst, &tmA, full0 + stage * 8, kb * 128, a_row);
-          tma_load_2d_pair(dst + HB, tb, full0 + stage * 8, kb * 128, b_row);
+          if constexpr (Cfg::kPair) {
+            if (leader) mbar_arrive_expect_tx(&full_bar[stage], 2 * Cfg::STAGE_BYTES);
+            tma_load_2d_pair(dst, &tmA, full0 + stage * 8, kb * 128, a_row);
+            tma_load_2d_pair(dst + HB, tb, full0 + stage * 8, kb * 128, b_row);
+          } else {
+            mbar_arrive_expect_tx(&full_bar[stage], Cfg::STAGE_BYTES);
+            tma_load_2d(dst, &tmA, &full_bar[stage], kb * 128, a_row);
+            tma_load_2d(dst + HB, &tmB, &full_bar[stage], kb * 128, b_row);
+            if constexpr (Cfg::kGate) tma_load_2d(dst + 2 * HB, &tmB2, &full_bar[stage], kb * 128, b_row);
+          }
           ++issued;
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
       }
       if (!ok && leader) wait_copies<STAGES>(full_bar, issued);
-    } else if (warp == 1 && lane == 0 && leader) {
+    } else if (warp == 1 && leader) {
+      // the whole warp walks the loop and one elected lane issues, so that what it
+      // issues is uniform (elect_one)
       int stage = 0, gkb = 0;
       uint32_t phase = 0;
       bool ok = true;
+      const uint64_t a_desc = umma_desc_sw128(smem_u32(smem), 16, 1024);
+      const uint64_t b_desc = umma_desc_sw128(smem_u32(smem) + HB, 16, 1024);
       for (int u = unit0; u < p.num_units && ok; u += unit_step) {
         const U w = unit(u);
         for (int kb = w.kb0; kb < w.kb1; ++kb, ++gkb) {
           const int buf = gkb & 1;
-          if (!mbar_wait(&kempty_bar[buf], ((gkb >> 1) & 1) ^ 1, s_abort) ||
-              !mbar_wait(&full_bar[stage], phase, s_abort)) {
-            ok = false;
-            break;
-          }
+          ok = mbar_wait(&full_bar[stage], phase, s_abort) && mbar_wait(&kempty_bar[buf], ((gkb >> 1) & 1) ^ 1, s_abort);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
           tc_fence_after();
-          const uint32_t a0 = smem_u32(smem + stage * Cfg::STAGE_BYTES);
+          const uint32_t off = stage * (Cfg::STAGE_BYTES >> 4);
+          if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_pair<true>(tmem_base + buf * 256, umma_desc_sw128(a0 + k * 32, 16, 1024),
-                            umma_desc_sw128(a0 + HB + k * 32, 16, 1024), Cfg::IDESC, k > 0 ? 1u : 0u);
-          umma_commit_pair(&empty_bar[stage], 0x3);
-          umma_commit_pair(&kfull_bar[buf], 0x3);
+            for (int k = 0; k < 4; ++k) {
+              if constexpr (Cfg::kPair)
+                umma_pair<true>(tmem_base + buf * 256, a_desc + off + 2 * k, b_desc + off + 2 * k, Cfg::IDESC, k > 0);
+              else
+                umma<true>(tmem_base + buf * 256, a_desc + off + 2 * k, b_desc + off + 2 * k, Cfg::IDESC, k > 0);
+            }
+            if constexpr (Cfg::kPair) {
+              umma_commit_pair(&kfull_bar[buf], 0x3);
+              umma_commit_pair(&empty_bar[stage], 0x3);
+            } else {
+              umma_commit(&kfull_bar[buf]);
+              umma_commit(&empty_bar[stage]);
+            }
+          }
+          __syncwarp();
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
       }
-      umma_commit_pair(drain_bar, 0x3);  // every MMA has completed (in both CTAs) before TMEM is freed
+      if (elect_one()) {  // every MMA has completed (in both CTAs) before TMEM is freed
+        if constexpr (Cfg::kPair)
+          umma_commit_pair(drain_bar, 0x3);
+        else
+          umma_commit(drain_bar);
+      }
+      __syncwarp();
       volatile int never = 0;
       mbar_wait(drain_bar, 0, &never);
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1) {
       volatile int never = 0;
       mbar_wait(drain_bar, 0, &never);
+    } else if (warp == 2) {
+      // scales by asynchronous copies that run ahead of the epilogue, SGROUP K blocks a slot:
+      // fetched in the epilogue's own loop, their latency bounded every K block
+      int g = 0;
+      bool ok = true;
+      for (int u = unit0; u < p.num_units && ok; u += unit_step) {
+        const U w = unit(u);
+        const int row = (w.tm * Cfg::CTAS + rank) * 128 + lane * 4;
+        for (int kb = w.kb0; kb < w.kb1; kb += SG, ++g) {
+          const int slot = g % NS;
+          ok = mbar_wait(&sempty_bar[slot], ((g / NS) & 1) ^ 1, s_abort);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          const int n = min(SG, w.kb1 - kb);
+          for (int j = 0; j < n; ++j) {
+            float* dst = s_scale + (slot * SG + j) * RS;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const bool in = row + i < p.M;
+              cp_async_4_zfill(dst + lane * 4 + i, p.a_scale + (in ? (size_t)(row + i) * KB + kb + j : 0), in ? 4 : 0);
+            }
+            if (lane < 2) {
+              const int blk = Cfg::kGate ? w.tn : 2 * w.tn + lane;
+              const float* src = Cfg::kGate && lane ? p.w_scale2 : p.w_scale;
+              const bool in = blk < p.w_blocks;
+              cp_async_4_zfill(dst + 128 + lane, src + (in ? (size_t)blk * KB + kb + j : 0), in ? 4 : 0);
+            }
+          }
+          cp_async_mbar_arrive(&sfull_bar[slot]);
+        }
+      }
+      cp_async_wait<0>();  // no copy into shared memory outlives the CTA
     }
     __syncwarp();
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::REGS_EPI));
     const int q = warp & 3, wg = (warp - 4) >> 2;
     const int lrow = q * 32 + lane;
-    const uint32_t kempty0 = mapa_shared(smem_u32(&kempty_bar[0]), 0);
+    const WarpTile wt{s_tile + (warp - 4) * 2048, lane};
+    const uint32_t kempty0 = Cfg::kPair ? mapa_shared(smem_u32(&kempty_bar[0]), 0) : 0;
+    // this thread's accumulators as columns of the tile: 64 from run0 on, 64 from run1 on
     const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
-    int gkb = 0;
+    const uint32_t run0 = Cfg::kGate ? wg * 64 : wg * 128, run1 = Cfg::kGate ? 128 + wg * 64 : wg * 128 + 64;
+    const int wsel = 128 + (Cfg::kGate ? 0 : wg);
+    int gkb = 0, gs = 0;  // K blocks, scale slots
     for (int u = unit0; u < p.num_units; u += unit_step) {
       const U w = unit(u);
-      const int row = w.tm * 256 + rank * 128 + lrow;
-      const bool row_ok = row < p.M;
-      const float* sa = p.a_scale + (size_t)(row_ok ? row : 0) * KB;
-      const int blk = Cfg::kGate ? w.tn : w.tn * 2 + wg;
-      const bool blk_ok = blk < p.w_blocks;
-      const float* sw = p.w_scale + (size_t)(blk_ok ? blk : 0) * KB;
-      const float* sw2 = Cfg::kGate ? p.w_scale2 + (size_t)blk * KB : sw;
+      const int row0 = (w.tm * Cfg::CTAS + rank) * 128 + q * 32;
       float2 acc[64];
 #pragma unroll
       for (int j = 0; j < 64; ++j) acc[j] = make_float2(0.f, 0.f);
-      // scales of this K block and the two after it
-      float s0 = 0.f, s1 = 0.f, g0 = 0.f, g1 = 0.f, h0 = 0.f, h1 = 0.f;
-      s0 = __ldg(sa + w.kb0);
-      g0 = __ldg(sw + w.kb0);
-      h0 = Cfg::kGate ? __ldg(sw2 + w.kb0) : g0;
-      if (w.kb0 + 1 < w.kb1) {
-        s1 = __ldg(sa + w.kb0 + 1);
-        g1 = __ldg(sw + w.kb0 + 1);
-        h1 = Cfg::kGate ? __ldg(sw2 + w.kb0 + 1) : g1;
-      }
-      bool good = true;
-      for (int kb = w.kb0; kb < w.kb1; ++kb, ++gkb) {
-        float s2 = 0.f, g2 = 0.f, h2 = 0.f;
-        if (kb + 2 < w.kb1) {
-          s2 = __ldg(sa + kb + 2);
-          g2 = __ldg(sw + kb + 2);
-          h2 = Cfg::kGate ? __ldg(sw2 + kb + 2) : g2;
-        }
-        const int buf = gkb & 1;
-        const bool got = mbar_wait(&kfull_bar[buf], (gkb >> 1) & 1, s_abort);
-        good = __all_sync(0xffffffffu, got);  // the TMEM loads are warp-collective
-        if (!good) break;
-        tc_fence_after();
-        const uint32_t t0 = t_row + buf * 256 + (Cfg::kGate ? wg * 64 : wg * 128);
-        // columns 0..63 and 64..127 of this warp: gate tiles have the up columns 128 further on
-        const uint32_t t1 = Cfg::kGate ? t0 + 128 : t0 + 64;
-        const float2 sg = make_float2(s0 * g0, s0 * g0), sh = make_float2(s0 * h0, s0 * h0);
-        uint32_t ra[32], rb[32];
-        auto add = [&](uint32_t(&r)[32], int base, float2 s) {
+      uint32_t ra[32], rb[32];
+      auto ready = [&](int g) {  // the product of K block g is in TMEM; the loads are warp-collective
+        const bool got = mbar_wait(&kfull_bar[g & 1], (g >> 1) & 1, s_abort);
+        return __all_sync(0xffffffffu, got) != 0;
+      };
+      auto add = [&](uint32_t(&r)[32], int base, float s) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j)
-            acc[base + j] = fma2(make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), s, acc[base + j]);
-        };
-        tmem_ld32(t0, ra);
+        for (int j = 0; j < 16; ++j)
+          acc[base + j] = fma2(make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), make_float2(s, s),
+                               acc[base + j]);
+      };
+      bool good = ready(gkb);
+      if (good) {
+        tc_fence_after();
+        tmem_ld32(t_row + (gkb & 1) * 256 + run0, ra);
+      }
+      for (int kb = w.kb0; kb < w.kb1 && good; ++kb, ++gkb) {
+        const int j = (kb - w.kb0) % SG, slot = gs % NS;
+        if (j == 0) {
+          const bool got = mbar_wait(&sfull_bar[slot], (gs / NS) & 1, s_abort);
+          good = __all_sync(0xffffffffu, got) != 0;
+        }
+        const float* xs = s_scale + (slot * SG + j) * RS;
+        const float s0 = xs[lrow] * xs[wsel], s1 = Cfg::kGate ? xs[lrow] * xs[129] : s0;
+        const int buf = gkb & 1;
+        const uint32_t t0 = t_row + buf * 256;
         tmem_ld_wait(ra);
-        tmem_ld32(t0 + 32, rb);
-        add(ra, 0, sg);
+        tmem_ld32(t0 + run0 + 32, rb);
+        add(ra, 0, s0);
         tmem_ld_wait(rb);
-        tmem_ld32(t1, ra);
-        add(rb, 16, sg);
+        tmem_ld32(t0 + run1, ra);
+        add(rb, 16, s0);
         tmem_ld_wait(ra);
-        tmem_ld32(t1 + 32, rb);
-        add(ra, 32, sh);
+        tmem_ld32(t0 + run1 + 32, rb);
+        add(ra, 32, s1);
         tmem_ld_wait(rb);
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(kempty0 + buf * 8);
-        add(rb, 48, sh);
-        s0 = s1; g0 = g1; h0 = h1;
-        s1 = s2; g1 = g2; h1 = h2;
+        if (lane == 0) {
+          if constexpr (Cfg::kPair)
+            mbar_arrive_cluster(kempty0 + buf * 8);
+          else
+            mbar_arrive(&kempty_bar[buf]);
+          if (j == SG - 1 || kb + 1 == w.kb1) mbar_arrive(&sempty_bar[slot]);
+        }
+        if (j == SG - 1 || kb + 1 == w.kb1) ++gs;
+        if (kb + 1 < w.kb1) {
+          good = good && ready(gkb + 1);
+          if (good) {
+            tc_fence_after();
+            tmem_ld32(t_row + (buf ^ 1) * 256 + run0, ra);
+          }
+        }
+        add(rb, 48, s1);
       }
       if constexpr (Cfg::kGate) {
-        // one decision for the eight warps: they meet for the groups' largest values
+        // one decision for the epilogue warps: they meet for the groups' largest values
         if (named_bar_red_or(1, 32 * Cfg::EPI_WARPS, good ? 0 : 1)) break;
+        const int row = row0 + lane;
         float* a = reinterpret_cast<float*>(acc);  // [0, 64) gate, [64, 128) up
         float m = 0.f;
         with_gate(p.gate, [&](auto fn) {
@@ -284,36 +375,26 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
         m = fmaxf(m, s_amax[(wg ^ 1) * 128 + lrow]);
         named_bar_sync(1, 32 * Cfg::EPI_WARPS);
         const float s = m > 0.f ? m / 448.0f : 1.0f;
-        if (row_ok) {
-          const int col = w.tn * 128 + wg * 64;
+        uint4 pk[4];
 #pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            if (col + g * 16 < p.N) {
-              uint32_t pk[4];
+        for (int g = 0; g < 4; ++g) {
+          uint32_t c[4];
 #pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float* v = a + g * 16 + i * 4;
-                pk[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[0] / s, v[1] / s), __NV_SATFINITE, __NV_E4M3) |
-                        ((uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[2] / s, v[3] / s), __NV_SATFINITE, __NV_E4M3)
-                         << 16);
-              }
-              *reinterpret_cast<uint4*>(p.codes + (size_t)row * p.N + col + g * 16) =
-                  make_uint4(pk[0], pk[1], pk[2], pk[3]);
-            }
+          for (int i = 0; i < 4; ++i) {
+            const float* v = a + g * 16 + i * 4;
+            c[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[0] / s, v[1] / s), __NV_SATFINITE, __NV_E4M3) |
+                   ((uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[2] / s, v[3] / s), __NV_SATFINITE, __NV_E4M3) << 16);
           }
-          if (wg == 0) p.scales[(size_t)row * p.tiles_n + w.tn] = s;
+          pk[g] = make_uint4(c[0], c[1], c[2], c[3]);
         }
+        store_warp<16>(wt, pk, p.codes, row0, p.M, w.tn * 128 + wg * 64, p.N);
+        if (wg == 0 && row < p.M) p.scales[(size_t)row * p.tiles_n + w.tn] = s;
       } else {
         if (!good) break;
-        if (row_ok) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int col = w.tn * 256 + wg * 128 + c * 32;
-            if (p.splits > 1)
-              fp8_block_store32(p, p.ws + (size_t)w.split * p.M * p.N, kOutFP32, (size_t)row * p.N, col, acc + c * 16);
-            else
-              fp8_block_store32(p, p.C, p.out_type, (size_t)row * p.N, col, acc + c * 16);
-          }
+        for (int c = 0; c < 4; ++c) {
+          const int col = w.tn * 256 + wg * 128 + c * 32;
+          fp8_block_store32(p, wt, w.split, row0, col, acc + c * 16);
         }
       }
     }
@@ -321,10 +402,10 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
 
   tc_fence_before();
   __syncthreads();
-  cluster_sync();  // no CTA leaves while its peer may still signal it
+  if constexpr (Cfg::kPair) cluster_sync();  // no CTA leaves while its peer may still signal it
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc<2>(tmem_base, 512);
+    tmem_dealloc<Cfg::CTAS>(tmem_base, 512);
   }
 }
 

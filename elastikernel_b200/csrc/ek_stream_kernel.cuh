@@ -47,7 +47,7 @@ struct StreamCfg {
   static constexpr int EPI_WARPS = 8;
   static constexpr int THREADS = 96 + 32 * EPI_WARPS;
   static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + SCALE_BYTES + 512 + 1024;
-  static constexpr uint32_t IDESC = umma_idesc(kElem == kBF16 ? 1u : 0u, false, 128, NT);
+  static constexpr uint32_t IDESC = umma_idesc(kElem == kBF16 ? 1u : 0u, false, 128, 0);  // N is the launch's
   static constexpr int CHUNK = NT < 32 || (kF8 && NT == 128) ? 16 : 32;  // 128 accumulators leave room for 16
   static_assert(NT == 16 || NT == 32 || NT == 64 || NT == 128, "token tile");
 };
@@ -62,6 +62,7 @@ struct StreamSplit {
 struct StreamParams {
   StreamSplit sp;
   int T;
+  int n;                   // tokens per MMA: T rounded up to 16 (the box's rows)
   const float* tok_scale;  // e4m3: [T][k_blocks]
   const float* w_scale;    // [rows / 128][k_blocks]; gate: W1's
   const float* w_scale2;   // gate: W3's
@@ -127,7 +128,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
       auto load_w = [&](int u, int stage) {
         const int tile = u / KB, k0 = (u - tile * KB) * Cfg::BK;
         uint8_t* dst = smem + stage * Cfg::STAGE_BYTES;
-        mbar_arrive_expect_tx(&full_bar[stage], Cfg::STAGE_BYTES);
+        mbar_arrive_expect_tx(&full_bar[stage], Cfg::A_BYTES + p.n * 128);
         if constexpr (Cfg::kGate) {
           tma_load_2d(dst, &tmW, &full_bar[stage], k0, tile * 128);
           tma_load_2d(dst + 128 * 128, &tmW2, &full_bar[stage], k0, tile * 128);
@@ -157,37 +158,40 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
-      int stage = 0, flush = 0;
-      uint32_t phase = 0;
-      bool fresh = true;  // the next MMA starts a sum
-      for (int u = u0; u < u1; ++u) {
-        const int buf = flush & 1;
-        if (fresh && !mbar_wait(&tempty_bar[buf], ((flush >> 1) & 1) ^ 1, s_abort)) break;
-        if (!mbar_wait(&full_bar[stage], phase, s_abort)) break;
-        tc_fence_after();
-        const uint32_t a0 = smem_u32(smem + stage * Cfg::STAGE_BYTES), b0 = a0 + Cfg::A_BYTES;
-        const uint32_t d = tmem_base + buf * 2 * NT;
+    int stage = 0, flush = 0;
+    uint32_t phase = 0;
+    bool fresh = true;  // the next MMA starts a sum
+    const uint32_t idesc = Cfg::IDESC | ((uint32_t)(p.n >> 3) << 17);
+    const uint64_t a_desc = umma_desc_sw128(smem_u32(smem), 16, 1024);
+    const uint64_t b_desc = umma_desc_sw128(smem_u32(smem) + Cfg::A_BYTES, 16, 1024);
+    for (int u = u0; u < u1; ++u) {
+      const int buf = flush & 1;
+      bool ok = !fresh || mbar_wait(&tempty_bar[buf], ((flush >> 1) & 1) ^ 1, s_abort);
+      ok = ok && mbar_wait(&full_bar[stage], phase, s_abort);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      tc_fence_after();
+      const uint32_t off = stage * (Cfg::STAGE_BYTES >> 4);
+      const uint32_t d = tmem_base + buf * 2 * NT;
+      const bool last = Cfg::kF8 || (u + 1) % KB == 0 || u + 1 == u1;
+      if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < Cfg::KSTEPS; ++k) {
-          const uint64_t bd = umma_desc_sw128(b0 + k * 32, 16, 1024);
+        for (int k = 0; k < Cfg::KSTEPS; ++k)
 #pragma unroll
           for (int h = 0; h < 2; ++h)
-            umma<Cfg::kF8>(d + h * NT, umma_desc_sw128(a0 + h * (128 * 128) + k * 32, 16, 1024), bd, Cfg::IDESC,
+            umma<Cfg::kF8>(d + h * NT, a_desc + off + h * (128 * 128 >> 4) + 2 * k, b_desc + off + 2 * k, idesc,
                            (!fresh || k > 0) ? 1u : 0u);
-        }
         umma_commit(&empty_bar[stage]);
-        if (++stage == STAGES) { stage = 0; phase ^= 1; }
-        fresh = Cfg::kF8 || (u + 1) % KB == 0 || u + 1 == u1;
-        if (fresh) {
-          umma_commit(&tfull_bar[buf]);
-          ++flush;
-        }
+        if (last) umma_commit(&tfull_bar[buf]);
       }
-      umma_commit(drain_bar);  // every MMA has completed before TMEM is freed
-      volatile int never = 0;
-      mbar_wait(drain_bar, 0, &never);
+      __syncwarp();
+      if (++stage == STAGES) { stage = 0; phase ^= 1; }
+      fresh = last;
+      flush += last;
     }
+    if (elect_one()) umma_commit(drain_bar);  // every MMA has completed before TMEM is freed
+    __syncwarp();
+    volatile int never = 0;
+    mbar_wait(drain_bar, 0, &never);
     __syncwarp();
   } else if (warp == 2) {
     if constexpr (Cfg::kF8) {
@@ -241,6 +245,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
           const float ws = xs[NT + rb];
 #pragma unroll
           for (int c = 0; c < NT / CH; ++c) {
+            if (c * CH >= p.n) break;
             uint32_t r[32];
             if constexpr (CH == 32)
               tmem_ld32(lane_base + buf * 2 * NT + c * CH, r);
@@ -274,15 +279,16 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
         good = mbar_wait(&tfull_bar[buf], (flush >> 1) & 1, s_abort);
         if (!__all_sync(0xffffffffu, good)) break;
         tc_fence_after();
+        const int chunks = (p.n + CH - 1) / CH;
 #pragma unroll 1
-        for (int c = 0; c < NT / CH; ++c) {
+        for (int c = 0; c < chunks; ++c) {
           uint32_t r[32];
           if constexpr (CH == 32)
             tmem_ld32(lane_base + buf * 2 * NT + c * CH, r);
           else
             tmem_ld16(lane_base + buf * 2 * NT + c * CH, r);
           tmem_ld_wait(r);
-          if (c == NT / CH - 1) release(buf);
+          if (c == chunks - 1) release(buf);
 #pragma unroll
           for (int j = 0; j < CH; ++j)
             if (c * CH + j < p.T) __stcg(out + (size_t)(c * CH + j) * 256, __uint_as_float(r[j]));
@@ -303,34 +309,6 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
 }
 
 // ------------------------------------------------------------ adding the segments
-// Sum over the segments of `tile`, in K order, of row r (and r2) of token t.
-template <int kN>
-__device__ __forceinline__ void stream_sum(const StreamSplit& sp, const float* __restrict__ ws, int T, int tile, int t,
-                                           const int (&r)[kN], float (&v)[kN]) {
-#pragma unroll
-  for (int i = 0; i < kN; ++i) v[i] = 0.f;
-  const int c0 = (int)((long long)tile * sp.k_blocks / sp.per_cta);
-  const int c1 = (int)(((long long)(tile + 1) * sp.k_blocks - 1) / sp.per_cta);
-  constexpr int U = 4;  // segments with their loads in flight
-  for (int c = c0; c <= c1; c += U) {
-    float x[U][kN];
-#pragma unroll
-    for (int j = 0; j < U; ++j) {
-      if (c + j > c1) break;
-      const int seg = tile - (int)((long long)(c + j) * sp.per_cta / sp.k_blocks);
-      const float* src = ws + ((size_t)((c + j) * sp.max_segs + seg) * T + t) * 256;
-#pragma unroll
-      for (int i = 0; i < kN; ++i) x[j][i] = __ldcg(src + r[i]);
-    }
-#pragma unroll
-    for (int j = 0; j < U; ++j) {
-      if (c + j > c1) break;
-#pragma unroll
-      for (int i = 0; i < kN; ++i) v[i] += x[j][i];
-    }
-  }
-}
-
 enum OutType : int { kOutBF16 = 0, kOutFP16 = 1, kOutFP32 = 3 };
 
 __device__ __forceinline__ void store_out(void* out, int type, size_t at, float v) {
@@ -342,54 +320,132 @@ __device__ __forceinline__ void store_out(void* out, int type, size_t at, float 
     reinterpret_cast<float*>(out)[at] = v;
 }
 
-// out[t, n] of a plain product; a block per (tile, token), a thread per row
-__global__ void __launch_bounds__(256) stream_store_reduce_kernel(const StreamSplit sp, const float* __restrict__ ws,
-                                                                  int T, int N, void* __restrict__ out, int type) {
-  pdl_launch();
-  pdl_wait();
-  const int tile = blockIdx.x, t = blockIdx.y, n = tile * 256 + threadIdx.x;
-  if (n >= N) return;
-  const int r[1] = {(int)threadIdx.x};
-  float v[1];
-  stream_sum<1>(sp, ws, T, tile, t, r, v);
-  store_out(out, type, (size_t)t * N + n, v[0]);
-}
-
-// a[t, f] = f(h1) h3 of the gate/up pair, h1 and h3 on request; a block per
-// (tile, token), a thread per feature. codes != null: a in e4m3 with the scale of
-// the block's 128 features (largest magnitude / 448, 1 for zeros) instead.
-__global__ void __launch_bounds__(128)
-    stream_gate_reduce_kernel(const StreamSplit sp, const float* __restrict__ ws, int T, int I, int gate, int type,
-                              void* __restrict__ a, void* __restrict__ h, uint8_t* __restrict__ codes,
-                              float* __restrict__ scales) {
-  pdl_launch();
-  pdl_wait();
-  const int tile = blockIdx.x, t = blockIdx.y, f = tile * 128 + threadIdx.x;
-  const int r[2] = {(int)threadIdx.x, 128 + (int)threadIdx.x};
-  float v[2];
-  stream_sum<2>(sp, ws, T, tile, t, r, v);  // rows past I hold zeros
-  float act;
-  with_gate(gate, [&](auto fn) { act = gate_f<decltype(fn)::value>(v[0]) * v[1]; });
-  const size_t at = (size_t)t * I + f;
-  if (codes == nullptr) {
-    if (f >= I) return;
-    store_out(a, type, at, act);
-    if (h != nullptr) {
-      store_out(h, type, at, v[0]);
-      store_out(h, type, (size_t)T * I + at, v[1]);
+// 4 consecutive values, `n` of them inside the row; wide: whole and aligned
+__device__ __forceinline__ void store_out4(void* out, int type, size_t at, const float4& v, int n, bool wide) {
+  if (wide && n >= 4) {
+    if (type == kOutFP32) {
+      *reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + at) = v;
+    } else {
+      uint2 pk;
+      pk.x = type == kOutBF16 ? Elem16<kBF16>::pack(v.x, v.y) : Elem16<kFP16>::pack(v.x, v.y);
+      pk.y = type == kOutBF16 ? Elem16<kBF16>::pack(v.z, v.w) : Elem16<kFP16>::pack(v.z, v.w);
+      *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(out) + at) = pk;
     }
     return;
   }
-  __shared__ float s_max[4];
-  float m = f < I ? fabsf(act) : 0.f;
+  const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (i < n) store_out(out, type, at + i, e[i]);
+}
+
+__device__ __forceinline__ void add4(float4& a, const float4& b) {
+  a.x += b.x;
+  a.y += b.y;
+  a.z += b.z;
+  a.w += b.w;
+}
+
+// A warp of a block of 8 sums 128 rows of a tile for one token, four rows a lane
+// (kN = 2: a second 128 rows beside them, the up rows of a gate tile). `ways` warps
+// share a token's segments, each taking every ways-th; their sums are added in
+// order by the first of them. So the block covers 8 / ways tokens, and a tile cut
+// into many segments has all its loads in flight at once. Returns whether this warp
+// holds the result.
+template <int kN>
+__device__ __forceinline__ bool stream_sum(const StreamSplit& sp, const float* __restrict__ ws, int T, int tile, int t,
+                                           int row, int ways, float4 (&v)[kN]) {
+  __shared__ float4 s_part[8][32][kN];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, way = warp % ways;
+#pragma unroll
+  for (int i = 0; i < kN; ++i) v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (t < T) {
+    const int c0 = (int)((long long)tile * sp.k_blocks / sp.per_cta);
+    const int c1 = (int)(((long long)(tile + 1) * sp.k_blocks - 1) / sp.per_cta);
+    constexpr int U = 4;  // segments with their loads in flight
+    for (int c = c0 + way; c <= c1; c += U * ways) {
+      float4 x[U][kN];
+#pragma unroll
+      for (int j = 0; j < U; ++j) {
+        const int cj = c + j * ways;
+        if (cj <= c1) {
+          const int seg = tile - (int)((long long)cj * sp.per_cta / sp.k_blocks);
+          const float* src = ws + ((size_t)(cj * sp.max_segs + seg) * T + t) * 256 + row + lane * 4;
+#pragma unroll
+          for (int i = 0; i < kN; ++i) x[j][i] = __ldcg(reinterpret_cast<const float4*>(src + i * 128));
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < U; ++j)
+        if (c + j * ways <= c1) {
+#pragma unroll
+          for (int i = 0; i < kN; ++i) add4(v[i], x[j][i]);
+        }
+    }
+  }
+  if (ways > 1) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) s_part[warp][lane][i] = v[i];
+    __syncthreads();
+    if (way == 0)
+      for (int w = 1; w < ways; ++w)
+#pragma unroll
+        for (int i = 0; i < kN; ++i) add4(v[i], s_part[warp + w][lane][i]);
+  }
+  return way == 0 && t < T;
+}
+
+// out[t, n] of a plain product; blockIdx.x: half tiles of 128 rows
+__global__ void __launch_bounds__(256) stream_store_reduce_kernel(const StreamSplit sp, const float* __restrict__ ws,
+                                                                  int T, int N, void* __restrict__ out, int type,
+                                                                  int wide, int ways) {
+  pdl_launch();
+  pdl_wait();
+  const int tile = blockIdx.x >> 1, row = (blockIdx.x & 1) * 128;
+  const int t = blockIdx.y * (8 / ways) + (threadIdx.x >> 5) / ways;
+  const int n = tile * 256 + row + (threadIdx.x & 31) * 4;
+  float4 v[1];
+  if (stream_sum<1>(sp, ws, T, tile, t, row, ways, v)) store_out4(out, type, (size_t)t * N + n, v[0], N - n, wide);
+}
+
+// a[t, f] = f(h1) h3 of the gate/up pair, h1 and h3 on request. codes != null: a in
+// e4m3 with the scale of the warp's 128 features (largest magnitude / 448, 1 for
+// zeros) instead. I is a multiple of 4.
+__global__ void __launch_bounds__(256)
+    stream_gate_reduce_kernel(const StreamSplit sp, const float* __restrict__ ws, int T, int I, int gate, int type,
+                              void* __restrict__ a, void* __restrict__ h, uint8_t* __restrict__ codes,
+                              float* __restrict__ scales, int ways) {
+  pdl_launch();
+  pdl_wait();
+  const int tile = blockIdx.x, t = blockIdx.y * (8 / ways) + (threadIdx.x >> 5) / ways;
+  const int f = tile * 128 + (threadIdx.x & 31) * 4;
+  float4 v[2];
+  if (!stream_sum<2>(sp, ws, T, tile, t, 0, ways, v)) return;  // rows past I hold zeros
+  float4 act;
+  with_gate(gate, [&](auto fn) {
+    constexpr int F = decltype(fn)::value;
+    act = make_float4(gate_f<F>(v[0].x) * v[1].x, gate_f<F>(v[0].y) * v[1].y, gate_f<F>(v[0].z) * v[1].z,
+                      gate_f<F>(v[0].w) * v[1].w);
+  });
+  const size_t at = (size_t)t * I + f;
+  if (codes == nullptr) {
+    store_out4(a, type, at, act, I - f, true);
+    if (h != nullptr) {
+      store_out4(h, type, at, v[0], I - f, true);
+      store_out4(h, type, (size_t)T * I + at, v[1], I - f, true);
+    }
+    return;
+  }
+  float m = fmaxf(fmaxf(fabsf(act.x), fabsf(act.y)), fmaxf(fabsf(act.z), fabsf(act.w)));  // zeros past I
 #pragma unroll
   for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if ((threadIdx.x & 31) == 0) s_max[threadIdx.x >> 5] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
   const float s = m > 0.f ? m / 448.0f : 1.0f;
-  if (f < I) codes[at] = static_cast<uint8_t>(__nv_cvt_float_to_fp8(act / s, __NV_SATFINITE, __NV_E4M3));
-  if (threadIdx.x == 0) scales[(size_t)t * ((I + 127) / 128) + tile] = s;
+  if (f < I) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(act.x / s, act.y / s), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(act.z / s, act.w / s), __NV_SATFINITE, __NV_E4M3);
+    *reinterpret_cast<uint32_t*>(codes + at) = lo | (hi << 16);
+  }
+  if ((threadIdx.x & 31) == 0) scales[(size_t)t * ((I + 127) / 128) + tile] = s;
 }
 
 }  // namespace ek
