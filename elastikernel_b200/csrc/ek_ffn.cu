@@ -402,6 +402,7 @@ int launch_fp8(const void* a, const void* w, const void* w2, int K, Fp8BlockPara
   const long long units = (long long)p.tiles_m * p.tiles_n * p.splits;
   if (units > 0x3fffffff) return set_error(EK_ERR_INVALID, "too many tiles");
   p.num_units = (int)units;
+  p.scale4 = p.k_blocks % 4 == 0 && aligned16(p.a_scale) && aligned16(p.w_scale) && aligned16(p.w_scale2);
   const int groups = (int)std::min<long long>(std::max(1, sms / Cfg::CTAS), units);
   return launch("block-scaled product", fp8_block_kernel<Cfg>, dim3(Cfg::CTAS * groups), Cfg::THREADS, Cfg::SMEM_BYTES, s,
                 kFp8Pair ? 2 : 0, false, ta, tb, tb2, p);

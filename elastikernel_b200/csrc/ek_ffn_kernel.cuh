@@ -47,6 +47,29 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
+// Whether the phase has completed, without waiting for it.
+__device__ __forceinline__ bool mbar_test(uint32_t bar_addr, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar_addr), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+
+// mbar_wait for a phase that is expected within a microsecond or so: the clock is read
+// only when it has not come by then.
+__device__ __forceinline__ bool mbar_wait_soon(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  const uint32_t a = smem_u32(bar);
+#pragma unroll 1
+  for (int i = 0; i < 64; ++i)
+    if (mbar_try_wait(a, parity)) return true;
+  return mbar_wait(bar, parity, abort_flag);
+}
+
 enum FfnEpi : int { kFfnStore = 0, kFfnGate = 1, kFfnGateGrad = 2 };
 
 template <int kElem_, bool kAMN_, bool kBMN_, int kEpi_>

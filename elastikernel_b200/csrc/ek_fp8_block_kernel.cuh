@@ -10,7 +10,7 @@
 // epilogue warps read the product, multiply it by its one scale per row and weight
 // block and add it to fp32 accumulators in registers.
 //
-//   warp 0  TMA producer; warp 1  TMEM and MMA; warp 2  scales; warp 3  idle
+//   warp 0  TMA producer; warp 1  TMEM and MMA; warps 2, 3  idle
 //   warps 4..11  epilogue, two per TMEM lane quarter, 128 accumulators a thread: group
 //   g has of a plain tile the columns [128 g, +128), of a gate tile 64 gate columns
 //   and the same features' 64 up columns. setmaxnreg gives them the registers that
@@ -31,12 +31,8 @@ struct Fp8BlockCfg {
   static constexpr int THREADS = 128 + 32 * EPI_WARPS;
   // 384 threads are launched with 168 registers each: 128 x 56 + 256 x 224 = 64512 = 384 x 168
   static constexpr int REGS_LOAD = 56, REGS_EPI = 224;
-  static constexpr uint32_t IDESC = umma_idesc(0u, false, 128 * CTAS, 256);
-  // Scales: slots of SGROUP K blocks, each 128 rows' and the two weight blocks' scales
-  static constexpr int SGROUP = 4, SLOTS = 3, SLOT_STRIDE = 132;
-  static constexpr int SCALE_BYTES = SLOTS * SGROUP * SLOT_STRIDE * 4;
-  static constexpr int SMEM_BYTES =
-      STAGES * STAGE_BYTES + EPI_WARPS * 2048 + 1024 /*largest values*/ + SCALE_BYTES + 256 + 1024;
+  static constexpr uint32_t IDESC = umma_idesc(0u, false, 128 * CTAS, 128);
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_WARPS * 2048 + 1024 /*largest values*/ + 256 + 1024;
 };
 
 struct Fp8BlockParams {
@@ -46,6 +42,7 @@ struct Fp8BlockParams {
   const float* w_scale;   // [w_blocks][k_blocks]; gate: W1's
   const float* w_scale2;  // gate: W3's
   int w_blocks;
+  int scale4;            // rows of scales are a multiple of 16 bytes
   void* C;               // plain result
   int out_type;          // OutType
   int wide;              // rows of C are a multiple of 16 bytes
@@ -106,19 +103,16 @@ template <class Cfg>
 __global__ void __launch_bounds__(Cfg::THREADS, 1)
     fp8_block_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                      const __grid_constant__ CUtensorMap tmB2, const Fp8BlockParams p) {
-  constexpr int STAGES = Cfg::STAGES, HB = Cfg::HALF_BYTES, NS = Cfg::SLOTS, SG = Cfg::SGROUP, RS = Cfg::SLOT_STRIDE;
+  constexpr int STAGES = Cfg::STAGES, HB = Cfg::HALF_BYTES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* s_tile = smem + STAGES * Cfg::STAGE_BYTES;                           // [EPI_WARPS] of 2 KB
   float* s_amax = reinterpret_cast<float*>(s_tile + Cfg::EPI_WARPS * 2048);     // [2][128]
-  float* s_scale = s_amax + 256;                                                // [SLOTS][SGROUP][SLOT_STRIDE]
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(s_scale + NS * SG * RS);
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(s_amax + 256);
   uint64_t* empty_bar = full_bar + STAGES;
   uint64_t* kfull_bar = empty_bar + STAGES;
-  uint64_t* kempty_bar = kfull_bar + 2;
-  uint64_t* sfull_bar = kempty_bar + 2;
-  uint64_t* sempty_bar = sfull_bar + NS;
-  uint64_t* drain_bar = sempty_bar + NS;
+  uint64_t* kempty_bar = kfull_bar + 4;  // both [half][buffer]
+  uint64_t* drain_bar = kempty_bar + 4;
   uint32_t* s_tmem_base = reinterpret_cast<uint32_t*>(drain_bar + 1);
   volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem_base + 1);
 
@@ -134,13 +128,9 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
       mbar_init(&full_bar[s], 1);
       mbar_init(&empty_bar[s], 1);
     }
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < 4; ++b) {
       mbar_init(&kfull_bar[b], 1);
-      mbar_init(&kempty_bar[b], Cfg::EPI_WARPS * Cfg::CTAS);
-    }
-    for (int s = 0; s < NS; ++s) {
-      mbar_init(&sfull_bar[s], 32);
-      mbar_init(&sempty_bar[s], Cfg::EPI_WARPS);
+      mbar_init(&kempty_bar[b], Cfg::EPI_WARPS / 2 * Cfg::CTAS);
     }
     mbar_init(drain_bar, 1);
     *s_abort = 0;
@@ -214,28 +204,35 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
         const U w = unit(u);
         for (int kb = w.kb0; kb < w.kb1; ++kb, ++gkb) {
           const int buf = gkb & 1;
-          ok = mbar_wait(&full_bar[stage], phase, s_abort) && mbar_wait(&kempty_bar[buf], ((gkb >> 1) & 1) ^ 1, s_abort);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          tc_fence_after();
+          ok = mbar_wait(&full_bar[stage], phase, s_abort);
           const uint32_t off = stage * (Cfg::STAGE_BYTES >> 4);
-          if (elect_one()) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              if constexpr (Cfg::kPair)
-                umma_pair<true>(tmem_base + buf * 256, a_desc + off + 2 * k, b_desc + off + 2 * k, Cfg::IDESC, k > 0);
-              else
-                umma<true>(tmem_base + buf * 256, a_desc + off + 2 * k, b_desc + off + 2 * k, Cfg::IDESC, k > 0);
+          for (int h = 0; h < 2; ++h) {
+            ok = ok && mbar_wait(&kempty_bar[2 * h + buf], ((gkb >> 1) & 1) ^ 1, s_abort);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc_fence_after();
+            if (elect_one()) {
+              // half h: rows [64 h, 64 h + 64) of each CTA's 128 weight rows (one CTA: [128 h, 128 h + 128) of 256)
+              const uint32_t d = tmem_base + h * 256 + buf * 128, boff = off + h * (128 / Cfg::CTAS * 128 >> 4);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                if constexpr (Cfg::kPair)
+                  umma_pair<true>(d, a_desc + off + 2 * k, b_desc + boff + 2 * k, Cfg::IDESC, k > 0);
+                else
+                  umma<true>(d, a_desc + off + 2 * k, b_desc + boff + 2 * k, Cfg::IDESC, k > 0);
+              }
+              if constexpr (Cfg::kPair) {
+                umma_commit_pair(&kfull_bar[2 * h + buf], 0x3);
+                if (h == 1) umma_commit_pair(&empty_bar[stage], 0x3);
+              } else {
+                umma_commit(&kfull_bar[2 * h + buf]);
+                if (h == 1) umma_commit(&empty_bar[stage]);
+              }
             }
-            if constexpr (Cfg::kPair) {
-              umma_commit_pair(&kfull_bar[buf], 0x3);
-              umma_commit_pair(&empty_bar[stage], 0x3);
-            } else {
-              umma_commit(&kfull_bar[buf]);
-              umma_commit(&empty_bar[stage]);
-            }
+            __syncwarp();
           }
-          __syncwarp();
+          if (!ok) break;
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
       }
@@ -251,38 +248,6 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
     } else if (warp == 1) {
       volatile int never = 0;
       mbar_wait(drain_bar, 0, &never);
-    } else if (warp == 2) {
-      // scales by asynchronous copies that run ahead of the epilogue, SGROUP K blocks a slot:
-      // fetched in the epilogue's own loop, their latency bounded every K block
-      int g = 0;
-      bool ok = true;
-      for (int u = unit0; u < p.num_units && ok; u += unit_step) {
-        const U w = unit(u);
-        const int row = (w.tm * Cfg::CTAS + rank) * 128 + lane * 4;
-        for (int kb = w.kb0; kb < w.kb1; kb += SG, ++g) {
-          const int slot = g % NS;
-          ok = mbar_wait(&sempty_bar[slot], ((g / NS) & 1) ^ 1, s_abort);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          const int n = min(SG, w.kb1 - kb);
-          for (int j = 0; j < n; ++j) {
-            float* dst = s_scale + (slot * SG + j) * RS;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const bool in = row + i < p.M;
-              cp_async_4_zfill(dst + lane * 4 + i, p.a_scale + (in ? (size_t)(row + i) * KB + kb + j : 0), in ? 4 : 0);
-            }
-            if (lane < 2) {
-              const int blk = Cfg::kGate ? w.tn : 2 * w.tn + lane;
-              const float* src = Cfg::kGate && lane ? p.w_scale2 : p.w_scale;
-              const bool in = blk < p.w_blocks;
-              cp_async_4_zfill(dst + 128 + lane, src + (in ? (size_t)blk * KB + kb + j : 0), in ? 4 : 0);
-            }
-          }
-          cp_async_mbar_arrive(&sfull_bar[slot]);
-        }
-      }
-      cp_async_wait<0>();  // no copy into shared memory outlives the CTA
     }
     __syncwarp();
   } else {
@@ -290,12 +255,10 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
     const int q = warp & 3, wg = (warp - 4) >> 2;
     const int lrow = q * 32 + lane;
     const WarpTile wt{s_tile + (warp - 4) * 2048, lane};
-    const uint32_t kempty0 = Cfg::kPair ? mapa_shared(smem_u32(&kempty_bar[0]), 0) : 0;
-    // this thread's accumulators as columns of the tile: 64 from run0 on, 64 from run1 on
-    const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
-    const uint32_t run0 = Cfg::kGate ? wg * 64 : wg * 128, run1 = Cfg::kGate ? 128 + wg * 64 : wg * 128 + 64;
-    const int wsel = 128 + (Cfg::kGate ? 0 : wg);
-    int gkb = 0, gs = 0;  // K blocks, scale slots
+    const uint32_t kempty0 = Cfg::kPair ? mapa_shared(smem_u32(&kempty_bar[2 * wg]), 0) : 0;
+    // group g reads half g: 64 columns of the first weight block (gate), 64 of the second (up)
+    const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + wg * 256;
+    int gkb = 0;
     for (int u = unit0; u < p.num_units; u += unit_step) {
       const U w = unit(u);
       const int row0 = (w.tm * Cfg::CTAS + rank) * 128 + q * 32;
@@ -303,64 +266,96 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
 #pragma unroll
       for (int j = 0; j < 64; ++j) acc[j] = make_float2(0.f, 0.f);
       uint32_t ra[32], rb[32];
-      auto ready = [&](int g) {  // the product of K block g is in TMEM; the loads are warp-collective
-        const bool got = mbar_wait(&kfull_bar[g & 1], (g >> 1) & 1, s_abort);
-        return __all_sync(0xffffffffu, got) != 0;
-      };
       auto add = [&](uint32_t(&r)[32], int base, float s) {
 #pragma unroll
         for (int j = 0; j < 16; ++j)
           acc[base + j] = fma2(make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), make_float2(s, s),
                                acc[base + j]);
       };
-      bool good = ready(gkb);
-      if (good) {
-        tc_fence_after();
-        tmem_ld32(t_row + (gkb & 1) * 256 + run0, ra);
-      }
-      for (int kb = w.kb0; kb < w.kb1 && good; ++kb, ++gkb) {
-        const int j = (kb - w.kb0) % SG, slot = gs % NS;
-        if (j == 0) {
-          const bool got = mbar_wait(&sfull_bar[slot], (gs / NS) & 1, s_abort);
-          good = __all_sync(0xffffffffu, got) != 0;
-        }
-        const float* xs = s_scale + (slot * SG + j) * RS;
-        const float s0 = xs[lrow] * xs[wsel], s1 = Cfg::kGate ? xs[lrow] * xs[129] : s0;
-        const int buf = gkb & 1;
-        const uint32_t t0 = t_row + buf * 256;
-        tmem_ld_wait(ra);
-        tmem_ld32(t0 + run0 + 32, rb);
-        add(ra, 0, s0);
-        tmem_ld_wait(rb);
-        tmem_ld32(t0 + run1, ra);
-        add(rb, 16, s0);
-        tmem_ld_wait(ra);
-        tmem_ld32(t0 + run1 + 32, rb);
-        add(ra, 32, s1);
-        tmem_ld_wait(rb);
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) {
-          if constexpr (Cfg::kPair)
-            mbar_arrive_cluster(kempty0 + buf * 8);
-          else
-            mbar_arrive(&kempty_bar[buf]);
-          if (j == SG - 1 || kb + 1 == w.kb1) mbar_arrive(&sempty_bar[slot]);
-        }
-        if (j == SG - 1 || kb + 1 == w.kb1) ++gs;
-        if (kb + 1 < w.kb1) {
-          good = good && ready(gkb + 1);
-          if (good) {
-            tc_fence_after();
-            tmem_ld32(t_row + (buf ^ 1) * 256 + run0, ra);
+      // The scales of four K blocks at a time, fetched four blocks ahead
+      const int row = row0 + lane;
+      const float* sa = p.a_scale + (size_t)(row < p.M ? row : 0) * KB;
+      const int blk = Cfg::kGate ? w.tn : 2 * w.tn;
+      const float* sw0 = p.w_scale + (size_t)blk * KB;
+      const float* sw1 = Cfg::kGate ? p.w_scale2 + (size_t)blk * KB
+                                    : p.w_scale + (size_t)(blk + 1 < p.w_blocks ? blk + 1 : blk) * KB;
+      const bool quads = p.scale4 && w.kb0 % 4 == 0;  // a slice of K may begin anywhere
+      float xa[4], xw[4], xv[4];                       // of the next four blocks
+      auto fetch = [&](int kb) {
+        if (quads && kb + 4 <= KB) {
+          const float4 a = __ldg(reinterpret_cast<const float4*>(sa + kb));
+          const float4 b = __ldg(reinterpret_cast<const float4*>(sw0 + kb));
+          const float4 c = __ldg(reinterpret_cast<const float4*>(sw1 + kb));
+          xa[0] = a.x; xa[1] = a.y; xa[2] = a.z; xa[3] = a.w;
+          xw[0] = b.x; xw[1] = b.y; xw[2] = b.z; xw[3] = b.w;
+          xv[0] = c.x; xv[1] = c.y; xv[2] = c.z; xv[3] = c.w;
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int k = min(kb + j, KB - 1);
+            xa[j] = __ldg(sa + k);
+            xw[j] = __ldg(sw0 + k);
+            xv[j] = __ldg(sw1 + k);
           }
         }
-        add(rb, 48, s1);
+      };
+      fetch(w.kb0);
+      // A failed wait has raised the abort flag: the loop then runs out without waiting and
+      // the tile is not stored.
+      mbar_wait_soon(&kfull_bar[2 * wg + (gkb & 1)], (gkb >> 1) & 1, s_abort);
+      __syncwarp();
+      tc_fence_after();
+      tmem_ld32(t_row + (gkb & 1) * 128, ra);
+#pragma unroll 1
+      for (int kb = w.kb0; kb < w.kb1; kb += 4) {
+        float s0[4], s1[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          s0[j] = xa[j] * xw[j];
+          s1[j] = xa[j] * xv[j];
+        }
+        if (kb + 4 < w.kb1) fetch(kb + 4);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (kb + j < w.kb1) {
+            const int buf = gkb & 1, nbuf = buf ^ 1;
+            const bool more = kb + j + 1 < w.kb1;
+            const uint32_t t0 = t_row + buf * 128, nphase = ((gkb + 1) >> 1) & 1;
+            uint64_t* nbar = &kfull_bar[2 * wg + nbuf];
+            tmem_ld_wait(ra);
+            tmem_ld32(t0 + 32, rb);
+            add(ra, 0, s0[j]);
+            tmem_ld_wait(rb);
+            tmem_ld32(t0 + 64, ra);
+            add(rb, 16, s0[j]);
+            tmem_ld_wait(ra);
+            tmem_ld32(t0 + 96, rb);
+            const bool early = more && mbar_test(smem_u32(nbar), nphase);
+            add(ra, 32, s1[j]);
+            tmem_ld_wait(rb);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              if constexpr (Cfg::kPair)
+                mbar_arrive_cluster(kempty0 + buf * 8);
+              else
+                mbar_arrive(&kempty_bar[2 * wg + buf]);
+            }
+            if (more) {
+              if (!early) mbar_wait_soon(nbar, nphase, s_abort);
+              __syncwarp();
+              tc_fence_after();
+              tmem_ld32(t_row + nbuf * 128, ra);
+            }
+            add(rb, 48, s1[j]);
+            ++gkb;
+          }
+        }
       }
+      const bool good = !__any_sync(0xffffffffu, *s_abort);
       if constexpr (Cfg::kGate) {
         // one decision for the epilogue warps: they meet for the groups' largest values
         if (named_bar_red_or(1, 32 * Cfg::EPI_WARPS, good ? 0 : 1)) break;
-        const int row = row0 + lane;
         float* a = reinterpret_cast<float*>(acc);  // [0, 64) gate, [64, 128) up
         float m = 0.f;
         with_gate(p.gate, [&](auto fn) {
@@ -393,7 +388,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
         if (!good) break;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          const int col = w.tn * 256 + wg * 128 + c * 32;
+          const int col = w.tn * 256 + (c >> 1) * 128 + wg * 64 + (c & 1) * 32;
           fp8_block_store32(p, wt, w.split, row0, col, acc + c * 16);
         }
       }
