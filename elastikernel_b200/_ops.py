@@ -1121,7 +1121,7 @@ _MAX_TOKENS = 0x7fffffff
 
 def _check_matrix(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple) -> torch.Tensor:
     """t, checked and 16-byte aligned (a view that starts mid-line is copied)."""
-    if t.dtype is not dtype or tuple(t.shape) != shape:
+    if t.dtype is not dtype or t.shape != shape:
         raise RuntimeError(f"{name} must be a {dtype} tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}")
     if not t.is_contiguous():
         raise RuntimeError(f"{name} must be contiguous")
@@ -1149,9 +1149,10 @@ def gemm_fp8_block(a_q: torch.Tensor, w_q: torch.Tensor, a_scale: torch.Tensor, 
     K is a multiple of 16; M, N and the last block of each axis are any size. The
     sums are fp32; C is bf16, fp16 or fp32 (`dtype`, or out's), rounded once."""
     dev = _require_cuda(a_q, w_q, a_scale, w_scale, out)
-    if _FP8 is None or a_q.dtype != _FP8 or w_q.dtype != _FP8 or a_q.dim() != 2 or w_q.dim() != 2:
+    shape = a_q.shape
+    if _FP8 is None or len(shape) != 2 or w_q.dim() != 2:
         raise RuntimeError("gemm_fp8_block takes 2-D float8_e4m3fn operands")
-    (M, K), N = a_q.shape, w_q.shape[0]
+    (M, K), N = shape, w_q.shape[0]
     if K == 0 or K % 16 or K > _MAX_FFN_DIM or max(M, N) > _MAX_TOKENS:
         raise RuntimeError(f"gemm_fp8_block: K must be a positive multiple of 16 up to 2^28, M and N within 2^31 "
                            f"(got {M} x {N} x {K})")
@@ -1164,26 +1165,27 @@ def gemm_fp8_block(a_q: torch.Tensor, w_q: torch.Tensor, a_scale: torch.Tensor, 
     if dtype not in _ROW_DTYPES:
         raise RuntimeError("gemm_fp8_block: the result is bf16, fp16 or fp32")
     if out is None:
-        out = torch.empty((M, N), dtype=dtype, device=dev)
-    elif tuple(out.shape) != (M, N) or not out.is_contiguous():
+        out = a_scale.new_empty((M, N), dtype=dtype)
+    elif out.shape != (M, N) or not out.is_contiguous():
         raise RuntimeError("out must be a contiguous [M, N] tensor")
     if M == 0 or N == 0:
         return out
     L = lib()
     stream, sms = current_stream_handle(dev), int(num_sms or 0)
-    ws = _bytes(L.ek_gemm_fp8_block_workspace_bytes(M, N, K, _most_sms(dev, sms)), dev)
+    need = L.ek_gemm_fp8_block_workspace_bytes(M, N, K, _most_sms(dev, sms))
+    ws = _bytes(need, a_scale)
     with _on_device(dev):
         check(L.ek_gemm_fp8_block(a_q.data_ptr(), w_q.data_ptr(), a_scale.data_ptr(), w_scale.data_ptr(),
-                                  out.data_ptr(), M, N, K, _ROW_DTYPES[dtype], sms, ws.data_ptr(), ws.numel(), stream),
+                                  out.data_ptr(), M, N, K, _ROW_DTYPES[dtype], sms, ws.data_ptr(), need, stream),
               "ek_gemm_fp8_block")
     return out
 
 
-def _bytes(n: int, dev: torch.device) -> torch.Tensor:
+def _bytes(n: int, like: torch.Tensor) -> torch.Tensor:
     """Workspace of one call, as _scratch."""
     if n == _SIZE_MAX:
         check(_lib.EK_ERR_INVALID, "workspace size")
-    return torch.empty(n, dtype=torch.uint8, device=dev)
+    return like.new_empty(n, dtype=torch.uint8)
 
 
 def _check_ffn(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, w3: torch.Tensor, dtype: torch.dtype,
@@ -1215,7 +1217,7 @@ def gated_ffn(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, w3: torch.Ten
     gate, dtype = _gate(act), x.dtype
     x, w1, w2, w3, T, H, I = _check_ffn(x, w1, w2, w3, dtype, 8)
     y = x.new_empty((T, H)) if out is None else out
-    if out is not None and (out.dtype != dtype or tuple(out.shape) != (T, H) or not out.is_contiguous()):
+    if out is not None and (out.dtype != dtype or out.shape != (T, H) or not out.is_contiguous()):
         raise RuntimeError("out must be a contiguous [T, H] tensor of x's dtype")
     if out is not None and out.data_ptr() % 16:
         y = x.new_empty((T, H))
@@ -1223,10 +1225,11 @@ def gated_ffn(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, w3: torch.Ten
     if T > 0:
         L = lib()
         stream, sms = current_stream_handle(dev), int(num_sms or 0)
-        ws = _bytes(L.ek_gated_ffn_workspace_bytes(T, H, I, _most_sms(dev, sms)), dev)
+        need = L.ek_gated_ffn_workspace_bytes(T, H, I, _most_sms(dev, sms))
+        ws = _bytes(need, x)
         with _on_device(dev):
             check(L.ek_gated_ffn(x.data_ptr(), w1.data_ptr(), w2.data_ptr(), w3.data_ptr(), y.data_ptr(), _ptr(h), T, H,
-                                 I, _DTYPES[dtype], gate, sms, ws.data_ptr(), ws.numel(), stream), "ek_gated_ffn")
+                                 I, _DTYPES[dtype], gate, sms, ws.data_ptr(), need, stream), "ek_gated_ffn")
     if out is not None and y is not out:
         y = out.copy_(y)
     return (y, h) if save else y
@@ -1250,11 +1253,12 @@ def gated_ffn_grad(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, w3: torc
     d_x, d_w13, d_w2 = x.new_empty((T, H)), x.new_empty((2, I, H)), x.new_empty((H, I))
     L = lib()
     stream, sms = current_stream_handle(dev), int(num_sms or 0)
-    ws = _bytes(L.ek_gated_ffn_grad_workspace_bytes(T, H, I, _most_sms(dev, sms)), dev)
+    need = L.ek_gated_ffn_grad_workspace_bytes(T, H, I, _most_sms(dev, sms))
+    ws = _bytes(need, x)
     with _on_device(dev):
         check(L.ek_gated_ffn_grad(x.data_ptr(), w1.data_ptr(), w2.data_ptr(), w3.data_ptr(), h.data_ptr(),
                                   d_out.data_ptr(), d_x.data_ptr(), d_w13.data_ptr(), d_w2.data_ptr(), T, H, I,
-                                  _DTYPES[dtype], gate, sms, ws.data_ptr(), ws.numel(), stream), "ek_gated_ffn_grad")
+                                  _DTYPES[dtype], gate, sms, ws.data_ptr(), need, stream), "ek_gated_ffn_grad")
     return d_x, d_w13[0], d_w2, d_w13[1]
 
 
@@ -1302,11 +1306,12 @@ def gated_ffn_fp8(x: torch.Tensor, qw: dict, act: str = "silu", out: torch.Tenso
     y = out if out.data_ptr() % 16 == 0 else x.new_empty((T, H))
     L = lib()
     stream, sms = current_stream_handle(dev), int(num_sms or 0)
-    ws = _bytes(L.ek_gated_ffn_fp8_workspace_bytes(T, H, I, _most_sms(dev, sms)), dev)
+    need = L.ek_gated_ffn_fp8_workspace_bytes(T, H, I, _most_sms(dev, sms))
+    ws = _bytes(need, x)
     with _on_device(dev):
         check(L.ek_gated_ffn_fp8(x.data_ptr(), w1.data_ptr(), w2.data_ptr(), w3.data_ptr(), s1.data_ptr(),
                                  s2.data_ptr(), s3.data_ptr(), y.data_ptr(), T, H, I, gate, sms, ws.data_ptr(),
-                                 ws.numel(), stream), "ek_gated_ffn_fp8")
+                                 need, stream), "ek_gated_ffn_fp8")
     return out if y is out else out.copy_(y)
 
 

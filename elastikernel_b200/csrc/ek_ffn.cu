@@ -43,11 +43,11 @@ int allow_smem(Kernel kernel, int bytes, bool (&done)[64]) {
   return rc;
 }
 
-// cluster: CTAs per cluster (0: none); overlap: may start before its predecessor
-// on the stream has ended, which must be a launch of the same call
+// Every kernel here waits for its predecessor itself (pdl_wait), so each launch may
+// begin before that has ended. cluster: CTAs per cluster (0: none).
 template <class... P, class... A>
 int launch(const char* what, void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t stream, int cluster,
-           bool overlap, const A&... args) {
+           const A&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
@@ -61,10 +61,8 @@ int launch(const char* what, void (*kernel)(P...), dim3 grid, int threads, size_
     attr[n].val.clusterDim.y = 1;
     attr[n++].val.clusterDim.z = 1;
   }
-  if (overlap) {
-    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[n++].val.programmaticStreamSerializationAllowed = 1;
-  }
+  attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[n++].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = n;
   return check_cuda(cudaLaunchKernelEx(&cfg, kernel, args...), what);
@@ -137,17 +135,16 @@ size_t stream_bytes_most(int rows, int rows_per_tile, int T, int sms) {
 
 template <class Cfg>
 int launch_stream(const CUtensorMap& tw, const CUtensorMap& tw2, const CUtensorMap& tx, const StreamParams& p,
-                  cudaStream_t s, bool overlap) {
+                  cudaStream_t s) {
   static bool done[64] = {false};
   const int rc = allow_smem(stream_kernel<Cfg>, Cfg::SMEM_BYTES, done);
   if (rc) return rc;
-  return launch("stream product", stream_kernel<Cfg>, dim3(p.sp.ctas), Cfg::THREADS, Cfg::SMEM_BYTES, s, 0, overlap, tw,
-                tw2, tx, p);
+  return launch("stream product", stream_kernel<Cfg>, dim3(p.sp.ctas), Cfg::THREADS, Cfg::SMEM_BYTES, s, 0, tw, tw2, tx,
+                p);
 }
 
 template <int kElem, bool kGate>
-int launch_stream_nt(const void* w, const void* w2, const void* x, int rows, int K, StreamParams& p, cudaStream_t s,
-                     bool overlap) {
+int launch_stream_nt(const void* w, const void* w2, const void* x, int rows, int K, StreamParams& p, cudaStream_t s) {
   const int nt = p.T <= 16 ? 16 : p.T <= 32 ? 32 : p.T <= 64 ? 64 : 128;
   p.n = (p.T + 15) / 16 * 16;
   CUtensorMap tw, tw2, tx;
@@ -157,10 +154,10 @@ int launch_stream_nt(const void* w, const void* w2, const void* x, int rows, int
   if (kGate && (rc = map_k(&tw2, w2, kElem, rows, K, 128))) return rc;
   if ((rc = map_k(&tx, x, kElem, p.T, K, p.n))) return rc;
   switch (nt) {
-    case 16: return launch_stream<StreamCfg<kElem, 16, kGate>>(tw, tw2, tx, p, s, overlap);
-    case 32: return launch_stream<StreamCfg<kElem, 32, kGate>>(tw, tw2, tx, p, s, overlap);
-    case 64: return launch_stream<StreamCfg<kElem, 64, kGate>>(tw, tw2, tx, p, s, overlap);
-    default: return launch_stream<StreamCfg<kElem, 128, kGate>>(tw, tw2, tx, p, s, overlap);
+    case 16: return launch_stream<StreamCfg<kElem, 16, kGate>>(tw, tw2, tx, p, s);
+    case 32: return launch_stream<StreamCfg<kElem, 32, kGate>>(tw, tw2, tx, p, s);
+    case 64: return launch_stream<StreamCfg<kElem, 64, kGate>>(tw, tw2, tx, p, s);
+    default: return launch_stream<StreamCfg<kElem, 128, kGate>>(tw, tw2, tx, p, s);
   }
 }
 
@@ -179,8 +176,9 @@ struct StreamScales {
 
 // out[t, n] = x[t] . w[n]
 int stream_store(int dtype, const void* w, const void* x, const StreamScales& sc, int T, int N, int K, void* out,
-                 int out_type, int sms, void* ws, size_t ws_bytes, cudaStream_t s, bool overlap) {
+                 int out_type, int sms, void* ws, size_t ws_bytes, cudaStream_t s, bool early) {
   StreamParams p{};
+  p.early = early;
   p.sp = stream_split(N, 256, K, 128 / elem_size(dtype), sms);
   if (ws_bytes < stream_bytes(p.sp, T)) return set_error(EK_ERR_INVALID, "workspace too small");
   p.T = T;
@@ -188,21 +186,22 @@ int stream_store(int dtype, const void* w, const void* x, const StreamScales& sc
   p.w_scale = sc.w;
   p.w_blocks = ceil_div(N, 128);
   p.ws = static_cast<float*>(ws);
-  int rc = dtype == EK_DTYPE_BF16 ? launch_stream_nt<kBF16, false>(w, w, x, N, K, p, s, overlap)
-           : dtype == EK_DTYPE_FP16 ? launch_stream_nt<kFP16, false>(w, w, x, N, K, p, s, overlap)
-                                    : launch_stream_nt<kE4M3, false>(w, w, x, N, K, p, s, overlap);
+  int rc = dtype == EK_DTYPE_BF16 ? launch_stream_nt<kBF16, false>(w, w, x, N, K, p, s)
+           : dtype == EK_DTYPE_FP16 ? launch_stream_nt<kFP16, false>(w, w, x, N, K, p, s)
+                                    : launch_stream_nt<kE4M3, false>(w, w, x, N, K, p, s);
   if (rc) return rc;
   const int ways = stream_ways(p.sp, T, 2 * p.sp.tiles, sms);
   const int wide = aligned16(out) && N % 4 == 0;
-  return launch("stream sums", stream_store_reduce_kernel, dim3(2 * p.sp.tiles, ceil_div(T, 8 / ways)), 256, 0, s, 0, true,
+  return launch("stream sums", stream_store_reduce_kernel, dim3(2 * p.sp.tiles, ceil_div(T, 8 / ways)), 256, 0, s, 0,
                 p.sp, (const float*)p.ws, T, N, out, out_type, wide, ways);
 }
 
 // a[t, i] = f(x[t] . w1[i]) (x[t] . w3[i]); e4m3: codes and scales of a
 int stream_gate(int dtype, const void* w1, const void* w3, const void* x, const StreamScales& sc, int T, int I, int H,
                 int gate, void* a, void* h, uint8_t* codes, float* scales, int sms, void* ws, size_t ws_bytes,
-                cudaStream_t s, bool overlap) {
+                cudaStream_t s, bool early) {
   StreamParams p{};
+  p.early = early;
   p.sp = stream_split(I, 128, H, 128 / elem_size(dtype), sms);
   if (ws_bytes < stream_bytes(p.sp, T)) return set_error(EK_ERR_INVALID, "workspace too small");
   p.T = T;
@@ -211,12 +210,12 @@ int stream_gate(int dtype, const void* w1, const void* w3, const void* x, const 
   p.w_scale2 = sc.w2;
   p.w_blocks = ceil_div(I, 128);
   p.ws = static_cast<float*>(ws);
-  int rc = dtype == EK_DTYPE_BF16 ? launch_stream_nt<kBF16, true>(w1, w3, x, I, H, p, s, overlap)
-           : dtype == EK_DTYPE_FP16 ? launch_stream_nt<kFP16, true>(w1, w3, x, I, H, p, s, overlap)
-                                    : launch_stream_nt<kE4M3, true>(w1, w3, x, I, H, p, s, overlap);
+  int rc = dtype == EK_DTYPE_BF16 ? launch_stream_nt<kBF16, true>(w1, w3, x, I, H, p, s)
+           : dtype == EK_DTYPE_FP16 ? launch_stream_nt<kFP16, true>(w1, w3, x, I, H, p, s)
+                                    : launch_stream_nt<kE4M3, true>(w1, w3, x, I, H, p, s);
   if (rc) return rc;
   const int ways = stream_ways(p.sp, T, p.sp.tiles, sms);
-  return launch("stream gate", stream_gate_reduce_kernel, dim3(p.sp.tiles, ceil_div(T, 8 / ways)), 256, 0, s, 0, true, p.sp,
+  return launch("stream gate", stream_gate_reduce_kernel, dim3(p.sp.tiles, ceil_div(T, 8 / ways)), 256, 0, s, 0, p.sp,
                 (const float*)p.ws, T, I, gate, dtype, a, h, codes, scales, ways);
 }
 
@@ -230,7 +229,7 @@ int launch_ffn(const CUtensorMap (&ta)[2], const CUtensorMap (&tb)[2], FfnParams
   if (units > 0x3fffffff) return set_error(EK_ERR_INVALID, "too many tiles");
   p.num_units = (int)units;
   const int pairs = (int)std::min<long long>(std::max(1, sms / 2), units);
-  return launch("feed-forward product", ffn_gemm_kernel<Cfg>, dim3(2 * pairs), Cfg::THREADS, Cfg::SMEM_BYTES, s, 2, false,
+  return launch("feed-forward product", ffn_gemm_kernel<Cfg>, dim3(2 * pairs), Cfg::THREADS, Cfg::SMEM_BYTES, s, 2,
                 ta[0], ta[1], tb[0], tb[1], p);
 }
 
@@ -269,7 +268,7 @@ int ffn_store(const FfnOperand& A, const FfnOperand& B, int M, int N, int k, int
   int rc = launch_ffn<FfnCfg<kElem, kAMN, kBMN, kFfnStore>>(ta, tb, p, sms, s);
   if (rc || p.splits == 1) return rc;
   const long long n8 = elems / 8;
-  return launch("feed-forward sums", ffn_reduce_kernel<kElem>, dim3(grid_for((n8 + 255) / 256, sms)), 256, 0, s, 0, false,
+  return launch("feed-forward sums", ffn_reduce_kernel<kElem>, dim3(grid_for((n8 + 255) / 256, sms)), 256, 0, s, 0,
                 (const float*)p.ws, p.splits, n8, C);
 }
 
@@ -319,7 +318,7 @@ int ffn_gate(const void* x, const void* w1, const void* w3, void* a, void* h, in
   rc = launch_ffn<FfnCfg<kElem, false, false, kFfnGate>>(ta, tb, p, sms, s);
   if (rc || p.splits == 1) return rc;
   return launch("feed-forward gate sums", ffn_gate_reduce_kernel<kElem>, dim3(grid_for(((long long)T * I / 8 + 255) / 256, sms)),
-                256, 0, s, 0, false, (const float*)p.ws, p.splits, T, I, gate, a, h);
+                256, 0, s, 0, (const float*)p.ws, p.splits, T, I, gate, a, h);
 }
 
 template <int kElem>
@@ -373,7 +372,7 @@ int gated_ffn_grad(const void* x, const void* w1, const void* w2, const void* w3
   if ((rc = launch_ffn<FfnCfg<kElem, false, true, kFfnGateGrad>>(ta, tb, p, sms, s))) return rc;
   if (p.splits > 1 &&
       (rc = launch("feed-forward gate gradient sums", ffn_gate_grad_reduce_kernel<kElem>,
-                   dim3(grid_for(((long long)T * I / 8 + 255) / 256, sms)), 256, 0, s, 0, false, (const float*)p.ws,
+                   dim3(grid_for(((long long)T * I / 8 + 255) / 256, sms)), 256, 0, s, 0, (const float*)p.ws,
                    p.splits, T, I, gate, h, (void*)dh, (void*)a)))
     return rc;
   const FfnOperand dh_planes = {{dh, dh + plane}, 2};
@@ -405,7 +404,7 @@ int launch_fp8(const void* a, const void* w, const void* w2, int K, Fp8BlockPara
   p.scale4 = p.k_blocks % 4 == 0 && aligned16(p.a_scale) && aligned16(p.w_scale) && aligned16(p.w_scale2);
   const int groups = (int)std::min<long long>(std::max(1, sms / Cfg::CTAS), units);
   return launch("block-scaled product", fp8_block_kernel<Cfg>, dim3(Cfg::CTAS * groups), Cfg::THREADS, Cfg::SMEM_BYTES, s,
-                kFp8Pair ? 2 : 0, false, ta, tb, tb2, p);
+                kFp8Pair ? 2 : 0, ta, tb, tb2, p);
 }
 
 int fp8_splits(int M, int N, int K, int sms, size_t cap) {
@@ -414,9 +413,9 @@ int fp8_splits(int M, int N, int K, int sms, size_t cap) {
 }
 
 int fp8_store(const void* a, const void* w, const float* as, const float* wsc, void* C, int M, int N, int K, int out_type,
-              int sms, void* ws, size_t ws_bytes, cudaStream_t s, bool overlap) {
+              int sms, void* ws, size_t ws_bytes, cudaStream_t s, bool early) {
   if (M <= kStreamTokens)
-    return stream_store(EK_DTYPE_E4M3, w, a, {as, wsc, nullptr}, M, N, K, C, out_type, sms, ws, ws_bytes, s, overlap);
+    return stream_store(EK_DTYPE_E4M3, w, a, {as, wsc, nullptr}, M, N, K, C, out_type, sms, ws, ws_bytes, s, early);
   Fp8BlockParams p{};
   p.M = M;
   p.N = N;
@@ -434,7 +433,7 @@ int fp8_store(const void* a, const void* w, const float* as, const float* wsc, v
   int rc = launch_fp8<false>(a, w, w, K, p, sms, s);
   if (rc || p.splits == 1) return rc;
   const long long n = (long long)M * N;
-  return launch("block-scaled sums", fp8_block_reduce_kernel, dim3(grid_for((n + 255) / 256, sms)), 256, 0, s, 0, false,
+  return launch("block-scaled sums", fp8_block_reduce_kernel, dim3(grid_for((n + 255) / 256, sms)), 256, 0, s, 0,
                 (const float*)p.ws, p.splits, n, C, out_type);
 }
 
@@ -600,10 +599,13 @@ int ek_gated_ffn_fp8(const void* x, const void* w1, const void* w2, const void* 
   float *xs = reinterpret_cast<float*>(ws + L.xs), *as = reinterpret_cast<float*>(ws + L.as);
   char* rest = ws + L.rest;
   const size_t rest_bytes = ws_bytes - L.rest;
-  if ((rc = ek_quant_e4m3_ex(x, EK_DTYPE_BF16, T, H, 1, 128, 0, xq, xs, stream))) return rc;
+  const long long groups = (long long)T * ceil_div(H, 128);
+  rc = launch("feed-forward quantisation", ffn_quant_kernel, dim3(grid_for((groups + 15) / 16, sms)), 256, 0, s, 0,
+              static_cast<const __nv_bfloat16*>(x), groups, H, xq, xs);
+  if (rc) return rc;
   if (T <= kStreamTokens) {
     rc = stream_gate(EK_DTYPE_E4M3, w1, w3, xq, {xs, s1, s3}, T, I, H, gate, nullptr, nullptr, aq, as, sms, rest,
-                     rest_bytes, s, false);
+                     rest_bytes, s, true);
   } else {
     Fp8BlockParams p{};
     p.M = T;

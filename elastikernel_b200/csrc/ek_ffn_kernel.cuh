@@ -36,6 +36,13 @@
 
 namespace ek {
 
+// Programmatic dependent launch. A call's first launch waits for whatever precedes it on
+// the stream before it reads, writes or lets its successor start, so that from then on
+// nothing the caller launched is still running: later launches of the call may fetch
+// the weights (which no launch of the call writes) before their own wait.
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // One lane of a converged warp, always the same. A loop that a whole warp walks with an
 // elected lane issuing keeps the operands of tcgen05.mma uniform; issued from inside a
 // one-lane branch they are moved to the uniform registers one by one, at about 100
@@ -291,6 +298,8 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
   cluster_sync();  // the peer's barriers exist before anyone signals them
   tc_fence_after();
   const uint32_t tmem_base = *s_tmem_base;
+  pdl_wait();
+  pdl_launch();
 
   if (warp == 0) {
     if (lane == 0) {
@@ -530,6 +539,8 @@ __device__ __forceinline__ void sum_slices8(const float* __restrict__ ws, int sp
 template <int kElem>
 __global__ void __launch_bounds__(256) ffn_reduce_kernel(const float* __restrict__ ws, int splits, long long n8,
                                                          void* __restrict__ out) {
+  pdl_wait();
+  pdl_launch();
   for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n8; i += gridDim.x * 256ll) {
     float v[8];
     sum_slices8(ws, splits, n8 * 8, i * 8, v);
@@ -541,6 +552,8 @@ __global__ void __launch_bounds__(256) ffn_reduce_kernel(const float* __restrict
 template <int kElem>
 __global__ void __launch_bounds__(256) ffn_gate_reduce_kernel(const float* __restrict__ ws, int splits, int T, int I,
                                                               int gate, void* __restrict__ a, void* __restrict__ h) {
+  pdl_wait();
+  pdl_launch();
   const long long n8 = (long long)T * I / 8;
   for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n8; i += gridDim.x * 256ll) {
     const long long row = i * 8 / I, at = row * 2 * I + (i * 8 - row * I);
@@ -564,6 +577,8 @@ template <int kElem>
 __global__ void __launch_bounds__(256)
     ffn_gate_grad_reduce_kernel(const float* __restrict__ ws, int splits, int T, int I, int gate,
                                 const void* __restrict__ h, void* __restrict__ dh, void* __restrict__ act) {
+  pdl_wait();
+  pdl_launch();
   const long long n8 = (long long)T * I / 8;
   for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n8; i += gridDim.x * 256ll) {
     const uint4* src = reinterpret_cast<const uint4*>(h) + i;

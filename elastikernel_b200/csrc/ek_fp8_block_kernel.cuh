@@ -145,6 +145,8 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
   if constexpr (Cfg::kPair) cluster_sync();  // the peer's barriers exist before anyone signals them
   tc_fence_after();
   const uint32_t tmem_base = *s_tmem_base;
+  pdl_wait();
+  pdl_launch();
 
   struct U {
     int tm, tn, split, kb0, kb1;
@@ -407,6 +409,8 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
 // out[i] = sum over the slices, in slice order, of ws[s][i]
 __global__ void __launch_bounds__(256) fp8_block_reduce_kernel(const float* __restrict__ ws, int splits, long long n,
                                                                void* __restrict__ out, int type) {
+  pdl_wait();
+  pdl_launch();
   for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
     float v = 0.f;
     for (int s = 0; s < splits; ++s) v += __ldcg(ws + s * n + i);

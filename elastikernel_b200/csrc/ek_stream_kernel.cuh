@@ -19,18 +19,14 @@
 //   warp 0  TMA producer; warp 1  TMEM and MMA; warp 2  scales (e4m3)
 //   warps 3..10  epilogue: two per TMEM lane quarter, one 128-row block each
 //
-// Launches of one call overlap (programmatic dependent launch): weights are not
-// written by a predecessor within the call, so a CTA fills its stages with them
-// before it waits; everything else is read and written after the wait.
+// Launches overlap (programmatic dependent launch): within a call a CTA fills its
+// stages with weights before it waits; everything else is read and written after.
 #pragma once
 #include <cuda_fp8.h>
 
 #include "ek_ffn_kernel.cuh"
 
 namespace ek {
-
-__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void pdl_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 template <int kElem_, int NT_, bool kGate_>
 struct StreamCfg {
@@ -62,6 +58,7 @@ struct StreamSplit {
 struct StreamParams {
   StreamSplit sp;
   int T;
+  int early;               // a later launch of its call: the weights may be fetched before the wait
   int n;                   // tokens per MMA: T rounded up to 16 (the box's rows)
   const float* tok_scale;  // e4m3: [T][k_blocks]
   const float* w_scale;    // [rows / 128][k_blocks]; gate: W1's
@@ -118,6 +115,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *s_tmem_base;
+  if (!p.early) pdl_wait();
   pdl_launch();
 
   if (warp == 0) {
@@ -446,6 +444,41 @@ __global__ void __launch_bounds__(256)
     *reinterpret_cast<uint32_t*>(codes + at) = lo | (hi << 16);
   }
   if ((threadIdx.x & 31) == 0) scales[(size_t)t * ((I + 127) / 128) + tile] = s;
+}
+
+// e4m3 codes [T][H] and scales [T][ceil(H / 128)] of bf16 rows: a scale per 128 elements
+// (largest magnitude / 448, 1 for zeros), IEEE quotients, as the row quantisation of the
+// library. A half warp per group, 8 elements a lane; H a multiple of 8. Memory bound at
+// many tokens, a launch at few: it lets the product after it fetch weights meanwhile.
+__global__ void __launch_bounds__(256) ffn_quant_kernel(const __nv_bfloat16* __restrict__ x, long long groups, int H,
+                                                        uint8_t* __restrict__ codes, float* __restrict__ scales) {
+  pdl_wait();
+  pdl_launch();
+  const int per_row = (H + 127) / 128, hl = threadIdx.x & 15;
+  // the bound is uniform over the warp, so that every lane reaches the exchanges
+  for (long long g0 = (blockIdx.x * 256ll + threadIdx.x) / 32 * 2; g0 < groups; g0 += gridDim.x * 16ll) {
+    const long long g = g0 + ((threadIdx.x >> 4) & 1);
+    const long long row = g / per_row;
+    const int c = (int)(g - row * per_row) * 128 + hl * 8;
+    const bool in = g < groups && c < H;
+    float v[8];
+    unpack8<kBF16>(in ? __ldg(reinterpret_cast<const uint4*>(x + row * H + c)) : make_uint4(0, 0, 0, 0), v);
+    float m = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(v[j]));
+#pragma unroll
+    for (int o = 8; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float s = m > 0.f ? m / 448.0f : 1.0f;
+    if (!in) continue;
+    uint32_t pk[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      pk[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[4 * i] / s, v[4 * i + 1] / s), __NV_SATFINITE, __NV_E4M3) |
+              ((uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[4 * i + 2] / s, v[4 * i + 3] / s), __NV_SATFINITE, __NV_E4M3)
+               << 16);
+    *reinterpret_cast<uint2*>(codes + row * H + c) = make_uint2(pk[0], pk[1]);
+    if (hl == 0) scales[g] = s;
+  }
 }
 
 }  // namespace ek
