@@ -384,16 +384,12 @@ int gated_ffn_grad(const void* x, const void* w1, const void* w2, const void* w3
 }
 
 // ------------------------------------------------------------------ 8-bit tiles
-#ifndef EXP_SINGLE
-#define EXP_SINGLE 0
-#endif
-constexpr bool kFp8Pair = !EXP_SINGLE;
 template <bool kGate>
 int launch_fp8(const void* a, const void* w, const void* w2, int K, Fp8BlockParams& p, int sms, cudaStream_t s) {
-  using Cfg = Fp8BlockCfg<kGate, kFp8Pair>;
+  using Cfg = Fp8BlockCfg<kGate>;
   CUtensorMap ta, tb, tb2;
   int rc = map_k(&ta, a, EK_DTYPE_E4M3, p.M, K, 128);
-  if (rc || (rc = map_k(&tb, w, EK_DTYPE_E4M3, p.N, K, kFp8Pair || kGate ? 128 : 256))) return rc;
+  if (rc || (rc = map_k(&tb, w, EK_DTYPE_E4M3, p.N, K, 128))) return rc;
   tb2 = tb;
   if (kGate && (rc = map_k(&tb2, w2, EK_DTYPE_E4M3, p.N, K, 128))) return rc;
   static bool done[64] = {false};
@@ -402,9 +398,9 @@ int launch_fp8(const void* a, const void* w, const void* w2, int K, Fp8BlockPara
   if (units > 0x3fffffff) return set_error(EK_ERR_INVALID, "too many tiles");
   p.num_units = (int)units;
   p.scale4 = p.k_blocks % 4 == 0 && aligned16(p.a_scale) && aligned16(p.w_scale) && aligned16(p.w_scale2);
-  const int groups = (int)std::min<long long>(std::max(1, sms / Cfg::CTAS), units);
-  return launch("block-scaled product", fp8_block_kernel<Cfg>, dim3(Cfg::CTAS * groups), Cfg::THREADS, Cfg::SMEM_BYTES, s,
-                kFp8Pair ? 2 : 0, ta, tb, tb2, p);
+  const int groups = (int)std::min<long long>(std::max(1, sms / 2), units);
+  return launch("block-scaled product", fp8_block_kernel<Cfg>, dim3(2 * groups), Cfg::THREADS, Cfg::SMEM_BYTES, s,
+                2, ta, tb, tb2, p);
 }
 
 int fp8_splits(int M, int N, int K, int sms, size_t cap) {
@@ -419,7 +415,7 @@ int fp8_store(const void* a, const void* w, const float* as, const float* wsc, v
   Fp8BlockParams p{};
   p.M = M;
   p.N = N;
-  p.tiles_m = ceil_div(M, kFp8Pair ? 256 : 128);
+  p.tiles_m = ceil_div(M, 256);
   p.tiles_n = ceil_div(N, 256);
   p.k_blocks = ceil_div(K, 128);
   p.splits = fp8_splits(M, N, K, sms, ws_bytes);
@@ -610,7 +606,7 @@ int ek_gated_ffn_fp8(const void* x, const void* w1, const void* w2, const void* 
     Fp8BlockParams p{};
     p.M = T;
     p.N = I;
-    p.tiles_m = ceil_div(T, kFp8Pair ? 256 : 128);
+    p.tiles_m = ceil_div(T, 256);
     p.tiles_n = ceil_div(I, 128);
     p.k_blocks = ceil_div(H, 128);
     p.splits = 1;

@@ -21,18 +21,17 @@
 
 namespace ek {
 
-template <bool kGate_, bool kPair_>
+template <bool kGate_>
 struct Fp8BlockCfg {
-  static constexpr bool kGate = kGate_, kPair = kPair_;
-  static constexpr int CTAS = kPair ? 2 : 1;
-  static constexpr int HALF_BYTES = 128 * 128, STAGE_BYTES = (kPair ? 2 : 3) * HALF_BYTES;
-  static constexpr int STAGES = kPair ? 6 : 4;
+  static constexpr bool kGate = kGate_;
+  static constexpr int HALF_BYTES = 128 * 128, STAGE_BYTES = 2 * HALF_BYTES;
+  static constexpr int STAGES = 5;
   static constexpr int EPI_WARPS = 8;
   static constexpr int THREADS = 128 + 32 * EPI_WARPS;
   // 384 threads are launched with 168 registers each: 128 x 56 + 256 x 224 = 64512 = 384 x 168
   static constexpr int REGS_LOAD = 56, REGS_EPI = 224;
-  static constexpr uint32_t IDESC = umma_idesc(0u, false, 128 * CTAS, 128);
-  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_WARPS * 2048 + 1024 /*largest values*/ + 256 + 1024;
+  static constexpr uint32_t IDESC = umma_idesc(0u, false, 256, 256);
+  static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_WARPS * 8192 + 1024 /*largest values*/ + 256 + 1024;
 };
 
 struct Fp8BlockParams {
@@ -52,47 +51,58 @@ struct Fp8BlockParams {
   float* scales;
 };
 
-// 32 consecutive columns, from column col, of the warp's rows [row0, row0 + 32): of the
-// result, or of a slice's sums
-__device__ __forceinline__ void fp8_block_store32(const Fp8BlockParams& p, const WarpTile& wt, int split, int row0, int col,
-                                                  const float2* v2) {
-  const float* v = reinterpret_cast<const float*>(v2);
+// The warp's 32 rows x 128 columns from (row0, col0), lane's row in v, to the result or to
+// a slice's sums. They cross 8 KB of shared memory, 32 rows of 16 pieces of 16 bytes (a
+// piece's place permuted by the row, so that no bank is met twice), so that a warp stores
+// 256 contiguous bytes of two rows at a time: 0.3 us a tile where pieces of 16 bytes of 32
+// rows took 3.5.
+__device__ __forceinline__ void fp8_block_store(const Fp8BlockParams& p, uint8_t* tile, int lane, int split, int row0,
+                                                int col0, const float* v) {
+  auto piece = [&](int r, int j) -> uint4& { return *reinterpret_cast<uint4*>(tile + r * 256 + ((j ^ (r & 7)) << 4)); };
   const bool sums = p.splits > 1;
-  if (p.wide && (sums || p.out_type == kOutFP32)) {
-    float* out = sums ? p.ws + (size_t)split * p.M * p.N : reinterpret_cast<float*>(p.C);
+  if (p.wide && !sums && p.out_type != kOutFP32) {
+    __syncwarp();
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      uint4 pk[4];
-#pragma unroll
-      for (int g = 0; g < 4; ++g) pk[g] = *reinterpret_cast<const uint4*>(v + h * 16 + g * 4);
-      store_warp<4>(wt, pk, out, row0, p.M, col + h * 16, p.N);
+    for (int j = 0; j < 16; ++j) piece(lane, j) = p.out_type == kOutBF16 ? pack8<kBF16>(v + j * 8) : pack8<kFP16>(v + j * 8);
+    __syncwarp();
+#pragma unroll 4
+    for (int i = 0; i < 16; ++i) {
+      const int r = 2 * i + (lane >> 4), row = row0 + r, col = col0 + (lane & 15) * 8;
+      if (row < p.M && col < p.N)
+        *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.C) + (size_t)row * p.N + col) = piece(r, lane & 15);
     }
-  } else if (p.wide) {
-    uint4 pk[4];
+    return;
+  }
+  float* out = sums ? p.ws + (size_t)split * p.M * p.N : reinterpret_cast<float*>(p.C);
 #pragma unroll
-    for (int g = 0; g < 4; ++g) pk[g] = p.out_type == kOutBF16 ? pack8<kBF16>(v + g * 8) : pack8<kFP16>(v + g * 8);
-    store_warp<8>(wt, pk, p.C, row0, p.M, col, p.N);
-  } else {
-    // rows that no 16-byte piece fits: 32 columns of a row at a time, one per lane
-    float* t = reinterpret_cast<float*>(wt.base);
-#pragma unroll 1
-    for (int h = 0; h < 2; ++h) {  // 2 KB hold 16 rows
-      __syncwarp();
-      if ((wt.lane >> 4) == h) {
+  for (int half = 0; half < 2; ++half) {
+    __syncwarp();
 #pragma unroll
-        for (int j = 0; j < 32; ++j) t[(wt.lane & 15) * 32 + ((j + wt.lane) & 31)] = v[j];
+    for (int j = 0; j < 16; ++j) piece(lane, j) = *reinterpret_cast<const uint4*>(v + half * 64 + j * 4);
+    __syncwarp();
+    const int c0 = col0 + half * 64;
+    if (p.wide) {
+#pragma unroll 4
+      for (int i = 0; i < 16; ++i) {
+        const int r = 2 * i + (lane >> 4), row = row0 + r, col = c0 + (lane & 15) * 4;
+        if (row < p.M && col < p.N) *reinterpret_cast<uint4*>(out + (size_t)row * p.N + col) = piece(r, lane & 15);
       }
-      __syncwarp();
-#pragma unroll 1
-      for (int r = 0; r < 16; ++r) {
-        const int row = row0 + h * 16 + r, c = col + wt.lane;
-        const float x = t[r * 32 + ((wt.lane + h * 16 + r) & 31)];
-        if (row < p.M && c < p.N) {
-          const size_t at = (size_t)row * p.N + c;
-          if (sums)
-            p.ws[(size_t)split * p.M * p.N + at] = x;
-          else
-            store_out(p.C, p.out_type, at, x);
+    } else {  // rows that no 16-byte piece fits: consecutive lanes, consecutive elements
+#pragma unroll 4
+      for (int r = 0; r < 32; ++r) {
+        const int row = row0 + r;
+        if (row >= p.M) break;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int c = k * 32 + lane;
+          const float x = reinterpret_cast<const float*>(&piece(r, c >> 2))[c & 3];
+          if (c0 + c < p.N) {
+            const size_t at = (size_t)row * p.N + c0 + c;
+            if (sums)
+              out[at] = x;
+            else
+              store_out(p.C, p.out_type, at, x);
+          }
         }
       }
     }
@@ -106,21 +116,20 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
   constexpr int STAGES = Cfg::STAGES, HB = Cfg::HALF_BYTES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* s_tile = smem + STAGES * Cfg::STAGE_BYTES;                           // [EPI_WARPS] of 2 KB
-  float* s_amax = reinterpret_cast<float*>(s_tile + Cfg::EPI_WARPS * 2048);     // [2][128]
+  uint8_t* s_tile = smem + STAGES * Cfg::STAGE_BYTES;                           // [EPI_WARPS] of 8 KB
+  float* s_amax = reinterpret_cast<float*>(s_tile + Cfg::EPI_WARPS * 8192);     // [2][128]
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(s_amax + 256);
   uint64_t* empty_bar = full_bar + STAGES;
   uint64_t* kfull_bar = empty_bar + STAGES;
-  uint64_t* kempty_bar = kfull_bar + 4;  // both [half][buffer]
-  uint64_t* drain_bar = kempty_bar + 4;
+  uint64_t* kempty_bar = kfull_bar + 2;
+  uint64_t* drain_bar = kempty_bar + 2;
   uint32_t* s_tmem_base = reinterpret_cast<uint32_t*>(drain_bar + 1);
   volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem_base + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = Cfg::kPair ? (int)cluster_ctarank() : 0;
+  const int rank = (int)cluster_ctarank();
   const bool leader = rank == 0;
-  const int unit0 = Cfg::kPair ? (int)cluster_id_x() : (int)blockIdx.x;
-  const int unit_step = Cfg::kPair ? (int)nclusters_x() : (int)gridDim.x;
+  const int unit0 = (int)cluster_id_x(), unit_step = (int)nclusters_x();
   const int KB = p.k_blocks;
 
   if (threadIdx.x == 0) {
@@ -128,21 +137,21 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
       mbar_init(&full_bar[s], 1);
       mbar_init(&empty_bar[s], 1);
     }
-    for (int b = 0; b < 4; ++b) {
+    for (int b = 0; b < 2; ++b) {
       mbar_init(&kfull_bar[b], 1);
-      mbar_init(&kempty_bar[b], Cfg::EPI_WARPS / 2 * Cfg::CTAS);
+      mbar_init(&kempty_bar[b], Cfg::EPI_WARPS * 2);
     }
     mbar_init(drain_bar, 1);
     *s_abort = 0;
     fence_mbar_init();
   }
   if (warp == 1) {
-    tmem_alloc<Cfg::CTAS>(s_tmem_base, 512);
-    tmem_relinquish<Cfg::CTAS>();
+    tmem_alloc<2>(s_tmem_base, 512);
+    tmem_relinquish<2>();
   }
   tc_fence_before();
   __syncthreads();
-  if constexpr (Cfg::kPair) cluster_sync();  // the peer's barriers exist before anyone signals them
+  cluster_sync();  // the peer's barriers exist before anyone signals them
   tc_fence_after();
   const uint32_t tmem_base = *s_tmem_base;
   pdl_wait();
@@ -170,25 +179,18 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
       int stage = 0, issued = 0;
       uint32_t phase = 0;
       bool ok = true;
-      const uint32_t full0 = Cfg::kPair ? mapa_shared(smem_u32(&full_bar[0]), 0) : 0;  // loads complete on the leader's
-      const CUtensorMap* tb = (Cfg::kPair && Cfg::kGate && !leader) ? &tmB2 : &tmB;
+      const uint32_t full0 = mapa_shared(smem_u32(&full_bar[0]), 0);  // both CTAs' loads complete on the leader's
+      const CUtensorMap* tb = (Cfg::kGate && !leader) ? &tmB2 : &tmB;
       for (int u = unit0; u < p.num_units && ok; u += unit_step) {
         const U w = unit(u);
-        const int a_row = (w.tm * Cfg::CTAS + rank) * 128;
+        const int a_row = w.tm * 256 + rank * 128;
         const int b_row = Cfg::kGate ? w.tn * 128 : w.tn * 256 + rank * 128;
         for (int kb = w.kb0; kb < w.kb1; ++kb) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1, s_abort)) { ok = false; break; }
           uint8_t* dst = smem + stage * Cfg::STAGE_BYTES;
-          if constexpr (Cfg::kPair) {
-            if (leader) mbar_arrive_expect_tx(&full_bar[stage], 2 * Cfg::STAGE_BYTES);
-            tma_load_2d_pair(dst, &tmA, full0 + stage * 8, kb * 128, a_row);
-            tma_load_2d_pair(dst + HB, tb, full0 + stage * 8, kb * 128, b_row);
-          } else {
-            mbar_arrive_expect_tx(&full_bar[stage], Cfg::STAGE_BYTES);
-            tma_load_2d(dst, &tmA, &full_bar[stage], kb * 128, a_row);
-            tma_load_2d(dst + HB, &tmB, &full_bar[stage], kb * 128, b_row);
-            if constexpr (Cfg::kGate) tma_load_2d(dst + 2 * HB, &tmB2, &full_bar[stage], kb * 128, b_row);
-          }
+          if (leader) mbar_arrive_expect_tx(&full_bar[stage], 2 * Cfg::STAGE_BYTES);
+          tma_load_2d_pair(dst, &tmA, full0 + stage * 8, kb * 128, a_row);
+          tma_load_2d_pair(dst + HB, tb, full0 + stage * 8, kb * 128, b_row);
           ++issued;
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
@@ -206,44 +208,23 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
         const U w = unit(u);
         for (int kb = w.kb0; kb < w.kb1; ++kb, ++gkb) {
           const int buf = gkb & 1;
-          ok = mbar_wait(&full_bar[stage], phase, s_abort);
-          const uint32_t off = stage * (Cfg::STAGE_BYTES >> 4);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            ok = ok && mbar_wait(&kempty_bar[2 * h + buf], ((gkb >> 1) & 1) ^ 1, s_abort);
-            ok = __all_sync(0xffffffffu, ok);
-            if (!ok) break;
-            tc_fence_after();
-            if (elect_one()) {
-              // half h: rows [64 h, 64 h + 64) of each CTA's 128 weight rows (one CTA: [128 h, 128 h + 128) of 256)
-              const uint32_t d = tmem_base + h * 256 + buf * 128, boff = off + h * (128 / Cfg::CTAS * 128 >> 4);
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                if constexpr (Cfg::kPair)
-                  umma_pair<true>(d, a_desc + off + 2 * k, b_desc + boff + 2 * k, Cfg::IDESC, k > 0);
-                else
-                  umma<true>(d, a_desc + off + 2 * k, b_desc + boff + 2 * k, Cfg::IDESC, k > 0);
-              }
-              if constexpr (Cfg::kPair) {
-                umma_commit_pair(&kfull_bar[2 * h + buf], 0x3);
-                if (h == 1) umma_commit_pair(&empty_bar[stage], 0x3);
-              } else {
-                umma_commit(&kfull_bar[2 * h + buf]);
-                if (h == 1) umma_commit(&empty_bar[stage]);
-              }
-            }
-            __syncwarp();
-          }
+          ok = mbar_wait(&full_bar[stage], phase, s_abort) && mbar_wait(&kempty_bar[buf], ((gkb >> 1) & 1) ^ 1, s_abort);
+          ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
+          tc_fence_after();
+          const uint32_t off = stage * (Cfg::STAGE_BYTES >> 4);
+          if (elect_one()) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              umma_pair<true>(tmem_base + buf * 256, a_desc + off + 2 * k, b_desc + off + 2 * k, Cfg::IDESC, k > 0);
+            umma_commit_pair(&kfull_bar[buf], 0x3);
+            umma_commit_pair(&empty_bar[stage], 0x3);
+          }
+          __syncwarp();
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
       }
-      if (elect_one()) {  // every MMA has completed (in both CTAs) before TMEM is freed
-        if constexpr (Cfg::kPair)
-          umma_commit_pair(drain_bar, 0x3);
-        else
-          umma_commit(drain_bar);
-      }
+      if (elect_one()) umma_commit_pair(drain_bar, 0x3);  // every MMA has completed (in both CTAs) before TMEM is freed
       __syncwarp();
       volatile int never = 0;
       mbar_wait(drain_bar, 0, &never);
@@ -256,14 +237,15 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Cfg::REGS_EPI));
     const int q = warp & 3, wg = (warp - 4) >> 2;
     const int lrow = q * 32 + lane;
-    const WarpTile wt{s_tile + (warp - 4) * 2048, lane};
-    const uint32_t kempty0 = Cfg::kPair ? mapa_shared(smem_u32(&kempty_bar[2 * wg]), 0) : 0;
+    uint8_t* tile = s_tile + (warp - 4) * 8192;
+    const uint32_t kempty0 = mapa_shared(smem_u32(&kempty_bar[0]), 0);
     // group g reads half g: 64 columns of the first weight block (gate), 64 of the second (up)
-    const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + wg * 256;
+    const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
+    const uint32_t run0 = Cfg::kGate ? wg * 64 : wg * 128, run1 = Cfg::kGate ? 128 + wg * 64 : wg * 128 + 64;
     int gkb = 0;
     for (int u = unit0; u < p.num_units; u += unit_step) {
       const U w = unit(u);
-      const int row0 = (w.tm * Cfg::CTAS + rank) * 128 + q * 32;
+      const int row0 = w.tm * 256 + rank * 128 + q * 32;
       float2 acc[64];
 #pragma unroll
       for (int j = 0; j < 64; ++j) acc[j] = make_float2(0.f, 0.f);
@@ -277,10 +259,10 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
       // The scales of four K blocks at a time, fetched four blocks ahead
       const int row = row0 + lane;
       const float* sa = p.a_scale + (size_t)(row < p.M ? row : 0) * KB;
-      const int blk = Cfg::kGate ? w.tn : 2 * w.tn;
+      const int blk0 = Cfg::kGate ? w.tn : 2 * w.tn + wg, blk = blk0 < p.w_blocks ? blk0 : 0;
       const float* sw0 = p.w_scale + (size_t)blk * KB;
       const float* sw1 = Cfg::kGate ? p.w_scale2 + (size_t)blk * KB
-                                    : p.w_scale + (size_t)(blk + 1 < p.w_blocks ? blk + 1 : blk) * KB;
+                                    : sw0;
       const bool quads = p.scale4 && w.kb0 % 4 == 0;  // a slice of K may begin anywhere
       float xa[4], xw[4], xv[4];                       // of the next four blocks
       auto fetch = [&](int kb) {
@@ -304,17 +286,17 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
       fetch(w.kb0);
       // A failed wait has raised the abort flag: the loop then runs out without waiting and
       // the tile is not stored.
-      mbar_wait_soon(&kfull_bar[2 * wg + (gkb & 1)], (gkb >> 1) & 1, s_abort);
+      mbar_wait_soon(&kfull_bar[gkb & 1], (gkb >> 1) & 1, s_abort);
       __syncwarp();
       tc_fence_after();
-      tmem_ld32(t_row + (gkb & 1) * 128, ra);
+      tmem_ld32(t_row + (gkb & 1) * 256 + run0, ra);
 #pragma unroll 1
       for (int kb = w.kb0; kb < w.kb1; kb += 4) {
         float s0[4], s1[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           s0[j] = xa[j] * xw[j];
-          s1[j] = xa[j] * xv[j];
+          s1[j] = Cfg::kGate ? xa[j] * xv[j] : s0[j];
         }
         if (kb + 4 < w.kb1) fetch(kb + 4);
 #pragma unroll
@@ -322,32 +304,27 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
           if (kb + j < w.kb1) {
             const int buf = gkb & 1, nbuf = buf ^ 1;
             const bool more = kb + j + 1 < w.kb1;
-            const uint32_t t0 = t_row + buf * 128, nphase = ((gkb + 1) >> 1) & 1;
-            uint64_t* nbar = &kfull_bar[2 * wg + nbuf];
+            const uint32_t t0 = t_row + buf * 256, nphase = ((gkb + 1) >> 1) & 1;
+            uint64_t* nbar = &kfull_bar[nbuf];
             tmem_ld_wait(ra);
-            tmem_ld32(t0 + 32, rb);
+            tmem_ld32(t0 + run0 + 32, rb);
             add(ra, 0, s0[j]);
             tmem_ld_wait(rb);
-            tmem_ld32(t0 + 64, ra);
+            tmem_ld32(t0 + run1, ra);
             add(rb, 16, s0[j]);
             tmem_ld_wait(ra);
-            tmem_ld32(t0 + 96, rb);
+            tmem_ld32(t0 + run1 + 32, rb);
             const bool early = more && mbar_test(smem_u32(nbar), nphase);
             add(ra, 32, s1[j]);
             tmem_ld_wait(rb);
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) {
-              if constexpr (Cfg::kPair)
-                mbar_arrive_cluster(kempty0 + buf * 8);
-              else
-                mbar_arrive(&kempty_bar[2 * wg + buf]);
-            }
+            if (lane == 0) mbar_arrive_cluster(kempty0 + buf * 8);
             if (more) {
               if (!early) mbar_wait_soon(nbar, nphase, s_abort);
               __syncwarp();
               tc_fence_after();
-              tmem_ld32(t_row + nbuf * 128, ra);
+              tmem_ld32(t_row + nbuf * 256 + run0, ra);
             }
             add(rb, 48, s1[j]);
             ++gkb;
@@ -371,7 +348,8 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
         named_bar_sync(1, 32 * Cfg::EPI_WARPS);
         m = fmaxf(m, s_amax[(wg ^ 1) * 128 + lrow]);
         named_bar_sync(1, 32 * Cfg::EPI_WARPS);
-        const float s = m > 0.f ? m / 448.0f : 1.0f;
+        // an activation times the scale's reciprocal is within an ulp of the quotient
+        const float s = m > 0.f ? m / 448.0f : 1.0f, rs = 1.0f / s;
         uint4 pk[4];
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
@@ -379,30 +357,26 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float* v = a + g * 16 + i * 4;
-            c[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[0] / s, v[1] / s), __NV_SATFINITE, __NV_E4M3) |
-                   ((uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[2] / s, v[3] / s), __NV_SATFINITE, __NV_E4M3) << 16);
+            c[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[0] * rs, v[1] * rs), __NV_SATFINITE, __NV_E4M3) |
+                   ((uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[2] * rs, v[3] * rs), __NV_SATFINITE, __NV_E4M3) << 16);
           }
           pk[g] = make_uint4(c[0], c[1], c[2], c[3]);
         }
-        store_warp<16>(wt, pk, p.codes, row0, p.M, w.tn * 128 + wg * 64, p.N);
+        store_warp<16>(WarpTile{tile, lane}, pk, p.codes, row0, p.M, w.tn * 128 + wg * 64, p.N);
         if (wg == 0 && row < p.M) p.scales[(size_t)row * p.tiles_n + w.tn] = s;
       } else {
         if (!good) break;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int col = w.tn * 256 + (c >> 1) * 128 + wg * 64 + (c & 1) * 32;
-          fp8_block_store32(p, wt, w.split, row0, col, acc + c * 16);
-        }
+        fp8_block_store(p, tile, lane, w.split, row0, w.tn * 256 + wg * 128, reinterpret_cast<const float*>(acc));
       }
     }
   }
 
   tc_fence_before();
   __syncthreads();
-  if constexpr (Cfg::kPair) cluster_sync();  // no CTA leaves while its peer may still signal it
+  cluster_sync();  // no CTA leaves while its peer may still signal it
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc<Cfg::CTAS>(tmem_base, 512);
+    tmem_dealloc<2>(tmem_base, 512);
   }
 }
 
