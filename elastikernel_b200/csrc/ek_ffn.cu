@@ -79,10 +79,10 @@ int map_k(CUtensorMap* m, const void* base, int dtype, int rows, int k, int box_
   const int es = elem_size(dtype);
   return make_tmap_2d(m, base, map_type(dtype), k, rows, (uint64_t)k * es, 128 / es, box_rows);
 }
-// k x cols, the reduction axis outermost (16 bits): both 64-column chunks of a box
-// of 128 columns x 64 of K in one 3-D box where every row holds whole chunks
-int map_mn(CUtensorMap* m, const void* base, int dtype, int k, int cols, int* box3) {
-  *box3 = cols % 64 == 0;
+// k x cols, the reduction axis outermost (16 bits), a box of box_cols (64 or 128) columns x
+// 64 of K: both 64-column chunks of 128 in one 3-D box where every row holds whole chunks
+int map_mn(CUtensorMap* m, const void* base, int dtype, int k, int cols, int box_cols, int* box3) {
+  *box3 = box_cols == 128 && cols % 64 == 0;
   if (*box3) return make_tmap_3d(m, base, map_type(dtype), 64, k, cols / 64, (uint64_t)cols * 2, 128, 64, 64, 2);
   return make_tmap_2d(m, base, map_type(dtype), cols, k, (uint64_t)cols * 2, 64, 64);
 }
@@ -90,30 +90,44 @@ int map_mn(CUtensorMap* m, const void* base, int dtype, int k, int cols, int* bo
 int grid_for(long long work, int sms) { return (int)std::max<long long>(1, std::min<long long>(work, (long long)sms * 8)); }
 
 // ------------------------------------------------------------------ splitting K
-// Slices per tile of a pair kernel: with rounds(s) = ceil(tiles s / pairs) units
-// of k_blocks / s one after the other, each block of K costing t_kb and each unit
-// its fill and its last epilogue (unit_us undivided, kSliceUs as a slice), against
-// the sums' way to memory and back and one more launch. cap: bytes the workspace
-// has for the sums.
-int pick_splits(long long tiles, int k_blocks, int pairs, long long elems, double t_kb, double unit_us, size_t cap) {
-  constexpr double kSliceUs = 2.5, kReduceUs = 3.0, kBytesPerUs = 4.0e6;
-  int best = 1;
+// The schedule of a pair kernel: tile columns and slices of K per tile. A pair runs
+// ceil(tiles slices / pairs) units one after the other; a unit's blocks of K (t_kb each)
+// run beside the epilogue of the unit before it (epi_us, kSliceUs for a slice), so it takes
+// the longer of the two, and the last epilogue stands alone. Against that, the sums' way to
+// memory and back and one more launch. A 128-column tile's block costs 0.7 of a 256-column
+// one's (less to multiply, three quarters to load), its epilogue 0.8. Measured, 333 x 1032 x
+// 2760: dx in 18 tiles of 128 columns cut in 4 takes 12 us, in 10 of 256 cut in 7 15 us;
+// dW1 and dW3, 6 blocks of K, 11.7 us in tiles of 256 and 15.5 in tiles of 128. cap: bytes
+// the workspace has for the sums.
+struct Plan {
+  int bn, splits;
+};
+Plan pick_plan(long long rows, int planes, int cols, int k_blocks, int pairs, long long elems, double t_kb, double epi_us,
+               bool narrow, size_t cap) {
+  constexpr double kSliceUs = 4.0, kReduceUs = 3.0, kBytesPerUs = 4.0e6;
+  Plan best{256, 1};
   double best_us = 1e30;
-  for (int s = 1; s <= 32 && (s == 1 || k_blocks / s >= 4); ++s) {
-    const size_t bytes = (size_t)s * elems * 4;
-    if (s > 1 && bytes > cap) break;
-    const double rounds = std::ceil((double)(tiles * s) / pairs);
-    double us = rounds * std::ceil((double)k_blocks / s) * t_kb + (s > 1 ? kSliceUs : unit_us);
-    if (s > 1) us += kReduceUs + 2.0 * bytes / kBytesPerUs;
-    if (us < 0.95 * best_us) {
-      best_us = us;
-      best = s;
+  for (int bn = 256; bn >= (narrow ? 128 : 256); bn /= 2) {
+    const long long tiles = (long long)ceil_div(rows, 256) * planes * ceil_div(cols, bn);
+    const double kb_us = bn == 256 ? t_kb : 0.7 * t_kb;
+    for (int s = 1; s <= 32 && (s == 1 || k_blocks / s >= 4); ++s) {
+      const size_t bytes = (size_t)s * elems * 4;
+      if (s > 1 && bytes > cap) break;
+      const double epi = (s > 1 ? kSliceUs : epi_us) * (bn == 256 ? 1.0 : 0.8);
+      double us = std::ceil((double)(tiles * s) / pairs) * std::max(std::ceil((double)k_blocks / s) * kb_us, epi) + epi;
+      if (s > 1) us += kReduceUs + 2.0 * bytes / kBytesPerUs;
+      if (us < 0.95 * best_us) {
+        best_us = us;
+        best = Plan{bn, s};
+      }
     }
   }
   return best;
 }
-constexpr double kFfnBlockUs = 0.30, kFp8BlockUs = 0.35;
-constexpr double kStoreUnitUs = 2.5, kGateUnitUs = 4.0, kGateGradUnitUs = 8.0;
+constexpr double kFfnBlockUs = 0.28, kFp8BlockUs = 0.55;
+constexpr double kStoreUs = 4.0, kGateUs = 5.0;
+// gelu's erfc makes the gradient's epilogue three times as long
+constexpr double gate_grad_us(int gate) { return gate == kGateGelu ? 18.0 : 7.0; }
 constexpr size_t kMostSplitBytes = 256u << 20;
 
 // ------------------------------------------------------------------ few tokens
@@ -221,7 +235,7 @@ int stream_gate(int dtype, const void* w1, const void* w3, const void* x, const 
 
 // ------------------------------------------------------------------ 16-bit tiles
 template <class Cfg>
-int launch_ffn(const CUtensorMap (&ta)[2], const CUtensorMap (&tb)[2], FfnParams& p, int sms, cudaStream_t s) {
+int launch_ffn_cfg(const CUtensorMap (&ta)[2], const CUtensorMap (&tb)[2], FfnParams& p, int sms, cudaStream_t s) {
   static bool done[64] = {false};
   const int rc = allow_smem(ffn_gemm_kernel<Cfg>, Cfg::SMEM_BYTES, done);
   if (rc) return rc;
@@ -229,8 +243,8 @@ int launch_ffn(const CUtensorMap (&ta)[2], const CUtensorMap (&tb)[2], FfnParams
   if (units > 0x3fffffff) return set_error(EK_ERR_INVALID, "too many tiles");
   p.num_units = (int)units;
   const int pairs = (int)std::min<long long>(std::max(1, sms / 2), units);
-  return launch("feed-forward product", ffn_gemm_kernel<Cfg>, dim3(2 * pairs), Cfg::THREADS, Cfg::SMEM_BYTES, s, 2,
-                ta[0], ta[1], tb[0], tb[1], p);
+  return launch("feed-forward product", ffn_gemm_kernel<Cfg>, dim3(2 * pairs), Cfg::THREADS, Cfg::SMEM_BYTES, s, 2, ta[0],
+                ta[1], tb[0], tb[1], p);
 }
 
 struct FfnOperand {
@@ -238,84 +252,93 @@ struct FfnOperand {
   int planes;
 };
 
+// The two planes' maps of an operand (one plane: the same map twice), `mn` of it along the
+// result's axis and k along the sum's; box: what a CTA loads of it along mn.
+template <bool kMN>
+int map_operand(CUtensorMap (&t)[2], const FfnOperand& op, int dtype, int mn, int k, int box, int* box3) {
+  for (int i = 0; i < 2; ++i) {
+    const void* base = op.base[op.planes > 1 ? i : 0];
+    const int rc = kMN ? map_mn(&t[i], base, dtype, k, mn, box, box3) : map_k(&t[i], base, dtype, mn, k, box);
+    if (rc) return rc;
+  }
+  return EK_OK;
+}
+
+// Maps and launch of one product: p.M rows (per plane) of p.N columns, k per plane of K.
+template <int kElem, bool kAMN, bool kBMN, int kEpi>
+int launch_ffn(const FfnOperand& A, const FfnOperand& B, int k, int planes_m, int planes_k, const Plan& plan, FfnParams& p,
+               int sms, cudaStream_t s) {
+  CUtensorMap ta[2], tb[2];
+  int rc = map_operand<kAMN>(ta, A, kElem, p.M, k, 128, &p.a_box3);
+  if (rc || (rc = map_operand<kBMN>(tb, B, kElem, p.N, k, plan.bn / 2, &p.b_box3))) return rc;
+  p.m_tiles_plane = ceil_div(p.M, 256);
+  p.tiles_m = p.m_tiles_plane * planes_m;
+  p.tiles_n = ceil_div(p.N, kEpi == kFfnGate ? plan.bn / 2 : plan.bn);
+  p.kb_plane = ceil_div(k, 64);
+  p.k_blocks = p.kb_plane * planes_k;
+  p.splits = plan.splits;
+  return plan.bn == 256 ? launch_ffn_cfg<FfnCfg<kElem, kAMN, kBMN, kEpi, 256>>(ta, tb, p, sms, s)
+                        : launch_ffn_cfg<FfnCfg<kElem, kAMN, kBMN, kEpi, 128>>(ta, tb, p, sms, s);
+}
+
+Plan store_plan(int M, int N, int k, int planes_m, int planes_k, int sms, size_t cap) {
+  return pick_plan(M, planes_m, N, ceil_div(k, 64) * planes_k, std::max(1, sms / 2), (long long)planes_m * M * N,
+                   kFfnBlockUs, kStoreUs, true, cap);
+}
+size_t ffn_store_bytes(int M, int N, int k, int planes_m, int planes_k, int sms) {
+  const int s = store_plan(M, N, k, planes_m, planes_k, sms, kMostSplitBytes).splits;
+  return s > 1 ? (size_t)s * planes_m * M * N * 4 : 0;
+}
+
 // C (planes_m stacked planes) = A . B with K = k per plane. ws holds the sums of a split.
 template <int kElem, bool kAMN, bool kBMN>
 int ffn_store(const FfnOperand& A, const FfnOperand& B, int M, int N, int k, int planes_m, int planes_k, void* C, int sms,
               void* ws, size_t ws_bytes, cudaStream_t s) {
-  CUtensorMap ta[2], tb[2];
   FfnParams p{};
-  for (int i = 0; i < 2; ++i) {
-    const void* a = A.base[A.planes > 1 ? i : 0];
-    const void* b = B.base[B.planes > 1 ? i : 0];
-    int rc = kAMN ? map_mn(&ta[i], a, kElem, k, M, &p.a_box3) : map_k(&ta[i], a, kElem, M, k, 128);
-    if (rc) return rc;
-    rc = kBMN ? map_mn(&tb[i], b, kElem, k, N, &p.b_box3) : map_k(&tb[i], b, kElem, N, k, 128);
-    if (rc) return rc;
-  }
   p.M = M;
   p.N = N;
-  p.m_tiles_plane = ceil_div(M, 256);
-  p.tiles_m = p.m_tiles_plane * planes_m;
-  p.tiles_n = ceil_div(N, 256);
-  p.kb_plane = ceil_div(k, 64);
-  p.k_blocks = p.kb_plane * planes_k;
   p.C = C;
   p.c_plane = (long long)M * N;
   p.ws = static_cast<float*>(ws);
-  const long long elems = (long long)planes_m * M * N;
-  p.splits = pick_splits((long long)p.tiles_m * p.tiles_n, p.k_blocks, std::max(1, sms / 2), elems, kFfnBlockUs,
-                         kStoreUnitUs, ws_bytes);
-  int rc = launch_ffn<FfnCfg<kElem, kAMN, kBMN, kFfnStore>>(ta, tb, p, sms, s);
+  const Plan plan = store_plan(M, N, k, planes_m, planes_k, sms, ws_bytes);
+  const int rc = launch_ffn<kElem, kAMN, kBMN, kFfnStore>(A, B, k, planes_m, planes_k, plan, p, sms, s);
   if (rc || p.splits == 1) return rc;
-  const long long n8 = elems / 8;
+  const long long n8 = (long long)planes_m * M * N / 8;
   return launch("feed-forward sums", ffn_reduce_kernel<kElem>, dim3(grid_for((n8 + 255) / 256, sms)), 256, 0, s, 0,
                 (const float*)p.ws, p.splits, n8, C);
 }
 
-size_t ffn_store_bytes(int M, int N, int k, int planes_m, int planes_k, int sms) {
-  const long long tiles = (long long)ceil_div(M, 256) * planes_m * ceil_div(N, 256), elems = (long long)planes_m * M * N;
-  const int s = pick_splits(tiles, ceil_div(k, 64) * planes_k, std::max(1, sms / 2), elems, kFfnBlockUs,
-                            kStoreUnitUs, kMostSplitBytes);
-  return s > 1 ? (size_t)s * elems * 4 : 0;
-}
-
-int gate_splits(int T, int H, int I, int sms, size_t cap) {
-  return pick_splits((long long)ceil_div(T, 256) * ceil_div(I, 128), ceil_div(H, 64), std::max(1, sms / 2), 2ll * T * I,
-                     kFfnBlockUs, kGateUnitUs, cap);
+// gate/up tiles hold half as many features as columns
+Plan gate_plan(int T, int H, int I, int sms, size_t cap) {
+  return pick_plan(T, 1, 2 * I, ceil_div(H, 64), std::max(1, sms / 2), 2ll * T * I, kFfnBlockUs, kGateUs, true, cap);
 }
 size_t gate_bytes(int T, int H, int I, int sms) {
-  const int s = gate_splits(T, H, I, sms, kMostSplitBytes);
+  const int s = gate_plan(T, H, I, sms, kMostSplitBytes).splits;
   return s > 1 ? (size_t)s * T * I * 8 : 0;
 }
-int gate_grad_splits(int T, int H, int I, int sms, size_t cap) {
-  return pick_splits((long long)ceil_div(T, 256) * ceil_div(I, 256), ceil_div(H, 64), std::max(1, sms / 2),
-                     (long long)T * I, kFfnBlockUs, kGateGradUnitUs, cap);
+Plan gate_grad_plan(int T, int H, int I, int gate, int sms, size_t cap) {
+  return pick_plan(T, 1, I, ceil_div(H, 64), std::max(1, sms / 2), (long long)T * I, kFfnBlockUs,
+                   gate_grad_us(gate), true, cap);
 }
-size_t gate_grad_bytes(int T, int H, int I, int sms) {
-  const int s = gate_grad_splits(T, H, I, sms, kMostSplitBytes);
+size_t gate_grad_bytes(int T, int H, int I, int sms) {  // of any gate function
+  const int s = std::max(gate_grad_plan(T, H, I, kGateSilu, sms, kMostSplitBytes).splits,
+                         gate_grad_plan(T, H, I, kGateGelu, sms, kMostSplitBytes).splits);
   return s > 1 ? (size_t)s * T * I * 4 : 0;
 }
 
 template <int kElem>
 int ffn_gate(const void* x, const void* w1, const void* w3, void* a, void* h, int T, int H, int I, int gate, int sms,
              void* ws, size_t ws_bytes, cudaStream_t s) {
-  CUtensorMap ta[2], tb[2];
-  int rc = map_k(&ta[0], x, kElem, T, H, 128);
-  if (rc || (rc = map_k(&tb[0], w1, kElem, I, H, 128)) || (rc = map_k(&tb[1], w3, kElem, I, H, 128))) return rc;
-  ta[1] = ta[0];
   FfnParams p{};
   p.M = T;
   p.N = I;
-  p.tiles_m = p.m_tiles_plane = ceil_div(T, 256);
-  p.tiles_n = ceil_div(I, 128);
-  p.k_blocks = p.kb_plane = ceil_div(H, 64);
-  p.splits = gate_splits(T, H, I, sms, ws_bytes);
   p.gate = gate;
   p.C = a;
   p.H = h;
   p.h_plane = (long long)T * I;
   p.ws = static_cast<float*>(ws);
-  rc = launch_ffn<FfnCfg<kElem, false, false, kFfnGate>>(ta, tb, p, sms, s);
+  const int rc = launch_ffn<kElem, false, false, kFfnGate>({{x}, 1}, {{w1, w3}, 2}, H, 1, 1,
+                                                           gate_plan(T, H, I, sms, ws_bytes), p, sms, s);
   if (rc || p.splits == 1) return rc;
   return launch("feed-forward gate sums", ffn_gate_reduce_kernel<kElem>, dim3(grid_for(((long long)T * I / 8 + 255) / 256, sms)),
                 256, 0, s, 0, (const float*)p.ws, p.splits, T, I, gate, a, h);
@@ -351,25 +374,18 @@ int gated_ffn_grad(const void* x, const void* w1, const void* w2, const void* w3
   char* a = dh + dh_bytes;
   char* rest = a + a_bytes;
   const size_t rest_bytes = ws_bytes - dh_bytes - a_bytes;
-  CUtensorMap ta[2], tb[2];
   FfnParams p{};
-  int rc = map_k(&ta[0], d_out, kElem, T, H, 128);
-  if (rc || (rc = map_mn(&tb[0], w2, kElem, H, I, &p.b_box3))) return rc;
-  ta[1] = ta[0];
-  tb[1] = tb[0];
   p.M = T;
   p.N = I;
-  p.tiles_m = p.m_tiles_plane = ceil_div(T, 256);
-  p.tiles_n = ceil_div(I, 256);
-  p.k_blocks = p.kb_plane = ceil_div(H, 64);
-  p.splits = gate_grad_splits(T, H, I, sms, rest_bytes);
   p.ws = reinterpret_cast<float*>(rest);
   p.gate = gate;
   p.C = dh;
   p.H = const_cast<void*>(h);
   p.c_plane = p.h_plane = (long long)T * I;
   p.Act = a;
-  if ((rc = launch_ffn<FfnCfg<kElem, false, true, kFfnGateGrad>>(ta, tb, p, sms, s))) return rc;
+  int rc = launch_ffn<kElem, false, true, kFfnGateGrad>({{d_out}, 1}, {{w2}, 1}, H, 1, 1,
+                                                        gate_grad_plan(T, H, I, gate, sms, rest_bytes), p, sms, s);
+  if (rc) return rc;
   if (p.splits > 1 &&
       (rc = launch("feed-forward gate gradient sums", ffn_gate_grad_reduce_kernel<kElem>,
                    dim3(grid_for(((long long)T * I / 8 + 255) / 256, sms)), 256, 0, s, 0, (const float*)p.ws,
@@ -404,8 +420,8 @@ int launch_fp8(const void* a, const void* w, const void* w2, int K, Fp8BlockPara
 }
 
 int fp8_splits(int M, int N, int K, int sms, size_t cap) {
-  return pick_splits((long long)ceil_div(M, 256) * ceil_div(N, 256), ceil_div(K, 128), std::max(1, sms / 2),
-                     (long long)M * N, kFp8BlockUs, kStoreUnitUs, cap);
+  return pick_plan(M, 1, N, ceil_div(K, 128), std::max(1, sms / 2), (long long)M * N, kFp8BlockUs, kStoreUs, false, cap)
+      .splits;
 }
 
 int fp8_store(const void* a, const void* w, const float* as, const float* wsc, void* C, int M, int N, int K, int out_type,

@@ -6,14 +6,14 @@
 //             dx = dh1 W1 + dh3 W3                            (kFfnStore, two K planes)
 //             dW1 = dh1^T x, dW3 = dh3^T x, dW2 = dy^T a      (kFfnStore, A MN-major)
 //
-// A persistent cluster of two CTAs computes a 256 x 256 tile with the 2-SM MMA:
-// each CTA loads its own 128 rows of A and half of the tile's B (32 KB per 64 of
-// K, no multicast) and its TMEM receives its 128 rows. Operands are used where
+// A persistent cluster of two CTAs computes a 256 x 256 (few tiles: 256 x 128) tile
+// with the 2-SM MMA: each CTA loads its own 128 rows of A and half of the tile's B
+// (32 KB per 64 of K, no multicast) and its TMEM receives its 128 rows. Operands are used where
 // they lie: an operand whose reduction axis is not the contiguous one (the
 // weights in a backward pass, everything under a weight's gradient) is read
 // MN-major by the MMA, so nothing is transposed. The two weights of the gate, and
 // the two planes of the pre-activations, are separate tensor maps: a plane is
-// chosen by the rank (gate/up: columns [0, 128) of a tile are W1's, [128, 256)
+// chosen by the rank (gate/up: the first half of a tile's columns is W1's, the second
 // W3's), by the K block (dx sums over both planes) or by the tile's row (dW1 and
 // dW3 are one launch), so no tail of one plane is ever read as the other's.
 //
@@ -79,14 +79,15 @@ __device__ __forceinline__ bool mbar_wait_soon(uint64_t* bar, uint32_t parity, v
 
 enum FfnEpi : int { kFfnStore = 0, kFfnGate = 1, kFfnGateGrad = 2 };
 
-template <int kElem_, bool kAMN_, bool kBMN_, int kEpi_>
+template <int kElem_, bool kAMN_, bool kBMN_, int kEpi_, int BN_>
 struct FfnCfg {
   static constexpr int kElem = kElem_;
   static constexpr bool kAMN = kAMN_, kBMN = kBMN_;  // operand stored with its reduction axis outermost
   static constexpr int kEpi = kEpi_;
-  static constexpr int BN = 256, BK = 64, STAGES = 6;
-  static constexpr int HALF_BYTES = 128 * 128;  // 128 rows (or 64 x 128 columns) of one operand
-  static constexpr int STAGE_BYTES = 2 * HALF_BYTES;
+  static constexpr int BN = BN_, BK = 64;       // tile columns (gate/up: half gate, half up); K per stage
+  static constexpr int A_BYTES = 128 * 128;     // a CTA's 128 rows (MN-major: two chunks of 64 columns) of A
+  static constexpr int B_BYTES = BN / 2 * 128;  // and its half of B
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES, STAGES = BN == 256 ? 6 : 8;
   static constexpr int EPI_WARPS = 8;
   static constexpr int THREADS = 64 + 32 * EPI_WARPS;
   static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_WARPS * 2048 + 1024 + 256;
@@ -260,7 +261,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
     ffn_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CUtensorMap tmA1,
                     const __grid_constant__ CUtensorMap tmB0, const __grid_constant__ CUtensorMap tmB1,
                     const FfnParams p) {
-  constexpr int STAGES = Cfg::STAGES, BN = Cfg::BN, BK = Cfg::BK, HB = Cfg::HALF_BYTES;
+  constexpr int STAGES = Cfg::STAGES, BN = Cfg::BN, BK = Cfg::BK, AB = Cfg::A_BYTES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + STAGES * Cfg::STAGE_BYTES + Cfg::EPI_WARPS * 2048);
@@ -290,7 +291,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
     fence_mbar_init();
   }
   if (warp == 1) {
-    tmem_alloc<2>(s_tmem_base, 512);
+    tmem_alloc<2>(s_tmem_base, 2 * BN);
     tmem_relinquish<2>();
   }
   tc_fence_before();
@@ -314,7 +315,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
       for (int u = unit0; u < p.num_units && ok; u += unit_step) {
         const FfnUnit w = ffn_unit<Cfg>(p, u);
         const int a_mn = w.m_row + rank * 128;
-        const int b_mn = Cfg::kEpi == kFfnGate ? w.tn * 128 : w.tn * BN + rank * 128;
+        const int b_mn = Cfg::kEpi == kFfnGate ? w.tn * (BN / 2) : w.tn * BN + rank * (BN / 2);
         for (int kb = w.kb0; kb < w.kb1; ++kb) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1, s_abort)) { ok = false; break; }
           const int k_plane = kb >= p.kb_plane ? 1 : 0;
@@ -322,7 +323,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
           const CUtensorMap* ta = (k_plane | w.m_plane) ? &tmA1 : &tmA0;
           const CUtensorMap* tb = (Cfg::kEpi == kFfnGate ? rank : k_plane) ? &tmB1 : &tmB0;
           uint8_t* a_dst = smem + stage * Cfg::STAGE_BYTES;
-          uint8_t* b_dst = a_dst + HB;
+          uint8_t* b_dst = a_dst + AB;
           if (leader) mbar_arrive_expect_tx(&full_bar[stage], 2 * Cfg::STAGE_BYTES);
           const uint32_t fb = full0 + stage * 8;
           if constexpr (Cfg::kAMN) {
@@ -330,7 +331,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
               tma_load_3d_pair(a_dst, ta, fb, 0, k0, a_mn / 64);
             } else {
               tma_load_2d_pair(a_dst, ta, fb, a_mn, k0);
-              tma_load_2d_pair(a_dst + HB / 2, ta, fb, a_mn + 64, k0);
+              tma_load_2d_pair(a_dst + AB / 2, ta, fb, a_mn + 64, k0);
             }
           } else {
             tma_load_2d_pair(a_dst, ta, fb, k0, a_mn);
@@ -340,7 +341,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
               tma_load_3d_pair(b_dst, tb, fb, 0, k0, b_mn / 64);
             } else {
               tma_load_2d_pair(b_dst, tb, fb, b_mn, k0);
-              tma_load_2d_pair(b_dst + HB / 2, tb, fb, b_mn + 64, k0);
+              if constexpr (BN == 256) tma_load_2d_pair(b_dst + Cfg::B_BYTES / 2, tb, fb, b_mn + 64, k0);
             }
           } else {
             tma_load_2d_pair(b_dst, tb, fb, k0, b_mn);
@@ -360,7 +361,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
       // MN-major: 16 rows of K are 2 KB on, the 64-column chunks BK * 128 bytes apart
       constexpr uint32_t a_step = Cfg::kAMN ? 2048 >> 4 : 32 >> 4, b_step = Cfg::kBMN ? 2048 >> 4 : 32 >> 4;
       const uint64_t a_desc = umma_desc_sw128(smem_u32(smem), Cfg::kAMN ? BK * 128 : 16, 1024);
-      const uint64_t b_desc = umma_desc_sw128(smem_u32(smem) + HB, Cfg::kBMN ? BK * 128 : 16, 1024);
+      const uint64_t b_desc = umma_desc_sw128(smem_u32(smem) + AB, Cfg::kBMN ? BK * 128 : 16, 1024);
       for (int u = unit0; u < p.num_units && ok; u += unit_step, ++acc_i) {
         const FfnUnit w = ffn_unit<Cfg>(p, u);
         const int buf = acc_i & 1;
@@ -415,7 +416,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
       auto fetch_h = [&](int c) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const long long at = warp_at<8>(i, lane, row0, p.M, w.tn * BN + half * 128 + c * 32, p.N, p.N);
+          const long long at = warp_at<8>(i, lane, row0, p.M, w.tn * BN + half * (BN / 2) + c * 32, p.N, p.N);
           const uint16_t* h = reinterpret_cast<const uint16_t*>(p.H);
           n1[i] = at >= 0 ? __ldg(reinterpret_cast<const uint4*>(h + at)) : make_uint4(0, 0, 0, 0);
           n3[i] = at >= 0 ? __ldg(reinterpret_cast<const uint4*>(h + p.h_plane + at)) : make_uint4(0, 0, 0, 0);
@@ -428,15 +429,15 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buf * BN;
       if constexpr (Cfg::kEpi == kFfnGate) {
 #pragma unroll 1
-        for (int c = 0; c < 2; ++c) {
-          const int f0 = half * 64 + c * 32;  // feature within the tile's 128
+        for (int c = 0; c < BN / 128; ++c) {
+          const int f0 = half * (BN / 4) + c * 32;  // feature within the tile's BN / 2
           uint32_t rg[32], ru[32];
           tmem_ld32(t_row + f0, rg);
-          tmem_ld32(t_row + 128 + f0, ru);
+          tmem_ld32(t_row + BN / 2 + f0, ru);
           tmem_ld_wait(rg);
           reg_dep(ru);
-          if (c == 1) release(buf);
-          const int col = w.tn * 128 + f0;
+          if (c == BN / 128 - 1) release(buf);
+          const int col = w.tn * (BN / 2) + f0;
           if (split) {
             float* out = p.ws + (size_t)w.split * p.M * (2ll * p.N);
             store_warp32(wt, rg, out, row0, p.M, col, p.N, 2ll * p.N);
@@ -460,12 +461,12 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
         }
       } else {
 #pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          const int c0 = half * 128 + c * 32, col = w.tn * BN + c0;
+        for (int c = 0; c < BN / 64; ++c) {
+          const int c0 = half * (BN / 2) + c * 32, col = w.tn * BN + c0;
           uint32_t r[32];
           tmem_ld32(t_row + c0, r);
           tmem_ld_wait(r);
-          if (c == 3) release(buf);
+          if (c == BN / 64 - 1) release(buf);
           if (split) {
             const int planes = p.tiles_m / p.m_tiles_plane;
             store_warp32(wt, r, p.ws + (size_t)(w.split * planes + w.m_plane) * p.M * p.N, row0, p.M, col, p.N, p.N);
@@ -486,7 +487,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
             __syncwarp();
 #pragma unroll
             for (int j = 0; j < 4; ++j) h3[j] = wt.own(j);
-            if (c < 3) fetch_h(c + 1);
+            if (c + 1 < BN / 64) fetch_h(c + 1);
             with_gate(p.gate, [&](auto fn) {
 #pragma unroll
               for (int g = 0; g < 4; ++g) {
@@ -516,7 +517,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
   cluster_sync();  // no CTA leaves while its peer may still signal it
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc<2>(tmem_base, 512);
+    tmem_dealloc<2>(tmem_base, 2 * BN);
   }
 }
 
