@@ -188,49 +188,55 @@ struct StreamScales {
   const float *tok = nullptr, *w = nullptr, *w2 = nullptr;
 };
 
-// out[t, n] = x[t] . w[n]
-int stream_store(int dtype, const void* w, const void* x, const StreamScales& sc, int T, int N, int K, void* out,
-                 int out_type, int sms, void* ws, size_t ws_bytes, cudaStream_t s, bool early) {
+// The product of weight rows w (gate: w and w2) with the tokens x and what follows it, o.
+template <bool kGate>
+int stream_product(int dtype, const void* w, const void* w2, const void* x, const StreamScales& sc, int K,
+                   const StreamOut& o, int sms, void* ws, size_t ws_bytes, cudaStream_t s, bool early) {
   StreamParams p{};
+  p.sp = stream_split(o.N, kGate ? 128 : 256, K, 128 / elem_size(dtype), sms);
+  if (ws_bytes < stream_bytes(p.sp, o.T)) return set_error(EK_ERR_INVALID, "workspace too small");
   p.early = early;
-  p.sp = stream_split(N, 256, K, 128 / elem_size(dtype), sms);
-  if (ws_bytes < stream_bytes(p.sp, T)) return set_error(EK_ERR_INVALID, "workspace too small");
-  p.T = T;
-  p.tok_scale = sc.tok;
-  p.w_scale = sc.w;
-  p.w_blocks = ceil_div(N, 128);
-  p.ws = static_cast<float*>(ws);
-  int rc = dtype == EK_DTYPE_BF16 ? launch_stream_nt<kBF16, false>(w, w, x, N, K, p, s)
-           : dtype == EK_DTYPE_FP16 ? launch_stream_nt<kFP16, false>(w, w, x, N, K, p, s)
-                                    : launch_stream_nt<kE4M3, false>(w, w, x, N, K, p, s);
-  if (rc) return rc;
-  const int ways = stream_ways(p.sp, T, 2 * p.sp.tiles, sms);
-  const int wide = aligned16(out) && N % 4 == 0;
-  return launch("stream sums", stream_store_reduce_kernel, dim3(2 * p.sp.tiles, ceil_div(T, 8 / ways)), 256, 0, s, 0,
-                p.sp, (const float*)p.ws, T, N, out, out_type, wide, ways);
-}
-
-// a[t, i] = f(x[t] . w1[i]) (x[t] . w3[i]); e4m3: codes and scales of a
-int stream_gate(int dtype, const void* w1, const void* w3, const void* x, const StreamScales& sc, int T, int I, int H,
-                int gate, void* a, void* h, uint8_t* codes, float* scales, int sms, void* ws, size_t ws_bytes,
-                cudaStream_t s, bool early) {
-  StreamParams p{};
-  p.early = early;
-  p.sp = stream_split(I, 128, H, 128 / elem_size(dtype), sms);
-  if (ws_bytes < stream_bytes(p.sp, T)) return set_error(EK_ERR_INVALID, "workspace too small");
-  p.T = T;
+  p.T = o.T;
   p.tok_scale = sc.tok;
   p.w_scale = sc.w;
   p.w_scale2 = sc.w2;
-  p.w_blocks = ceil_div(I, 128);
+  p.w_blocks = ceil_div(o.N, 128);
   p.ws = static_cast<float*>(ws);
-  int rc = dtype == EK_DTYPE_BF16 ? launch_stream_nt<kBF16, true>(w1, w3, x, I, H, p, s)
-           : dtype == EK_DTYPE_FP16 ? launch_stream_nt<kFP16, true>(w1, w3, x, I, H, p, s)
-                                    : launch_stream_nt<kE4M3, true>(w1, w3, x, I, H, p, s);
+  const int rc = dtype == EK_DTYPE_BF16 ? launch_stream_nt<kBF16, kGate>(w, w2, x, o.N, K, p, s)
+                 : dtype == EK_DTYPE_FP16 ? launch_stream_nt<kFP16, kGate>(w, w2, x, o.N, K, p, s)
+                                          : launch_stream_nt<kE4M3, kGate>(w, w2, x, o.N, K, p, s);
   if (rc) return rc;
-  const int ways = stream_ways(p.sp, T, p.sp.tiles, sms);
-  return launch("stream gate", stream_gate_reduce_kernel, dim3(p.sp.tiles, ceil_div(T, 8 / ways)), 256, 0, s, 0, p.sp,
-                (const float*)p.ws, T, I, gate, dtype, a, h, codes, scales, ways);
+  const int row_tiles = kGate ? p.sp.tiles : 2 * p.sp.tiles, ways = stream_ways(p.sp, o.T, row_tiles, sms);
+  return launch("stream sums", kGate ? stream_gate_reduce_kernel : stream_store_reduce_kernel,
+                dim3(row_tiles, ceil_div(o.T, 8 / ways)), 256, 0, s, 0, p.sp, (const float*)p.ws, o, ways);
+}
+
+// out[t, n] = x[t] . w[n]
+int stream_store(int dtype, const void* w, const void* x, const StreamScales& sc, int T, int N, int K, void* out,
+                 int out_type, int sms, void* ws, size_t ws_bytes, cudaStream_t s, bool early) {
+  StreamOut o{};
+  o.T = T;
+  o.N = N;
+  o.out = out;
+  o.type = out_type;
+  o.wide = aligned16(out) && N % 4 == 0;
+  return stream_product<false>(dtype, w, w, x, sc, K, o, sms, ws, ws_bytes, s, early);
+}
+
+// a[t, i] = f(x[t] . w1[i]) (x[t] . w3[i]); with codes, those and scales of a
+int stream_gate(int dtype, const void* w1, const void* w3, const void* x, const StreamScales& sc, int T, int I, int H,
+                int gate, void* a, void* h, uint8_t* codes, float* scales, int sms, void* ws, size_t ws_bytes,
+                cudaStream_t s, bool early) {
+  StreamOut o{};
+  o.T = T;
+  o.N = I;
+  o.out = a;
+  o.type = dtype;
+  o.gate = gate;
+  o.h = h;
+  o.codes = codes;
+  o.scales = scales;
+  return stream_product<true>(dtype, w1, w3, x, sc, H, o, sms, ws, ws_bytes, s, early);
 }
 
 // ------------------------------------------------------------------ 16-bit tiles

@@ -19,6 +19,12 @@
 //   warp 0  TMA producer; warp 1  TMEM and MMA; warp 2  scales (e4m3)
 //   warps 3..10  epilogue: two per TMEM lane quarter, one 128-row block each
 //
+// A tile cut over a cluster instead, its parts added over distributed shared memory in the
+// same launch, was tried and left out: an SM draws about 46 GB/s, so what counts is that
+// all of them stream, and whole tiles over clusters of 4 and 8 leave too many without work
+// (16 tokens through 7168 x 2048 in 8 bits 22.4 us, 64 through 4096 x 14336 23.7 us, against
+// 18.4 and 19.3).
+//
 // Launches overlap (programmatic dependent launch): within a call a CTA fills its
 // stages with weights before it waits; everything else is read and written after.
 #pragma once
@@ -34,9 +40,9 @@ struct StreamCfg {
   static constexpr bool kGate = kGate_, kF8 = kElem == kE4M3;
   static constexpr int BK = kF8 ? 128 : 64, KSTEPS = 4;
   static constexpr int A_BYTES = 256 * 128, B_BYTES = NT * 128, STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr int SLOTS = 8;          // K blocks of scales in flight
-  static constexpr int SLOT_STRIDE = NT + 4;  // token scales, then the two row blocks'
-  static constexpr int SCALE_BYTES = kF8 ? SLOTS * SLOT_STRIDE * 4 : 0;
+  // scales: slots of SGROUP K blocks, each the tokens' scales and then the two row blocks'
+  static constexpr int SLOTS = 3, SGROUP = 4, SLOT_STRIDE = NT + 4;
+  static constexpr int SCALE_BYTES = kF8 ? SLOTS * SGROUP * SLOT_STRIDE * 4 : 0;
   static constexpr int STAGES_FIT = (224 * 1024 - SCALE_BYTES - 512) / STAGE_BYTES;
   static constexpr int STAGES = STAGES_FIT > 6 ? 6 : STAGES_FIT;
   static constexpr int TMEM_COLS = 4 * NT;  // two buffers of two accumulators
@@ -47,6 +53,85 @@ struct StreamCfg {
   static constexpr int CHUNK = NT < 32 || (kF8 && NT == 128) ? 16 : 32;  // 128 accumulators leave room for 16
   static_assert(NT == 16 || NT == 32 || NT == 64 || NT == 128, "token tile");
 };
+
+enum OutType : int { kOutBF16 = 0, kOutFP16 = 1, kOutFP32 = 3 };
+
+__device__ __forceinline__ void store_out(void* out, int type, size_t at, float v) {
+  if (type == kOutBF16)
+    reinterpret_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(v);
+  else if (type == kOutFP16)
+    reinterpret_cast<__half*>(out)[at] = __float2half_rn(v);
+  else
+    reinterpret_cast<float*>(out)[at] = v;
+}
+
+// 4 consecutive values, `n` of them inside the row; wide: whole and aligned
+__device__ __forceinline__ void store_out4(void* out, int type, size_t at, const float4& v, int n, bool wide) {
+  if (wide && n >= 4) {
+    if (type == kOutFP32) {
+      *reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + at) = v;
+    } else {
+      uint2 pk;
+      pk.x = type == kOutBF16 ? Elem16<kBF16>::pack(v.x, v.y) : Elem16<kFP16>::pack(v.x, v.y);
+      pk.y = type == kOutBF16 ? Elem16<kBF16>::pack(v.z, v.w) : Elem16<kFP16>::pack(v.z, v.w);
+      *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(out) + at) = pk;
+    }
+    return;
+  }
+  const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (i < n) store_out(out, type, at + i, e[i]);
+}
+
+__device__ __forceinline__ void add4(float4& a, const float4& b) {
+  a.x += b.x;
+  a.y += b.y;
+  a.z += b.z;
+  a.w += b.w;
+}
+
+// What follows the sums. Plain: 4 values of token t from row n on.
+struct StreamOut {
+  int T, N;            // tokens; rows of the weight (gate: features)
+  void* out;           // plain: the result; gate: a (or null)
+  int type, wide;      // OutType; rows of the result take whole 16-byte stores
+  int gate;            // GateFn
+  void* h;             // gate: the pre-activations (or null)
+  uint8_t* codes;      // gate: a in e4m3 and its scales instead of a
+  float* scales;
+};
+
+// a[t, f] = f(h1) h3 for 4 features a lane, from feature f on, and h1 and h3 on request;
+// with codes, a in e4m3 with the scale of the warp's 128 features (largest magnitude / 448,
+// 1 for zeros). Rows past the weight's hold zeros.
+__device__ __forceinline__ void finish_gate(const StreamOut& o, int t, int tile, const float4& h1, const float4& h3) {
+  const int f = tile * 128 + (threadIdx.x & 31) * 4, I = o.N;
+  float4 act;
+  with_gate(o.gate, [&](auto fn) {
+    constexpr int F = decltype(fn)::value;
+    act = make_float4(gate_f<F>(h1.x) * h3.x, gate_f<F>(h1.y) * h3.y, gate_f<F>(h1.z) * h3.z, gate_f<F>(h1.w) * h3.w);
+  });
+  const size_t at = (size_t)t * I + f;
+  if (o.codes == nullptr) {
+    store_out4(o.out, o.type, at, act, I - f, true);
+    if (o.h != nullptr) {
+      store_out4(o.h, o.type, at, h1, I - f, true);
+      store_out4(o.h, o.type, (size_t)o.T * I + at, h3, I - f, true);
+    }
+    return;
+  }
+  float m = fmaxf(fmaxf(fabsf(act.x), fabsf(act.y)), fmaxf(fabsf(act.z), fabsf(act.w)));  // zeros past I
+#pragma unroll
+  for (int i = 16; i; i >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, i));
+  const float s = m > 0.f ? m / 448.0f : 1.0f;
+  if (f < I) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(act.x / s, act.y / s), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(act.z / s, act.w / s), __NV_SATFINITE, __NV_E4M3);
+    *reinterpret_cast<uint32_t*>(o.codes + at) = lo | (hi << 16);
+  }
+  if ((threadIdx.x & 31) == 0) o.scales[(size_t)t * ((I + 127) / 128) + tile] = s;
+}
 
 // How the units are dealt out; the reducing launch reads it too.
 struct StreamSplit {
@@ -71,7 +156,7 @@ template <class Cfg>
 __global__ void __launch_bounds__(Cfg::THREADS, 1)
     stream_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmW2,
                   const __grid_constant__ CUtensorMap tmX, const StreamParams p) {
-  constexpr int STAGES = Cfg::STAGES, NT = Cfg::NT, CH = Cfg::CHUNK, NS = Cfg::SLOTS, RS = Cfg::SLOT_STRIDE;
+  constexpr int STAGES = Cfg::STAGES, NT = Cfg::NT, CH = Cfg::CHUNK, NS = Cfg::SLOTS, SG = Cfg::SGROUP, RS = Cfg::SLOT_STRIDE;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* s_scale = reinterpret_cast<float*>(smem + STAGES * Cfg::STAGE_BYTES);
@@ -194,19 +279,21 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
   } else if (warp == 2) {
     if constexpr (Cfg::kF8) {
       pdl_wait();
-      for (int u = u0; u < u1; ++u) {
-        const int g = u - u0, slot = g % NS;
+      for (int u = u0, g = 0; u < u1; u += SG, ++g) {
+        const int slot = g % NS;
         const bool ok = mbar_wait(&sempty_bar[slot], ((g / NS) & 1) ^ 1, s_abort);
         if (__any_sync(0xffffffffu, !ok)) break;
-        const int tile = u / KB, kb = u - tile * KB;
-        float* dst = s_scale + slot * RS;
-        for (int t = lane; t < NT; t += 32)
-          cp_async_4_zfill(dst + t, t < p.T ? p.tok_scale + (size_t)t * KB + kb : p.tok_scale, t < p.T ? 4 : 0);
-        if (lane < 2) {
-          const int blk = Cfg::kGate ? tile : 2 * tile + lane;
-          const float* src = Cfg::kGate && lane ? p.w_scale2 : p.w_scale;
-          cp_async_4_zfill(dst + NT + lane, blk < p.w_blocks ? src + (size_t)blk * KB + kb : src,
-                           blk < p.w_blocks ? 4 : 0);
+        for (int j = 0; j < SG && u + j < u1; ++j) {
+          const int tile = (u + j) / KB, kb = u + j - tile * KB;
+          float* dst = s_scale + (slot * SG + j) * RS;
+          for (int t = lane; t < NT; t += 32)
+            cp_async_4_zfill(dst + t, t < p.T ? p.tok_scale + (size_t)t * KB + kb : p.tok_scale, t < p.T ? 4 : 0);
+          if (lane < 2) {
+            const int blk = Cfg::kGate ? tile : 2 * tile + lane;
+            const float* src = Cfg::kGate && lane ? p.w_scale2 : p.w_scale;
+            cp_async_4_zfill(dst + NT + lane, blk < p.w_blocks ? src + (size_t)blk * KB + kb : src,
+                             blk < p.w_blocks ? 4 : 0);
+          }
         }
         cp_async_mbar_arrive(&sfull_bar[slot]);
       }
@@ -223,7 +310,14 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&tempty_bar[buf]);
     };
-    int flush = 0, seg = 0;
+    auto load = [](uint32_t(&r)[32], uint32_t at) {
+      if constexpr (CH == 32)
+        tmem_ld32(at, r);
+      else
+        tmem_ld16(at, r);
+    };
+    int flush = 0, seg = 0, slot = 0;
+    uint32_t sphase = 0;
     for (int u = u0; u < u1;) {
       const int tile_end = min(u1, (u / KB + 1) * KB);
       float* out = p.ws + ((size_t)(blockIdx.x * p.sp.max_segs + seg) * p.T) * 256 + n0;
@@ -232,42 +326,49 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
         float2 acc[NT / 2];
 #pragma unroll
         for (int j = 0; j < NT / 2; ++j) acc[j] = make_float2(0.f, 0.f);
+        // A failed wait has raised the abort flag: the loop then runs out without waiting and
+        // nothing is written. A chunk of columns is in flight while the one before is added;
+        // columns past the tokens are added too, and never used.
         for (; u < tile_end; ++u, ++flush) {
-          const int buf = flush & 1, slot = flush % NS;
-          const bool got = mbar_wait(&tfull_bar[buf], (flush >> 1) & 1, s_abort) &&
-                           mbar_wait(&sfull_bar[slot], (flush / NS) & 1, s_abort);
-          good = __all_sync(0xffffffffu, got);
-          if (!good) break;
-          tc_fence_after();
-          const float* xs = s_scale + slot * RS;
+          const int buf = flush & 1, j = (u - u0) % SG;
+          if (j == 0) mbar_wait_soon(&sfull_bar[slot], sphase, s_abort);
+          const float* xs = s_scale + (slot * SG + j) * RS;
           const float ws = xs[NT + rb];
+          mbar_wait_soon(&tfull_bar[buf], (flush >> 1) & 1, s_abort);
+          __syncwarp();
+          tc_fence_after();
+          constexpr int C = NT / CH;
+          uint32_t r[2][32];
+          load(r[0], lane_base + buf * 2 * NT);
 #pragma unroll
-          for (int c = 0; c < NT / CH; ++c) {
-            if (c * CH >= p.n) break;
-            uint32_t r[32];
-            if constexpr (CH == 32)
-              tmem_ld32(lane_base + buf * 2 * NT + c * CH, r);
-            else
-              tmem_ld16(lane_base + buf * 2 * NT + c * CH, r);
-            tmem_ld_wait(r);
+          for (int c = 0; c < C; ++c) {
+            tmem_ld_wait(r[c & 1]);
+            if (c + 1 < C) {
+              load(r[(c + 1) & 1], lane_base + buf * 2 * NT + (c + 1) * CH);
+            } else {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&tempty_bar[buf]);
+            }
             const float4* xs4 = reinterpret_cast<const float4*>(xs + c * CH);
+            const uint32_t(&v)[32] = r[c & 1];
 #pragma unroll
-            for (int j = 0; j < CH / 4; ++j) {
-              const float4 s = xs4[j];
-              float2* a = acc + (c * CH + 4 * j) / 2;
-              a[0] = fma2(make_float2(__uint_as_float(r[4 * j]), __uint_as_float(r[4 * j + 1])),
-                          mul2(make_float2(s.x, s.y), make_float2(ws, ws)), a[0]);
-              a[1] = fma2(make_float2(__uint_as_float(r[4 * j + 2]), __uint_as_float(r[4 * j + 3])),
-                          mul2(make_float2(s.z, s.w), make_float2(ws, ws)), a[1]);
+            for (int i = 0; i < CH / 4; ++i) {
+              const float4 x = xs4[i];
+              float2* a = acc + (c * CH + 4 * i) / 2;
+              a[0] = fma2(make_float2(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1])),
+                          mul2(make_float2(x.x, x.y), make_float2(ws, ws)), a[0]);
+              a[1] = fma2(make_float2(__uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3])),
+                          mul2(make_float2(x.z, x.w), make_float2(ws, ws)), a[1]);
             }
           }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(&tempty_bar[buf]);
-            mbar_arrive(&sempty_bar[slot]);
+          if (j == SG - 1 || u + 1 == u1) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sempty_bar[slot]);
+            if (++slot == NS) { slot = 0; sphase ^= 1; }
           }
         }
+        good = !__any_sync(0xffffffffu, *s_abort);
         if (!good) break;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
@@ -281,10 +382,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
 #pragma unroll 1
         for (int c = 0; c < chunks; ++c) {
           uint32_t r[32];
-          if constexpr (CH == 32)
-            tmem_ld32(lane_base + buf * 2 * NT + c * CH, r);
-          else
-            tmem_ld16(lane_base + buf * 2 * NT + c * CH, r);
+          load(r, lane_base + buf * 2 * NT + c * CH);
           tmem_ld_wait(r);
           if (c == chunks - 1) release(buf);
 #pragma unroll
@@ -307,43 +405,6 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
 }
 
 // ------------------------------------------------------------ adding the segments
-enum OutType : int { kOutBF16 = 0, kOutFP16 = 1, kOutFP32 = 3 };
-
-__device__ __forceinline__ void store_out(void* out, int type, size_t at, float v) {
-  if (type == kOutBF16)
-    reinterpret_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(v);
-  else if (type == kOutFP16)
-    reinterpret_cast<__half*>(out)[at] = __float2half_rn(v);
-  else
-    reinterpret_cast<float*>(out)[at] = v;
-}
-
-// 4 consecutive values, `n` of them inside the row; wide: whole and aligned
-__device__ __forceinline__ void store_out4(void* out, int type, size_t at, const float4& v, int n, bool wide) {
-  if (wide && n >= 4) {
-    if (type == kOutFP32) {
-      *reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + at) = v;
-    } else {
-      uint2 pk;
-      pk.x = type == kOutBF16 ? Elem16<kBF16>::pack(v.x, v.y) : Elem16<kFP16>::pack(v.x, v.y);
-      pk.y = type == kOutBF16 ? Elem16<kBF16>::pack(v.z, v.w) : Elem16<kFP16>::pack(v.z, v.w);
-      *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(out) + at) = pk;
-    }
-    return;
-  }
-  const float e[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (i < n) store_out(out, type, at + i, e[i]);
-}
-
-__device__ __forceinline__ void add4(float4& a, const float4& b) {
-  a.x += b.x;
-  a.y += b.y;
-  a.z += b.z;
-  a.w += b.w;
-}
-
 // A warp of a block of 8 sums 128 rows of a tile for one token, four rows a lane
 // (kN = 2: a second 128 rows beside them, the up rows of a gate tile). `ways` warps
 // share a token's segments, each taking every ways-th; their sums are added in
@@ -393,57 +454,27 @@ __device__ __forceinline__ bool stream_sum(const StreamSplit& sp, const float* _
   return way == 0 && t < T;
 }
 
-// out[t, n] of a plain product; blockIdx.x: half tiles of 128 rows
-__global__ void __launch_bounds__(256) stream_store_reduce_kernel(const StreamSplit sp, const float* __restrict__ ws,
-                                                                  int T, int N, void* __restrict__ out, int type,
-                                                                  int wide, int ways) {
+// A plain product's result; blockIdx.x: half tiles of 128 rows
+__global__ void __launch_bounds__(256)
+    stream_store_reduce_kernel(const StreamSplit sp, const float* __restrict__ ws, const StreamOut o, int ways) {
   pdl_launch();
   pdl_wait();
   const int tile = blockIdx.x >> 1, row = (blockIdx.x & 1) * 128;
   const int t = blockIdx.y * (8 / ways) + (threadIdx.x >> 5) / ways;
   const int n = tile * 256 + row + (threadIdx.x & 31) * 4;
   float4 v[1];
-  if (stream_sum<1>(sp, ws, T, tile, t, row, ways, v)) store_out4(out, type, (size_t)t * N + n, v[0], N - n, wide);
+  if (stream_sum<1>(sp, ws, o.T, tile, t, row, ways, v))
+    store_out4(o.out, o.type, (size_t)t * o.N + n, v[0], o.N - n, o.wide);
 }
 
-// a[t, f] = f(h1) h3 of the gate/up pair, h1 and h3 on request. codes != null: a in
-// e4m3 with the scale of the warp's 128 features (largest magnitude / 448, 1 for
-// zeros) instead. I is a multiple of 4.
+// A gate/up pair's
 __global__ void __launch_bounds__(256)
-    stream_gate_reduce_kernel(const StreamSplit sp, const float* __restrict__ ws, int T, int I, int gate, int type,
-                              void* __restrict__ a, void* __restrict__ h, uint8_t* __restrict__ codes,
-                              float* __restrict__ scales, int ways) {
+    stream_gate_reduce_kernel(const StreamSplit sp, const float* __restrict__ ws, const StreamOut o, int ways) {
   pdl_launch();
   pdl_wait();
-  const int tile = blockIdx.x, t = blockIdx.y * (8 / ways) + (threadIdx.x >> 5) / ways;
-  const int f = tile * 128 + (threadIdx.x & 31) * 4;
+  const int t = blockIdx.y * (8 / ways) + (threadIdx.x >> 5) / ways;
   float4 v[2];
-  if (!stream_sum<2>(sp, ws, T, tile, t, 0, ways, v)) return;  // rows past I hold zeros
-  float4 act;
-  with_gate(gate, [&](auto fn) {
-    constexpr int F = decltype(fn)::value;
-    act = make_float4(gate_f<F>(v[0].x) * v[1].x, gate_f<F>(v[0].y) * v[1].y, gate_f<F>(v[0].z) * v[1].z,
-                      gate_f<F>(v[0].w) * v[1].w);
-  });
-  const size_t at = (size_t)t * I + f;
-  if (codes == nullptr) {
-    store_out4(a, type, at, act, I - f, true);
-    if (h != nullptr) {
-      store_out4(h, type, at, v[0], I - f, true);
-      store_out4(h, type, (size_t)T * I + at, v[1], I - f, true);
-    }
-    return;
-  }
-  float m = fmaxf(fmaxf(fabsf(act.x), fabsf(act.y)), fmaxf(fabsf(act.z), fabsf(act.w)));  // zeros past I
-#pragma unroll
-  for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const float s = m > 0.f ? m / 448.0f : 1.0f;
-  if (f < I) {
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(act.x / s, act.y / s), __NV_SATFINITE, __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(act.z / s, act.w / s), __NV_SATFINITE, __NV_E4M3);
-    *reinterpret_cast<uint32_t*>(codes + at) = lo | (hi << 16);
-  }
-  if ((threadIdx.x & 31) == 0) scales[(size_t)t * ((I + 127) / 128) + tile] = s;
+  if (stream_sum<2>(sp, ws, o.T, blockIdx.x, t, 0, ways, v)) finish_gate(o, t, blockIdx.x, v[0], v[1]);
 }
 
 // e4m3 codes [T][H] and scales [T][ceil(H / 128)] of bf16 rows: a scale per 128 elements
