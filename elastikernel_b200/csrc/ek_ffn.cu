@@ -369,6 +369,47 @@ int gated_ffn(const void* x, const void* w1, const void* w2, const void* w3, voi
   return ffn_store<kElem, false, false>({{a}, 1}, {{w2}, 1}, T, H, I, 1, 1, y, sms, rest, rest_bytes, s);
 }
 
+// Tile columns and dx's slices for the gradient's three products in one launch: the pairs
+// share the units' time (a unit: its blocks, or the epilogue beside them), but not less than
+// dx's own rounds.
+Plan grads_plan(int T, int H, int I, int sms, size_t cap) {
+  const int pairs = std::max(1, sms / 2), kb_x = 2 * ceil_div(I, 64), kb_w = ceil_div(T, 64);
+  Plan best{256, 1};
+  double best_us = 1e30;
+  for (int bn = 256; bn >= 128; bn /= 2) {
+    const double kb_us = bn == 256 ? kFfnBlockUs : 0.7 * kFfnBlockUs, epi = bn == 256 ? kStoreUs : 0.8 * kStoreUs;
+    const double n_w = 2.0 * ceil_div(I, 256) * ceil_div(H, bn) + (double)ceil_div(H, 256) * ceil_div(I, bn);
+    const double t_w = std::max(kb_w * kb_us, epi);
+    for (int s = 1; s <= 32 && (s == 1 || kb_x / s >= 4); ++s) {
+      const size_t bytes = (size_t)s * T * H * 4;
+      if (s > 1 && bytes > cap) break;
+      const double n_x = (double)ceil_div(T, 256) * ceil_div(H, bn) * s, t_x = std::max(ceil_div(kb_x, s) * kb_us, epi);
+      double us = std::max(std::ceil(n_x / pairs) * t_x, (n_x * t_x + n_w * t_w) / pairs + 0.5 * t_w) + epi;
+      if (s > 1) us += 3.0 + 2.0 * bytes / 4.0e6;
+      if (us < 0.97 * best_us) {
+        best_us = us;
+        best = Plan{bn, s};
+      }
+    }
+  }
+  return best;
+}
+size_t grads_bytes(int T, int H, int I, int sms) {
+  const int s = grads_plan(T, H, I, sms, kMostSplitBytes).splits;
+  return s > 1 ? (size_t)s * T * H * 4 : 0;
+}
+
+template <int kElem, int kBN>
+int launch_grads(FfnGradMaps& m, FfnGradParams& p, int sms, cudaStream_t s) {
+  using Cfg = FfnCfg<kElem, false, true, kFfnStore, kBN>;
+  static bool done[64] = {false};
+  const int rc = allow_smem(ffn_grad_kernel<Cfg>, Cfg::SMEM_BYTES, done);
+  if (rc) return rc;
+  const long long units = (long long)p.n_x + p.n_13 + p.n_2;
+  const int pairs = (int)std::min<long long>(std::max(1, sms / 2), units);
+  return launch("feed-forward gradients", ffn_grad_kernel<Cfg>, dim3(2 * pairs), Cfg::THREADS, Cfg::SMEM_BYTES, s, 2, m, p);
+}
+
 template <int kElem>
 int gated_ffn_grad(const void* x, const void* w1, const void* w2, const void* w3, const void* h, const void* d_out,
                    void* d_x, void* d_w13, void* d_w2, int T, int H, int I, int gate, int sms, char* ws, size_t ws_bytes,
@@ -397,12 +438,50 @@ int gated_ffn_grad(const void* x, const void* w1, const void* w2, const void* w3
                    dim3(grid_for(((long long)T * I / 8 + 255) / 256, sms)), 256, 0, s, 0, (const float*)p.ws,
                    p.splits, T, I, gate, h, (void*)dh, (void*)a)))
     return rc;
-  const FfnOperand dh_planes = {{dh, dh + plane}, 2};
   // plane 1 of dh starts on a 16-byte boundary: a plane is T * I elements, I a multiple of 8
-  if ((rc = ffn_store<kElem, false, true>(dh_planes, {{w1, w3}, 2}, T, H, I, 1, 2, d_x, sms, rest, rest_bytes, s)))
+  const Plan plan = grads_plan(T, H, I, sms, rest_bytes);
+  const int bn = plan.bn;
+  FfnGradMaps m;
+  int box[5];
+  const void* w13[2] = {w1, w3};
+  for (int i = 0; i < 2; ++i) {
+    const char* dh_i = dh + i * plane;
+    if ((rc = map_k(&m.dh[i], dh_i, kElem, T, I, 128)) || (rc = map_mn(&m.w[i], w13[i], kElem, I, H, bn / 2, &box[0])) ||
+        (rc = map_mn(&m.dht[i], dh_i, kElem, T, I, 128, &box[1])))
+      return rc;
+  }
+  if ((rc = map_mn(&m.x, x, kElem, T, H, bn / 2, &box[2])) || (rc = map_mn(&m.dyt, d_out, kElem, T, H, 128, &box[3])) ||
+      (rc = map_mn(&m.a, a, kElem, T, I, bn / 2, &box[4])))
     return rc;
-  if ((rc = ffn_store<kElem, true, true>(dh_planes, {{x}, 1}, I, H, T, 2, 1, d_w13, sms, rest, rest_bytes, s))) return rc;
-  return ffn_store<kElem, true, true>({{d_out}, 1}, {{a}, 1}, H, I, T, 1, 1, d_w2, sms, rest, rest_bytes, s);
+  FfnGradParams g{};
+  g.T = T;
+  g.H = H;
+  g.I = I;
+  g.tm_x = ceil_div(T, 256);
+  g.tn_x = g.tn_13 = ceil_div(H, bn);
+  g.kb_plane = ceil_div(I, 64);
+  g.kb_x = 2 * g.kb_plane;
+  g.splits = plan.splits;
+  g.tm_13 = ceil_div(I, 256);
+  g.tm_2 = ceil_div(H, 256);
+  g.tn_2 = ceil_div(I, bn);
+  g.kb_w = ceil_div(T, 64);
+  const long long n_x = (long long)g.tm_x * g.tn_x * g.splits, n_13 = 2ll * g.tm_13 * g.tn_13, n_2 = (long long)g.tm_2 * g.tn_2;
+  if (n_x + n_13 + n_2 > 0x3fffffff) return set_error(EK_ERR_INVALID, "too many tiles");
+  g.n_x = (int)n_x;
+  g.n_13 = (int)n_13;
+  g.n_2 = (int)n_2;
+  g.lead = g.kb_x / g.splits / g.kb_w;
+  for (int i = 0; i < 5; ++i) g.box3 |= box[i] << i;
+  g.dx = d_x;
+  g.dw13 = d_w13;
+  g.dw2 = d_w2;
+  g.ws = reinterpret_cast<float*>(rest);
+  rc = bn == 256 ? launch_grads<kElem, 256>(m, g, sms, s) : launch_grads<kElem, 128>(m, g, sms, s);
+  if (rc || g.splits == 1) return rc;
+  const long long n8 = (long long)T * H / 8;
+  return launch("feed-forward sums", ffn_reduce_kernel<kElem>, dim3(grid_for((n8 + 255) / 256, sms)), 256, 0, s, 0,
+                (const float*)g.ws, g.splits, n8, d_x);
 }
 
 // ------------------------------------------------------------------ 8-bit tiles
@@ -565,8 +644,7 @@ int ek_gated_ffn(const void* x, const void* w1, const void* w2, const void* w3, 
 size_t ek_gated_ffn_grad_workspace_bytes(int T, int H, int I, int num_sms) {
   if (!sizes_ok(T, H, I, 8) || !sms_ok(num_sms)) return kBad;
   if (T == 0) return 0;
-  const size_t sums = std::max({ffn_store_bytes(T, H, I, 1, 2, num_sms), ffn_store_bytes(I, H, T, 2, 1, num_sms),
-                                ffn_store_bytes(H, I, T, 1, 1, num_sms), gate_grad_bytes(T, H, I, num_sms)});
+  const size_t sums = std::max(grads_bytes(T, H, I, num_sms), gate_grad_bytes(T, H, I, num_sms));
   return round256((size_t)T * I * 4) + round256((size_t)T * I * 2) + sums;
 }
 

@@ -225,6 +225,20 @@ __device__ __forceinline__ void pack32(const uint32_t (&r)[32], uint4 (&v)[4]) {
   for (int g = 0; g < 4; ++g) v[g] = pack8<kElem>(reinterpret_cast<const float*>(r) + g * 8);
 }
 
+// A CTA's kRows of an operand's mn axis x 64 of K, from (mn, k0): K-major one box; MN-major
+// its 64-column chunks in one 3-D box or a box each
+template <bool kMN, int kRows>
+__device__ __forceinline__ void load_half(uint8_t* dst, const CUtensorMap* m, uint32_t bar, int box3, int mn, int k0) {
+  if constexpr (!kMN) {
+    tma_load_2d_pair(dst, m, bar, k0, mn);
+  } else if (kRows == 128 && box3) {
+    tma_load_3d_pair(dst, m, bar, 0, k0, mn / 64);
+  } else {
+    tma_load_2d_pair(dst, m, bar, mn, k0);
+    if constexpr (kRows == 128) tma_load_2d_pair(dst + 64 * 128, m, bar, mn + 64, k0);
+  }
+}
+
 struct FfnUnit {
   int tm, tn, m_plane, m_row, split, kb0, kb1;
 };
@@ -303,55 +317,42 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
   pdl_launch();
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (elect_one()) {
       tma_prefetch_desc(&tmA0);
       tma_prefetch_desc(&tmB0);
       tma_prefetch_desc(&tmA1);
       tma_prefetch_desc(&tmB1);
-      int stage = 0, issued = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      const uint32_t full0 = mapa_shared(smem_u32(&full_bar[0]), 0);  // both CTAs' loads complete on the leader's
-      for (int u = unit0; u < p.num_units && ok; u += unit_step) {
-        const FfnUnit w = ffn_unit<Cfg>(p, u);
-        const int a_mn = w.m_row + rank * 128;
-        const int b_mn = Cfg::kEpi == kFfnGate ? w.tn * (BN / 2) : w.tn * BN + rank * (BN / 2);
-        for (int kb = w.kb0; kb < w.kb1; ++kb) {
-          if (!mbar_wait(&empty_bar[stage], phase ^ 1, s_abort)) { ok = false; break; }
-          const int k_plane = kb >= p.kb_plane ? 1 : 0;
-          const int k0 = (kb - k_plane * p.kb_plane) * BK;
+    }
+    __syncwarp();
+    int stage = 0, issued = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    const uint32_t full0 = mapa_shared(smem_u32(&full_bar[0]), 0);  // both CTAs' loads complete on the leader's
+    for (int u = unit0; u < p.num_units && ok; u += unit_step) {
+      const FfnUnit w = ffn_unit<Cfg>(p, u);
+      const int a_mn = w.m_row + rank * 128;
+      const int b_mn = Cfg::kEpi == kFfnGate ? w.tn * (BN / 2) : w.tn * BN + rank * (BN / 2);
+      for (int kb = w.kb0; kb < w.kb1; ++kb) {
+        ok = mbar_wait(&empty_bar[stage], phase ^ 1, s_abort);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const int k_plane = kb >= p.kb_plane ? 1 : 0;
+        const int k0 = (kb - k_plane * p.kb_plane) * BK;
+        if (elect_one()) {
           const CUtensorMap* ta = (k_plane | w.m_plane) ? &tmA1 : &tmA0;
           const CUtensorMap* tb = (Cfg::kEpi == kFfnGate ? rank : k_plane) ? &tmB1 : &tmB0;
           uint8_t* a_dst = smem + stage * Cfg::STAGE_BYTES;
-          uint8_t* b_dst = a_dst + AB;
-          if (leader) mbar_arrive_expect_tx(&full_bar[stage], 2 * Cfg::STAGE_BYTES);
           const uint32_t fb = full0 + stage * 8;
-          if constexpr (Cfg::kAMN) {
-            if (p.a_box3) {
-              tma_load_3d_pair(a_dst, ta, fb, 0, k0, a_mn / 64);
-            } else {
-              tma_load_2d_pair(a_dst, ta, fb, a_mn, k0);
-              tma_load_2d_pair(a_dst + AB / 2, ta, fb, a_mn + 64, k0);
-            }
-          } else {
-            tma_load_2d_pair(a_dst, ta, fb, k0, a_mn);
-          }
-          if constexpr (Cfg::kBMN) {
-            if (p.b_box3) {
-              tma_load_3d_pair(b_dst, tb, fb, 0, k0, b_mn / 64);
-            } else {
-              tma_load_2d_pair(b_dst, tb, fb, b_mn, k0);
-              if constexpr (BN == 256) tma_load_2d_pair(b_dst + Cfg::B_BYTES / 2, tb, fb, b_mn + 64, k0);
-            }
-          } else {
-            tma_load_2d_pair(b_dst, tb, fb, k0, b_mn);
-          }
-          ++issued;
-          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+          if (leader) mbar_arrive_expect_tx(&full_bar[stage], 2 * Cfg::STAGE_BYTES);
+          load_half<Cfg::kAMN, 128>(a_dst, ta, fb, p.a_box3, a_mn, k0);
+          load_half<Cfg::kBMN, BN / 2>(a_dst + AB, tb, fb, p.b_box3, b_mn, k0);
         }
+        __syncwarp();
+        ++issued;
+        if (++stage == STAGES) { stage = 0; phase ^= 1; }
       }
-      if (!ok && leader) wait_copies<STAGES>(full_bar, issued);
     }
+    if (!ok && leader) wait_copies<STAGES>(full_bar, issued);
     __syncwarp();
   } else if (warp == 1) {
     if (leader) {
@@ -507,6 +508,251 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
             pack32<Cfg::kElem>(r, v);
             store_warp<8>(wt, v, reinterpret_cast<uint16_t*>(p.C) + w.m_plane * p.c_plane, row0, p.M, col, p.N);
           }
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // no CTA leaves while its peer may still signal it
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc<2>(tmem_base, 2 * BN);
+  }
+}
+
+// ------------------------------------------------------------ the three products of a gradient
+// dx = dh1 W1 + dh3 W3 (A K-major, two planes in K, `splits` slices), dW1 and dW3 = dh^T x
+// (two planes in M) and dW2 = dy^T a in one launch: they wait for the same thing, and the
+// pairs that a product's last round leaves idle go on with the next product's tiles. dx's
+// units come first, pair by pair; then the weights' tiles, all of one length, of which the
+// pairs without a unit in dx's last round take `lead` rounds more. Against one launch each,
+// 4096 x 4096 x 14336 takes XX us for YY and 333 x 1032 x 2760 XX for YY.
+struct FfnGradMaps {
+  CUtensorMap dh[2], w[2];    // dx: dh's planes K-major, W1 and W3
+  CUtensorMap dht[2], x;      // dW1, dW3: dh's planes and x, T outermost
+  CUtensorMap dyt, a;         // dW2: dy and a
+};
+struct FfnGradParams {
+  int T, H, I;
+  int tm_x, tn_x, kb_x, kb_plane, splits, n_x;  // dx: tiles, K blocks, units
+  int tm_13, tn_13, n_13;                       // dW1 and dW3: row tiles of a plane, column tiles, tiles in all
+  int tm_2, tn_2, n_2;                          // dW2
+  int kb_w;                                     // K blocks of a weight's tile
+  int lead;
+  int box3;                                     // bits: w, dht, x, dyt, a in 3-D boxes
+  void *dx, *dw13, *dw2;
+  float* ws;
+};
+struct FfnGradUnit {
+  int job, tm, tn, plane, split, kb0, kb1;
+};
+
+// The k-th unit of pair c out of n; false past the last
+__device__ __forceinline__ bool ffn_grad_unit(const FfnGradParams& p, int c, int n, int k, FfnGradUnit& w) {
+  const int mine = c < p.n_x ? (p.n_x - 1 - c) / n + 1 : 0;
+  w.plane = w.split = 0;
+  if (k < mine) {
+    const int u = c + k * n, tile = u / p.splits;
+    w.job = 0;
+    w.split = u - tile * p.splits;
+    raster(tile, p.tm_x, p.tn_x, 8, w.tm, w.tn);
+    w.kb0 = (int)((long long)w.split * p.kb_x / p.splits);
+    w.kb1 = (int)((long long)(w.split + 1) * p.kb_x / p.splits);
+    return true;
+  }
+  const int k2 = k - mine, busy = p.n_x % n;  // pairs with a unit in dx's last round
+  const int idle = busy ? n - busy : 0, lead = busy ? p.lead : 0;
+  long long t;
+  if (c < busy)
+    t = (long long)lead * idle + (long long)k2 * n + c;
+  else if (k2 < lead)
+    t = (long long)k2 * idle + c - busy;
+  else
+    t = (long long)lead * idle + (long long)(k2 - lead) * n + c;
+  if (t >= p.n_13 + p.n_2) return false;
+  w.kb0 = 0;
+  w.kb1 = p.kb_w;
+  w.job = t < p.n_13 ? 1 : 2;
+  if (w.job == 1) {
+    raster((int)t, 2 * p.tm_13, p.tn_13, 8, w.tm, w.tn);
+    w.plane = w.tm >= p.tm_13;
+    w.tm -= w.plane * p.tm_13;
+  } else {
+    raster((int)t - p.n_13, p.tm_2, p.tn_2, 8, w.tm, w.tn);
+  }
+  return true;
+}
+
+template <class Cfg>
+__global__ void __launch_bounds__(Cfg::THREADS, 1)
+    ffn_grad_kernel(const __grid_constant__ FfnGradMaps maps, const FfnGradParams p) {
+  constexpr int STAGES = Cfg::STAGES, BN = Cfg::BN, BK = Cfg::BK, AB = Cfg::A_BYTES;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + STAGES * Cfg::STAGE_BYTES + Cfg::EPI_WARPS * 2048);
+  uint64_t* empty_bar = full_bar + STAGES;
+  uint64_t* tfull_bar = empty_bar + STAGES;
+  uint64_t* tempty_bar = tfull_bar + 2;
+  uint64_t* drain_bar = tempty_bar + 2;
+  uint32_t* s_tmem_base = reinterpret_cast<uint32_t*>(drain_bar + 1);
+  volatile int* s_abort = reinterpret_cast<volatile int*>(s_tmem_base + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = (int)cluster_ctarank();
+  const bool leader = rank == 0;
+  const int pair = (int)cluster_id_x(), pairs = (int)nclusters_x();
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&tfull_bar[b], 1);
+      mbar_init(&tempty_bar[b], Cfg::EPI_WARPS * 2);
+    }
+    mbar_init(drain_bar, 1);
+    *s_abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc<2>(s_tmem_base, 2 * BN);
+    tmem_relinquish<2>();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // the peer's barriers exist before anyone signals them
+  tc_fence_after();
+  const uint32_t tmem_base = *s_tmem_base;
+  pdl_wait();
+  pdl_launch();
+
+  FfnGradUnit w;
+  if (warp == 0) {
+    if (elect_one()) {
+      const CUtensorMap* m = maps.dh;
+      for (int i = 0; i < 9; ++i) tma_prefetch_desc(m + i);
+    }
+    __syncwarp();
+    int stage = 0, issued = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    const uint32_t full0 = mapa_shared(smem_u32(&full_bar[0]), 0);  // both CTAs' loads complete on the leader's
+    // K blocks [kb0, kb1) of a unit through one pair of maps, its k0 counted from block `from`
+    auto blocks = [&](auto a_mn_major, const CUtensorMap* ta, const CUtensorMap* tb, int a3, int b3, int a_mn, int b_mn,
+                      int kb0, int kb1, int from) {
+      constexpr bool kAMN = decltype(a_mn_major)::value;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        ok = mbar_wait(&empty_bar[stage], phase ^ 1, s_abort);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) return;
+        if (elect_one()) {
+          uint8_t* a_dst = smem + stage * Cfg::STAGE_BYTES;
+          const uint32_t fb = full0 + stage * 8;
+          if (leader) mbar_arrive_expect_tx(&full_bar[stage], 2 * Cfg::STAGE_BYTES);
+          load_half<kAMN, 128>(a_dst, ta, fb, a3, a_mn, (kb - from) * BK);
+          load_half<true, BN / 2>(a_dst + AB, tb, fb, b3, b_mn, (kb - from) * BK);
+        }
+        __syncwarp();
+        ++issued;
+        if (++stage == STAGES) { stage = 0; phase ^= 1; }
+      }
+    };
+    for (int k = 0; ok && ffn_grad_unit(p, pair, pairs, k, w); ++k) {
+      const int a_mn = w.tm * 256 + rank * 128, b_mn = w.tn * BN + rank * (BN / 2);
+      if (w.job == 0) {
+        blocks(std::false_type{}, &maps.dh[0], &maps.w[0], 0, p.box3 & 1, a_mn, b_mn, w.kb0, min(w.kb1, p.kb_plane), 0);
+        if (ok)
+          blocks(std::false_type{}, &maps.dh[1], &maps.w[1], 0, p.box3 & 1, a_mn, b_mn, max(w.kb0, p.kb_plane), w.kb1,
+                 p.kb_plane);
+      } else if (w.job == 1) {
+        blocks(std::true_type{}, w.plane ? &maps.dht[1] : &maps.dht[0], &maps.x, p.box3 >> 1 & 1, p.box3 >> 2 & 1, a_mn,
+               b_mn, w.kb0, w.kb1, 0);
+      } else {
+        blocks(std::true_type{}, &maps.dyt, &maps.a, p.box3 >> 3 & 1, p.box3 >> 4 & 1, a_mn, b_mn, w.kb0, w.kb1, 0);
+      }
+    }
+    if (!ok && leader) wait_copies<STAGES>(full_bar, issued);
+    __syncwarp();
+  } else if (warp == 1) {
+    if (leader) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      const uint64_t b_desc = umma_desc_sw128(smem_u32(smem) + AB, BK * 128, 1024);
+      // One loop for each form of A: what the MMA reads then stays uniform (elect_one).
+      auto blocks = [&](auto a_mn, const FfnGradUnit& w, int buf) {
+        constexpr bool kAMN = decltype(a_mn)::value;
+        constexpr uint32_t a_step = kAMN ? 2048 >> 4 : 32 >> 4, idesc = Cfg::IDESC | (kAMN ? 1u << 15 : 0u);
+        const uint64_t a_desc = umma_desc_sw128(smem_u32(smem), kAMN ? BK * 128 : 16, 1024);
+        const uint32_t d_tmem = tmem_base + buf * BN;
+        for (int kb = w.kb0; kb < w.kb1; ++kb) {
+          ok = mbar_wait(&full_bar[stage], phase, s_abort);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) return;
+          tc_fence_after();
+          const uint32_t off = stage * (Cfg::STAGE_BYTES >> 4);
+          if (elect_one()) {
+#pragma unroll
+            for (int i = 0; i < BK / 16; ++i)
+              umma_pair<false>(d_tmem, a_desc + off + i * a_step, b_desc + off + i * (2048 >> 4), idesc,
+                               (kb > w.kb0 || i > 0) ? 1u : 0u);
+            umma_commit_pair(&empty_bar[stage], 0x3);
+            if (kb + 1 == w.kb1) umma_commit_pair(&tfull_bar[buf], 0x3);
+          }
+          __syncwarp();
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+      };
+      for (int k = 0; ok && ffn_grad_unit(p, pair, pairs, k, w); ++k) {
+        const int buf = k & 1;
+        ok = mbar_wait(&tempty_bar[buf], ((k >> 1) & 1) ^ 1, s_abort);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        if (w.job == 0)
+          blocks(std::false_type{}, w, buf);
+        else
+          blocks(std::true_type{}, w, buf);
+      }
+      if (elect_one()) umma_commit_pair(drain_bar, 0x3);  // every MMA has completed (in both CTAs) before TMEM is freed
+      __syncwarp();
+    }
+    volatile int never = 0;
+    mbar_wait(drain_bar, 0, &never);
+    __syncwarp();
+  } else {
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    const uint32_t tempty0 = mapa_shared(smem_u32(&tempty_bar[0]), 0);
+    const WarpTile wt{smem + STAGES * Cfg::STAGE_BYTES + (warp - 2) * 2048, lane};
+    for (int k = 0; ffn_grad_unit(p, pair, pairs, k, w); ++k) {
+      const int buf = k & 1, row0 = w.tm * 256 + rank * 128 + q * 32;
+      const bool got = mbar_wait(&tfull_bar[buf], (k >> 1) & 1, s_abort);
+      if (!__all_sync(0xffffffffu, got)) break;  // the TMEM loads are warp-collective
+      tc_fence_after();
+      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buf * BN;
+      const int M = w.job == 0 ? p.T : w.job == 1 ? p.I : p.H, N = w.job == 2 ? p.I : p.H;
+      uint16_t* out = reinterpret_cast<uint16_t*>(w.job == 0 ? p.dx : w.job == 1 ? p.dw13 : p.dw2) +
+                      (size_t)w.plane * p.I * p.H;
+#pragma unroll 1
+      for (int c = 0; c < BN / 64; ++c) {
+        const int c0 = half * (BN / 2) + c * 32, col = w.tn * BN + c0;
+        uint32_t r[32];
+        tmem_ld32(t_row + c0, r);
+        tmem_ld_wait(r);
+        if (c == BN / 64 - 1) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(tempty0 + buf * 8);
+        }
+        if (w.job == 0 && p.splits > 1) {
+          store_warp32(wt, r, p.ws + (size_t)w.split * M * N, row0, M, col, N, N);
+        } else {
+          uint4 v[4];
+          pack32<Cfg::kElem>(r, v);
+          store_warp<8>(wt, v, out, row0, M, col, N);
         }
       }
     }

@@ -172,10 +172,13 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Cfg::REGS_LOAD));
-    if (warp == 0 && lane == 0) {
-      tma_prefetch_desc(&tmA);
-      tma_prefetch_desc(&tmB);
-      if (Cfg::kGate) tma_prefetch_desc(&tmB2);
+    if (warp == 0) {
+      if (elect_one()) {
+        tma_prefetch_desc(&tmA);
+        tma_prefetch_desc(&tmB);
+        if (Cfg::kGate) tma_prefetch_desc(&tmB2);
+      }
+      __syncwarp();
       int stage = 0, issued = 0;
       uint32_t phase = 0;
       bool ok = true;
@@ -186,11 +189,16 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
         const int a_row = w.tm * 256 + rank * 128;
         const int b_row = Cfg::kGate ? w.tn * 128 : w.tn * 256 + rank * 128;
         for (int kb = w.kb0; kb < w.kb1; ++kb) {
-          if (!mbar_wait(&empty_bar[stage], phase ^ 1, s_abort)) { ok = false; break; }
-          uint8_t* dst = smem + stage * Cfg::STAGE_BYTES;
-          if (leader) mbar_arrive_expect_tx(&full_bar[stage], 2 * Cfg::STAGE_BYTES);
-          tma_load_2d_pair(dst, &tmA, full0 + stage * 8, kb * 128, a_row);
-          tma_load_2d_pair(dst + HB, tb, full0 + stage * 8, kb * 128, b_row);
+          ok = mbar_wait(&empty_bar[stage], phase ^ 1, s_abort);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          if (elect_one()) {
+            uint8_t* dst = smem + stage * Cfg::STAGE_BYTES;
+            if (leader) mbar_arrive_expect_tx(&full_bar[stage], 2 * Cfg::STAGE_BYTES);
+            tma_load_2d_pair(dst, &tmA, full0 + stage * 8, kb * 128, a_row);
+            tma_load_2d_pair(dst + HB, tb, full0 + stage * 8, kb * 128, b_row);
+          }
+          __syncwarp();
           ++issued;
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }

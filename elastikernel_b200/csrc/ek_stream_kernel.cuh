@@ -204,12 +204,9 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
   pdl_launch();
 
   if (warp == 0) {
-    if (lane == 0) {
-      tma_prefetch_desc(&tmW);
-      if (Cfg::kGate) tma_prefetch_desc(&tmW2);
-      tma_prefetch_desc(&tmX);
-      auto load_w = [&](int u, int stage) {
-        const int tile = u / KB, k0 = (u - tile * KB) * Cfg::BK;
+    auto load_w = [&](int u, int stage) {
+      const int tile = u / KB, k0 = (u - tile * KB) * Cfg::BK;
+      if (elect_one()) {
         uint8_t* dst = smem + stage * Cfg::STAGE_BYTES;
         mbar_arrive_expect_tx(&full_bar[stage], Cfg::A_BYTES + p.n * 128);
         if constexpr (Cfg::kGate) {
@@ -218,26 +215,30 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
         } else {
           tma_load_2d(dst, &tmW, &full_bar[stage], k0, tile * 256);
         }
-      };
-      auto load_x = [&](int u, int stage) {
-        tma_load_2d(smem + stage * Cfg::STAGE_BYTES + Cfg::A_BYTES, &tmX, &full_bar[stage], (u % KB) * Cfg::BK, 0);
-      };
-      // the stages' first fill: the weights before the wait, the tokens after it
-      const int first = min(u1 - u0, STAGES);
-      for (int i = 0; i < first; ++i) load_w(u0 + i, i);
-      pdl_wait();
-      for (int i = 0; i < first; ++i) load_x(u0 + i, i);
-      int stage = 0;
-      uint32_t phase = 0;
-      for (int u = u0 + STAGES; u < u1; ++u) {
-        if (!mbar_wait(&empty_bar[stage], phase, s_abort)) {
-          wait_copies<STAGES>(full_bar, u - u0);
-          break;
-        }
-        load_w(u, stage);
-        load_x(u, stage);
-        if (++stage == STAGES) { stage = 0; phase ^= 1; }
       }
+      __syncwarp();
+    };
+    auto load_x = [&](int u, int stage) {
+      if (elect_one())
+        tma_load_2d(smem + stage * Cfg::STAGE_BYTES + Cfg::A_BYTES, &tmX, &full_bar[stage], (u % KB) * Cfg::BK, 0);
+      __syncwarp();
+    };
+    // the stages' first fill: the weights before the wait, the tokens after it
+    const int first = min(u1 - u0, STAGES);
+    for (int i = 0; i < first; ++i) load_w(u0 + i, i);
+    pdl_wait();
+    for (int i = 0; i < first; ++i) load_x(u0 + i, i);
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int u = u0 + STAGES; u < u1; ++u) {
+      const bool ok = mbar_wait(&empty_bar[stage], phase, s_abort);
+      if (!__all_sync(0xffffffffu, ok)) {
+        wait_copies<STAGES>(full_bar, u - u0);
+        break;
+      }
+      load_w(u, stage);
+      load_x(u, stage);
+      if (++stage == STAGES) { stage = 0; phase ^= 1; }
     }
     __syncwarp();
   } else if (warp == 1) {
