@@ -14,8 +14,11 @@
 //   warps 4..11  epilogue, two per TMEM lane quarter, 128 accumulators a thread: group
 //   g has of a plain tile the columns [128 g, +128), of a gate tile 64 gate columns
 //   and the same features' 64 up columns. setmaxnreg gives them the registers that
-//   the other warps do not need. A chunk of 32 columns is always in flight from TMEM
-//   while the one before it is added, the first chunk of the next K block among them.
+//   the other warps do not need. The loads from TMEM are of 64 columns, so that a K
+//   block costs two waits: the epilogue's chain of waits, not its sums, is what bounds
+//   the kernel (4096 x 18944 x 4096: 279 us, 302 with 32 columns a load and the next
+//   load in flight; 16 epilogue warps of half the accumulators 373; 232 with the loads and
+//   sums taken out).
 #pragma once
 #include "ek_stream_kernel.cuh"
 
@@ -107,6 +110,41 @@ __device__ __forceinline__ void fp8_block_store(const Fp8BlockParams& p, uint8_t
       }
     }
   }
+}
+
+// 32 lanes x 64 consecutive 32-bit columns: one wait where two loads of 32 take two.
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t (&r)[64]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+      "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+      "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];"
+      :
+        "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31]),
+        "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+        "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]),
+        "=r"(r[48]), "=r"(r[49]), "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]),
+        "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+      : "r"(taddr));
+}
+// Wait for it, tying the registers to the wait.
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[64]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+      :
+        "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+        "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+        "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]),
+        "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]),
+        "+r"(r[32]), "+r"(r[33]), "+r"(r[34]), "+r"(r[35]), "+r"(r[36]), "+r"(r[37]), "+r"(r[38]), "+r"(r[39]),
+        "+r"(r[40]), "+r"(r[41]), "+r"(r[42]), "+r"(r[43]), "+r"(r[44]), "+r"(r[45]), "+r"(r[46]), "+r"(r[47]),
+        "+r"(r[48]), "+r"(r[49]), "+r"(r[50]), "+r"(r[51]), "+r"(r[52]), "+r"(r[53]), "+r"(r[54]), "+r"(r[55]),
+        "+r"(r[56]), "+r"(r[57]), "+r"(r[58]), "+r"(r[59]), "+r"(r[60]), "+r"(r[61]), "+r"(r[62]), "+r"(r[63])
+      :
+      : "memory");
 }
 
 template <class Cfg>
@@ -257,11 +295,11 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
       float2 acc[64];
 #pragma unroll
       for (int j = 0; j < 64; ++j) acc[j] = make_float2(0.f, 0.f);
-      uint32_t ra[32], rb[32];
-      auto add = [&](uint32_t(&r)[32], int base, float s) {
+      uint32_t r[64];
+      auto add = [&](int base, float x) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
-          acc[base + j] = fma2(make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), make_float2(s, s),
+        for (int j = 0; j < 32; ++j)
+          acc[base + j] = fma2(make_float2(__uint_as_float(r[2 * j]), __uint_as_float(r[2 * j + 1])), make_float2(x, x),
                                acc[base + j]);
       };
       // The scales of four K blocks at a time, fetched four blocks ahead
@@ -294,10 +332,6 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
       fetch(w.kb0);
       // A failed wait has raised the abort flag: the loop then runs out without waiting and
       // the tile is not stored.
-      mbar_wait_soon(&kfull_bar[gkb & 1], (gkb >> 1) & 1, s_abort);
-      __syncwarp();
-      tc_fence_after();
-      tmem_ld32(t_row + (gkb & 1) * 256 + run0, ra);
 #pragma unroll 1
       for (int kb = w.kb0; kb < w.kb1; kb += 4) {
         float s0[4], s1[4];
@@ -310,31 +344,19 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           if (kb + j < w.kb1) {
-            const int buf = gkb & 1, nbuf = buf ^ 1;
-            const bool more = kb + j + 1 < w.kb1;
-            const uint32_t t0 = t_row + buf * 256, nphase = ((gkb + 1) >> 1) & 1;
-            uint64_t* nbar = &kfull_bar[nbuf];
-            tmem_ld_wait(ra);
-            tmem_ld32(t0 + run0 + 32, rb);
-            add(ra, 0, s0[j]);
-            tmem_ld_wait(rb);
-            tmem_ld32(t0 + run1, ra);
-            add(rb, 16, s0[j]);
-            tmem_ld_wait(ra);
-            tmem_ld32(t0 + run1 + 32, rb);
-            const bool early = more && mbar_test(smem_u32(nbar), nphase);
-            add(ra, 32, s1[j]);
-            tmem_ld_wait(rb);
+            const int buf = gkb & 1;
+            mbar_wait_soon(&kfull_bar[buf], (gkb >> 1) & 1, s_abort);
+            __syncwarp();
+            tc_fence_after();
+            tmem_ld64(t_row + buf * 256 + run0, r);
+            tmem_ld_wait(r);
+            add(0, s0[j]);
+            tmem_ld64(t_row + buf * 256 + run1, r);
+            tmem_ld_wait(r);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(kempty0 + buf * 8);
-            if (more) {
-              if (!early) mbar_wait_soon(nbar, nphase, s_abort);
-              __syncwarp();
-              tc_fence_after();
-              tmem_ld32(t_row + nbuf * 256 + run0, ra);
-            }
-            add(rb, 48, s1[j]);
+            add(32, s1[j]);
             ++gkb;
           }
         }
