@@ -509,9 +509,26 @@ int fp8_splits(int M, int N, int K, int sms, size_t cap) {
       .splits;
 }
 
+// Whether an e4m3 product (gate: a gate/up pair of N features) of M tokens runs in
+// stream_kernel. Up to 64 tokens it does. From there to kStreamTokens its unit of 32 KB
+// takes 0.9 us and 9 ns a token (the sums of 128 tokens leave no registers to hide the loads
+// behind), a block of the 256-row tiles 0.5 us whatever the tokens: 14336 x 4096 takes 18.7,
+// 28 and 31 us for 64, 96 and 128 tokens in the one and 19 in the other, the 8-bit block of
+// 7168 x 2048, with few tiles, 34 us for 128 tokens in the one and 41 in the other.
+bool fp8_streams(int M, int N, int K, bool gate, int sms) {
+  if (M <= 64) return true;
+  if (M > kStreamTokens) return false;
+  const int kb = ceil_div(K, 128), pairs = std::max(1, sms / 2);
+  const double stream_us = stream_split(N, gate ? 128 : 256, K, 128, sms).per_cta * (0.9 + 0.009 * M) + 4.0;
+  const int splits = gate ? 1 : fp8_splits(M, N, K, sms, kMostSplitBytes);
+  const double rounds = std::ceil((double)ceil_div(N, gate ? 128 : 256) * splits / pairs);
+  const double tile_us = rounds * ceil_div(kb, splits) * 0.5 + (splits > 1 ? 9.0 : 4.0);
+  return stream_us < tile_us;
+}
+
 int fp8_store(const void* a, const void* w, const float* as, const float* wsc, void* C, int M, int N, int K, int out_type,
               int sms, void* ws, size_t ws_bytes, cudaStream_t s, bool early) {
-  if (M <= kStreamTokens)
+  if (fp8_streams(M, N, K, false, sms))
     return stream_store(EK_DTYPE_E4M3, w, a, {as, wsc, nullptr}, M, N, K, C, out_type, sms, ws, ws_bytes, s, early);
   Fp8BlockParams p{};
   p.M = M;
@@ -535,9 +552,10 @@ int fp8_store(const void* a, const void* w, const float* as, const float* wsc, v
 }
 
 size_t fp8_store_bytes(int M, int N, int K, int sms) {
-  if (M <= kStreamTokens) return stream_bytes_most(N, 256, M, sms);
-  const int s = fp8_splits(M, N, K, sms, kMostSplitBytes);
-  return s > 1 ? (size_t)s * M * N * 4 : 0;
+  // for either kernel: on a smaller partition the choice may be the other one
+  const size_t stream = M <= kStreamTokens ? stream_bytes_most(N, 256, M, sms) : 0;
+  const int s = M <= 64 ? 1 : fp8_splits(M, N, K, sms, kMostSplitBytes);
+  return std::max(stream, s > 1 ? (size_t)s * M * N * 4 : 0);
 }
 
 struct Fp8FfnLayout {
@@ -699,7 +717,7 @@ int ek_gated_ffn_fp8(const void* x, const void* w1, const void* w2, const void* 
   rc = launch("feed-forward quantisation", ffn_quant_kernel, dim3(grid_for((groups + 15) / 16, sms)), 256, 0, s, 0,
               static_cast<const __nv_bfloat16*>(x), groups, H, xq, xs);
   if (rc) return rc;
-  if (T <= kStreamTokens) {
+  if (fp8_streams(T, I, H, true, sms)) {
     rc = stream_gate(EK_DTYPE_E4M3, w1, w3, xq, {xs, s1, s3}, T, I, H, gate, nullptr, nullptr, aq, as, sms, rest,
                      rest_bytes, s, true);
   } else {
