@@ -124,7 +124,7 @@ Plan pick_plan(long long rows, int planes, int cols, int k_blocks, int pairs, lo
   }
   return best;
 }
-constexpr double kFfnBlockUs = 0.28, kFp8BlockUs = 0.55;
+constexpr double kFfnBlockUs = 0.28, kFp8BlockUs = 0.5;
 constexpr double kStoreUs = 4.0, kGateUs = 5.0;
 // gelu's erfc makes the gradient's epilogue three times as long
 constexpr double gate_grad_us(int gate) { return gate == kGateGelu ? 18.0 : 7.0; }
@@ -509,6 +509,12 @@ int fp8_splits(int M, int N, int K, int sms, size_t cap) {
       .splits;
 }
 
+// of a gate/up pair, whose tiles hold 128 features
+int fp8_gate_splits(int T, int I, int H, int sms, size_t cap) {
+  if (T > 65535 * 8) return 1;  // the launch that adds the slices has a block for every 8 tokens
+  return pick_plan(T, 1, 2 * I, ceil_div(H, 128), std::max(1, sms / 2), 2ll * T * I, kFp8BlockUs, kGateUs, false, cap).splits;
+}
+
 // Whether an e4m3 product (gate: a gate/up pair of N features) of M tokens runs in
 // stream_kernel. Up to 64 tokens it does. From there to kStreamTokens its unit of 32 KB
 // takes 0.9 us and 9 ns a token (the sums of 128 tokens leave no registers to hide the loads
@@ -520,7 +526,7 @@ bool fp8_streams(int M, int N, int K, bool gate, int sms) {
   if (M > kStreamTokens) return false;
   const int kb = ceil_div(K, 128), pairs = std::max(1, sms / 2);
   const double stream_us = stream_split(N, gate ? 128 : 256, K, 128, sms).per_cta * (0.9 + 0.009 * M) + 4.0;
-  const int splits = gate ? 1 : fp8_splits(M, N, K, sms, kMostSplitBytes);
+  const int splits = (gate ? fp8_gate_splits : fp8_splits)(M, N, K, sms, kMostSplitBytes);
   const double rounds = std::ceil((double)ceil_div(N, gate ? 128 : 256) * splits / pairs);
   const double tile_us = rounds * ceil_div(kb, splits) * 0.5 + (splits > 1 ? 9.0 : 4.0);
   return stream_us < tile_us;
@@ -568,7 +574,9 @@ Fp8FfnLayout fp8_ffn_layout(int T, int H, int I, int sms) {
   L.aq = L.xs + round256((size_t)T * ceil_div(H, 128) * 4);
   L.as = L.aq + round256((size_t)T * I);
   L.rest = L.as + round256((size_t)T * ceil_div(I, 128) * 4);
-  const size_t gate = T <= kStreamTokens ? stream_bytes_most(I, 128, T, sms) : 0;
+  const int splits = T <= 64 ? 1 : fp8_gate_splits(T, I, H, sms, kMostSplitBytes);
+  const size_t gate = std::max(T <= kStreamTokens ? stream_bytes_most(I, 128, T, sms) : 0,
+                               splits > 1 ? (size_t)splits * T * I * 8 : 0);
   L.total = L.rest + std::max(gate, fp8_store_bytes(T, H, I, sms));
   return L;
 }
@@ -727,7 +735,8 @@ int ek_gated_ffn_fp8(const void* x, const void* w1, const void* w2, const void* 
     p.tiles_m = ceil_div(T, 256);
     p.tiles_n = ceil_div(I, 128);
     p.k_blocks = ceil_div(H, 128);
-    p.splits = 1;
+    p.splits = fp8_gate_splits(T, I, H, sms, rest_bytes);
+    p.ws = reinterpret_cast<float*>(rest);
     p.a_scale = xs;
     p.w_scale = s1;
     p.w_scale2 = s3;
@@ -736,6 +745,16 @@ int ek_gated_ffn_fp8(const void* x, const void* w1, const void* w2, const void* 
     p.codes = aq;
     p.scales = as;
     rc = launch_fp8<true>(xq, w1, w3, H, p, sms, s);
+    if (!rc && p.splits > 1) {
+      StreamOut o{};
+      o.T = T;
+      o.N = I;
+      o.gate = gate;
+      o.codes = aq;
+      o.scales = as;
+      rc = launch("block-scaled gate sums", fp8_gate_reduce_kernel, dim3(p.tiles_n, ceil_div(T, 8)), 256, 0, s, 0,
+                  (const float*)p.ws, p.splits, o);
+    }
   }
   if (rc) return rc;
   return fp8_store(aq, w2, as, s2, y, T, H, I, kOutBF16, sms, rest, rest_bytes, s, true);

@@ -48,11 +48,29 @@ struct Fp8BlockParams {
   void* C;               // plain result
   int out_type;          // OutType
   int wide;              // rows of C are a multiple of 16 bytes
-  float* ws;             // splits > 1: fp32 sums [splits][M][N]
+  float* ws;             // splits > 1: fp32 sums [splits][M][N] (gate: [splits][M][2 N])
   int gate;
   uint8_t* codes;        // gate: a [M][N] and its scales [M][ceil(N / 128)]
   float* scales;
 };
+
+// 64 fp32 sums of the lane's row to out[row0 + lane][col0 ..], n columns in rows of ld
+// elements, n a multiple of 4; by way of 8 KB of shared memory as below
+__device__ __forceinline__ void store_sums64(uint8_t* tile, int lane, float* out, long long ld, int row0, int rows, int col0,
+                                             int n, const float* v) {
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 16; ++j)
+    *reinterpret_cast<uint4*>(tile + lane * 256 + ((j ^ (lane & 7)) << 4)) = *reinterpret_cast<const uint4*>(v + j * 4);
+  __syncwarp();
+#pragma unroll 4
+  for (int i = 0; i < 16; ++i) {
+    const int r = 2 * i + (lane >> 4), row = row0 + r, col = col0 + (lane & 15) * 4;
+    if (row < rows && col < n)
+      *reinterpret_cast<uint4*>(out + row * ld + col) =
+          *reinterpret_cast<const uint4*>(tile + r * 256 + (((lane & 15) ^ (r & 7)) << 4));
+  }
+}
 
 // The warp's 32 rows x 128 columns from (row0, col0), lane's row in v, to the result or to
 // a slice's sums. They cross 8 KB of shared memory, 32 rows of 16 pieces of 16 bytes (a
@@ -362,7 +380,13 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
         }
       }
       const bool good = !__any_sync(0xffffffffu, *s_abort);
-      if constexpr (Cfg::kGate) {
+      if (Cfg::kGate && p.splits > 1) {
+        if (!good) break;
+        const float* a = reinterpret_cast<const float*>(acc);  // [0, 64) gate, [64, 128) up
+        float* out = p.ws + (size_t)w.split * p.M * (2ll * p.N);
+        store_sums64(tile, lane, out, 2ll * p.N, row0, p.M, w.tn * 128 + wg * 64, p.N, a);
+        store_sums64(tile, lane, out + p.N, 2ll * p.N, row0, p.M, w.tn * 128 + wg * 64, p.N, a + 64);
+      } else if constexpr (Cfg::kGate) {
         // one decision for the epilogue warps: they meet for the groups' largest values
         if (named_bar_red_or(1, 32 * Cfg::EPI_WARPS, good ? 0 : 1)) break;
         float* a = reinterpret_cast<float*>(acc);  // [0, 64) gate, [64, 128) up
@@ -408,6 +432,23 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
     tc_fence_after();
     tmem_dealloc<2>(tmem_base, 512);
   }
+}
+
+// What a gate tile's epilogue does, from the slices' sums: a warp per token and 128 features
+__global__ void __launch_bounds__(256)
+    fp8_gate_reduce_kernel(const float* __restrict__ ws, int splits, const StreamOut o) {
+  pdl_wait();
+  pdl_launch();
+  const int t = blockIdx.y * 8 + (threadIdx.x >> 5), f = blockIdx.x * 128 + (threadIdx.x & 31) * 4;
+  if (t >= o.T) return;
+  float4 h1 = make_float4(0.f, 0.f, 0.f, 0.f), h3 = h1;
+  if (f < o.N)
+    for (int s = 0; s < splits; ++s) {
+      const float* src = ws + ((size_t)s * o.T + t) * (2ll * o.N) + f;
+      add4(h1, __ldcg(reinterpret_cast<const float4*>(src)));
+      add4(h3, __ldcg(reinterpret_cast<const float4*>(src + o.N)));
+    }
+  finish_gate(o, t, blockIdx.x, h1, h3);
 }
 
 // out[i] = sum over the slices, in slice order, of ws[s][i]

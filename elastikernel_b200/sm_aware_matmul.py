@@ -228,6 +228,14 @@ def call_sm_aware_w4(a, qw, num_sms=None):
     return _ops.gemm_w4(a, qw, num_sms=num_sms)
 
 
+def call_sm_aware_fp8_block(a_q, w_q, a_scale, w_scale, num_sms=None):
+    """bf16 C = A @ W^T of e4m3 operands with a scale per 1 x 128 group of A and per
+    128 x 128 block of W (_ops.quant_e4m3) on the current stream's partition."""
+    from . import _ops
+
+    return _ops.gemm_fp8_block(a_q, w_q, a_scale, w_scale, num_sms=num_sms)
+
+
 def run_benchmark(sm_levels=None, test_cases=None, rep_ms: float = 50.0) -> list:
     """Vanilla vs SM-aware tcgen05 GEMM under green-context partitions
     (the reference's benchmark, sm_aware_matmul.py:237-295), timed with CUDA

@@ -30,6 +30,7 @@ import torch
 
 from elastikernel_b200 import _lib, _ops
 from elastikernel_b200.green_ctx import create_sm_partition
+from elastikernel_b200.sm_aware_matmul import call_sm_aware_fp8_block
 from oracle import ffn as off
 
 pytestmark = pytest.mark.gpu
@@ -170,6 +171,14 @@ def test_block_product_misaligned_views_and_guards(M, N, cuda_dev):
     assert torch.equal(out, ref) and guard[0] == 7 and (guard[1 + M * N:] == 7).all()
 
 
+@pytest.mark.parametrize("num_sms", [1, 2, 3, 16, 50, 148, 300])
+@pytest.mark.parametrize("M,N,K", [(9, 600, 784), (100, 2100, 1040), (300, 700, 2064)])
+def test_block_product_planned_for_any_size(M, N, K, num_sms, cuda_dev):
+    """Other runs, tiles and slices of K: the same product."""
+    a, w, sa, sw = _block_case(M, N, K)
+    _block_check(_ops.gemm_fp8_block(a, w, sa, sw, dtype=F32, num_sms=num_sms), a, w, sa, sw)
+
+
 def test_block_product_empty(cuda_dev):
     a, w, sa, sw = _block_case(4, 5, 32)
     assert _ops.gemm_fp8_block(a[:0], w, sa[:0], sw).shape == (0, 5)
@@ -202,6 +211,42 @@ def _forward_bound(x, w1, w2, w3, r, act):
             _rounded(r["a"], W2.T, x.dtype) + (da + _acc(I) * r["a"].abs()) @ W2.abs().T)
 
 
+def _check_grads(x, w1, w2, w3, h, act, num_sms=None, d_out=None, got=None):
+    (T, H), I, dtype = x.shape, w1.shape[0], x.dtype
+    if d_out is None:
+        d_out = (torch.randn((T, H), generator=_gen(5), device="cuda") * 0.5).to(dtype)
+    r = off.backward(x, w1, w2, w3, h, d_out, act)
+    X, W1, W2, W3, D = (t.double() for t in (x, w1, w2, w3, d_out))
+    hd = h.double()
+    f, df = off.gate(hd[0], act), off.slope(hd[0], act)
+    e_da = _acc(H) * (D.abs() @ W2.abs())  # error of da
+    eps = 2.0 ** -19                        # of the gate function and the products beside it
+    e1 = e_da * (hd[1] * df).abs() + eps * (r["da"] * hd[1]).abs()
+    e3 = e_da * f.abs() + eps * (r["da"] * hd[0]).abs()
+    ea = eps * (hd[0] * hd[1]).abs()
+    if got is None:
+        got = _ops.gated_ffn_grad(x, w1, w2, w3, h, d_out, act=act, num_sms=num_sms)
+    bx = torch.sqrt(_rounded(r["d1"], W1, dtype) ** 2 + _rounded(r["d3"], W3, dtype) ** 2)
+    _within("d_x", got[0], r["x"], bx + (e1 + _acc(2 * I) * r["d1"].abs()) @ W1.abs() +
+            (e3 + _acc(2 * I) * r["d3"].abs()) @ W3.abs())
+    for name, at, d, e in (("w1", 1, r["d1"], e1), ("w3", 3, r["d3"], e3)):
+        _within("d_" + name, got[at], r[name], _rounded(d.T, X, dtype) + (e + _acc(T) * d.abs()).T @ X.abs())
+    _within("d_w2", got[2], r["w2"], _rounded(r["a"].T, D, dtype).T + D.abs().T @ (ea + _acc(T) * r["a"].abs()))
+
+
+def _check_fp8(x, w1, w2, w3, act, y=None):
+    I = w1.shape[0]
+    qw = _ops.quant_ffn_weights_fp8(w1, w2, w3)
+    W = {n: off.expand(qw[n + "q"], qw[n + "s"], 128) for n in ("w1", "w2", "w3")}
+    r = off.forward_fp8(x, W["w1"], W["w2"], W["w3"], act)
+    y = _ops.gated_ffn_fp8(x, qw, act=act) if y is None else y
+    flips = 3 * 2.0 ** -3 * r["a"].abs().amax(dim=1, keepdim=True) * W["w2"].abs().amax(dim=1)
+    _within("y", y, r["y"], flips + _acc(I) * (r["aq"].abs() @ W["w2"].abs().T))
+    rms = (y.double() - r["y"]).square().mean().sqrt() / r["y"].square().mean().sqrt().clamp(min=1e-30)
+    assert rms <= _u(BF)
+    return y
+
+
 SIZES = [(1, 8, 8), (2, 136, 72), (16, 64, 256), (17, 1032, 520), (33, 256, 128), (64, 72, 1000), (65, 520, 264),
          (128, 256, 384), (129, 256, 384), (200, 8, 1016), (256, 1032, 136), (257, 136, 72), (600, 320, 712)]
 
@@ -223,24 +268,7 @@ def test_gated_ffn(T, H, I, dtype, act, cuda_dev):
 @pytest.mark.parametrize("dtype,act", [(BF, "silu"), (FP, "gelu"), (BF, "gelu_tanh")])
 def test_gated_ffn_grad(T, H, I, dtype, act, cuda_dev):
     x, w1, w2, w3 = _ffn_case(T, H, I, dtype)
-    h = off.forward(x, w1, w2, w3, act)["h"].to(dtype)
-    d_out = (torch.randn((T, H), generator=_gen(5), device="cuda") * 0.5).to(dtype)
-    r = off.backward(x, w1, w2, w3, h, d_out, act)
-    X, W1, W2, W3, D = (t.double() for t in (x, w1, w2, w3, d_out))
-    hd = h.double()
-    f, df = off.gate(hd[0], act), off.slope(hd[0], act)
-    e_da = _acc(H) * (D.abs() @ W2.abs())  # error of da
-    eps = 2.0 ** -19                        # of the gate function and the products beside it
-    e1 = e_da * (hd[1] * df).abs() + eps * (r["da"] * hd[1]).abs()
-    e3 = e_da * f.abs() + eps * (r["da"] * hd[0]).abs()
-    ea = eps * (hd[0] * hd[1]).abs()
-    got = _ops.gated_ffn_grad(x, w1, w2, w3, h, d_out, act=act)
-    bx = torch.sqrt(_rounded(r["d1"], W1, dtype) ** 2 + _rounded(r["d3"], W3, dtype) ** 2)
-    _within("d_x", got[0], r["x"], bx + (e1 + _acc(2 * I) * r["d1"].abs()) @ W1.abs() +
-            (e3 + _acc(2 * I) * r["d3"].abs()) @ W3.abs())
-    for name, at, d, e in (("w1", 1, r["d1"], e1), ("w3", 3, r["d3"], e3)):
-        _within("d_" + name, got[at], r[name], _rounded(d.T, X, dtype) + (e + _acc(T) * d.abs()).T @ X.abs())
-    _within("d_w2", got[2], r["w2"], _rounded(r["a"].T, D, dtype).T + D.abs().T @ (ea + _acc(T) * r["a"].abs()))
+    _check_grads(x, w1, w2, w3, off.forward(x, w1, w2, w3, act)["h"].to(dtype), act)
 
 
 @pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
@@ -271,6 +299,34 @@ def test_gradient_against_differences(act, cuda_dev):
         # rounding of h, dh, a: each relative u of terms whose sum has this scale; the
         # difference's own error: step^2 / 6 of a third derivative of the same scale
         assert abs(grads[i][at].item() - diff) <= 16 * _u(FP) * scale + 4 * step ** 2 * scale
+
+
+@pytest.mark.parametrize("T,H,I", [(150, 4096, 264), (200, 2056, 136), (140, 1544, 72)])
+@pytest.mark.parametrize("dtype,act", [(BF, "gelu"), (FP, "silu"), (BF, "gelu_tanh")])
+def test_gate_cut_along_k(T, H, I, dtype, act, cuda_dev):
+    """Few tiles over a long axis: the gate functions and their gradient work on summed
+    slices (in 8 bits with the quantisation)."""
+    x, w1, w2, w3 = _ffn_case(T, H, I, dtype)
+    r = off.forward(x, w1, w2, w3, act)
+    bh, by = _forward_bound(x, w1, w2, w3, r, act)
+    y, h = _ops.gated_ffn(x, w1, w2, w3, act=act, save=True)
+    _within("y", y, r["y"], by)
+    _within("h", h, r["h"], bh)
+    _check_grads(x, w1, w2, w3, r["h"].to(dtype), act)
+    if dtype == BF:
+        I16 = I // 16 * 16
+        H16 = H // 16 * 16
+        _check_fp8(*(t.contiguous() for t in (x[:, :H16], w1[:I16, :H16], w2[:H16, :I16], w3[:I16, :H16])), act)
+
+
+@pytest.mark.parametrize("num_sms", [1, 2, 6, 16, 50, 148, 300])
+@pytest.mark.parametrize("T,H,I", [(520, 776, 1288), (70, 264, 2504)])
+def test_gated_ffn_planned_for_any_size(T, H, I, num_sms, cuda_dev):
+    """Other numbers of pairs deal the gradients' units out otherwise, none left out."""
+    x, w1, w2, w3 = _ffn_case(T, H, I, BF)
+    r = off.forward(x, w1, w2, w3, "silu")
+    _within("y", _ops.gated_ffn(x, w1, w2, w3, num_sms=num_sms), r["y"], _forward_bound(x, w1, w2, w3, r, "silu")[1])
+    _check_grads(x, w1, w2, w3, r["h"].to(BF), "silu", num_sms)
 
 
 def test_extreme_activations(cuda_dev):
@@ -367,16 +423,10 @@ def test_gated_ffn_empty_misaligned_and_in_place(cuda_dev):
 def test_gated_ffn_fp8(T, H, I, act, cuda_dev):
     x, w1, w2, w3 = _ffn_case(T, H, I, BF)
     x[0] = 0
-    qw = _ops.quant_ffn_weights_fp8(w1, w2, w3)
-    W = {n: off.expand(qw[n + "q"], qw[n + "s"], 128) for n in ("w1", "w2", "w3")}
-    r = off.forward_fp8(x, W["w1"], W["w2"], W["w3"], act)
-    y = _ops.gated_ffn_fp8(x, qw, act=act)
-    flips = 3 * 2.0 ** -3 * r["a"].abs().amax(dim=1, keepdim=True) * W["w2"].abs().amax(dim=1)
-    _within("y", y, r["y"], flips + _acc(I) * (r["aq"].abs() @ W["w2"].abs().T))
+    y = _check_fp8(x, w1, w2, w3, act)
     assert (y[0] == 0).all()
-    rms = (y.double() - r["y"]).square().mean().sqrt() / r["y"].square().mean().sqrt().clamp(min=1e-30)
-    assert rms <= _u(BF)
     out = torch.empty_like(x)
+    qw = _ops.quant_ffn_weights_fp8(w1, w2, w3)
     assert _ops.gated_ffn_fp8(x, qw, act=act, out=out) is out
     assert torch.equal(out, y)
 
@@ -407,6 +457,45 @@ def test_gated_ffn_fp8_empty(cuda_dev):
     x, w1, w2, w3 = _ffn_case(4, 32, 48, BF)
     qw = _ops.quant_ffn_weights_fp8(w1, w2, w3)
     assert _ops.gated_ffn_fp8(x[:0], qw).shape == (0, 32)
+
+
+# ------------------------------------------------------------------ past 32 bits
+def _picked(n, m=40):
+    """Some of n indices, the first and the last ones among them."""
+    g = torch.Generator().manual_seed(n)
+    i = torch.cat([torch.arange(3), torch.randint(0, n, (m,), generator=g), torch.arange(n - 3, n)])
+    return i.unique().cuda()
+
+
+def test_block_product_past_2_31_elements(cuda_dev):
+    M, N, K = 70001, 32768, 32
+    a, w, sa, sw = _block_case(M, N, K)
+    out = _ops.gemm_fp8_block(a, w, sa, sw)
+    r = _picked(M)
+    va, vw = off.expand(a[r], sa[r], 1), off.expand(w, sw, 128)
+    _within("C", out[r], va @ vw.T, _acc(K) * (va.abs() @ vw.abs().T))
+
+
+def test_gated_ffn_past_2_31_elements(cuda_dev):
+    """150,000 tokens of 16,384 activations: planes of 2.46e9 elements."""
+    T, H, I = 150001, 64, 16384
+    x, w1, w2, w3 = _ffn_case(T, H, I, BF)
+    y, h = _ops.gated_ffn(x, w1, w2, w3, save=True)
+    d = torch.zeros_like(x)
+    r = _picked(T)
+    d[r] = torch.randn((r.numel(), H), generator=_gen(3), device="cuda").to(BF)
+    f = off.forward(x[r], w1, w2, w3, "silu")
+    bh, by = _forward_bound(x[r], w1, w2, w3, f, "silu")
+    _within("y", y[r], f["y"], by)
+    _within("h", h[:, r], f["h"], bh)
+    got = _ops.gated_ffn_grad(x, w1, w2, w3, h, d)
+    assert (got[0][[i for i in range(7, 4000) if i not in set(r.tolist())]] == 0).all()
+    # the other tokens' gradients are zero: the sums are those of the picked ones alone
+    _check_grads(x[r], w1, w2, w3, h[:, r].contiguous(), "silu", d_out=d[r], got=(got[0][r], *got[1:]))
+    del h, got
+    qw = _ops.quant_ffn_weights_fp8(w1, w2, w3)
+    q = _ops.gated_ffn_fp8(x, qw)
+    _check_fp8(x[r], w1, w2, w3, "silu", y=q[r])
 
 
 # ------------------------------------------------------------------ as they are used
@@ -491,9 +580,12 @@ def test_on_a_partition(T, cuda_dev):
     refs = [f() for f in calls]
     stream, sms = create_sm_partition(cuda_dev, 16)
     torch.cuda.synchronize()
+    a, w, sa, sw = _block_case(T, 333, 400)
     with torch.cuda.stream(stream):
         got = [f() for f in calls]
+        c = call_sm_aware_fp8_block(a, w, sa, sw)
     torch.cuda.synchronize()
+    _block_check(c, a, w, sa, sw)
     for ts, rs in zip(got, refs):
         for t, r in zip(ts, rs):
             # the sums' order differs: a code or a rounding may fall on the other side
