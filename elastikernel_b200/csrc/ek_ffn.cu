@@ -79,12 +79,17 @@ int map_k(CUtensorMap* m, const void* base, int dtype, int rows, int k, int box_
   const int es = elem_size(dtype);
   return make_tmap_2d(m, base, map_type(dtype), k, rows, (uint64_t)k * es, 128 / es, box_rows);
 }
-// k x cols, the reduction axis outermost (16 bits), a box of box_cols (64 or 128) columns x
-// 64 of K: both 64-column chunks of 128 in one 3-D box where every row holds whole chunks
-int map_mn(CUtensorMap* m, const void* base, int dtype, int k, int cols, int box_cols, int* box3) {
-  *box3 = box_cols == 128 && cols % 64 == 0;
-  if (*box3) return make_tmap_3d(m, base, map_type(dtype), 64, k, cols / 64, (uint64_t)cols * 2, 128, 64, 64, 2);
-  return make_tmap_2d(m, base, map_type(dtype), cols, k, (uint64_t)cols * 2, 64, 64);
+// k x cols, the reduction axis outermost (16 bits): the 3-D map of its whole 64-column
+// chunks, two to a box, and the 2-D map of all columns (load_half); fewer than two whole
+// chunks: the 2-D map twice.
+int whole_chunks(int cols) { return cols >= 128 ? cols / 64 * 64 : 0; }
+int map_mn(CUtensorMap* m, CUtensorMap* m2, const void* base, int dtype, int k, int cols) {
+  int rc = make_tmap_2d(m2, base, map_type(dtype), cols, k, (uint64_t)cols * 2, 64, 64);
+  if (rc) return rc;
+  if (whole_chunks(cols))
+    return make_tmap_3d(m, base, map_type(dtype), 64, k, cols / 64, (uint64_t)cols * 2, 128, 64, 64, 2);
+  *m = *m2;
+  return EK_OK;
 }
 
 int grid_for(long long work, int sms) { return (int)std::max<long long>(1, std::min<long long>(work, (long long)sms * 8)); }
@@ -102,13 +107,13 @@ int grid_for(long long work, int sms) { return (int)std::max<long long>(1, std::
 struct Plan {
   int bn, splits;
 };
-Plan pick_plan(long long rows, int planes, int cols, int k_blocks, int pairs, long long elems, double t_kb, double epi_us,
+Plan pick_plan(long long rows, int cols, int k_blocks, int pairs, long long elems, double t_kb, double epi_us,
                bool narrow, size_t cap) {
   constexpr double kSliceUs = 4.0, kReduceUs = 3.0, kBytesPerUs = 4.0e6;
   Plan best{256, 1};
   double best_us = 1e30;
   for (int bn = 256; bn >= (narrow ? 128 : 256); bn /= 2) {
-    const long long tiles = (long long)ceil_div(rows, 256) * planes * ceil_div(cols, bn);
+    const long long tiles = (long long)ceil_div(rows, 256) * ceil_div(cols, bn);
     const double kb_us = bn == 256 ? t_kb : 0.7 * t_kb;
     for (int s = 1; s <= 32 && (s == 1 || k_blocks / s >= 4); ++s) {
       const size_t bytes = (size_t)s * elems * 4;
@@ -241,7 +246,8 @@ int stream_gate(int dtype, const void* w1, const void* w3, const void* x, const 
 
 // ------------------------------------------------------------------ 16-bit tiles
 template <class Cfg>
-int launch_ffn_cfg(const CUtensorMap (&ta)[2], const CUtensorMap (&tb)[2], FfnParams& p, int sms, cudaStream_t s) {
+int launch_ffn_cfg(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tb2, FfnParams& p, int sms,
+                   cudaStream_t s) {
   static bool done[64] = {false};
   const int rc = allow_smem(ffn_gemm_kernel<Cfg>, Cfg::SMEM_BYTES, done);
   if (rc) return rc;
@@ -249,81 +255,67 @@ int launch_ffn_cfg(const CUtensorMap (&ta)[2], const CUtensorMap (&tb)[2], FfnPa
   if (units > 0x3fffffff) return set_error(EK_ERR_INVALID, "too many tiles");
   p.num_units = (int)units;
   const int pairs = (int)std::min<long long>(std::max(1, sms / 2), units);
-  return launch("feed-forward product", ffn_gemm_kernel<Cfg>, dim3(2 * pairs), Cfg::THREADS, Cfg::SMEM_BYTES, s, 2, ta[0],
-                ta[1], tb[0], tb[1], p);
+  return launch("feed-forward product", ffn_gemm_kernel<Cfg>, dim3(2 * pairs), Cfg::THREADS, Cfg::SMEM_BYTES, s, 2, ta, tb,
+                tb2, p);
 }
 
-struct FfnOperand {
-  const void* base[2];
-  int planes;
-};
-
-// The two planes' maps of an operand (one plane: the same map twice), `mn` of it along the
-// result's axis and k along the sum's; box: what a CTA loads of it along mn.
-template <bool kMN>
-int map_operand(CUtensorMap (&t)[2], const FfnOperand& op, int dtype, int mn, int k, int box, int* box3) {
-  for (int i = 0; i < 2; ++i) {
-    const void* base = op.base[op.planes > 1 ? i : 0];
-    const int rc = kMN ? map_mn(&t[i], base, dtype, k, mn, box, box3) : map_k(&t[i], base, dtype, mn, k, box);
-    if (rc) return rc;
+// Maps and launch of one product of p.M rows and p.N columns over k: A K-major, B K-major (w2
+// the gate's second) or MN-major.
+template <int kElem, bool kBMN, int kEpi>
+int launch_ffn(const void* a, const void* b, const void* b2, int k, const Plan& plan, FfnParams& p, int sms, cudaStream_t s) {
+  CUtensorMap ta, tb, tb2;
+  int rc = map_k(&ta, a, kElem, p.M, k, 128);
+  if (rc) return rc;
+  if (kBMN) {
+    rc = map_mn(&tb, &tb2, b, kElem, k, p.N);
+    p.b_full = whole_chunks(p.N);
+  } else {
+    rc = map_k(&tb, b, kElem, p.N, k, plan.bn / 2);
+    if (!rc) rc = map_k(&tb2, b2, kElem, p.N, k, plan.bn / 2);
   }
-  return EK_OK;
-}
-
-// Maps and launch of one product: p.M rows (per plane) of p.N columns, k per plane of K.
-template <int kElem, bool kAMN, bool kBMN, int kEpi>
-int launch_ffn(const FfnOperand& A, const FfnOperand& B, int k, int planes_m, int planes_k, const Plan& plan, FfnParams& p,
-               int sms, cudaStream_t s) {
-  CUtensorMap ta[2], tb[2];
-  int rc = map_operand<kAMN>(ta, A, kElem, p.M, k, 128, &p.a_box3);
-  if (rc || (rc = map_operand<kBMN>(tb, B, kElem, p.N, k, plan.bn / 2, &p.b_box3))) return rc;
-  p.m_tiles_plane = ceil_div(p.M, 256);
-  p.tiles_m = p.m_tiles_plane * planes_m;
+  if (rc) return rc;
+  p.tiles_m = ceil_div(p.M, 256);
   p.tiles_n = ceil_div(p.N, kEpi == kFfnGate ? plan.bn / 2 : plan.bn);
-  p.kb_plane = ceil_div(k, 64);
-  p.k_blocks = p.kb_plane * planes_k;
+  p.k_blocks = ceil_div(k, 64);
   p.splits = plan.splits;
-  return plan.bn == 256 ? launch_ffn_cfg<FfnCfg<kElem, kAMN, kBMN, kEpi, 256>>(ta, tb, p, sms, s)
-                        : launch_ffn_cfg<FfnCfg<kElem, kAMN, kBMN, kEpi, 128>>(ta, tb, p, sms, s);
+  return plan.bn == 256 ? launch_ffn_cfg<FfnCfg<kElem, kBMN, kEpi, 256>>(ta, tb, tb2, p, sms, s)
+                        : launch_ffn_cfg<FfnCfg<kElem, kBMN, kEpi, 128>>(ta, tb, tb2, p, sms, s);
 }
 
-Plan store_plan(int M, int N, int k, int planes_m, int planes_k, int sms, size_t cap) {
-  return pick_plan(M, planes_m, N, ceil_div(k, 64) * planes_k, std::max(1, sms / 2), (long long)planes_m * M * N,
-                   kFfnBlockUs, kStoreUs, true, cap);
+Plan store_plan(int M, int N, int k, int sms, size_t cap) {
+  return pick_plan(M, N, ceil_div(k, 64), std::max(1, sms / 2), (long long)M * N, kFfnBlockUs, kStoreUs, true, cap);
 }
-size_t ffn_store_bytes(int M, int N, int k, int planes_m, int planes_k, int sms) {
-  const int s = store_plan(M, N, k, planes_m, planes_k, sms, kMostSplitBytes).splits;
-  return s > 1 ? (size_t)s * planes_m * M * N * 4 : 0;
+size_t ffn_store_bytes(int M, int N, int k, int sms) {
+  const int s = store_plan(M, N, k, sms, kMostSplitBytes).splits;
+  return s > 1 ? (size_t)s * M * N * 4 : 0;
 }
 
-// C (planes_m stacked planes) = A . B with K = k per plane. ws holds the sums of a split.
-template <int kElem, bool kAMN, bool kBMN>
-int ffn_store(const FfnOperand& A, const FfnOperand& B, int M, int N, int k, int planes_m, int planes_k, void* C, int sms,
-              void* ws, size_t ws_bytes, cudaStream_t s) {
+// C [M, N] = a [M, k] . w [N, k]^T. ws holds the sums of a split.
+template <int kElem>
+int ffn_store(const void* a, const void* w, int M, int N, int k, void* C, int sms, void* ws, size_t ws_bytes,
+              cudaStream_t s) {
   FfnParams p{};
   p.M = M;
   p.N = N;
   p.C = C;
-  p.c_plane = (long long)M * N;
   p.ws = static_cast<float*>(ws);
-  const Plan plan = store_plan(M, N, k, planes_m, planes_k, sms, ws_bytes);
-  const int rc = launch_ffn<kElem, kAMN, kBMN, kFfnStore>(A, B, k, planes_m, planes_k, plan, p, sms, s);
+  const int rc = launch_ffn<kElem, false, kFfnStore>(a, w, w, k, store_plan(M, N, k, sms, ws_bytes), p, sms, s);
   if (rc || p.splits == 1) return rc;
-  const long long n8 = (long long)planes_m * M * N / 8;
+  const long long n8 = (long long)M * N / 8;
   return launch("feed-forward sums", ffn_reduce_kernel<kElem>, dim3(grid_for((n8 + 255) / 256, sms)), 256, 0, s, 0,
                 (const float*)p.ws, p.splits, n8, C);
 }
 
 // gate/up tiles hold half as many features as columns
 Plan gate_plan(int T, int H, int I, int sms, size_t cap) {
-  return pick_plan(T, 1, 2 * I, ceil_div(H, 64), std::max(1, sms / 2), 2ll * T * I, kFfnBlockUs, kGateUs, true, cap);
+  return pick_plan(T, 2 * I, ceil_div(H, 64), std::max(1, sms / 2), 2ll * T * I, kFfnBlockUs, kGateUs, true, cap);
 }
 size_t gate_bytes(int T, int H, int I, int sms) {
   const int s = gate_plan(T, H, I, sms, kMostSplitBytes).splits;
   return s > 1 ? (size_t)s * T * I * 8 : 0;
 }
 Plan gate_grad_plan(int T, int H, int I, int gate, int sms, size_t cap) {
-  return pick_plan(T, 1, I, ceil_div(H, 64), std::max(1, sms / 2), (long long)T * I, kFfnBlockUs,
+  return pick_plan(T, I, ceil_div(H, 64), std::max(1, sms / 2), (long long)T * I, kFfnBlockUs,
                    gate_grad_us(gate), true, cap);
 }
 size_t gate_grad_bytes(int T, int H, int I, int sms) {  // of any gate function
@@ -343,8 +335,7 @@ int ffn_gate(const void* x, const void* w1, const void* w3, void* a, void* h, in
   p.H = h;
   p.h_plane = (long long)T * I;
   p.ws = static_cast<float*>(ws);
-  const int rc = launch_ffn<kElem, false, false, kFfnGate>({{x}, 1}, {{w1, w3}, 2}, H, 1, 1,
-                                                           gate_plan(T, H, I, sms, ws_bytes), p, sms, s);
+  const int rc = launch_ffn<kElem, false, kFfnGate>(x, w1, w3, H, gate_plan(T, H, I, sms, ws_bytes), p, sms, s);
   if (rc || p.splits == 1) return rc;
   return launch("feed-forward gate sums", ffn_gate_reduce_kernel<kElem>, dim3(grid_for(((long long)T * I / 8 + 255) / 256, sms)),
                 256, 0, s, 0, (const float*)p.ws, p.splits, T, I, gate, a, h);
@@ -366,7 +357,7 @@ int gated_ffn(const void* x, const void* w1, const void* w2, const void* w3, voi
   }
   rc = ffn_gate<kElem>(x, w1, w3, a, h, T, H, I, gate, sms, rest, rest_bytes, s);
   if (rc) return rc;
-  return ffn_store<kElem, false, false>({{a}, 1}, {{w2}, 1}, T, H, I, 1, 1, y, sms, rest, rest_bytes, s);
+  return ffn_store<kElem>(a, w2, T, H, I, y, sms, rest, rest_bytes, s);
 }
 
 // Tile columns and dx's slices for the gradient's three products in one launch: the pairs
@@ -401,7 +392,7 @@ size_t grads_bytes(int T, int H, int I, int sms) {
 
 template <int kElem, int kBN>
 int launch_grads(FfnGradMaps& m, FfnGradParams& p, int sms, cudaStream_t s) {
-  using Cfg = FfnCfg<kElem, false, true, kFfnStore, kBN>;
+  using Cfg = FfnCfg<kElem, true, kFfnStore, kBN>;
   static bool done[64] = {false};
   const int rc = allow_smem(ffn_grad_kernel<Cfg>, Cfg::SMEM_BYTES, done);
   if (rc) return rc;
@@ -430,8 +421,8 @@ int gated_ffn_grad(const void* x, const void* w1, const void* w2, const void* w3
   p.H = const_cast<void*>(h);
   p.c_plane = p.h_plane = (long long)T * I;
   p.Act = a;
-  int rc = launch_ffn<kElem, false, true, kFfnGateGrad>({{d_out}, 1}, {{w2}, 1}, H, 1, 1,
-                                                        gate_grad_plan(T, H, I, gate, sms, rest_bytes), p, sms, s);
+  int rc = launch_ffn<kElem, true, kFfnGateGrad>(d_out, w2, nullptr, H, gate_grad_plan(T, H, I, gate, sms, rest_bytes), p,
+                                                 sms, s);
   if (rc) return rc;
   if (p.splits > 1 &&
       (rc = launch("feed-forward gate gradient sums", ffn_gate_grad_reduce_kernel<kElem>,
@@ -442,16 +433,15 @@ int gated_ffn_grad(const void* x, const void* w1, const void* w2, const void* w3
   const Plan plan = grads_plan(T, H, I, sms, rest_bytes);
   const int bn = plan.bn;
   FfnGradMaps m;
-  int box[5];
   const void* w13[2] = {w1, w3};
   for (int i = 0; i < 2; ++i) {
     const char* dh_i = dh + i * plane;
-    if ((rc = map_k(&m.dh[i], dh_i, kElem, T, I, 128)) || (rc = map_mn(&m.w[i], w13[i], kElem, I, H, bn / 2, &box[0])) ||
-        (rc = map_mn(&m.dht[i], dh_i, kElem, T, I, 128, &box[1])))
+    if ((rc = map_k(&m.dh[i], dh_i, kElem, T, I, 128)) || (rc = map_mn(&m.w[i], &m.w2d[i], w13[i], kElem, I, H)) ||
+        (rc = map_mn(&m.dht[i], &m.dht2d[i], dh_i, kElem, T, I)))
       return rc;
   }
-  if ((rc = map_mn(&m.x, x, kElem, T, H, bn / 2, &box[2])) || (rc = map_mn(&m.dyt, d_out, kElem, T, H, 128, &box[3])) ||
-      (rc = map_mn(&m.a, a, kElem, T, I, bn / 2, &box[4])))
+  if ((rc = map_mn(&m.x, &m.x2d, x, kElem, T, H)) || (rc = map_mn(&m.dyt, &m.dyt2d, d_out, kElem, T, H)) ||
+      (rc = map_mn(&m.a, &m.a2d, a, kElem, T, I)))
     return rc;
   FfnGradParams g{};
   g.T = T;
@@ -472,7 +462,8 @@ int gated_ffn_grad(const void* x, const void* w1, const void* w2, const void* w3
   g.n_13 = (int)n_13;
   g.n_2 = (int)n_2;
   g.lead = g.kb_x / g.splits / g.kb_w;
-  for (int i = 0; i < 5; ++i) g.box3 |= box[i] << i;
+  g.full_h = whole_chunks(H);
+  g.full_i = whole_chunks(I);
   g.dx = d_x;
   g.dw13 = d_w13;
   g.dw2 = d_w2;
@@ -505,14 +496,14 @@ int launch_fp8(const void* a, const void* w, const void* w2, int K, Fp8BlockPara
 }
 
 int fp8_splits(int M, int N, int K, int sms, size_t cap) {
-  return pick_plan(M, 1, N, ceil_div(K, 128), std::max(1, sms / 2), (long long)M * N, kFp8BlockUs, kStoreUs, false, cap)
+  return pick_plan(M, N, ceil_div(K, 128), std::max(1, sms / 2), (long long)M * N, kFp8BlockUs, kStoreUs, false, cap)
       .splits;
 }
 
 // of a gate/up pair, whose tiles hold 128 features
 int fp8_gate_splits(int T, int I, int H, int sms, size_t cap) {
   if (T > 65535 * 8) return 1;  // the launch that adds the slices has a block for every 8 tokens
-  return pick_plan(T, 1, 2 * I, ceil_div(H, 128), std::max(1, sms / 2), 2ll * T * I, kFp8BlockUs, kGateUs, false, cap).splits;
+  return pick_plan(T, 2 * I, ceil_div(H, 128), std::max(1, sms / 2), 2ll * T * I, kFp8BlockUs, kGateUs, false, cap).splits;
 }
 
 // Whether an e4m3 product (gate: a gate/up pair of N features) of M tokens runs in
@@ -645,7 +636,7 @@ size_t ek_gated_ffn_workspace_bytes(int T, int H, int I, int num_sms) {
   if (T == 0) return 0;
   const size_t sums = T <= kStreamTokens
                           ? std::max(stream_bytes_most(I, 128, T, num_sms), stream_bytes_most(H, 256, T, num_sms))
-                          : std::max(gate_bytes(T, H, I, num_sms), ffn_store_bytes(T, H, I, 1, 1, num_sms));
+                          : std::max(gate_bytes(T, H, I, num_sms), ffn_store_bytes(T, H, I, num_sms));
   return round256((size_t)T * I * 2) + sums;
 }
 

@@ -1,21 +1,25 @@
 // Products of the gated feed-forward block on tcgen05 CTA pairs, bf16 and fp16.
 //
-//   gate/up   h1 = x W1^T, h3 = x W3^T, a = f(h1) h3          (kFfnGate)
-//   down      y = a W2^T                                      (kFfnStore, A and B K-major)
+//   gate/up   h1 = x W1^T, h3 = x W3^T, a = f(h1) h3          (ffn_gemm_kernel, kFfnGate)
+//   down      y = a W2^T                                      (kFfnStore)
 //   backward  da = dy W2; dh1 = da h3 f'(h1); dh3 = da f(h1)  (kFfnGateGrad)
-//             dx = dh1 W1 + dh3 W3                            (kFfnStore, two K planes)
-//             dW1 = dh1^T x, dW3 = dh3^T x, dW2 = dy^T a      (kFfnStore, A MN-major)
+//             dx = dh1 W1 + dh3 W3, dW1 = dh1^T x, dW3 = dh3^T x, dW2 = dy^T a
+//                                                             (ffn_grad_kernel)
 //
 // A persistent cluster of two CTAs computes a 256 x 256 (few tiles: 256 x 128) tile
 // with the 2-SM MMA: each CTA loads its own 128 rows of A and half of the tile's B
-// (32 KB per 64 of K, no multicast) and its TMEM receives its 128 rows. Operands are used where
-// they lie: an operand whose reduction axis is not the contiguous one (the
-// weights in a backward pass, everything under a weight's gradient) is read
-// MN-major by the MMA, so nothing is transposed. The two weights of the gate, and
-// the two planes of the pre-activations, are separate tensor maps: a plane is
-// chosen by the rank (gate/up: the first half of a tile's columns is W1's, the second
-// W3's), by the K block (dx sums over both planes) or by the tile's row (dW1 and
-// dW3 are one launch), so no tail of one plane is ever read as the other's.
+// (32 KB per 64 of K, no multicast) and its TMEM receives its 128 rows. Operands are
+// used where they lie: one whose reduction axis is not the contiguous one (the
+// weights in a backward pass, everything under a weight's gradient) is read MN-major
+// by the MMA, so nothing is transposed. The two weights of the gate, and the two
+// planes of the pre-activations, are separate tensor maps, so no tail of one is ever
+// read as the other's (gate/up: the first half of a tile's columns is W1's, the second
+// W3's, chosen by the CTA's rank).
+//
+// Bound by the tensor cores: 4096 x 4096 x 14336 in bf16 takes 925 us forward with the
+// pre-activations kept (1560 TFLOP/s, 0.95 of the measured burst) and 1791 us backward (1612,
+// 0.98), on a device whose power cap does not bind; the gate's gradient alone is bound by L2
+// (its five planes of activations beside the operands: 400 us, 335 without them).
 //
 //   warp 0      TMA producer; warp 1  TMEM and MMA issue
 //   warps 2..9  epilogue, two per TMEM lane quarter, half of the columns each
@@ -79,10 +83,10 @@ __device__ __forceinline__ bool mbar_wait_soon(uint64_t* bar, uint32_t parity, v
 
 enum FfnEpi : int { kFfnStore = 0, kFfnGate = 1, kFfnGateGrad = 2 };
 
-template <int kElem_, bool kAMN_, bool kBMN_, int kEpi_, int BN_>
+template <int kElem_, bool kBMN_, int kEpi_, int BN_>
 struct FfnCfg {
   static constexpr int kElem = kElem_;
-  static constexpr bool kAMN = kAMN_, kBMN = kBMN_;  // operand stored with its reduction axis outermost
+  static constexpr bool kBMN = kBMN_;  // B stored with its reduction axis outermost
   static constexpr int kEpi = kEpi_;
   static constexpr int BN = BN_, BK = 64;       // tile columns (gate/up: half gate, half up); K per stage
   static constexpr int A_BYTES = 128 * 128;     // a CTA's 128 rows (MN-major: two chunks of 64 columns) of A
@@ -92,23 +96,20 @@ struct FfnCfg {
   static constexpr int THREADS = 64 + 32 * EPI_WARPS;
   static constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + EPI_WARPS * 2048 + 1024 + 256;
   static constexpr uint32_t IDESC =
-      umma_idesc(kElem == kBF16 ? 1u : 0u, kBMN, 256, BN) | ((kAMN ? 1u : 0u) << 15);
+      umma_idesc(kElem == kBF16 ? 1u : 0u, kBMN, 256, BN);
 };
 
 struct FfnParams {
-  int M, N;              // rows and columns of the result (per plane)
-  int tiles_m, tiles_n;  // tiles_m counts the rows of all planes
-  int m_tiles_plane;     // row tiles of one plane (dW: two planes in M)
-  int k_blocks, kb_plane;  // K blocks in all and per plane (dx: two planes in K)
-  int splits, num_units;
-  int a_box3, b_box3;    // MN-major operand: its two 64-column chunks in one 3-D box
+  int M, N;              // rows and columns of the result
+  int tiles_m, tiles_n, k_blocks, splits, num_units;
+  int b_full;            // MN-major B: columns in whole 64-column chunks (see load_half)
   int gate;              // GateFn
   void* C;               // result; gate: a; gate gradient: dh
-  long long c_plane;     // elements between the planes of C (dW1 / dW3, dh1 / dh3)
+  long long c_plane;     // gate gradient: elements between dh1 and dh3
   void* H;               // gate: the pre-activations to write (or null); gate gradient: those to read
   long long h_plane;
   void* Act;             // gate gradient: a
-  float* ws;             // splits > 1: fp32 sums [splits][planes * M][N] (gate/up: [splits][M][2 N])
+  float* ws;             // splits > 1: fp32 sums [splits][M][N] (gate/up: [splits][M][2 N])
 };
 
 template <int kElem>
@@ -225,22 +226,26 @@ __device__ __forceinline__ void pack32(const uint32_t (&r)[32], uint4 (&v)[4]) {
   for (int g = 0; g < 4; ++g) v[g] = pack8<kElem>(reinterpret_cast<const float*>(r) + g * 8);
 }
 
-// A CTA's kRows of an operand's mn axis x 64 of K, from (mn, k0): K-major one box; MN-major
-// its 64-column chunks in one 3-D box or a box each
+// A CTA's kRows of an operand's mn axis x 64 of K, from (mn, k0): K-major one box. MN-major
+// 128 columns are two chunks of 64, the swizzle's width: one 3-D box of map m where both are
+// whole (the columns up to `full`, whatever follows them), else a 2-D box each of map m2,
+// whose bounds fill the rest with zeros. (8192 x 2048 x 14000, no multiple of 64: the
+// gradients take 2166 us so and 2253 with 2-D boxes throughout.)
 template <bool kMN, int kRows>
-__device__ __forceinline__ void load_half(uint8_t* dst, const CUtensorMap* m, uint32_t bar, int box3, int mn, int k0) {
+__device__ __forceinline__ void load_half(uint8_t* dst, const CUtensorMap* m, const CUtensorMap* m2, uint32_t bar, int full,
+                                          int mn, int k0) {
   if constexpr (!kMN) {
     tma_load_2d_pair(dst, m, bar, k0, mn);
-  } else if (kRows == 128 && box3) {
+  } else if (kRows == 128 && mn + 128 <= full) {
     tma_load_3d_pair(dst, m, bar, 0, k0, mn / 64);
   } else {
-    tma_load_2d_pair(dst, m, bar, mn, k0);
-    if constexpr (kRows == 128) tma_load_2d_pair(dst + 64 * 128, m, bar, mn + 64, k0);
+    tma_load_2d_pair(dst, m2, bar, mn, k0);
+    if constexpr (kRows == 128) tma_load_2d_pair(dst + 64 * 128, m2, bar, mn + 64, k0);
   }
 }
 
 struct FfnUnit {
-  int tm, tn, m_plane, m_row, split, kb0, kb1;
+  int tm, tn, split, kb0, kb1;
 };
 
 template <class Cfg>
@@ -249,8 +254,6 @@ __device__ __forceinline__ FfnUnit ffn_unit(const FfnParams& p, int u) {
   const int tile = u / p.splits;
   w.split = u - tile * p.splits;
   raster(tile, p.tiles_m, p.tiles_n, 8, w.tm, w.tn);
-  w.m_plane = w.tm >= p.m_tiles_plane ? 1 : 0;
-  w.m_row = (w.tm - w.m_plane * p.m_tiles_plane) * 256;
   w.kb0 = (int)((long long)w.split * p.k_blocks / p.splits);
   w.kb1 = (int)((long long)(w.split + 1) * p.k_blocks / p.splits);
   return w;
@@ -272,9 +275,8 @@ __device__ __forceinline__ void gate_grad8(const float* da, const float* h1, con
 
 template <class Cfg>
 __global__ void __launch_bounds__(Cfg::THREADS, 1)
-    ffn_gemm_kernel(const __grid_constant__ CUtensorMap tmA0, const __grid_constant__ CUtensorMap tmA1,
-                    const __grid_constant__ CUtensorMap tmB0, const __grid_constant__ CUtensorMap tmB1,
-                    const FfnParams p) {
+    ffn_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                    const __grid_constant__ CUtensorMap tmB2, const FfnParams p) {
   constexpr int STAGES = Cfg::STAGES, BN = Cfg::BN, BK = Cfg::BK, AB = Cfg::A_BYTES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -318,10 +320,9 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
 
   if (warp == 0) {
     if (elect_one()) {
-      tma_prefetch_desc(&tmA0);
-      tma_prefetch_desc(&tmB0);
-      tma_prefetch_desc(&tmA1);
-      tma_prefetch_desc(&tmB1);
+      tma_prefetch_desc(&tmA);
+      tma_prefetch_desc(&tmB);
+      tma_prefetch_desc(&tmB2);
     }
     __syncwarp();
     int stage = 0, issued = 0;
@@ -330,22 +331,20 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
     const uint32_t full0 = mapa_shared(smem_u32(&full_bar[0]), 0);  // both CTAs' loads complete on the leader's
     for (int u = unit0; u < p.num_units && ok; u += unit_step) {
       const FfnUnit w = ffn_unit<Cfg>(p, u);
-      const int a_mn = w.m_row + rank * 128;
+      const int a_mn = w.tm * 256 + rank * 128;
       const int b_mn = Cfg::kEpi == kFfnGate ? w.tn * (BN / 2) : w.tn * BN + rank * (BN / 2);
+      // tmB2: gate/up W3's map, MN-major B its 2-D map
+      const CUtensorMap* tb = Cfg::kEpi == kFfnGate && rank ? &tmB2 : &tmB;
       for (int kb = w.kb0; kb < w.kb1; ++kb) {
         ok = mbar_wait(&empty_bar[stage], phase ^ 1, s_abort);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        const int k_plane = kb >= p.kb_plane ? 1 : 0;
-        const int k0 = (kb - k_plane * p.kb_plane) * BK;
         if (elect_one()) {
-          const CUtensorMap* ta = (k_plane | w.m_plane) ? &tmA1 : &tmA0;
-          const CUtensorMap* tb = (Cfg::kEpi == kFfnGate ? rank : k_plane) ? &tmB1 : &tmB0;
           uint8_t* a_dst = smem + stage * Cfg::STAGE_BYTES;
           const uint32_t fb = full0 + stage * 8;
           if (leader) mbar_arrive_expect_tx(&full_bar[stage], 2 * Cfg::STAGE_BYTES);
-          load_half<Cfg::kAMN, 128>(a_dst, ta, fb, p.a_box3, a_mn, k0);
-          load_half<Cfg::kBMN, BN / 2>(a_dst + AB, tb, fb, p.b_box3, b_mn, k0);
+          tma_load_2d_pair(a_dst, &tmA, fb, kb * BK, a_mn);
+          load_half<Cfg::kBMN, BN / 2>(a_dst + AB, tb, &tmB2, fb, p.b_full, b_mn, kb * BK);
         }
         __syncwarp();
         ++issued;
@@ -360,8 +359,8 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
       uint32_t phase = 0;
       bool ok = true;
       // MN-major: 16 rows of K are 2 KB on, the 64-column chunks BK * 128 bytes apart
-      constexpr uint32_t a_step = Cfg::kAMN ? 2048 >> 4 : 32 >> 4, b_step = Cfg::kBMN ? 2048 >> 4 : 32 >> 4;
-      const uint64_t a_desc = umma_desc_sw128(smem_u32(smem), Cfg::kAMN ? BK * 128 : 16, 1024);
+      constexpr uint32_t b_step = Cfg::kBMN ? 2048 >> 4 : 32 >> 4;
+      const uint64_t a_desc = umma_desc_sw128(smem_u32(smem), 16, 1024);
       const uint64_t b_desc = umma_desc_sw128(smem_u32(smem) + AB, Cfg::kBMN ? BK * 128 : 16, 1024);
       for (int u = unit0; u < p.num_units && ok; u += unit_step, ++acc_i) {
         const FfnUnit w = ffn_unit<Cfg>(p, u);
@@ -380,7 +379,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
           if (elect_one()) {
 #pragma unroll
             for (int k = 0; k < BK / 16; ++k)
-              umma_pair<false>(d_tmem, a_desc + off + k * a_step, b_desc + off + k * b_step, Cfg::IDESC,
+              umma_pair<false>(d_tmem, a_desc + off + 2 * k, b_desc + off + k * b_step, Cfg::IDESC,
                                (kb > w.kb0 || k > 0) ? 1u : 0u);
             umma_commit_pair(&empty_bar[stage], 0x3);
             if (kb + 1 == w.kb1) umma_commit_pair(&tfull_bar[buf], 0x3);
@@ -410,7 +409,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
     for (int u = unit0; u < p.num_units; u += unit_step, ++acc_i) {
       const FfnUnit w = ffn_unit<Cfg>(p, u);
       const int buf = acc_i & 1;
-      const int row0 = w.m_row + rank * 128 + q * 32;  // first row of this warp
+      const int row0 = w.tm * 256 + rank * 128 + q * 32;  // first row of this warp
       const bool split = p.splits > 1;
       // gradient of the gate: the pre-activations of a 32-column chunk, 64 bytes of 8 rows a load
       uint4 n1[4], n3[4];
@@ -469,8 +468,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
           tmem_ld_wait(r);
           if (c == BN / 64 - 1) release(buf);
           if (split) {
-            const int planes = p.tiles_m / p.m_tiles_plane;
-            store_warp32(wt, r, p.ws + (size_t)(w.split * planes + w.m_plane) * p.M * p.N, row0, p.M, col, p.N, p.N);
+            store_warp32(wt, r, p.ws + (size_t)w.split * p.M * p.N, row0, p.M, col, p.N, p.N);
             continue;
           }
           uint4 v[4];
@@ -506,7 +504,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
             store_warp<8>(wt, va, p.Act, row0, p.M, col, p.N);
           } else {
             pack32<Cfg::kElem>(r, v);
-            store_warp<8>(wt, v, reinterpret_cast<uint16_t*>(p.C) + w.m_plane * p.c_plane, row0, p.M, col, p.N);
+            store_warp<8>(wt, v, p.C, row0, p.M, col, p.N);
           }
         }
       }
@@ -527,12 +525,14 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
 // (two planes in M) and dW2 = dy^T a in one launch: they wait for the same thing, and the
 // pairs that a product's last round leaves idle go on with the next product's tiles. dx's
 // units come first, pair by pair; then the weights' tiles, all of one length, of which the
-// pairs without a unit in dx's last round take `lead` rounds more. Against one launch each,
-// 4096 x 4096 x 14336 takes XX us for YY and 333 x 1032 x 2760 XX for YY.
+// pairs without a unit in dx's last round take `lead` rounds more. 333 x 1032 x 2760 takes
+// 27 us so and 35 in a launch each; at 2048 x 4096 x 4736 the tensor pipe is busy in 95 % of
+// the active cycles.
 struct FfnGradMaps {
   CUtensorMap dh[2], w[2];    // dx: dh's planes K-major, W1 and W3
   CUtensorMap dht[2], x;      // dW1, dW3: dh's planes and x, T outermost
   CUtensorMap dyt, a;         // dW2: dy and a
+  CUtensorMap w2d[2], dht2d[2], x2d, dyt2d, a2d;  // 2-D maps of the MN-major ones (load_half)
 };
 struct FfnGradParams {
   int T, H, I;
@@ -541,7 +541,7 @@ struct FfnGradParams {
   int tm_2, tn_2, n_2;                          // dW2
   int kb_w;                                     // K blocks of a weight's tile
   int lead;
-  int box3;                                     // bits: w, dht, x, dyt, a in 3-D boxes
+  int full_h, full_i;                           // columns of H and I in whole chunks (load_half)
   void *dx, *dw13, *dw2;
   float* ws;
 };
@@ -633,17 +633,17 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
   if (warp == 0) {
     if (elect_one()) {
       const CUtensorMap* m = maps.dh;
-      for (int i = 0; i < 9; ++i) tma_prefetch_desc(m + i);
+      for (int i = 0; i < 16; ++i) tma_prefetch_desc(m + i);
     }
     __syncwarp();
     int stage = 0, issued = 0;
     uint32_t phase = 0;
     bool ok = true;
     const uint32_t full0 = mapa_shared(smem_u32(&full_bar[0]), 0);  // both CTAs' loads complete on the leader's
-    // K blocks [kb0, kb1) of a unit through one pair of maps, its k0 counted from block `from`
-    auto blocks = [&](auto a_mn_major, const CUtensorMap* ta, const CUtensorMap* tb, int a3, int b3, int a_mn, int b_mn,
-                      int kb0, int kb1, int from) {
-      constexpr bool kAMN = decltype(a_mn_major)::value;
+    // K blocks [kb0, kb1) of a unit through one set of maps, K counted from block `from`
+    auto blocks = [&](auto a_mn_major, const CUtensorMap* ta, const CUtensorMap* ta2, int a_full, const CUtensorMap* tb,
+                      const CUtensorMap* tb2, int b_full, int kb0, int kb1, int from) {
+      const int a_mn = w.tm * 256 + rank * 128, b_mn = w.tn * BN + rank * (BN / 2);
       for (int kb = kb0; kb < kb1; ++kb) {
         ok = mbar_wait(&empty_bar[stage], phase ^ 1, s_abort);
         ok = __all_sync(0xffffffffu, ok);
@@ -652,8 +652,8 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
           uint8_t* a_dst = smem + stage * Cfg::STAGE_BYTES;
           const uint32_t fb = full0 + stage * 8;
           if (leader) mbar_arrive_expect_tx(&full_bar[stage], 2 * Cfg::STAGE_BYTES);
-          load_half<kAMN, 128>(a_dst, ta, fb, a3, a_mn, (kb - from) * BK);
-          load_half<true, BN / 2>(a_dst + AB, tb, fb, b3, b_mn, (kb - from) * BK);
+          load_half<decltype(a_mn_major)::value, 128>(a_dst, ta, ta2, fb, a_full, a_mn, (kb - from) * BK);
+          load_half<true, BN / 2>(a_dst + AB, tb, tb2, fb, b_full, b_mn, (kb - from) * BK);
         }
         __syncwarp();
         ++issued;
@@ -661,17 +661,16 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
       }
     };
     for (int k = 0; ok && ffn_grad_unit(p, pair, pairs, k, w); ++k) {
-      const int a_mn = w.tm * 256 + rank * 128, b_mn = w.tn * BN + rank * (BN / 2);
       if (w.job == 0) {
-        blocks(std::false_type{}, &maps.dh[0], &maps.w[0], 0, p.box3 & 1, a_mn, b_mn, w.kb0, min(w.kb1, p.kb_plane), 0);
+        const int mid = p.kb_plane;
+        blocks(std::false_type{}, &maps.dh[0], nullptr, 0, &maps.w[0], &maps.w2d[0], p.full_h, w.kb0, min(w.kb1, mid), 0);
         if (ok)
-          blocks(std::false_type{}, &maps.dh[1], &maps.w[1], 0, p.box3 & 1, a_mn, b_mn, max(w.kb0, p.kb_plane), w.kb1,
-                 p.kb_plane);
+          blocks(std::false_type{}, &maps.dh[1], nullptr, 0, &maps.w[1], &maps.w2d[1], p.full_h, max(w.kb0, mid), w.kb1, mid);
       } else if (w.job == 1) {
-        blocks(std::true_type{}, w.plane ? &maps.dht[1] : &maps.dht[0], &maps.x, p.box3 >> 1 & 1, p.box3 >> 2 & 1, a_mn,
-               b_mn, w.kb0, w.kb1, 0);
+        blocks(std::true_type{}, &maps.dht[w.plane], &maps.dht2d[w.plane], p.full_i, &maps.x, &maps.x2d, p.full_h, w.kb0,
+               w.kb1, 0);
       } else {
-        blocks(std::true_type{}, &maps.dyt, &maps.a, p.box3 >> 3 & 1, p.box3 >> 4 & 1, a_mn, b_mn, w.kb0, w.kb1, 0);
+        blocks(std::true_type{}, &maps.dyt, &maps.dyt2d, p.full_h, &maps.a, &maps.a2d, p.full_i, w.kb0, w.kb1, 0);
       }
     }
     if (!ok && leader) wait_copies<STAGES>(full_bar, issued);

@@ -10,6 +10,9 @@
 // epilogue warps read the product, multiply it by its one scale per row and weight
 // block and add it to fp32 accumulators in registers.
 //
+// 4096 x 14336 x 4096 takes 220 us (2190 TFLOP/s; the product with a scale per row, whose
+// MMA never waits for an epilogue, 176).
+//
 //   warp 0  TMA producer; warp 1  TMEM and MMA; warps 2, 3  idle
 //   warps 4..11  epilogue, two per TMEM lane quarter, 128 accumulators a thread: group
 //   g has of a plain tile the columns [128 g, +128), of a gate tile 64 gate columns

@@ -19,6 +19,11 @@
 //   warp 0  TMA producer; warp 1  TMEM and MMA; warp 2  scales (e4m3)
 //   warps 3..10  epilogue: two per TMEM lane quarter, one 128-row block each
 //
+// Measured (calls back to back in a graph): one token through the bf16 block of 4096 x
+// 14336 61.5 us, 5.7 TB/s of weights; 14336 x 4096 in 8 bits 11, 12.2, 13.9 and 18.7 us for
+// 1, 16, 32 and 64 tokens (bound at 64 by the epilogue's chain of waits per K block and the
+// token rows beside the weights, 40 KB a unit).
+//
 // A tile cut over a cluster instead, its parts added over distributed shared memory in the
 // same launch, was tried and left out: an SM draws about 46 GB/s, so what counts is that
 // all of them stream, and whole tiles over clusters of 4 and 8 leave too many without work
