@@ -485,36 +485,47 @@ __global__ void __launch_bounds__(256)
 
 // e4m3 codes [T][H] and scales [T][ceil(H / 128)] of bf16 rows: a scale per 128 elements
 // (largest magnitude / 448, 1 for zeros), IEEE quotients, as the row quantisation of the
-// library. A half warp per group, 8 elements a lane; H a multiple of 8. Memory bound at
-// many tokens, a launch at few: it lets the product after it fetch weights meanwhile.
+// library. A half warp per group, 8 elements a lane, the loads of kU pairs of groups in
+// flight; H a multiple of 8. Memory bound at many tokens, a launch at few: it lets the
+// product after it fetch weights meanwhile.
+template <int kU>
 __global__ void __launch_bounds__(256) ffn_quant_kernel(const __nv_bfloat16* __restrict__ x, long long groups, int H,
                                                         uint8_t* __restrict__ codes, float* __restrict__ scales) {
   pdl_wait();
   pdl_launch();
   const int per_row = (H + 127) / 128, hl = threadIdx.x & 15;
   // the bound is uniform over the warp, so that every lane reaches the exchanges
-  for (long long g0 = (blockIdx.x * 256ll + threadIdx.x) / 32 * 2; g0 < groups; g0 += gridDim.x * 16ll) {
-    const long long g = g0 + ((threadIdx.x >> 4) & 1);
-    const long long row = g / per_row;
-    const int c = (int)(g - row * per_row) * 128 + hl * 8;
-    const bool in = g < groups && c < H;
-    float v[8];
-    unpack8<kBF16>(in ? __ldg(reinterpret_cast<const uint4*>(x + row * H + c)) : make_uint4(0, 0, 0, 0), v);
-    float m = 0.f;
+  for (long long g0 = (blockIdx.x * 256ll + threadIdx.x) / 32 * (2 * kU); g0 < groups; g0 += gridDim.x * (16ll * kU)) {
+    uint4 raw[kU];
+    long long at[kU];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(v[j]));
+    for (int i = 0; i < kU; ++i) {
+      const long long g = g0 + 2 * i + ((threadIdx.x >> 4) & 1), row = g / per_row;
+      const int c = (int)(g - row * per_row) * 128 + hl * 8;
+      at[i] = g < groups && c < H ? row * H + c : -1;
+      raw[i] = at[i] >= 0 ? __ldg(reinterpret_cast<const uint4*>(x + at[i])) : make_uint4(0, 0, 0, 0);
+    }
 #pragma unroll
-    for (int o = 8; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float s = m > 0.f ? m / 448.0f : 1.0f;
-    if (!in) continue;
-    uint32_t pk[2];
+    for (int i = 0; i < kU; ++i) {
+      float v[8];
+      unpack8<kBF16>(raw[i], v);
+      float m = 0.f;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      pk[i] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[4 * i] / s, v[4 * i + 1] / s), __NV_SATFINITE, __NV_E4M3) |
-              ((uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[4 * i + 2] / s, v[4 * i + 3] / s), __NV_SATFINITE, __NV_E4M3)
-               << 16);
-    *reinterpret_cast<uint2*>(codes + row * H + c) = make_uint2(pk[0], pk[1]);
-    if (hl == 0) scales[g] = s;
+      for (int j = 0; j < 8; ++j) m = fmaxf(m, fabsf(v[j]));
+#pragma unroll
+      for (int o = 8; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      const float s = m > 0.f ? m / 448.0f : 1.0f;
+      if (at[i] < 0) continue;
+      uint32_t pk[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        pk[j] =
+            (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[4 * j] / s, v[4 * j + 1] / s), __NV_SATFINITE, __NV_E4M3) |
+            ((uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[4 * j + 2] / s, v[4 * j + 3] / s), __NV_SATFINITE, __NV_E4M3)
+             << 16);
+      *reinterpret_cast<uint2*>(codes + at[i]) = make_uint2(pk[0], pk[1]);
+      if (hl == 0) scales[g0 + 2 * i + ((threadIdx.x >> 4) & 1)] = s;
+    }
   }
 }
 

@@ -431,6 +431,12 @@ def test_gated_ffn_fp8(T, H, I, act, cuda_dev):
     assert torch.equal(out, y)
 
 
+def test_gated_ffn_fp8_many_groups(cuda_dev):
+    """So many groups that the quantisation takes several a turn, the last of a row short,
+    the rows' end inside a turn."""
+    _check_fp8(*_ffn_case(38011, 528, 144, BF), "silu")
+
+
 def test_gated_ffn_fp8_is_its_stages(cuda_dev):
     """The block's second product is gemm_fp8_block over quantised activations: with
     weights that make every pre-activation exact, the stages agree bit for bit."""
@@ -553,6 +559,61 @@ def test_in_a_graph(T, cuda_dev):
             for ts, rs in zip(o, refs):
                 for t, r in zip(ts, rs):
                     assert torch.equal(t, r)
+
+
+@pytest.mark.parametrize("T", [2, 300])
+def test_in_a_graph_behind_copies_and_joined_streams(T, cuda_dev):
+    """A captured call whose predecessors are a copy, a launch of another stream that was
+    joined, and a fill of the inputs themselves."""
+    x, w1, w2, w3 = _ffn_case(T, 272, 528, BF)
+    qw = _ops.quant_ffn_weights_fp8(w1, w2, w3)
+    refs = [_ops.gated_ffn(x, w1, w2, w3), _ops.gated_ffn_fp8(x, qw), _ops.gated_ffn(x * 2, w1, w2, w3)]
+    src, at, weight = x.clone(), torch.zeros_like(x), torch.zeros_like(w2)
+    side, s = torch.cuda.Stream(), torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(s):
+        with torch.cuda.graph(g, stream=s):
+            at.copy_(src)
+            first = _ops.gated_ffn(at, w1, w2, w3)
+            side.wait_stream(s)
+            with torch.cuda.stream(side):
+                weight.copy_(w2)
+                second = _ops.gated_ffn_fp8(at, qw)
+            s.wait_stream(side)
+            at.mul_(2)
+            third = _ops.gated_ffn(at, w1, weight, w3)
+    for _ in range(3):
+        weight.zero_()
+        for o in (first, second, third):
+            o.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        for o, r in zip((first, second, third), refs):
+            assert torch.equal(o, r)
+
+
+@pytest.mark.parametrize("T", [2, 300])
+def test_weights_written_right_before_the_call(T, cuda_dev):
+    """The weights' last writer is the launch before the call: no launch of the call may
+    fetch them earlier."""
+    x, w1, w2, w3 = _ffn_case(T, 1032, 2056, BF)
+    ref = _ops.gated_ffn(x, w1, w2, w3)
+    h = _ops.gated_ffn(x, w1, w2, w3, save=True)[1]
+    grads = _ops.gated_ffn_grad(x, w1, w2, w3, h, x)
+    live = [torch.empty_like(w) for w in (w1, w2, w3)]
+    for _ in range(20):
+        for t in live:
+            t.fill_(float("nan"))
+        for t, w in zip(live, (w1, w2, w3)):
+            t.copy_(w)
+        assert torch.equal(_ops.gated_ffn(x, *live), ref)
+        for t in live:
+            t.fill_(float("nan"))
+        for t, w in zip(live, (w1, w2, w3)):
+            torch.mul(w, 1, out=t)
+        for a, b in zip(_ops.gated_ffn_grad(x, *live, h, x), grads):
+            assert torch.equal(a, b)
 
 
 def test_two_streams_at_once(cuda_dev):
