@@ -1280,8 +1280,8 @@ def gated_ffn_fp8(x: torch.Tensor, qw: dict, act: str = "silu", out: torch.Tenso
     and y [T, H], H and I multiples of 16.
 
     The tokens, and the activations from their fp32 sums, are quantised per 1 x 128
-    group as quant_e4m3(x, block=(1, 128)) does; both products are
-    gemm_fp8_block's. The result is rounded once."""
+    group as quant_e4m3(x, block=(1, 128)) does (the activations' scales not below
+    2^-126); both products are gemm_fp8_block's. The result is rounded once."""
     H, I = int(qw["H"]), int(qw["I"])
     w1, w3, w2, s1, s3, s2 = (qw[n] for n in ("w1q", "w3q", "w2q", "w1s", "w3s", "w2s"))
     dev = _require_cuda(x, w1, w2, w3, s1, s2, s3, out)

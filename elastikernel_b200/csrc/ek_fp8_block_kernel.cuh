@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
         m = fmaxf(m, s_amax[(wg ^ 1) * 128 + lrow]);
         named_bar_sync(1, 32 * Cfg::EPI_WARPS);
         // an activation times the scale's reciprocal is within an ulp of the quotient
-        const float s = m > 0.f ? m / 448.0f : 1.0f, rs = 1.0f / s;
+        const float s = act_scale(m), rs = 1.0f / s;
         uint4 pk[4];
 #pragma unroll
         for (int g = 0; g < 4; ++g) {

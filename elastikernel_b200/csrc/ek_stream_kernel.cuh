@@ -107,9 +107,13 @@ struct StreamOut {
   float* scales;
 };
 
+// The scale of a group of activations whose largest magnitude is m: m / 448, 1 for zeros.
+// Not below 2^-126: under that its reciprocal overflows, further down it is zero itself, and
+// a zero beside such values would become NaN.
+__device__ __forceinline__ float act_scale(float m) { return m > 0.f ? fmaxf(m / 448.0f, 0x1p-126f) : 1.0f; }
+
 // a[t, f] = f(h1) h3 for 4 features a lane, from feature f on, and h1 and h3 on request;
-// with codes, a in e4m3 with the scale of the warp's 128 features (largest magnitude / 448,
-// 1 for zeros). Rows past the weight's hold zeros.
+// with codes, a in e4m3 with the scale of the warp's 128 features (act_scale). Rows past the weight's hold zeros.
 __device__ __forceinline__ void finish_gate(const StreamOut& o, int t, int tile, const float4& h1, const float4& h3) {
   const int f = tile * 128 + (threadIdx.x & 31) * 4, I = o.N;
   float4 act;
@@ -129,7 +133,7 @@ __device__ __forceinline__ void finish_gate(const StreamOut& o, int t, int tile,
   float m = fmaxf(fmaxf(fabsf(act.x), fabsf(act.y)), fmaxf(fabsf(act.z), fabsf(act.w)));  // zeros past I
 #pragma unroll
   for (int i = 16; i; i >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, i));
-  const float s = m > 0.f ? m / 448.0f : 1.0f;
+  const float s = act_scale(m);
   if (f < I) {
     const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(act.x / s, act.y / s), __NV_SATFINITE, __NV_E4M3);
     const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(act.z / s, act.w / s), __NV_SATFINITE, __NV_E4M3);
@@ -484,8 +488,8 @@ __global__ void __launch_bounds__(256)
 }
 
 // e4m3 codes [T][H] and scales [T][ceil(H / 128)] of bf16 rows: a scale per 128 elements
-// (largest magnitude / 448, 1 for zeros), IEEE quotients, as the row quantisation of the
-// library. A half warp per group, 8 elements a lane, the loads of kU pairs of groups in
+// (largest magnitude / 448, 1 for zeros; of bf16 values never zero itself), IEEE quotients,
+// as the row quantisation of the library. A half warp per group, 8 elements a lane, the loads of kU pairs of groups in
 // flight; H a multiple of 8. Memory bound at many tokens, a launch at few: it lets the
 // product after it fetch weights meanwhile.
 template <int kU>

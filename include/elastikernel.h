@@ -609,7 +609,7 @@ int ek_gated_ffn_grad(const void* x, const void* w1, const void* w2, const void*
 /* The block over e4m3 weights with 128 x 128 block scales (s1, s3 [ceil(I / 128),
  * ceil(H / 128)], s2 [ceil(H / 128), ceil(I / 128)]); x and y bf16 [T, H], H and I
  * multiples of 16. x, and a from its fp32 sums, are quantised per 1 x 128 group as
- * ek_quant_e4m3 does (largest magnitude / 448). */
+ * ek_quant_e4m3 does (largest magnitude / 448; a's scales not below 2^-126). */
 size_t ek_gated_ffn_fp8_workspace_bytes(int T, int H, int I, int num_sms);
 int ek_gated_ffn_fp8(const void* x, const void* w1, const void* w2, const void* w3, const float* s1, const float* s2,
                      const float* s3, void* y, int T, int H, int I, int gate, int num_sms, void* workspace,

@@ -437,6 +437,31 @@ def test_gated_ffn_fp8_many_groups(cuda_dev):
     _check_fp8(*_ffn_case(38011, 528, 144, BF), "silu")
 
 
+@pytest.mark.parametrize("T", [3, 40, 200, 700])
+@pytest.mark.parametrize("by,back", [(2.0 ** -62, 2.0 ** 118), (2.0 ** -74, 1.0)])
+def test_gated_ffn_fp8_of_vanishing_activations(T, by, back, cuda_dev):
+    """Activations whose scale has no reciprocal in fp32, or is none itself, with exact
+    zeros among them.
+
+    A code is off by at most 2^-4 of a value, or half a step of the least code, 2^-10, of a
+    scale that is at most largest / 448 + 2^-126; 2^-3 more of either for the quotient's
+    rounding; a itself by the sums' errors and half an fp32 denormal step, 2^-150, twice."""
+    H, I = 528, 400
+    x, w1, w2, w3 = _ffn_case(T, H, I, BF)
+    w3[::5] = 0
+    qw = _ops.quant_ffn_weights_fp8(w1, w2, w3)
+    qw["w1s"], qw["w3s"], qw["w2s"] = qw["w1s"] * by, qw["w3s"] * by, qw["w2s"] * back
+    W1, W2, W3 = (off.expand(qw[n + "q"], qw[n + "s"], 128) for n in ("w1", "w2", "w3"))
+    X = off.e4m3_groups(x.double())
+    h1, h3 = X @ W1.T, X @ W3.T
+    a = off.gate(h1, "silu") * h3
+    da = _acc(H) * ((X.abs() @ W1.abs().T) * (off.slope(h1, "silu") * h3).abs() +
+                    (X.abs() @ W3.abs().T) * off.gate(h1, "silu").abs()) + 2.0 ** -20 * (h1 * h3).abs() + 2.0 ** -149
+    top = (a.abs() + da).amax(dim=1, keepdim=True)
+    code = (1 + 2.0 ** -3) * (2.0 ** -4 * (a.abs() + da) + 2.0 ** -10 * (top / 448 + 2.0 ** -126))
+    _within("y", _ops.gated_ffn_fp8(x, qw), a @ W2.T, (da + code + _acc(I) * (a.abs() + da + code)) @ W2.abs().T)
+
+
 def test_gated_ffn_fp8_is_its_stages(cuda_dev):
     """The block's second product is gemm_fp8_block over quantised activations: with
     weights that make every pre-activation exact, the stages agree bit for bit."""
