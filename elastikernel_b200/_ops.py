@@ -1116,7 +1116,7 @@ def fused_moe_w4(hidden_states: torch.Tensor, gate_logits: torch.Tensor, qw: dic
 # ---------------------------------------------------- dense feed-forward blocks
 GATES = {"silu": _lib.EK_GATE_SILU, "gelu": _lib.EK_GATE_GELU, "gelu_tanh": _lib.EK_GATE_GELU_TANH}
 _MAX_FFN_DIM = 1 << 28  # of H and I, and _MAX_TOKENS of the rows: the library's ints
-_MAX_TOKENS = 0x7fffffff
+_MAX_TOKENS = (1 << 31) - 256
 
 
 def _check_matrix(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple) -> torch.Tensor:
@@ -1146,16 +1146,17 @@ def gemm_fp8_block(a_q: torch.Tensor, w_q: torch.Tensor, a_scale: torch.Tensor, 
     a_scale [M, ceil(K/128)] holds a scale per 1 x 128 group of a row, w_scale
     [ceil(N/128), ceil(K/128)] one per 128 x 128 block, both fp32 of any value:
     what quant_e4m3(x, block=(1, 128)) and quant_e4m3(w, block=(128, 128)) give.
-    K is a multiple of 16; M, N and the last block of each axis are any size. The
-    sums are fp32; C is bf16, fp16 or fp32 (`dtype`, or out's), rounded once."""
+    K is a multiple of 16; M, N (up to 2^31 - 256) and the last block of each axis
+    are any size. The sums are fp32; C is bf16, fp16 or fp32 (`dtype`, or out's),
+    rounded once."""
     dev = _require_cuda(a_q, w_q, a_scale, w_scale, out)
     shape = a_q.shape
     if _FP8 is None or len(shape) != 2 or w_q.dim() != 2:
         raise RuntimeError("gemm_fp8_block takes 2-D float8_e4m3fn operands")
     (M, K), N = shape, w_q.shape[0]
     if K == 0 or K % 16 or K > _MAX_FFN_DIM or max(M, N) > _MAX_TOKENS:
-        raise RuntimeError(f"gemm_fp8_block: K must be a positive multiple of 16 up to 2^28, M and N within 2^31 "
-                           f"(got {M} x {N} x {K})")
+        raise RuntimeError(f"gemm_fp8_block: K must be a positive multiple of 16 up to 2^28, M and N up to "
+                           f"2^31 - 256 (got {M} x {N} x {K})")
     a_q = _check_matrix("a_q", a_q, _FP8, (M, K))
     w_q = _check_matrix("w_q", w_q, _FP8, (N, K))
     a_scale = _check_matrix("a_scale", a_scale, torch.float32, (M, _blocks128(K)))
@@ -1195,7 +1196,7 @@ def _check_ffn(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, w3: torch.Te
         raise RuntimeError("x must be [T, H] and w1 [I, H]")
     (T, H), I = x.shape, w1.shape[0]
     if not (0 < H <= _MAX_FFN_DIM and 0 < I <= _MAX_FFN_DIM) or H % unit or I % unit or T > _MAX_TOKENS:
-        raise RuntimeError(f"H and I must be positive multiples of {unit} up to 2^28, T within 2^31 "
+        raise RuntimeError(f"H and I must be positive multiples of {unit} up to 2^28, T up to 2^31 - 256 "
                            f"(got T={T}, H={H}, I={I})")
     wt = dtype if unit == 8 else _FP8
     return (_check_matrix("x", x, dtype, (T, H)), _check_matrix("w1", w1, wt, (I, H)),
@@ -1207,10 +1208,10 @@ def gated_ffn(x: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, w3: torch.Ten
     """Dense gated feed-forward block: y = (f(x W1^T) * (x W3^T)) W2^T.
 
     x [T, H], w1 and w3 [I, H], w2 [H, I] in bf16 or fp16 (H and I multiples of 8,
-    any T); f is "silu", "gelu" or "gelu_tanh". Sums are fp32; the activations are
-    rounded to x's dtype between the two products. With save=True returns (y, h),
-    h [2, T, I] the rounded pre-activations x W1^T and x W3^T that gated_ffn_grad
-    takes."""
+    T up to 2^31 - 256); f is "silu", "gelu" or "gelu_tanh". Sums are fp32; the
+    activations are rounded to x's dtype between the two products. With save=True
+    returns (y, h), h [2, T, I] the rounded pre-activations x W1^T and x W3^T that
+    gated_ffn_grad takes."""
     dev = _require_cuda(x, w1, w2, w3, out)
     if x.dtype not in _DTYPES:
         raise RuntimeError("gated_ffn takes bf16 or fp16")

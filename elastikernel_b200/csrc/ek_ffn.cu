@@ -573,15 +573,19 @@ Fp8FfnLayout fp8_ffn_layout(int T, int H, int I, int sms) {
 }
 
 // ------------------------------------------------------------------ checks
+constexpr int kMostRows = 0x7fffff00;  // a tile of 256 rows ends within an int
+bool block_sizes_ok(int M, int N, int K) {
+  return M >= 0 && M <= kMostRows && N >= 0 && N <= kMostRows && K > 0 && K % 16 == 0 && K <= (1 << 28);
+}
 bool sizes_ok(int T, int H, int I, int unit) {
-  return T >= 0 && H > 0 && I > 0 && H % unit == 0 && I % unit == 0 && H <= (1 << 28) && I <= (1 << 28);
+  return T >= 0 && T <= kMostRows && H > 0 && I > 0 && H % unit == 0 && I % unit == 0 && H <= (1 << 28) && I <= (1 << 28);
 }
 bool sms_ok(int sms) { return sms > 0 && sms <= kGemmMaxSms; }
 
 int check_ffn(int T, int H, int I, int unit, int gate) {
   if (!sizes_ok(T, H, I, unit))
-    return set_error(EK_ERR_INVALID, "feed-forward: H and I must be positive multiples of %d up to 2^28 (got T=%d H=%d I=%d)",
-                     unit, T, H, I);
+    return set_error(EK_ERR_INVALID, "feed-forward: H and I must be positive multiples of %d up to 2^28, T up to 2^31 - 256 "
+                     "(got T=%d H=%d I=%d)", unit, T, H, I);
   if (gate < kGateSilu || gate > kGateGeluTanh) return set_error(EK_ERR_INVALID, "unknown gate function %d", gate);
   return EK_OK;
 }
@@ -610,15 +614,16 @@ using namespace ek;
 extern "C" {
 
 size_t ek_gemm_fp8_block_workspace_bytes(int M, int N, int K, int num_sms) {
-  if (M < 0 || N < 0 || K <= 0 || K % 16 || !sms_ok(num_sms)) return kBad;
+  if (!block_sizes_ok(M, N, K) || !sms_ok(num_sms)) return kBad;
   return M == 0 || N == 0 ? 0 : fp8_store_bytes(M, N, K, num_sms);
 }
 
 int ek_gemm_fp8_block(const void* A, const void* W, const float* a_scale, const float* w_scale, void* C, int M, int N,
                       int K, int out_dtype, int num_sms, void* workspace, size_t ws_bytes, void* stream) {
   clear_error();
-  if (M < 0 || N < 0 || K <= 0 || K % 16)
-    return set_error(EK_ERR_INVALID, "block-scaled product: K must be a positive multiple of 16 (got %d x %d x %d)", M, N, K);
+  if (!block_sizes_ok(M, N, K))
+    return set_error(EK_ERR_INVALID, "block-scaled product: K must be a positive multiple of 16 up to 2^28, M and N up to "
+                     "2^31 - 256 (got %d x %d x %d)", M, N, K);
   if (out_dtype != kOutBF16 && out_dtype != kOutFP16 && out_dtype != kOutFP32)
     return set_error(EK_ERR_INVALID, "block-scaled product: result in bf16, fp16 or fp32 (got dtype %d)", out_dtype);
   if (M == 0 || N == 0) return EK_OK;

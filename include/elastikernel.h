@@ -577,19 +577,19 @@ int ek_fused_moe_w4(const void* x, const float* logits, int T, int topk, const v
  * A [M, K] and W [N, K] e4m3, blocks of 128 along K (the last may be short),
  * a_scale [M, ceil(K / 128)] and w_scale [ceil(N / 128), ceil(K / 128)] fp32 of any
  * value. Products of a block and the sum over blocks are fp32; C [M, N] is bf16,
- * fp16 or fp32 (out_dtype), rounded once. K a multiple of 16, any M and N; A, W and
- * the workspace 16-byte aligned. workspace: ek_gemm_fp8_block_workspace_bytes
- * bytes for the launch's SMs or more; its contents before and after do not
- * matter, but no two calls in flight may share it. */
+ * fp16 or fp32 (out_dtype), rounded once. K a multiple of 16 up to 2^28, M and N up
+ * to 2^31 - 256; A, W and the workspace 16-byte aligned. workspace:
+ * ek_gemm_fp8_block_workspace_bytes bytes for the launch's SMs or more; its contents
+ * before and after do not matter, but no two calls in flight may share it. */
 size_t ek_gemm_fp8_block_workspace_bytes(int M, int N, int K, int num_sms);
 int ek_gemm_fp8_block(const void* A, const void* W, const float* a_scale, const float* w_scale, void* C, int M, int N,
                       int K, int out_dtype, int num_sms, void* workspace, size_t ws_bytes, void* stream);
 
 /* Gated feed-forward block, bf16 or fp16, fp32 sums:
  *   h1 = x W1^T, h3 = x W3^T, a = f(h1) h3, y = a W2^T
- * x [T, H], w1 and w3 [I, H], w2 [H, I], y [T, H]; H and I multiples of 8. a comes
- * from the unrounded sums and is rounded to the inputs' type between the two
- * products. h (may be NULL): h1 and h3 rounded, [2, T, I], for the gradient.
+ * x [T, H], w1 and w3 [I, H], w2 [H, I], y [T, H]; H and I multiples of 8 up
+ * to 2^28, T up to 2^31 - 256 (here and in the forms below). a comes from the
+ * unrounded sums and is rounded to the inputs' type between the two products. h (may be NULL): h1 and h3 rounded, [2, T, I], for the gradient.
  * All pointers 16-byte aligned; workspace as above. */
 size_t ek_gated_ffn_workspace_bytes(int T, int H, int I, int num_sms);
 int ek_gated_ffn(const void* x, const void* w1, const void* w2, const void* w3, void* y, void* h, int T, int H, int I,

@@ -150,6 +150,19 @@ def test_gated_ffn_fp8_refusals():
     assert f(4, 24, 32, 148) == f(4, 16, 32, 2000) == _ops._SIZE_MAX and f(0, 16, 32, 148) == 0
 
 
+def test_sizes_whose_last_tile_passes_an_int_are_refused():
+    L, top = lib(), (1 << 31) - 1
+    for n in (top - 254, top):
+        _bad(L.ek_gemm_fp8_block(_p(), _p(), _p(), _p(), _p(), n, 16, 16, 0, 148, _p(), BIG, None), "2^31")
+        _bad(L.ek_gemm_fp8_block(_p(), _p(), _p(), _p(), _p(), 16, n, 16, 0, 148, _p(), BIG, None), "2^31")
+        _bad(L.ek_gated_ffn(*[_p()] * 6, n, 16, 16, 0, 0, 148, _p(), BIG, None), "2^31")
+        _bad(L.ek_gated_ffn_grad(*[_p()] * 9, n, 16, 16, 0, 0, 148, _p(), BIG, None), "2^31")
+        _bad(L.ek_gated_ffn_fp8(*[_p()] * 8, n, 16, 16, 0, 148, _p(), BIG, None), "2^31")
+        assert L.ek_gated_ffn_workspace_bytes(n, 16, 16, 148) == _ops._SIZE_MAX
+    _bad(L.ek_gemm_fp8_block(_p(), _p(), _p(), _p(), _p(), 16, 16, top - 15, 0, 148, _p(), BIG, None), "2^28")
+    assert L.ek_gated_ffn_workspace_bytes(top - 255, 16, 16, 148) < _ops._SIZE_MAX
+
+
 @pytest.mark.parametrize("T,H,I", [(1, 8, 8), (64, 4096, 14336), (128, 256, 384), (129, 4096, 264), (4096, 4096, 14336)])
 def test_workspaces_hold_any_smaller_partition(T, H, I):
     """A call sized for the whole device may run in a partition of it, for which the
