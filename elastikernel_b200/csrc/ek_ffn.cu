@@ -100,10 +100,10 @@ int grid_for(long long work, int sms) { return (int)std::max<long long>(1, std::
 // run beside the epilogue of the unit before it (epi_us, kSliceUs for a slice), so it takes
 // the longer of the two, and the last epilogue stands alone. Against that, the sums' way to
 // memory and back and one more launch. A 128-column tile's block costs 0.7 of a 256-column
-// one's (less to multiply, three quarters to load), its epilogue 0.8. Measured, 333 x 1032 x
-// 2760: dx in 18 tiles of 128 columns cut in 4 takes 12 us, in 10 of 256 cut in 7 15 us;
-// dW1 and dW3, 6 blocks of K, 11.7 us in tiles of 256 and 15.5 in tiles of 128. cap: bytes
-// the workspace has for the sums.
+// one's (less to multiply, three quarters to load), its epilogue 0.8. Measured, launches of
+// their own: 333 x 1032 over 5520 in 18 tiles of 128 columns cut in 4 takes 12 us, in 10 of
+// 256 cut in 7 15 us; 5520 x 1032 over 333, 6 blocks of K, 11.7 us in tiles of 256 and 15.5
+// in tiles of 128. cap: bytes the workspace has for the sums.
 struct Plan {
   int bn, splits;
 };
@@ -259,7 +259,7 @@ int launch_ffn_cfg(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorM
                 tb2, p);
 }
 
-// Maps and launch of one product of p.M rows and p.N columns over k: A K-major, B K-major (w2
+// Maps and launch of one product of p.M rows and p.N columns over k: A K-major, B K-major (b2
 // the gate's second) or MN-major.
 template <int kElem, bool kBMN, int kEpi>
 int launch_ffn(const void* a, const void* b, const void* b2, int k, const Plan& plan, FfnParams& p, int sms, cudaStream_t s) {

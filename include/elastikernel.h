@@ -589,8 +589,9 @@ int ek_gemm_fp8_block(const void* A, const void* W, const float* a_scale, const 
  *   h1 = x W1^T, h3 = x W3^T, a = f(h1) h3, y = a W2^T
  * x [T, H], w1 and w3 [I, H], w2 [H, I], y [T, H]; H and I multiples of 8 up
  * to 2^28, T up to 2^31 - 256 (here and in the forms below). a comes from the
- * unrounded sums and is rounded to the inputs' type between the two products. h (may be NULL): h1 and h3 rounded, [2, T, I], for the gradient.
- * All pointers 16-byte aligned; workspace as above. */
+ * unrounded sums and is rounded to the inputs' type between the two products. h (may
+ * be NULL): h1 and h3 rounded, [2, T, I], for the gradient. All pointers 16-byte
+ * aligned; workspace as above. */
 size_t ek_gated_ffn_workspace_bytes(int T, int H, int I, int num_sms);
 int ek_gated_ffn(const void* x, const void* w1, const void* w2, const void* w3, void* y, void* h, int T, int H, int I,
                  int dtype, int gate, int num_sms, void* workspace, size_t ws_bytes, void* stream);
