@@ -8,7 +8,8 @@
 // s is the logistic function, Phi and phi the normal distribution and density.
 // Phi is taken as erfc(-z / sqrt 2) / 2, which keeps its relative precision for
 // negative z where 1 + erf cancels. u's argument is held within +-30, where s
-// has long reached 0 or 1, so that z^3 cannot overflow into inf * 0.
+// has long reached 0 or 1, so that z^3 cannot overflow into inf * 0, by comparisons
+// that a NaN passes: a minimum or maximum would take the bound for it.
 #pragma once
 #include "ek_ptx.cuh"
 
@@ -21,7 +22,7 @@ __device__ __forceinline__ float logistic_f(float z) { return __fdividef(1.0f, 1
 // s(2u(z)) and, with slope, z s (1 - s) 2u'(z)
 __device__ __forceinline__ float gelu_tanh_s(float z, float& tail) {
   constexpr float k2 = 1.5957691216057308f, c = 0.044715f;  // 2 sqrt(2 / pi)
-  const float zc = fminf(fmaxf(z, -30.0f), 30.0f), z2 = zc * zc;
+  const float zc = z < -30.0f ? -30.0f : z > 30.0f ? 30.0f : z, z2 = zc * zc;
   const float s = logistic_f(k2 * zc * (1.0f + c * z2));
   tail = zc * s * (1.0f - s) * k2 * (1.0f + 3.0f * c * z2);
   return s;
