@@ -1144,7 +1144,7 @@ def gemm_fp8_block(a_q: torch.Tensor, w_q: torch.Tensor, a_scale: torch.Tensor, 
     """C[M, N] = A @ W^T for e4m3 a_q [M, K] and w_q [N, K] with block scales.
 
     a_scale [M, ceil(K/128)] holds a scale per 1 x 128 group of a row, w_scale
-    [ceil(N/128), ceil(K/128)] one per 128 x 128 block, both fp32 of any value:
+    [ceil(N/128), ceil(K/128)] one per 128 x 128 block, both fp32 of any finite value:
     what quant_e4m3(x, block=(1, 128)) and quant_e4m3(w, block=(128, 128)) give.
     K is a multiple of 16; M, N (up to 2^31 - 256) and the last block of each axis
     are any size. The sums are fp32; C is bf16, fp16 or fp32 (`dtype`, or out's),

@@ -8,7 +8,9 @@
 // scales are fp32, so the tensor cores cannot apply them: each 128-wide K block is
 // multiplied into one of two TMEM buffers, and while the next block's MMA runs, the
 // epilogue warps read the product, multiply it by its one scale per row and weight
-// block and add it to fp32 accumulators in registers.
+// block and add it to fp32 accumulators in registers. Scales whose product is no normal
+// number are applied one after the other (scale_pair): four blocks' scales are tested at
+// once, which is 0.3 to 1.4 % of the time (4096 x 14336 x 4096: 220.8 and 221.4 us).
 //
 // 4096 x 14336 x 4096 takes 220 us (2190 TFLOP/s; the product with a scale per row, whose
 // MMA never waits for an epilogue, 176).
@@ -354,34 +356,56 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
       fetch(w.kb0);
       // A failed wait has raised the abort flag: the loop then runs out without waiting and
       // the tile is not stored.
+      auto block = [&](auto pairs, float f0, float x0, float f1, float x1) {
+        auto scale = [&](float f) {
+          if constexpr (decltype(pairs)::value) {
+#pragma unroll
+            for (int j = 0; j < 64; ++j) r[j] = __float_as_uint(__uint_as_float(r[j]) * f);
+          }
+        };
+        const int buf = gkb & 1;
+        mbar_wait_soon(&kfull_bar[buf], (gkb >> 1) & 1, s_abort);
+        __syncwarp();
+        tc_fence_after();
+        tmem_ld64(t_row + buf * 256 + run0, r);
+        tmem_ld_wait(r);
+        scale(f0);
+        add(0, x0);
+        tmem_ld64(t_row + buf * 256 + run1, r);
+        tmem_ld_wait(r);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(kempty0 + buf * 8);
+        scale(f1);
+        add(32, x1);
+        ++gkb;
+      };
 #pragma unroll 1
       for (int kb = w.kb0; kb < w.kb1; kb += 4) {
-        float s0[4], s1[4];
+        float s0[4], s1[4], lo = 1.f, hi = 1.f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           s0[j] = xa[j] * xw[j];
           s1[j] = Cfg::kGate ? xa[j] * xv[j] : s0[j];
+          lo = fminf(lo, fminf(fabsf(s0[j]), fabsf(s1[j])));
+          hi = fmaxf(hi, fmaxf(fabsf(s0[j]), fabsf(s1[j])));
         }
+        // a product of scales below or past fp32's normal numbers (scale_pair)
+        const bool far = lo < 0x1p-126f || hi > 0x1.fffffep127f;
         if (kb + 4 < w.kb1) fetch(kb + 4);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (kb + j < w.kb1) {
-            const int buf = gkb & 1;
-            mbar_wait_soon(&kfull_bar[buf], (gkb >> 1) & 1, s_abort);
-            __syncwarp();
-            tc_fence_after();
-            tmem_ld64(t_row + buf * 256 + run0, r);
-            tmem_ld_wait(r);
-            add(0, s0[j]);
-            tmem_ld64(t_row + buf * 256 + run1, r);
-            tmem_ld_wait(r);
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(kempty0 + buf * 8);
-            add(32, s1[j]);
-            ++gkb;
+        if (__any_sync(0xffffffffu, far)) {
+#pragma unroll 1
+          for (int k = kb; k < min(kb + 4, w.kb1); ++k) {
+            float f0 = __ldg(sw0 + k), x0 = __ldg(sa + k), f1 = __ldg(sw1 + k), x1 = x0;
+            scale_pair(x0, f0);
+            scale_pair(x1, f1);
+            block(std::true_type{}, f0, x0, f1, x1);
           }
+          continue;
         }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (kb + j < w.kb1) block(std::false_type{}, 1.f, s0[j], 1.f, s1[j]);
       }
       const bool good = !__any_sync(0xffffffffu, *s_abort);
       if (Cfg::kGate && p.splits > 1) {

@@ -13,8 +13,9 @@
 // gate function and its rounding or quantisation. No atomics, no tickets.
 //
 // Block-scaled e4m3: a 128-byte stage is one scale block. Each K block is
-// multiplied into its own TMEM buffer, and the epilogue adds (weight-block scale x
-// token scale) x product to fp32 registers while the next block's MMA runs.
+// multiplied into its own TMEM buffer, and the epilogue adds (product x weight-block
+// scale) x token scale to fp32 registers while the next block's MMA runs (see
+// scale_pair for the order).
 //
 //   warp 0  TMA producer; warp 1  TMEM and MMA; warp 2  scales (e4m3)
 //   warps 3..10  epilogue: two per TMEM lane quarter, one 128-row block each
@@ -140,6 +141,21 @@ __device__ __forceinline__ void finish_gate(const StreamOut& o, int t, int tile,
     *reinterpret_cast<uint32_t*>(o.codes + at) = lo | (hi << 16);
   }
   if ((threadIdx.x & 31) == 0) o.scales[(size_t)t * ((I + 127) / 128) + tile] = s;
+}
+
+// Scales are fp32 of any finite value: the product of two of them may overflow where the
+// scaled sum does not (0 * inf is no zero), or be a denormal of a few bits where the
+// scaled sum is an ordinary number. A block's sum r of e4m3 products is 0 or has a
+// magnitude in [2^-18, 2^25], so it comes between the two that would leave fp32's range:
+// r * first * second, first the smaller one where their product is too large, the larger
+// one where it is too small, never leaves it before the result does. Where the product is
+// normal it comes second and 1 first.
+__device__ __forceinline__ bool normal_f(float v) { return fabsf(v) >= 0x1p-126f && fabsf(v) < __int_as_float(0x7f800000); }
+__device__ __forceinline__ void scale_pair(float& second, float& first) {
+  const float a = second, b = first, p = a * b;
+  const bool swap = (fabsf(a) > fabsf(b)) == (fabsf(p) < 1.0f);
+  first = normal_f(p) ? 1.0f : swap ? a : b;
+  second = normal_f(p) ? p : swap ? b : a;
 }
 
 // How the units are dealt out; the reducing launch reads it too.
@@ -336,48 +352,66 @@ __global__ void __launch_bounds__(Cfg::THREADS, 1)
         float2 acc[NT / 2];
 #pragma unroll
         for (int j = 0; j < NT / 2; ++j) acc[j] = make_float2(0.f, 0.f);
+        // Product x weight scale is 0 or in [2^-118, 2^125] where the weight's is in
+        // [2^-100, 2^100], whatever the token's that follows; a segment with another one
+        // takes the scales pair by pair (a loop of its own: a branch in one loop spills).
+        const int nb = tile_end - u, tile = u / KB, blk = Cfg::kGate ? tile : 2 * tile + rb;
+        const float* wsc = (Cfg::kGate && rb ? p.w_scale2 : p.w_scale) + (size_t)min(blk, p.w_blocks - 1) * KB + (u - tile * KB);
+        bool far = false;
+        for (int i = lane; i < nb; i += 32) {
+          const float w = fabsf(__ldg(wsc + i));
+          far |= !(w >= 0x1p-100f && w <= 0x1p100f);
+        }
         // A failed wait has raised the abort flag: the loop then runs out without waiting and
         // nothing is written. A chunk of columns is in flight while the one before is added;
         // columns past the tokens are added too, and never used.
-        for (; u < tile_end; ++u, ++flush) {
-          const int buf = flush & 1, j = (u - u0) % SG;
-          if (j == 0) mbar_wait_soon(&sfull_bar[slot], sphase, s_abort);
-          const float* xs = s_scale + (slot * SG + j) * RS;
-          const float ws = xs[NT + rb];
-          mbar_wait_soon(&tfull_bar[buf], (flush >> 1) & 1, s_abort);
-          __syncwarp();
-          tc_fence_after();
-          constexpr int C = NT / CH;
-          uint32_t r[2][32];
-          load(r[0], lane_base + buf * 2 * NT);
-#pragma unroll
-          for (int c = 0; c < C; ++c) {
-            tmem_ld_wait(r[c & 1]);
-            if (c + 1 < C) {
-              load(r[(c + 1) & 1], lane_base + buf * 2 * NT + (c + 1) * CH);
-            } else {
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&tempty_bar[buf]);
-            }
-            const float4* xs4 = reinterpret_cast<const float4*>(xs + c * CH);
-            const uint32_t(&v)[32] = r[c & 1];
-#pragma unroll
-            for (int i = 0; i < CH / 4; ++i) {
-              const float4 x = xs4[i];
-              float2* a = acc + (c * CH + 4 * i) / 2;
-              a[0] = fma2(make_float2(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1])),
-                          mul2(make_float2(x.x, x.y), make_float2(ws, ws)), a[0]);
-              a[1] = fma2(make_float2(__uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3])),
-                          mul2(make_float2(x.z, x.w), make_float2(ws, ws)), a[1]);
-            }
-          }
-          if (j == SG - 1 || u + 1 == u1) {
+        auto blocks = [&](auto pairs) {
+          for (; u < tile_end; ++u, ++flush) {
+            const int buf = flush & 1, j = (u - u0) % SG;
+            if (j == 0) mbar_wait_soon(&sfull_bar[slot], sphase, s_abort);
+            const float* xs = s_scale + (slot * SG + j) * RS;
+            const float ws = xs[NT + rb];
+            mbar_wait_soon(&tfull_bar[buf], (flush >> 1) & 1, s_abort);
             __syncwarp();
-            if (lane == 0) mbar_arrive(&sempty_bar[slot]);
-            if (++slot == NS) { slot = 0; sphase ^= 1; }
+            tc_fence_after();
+            constexpr int C = NT / CH;
+            uint32_t r[2][32];
+            load(r[0], lane_base + buf * 2 * NT);
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+              tmem_ld_wait(r[c & 1]);
+              if (c + 1 < C)
+                load(r[(c + 1) & 1], lane_base + buf * 2 * NT + (c + 1) * CH);
+              else
+                release(buf);
+              const float4* xs4 = reinterpret_cast<const float4*>(xs + c * CH);
+              const uint32_t(&v)[32] = r[c & 1];
+#pragma unroll
+              for (int i = 0; i < CH / 4; ++i) {
+                const float4 x = xs4[i];
+                float2* a = acc + (c * CH + 4 * i) / 2;
+                float2 f0 = make_float2(ws, ws), f1 = f0, s0 = make_float2(x.x, x.y), s1 = make_float2(x.z, x.w);
+                if constexpr (decltype(pairs)::value) {
+                  scale_pair(s0.x, f0.x);
+                  scale_pair(s0.y, f0.y);
+                  scale_pair(s1.x, f1.x);
+                  scale_pair(s1.y, f1.y);
+                }
+                a[0] = fma2(mul2(make_float2(__uint_as_float(v[4 * i]), __uint_as_float(v[4 * i + 1])), f0), s0, a[0]);
+                a[1] = fma2(mul2(make_float2(__uint_as_float(v[4 * i + 2]), __uint_as_float(v[4 * i + 3])), f1), s1, a[1]);
+              }
+            }
+            if (j == SG - 1 || u + 1 == u1) {
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&sempty_bar[slot]);
+              if (++slot == NS) { slot = 0; sphase ^= 1; }
+            }
           }
-        }
+        };
+        if (__any_sync(0xffffffffu, far))
+          blocks(std::true_type{});
+        else
+          blocks(std::false_type{});
         good = !__any_sync(0xffffffffu, *s_abort);
         if (!good) break;
 #pragma unroll

@@ -1,5 +1,5 @@
 """Dense feed-forward operators at the ends of what their inputs may hold: NaN that has
-to reach every gradient it belongs to."""
+to reach every gradient it belongs to, and scales of any value."""
 from __future__ import annotations
 
 import pytest
@@ -11,6 +11,7 @@ from oracle import ffn as off
 pytestmark = pytest.mark.gpu
 
 BF, FP = torch.bfloat16, torch.float16
+F8 = torch.float8_e4m3fn
 NAN = float("nan")
 
 
@@ -67,3 +68,120 @@ def test_nan_reaches_every_result_it_belongs_to(T, act, where, cuda_dev):
     if where == "x":  # the quantisation of a weight has no NaN
         q = _ops.gated_ffn_fp8(x, _ops.quant_ffn_weights_fp8(w1, w2, w3), act=act)
         assert torch.equal(torch.isnan(q), torch.isnan(ref["y"]))
+
+
+# ------------------------------------------------------------------ scales of any value
+def _sums_bound(va, vw, K):
+    """Of a product of fp32 sums (test_ffn_gpu's first rule) of K blocks, each of which, and
+    each sum so far, may end below fp32's normal numbers: half a denormal step apiece."""
+    return (K / 16 + 16) * 2.0 ** -22 * (va.abs() @ vw.abs().T) + 2 * (K // 128 + 1) * 2.0 ** -150
+
+
+def _fits(got, ref, bound):
+    """got is ref within the bound and one rounding of its type; past the type's largest
+    number, infinite with ref's sign."""
+    g, info = got.double(), torch.finfo(got.dtype)
+    past = ref.abs() > info.max * (1 + 2.0 ** -10)
+    assert (ref[~past].abs() < info.max * (1 - 2.0 ** -10)).all()  # no case is at the border
+    assert torch.equal(g[past], torch.inf * ref[past].sign())
+    assert torch.isfinite(g[~past]).all()
+    bound = bound + info.eps / 2 * ref.abs() * (1 + 2.0 ** -6) + info.smallest_normal * info.eps / 2
+    over = ((g - ref).abs() - bound)[~past]
+    assert over.numel() == 0 or over.max() <= 0, f"{over.max():.3e} over its bound"
+
+
+def _far_scales(g, exponent, *shape):
+    """fp32 of magnitude 2^exponent to 2^(exponent + 1), some negative"""
+    s = torch.rand(shape, generator=g, device="cuda", dtype=torch.float64) + 1
+    s = torch.where(torch.rand(shape, generator=g, device="cuda") < 0.2, -s, s)
+    return (s * 2.0 ** exponent).float()
+
+
+# few tokens; the kernel of tiles, whole and cut along K, its scales read one by one (3
+# blocks of K) and four at a time; a device's and a small partition's plans
+@pytest.mark.parametrize("M,N,K,num_sms", [(1, 300, 512, None), (15, 200, 384, 8), (40, 130, 272, None), (64, 300, 512, 4),
+                                           (120, 520, 512, 2), (128, 300, 272, None), (200, 300, 512, 4),
+                                           (300, 130, 400, 2), (200, 300, 4096, None), (260, 77, 2000, None)])
+@pytest.mark.parametrize("ea,ew", [(-70, -70), (-75, -74), (-21, -121), (-126, -11), (-2, -148), (-148, -2), (-60, -66),
+                                   (-126, 126), (126, -126), (-148, 120), (120, -148), (104, -104), (-104, 104)])
+def test_block_product_of_far_scales(M, N, K, num_sms, ea, ew, cuda_dev):
+    """Scales whose product fp32 holds badly or not at all, the results of which it does; and
+    scales far apart whose product is ordinary."""
+    g = _gen(M + N + K)
+    a, w = (torch.randn((r, K), generator=g, device="cuda").mul(60).clamp(-448, 448).to(F8) for r in (M, N))
+    sa, sw = _far_scales(g, ea, M, -(-K // 128)), _far_scales(g, ew, -(-N // 128), -(-K // 128))
+    va, vw = off.expand(a, sa, 1), off.expand(w, sw, 128)
+    _fits(_ops.gemm_fp8_block(a, w, sa, sw, dtype=torch.float32, num_sms=num_sms), va @ vw.T, _sums_bound(va, vw, K))
+
+
+@pytest.mark.parametrize("M,N,K,num_sms", [(1, 300, 512, None), (40, 130, 272, None), (64, 300, 512, 4), (128, 300, 400, 2),
+                                           (200, 300, 512, 4), (300, 130, 272, 2), (200, 300, 4096, None)])
+@pytest.mark.parametrize("ea,ew", [(70, 66), (66, 70), (127, 10), (10, 127), (120, 120)])
+def test_block_product_of_huge_scales(M, N, K, num_sms, ea, ew, cuda_dev):
+    """Products of scales past fp32's largest number: what the codes leave at zero is zero,
+    what they make large is infinite, and least codes (2^-18 together) bring the first
+    two's product back into range."""
+    g = _gen(M * N + K)
+    a = torch.rand((M, K), generator=g, device="cuda").add(0.5).to(F8)
+    w = torch.rand((N, K), generator=g, device="cuda").add(0.5).to(F8)
+    a[::3] = 0          # rows of zeros
+    w[1::4] = 0         # columns of zeros
+    w[:, :128] = 0      # and a block of K that is zero for all
+    w[2::4, 128:] = 0
+    a[:, 160] = 0
+    a[1::3, 160], w[2::4, 160] = 2.0 ** -9, 2.0 ** -9  # a single product of 2^-18
+    sa, sw = _far_scales(g, ea, M, -(-K // 128)).abs(), _far_scales(g, ew, -(-N // 128), -(-K // 128)).abs()
+    va, vw = off.expand(a, sa, 1), off.expand(w, sw, 128)
+    ref = va @ vw.T
+    got = _ops.gemm_fp8_block(a, w, sa, sw, dtype=torch.float32, num_sms=num_sms)
+    _fits(got, ref, _sums_bound(va, vw, K))
+    assert (got[::3] == 0).all() and (got[:, 1::4] == 0).all()
+
+
+@pytest.mark.parametrize("T,num_sms", [(3, None), (40, None), (100, None), (300, None), (300, 4)])
+def test_gated_ffn_fp8_of_zero_blocks_under_huge_scales(T, num_sms, cuda_dev):
+    """Blocks of zero codes under any finite scale add nothing: not NaN."""
+    H, I = 512, 384
+    g = _gen(T)
+    x, w1, w2, w3 = (torch.randn(s, generator=g, device="cuda").to(BF) for s in ((T, H), (I, H), (H, I), (I, H)))
+    qw = _ops.quant_ffn_weights_fp8(w1 * H ** -0.5, w2 * I ** -0.5, w3 * H ** -0.5)
+    for n in ("w1", "w3", "w2"):
+        qw[n + "q"][:, 128:256] = 0
+    plain = _ops.gated_ffn_fp8(x, qw, num_sms=num_sms)
+    x[:, 128:256] *= 2.0 ** 70  # tokens' scales of about 2^63
+    far = dict(qw)
+    for n in ("w1", "w3", "w2"):
+        far[n + "s"] = qw[n + "s"].clone()
+        far[n + "s"][:, 1] = 2.0 ** 127
+    assert torch.isfinite(plain).all() and (plain != 0).any()
+    assert torch.equal(_ops.gated_ffn_fp8(x, far, num_sms=num_sms), plain)
+
+
+@pytest.mark.parametrize("T,num_sms", [(3, None), (40, None), (100, None), (300, None), (300, 4)])
+def test_gated_ffn_fp8_of_vanishing_products_of_scales(T, num_sms, cuda_dev):
+    """Tokens and W3 of 2^-69 each, products of scales of one bit or none; W1 and W2 bring
+    the result back.
+
+    A code is off by at most 2^-4 of a value or 2^-10 of its scale, 2^-3 more of either for
+    the quotient's rounding, as in ordinary ranges; h3 by the sums' errors and, around its
+    blocks and their sums, half a denormal step each."""
+    H, I = 528, 400
+    g = _gen(T + 1)
+    x, w1, w2, w3 = (torch.randn(s, generator=g, device="cuda").to(BF) for s in ((T, H), (I, H), (H, I), (I, H)))
+    qw = _ops.quant_ffn_weights_fp8(w1 * H ** -0.5, w2 * I ** -0.5, w3 * H ** -0.5)
+    x = x * 2.0 ** -69
+    qw["w1s"], qw["w3s"], qw["w2s"] = qw["w1s"] * 2.0 ** 120, qw["w3s"] * 2.0 ** -69, qw["w2s"] * 2.0 ** 90
+    W1, W2, W3 = (off.expand(qw[n + "q"], qw[n + "s"], 128) for n in ("w1", "w2", "w3"))
+    X = off.e4m3_groups(x.double())
+    acc = (H / 16 + 16) * 2.0 ** -22
+    h1, h3 = X @ W1.T, X @ W3.T
+    a = off.gate(h1, "silu") * h3
+    da = (acc * (X.abs() @ W1.abs().T) * (off.slope(h1, "silu") * h3).abs() +
+          (acc * (X.abs() @ W3.abs().T) + 12 * 2.0 ** -150) * off.gate(h1, "silu").abs() + 2.0 ** -20 * a.abs())
+    top = (a.abs() + da).amax(dim=1, keepdim=True)
+    code = (1 + 2.0 ** -3) * (2.0 ** -4 * (a.abs() + da) + 2.0 ** -10 * top / 448)
+    bound = (da + code + (I / 16 + 16) * 2.0 ** -22 * (a.abs() + da + code)) @ W2.abs().T
+    got = _ops.gated_ffn_fp8(x, qw, num_sms=num_sms)
+    ref = a @ W2.T
+    _fits(got, ref, bound)
+    assert (got.double() - ref).square().mean().sqrt() <= 2.0 ** -4 * ref.square().mean().sqrt()
