@@ -113,6 +113,12 @@ struct StreamOut {
 // a zero beside such values would become NaN.
 __device__ __forceinline__ float act_scale(float m) { return m > 0.f ? fmaxf(m / 448.0f, 0x1p-126f) : 1.0f; }
 
+// Four values' e4m3 codes
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+  return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3) |
+         ((uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3) << 16);
+}
+
 // a[t, f] = f(h1) h3 for 4 features a lane, from feature f on, and h1 and h3 on request;
 // with codes, a in e4m3 with the scale of the warp's 128 features (act_scale). Rows past the weight's hold zeros.
 __device__ __forceinline__ void finish_gate(const StreamOut& o, int t, int tile, const float4& h1, const float4& h3) {
@@ -135,11 +141,7 @@ __device__ __forceinline__ void finish_gate(const StreamOut& o, int t, int tile,
 #pragma unroll
   for (int i = 16; i; i >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, i));
   const float s = act_scale(m);
-  if (f < I) {
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(act.x / s, act.y / s), __NV_SATFINITE, __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(act.z / s, act.w / s), __NV_SATFINITE, __NV_E4M3);
-    *reinterpret_cast<uint32_t*>(o.codes + at) = lo | (hi << 16);
-  }
+  if (f < I) *reinterpret_cast<uint32_t*>(o.codes + at) = e4m3x4(act.x / s, act.y / s, act.z / s, act.w / s);
   if ((threadIdx.x & 31) == 0) o.scales[(size_t)t * ((I + 127) / 128) + tile] = s;
 }
 
@@ -556,11 +558,7 @@ __global__ void __launch_bounds__(256) ffn_quant_kernel(const __nv_bfloat16* __r
       if (at[i] < 0) continue;
       uint32_t pk[2];
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-        pk[j] =
-            (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[4 * j] / s, v[4 * j + 1] / s), __NV_SATFINITE, __NV_E4M3) |
-            ((uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(v[4 * j + 2] / s, v[4 * j + 3] / s), __NV_SATFINITE, __NV_E4M3)
-             << 16);
+      for (int j = 0; j < 2; ++j) pk[j] = e4m3x4(v[4 * j] / s, v[4 * j + 1] / s, v[4 * j + 2] / s, v[4 * j + 3] / s);
       *reinterpret_cast<uint2*>(codes + at[i]) = make_uint2(pk[0], pk[1]);
       if (hl == 0) scales[g0 + 2 * i + ((threadIdx.x >> 4) & 1)] = s;
     }

@@ -576,8 +576,8 @@ int ek_fused_moe_w4(const void* x, const float* logits, int T, int topk, const v
  *   C[m, n] = sum_b a_scale[m, b] * w_scale[n / 128, b] * sum_{k in block b} A[m, k] * W[n, k]
  * A [M, K] and W [N, K] e4m3, blocks of 128 along K (the last may be short),
  * a_scale [M, ceil(K / 128)] and w_scale [ceil(N / 128), ceil(K / 128)] fp32 of any
- * finite value, whatever their product. Products of a block and the sum over blocks are fp32; C [M, N] is bf16,
- * fp16 or fp32 (out_dtype), rounded once. K a multiple of 16 up to 2^28, M and N up
+ * finite value, whatever their product. Products of a block and the sum over blocks are
+ * fp32; C [M, N] is bf16, fp16 or fp32 (out_dtype), rounded once. K a multiple of 16 up to 2^28, M and N up
  * to 2^31 - 256; A, W and the workspace 16-byte aligned. workspace:
  * ek_gemm_fp8_block_workspace_bytes bytes for the launch's SMs or more; its contents
  * before and after do not matter, but no two calls in flight may share it. */

@@ -1,5 +1,6 @@
 """Dense feed-forward operators at the ends of what their inputs may hold: NaN that has
-to reach every gradient it belongs to, and scales of any value."""
+to reach every gradient it belongs to, scales of any value, quotients on a border between
+two codes."""
 from __future__ import annotations
 
 import pytest
@@ -185,3 +186,40 @@ def test_gated_ffn_fp8_of_vanishing_products_of_scales(T, num_sms, cuda_dev):
     ref = a @ W2.T
     _fits(got, ref, bound)
     assert (got.double() - ref).square().mean().sqrt() <= 2.0 ** -4 * ref.square().mean().sqrt()
+
+
+# ------------------------------------------------------------------ codes on a border
+@pytest.mark.parametrize("T,num_sms", [(20, None), (100, None), (128, 2), (300, None), (300, 2), (600, 8), (1300, None)])
+def test_gated_ffn_fp8_codes_are_ieee_quotients(T, num_sms, cuda_dev):
+    """Activations that fp32 holds exactly as the formula has them, many of them halfway
+    between two codes but for the rounding of their scale; the second weight the identity, so
+    that every code shows: bit for bit quant_e4m3's, by whichever kernel.
+
+    Token t has one nonzero value, 448, in block b = t % 16 of K (scale 1, code 448). W1 is 1
+    there, so f(h1) = 448 exactly (silu's exp(-448) is zero); h3 = 448 c s with one rounding,
+    a = 448 h3 with another. Of a code c of 12 x 2^j under a largest of 8 x 2^j the quotient is 84
+    2^j, a tie, within an ulp."""
+    H = I = 2048
+    g = _gen(7)
+    B = H // 128
+    x = torch.zeros((T, H), device="cuda", dtype=BF)
+    b = torch.arange(T, device="cuda") % B
+    x[torch.arange(T, device="cuda"), 128 * b] = 448.0
+    w1 = torch.zeros((I, H), device="cuda")
+    w3 = torch.zeros((I, H), device="cuda")
+    w1[:, ::128] = 1.0
+    c = 12.0 * torch.exp2(torch.randint(-9, -1, (I, B), generator=g, device="cuda").float())
+    c = torch.where(torch.rand((I, B), generator=g, device="cuda") < 0.5, c, c * 13 / 12)
+    c[::128] = 8.0      # the largest of each group
+    w3[:, ::128] = c * torch.where(torch.rand((I, B), generator=g, device="cuda") < 0.5, 1.0, -1.0)
+    one = torch.ones((B, B), device="cuda")
+    s3 = torch.rand((B, B), generator=g, device="cuda") + 1
+    eye = torch.eye(H, device="cuda")
+    qw = {"H": H, "I": I, "w1q": w1.to(F8), "w1s": one, "w3q": w3.to(F8), "w3s": s3, "w2q": eye.to(F8), "w2s": one}
+    a = 448.0 * ((448.0 * w3[:, ::128]) * s3.repeat_interleave(128, dim=0))  # [I, B]: feature, block of the token
+    q, s = _ops.quant_e4m3(a.t().contiguous(), block=(1, 128))
+    want = (q.float() * s.repeat_interleave(128, dim=1)).to(BF)[b]
+    # the border is met: some codes are not those of products with the scale's reciprocal
+    rough = (a.t() * (1.0 / s).repeat_interleave(128, dim=1)).to(F8)
+    assert not torch.equal(rough.float(), q.float())
+    assert torch.equal(_ops.gated_ffn_fp8(x, qw, num_sms=num_sms), want)
