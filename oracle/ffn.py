@@ -17,11 +17,16 @@ def expand(q: torch.Tensor, s: torch.Tensor, rows: int) -> torch.Tensor:
     return q.double() * s.double()[r][:, k]
 
 
+def normal_cdf(z: torch.Tensor) -> torch.Tensor:
+    # torch.special.ndtr is (1 + erf) / 2: zero from -9 down, where this keeps its digits
+    return torch.special.erfc(z * -math.sqrt(0.5)) / 2
+
+
 def gate(z: torch.Tensor, act: str) -> torch.Tensor:
     if act == "silu":
         return z * torch.sigmoid(z)
     if act == "gelu":
-        return z * torch.special.ndtr(z)
+        return z * normal_cdf(z)
     return z * torch.sigmoid(2 * math.sqrt(2 / math.pi) * (z + 0.044715 * z ** 3))
 
 
@@ -30,7 +35,7 @@ def slope(z: torch.Tensor, act: str) -> torch.Tensor:
         s = torch.sigmoid(z)
         return s * (1 + z * (1 - s))
     if act == "gelu":
-        return torch.special.ndtr(z) + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+        return normal_cdf(z) + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
     c = 2 * math.sqrt(2 / math.pi)
     s = torch.sigmoid(c * (z + 0.044715 * z ** 3))
     return s + z * s * (1 - s) * c * (1 + 3 * 0.044715 * z ** 2)
