@@ -223,3 +223,89 @@ def test_gated_ffn_fp8_codes_are_ieee_quotients(T, num_sms, cuda_dev):
     rough = (a.t() * (1.0 / s).repeat_interleave(128, dim=1)).to(F8)
     assert not torch.equal(rough.float(), q.float())
     assert torch.equal(_ops.gated_ffn_fp8(x, qw, num_sms=num_sms), want)
+
+
+# ------------------------------------------------------------------ the kernels against themselves
+@pytest.mark.parametrize("T", [24, 160])
+@pytest.mark.parametrize("act", list(_ops.GATES))
+def test_gradient_against_the_forward_kernels_own_differences(T, act, cuda_dev):
+    """The kernels' gradient of sum(y * d) against central differences of the forward
+    kernels, at the largest element of each gradient.
+
+    The tolerance is the sum of what 64 bits say of this difference (its distance from the
+    derivative), what they say of taking the derivative at the rounded h, and roundings.
+    In the difference: u |y| d of every y that moves, in both passes, and u |a| through w2
+    and d of every a that moves; in the gradient u of each product's rounded factor and of the
+    result. Independent and of either sign, they leave 7.5 root mean squares with a probability of
+    1e-12 (Hoeffding); 8 for the fp32 sums beside them. At most a fourth of the gradient is left
+    to them: an error of sign, factor or index does not pass."""
+    H, I, u = 64, 96, torch.finfo(FP).eps / 2
+    g = _gen(T)
+    x, w1, w2, w3, d = (torch.randn(s, generator=g, device="cuda").mul(by).to(FP) for s, by in
+                        (((T, H), 1.0), ((I, H), 2 * H ** -0.5), ((H, I), I ** -0.5), ((I, H), H ** -0.5), ((T, H), 1.0)))
+    ts = [x, w1, w2, w3]
+    _, h = _ops.gated_ffn(*ts, act=act, save=True)
+    got = _ops.gated_ffn_grad(*ts, h, d, act=act)
+    f = off.forward(*ts, act)
+    at_h, exact = off.backward(*ts, h, d, act), off.backward(*ts, f["h"], d, act)
+    X, W1, W2, W3, D = (t.double() for t in (*ts, d))
+    through = (D @ W2).abs()  # what an error of a costs
+    for i, name in enumerate(("x", "w1", "w2", "w3")):
+        r, c = divmod(exact[name].abs().argmax().item(), exact[name].shape[1])
+        step = 2.0 ** (-2 if name == "x" else -3)
+        sums, sums64, reals = [], [], []
+        for sign in (1, -1):
+            moved = [t.clone() for t in ts]
+            moved[i][r, c] += sign * step
+            reals.append(moved[i][r, c].item())
+            sums.append((_ops.gated_ffn(*moved, act=act).double() * D).sum().item())
+            sums64.append((off.forward(*moved, act)["y"] * D).sum().item())
+        width = reals[0] - reals[1]
+        diff, diff64 = (sums[0] - sums[1]) / width, (sums64[0] - sums64[1]) / width
+        ya = 2 * u * (f["y"] * D).abs()      # both passes' roundings of y
+        aa = 2 * u * f["a"].abs() * through  # and of a
+        if name == "x":
+            ya, aa = ya[r], aa[r]
+            terms = torch.cat([exact["d1"][r] * W1[:, c], exact["d3"][r] * W3[:, c]])
+        elif name == "w2":
+            ya, aa, terms = ya[:, r], aa[:0], D[:, r] * f["a"][:, c]
+        else:
+            aa, terms = aa[:, r], exact["d1" if name == "w1" else "d3"][:, r] * X[:, c]
+        ref = exact[name][r, c].item()
+        rounding = 8 * ((ya.square().sum() + aa.square().sum()).sqrt().item() / width + u * terms.square().sum().sqrt().item())
+        assert rounding <= abs(ref) / 4, name
+        tol = rounding + u * abs(ref) + abs(diff64 - ref) + abs(at_h[name][r, c].item() - ref)
+        assert abs(got[i][r, c].item() - diff) <= tol, (name, got[i][r, c].item(), diff, ref, tol)
+
+
+@pytest.mark.parametrize("T", [3, 140])
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("act", list(_ops.GATES))
+def test_each_extreme_activation_by_itself(T, dtype, act, cuda_dev):
+    """Pre-activations far past where the gate saturates, the second weight the identity: each
+    activation is a column of the result.
+
+    h1 and h3 are exact (one product each, in the type); a is off by its rounding, half a
+    step below the type's normal numbers, and 2^-13 of |z| for the gate's exponential, whose
+    argument has 2^-24 of up to 100 in it and an error of 2 + |z| ulp; y by one more rounding
+    of the same value, which changes nothing."""
+    z = [0.0, -3e4, 3e4, -100, 100, -20, 20, -1e-3, 1e-3, 5, -5, 30, -30, 1.0, -1.0, 0.5]
+    z += [-1e30, 1e30, -1e-30, 1e-30, -87.0, -88.5, 88.5, -10] if dtype == BF else [-87.0, -88.5, 88.5, -10, 11, -12, 2, -2]
+    n = len(z)
+    x = torch.zeros((T, n), device="cuda", dtype=dtype)
+    x[:, 0], x[:, 1] = 1.0, 0.5
+    w1 = torch.zeros((n, n), device="cuda", dtype=dtype)
+    w1[:, 0] = torch.tensor(z)
+    w3 = torch.zeros((n, n), device="cuda", dtype=dtype)
+    w3[:, 1] = 1.0
+    w2 = torch.eye(n, device="cuda", dtype=dtype)
+    r = off.forward(x, w1, w2, w3, act)
+    y, h = _ops.gated_ffn(x, w1, w2, w3, act=act, save=True)
+    assert torch.equal(h.double(), r["h"])
+    info = torch.finfo(dtype)
+    ref = r["a"]
+    bound = info.eps / 2 * ref.abs() + info.smallest_normal * info.eps / 2 + 2.0 ** -13 * ref.abs()
+    # under exp(-87) the logistic function's reciprocal is zero in fp32: |z| 2^-126 at most
+    bound = bound + r["h"][0].abs().clamp(max=100) * 2.0 ** -126
+    over = (y.double() - ref).abs() - bound
+    assert (over <= 0).all(), (act, torch.tensor(z)[(over > 0).any(dim=0).cpu()])
