@@ -1,7 +1,8 @@
 // Entry points of the dense feed-forward operators: the block-scaled e4m3 product,
 // the gated block in 16 bits and its gradients, and the gated block in 8 bits.
-// Up to kStreamTokens tokens the products run in stream_kernel, whose time is the
-// weights' bytes; past it in the 256 x 256 CTA-pair kernels.
+// Up to kStreamTokens tokens the forward products run in stream_kernel, whose time is the
+// weights' bytes; past it, in 8 bits from 65 tokens on where they are the faster
+// (fp8_streams), and for the gradients always, in the 256-row CTA-pair kernels.
 #include <algorithm>
 #include <cmath>
 
@@ -461,6 +462,10 @@ int gated_ffn_grad(const void* x, const void* w1, const void* w2, const void* w3
   g.n_x = (int)n_x;
   g.n_13 = (int)n_13;
   g.n_2 = (int)n_2;
+  // in blocks of K alone, although grads_plan takes a weight's tile for its stores at least: while
+  // dx's pairs multiply, the others' stores run faster than that. The ratio of the plan's own
+  // times leaves tiles for after dx (64 x 4096 x 14336: 229 us for 204; 256 x 4096 x 4096: 81
+  // for 69; 8 x 7168 x 2048: 62.6 for 56.8).
   g.lead = g.kb_x / g.splits / g.kb_w;
   g.full_h = whole_chunks(H);
   g.full_i = whole_chunks(I);

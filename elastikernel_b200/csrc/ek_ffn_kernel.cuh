@@ -58,19 +58,6 @@ __device__ __forceinline__ bool elect_one() {
   return p != 0;
 }
 
-// Whether the phase has completed, without waiting for it.
-__device__ __forceinline__ bool mbar_test(uint32_t bar_addr, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(bar_addr), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
-
 // mbar_wait for a phase that is expected within a microsecond or so: the clock is read
 // only when it has not come by then.
 __device__ __forceinline__ bool mbar_wait_soon(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
@@ -780,8 +767,8 @@ __device__ __forceinline__ void sum_slices8(const float* __restrict__ ws, int sp
   }
 }
 
-// out[i] = sum of the slices, rounded once; n8: groups of 8 elements of the result
-// (both planes), which lie end to end in both
+// out[i] = sum of the slices, rounded once; n8: groups of 8 elements of the result, which
+// lie end to end in it and in each slice
 template <int kElem>
 __global__ void __launch_bounds__(256) ffn_reduce_kernel(const float* __restrict__ ws, int splits, long long n8,
                                                          void* __restrict__ out) {

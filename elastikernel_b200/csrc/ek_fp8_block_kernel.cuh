@@ -1,4 +1,5 @@
-// Dense e4m3 product with block scales for more than 128 tokens:
+// Dense e4m3 product with block scales for more tokens than stream_kernel takes (past 128
+// always, from 65 on where it is the faster: fp8_streams):
 //   C[m, n] = sum over K blocks b of  sa[m, b] sw[n / 128, b] (sum over k in b of a[m, k] w[n, k])
 // and the gate/up pair of the feed-forward block, whose epilogue applies the gate
 // function and quantises the activations per 1 x 128 group.
