@@ -155,7 +155,7 @@ __device__ __forceinline__ void finish_gate(const StreamOut& o, int t, int tile,
 __device__ __forceinline__ bool normal_f(float v) { return fabsf(v) >= 0x1p-126f && fabsf(v) < __int_as_float(0x7f800000); }
 __device__ __forceinline__ void scale_pair(float& second, float& first) {
   const float a = second, b = first, p = a * b;
-  const bool swap = (fabsf(a) > fabsf(b)) == (fabsf(p) < 1.0f);
+  const bool swap = (fabsf(a) > fabsf(b)) == (fabsf(p) < 1.0f && p != 0.0f);  // a zero comes first
   first = normal_f(p) ? 1.0f : swap ? a : b;
   second = normal_f(p) ? p : swap ? b : a;
 }

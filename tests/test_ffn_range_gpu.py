@@ -139,6 +139,21 @@ def test_block_product_of_huge_scales(M, N, K, num_sms, ea, ew, cuda_dev):
     assert (got[::3] == 0).all() and (got[:, 1::4] == 0).all()
 
 
+@pytest.mark.parametrize("M,N,K,num_sms", [(1, 300, 512, None), (40, 130, 272, None), (128, 300, 400, 2), (200, 300, 512, 4),
+                                           (300, 130, 272, 2), (200, 300, 4096, None)])
+@pytest.mark.parametrize("which", ["a", "w", "both"])
+def test_block_product_of_zero_scales_beside_huge_ones(M, N, K, num_sms, which, cuda_dev):
+    """A scale of zero makes its block zero, whatever the sum and the other scale."""
+    g = _gen(M + K)
+    a, w = (torch.full((r, K), 448.0, device="cuda").to(F8) for r in (M, N))
+    sa, sw = _far_scales(g, 126, M, -(-K // 128)), _far_scales(g, 126, -(-N // 128), -(-K // 128))
+    if which != "w":
+        sa.zero_()
+    if which != "a":
+        sw.zero_()
+    assert (_ops.gemm_fp8_block(a, w, sa, sw, dtype=torch.float32, num_sms=num_sms) == 0).all()
+
+
 @pytest.mark.parametrize("T,num_sms", [(3, None), (40, None), (100, None), (300, None), (300, 4)])
 def test_gated_ffn_fp8_of_zero_blocks_under_huge_scales(T, num_sms, cuda_dev):
     """Blocks of zero codes under any finite scale add nothing: not NaN."""
