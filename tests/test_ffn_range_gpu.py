@@ -205,7 +205,8 @@ def test_gated_ffn_fp8_of_vanishing_products_of_scales(T, num_sms, cuda_dev):
 
 # ------------------------------------------------------------------ codes on a border
 @pytest.mark.parametrize("T,num_sms", [(20, None), (100, None), (128, 2), (300, None), (300, 2), (600, 8), (1300, None)])
-def test_gated_ffn_fp8_codes_are_ieee_quotients(T, num_sms, cuda_dev):
+@pytest.mark.parametrize("by", [0, 100, -105])
+def test_gated_ffn_fp8_codes_are_ieee_quotients(T, num_sms, by, cuda_dev):
     """Activations that fp32 holds exactly as the formula has them, many of them halfway
     between two codes but for the rounding of their scale; the second weight the identity, so
     that every code shows: bit for bit quant_e4m3's, by whichever kernel.
@@ -213,7 +214,8 @@ def test_gated_ffn_fp8_codes_are_ieee_quotients(T, num_sms, cuda_dev):
     Token t has one nonzero value, 448, in block b = t % 16 of K (scale 1, code 448). W1 is 1
     there, so f(h1) = 448 exactly (silu's exp(-448) is zero); h3 = 448 c s with one rounding,
     a = 448 h3 with another. Of a code c of 12 x 2^j under a largest of 8 x 2^j the quotient is 84
-    2^j, a tie, within an ulp."""
+    2^j, a tie, within an ulp. W3's scales of about 2^by bring the activations' scales to where
+    a quotient's residues would leave fp32's range."""
     H = I = 2048
     g = _gen(7)
     B = H // 128
@@ -228,7 +230,7 @@ def test_gated_ffn_fp8_codes_are_ieee_quotients(T, num_sms, cuda_dev):
     c[::128] = 8.0      # the largest of each group
     w3[:, ::128] = c * torch.where(torch.rand((I, B), generator=g, device="cuda") < 0.5, 1.0, -1.0)
     one = torch.ones((B, B), device="cuda")
-    s3 = torch.rand((B, B), generator=g, device="cuda") + 1
+    s3 = (torch.rand((B, B), generator=g, device="cuda") + 1) * 2.0 ** by
     eye = torch.eye(H, device="cuda")
     qw = {"H": H, "I": I, "w1q": w1.to(F8), "w1s": one, "w3q": w3.to(F8), "w3s": s3, "w2q": eye.to(F8), "w2s": one}
     a = 448.0 * ((448.0 * w3[:, ::128]) * s3.repeat_interleave(128, dim=0))  # [I, B]: feature, block of the token
